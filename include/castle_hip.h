@@ -408,6 +408,22 @@ int64_t castle_embedding_grad_workspace_bytes(int64_t rows, int vocabulary, int 
 int castle_embedding_grad(const void* dy, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows, int vocabulary, int width,
                           void* dweight, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* y[r] = scale * table[token r] in the type `dtype`, rounded once: rows of `width` elements, `ld` apart in the table, contiguous in y; the token of row r is
+ * index[(r / index_n) * index_ld + r % index_n].  A token outside 0 .. vocabulary - 1 gives a row of NaNs.  Any width and vocabulary; whole 16-byte pieces are faster.
+ *
+ * Its gradient for vocabularies of any size: dtable[v] = scale * the sum of the dy rows whose token is v, in the order of the rows (the same sum every time), rounded once;
+ * zeros where there is none.  Rows whose token is `padding` (-1: none) or outside of the vocabulary have no part in it. */
+int castle_embedding(const void* table, int64_t ld, int vocabulary, int width, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows, float scale,
+                     void* y, int dtype, void* stream);
+int64_t castle_embedding_sorted_grad_workspace_bytes(int64_t rows, int vocabulary, int width);
+int castle_embedding_sorted_grad(const void* dy, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows, int vocabulary, int width, float scale, int padding,
+                                 void* dtable, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* y = residual + (x where it stays, times 1 / (1 - p), else 0): n contiguous elements of the type `dtype`, 16-byte aligned; residual may be NULL.  p is rounded to t / 65536.  Elements
+ * 8 i .. 8 i + 7 take the eight 16-bit halves, low half first, of the four words that Philox4x32-10 makes of the counter (i, seed[1]) and the key seed[0] (low words first), and
+ * stay where theirs is at least t.  seed: two numbers in device memory.  The backward pass is the same call on dy without a residual: nothing is kept. */
+int castle_dropout(const void* x, const void* residual, void* y, int64_t n, double p, const int64_t* seed, int dtype, void* stream);
+
 /* Per-kernel timing (no counterpart in the reference; for benchmarks).  While enabled, every
  * kernel launched by the entry points above is bracketed by a HIP event pair on its stream.
  * castle_profile_enable(on) also discards pending records.  castle_profile_read waits for the

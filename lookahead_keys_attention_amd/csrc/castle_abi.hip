@@ -5,12 +5,14 @@
 
 #include "../../include/castle_hip.h"
 #include <algorithm>
+#include <cmath>
 #include <stdlib.h>
 #include <initializer_list>
 #include "castle_params.h"
 #include "castle_gemm.h"
 #include "castle_profile.h"
 #include "castle_rows.h"
+#include "castle_tokens.h"
 #include "castle_tiles.h"
 
 namespace castle {
@@ -836,6 +838,72 @@ int castle_embedding_grad(const void* dy, const int64_t* index, int64_t index_n,
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need) return CASTLE_ERR_WORKSPACE;
   const castle::EmbeddingGradArgs a = {dy, index, rows, index_n, index_ld, vocabulary, width, static_cast<float*>(workspace)};
   return castle::launch_embedding_grad(a, dweight, dtype, static_cast<hipStream_t>(stream));
+}
+
+static int token_rows(castle::TokenRows& t, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows) {
+  if (rows <= 0 || rows > kMaxRows || index_n <= 0 || rows % index_n != 0) return CASTLE_ERR_SHAPE;
+  if (index == nullptr || reinterpret_cast<uintptr_t>(index) % 8 != 0) return CASTLE_ERR_ARG;
+  t = {index, rows, index_n, index_ld};
+  return CASTLE_OK;
+}
+static bool aligned_to(std::initializer_list<const void*> ps, int es) {
+  for (const void* p : ps)
+    if (p == nullptr || reinterpret_cast<uintptr_t>(p) % es != 0) return false;
+  return true;
+}
+
+int castle_embedding(const void* table, int64_t ld, int vocabulary, int width, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows, float scale,
+                     void* y, int dtype, void* stream) {
+  const int es = elem_size(dtype);
+  if (es == 0) return CASTLE_ERR_DTYPE;
+  castle::EmbeddingArgs a = {};
+  const int rc = token_rows(a.tokens, index, index_n, index_ld, rows);
+  if (rc != CASTLE_OK) return rc;
+  if (vocabulary <= 0 || width <= 0) return CASTLE_ERR_SHAPE;
+  if (!aligned_to({table, y}, es) || ld < 0) return CASTLE_ERR_ARG;
+  a.table = table;
+  a.ld = ld;
+  a.y = y;
+  a.V = vocabulary;
+  a.D = width;
+  a.scale = scale;
+  return castle::launch_embedding(a, dtype, static_cast<hipStream_t>(stream));
+}
+
+int64_t castle_embedding_sorted_grad_workspace_bytes(int64_t rows, int vocabulary, int width) {
+  if (rows <= 0 || rows > kMaxRows || vocabulary <= 0 || width <= 0 || vocabulary == INT32_MAX) return CASTLE_ERR_SHAPE;
+  return castle::sorted_grad_plan(rows, vocabulary, width).total;
+}
+
+int castle_embedding_sorted_grad(const void* dy, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows, int vocabulary, int width, float scale, int padding,
+                                 void* dtable, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int es = elem_size(dtype);
+  if (es == 0) return CASTLE_ERR_DTYPE;
+  castle::SortedGradArgs a = {};
+  const int rc = token_rows(a.tokens, index, index_n, index_ld, rows);
+  if (rc != CASTLE_OK) return rc;
+  const int64_t need = castle_embedding_sorted_grad_workspace_bytes(rows, vocabulary, width);
+  if (need < 0) return (int)need;
+  if (padding < -1 || padding >= vocabulary || !aligned_to({dy, dtable}, es)) return CASTLE_ERR_ARG;
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need) return CASTLE_ERR_WORKSPACE;
+  a.dy = dy;
+  a.dw = dtable;
+  a.V = vocabulary;
+  a.D = width;
+  a.padding = padding;
+  a.scale = scale;
+  a.plan = castle::sorted_grad_plan(rows, vocabulary, width);
+  a.workspace = workspace;
+  return castle::launch_sorted_grad(a, dtype, static_cast<hipStream_t>(stream));
+}
+
+int castle_dropout(const void* x, const void* residual, void* y, int64_t n, double p, const int64_t* seed, int dtype, void* stream) {
+  if (elem_size(dtype) == 0) return CASTLE_ERR_DTYPE;
+  if (n <= 0 || n > (int64_t)1 << 40) return CASTLE_ERR_SHAPE;
+  if (x == nullptr || y == nullptr || seed == nullptr || !aligned16({x, residual, y}) || reinterpret_cast<uintptr_t>(seed) % 8 != 0 || !(p >= 0 && p <= 1)) return CASTLE_ERR_ARG;
+  const int t = (int)std::nearbyint(65536 * p);
+  const castle::DropoutArgs a = {x, residual, y, seed, n, (uint32_t)t, t < 65536 ? 65536.f / (float)(65536 - t) : 0.f};
+  return castle::launch_dropout(a, dtype, static_cast<hipStream_t>(stream));
 }
 
 int castle_profile_enable(int on) { return castle::profile_enable(on); }

@@ -15,6 +15,15 @@ template <typename F> int by_type(int dtype, bool bf16_operands, F&& f) {
     default: return -1;
   }
 }
+// f(tensor type)
+template <typename F> int by_tensor_type(int dtype, F&& f) {
+  switch (dtype) {
+    case 0: return f(float());
+    case 1: return f(bf16_t());
+    case 2: return f(fp16_t());
+    default: return -1;
+  }
+}
 template <typename F> int by_type16(int dtype, bool bf16_operands, F&& f) {   // 16-bit tensors only
   if (dtype == 1) return bf16_operands ? f(bf16_t(), bf16_t()) : f(fp16_t(), bf16_t());
   return dtype == 2 ? f(fp16_t(), fp16_t()) : -1;

@@ -1,0 +1,323 @@
+// Token embedding of any vocabulary: rows of the table times a scale, and the table's gradient by sorted tokens.
+//
+//   y[r] = scale table[token r]          dtable[v] = scale sum over the r whose token is v of dy[r]
+//
+// Both are bound by HBM: the forward pass reads a row and writes one, the gradient reads dy and writes the whole table once.  The gradient needs the rows of
+// each token together, in an order of their own (atomic additions would leave the order, and with it the last bits, to chance): (token, place) pairs are sorted, stable, by
+// digits of up to ten bits, a counting and a placing launch for each.  Pieces of 64 sorted places that hold one token alone are summed first, so that a token that takes a tenth of a text
+// does not keep one workgroup busy when the rest is done; then every row of the table is summed and written once, zeros where there is no token.
+#include "castle_tiles.h"
+#include "castle_dispatch.h"
+#include "castle_tokens.h"
+#include <algorithm>
+
+namespace castle {
+namespace {
+
+constexpr int kWaves = kThreads / 64;
+constexpr int kRun = 64;   // sorted places of a piece
+
+__device__ __forceinline__ int64_t token_of(const TokenRows& t, int64_t r) {
+  if (t.n == t.rows) return t.index[r];
+  const uint32_t q = (uint32_t)r / (uint32_t)t.n;   // (rows are fewer than 2^31)
+  return t.index[q * t.index_ld + ((uint32_t)r - q * (uint32_t)t.n)];
+}
+
+// N elements at a time: a 16-byte piece, or one where rows are no whole pieces
+template <typename T, int N> __device__ __forceinline__ vec<float, N> load_n(const T* p) {
+  return __builtin_convertvector(*reinterpret_cast<const vec<T, N>*>(p), vec<float, N>);
+}
+template <typename T, int N> __device__ __forceinline__ void store_n(T* p, vec<float, N> v) { *reinterpret_cast<vec<T, N>*>(p) = __builtin_convertvector(v, vec<T, N>); }
+template <int N> __device__ __forceinline__ vec<float, N> fill_n(float x) {
+  vec<float, N> v;
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = x;
+  return v;
+}
+
+// LPR lanes to a row
+template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) void embedding_kernel(EmbeddingArgs a) {
+  constexpr int RPG = kThreads / LPR;
+  const int64_t r = (int64_t)blockIdx.x * RPG + threadIdx.x / LPR;
+  if (r >= a.tokens.rows) return;
+  const int64_t t = token_of(a.tokens, r);
+  const bool there = t >= 0 && t < a.V;
+  const T* row = static_cast<const T*>(a.table) + (there ? t : 0) * a.ld;
+  T* y = static_cast<T*>(a.y) + r * a.D;
+#pragma unroll 4
+  for (int i = threadIdx.x % LPR; i < a.D / N; i += LPR) {
+    const vec<float, N> v = load_n<T, N>(row + i * N) * a.scale;
+    store_n<T, N>(y + i * N, there ? v : fill_n<N>(NAN));
+  }
+}
+
+// ---- sorting -------------------------------------------------------------------------------------------------------
+// Every wave has a range of its own, in order; workgroup g has those of four waves.
+struct SortArgs {
+  TokenRows tokens;
+  int V, padding;
+  int shift, bits;
+  int64_t wave_tokens;
+  const uint32_t *keys_in, *places_in;   // nullptr: the tokens themselves
+  uint32_t *keys, *places;
+  uint32_t* counts;                      // [workgroup][digit]
+};
+__device__ __forceinline__ uint32_t key_of(const SortArgs& a, int64_t i) {
+  if (a.keys_in != nullptr) return a.keys_in[i];
+  const int64_t t = token_of(a.tokens, i);
+  return t >= 0 && t < a.V && t != a.padding ? (uint32_t)t : (uint32_t)a.V;   // behind all others
+}
+extern __shared__ __attribute__((aligned(16))) uint32_t castle_digits[];   // [wave][digit]
+// how many of each digit there are in the range of this wave
+__device__ __forceinline__ void wave_counts(const SortArgs& a, uint32_t* mine, int64_t first, int64_t last) {
+  for (int64_t i = first + lane_id(); i < last; i += 64) atomicAdd(mine + (key_of(a, i) >> a.shift & ((1u << a.bits) - 1)), 1u);
+}
+__global__ __launch_bounds__(kThreads) void sort_count_kernel(SortArgs a) {
+  const int digits = 1 << a.bits;
+  for (int d = threadIdx.x; d < digits; d += kThreads) castle_digits[d] = 0;
+  __syncthreads();
+  const int64_t first = ((int64_t)blockIdx.x * kWaves + wave_id()) * a.wave_tokens;
+  wave_counts(a, castle_digits, first, min(a.tokens.rows, first + a.wave_tokens));
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kThreads) a.counts[(int64_t)blockIdx.x * digits + d] = castle_digits[d];
+}
+// From the counts of all workgroups to the place of each digit's first key of each wave here, then the keys to their places: equal digits in the order they came.
+__global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
+  const int digits = 1 << a.bits, wave = wave_id(), lane = lane_id();
+  uint32_t* const s_sum = castle_digits + kWaves * digits;   // [kThreads]
+  for (int d = threadIdx.x; d < kWaves * digits; d += kThreads) castle_digits[d] = 0;
+  __syncthreads();
+  const int64_t first = ((int64_t)blockIdx.x * kWaves + wave) * a.wave_tokens, last = min(a.tokens.rows, first + a.wave_tokens);
+  uint32_t* const mine = castle_digits + wave * digits;
+  wave_counts(a, mine, first, last);
+  // a thread has `per` digits in a row
+  const int per = max(1, digits / kThreads), d0 = threadIdx.x * per;
+  constexpr int kMaxPer = 4;
+  uint32_t before[kMaxPer] = {}, all[kMaxPer] = {}, sum = 0;
+  if (d0 < digits) {
+#pragma unroll
+    for (int p = 0; p < kMaxPer; ++p) {
+      if (p >= per) break;
+#pragma unroll 8
+      for (int g = 0; g < (int)gridDim.x; ++g) {
+        const uint32_t n = a.counts[(int64_t)g * digits + d0 + p];
+        all[p] += n;
+        before[p] += g < (int)blockIdx.x ? n : 0;
+      }
+      sum += all[p];
+    }
+  }
+  s_sum[threadIdx.x] = sum;
+  __syncthreads();
+  for (int o = 1; o < kThreads; o <<= 1) {
+    const uint32_t left = (int)threadIdx.x >= o ? s_sum[threadIdx.x - o] : 0;
+    __syncthreads();
+    s_sum[threadIdx.x] += left;
+    __syncthreads();
+  }
+  if (d0 < digits) {
+    uint32_t at = s_sum[threadIdx.x] - sum;
+#pragma unroll
+    for (int p = 0; p < kMaxPer; ++p) {
+      if (p >= per) break;
+      uint32_t place = at + before[p];
+      at += all[p];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const uint32_t n = castle_digits[w * digits + d0 + p];
+        castle_digits[w * digits + d0 + p] = place;
+        place += n;
+      }
+    }
+  }
+  __syncthreads();
+  for (int64_t base = first; base < last; base += 64) {
+    const int64_t i = base + lane;
+    const bool there = i < last;
+    const uint32_t key = there ? key_of(a, i) : 0, d = key >> a.shift & (digits - 1);
+    uint64_t same = __ballot(there);   // lanes of the same digit
+    for (int b = 0; b < a.bits; ++b) {
+      const uint64_t ones = __ballot(d >> b & 1);
+      same &= d >> b & 1 ? ones : ~ones;
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t at = 0;
+    if (there) at = mine[d] + __popcll(same & below);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (there && (same & below) == 0) mine[d] += __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (there) {
+      a.keys[at] = key;
+      a.places[at] = a.places_in != nullptr ? a.places_in[i] : (uint32_t)i;
+    }
+  }
+}
+
+// ---- sums ----------------------------------------------------------------------------------------------------------
+struct SumArgs {
+  const uint32_t *keys, *places;
+  int64_t rows;
+  const void* dy;
+  void* dw;
+  float* parts;   // [piece][D], of pieces of one token
+  int V, D, rows_per_group;
+  float scale;
+};
+// dy rows of the sorted places first, first + step, ...
+template <typename T, int N> __device__ __forceinline__ vec<float, N> sum_places(const SumArgs& a, int64_t first, int64_t last, int step, int i) {
+  vec<float, N> acc = fill_n<N>(0.f);
+#pragma unroll 8
+  for (int64_t k = first; k < last; k += step) acc += load_n<T, N>(static_cast<const T*>(a.dy) + (int64_t)a.places[k] * a.D + i * N);
+  return acc;
+}
+// f(wave's sum of column piece i) added over the waves, in their order, handed to `out` in wave 0
+template <int N, typename F, typename G> __device__ __forceinline__ void over_waves(float* s_acc, int pieces, F&& f, G&& out) {
+  const int wave = wave_id(), lane = lane_id();
+  for (int p0 = 0; p0 < pieces; p0 += 64) {
+    const int i = p0 + lane;
+    vec<float, N> acc = fill_n<N>(0.f);
+    if (i < pieces) acc = f(i);
+    if (wave > 0)
+#pragma unroll
+      for (int e = 0; e < N; ++e) s_acc[((wave - 1) * N + e) * 64 + lane] = acc[e];
+    __syncthreads();
+    if (wave == 0 && i < pieces) {
+#pragma unroll
+      for (int w = 0; w < kWaves - 1; ++w)
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += s_acc[(w * N + e) * 64 + lane];
+      out(i, acc);
+    }
+    __syncthreads();
+  }
+}
+template <typename T, int N> __global__ __launch_bounds__(kThreads) void run_sum_kernel(SumArgs a) {
+  __shared__ float s_acc[(kWaves - 1) * N * 64];
+  const int64_t first = (int64_t)blockIdx.x * kRun;
+  const uint32_t key = a.keys[first];
+  if (key >= (uint32_t)a.V || a.keys[first + kRun - 1] != key) return;
+  over_waves<N>(s_acc, a.D / N, [&](int i) { return sum_places<T, N>(a, first + wave_id(), first + kRun, kWaves, i); },
+                [&](int i, vec<float, N> v) { *reinterpret_cast<vec<float, N>*>(a.parts + (int64_t)blockIdx.x * a.D + i * N) = v; });
+}
+
+// first sorted place whose key is not below `key`
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (keys[mid] < key) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that one wave sums by itself
+template <typename T, int N> __global__ __launch_bounds__(kThreads) void table_grad_kernel(SumArgs a) {
+  __shared__ int64_t s_start[kMaxRowsPerGroup + 1];
+  __shared__ float s_acc[(kWaves - 1) * N * 64];
+  const int v0 = blockIdx.x * a.rows_per_group, rows = min(a.rows_per_group, a.V - v0), wave = wave_id(), lane = lane_id(), pieces = a.D / N;
+  if ((int)threadIdx.x <= rows) s_start[threadIdx.x] = lower_bound(a.keys, a.rows, (uint32_t)(v0 + threadIdx.x));
+  __syncthreads();
+  auto write = [&](int v, int i, vec<float, N> acc) { store_n<T, N>(static_cast<T*>(a.dw) + (int64_t)v * a.D + i * N, acc * a.scale); };
+  for (int v = wave; v < rows; v += kWaves) {
+    const int64_t s = s_start[v], e = s_start[v + 1];
+    if (e - s > kFew) continue;
+    for (int i = lane; i < pieces; i += 64) write(v0 + v, i, sum_places<T, N>(a, s, e, 1, i));
+  }
+  for (int v = 0; v < rows; ++v) {   // by all waves: places in front of the first whole piece, whole pieces, places behind
+    const int64_t s = s_start[v], e = s_start[v + 1];
+    if (e - s <= kFew) continue;
+    const int64_t c0 = (s + kRun - 1) / kRun, c1 = e / kRun;
+    over_waves<N>(s_acc, pieces, [&](int i) {
+      if (c1 <= c0) return sum_places<T, N>(a, s + wave, e, kWaves, i);
+      vec<float, N> acc = sum_places<T, N>(a, s + wave, c0 * kRun, kWaves, i);
+#pragma unroll 4
+      for (int64_t c = c0 + wave; c < c1; c += kWaves) acc += *reinterpret_cast<const vec<float, N>*>(a.parts + c * a.D + i * N);
+      return acc + sum_places<T, N>(a, c1 * kRun + wave, e, kWaves, i);
+    }, [&](int i, vec<float, N> acc) { write(v0 + v, i, acc); });
+  }
+}
+
+// f(type, std::integral_constant elements at a time)
+template <typename F> int by_pieces(int dtype, bool whole, F&& f) {
+  return by_tensor_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (whole) return f(t, std::integral_constant<int, elem_traits<T>::vec16>());
+    return f(t, std::integral_constant<int, 1>());
+  });
+}
+bool whole_pieces(int D, int64_t ld, int dtype, std::initializer_list<const void*> ps) {
+  const int es = dtype == 0 ? 4 : 2;
+  bool whole = (int64_t)D * es % 16 == 0 && ld * es % 16 == 0;
+  for (const void* p : ps) whole = whole && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  return whole;
+}
+int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
+
+}  // namespace
+
+int launch_embedding(const EmbeddingArgs& a, int dtype, hipStream_t stream) {
+  return by_pieces(dtype, whole_pieces(a.D, a.ld, dtype, {a.table, a.y}), [&](auto t, auto n) {
+    using T = decltype(t);
+    auto go = [&](auto lpr) {
+      constexpr int LPR = decltype(lpr)::value, rows = kThreads / LPR;
+      hipLaunchKernelGGL((embedding_kernel<T, n.value, LPR>), dim3((unsigned)((a.tokens.rows + rows - 1) / rows)), dim3(kThreads), 0, stream, a);
+      return launched();
+    };
+    const int pieces = a.D / n.value;
+    if (pieces <= 16) return go(std::integral_constant<int, 16>());
+    if (pieces <= 32) return go(std::integral_constant<int, 32>());
+    return go(std::integral_constant<int, 64>());
+  });
+}
+
+SortedGradPlan sorted_grad_plan(int64_t rows, int V, int D) {
+  SortedGradPlan p = {};
+  int bits = 1;
+  while (bits < 31 && (int64_t)V >> bits != 0) ++bits;   // the keys are 0 .. V
+  p.passes = (bits + 9) / 10;
+  p.bits = (bits + p.passes - 1) / p.passes;
+  // 256 tokens to a wave until there are 256 workgroups, whose counts each of them adds up
+  const int64_t waves = std::min<int64_t>(256 * kWaves, std::max<int64_t>(1, (rows + 255) / 256));
+  p.wave_tokens = ((rows + waves - 1) / waves + 63) / 64 * 64;
+  p.groups = (int)((rows + p.wave_tokens * kWaves - 1) / (p.wave_tokens * kWaves));
+  p.rows_per_group = std::max(1, std::min(kMaxRowsPerGroup, V / 1024));
+  auto bytes = [](int64_t n) { return (n + 255) / 256 * 256; };
+  p.counts = bytes((int64_t)p.groups * (4 << p.bits));
+  p.keys = bytes(4 * rows);
+  p.places = bytes(4 * rows);
+  p.parts = bytes(rows / kRun * D * 4);
+  p.total = p.counts + 2 * (p.keys + p.places) + p.parts;
+  return p;
+}
+
+int launch_sorted_grad(const SortedGradArgs& g, int dtype, hipStream_t stream) {
+  const SortedGradPlan& p = g.plan;
+  char* at = static_cast<char*>(g.workspace);
+  auto take = [&](int64_t n) { char* r = at; at += n; return r; };
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(take(p.counts));
+  uint32_t *keys[2], *places[2];
+  for (int i = 0; i < 2; ++i) {
+    keys[i] = reinterpret_cast<uint32_t*>(take(p.keys));
+    places[i] = reinterpret_cast<uint32_t*>(take(p.places));
+  }
+  float* const parts = reinterpret_cast<float*>(take(p.parts));
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int to = pass % 2;
+    const SortArgs a = {g.tokens, g.V, g.padding, pass * p.bits, p.bits, p.wave_tokens, pass > 0 ? keys[1 - to] : nullptr, pass > 0 ? places[1 - to] : nullptr,
+                        keys[to], places[to], counts};
+    hipLaunchKernelGGL(sort_count_kernel, dim3(p.groups), dim3(kThreads), 4 << p.bits, stream, a);
+    hipLaunchKernelGGL(sort_place_kernel, dim3(p.groups), dim3(kThreads), (kWaves * 4 << p.bits) + kThreads * 4, stream, a);
+  }
+  const int sorted = (p.passes - 1) % 2;
+  const SumArgs s = {keys[sorted], places[sorted], g.tokens.rows, g.dy, g.dw, parts, g.V, g.D, p.rows_per_group, g.scale};
+  return by_pieces(dtype, whole_pieces(g.D, g.D, dtype, {g.dy, g.dw}), [&](auto t, auto n) {
+    using T = decltype(t);
+    if (s.rows >= kRun) hipLaunchKernelGGL((run_sum_kernel<T, n.value>), dim3((unsigned)(s.rows / kRun)), dim3(kThreads), 0, stream, s);
+    hipLaunchKernelGGL((table_grad_kernel<T, n.value>), dim3((unsigned)((g.V + p.rows_per_group - 1) / p.rows_per_group)), dim3(kThreads), 0, stream, s);
+    return launched();
+  });
+}
+
+}  // namespace castle

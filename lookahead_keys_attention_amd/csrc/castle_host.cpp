@@ -1018,6 +1018,142 @@ Tensor embedding(const Tensor& weight, const Tensor& index) {
   return EmbeddingFn::apply(weight, index);
 }
 
+// ---- token embedding of any vocabulary, dropout ------------------------------------------------------------------
+// token numbers as the kernels address them: the rows of a matrix, a distance apart
+struct TokenRows {
+  Tensor t;
+  int64_t n, ld;
+  explicit TokenRows(const Tensor& index) {
+    t = index.scalar_type() == at::kLong ? index : index.to(at::kLong);
+    if (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= 0 && !t.is_contiguous()) {
+      n = t.size(1);
+      ld = t.stride(0);
+      return;
+    }
+    t = t.contiguous();
+    n = ld = t.numel();
+  }
+  const int64_t* ptr() const { return static_cast<const int64_t*>(t.data_ptr()); }
+};
+void check_tokens(const Tensor& index, const Tensor& like, const char* what) {
+  TORCH_CHECK_VALUE(index.scalar_type() == at::kLong || index.scalar_type() == at::kInt, what, ": token numbers are int64 or int32, got ", index.scalar_type());
+  TORCH_CHECK_VALUE(index.device() == like.device(), what, ": the token numbers are on ", index.device(), ", the rest on ", like.device());
+}
+std::vector<int64_t> with_width(const Tensor& index, int64_t width) {
+  std::vector<int64_t> shape(index.sizes().begin(), index.sizes().end());
+  shape.push_back(width);
+  return shape;
+}
+
+Tensor embedding_op(const Tensor& weight, const Tensor& index, double scale, int64_t padding_idx) {
+  require_gpu(weight, "embedding");
+  TORCH_CHECK_VALUE(weight.dim() == 2, "embedding: the table is a matrix of (vocabulary, width)");
+  const int dtype = dtype_code(weight);
+  check_tokens(index, weight, "embedding");
+  TORCH_CHECK_VALUE(padding_idx >= -1 && padding_idx < weight.size(0), "embedding: no row ", padding_idx, " in a vocabulary of ", weight.size(0));
+  const c10::DeviceGuard guard(weight.device());
+  Tensor y = at::empty(with_width(index, weight.size(1)), weight.options());
+  if (y.numel() == 0) return y;
+  TORCH_CHECK_VALUE(weight.size(0) > 0, "embedding: tokens, but no vocabulary");
+  const Tensor table = weight.stride(1) == 1 && weight.stride(0) >= 0 ? weight : weight.contiguous();
+  const TokenRows tokens(index);
+  check(castle_embedding(table.data_ptr(), table.stride(0), (int)table.size(0), (int)table.size(1), tokens.ptr(), tokens.n, tokens.ld, index.numel(), (float)scale,
+                         y.data_ptr(), dtype, stream_of(weight)),
+        "castle_embedding");
+  return y;
+}
+Tensor embedding_bwd_op(const Tensor& dy_, const Tensor& index, int64_t vocabulary, double scale, int64_t padding_idx) {
+  require_gpu(dy_, "embedding_bwd");
+  const int dtype = dtype_code(dy_);
+  check_tokens(index, dy_, "embedding_bwd");
+  TORCH_CHECK_VALUE(dy_.dim() == index.dim() + 1 && dy_.sizes().slice(0, index.dim()) == index.sizes(), "embedding_bwd: a row for each token");
+  const c10::DeviceGuard guard(dy_.device());
+  const int64_t rows = index.numel(), width = dy_.size(-1);
+  if (dy_.numel() == 0 || vocabulary == 0) return at::zeros({vocabulary, width}, dy_.options());
+  const Tensor dy = row_major(dy_);
+  const TokenRows tokens(index);
+  const int64_t nbytes = check(castle_embedding_sorted_grad_workspace_bytes(rows, (int)vocabulary, (int)width), "castle_embedding_sorted_grad_workspace_bytes");
+  Tensor dw = at::empty({vocabulary, width}, dy.options()), ws = bytes(nbytes, dy);
+  check(castle_embedding_sorted_grad(dy.data_ptr(), tokens.ptr(), tokens.n, tokens.ld, rows, (int)vocabulary, (int)width, (float)scale, (int)padding_idx, dw.data_ptr(), dtype,
+                                     ws.data_ptr(), nbytes, stream_of(dy)),
+        "castle_embedding_sorted_grad");
+  return dw;
+}
+struct ScaledEmbeddingFn : torch::autograd::Function<ScaledEmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& index, double scale, int64_t padding_idx) {
+    static const auto op = op_handle<decltype(embedding_op)>("castle_hip::embedding");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({index});
+    ctx->saved_data["vocabulary"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding_idx"] = padding_idx;
+    return op.call(weight, index, scale, padding_idx);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    static const auto op = op_handle<decltype(embedding_bwd_op)>("castle_hip::embedding_bwd");
+    return {op.call(g[0], ctx->get_saved_variables()[0], ctx->saved_data["vocabulary"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding_idx"].toInt()),
+            Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor embedding_bwd_autograd(const Tensor& dy, const Tensor& index, int64_t vocabulary, double scale, int64_t padding_idx) {
+  static const auto op = op_handle<decltype(embedding_bwd_op)>("castle_hip::embedding_bwd");
+  const bool graph = wants_graph({dy});
+  const at::AutoDispatchBelowADInplaceOrView below;
+  const Tensor d = op.call(dy, index, vocabulary, scale, padding_idx);
+  return graph ? no_second_derivatives({d})[0] : d;
+}
+Tensor embedding_autograd(const Tensor& weight, const Tensor& index, double scale, int64_t padding_idx) {
+  if (!wants_graph({weight})) {
+    static const auto op = op_handle<decltype(embedding_op)>("castle_hip::embedding");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(weight, index, scale, padding_idx);
+  }
+  return ScaledEmbeddingFn::apply(weight, index, scale, padding_idx);
+}
+
+Tensor dropout_op(const Tensor& x_, const std::optional<Tensor>& residual_, double p, const Tensor& seed_) {
+  require_gpu(x_, "dropout_add");
+  const int dtype = dtype_code(x_);
+  TORCH_CHECK_VALUE(p >= 0 && p <= 1, "dropout_add: p is a probability, got ", p);
+  TORCH_CHECK_VALUE(seed_.scalar_type() == at::kLong && seed_.dim() == 1 && seed_.numel() == 2 && seed_.device() == x_.device(),
+                    "dropout_add: the seed is a tensor of two int64 numbers on ", x_.device());
+  TORCH_CHECK_VALUE(!residual_ || (residual_->sizes() == x_.sizes() && residual_->scalar_type() == x_.scalar_type() && residual_->device() == x_.device()),
+                    "dropout_add: the residual has the shape, type and device of x");
+  const c10::DeviceGuard guard(x_.device());
+  const Tensor x = row_major(x_), residual = residual_ ? row_major(*residual_) : Tensor(), seed = seed_.contiguous();
+  Tensor y = at::empty(x.sizes(), x.options());
+  if (y.numel() == 0) return y;
+  check(castle_dropout(x.data_ptr(), residual.defined() ? residual.data_ptr() : nullptr, y.data_ptr(), x.numel(), p, static_cast<const int64_t*>(seed.data_ptr()), dtype,
+                       stream_of(x)),
+        "castle_dropout");
+  return y;
+}
+struct DropoutFn : torch::autograd::Function<DropoutFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& residual, double p, const Tensor& seed) {
+    static const auto op = op_handle<decltype(dropout_op)>("castle_hip::dropout_add");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({seed});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["residual"] = residual.has_value();
+    return op.call(x, residual, p, seed);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {   // (linear in x: differentiable any number of times)
+    static const auto op = op_handle<decltype(dropout_op)>("castle_hip::dropout_add");
+    const bool residual = ctx->saved_data["residual"].toBool();
+    Tensor dx;
+    if (ctx->needs_input_grad(0)) dx = op.call(g[0], std::nullopt, ctx->saved_data["p"].toDouble(), ctx->get_saved_variables()[0]);
+    return {dx, residual ? g[0] : Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor dropout_autograd(const Tensor& x, const std::optional<Tensor>& residual, double p, const Tensor& seed) {
+  if (!wants_graph({x, residual.value_or(Tensor())})) {
+    static const auto op = op_handle<decltype(dropout_op)>("castle_hip::dropout_add");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(x, residual, p, seed);
+  }
+  return DropoutFn::apply(x, residual, p, seed);
+}
+
 // ---- the cached single-token step ------------------------------------------------------------------------------
 // rows of a matrix that the kernels can read 16 bytes at a time
 bool rows_readable(const Tensor& t) {
@@ -1215,6 +1351,9 @@ TORCH_LIBRARY(castle_hip, m) {
   m.def("rms_norm_bwd(Tensor dh, Tensor x, Tensor rstd, Tensor weight, bool need_x=True, bool need_w=True) -> (Tensor, Tensor)", tags);
   m.def("linear(Tensor x, Tensor weight) -> Tensor", tags);
   m.def("linear_bwd(Tensor dy, Tensor x, Tensor weight, bool need_x=True, bool need_w=True) -> (Tensor, Tensor)", tags);
+  m.def("embedding(Tensor weight, Tensor index, float scale, int padding_idx) -> Tensor", tags);
+  m.def("embedding_bwd(Tensor dy, Tensor index, int vocabulary, float scale, int padding_idx) -> Tensor", tags);
+  m.def("dropout_add(Tensor x, Tensor? residual, float p, Tensor seed) -> Tensor", tags);
 }
 TORCH_LIBRARY_IMPL(castle_hip, CUDA, m) {
   m.impl("attention", &attention);
@@ -1225,11 +1364,16 @@ TORCH_LIBRARY_IMPL(castle_hip, CUDA, m) {
   m.impl("rms_norm_bwd", &rms_norm_bwd_op);
   m.impl("linear", &linear_op);
   m.impl("linear_bwd", &linear_bwd_op);
+  m.impl("embedding", &embedding_op);
+  m.impl("embedding_bwd", &embedding_bwd_op);
+  m.impl("dropout_add", &dropout_op);
 }
 // CPU tensors: an error that says what is wrong
 TORCH_LIBRARY_IMPL(castle_hip, CPU, m) {
   m.impl("attention", &attention);
   m.impl("attention_packed", &attention_packed);
+  m.impl("embedding", &embedding_op);
+  m.impl("dropout_add", &dropout_op);
 }
 TORCH_LIBRARY_IMPL(castle_hip, Autograd, m) {
   m.impl("attention", &attention_autograd);
@@ -1240,6 +1384,9 @@ TORCH_LIBRARY_IMPL(castle_hip, Autograd, m) {
   m.impl("rms_norm_bwd", &rms_norm_bwd_autograd);
   m.impl("linear", &linear_autograd);
   m.impl("linear_bwd", &linear_bwd_autograd);
+  m.impl("embedding", &embedding_autograd);
+  m.impl("embedding_bwd", &embedding_bwd_autograd);
+  m.impl("dropout_add", &dropout_autograd);
 }
 
 PYBIND11_MODULE(_castle_host, m) {

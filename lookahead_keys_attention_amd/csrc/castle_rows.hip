@@ -6,6 +6,7 @@
 // gradients 9; here sum and norm together read two tensors and write two, and the backward pass reads three and writes
 // one (figures at the kernels).  A row belongs to a group of 16, 32 or 64 lanes of one wave, so nothing crosses waves.
 #include "castle_tiles.h"
+#include "castle_dispatch.h"
 #include "castle_rows.h"
 
 namespace castle {
@@ -324,14 +325,6 @@ template <typename F> int by_row_length(int pieces, F&& f) {
   if (pieces <= 256) return f(integral_constant<int, 64>(), integral_constant<int, 4>());
   if (pieces <= kMaxRowPieces) return f(integral_constant<int, 64>(), integral_constant<int, 8>());
   return -2;
-}
-template <typename F> int by_tensor_type(int dtype, F&& f) {
-  switch (dtype) {
-    case 0: return f(float());
-    case 1: return f(bf16_t());
-    case 2: return f(fp16_t());
-    default: return -1;
-  }
 }
 int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 

@@ -84,8 +84,10 @@ def _as_readable(t: torch.Tensor) -> torch.Tensor:
 #                                 rows of a (B,H,row_capacity,d) buffer (a cache buffer)
 #   castle_hip::rms_norm          rows, weight -> (normalised rows, their factors): the norm of a layer that is traced
 #   castle_hip::linear            rows, weight -> rows weight^T: its projections
-#   castle_hip::attention_bwd / attention_packed_bwd / rms_norm_bwd / linear_bwd   their backward passes (of the last
-#                                 two: a gradient that is not asked for comes back empty)
+#   castle_hip::embedding        table, token numbers, scale -> rows
+#   castle_hip::dropout_add      x, a residual or None, p, seed -> residual + what stays of x
+#   castle_hip::attention_bwd / attention_packed_bwd / rms_norm_bwd / linear_bwd / embedding_bwd   their backward passes
+#                                 (rms_norm_bwd, linear_bwd: a gradient that is not asked for comes back empty; dropout_add is its own)
 # `U` is an empty tensor when the lookahead keys are not asked for.  The workspace output is what
 # the backward pass needs back (operand copies, log-sum-exp), the state output the snapshots (empty
 # when they are not kept); they carry no gradient.
@@ -169,13 +171,27 @@ def _fake_linear_bwd(dy, x, weight, need_x=True, need_w=True):
     return _fake_gradients(x, weight, need_x, need_w)
 
 
+def _fake_embedding(weight, index, scale, padding_idx):
+    return torch.empty((*index.shape, weight.shape[1]), dtype=weight.dtype, device=weight.device)
+
+
+def _fake_embedding_bwd(dy, index, vocabulary, scale, padding_idx):
+    return torch.empty((vocabulary, dy.shape[-1]), dtype=dy.dtype, device=dy.device)
+
+
+def _fake_dropout_add(x, residual, p, seed):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _register_fakes():
     """Called once, when _castle_host.so has defined the operators."""
     for name, fake in (("attention", _fake_attention), ("attention_bwd", _fake_attention_bwd),
                        ("attention_packed", _fake_attention_packed), ("attention_packed_bwd", _fake_attention_packed_bwd),
                        ("rms_norm", _fake_rms_norm), ("rms_norm_bwd", _fake_rms_norm_bwd),
-                       ("linear", _fake_linear), ("linear_bwd", _fake_linear_bwd)):
-        torch.library.register_fake("castle_hip::" + name, fake)
+                       ("linear", _fake_linear), ("linear_bwd", _fake_linear_bwd),
+                       ("embedding", _fake_embedding), ("embedding_bwd", _fake_embedding_bwd), ("dropout_add", _fake_dropout_add)):
+        if hasattr(torch.ops.castle_hip, name):   # (an older build, until it is built again: the package is imported for that)
+            torch.library.register_fake("castle_hip::" + name, fake)
 
 
 def _check_range(ws):
@@ -314,6 +330,31 @@ def small_linear(x: torch.Tensor, weight: torch.Tensor, norm=None, activation=No
     if residual is not None and (residual.shape != (B, 1, weight.shape[0]) or residual.dtype != x.dtype or residual.stride(2) != 1):
         raise ValueError("small_linear: the residual must have the output's shape and type")
     return N.host().small_linear(x, weight, norm_weight, eps, 1 if activation == "gelu" else 0, residual)
+
+
+def embedding(weight: torch.Tensor, index: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
+    """scale * weight[index], rounded once: (V, D) table, token numbers of any shape -> (..., D).  The token embedding of a
+    language model (train_triton.py:86), for vocabularies of any size.
+
+    Differentiable in the table: its gradient is summed by sorted tokens, the same bits every time, with no work on the host.
+    `padding_idx`: rows of this token have no part in it.  A token outside 0 .. V - 1 gives a row of NaNs and has none either."""
+    if N._host is None:
+        N.host()
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"embedding: no row {padding_idx} in a vocabulary of {weight.shape[0]}")
+    return torch.ops.castle_hip.embedding(weight, index, float(scale), -1 if padding_idx is None else int(padding_idx))
+
+
+def dropout_add(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: torch.Tensor) -> torch.Tensor:
+    """residual + dropout(x), or dropout(x) without a residual, rounded once: an element of x stays with probability 1 - p and is divided by
+    it, p rounded to 1 / 65536.
+
+    `seed`: two int64 numbers on the GPU, which decide the mask together with an element's place and nothing else
+    (castle_dropout in include/castle_hip.h says how); the mask is not stored, the backward pass draws it again.  A call that is replayed in a
+    captured graph reads them anew: write other numbers there for another mask."""
+    if N._host is None:
+        N.host()
+    return torch.ops.castle_hip.dropout_add(x, residual, float(p), seed)
 
 
 @torch.no_grad()
