@@ -214,19 +214,21 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, 
 }
 constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that one wave sums by itself
 template <typename T, int N> __global__ __launch_bounds__(kThreads) void table_grad_kernel(SumArgs a) {
-  __shared__ int64_t s_start[kMaxRowsPerGroup + 1];
+  __shared__ int64_t s_bound[2 * kMaxRowsPerGroup];   // first place of a row and of the next one
   __shared__ float s_acc[(kWaves - 1) * N * 64];
-  const int v0 = blockIdx.x * a.rows_per_group, rows = min(a.rows_per_group, a.V - v0), wave = wave_id(), lane = lane_id(), pieces = a.D / N;
-  if ((int)threadIdx.x <= rows) s_start[threadIdx.x] = lower_bound(a.keys, a.rows, (uint32_t)(v0 + threadIdx.x));
+  // Rows gridDim.x apart: the frequent tokens of a vocabulary stand together (a workgroup to 31 rows in a row: 162 us for 16384 tokens of 512 bf16 over 32000, the one of
+  // the first tokens alone with all of it).
+  const int G = gridDim.x, rows = ((int)a.V - (int)blockIdx.x + G - 1) / G, wave = wave_id(), lane = lane_id(), pieces = a.D / N;
+  if ((int)threadIdx.x < 2 * rows) s_bound[threadIdx.x] = lower_bound(a.keys, a.rows, (uint32_t)(blockIdx.x + threadIdx.x / 2 * G + threadIdx.x % 2));
   __syncthreads();
   auto write = [&](int v, int i, vec<float, N> acc) { store_n<T, N>(static_cast<T*>(a.dw) + (int64_t)v * a.D + i * N, acc * a.scale); };
-  for (int v = wave; v < rows; v += kWaves) {
-    const int64_t s = s_start[v], e = s_start[v + 1];
+  for (int k = wave; k < rows; k += kWaves) {
+    const int64_t s = s_bound[2 * k], e = s_bound[2 * k + 1];
     if (e - s > kFew) continue;
-    for (int i = lane; i < pieces; i += 64) write(v0 + v, i, sum_places<T, N>(a, s, e, 1, i));
+    for (int i = lane; i < pieces; i += 64) write(blockIdx.x + k * G, i, sum_places<T, N>(a, s, e, 1, i));
   }
-  for (int v = 0; v < rows; ++v) {   // by all waves: places in front of the first whole piece, whole pieces, places behind
-    const int64_t s = s_start[v], e = s_start[v + 1];
+  for (int k = 0; k < rows; ++k) {   // by all waves: places in front of the first whole piece, whole pieces, places behind
+    const int64_t s = s_bound[2 * k], e = s_bound[2 * k + 1];
     if (e - s <= kFew) continue;
     const int64_t c0 = (s + kRun - 1) / kRun, c1 = e / kRun;
     over_waves<N>(s_acc, pieces, [&](int i) {
@@ -235,7 +237,7 @@ template <typename T, int N> __global__ __launch_bounds__(kThreads) void table_g
 #pragma unroll 4
       for (int64_t c = c0 + wave; c < c1; c += kWaves) acc += *reinterpret_cast<const vec<float, N>*>(a.parts + c * a.D + i * N);
       return acc + sum_places<T, N>(a, c1 * kRun + wave, e, kWaves, i);
-    }, [&](int i, vec<float, N> acc) { write(v0 + v, i, acc); });
+    }, [&](int i, vec<float, N> acc) { write(blockIdx.x + k * G, i, acc); });
   }
 }
 
