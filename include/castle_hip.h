@@ -408,6 +408,27 @@ int64_t castle_embedding_grad_workspace_bytes(int64_t rows, int vocabulary, int 
 int castle_embedding_grad(const void* dy, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows, int vocabulary, int width,
                           void* dweight, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Cross entropy of hidden rows against a vocabulary, without the logits x w^T (the end of a language model, train_triton.py:110-111, 164-171): loss r =
+ * log sum_v exp(x[r] . w[v]) - x[r] . w[target r].  x: rows of `width` elements ld_x apart, w: `vocabulary` rows ld_w apart; width and leading dimensions are multiples of 8,
+ * x and w 16-byte aligned.  Row r's target is target[(r / target_n) * target_ld + r % target_n]; rows whose target is ignore_index do not count, whatever they hold: their loss
+ * and gradient are zero.  A target outside 0 .. vocabulary - 1 makes the loss and the gradients NaN.  reduction: the mean over the rows that count (NaN if there is none), the sum, or each row's
+ * loss.  loss: one element of the type, or `rows` of them.  `state`: castle_linear_cross_entropy_state_bytes for the backward pass.
+ *
+ * _bwd: dx (rows x width) and dweight (vocabulary x width), contiguous, either may be NULL; dloss is one element, or `rows` of them.  All in a fixed order.  The logits are formed
+ * again, as many columns of the vocabulary at a time as a workspace of about 1 GB holds; 16-bit types: what is multiplied with w and x is rounded to the type, under a power of two that
+ * keeps it among its normal numbers.  gradients of _workspace_bytes: 0 for the forward pass, else the sum of 1 (dx) and 2 (dweight). */
+#define CASTLE_LOSS_MEAN 0
+#define CASTLE_LOSS_SUM 1
+#define CASTLE_LOSS_EACH 2
+int64_t castle_linear_cross_entropy_state_bytes(int rows);
+int64_t castle_linear_cross_entropy_workspace_bytes(int rows, int vocabulary, int width, int dtype, int gradients);
+int castle_linear_cross_entropy(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t target_n, int64_t target_ld, int64_t ignore_index,
+                                int rows, int vocabulary, int width, int reduction, void* loss, void* state, int64_t state_bytes, int dtype, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+int castle_linear_cross_entropy_bwd(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t target_n, int64_t target_ld, int64_t ignore_index,
+                                    int rows, int vocabulary, int width, int reduction, const void* dloss, const void* state, int64_t state_bytes, void* dx, void* dweight,
+                                    int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* y[r] = scale * table[token r] in the type `dtype`, rounded once: rows of `width` elements, `ld` apart in the table, contiguous in y; the token of row r is
  * index[(r / index_n) * index_ld + r % index_n].  A token outside 0 .. vocabulary - 1 gives a row of NaNs.  Any width and vocabulary; whole 16-byte pieces are faster.
  *

@@ -75,6 +75,10 @@ EXPORTED_SYMBOLS = (
     "castle_cross_entropy_bwd",
     "castle_embedding_grad_workspace_bytes",
     "castle_embedding_grad",
+    "castle_linear_cross_entropy_state_bytes",
+    "castle_linear_cross_entropy_workspace_bytes",
+    "castle_linear_cross_entropy",
+    "castle_linear_cross_entropy_bwd",
     "castle_embedding",
     "castle_embedding_sorted_grad_workspace_bytes",
     "castle_embedding_sorted_grad",

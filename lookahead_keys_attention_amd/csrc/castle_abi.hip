@@ -13,6 +13,7 @@
 #include "castle_profile.h"
 #include "castle_rows.h"
 #include "castle_tokens.h"
+#include "castle_vocab.h"
 #include "castle_tiles.h"
 
 namespace castle {
@@ -904,6 +905,61 @@ int castle_dropout(const void* x, const void* residual, void* y, int64_t n, doub
   const int t = (int)std::nearbyint(65536 * p);
   const castle::DropoutArgs a = {x, residual, y, seed, n, (uint32_t)t, t < 65536 ? 65536.f / (float)(65536 - t) : 0.f};
   return castle::launch_dropout(a, dtype, static_cast<hipStream_t>(stream));
+}
+
+static int vocab_sizes_ok(int rows, int vocabulary, int width) {
+  // (tiles of a product are counted in 31 bits, and 256 rows of an operand lie within 32 bits of bytes)
+  return rows > 0 && rows <= 1 << 24 && vocabulary > 0 && vocabulary <= 1 << 22 && width > 0 && width <= 1 << 16 && width % 8 == 0;
+}
+static int vocab_args(castle::VocabArgs& a, const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t target_n, int64_t target_ld,
+                      int64_t ignore_index, int rows, int vocabulary, int width, int reduction, int dtype) {
+  if (elem_size(dtype) == 0) return CASTLE_ERR_DTYPE;
+  if (!vocab_sizes_ok(rows, vocabulary, width) || target_n <= 0 || rows % target_n != 0) return CASTLE_ERR_SHAPE;
+  if (x == nullptr || w == nullptr || target == nullptr || !aligned16({x, w}) || reinterpret_cast<uintptr_t>(target) % 8 != 0 || ld_x < 0 || ld_x % 8 != 0 || ld_w < 0 ||
+      ld_w % 8 != 0 || ld_w > 1 << 22 || reduction < CASTLE_LOSS_MEAN || reduction > CASTLE_LOSS_EACH)
+    return CASTLE_ERR_ARG;
+  a = {x, w, ld_x, ld_w, target, target_n, target_ld, ignore_index, rows, vocabulary, width, reduction};
+  return CASTLE_OK;
+}
+static_assert(CASTLE_LOSS_MEAN == castle::kMeanLoss && CASTLE_LOSS_SUM == castle::kSumLoss && CASTLE_LOSS_EACH == castle::kEachLoss, "");
+
+int64_t castle_linear_cross_entropy_state_bytes(int rows) { return rows > 0 && rows <= 1 << 24 ? castle::vocab_state_bytes(rows) : CASTLE_ERR_SHAPE; }
+int64_t castle_linear_cross_entropy_workspace_bytes(int rows, int vocabulary, int width, int dtype, int gradients) {
+  const int es = elem_size(dtype);
+  if (es == 0) return CASTLE_ERR_DTYPE;
+  if (!vocab_sizes_ok(rows, vocabulary, width)) return CASTLE_ERR_SHAPE;
+  if (gradients < 0 || gradients > 3) return CASTLE_ERR_ARG;
+  castle::VocabArgs a = {};
+  a.R = rows;
+  a.V = vocabulary;
+  a.D = width;
+  return gradients == 0 ? castle::vocab_fwd_bytes(a, es) : castle::vocab_bwd_bytes(a, es, gradients & 1, gradients & 2);
+}
+static bool workspace_ok(const void* p, int64_t have, int64_t need) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % 256 == 0 && have >= need; }
+
+int castle_linear_cross_entropy(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t target_n, int64_t target_ld, int64_t ignore_index,
+                                int rows, int vocabulary, int width, int reduction, void* loss, void* state, int64_t state_bytes, int dtype, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  castle::VocabArgs a;
+  const int rc = vocab_args(a, x, ld_x, w, ld_w, target, target_n, target_ld, ignore_index, rows, vocabulary, width, reduction, dtype);
+  if (rc != CASTLE_OK) return rc;
+  if (!aligned_to({loss}, elem_size(dtype))) return CASTLE_ERR_ARG;
+  if (!workspace_ok(state, state_bytes, castle::vocab_state_bytes(rows)) || !workspace_ok(workspace, workspace_bytes, castle::vocab_fwd_bytes(a, elem_size(dtype))))
+    return CASTLE_ERR_WORKSPACE;
+  return castle::launch_vocab_fwd(a, dtype, loss, state, workspace, static_cast<hipStream_t>(stream));
+}
+
+int castle_linear_cross_entropy_bwd(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t target_n, int64_t target_ld, int64_t ignore_index,
+                                    int rows, int vocabulary, int width, int reduction, const void* dloss, const void* state, int64_t state_bytes, void* dx, void* dweight,
+                                    int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  castle::VocabArgs a;
+  const int rc = vocab_args(a, x, ld_x, w, ld_w, target, target_n, target_ld, ignore_index, rows, vocabulary, width, reduction, dtype);
+  if (rc != CASTLE_OK) return rc;
+  if (!aligned_to({dloss}, elem_size(dtype)) || !aligned16({dx, dweight}) || (dx == nullptr && dweight == nullptr)) return CASTLE_ERR_ARG;
+  if (!workspace_ok(state, state_bytes, castle::vocab_state_bytes(rows)) ||
+      !workspace_ok(workspace, workspace_bytes, castle::vocab_bwd_bytes(a, elem_size(dtype), dx != nullptr, dweight != nullptr)))
+    return CASTLE_ERR_WORKSPACE;
+  return castle::launch_vocab_bwd(a, dtype, dloss, state, dx, dweight, workspace, static_cast<hipStream_t>(stream));
 }
 
 int castle_profile_enable(int on) { return castle::profile_enable(on); }

@@ -17,6 +17,7 @@
 #include "castle_gemm.h"
 #include "castle_gelu.h"
 #include "castle_waves.h"
+#include "castle_wide.h"
 #include <algorithm>
 #include <cmath>
 #include "castle_rows.h"
@@ -339,10 +340,7 @@ template <typename T, int G> __global__ __launch_bounds__(kThreads * G, 4) void 
 // 256), the next ones on their way while one is multiplied, over the end of a tile too; the stores of a tile are not waited for.
 // 16384 rows, us, gemm_kernel / here / the library (outputs not in a cache): 512 -> 2048 59 / 43 / 45, with gelu 80 / 64 / 76; 512 -> 3072
 // 86 / 61 / 66; 512 -> 512 18 / 16 / 20; 8192 rows of 512 -> 3072 46 / 36 / 51, 3072 -> 512 49 / 44 / 39.
-// 16-byte pieces go to LDS in the order of the lanes, so rows cannot be padded: a piece takes another place in its row instead, such that
-// the lanes of a read spread over all banks (contraction-contiguous: piece p of row r at p ^ (r / 2 % 8); else the pieces of row k
-// at p ^ 4 (k % 4)).
-constexpr int kWideM = 256, kWideK = 64, kWideThreads = 512;
+constexpr int kWideM = 256;
 template <int BN> struct Wide {
   static constexpr int kStages = BN == 256 ? 2 : 3;
   static constexpr int kStage = (kWideM + BN) * kWideK * 2;   // bytes
@@ -350,48 +348,6 @@ template <int BN> struct Wide {
   // where a wave turns 32 rows of its outputs, 4 KB: behind the buffers if there is room, else in the one of the last step
   static constexpr bool kOwnTurn = BN == 256;
   static constexpr int kLds = kStages * kStage + (kOwnTurn ? 4096 * kWideThreads / 64 : 4 * kWideThreads / 64);   // and a maximum of each wave
-};
-template <typename T, bool KC, int FREE> struct WideOperand {
-  static constexpr int N = FREE / 64;   // loads of a wave
-  const T* at;
-  uint32_t off[N];   // bytes
-  __device__ __forceinline__ void start(const T* p, int64_t ld, int free0, int free_end, int k0) {
-    const int lane = lane_id(), first = wave_id() * N;
-    at = KC ? p + free0 * ld + k0 : p + k0 * ld + free0;
-#pragma unroll
-    for (int q = 0; q < N; ++q) {
-      if constexpr (KC) {
-        const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7);
-        off[q] = 2 * (uint32_t)((int)ld * min(row, free_end - 1 - free0) + 8 * piece);
-      } else {
-        constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
-        const int k = ROWS * (first + q) + lane / PIECES, piece = lane % PIECES ^ 4 * (k & 3);
-        off[q] = 2 * (uint32_t)(k * (int)ld + (free0 + 8 * piece < free_end ? 8 * piece : 0));
-      }
-    }
-  }
-  __device__ __forceinline__ void load(int64_t ld, uint32_t lds) {
-#pragma unroll
-    for (int q = 0; q < N; ++q) load_to_lds(at, off[q], lds + 1024 * (wave_id() * N + q));
-    at += KC ? kWideK : kWideK * ld;
-  }
-  // operand fragments of the wave's 32 W columns from free0, 16 contraction steps from 16 s
-  template <int W> static __device__ __forceinline__ void read(const T* lds, frag<T> (&f)[W], int free0, int s, int c, int g) {
-    if constexpr (KC) {
-      const T* p = lds + (free0 + c) * kWideK + 8 * ((2 * s + g) ^ (c >> 1 & 7));
-#pragma unroll
-      for (int i = 0; i < W; ++i) f[i] = *reinterpret_cast<const frag<T>*>(p + 32 * kWideK * i);
-    } else {
-      const int lp = c & 15, k = 16 * s + 8 * g + (lp >> 2);
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const T* p = lds + k * FREE + 32 * ((free0 / 32 + i) ^ (lp >> 2)) + 16 * (c >> 4) + 4 * (lp & 3);
-        const vec<T, 4> lo = lds_tr4<T>(p), hi = lds_tr4<T>(p + 4 * FREE);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { f[i][e] = lo[e]; f[i][4 + e] = hi[e]; }
-      }
-    }
-  }
 };
 extern __shared__ __attribute__((aligned(16))) unsigned char castle_wide[];
 
@@ -757,7 +713,7 @@ bool gemm_norm_ok(int M, int N, int K, int elem_size) {
 
 int launch_gemm(GemmArgs a, bool a_kc, bool b_kc, int dtype, float* workspace, hipStream_t stream) {
   const int es = dtype == 0 ? 4 : 2, step = dtype == 0 ? 32 : kStep16;
-  Plan p = plan(a.M, a.N, a.K, a.epilogue == kGemmPlain || a.amax != nullptr, es);   // (the slots of the maxima follow from the plain plan)
+  Plan p = plan(a.M, a.N, a.K, (a.epilogue == kGemmPlain && !a.whole) || a.amax != nullptr, es);   // (the slots of the maxima follow from the plain plan)
   a.k_per_split = ((a.K + p.splits - 1) / p.splits + step - 1) / step * step;
   p.splits = (a.K + a.k_per_split - 1) / a.k_per_split;   // rounding up may leave the last ones empty
   a.part = p.splits > 1 ? workspace : nullptr;

@@ -16,6 +16,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
+#include <limits>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -1018,7 +1019,6 @@ Tensor embedding(const Tensor& weight, const Tensor& index) {
   return EmbeddingFn::apply(weight, index);
 }
 
-// ---- token embedding of any vocabulary, dropout ------------------------------------------------------------------
 // token numbers as the kernels address them: the rows of a matrix, a distance apart
 struct TokenRows {
   Tensor t;
@@ -1039,6 +1039,114 @@ void check_tokens(const Tensor& index, const Tensor& like, const char* what) {
   TORCH_CHECK_VALUE(index.scalar_type() == at::kLong || index.scalar_type() == at::kInt, what, ": token numbers are int64 or int32, got ", index.scalar_type());
   TORCH_CHECK_VALUE(index.device() == like.device(), what, ": the token numbers are on ", index.device(), ", the rest on ", like.device());
 }
+
+// ---- cross entropy against a vocabulary, without the logits --------------------------------------------------------
+// rows of a matrix that the kernels can read 16 bytes at a time, as far as eight elements are that or a multiple
+Tensor rows_of_eight(const Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) >= 0 && t.stride(0) % 8 == 0 && t.stride(0) <= 1 << 22 && aligned16(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+struct VocabCall {
+  Tensor x, w;
+  TokenRows target;
+  int rows, vocabulary, width, dtype;
+  VocabCall(const Tensor& x_, const Tensor& weight, const Tensor& target_, int64_t reduction)
+      : target((check_tokens(target_, x_, "linear_cross_entropy"), target_)) {
+    dtype = dtype_code(x_);
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x_.size(-1) && weight.scalar_type() == x_.scalar_type() && weight.device() == x_.device(),
+                      "linear_cross_entropy: x is (..., D) and the weight (V, D), of one type on one device");
+    TORCH_CHECK_VALUE(target_.sizes() == x_.sizes().slice(0, x_.dim() - 1), "linear_cross_entropy: a target for each row of x");
+    TORCH_CHECK_VALUE(reduction >= CASTLE_LOSS_MEAN && reduction <= CASTLE_LOSS_EACH, "linear_cross_entropy: unknown reduction");
+    TORCH_CHECK_VALUE(weight.size(0) > 0 && weight.size(0) <= 1 << 22, "linear_cross_entropy: a vocabulary of 1 to 2^22, got ", weight.size(0));
+    TORCH_CHECK_VALUE(weight.size(1) > 0 && weight.size(1) <= 1 << 16 && weight.size(1) % 8 == 0, "linear_cross_entropy: a width of 8, 16 ... 65536, got ", weight.size(1));
+    TORCH_CHECK_VALUE(target_.numel() <= 1 << 24, "linear_cross_entropy: at most 2^24 rows, got ", target_.numel());
+    rows = (int)target_.numel();
+    vocabulary = (int)weight.size(0);
+    width = (int)weight.size(1);
+    x = rows_of_eight(x_.reshape({rows, width}));
+    w = rows_of_eight(weight);
+  }
+};
+std::tuple<Tensor, Tensor> linear_cross_entropy_op(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t reduction, int64_t ignore_index) {
+  require_gpu(x, "linear_cross_entropy");
+  const c10::DeviceGuard guard(x.device());
+  const VocabCall c(x, weight, target, reduction);
+  Tensor loss = reduction == CASTLE_LOSS_EACH ? at::empty(target.sizes(), x.options()) : at::empty({}, x.options());
+  if (c.rows == 0) {
+    if (reduction != CASTLE_LOSS_EACH) loss.fill_(reduction == CASTLE_LOSS_MEAN ? std::numeric_limits<double>::quiet_NaN() : 0.0);
+    return {loss, bytes(0, x)};
+  }
+  const int64_t sbytes = check(castle_linear_cross_entropy_state_bytes(c.rows), "castle_linear_cross_entropy_state_bytes");
+  const int64_t nbytes = check(castle_linear_cross_entropy_workspace_bytes(c.rows, c.vocabulary, c.width, c.dtype, 0), "castle_linear_cross_entropy_workspace_bytes");
+  Tensor state = bytes(sbytes, x), ws = bytes(nbytes, x);
+  check(castle_linear_cross_entropy(c.x.data_ptr(), c.x.stride(0), c.w.data_ptr(), c.w.stride(0), c.target.ptr(), c.target.n, c.target.ld, ignore_index, c.rows, c.vocabulary,
+                                    c.width, (int)reduction, loss.data_ptr(), state.data_ptr(), sbytes, c.dtype, ws.data_ptr(), nbytes, stream_of(x)),
+        "castle_linear_cross_entropy");
+  return {loss, state};
+}
+// (a gradient that is not asked for comes back empty)
+std::tuple<Tensor, Tensor> linear_cross_entropy_bwd_op(const Tensor& dloss_, const Tensor& x, const Tensor& weight, const Tensor& target, const Tensor& state, int64_t reduction,
+                                                       int64_t ignore_index, bool need_x, bool need_w) {
+  require_gpu(x, "linear_cross_entropy_bwd");
+  const c10::DeviceGuard guard(x.device());
+  const VocabCall c(x, weight, target, reduction);
+  TORCH_CHECK_VALUE(dloss_.scalar_type() == x.scalar_type() && dloss_.device() == x.device() && dloss_.numel() == (reduction == CASTLE_LOSS_EACH ? c.rows : 1),
+                    "linear_cross_entropy_bwd: the loss has another shape, type or device");
+  Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  Tensor dw = need_w ? at::empty(weight.sizes(), weight.options()) : at::empty({0}, weight.options());
+  if (c.rows == 0 && need_w) dw.zero_();
+  if (c.rows == 0 || (!need_x && !need_w)) return {dx, dw};
+  const Tensor dloss = dloss_.contiguous();
+  const int64_t nbytes = check(castle_linear_cross_entropy_workspace_bytes(c.rows, c.vocabulary, c.width, c.dtype, (need_x ? 1 : 0) + (need_w ? 2 : 0)),
+                               "castle_linear_cross_entropy_workspace_bytes");
+  Tensor ws = bytes(nbytes, x);
+  check(castle_linear_cross_entropy_bwd(c.x.data_ptr(), c.x.stride(0), c.w.data_ptr(), c.w.stride(0), c.target.ptr(), c.target.n, c.target.ld, ignore_index, c.rows, c.vocabulary,
+                                        c.width, (int)reduction, dloss.data_ptr(), state.data_ptr(), state.numel(), need_x ? dx.data_ptr() : nullptr,
+                                        need_w ? dw.data_ptr() : nullptr, c.dtype, ws.data_ptr(), nbytes, stream_of(x)),
+        "castle_linear_cross_entropy_bwd");
+  return {dx, dw};
+}
+struct LinearCrossEntropyFn : torch::autograd::Function<LinearCrossEntropyFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& target, int64_t reduction, int64_t ignore_index) {
+    static const auto op = op_handle<decltype(linear_cross_entropy_op)>("castle_hip::linear_cross_entropy");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    auto [loss, state] = op.call(x, weight, target, reduction, ignore_index);
+    ctx->save_for_backward({x, weight, target, state});
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->mark_non_differentiable({state});
+    ctx->set_materialize_grads(false);
+    return {loss, state};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    static const auto op = op_handle<decltype(linear_cross_entropy_bwd_op)>("castle_hip::linear_cross_entropy_bwd");
+    if (!g[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto s = ctx->get_saved_variables();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    auto [dx, dw] = op.call(g[0], s[0], s[1], s[2], s[3], ctx->saved_data["reduction"].toInt(), ctx->saved_data["ignore_index"].toInt(), need_x, need_w);
+    return {need_x ? dx : Tensor(), need_w ? dw : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+std::tuple<Tensor, Tensor> linear_cross_entropy_bwd_autograd(const Tensor& dloss, const Tensor& x, const Tensor& weight, const Tensor& target, const Tensor& state,
+                                                             int64_t reduction, int64_t ignore_index, bool need_x, bool need_w) {
+  static const auto op = op_handle<decltype(linear_cross_entropy_bwd_op)>("castle_hip::linear_cross_entropy_bwd");
+  const bool graph = wants_graph({dloss, x, weight});
+  const at::AutoDispatchBelowADInplaceOrView below;
+  const auto [dx, dw] = op.call(dloss, x, weight, target, state, reduction, ignore_index, need_x, need_w);
+  if (!graph) return {dx, dw};
+  const auto r = no_second_derivatives({dx, dw});
+  return {r[0], r[1]};
+}
+std::tuple<Tensor, Tensor> linear_cross_entropy_autograd(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t reduction, int64_t ignore_index) {
+  if (!wants_graph({x, weight})) {
+    static const auto op = op_handle<decltype(linear_cross_entropy_op)>("castle_hip::linear_cross_entropy");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(x, weight, target, reduction, ignore_index);
+  }
+  auto r = LinearCrossEntropyFn::apply(x, weight, target, reduction, ignore_index);
+  return {r[0], r[1]};
+}
+
+// ---- token embedding of any vocabulary, dropout ------------------------------------------------------------------
 std::vector<int64_t> with_width(const Tensor& index, int64_t width) {
   std::vector<int64_t> shape(index.sizes().begin(), index.sizes().end());
   shape.push_back(width);
@@ -1351,6 +1459,9 @@ TORCH_LIBRARY(castle_hip, m) {
   m.def("rms_norm_bwd(Tensor dh, Tensor x, Tensor rstd, Tensor weight, bool need_x=True, bool need_w=True) -> (Tensor, Tensor)", tags);
   m.def("linear(Tensor x, Tensor weight) -> Tensor", tags);
   m.def("linear_bwd(Tensor dy, Tensor x, Tensor weight, bool need_x=True, bool need_w=True) -> (Tensor, Tensor)", tags);
+  m.def("linear_cross_entropy(Tensor x, Tensor weight, Tensor target, int reduction, int ignore_index) -> (Tensor, Tensor)", tags);
+  m.def("linear_cross_entropy_bwd(Tensor dloss, Tensor x, Tensor weight, Tensor target, Tensor state, int reduction, int ignore_index, bool need_x=True, bool need_w=True) "
+        "-> (Tensor, Tensor)", tags);
   m.def("embedding(Tensor weight, Tensor index, float scale, int padding_idx) -> Tensor", tags);
   m.def("embedding_bwd(Tensor dy, Tensor index, int vocabulary, float scale, int padding_idx) -> Tensor", tags);
   m.def("dropout_add(Tensor x, Tensor? residual, float p, Tensor seed) -> Tensor", tags);
@@ -1364,6 +1475,8 @@ TORCH_LIBRARY_IMPL(castle_hip, CUDA, m) {
   m.impl("rms_norm_bwd", &rms_norm_bwd_op);
   m.impl("linear", &linear_op);
   m.impl("linear_bwd", &linear_bwd_op);
+  m.impl("linear_cross_entropy", &linear_cross_entropy_op);
+  m.impl("linear_cross_entropy_bwd", &linear_cross_entropy_bwd_op);
   m.impl("embedding", &embedding_op);
   m.impl("embedding_bwd", &embedding_bwd_op);
   m.impl("dropout_add", &dropout_op);
@@ -1372,6 +1485,7 @@ TORCH_LIBRARY_IMPL(castle_hip, CUDA, m) {
 TORCH_LIBRARY_IMPL(castle_hip, CPU, m) {
   m.impl("attention", &attention);
   m.impl("attention_packed", &attention_packed);
+  m.impl("linear_cross_entropy", &linear_cross_entropy_op);
   m.impl("embedding", &embedding_op);
   m.impl("dropout_add", &dropout_op);
 }
@@ -1384,6 +1498,8 @@ TORCH_LIBRARY_IMPL(castle_hip, Autograd, m) {
   m.impl("rms_norm_bwd", &rms_norm_bwd_autograd);
   m.impl("linear", &linear_autograd);
   m.impl("linear_bwd", &linear_bwd_autograd);
+  m.impl("linear_cross_entropy", &linear_cross_entropy_autograd);
+  m.impl("linear_cross_entropy_bwd", &linear_cross_entropy_bwd_autograd);
   m.impl("embedding", &embedding_autograd);
   m.impl("embedding_bwd", &embedding_bwd_autograd);
   m.impl("dropout_add", &dropout_autograd);

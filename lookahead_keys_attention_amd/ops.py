@@ -84,10 +84,11 @@ def _as_readable(t: torch.Tensor) -> torch.Tensor:
 #                                 rows of a (B,H,row_capacity,d) buffer (a cache buffer)
 #   castle_hip::rms_norm          rows, weight -> (normalised rows, their factors): the norm of a layer that is traced
 #   castle_hip::linear            rows, weight -> rows weight^T: its projections
+#   castle_hip::linear_cross_entropy   rows, weight, classes -> (loss, what its backward pass needs back)
 #   castle_hip::embedding        table, token numbers, scale -> rows
 #   castle_hip::dropout_add      x, a residual or None, p, seed -> residual + what stays of x
-#   castle_hip::attention_bwd / attention_packed_bwd / rms_norm_bwd / linear_bwd / embedding_bwd   their backward passes
-#                                 (rms_norm_bwd, linear_bwd: a gradient that is not asked for comes back empty; dropout_add is its own)
+#   castle_hip::attention_bwd / attention_packed_bwd / rms_norm_bwd / linear_bwd / linear_cross_entropy_bwd / embedding_bwd   their backward passes
+#                                 (rms_norm_bwd, linear_bwd, linear_cross_entropy_bwd: a gradient that is not asked for comes back empty; dropout_add is its own)
 # `U` is an empty tensor when the lookahead keys are not asked for.  The workspace output is what
 # the backward pass needs back (operand copies, log-sum-exp), the state output the snapshots (empty
 # when they are not kept); they carry no gradient.
@@ -171,6 +172,21 @@ def _fake_linear_bwd(dy, x, weight, need_x=True, need_w=True):
     return _fake_gradients(x, weight, need_x, need_w)
 
 
+LOSS_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+
+
+def _fake_linear_cross_entropy(x, weight, target, reduction, ignore_index):
+    rows = target.numel()
+    # three parts of whole 256 bytes: two numbers, and for each row its place among those that count and its log-sum-exp
+    nbytes = 256 + 2 * ((4 * rows + 255) // 256 * 256) if rows else 0
+    return (torch.empty(target.shape if reduction == LOSS_REDUCTIONS["none"] else (), dtype=x.dtype, device=x.device),
+            torch.empty(nbytes, dtype=torch.uint8, device=x.device))
+
+
+def _fake_linear_cross_entropy_bwd(dloss, x, weight, target, state, reduction, ignore_index, need_x=True, need_w=True):
+    return _fake_gradients(x, weight, need_x, need_w)
+
+
 def _fake_embedding(weight, index, scale, padding_idx):
     return torch.empty((*index.shape, weight.shape[1]), dtype=weight.dtype, device=weight.device)
 
@@ -189,6 +205,7 @@ def _register_fakes():
                        ("attention_packed", _fake_attention_packed), ("attention_packed_bwd", _fake_attention_packed_bwd),
                        ("rms_norm", _fake_rms_norm), ("rms_norm_bwd", _fake_rms_norm_bwd),
                        ("linear", _fake_linear), ("linear_bwd", _fake_linear_bwd),
+                       ("linear_cross_entropy", _fake_linear_cross_entropy), ("linear_cross_entropy_bwd", _fake_linear_cross_entropy_bwd),
                        ("embedding", _fake_embedding), ("embedding_bwd", _fake_embedding_bwd), ("dropout_add", _fake_dropout_add)):
         if hasattr(torch.ops.castle_hip, name):   # (an older build, until it is built again: the package is imported for that)
             torch.library.register_fake("castle_hip::" + name, fake)
@@ -330,6 +347,20 @@ def small_linear(x: torch.Tensor, weight: torch.Tensor, norm=None, activation=No
     if residual is not None and (residual.shape != (B, 1, weight.shape[0]) or residual.dtype != x.dtype or residual.stride(2) != 1):
         raise ValueError("small_linear: the residual must have the output's shape and type")
     return N.host().small_linear(x, weight, norm_weight, eps, 1 if activation == "gelu" else 0, residual)
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduction: str = "mean", ignore_index: int = -100) -> torch.Tensor:
+    """F.cross_entropy(x @ weight.T, target) of hidden rows x (..., D), a vocabulary (V, D) and classes (...), without the logits in memory
+    (the end of a language model, train_triton.py:164-171): what it keeps for the backward pass is one number per row.
+
+    Sums and the loss are formed in 32 bits from unrounded logits; the result has the type of x.  reduction: "mean" over the rows that count,
+    "sum", or "none" for the loss of each row, shaped like `target`.  Rows of class `ignore_index` cost nothing and have no part in anything, whatever they
+    hold.  A class outside 0 .. V - 1 makes the loss and the gradients NaN.  Differentiable in x and weight, once; D is a multiple of 8."""
+    if N._host is None:
+        N.host()
+    if reduction not in LOSS_REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}")
+    return torch.ops.castle_hip.linear_cross_entropy(x, weight, target, LOSS_REDUCTIONS[reduction], int(ignore_index))[0]
 
 
 def embedding(weight: torch.Tensor, index: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
