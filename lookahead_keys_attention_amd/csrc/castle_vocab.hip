@@ -25,7 +25,7 @@ namespace {
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 constexpr int kWaves = kThreads / 64;
 constexpr int kCountRows = 1024;   // rows of a workgroup that counts
-constexpr int kGatherRows = 64;    // rows of a workgroup that copies
+constexpr int kGatherRows = 16;    // rows of a workgroup that copies
 constexpr int kLossRows = 16;      // rows of a workgroup that joins maxima and sums
 
 // Where maxima start: a score of -inf has weight 0 behind it wherever it stands, and log2(e) times it is finite.
@@ -92,22 +92,24 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
     before = sum_over_threads<kWaves>(before, s);
     all = sum_over_threads<kWaves>(total, s);
     if (wave_id() == 0) {
-      const int64_t r = first + lane_id(), t = r < a.v.R ? class_of(a.v, r) : a.v.ignore;
+      const int64_t r = first + lane_id();
+      const bool mine = lane_id() < kGatherRows, there = mine && r < a.v.R;
+      const int64_t t = there ? class_of(a.v, r) : a.v.ignore;
       const bool counts = t != a.v.ignore;
       const uint64_t mask = __ballot(counts);
       const int rank = counts ? before + __popcll(mask & ((1ull << lane_id()) - 1)) : -1;
-      s_rank[lane_id()] = rank;
-      if (r < a.v.R) a.rank[r] = rank;
+      if (mine) s_rank[lane_id()] = rank;
+      if (there) a.rank[r] = rank;
       if (counts) {
         a.tc[rank] = t >= 0 && t < a.v.V ? (int32_t)t : -1;
         a.tl[rank] = NAN;
       }
-      if (a.v.reduction == kEachLoss && !counts && r < a.v.R) static_cast<T*>(a.loss)[r] = (T)0.f;
+      if (a.v.reduction == kEachLoss && there && !counts) static_cast<T*>(a.loss)[r] = (T)0.f;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.head = {all, 1.f / (float)all};
   } else {
     all = a.head->count;
-    if (wave_id() == 0) {
+    if (threadIdx.x < kGatherRows) {
       const int64_t r = first + lane_id();
       const int rank = r < a.v.R ? a.rank[r] : -1;
       s_rank[lane_id()] = rank;
@@ -129,7 +131,7 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
 #pragma unroll 4
       for (int i = lane_id(); i < pieces; i += 64) *reinterpret_cast<vt*>(to + i * V) = i < have ? *reinterpret_cast<const vt*>(from + i * V) : none;
     }
-    const int64_t r = first + k;   // (the last workgroup reaches to the next multiple of 64)
+    const int64_t r = first + k;   // (the workgroups reach to the next multiple of 64)
     if (r >= all && r < zero_end) {
       T* to = static_cast<T*>(a.xc) + r * a.Dp;
       for (int i = lane_id(); i < pieces; i += 64) *reinterpret_cast<vt*>(to + i * V) = none;
@@ -239,6 +241,10 @@ template <typename T> __global__ __launch_bounds__(1024) void factor_kernel(Fact
   }
 }
 
+// steps of each range of a contraction that is split, the last one may have fewer
+__host__ __device__ constexpr int steps_of_range(int steps, int splits) { return steps > 0 ? (steps + splits - 1) / splits : 1; }
+__host__ __device__ constexpr int ranges(int steps, int splits) { return (steps + steps_of_range(steps, splits) - 1) / steps_of_range(steps, splits); }
+
 // dx[r] = 2^-shift times the sum of its partial results, zeros where it does not count
 struct JoinArgs {
   const float* parts;   // [splits][R][D]
@@ -247,6 +253,7 @@ struct JoinArgs {
   void* out;
   int splits, D;
   int64_t R;
+  const int* count;     // nullptr, or the contraction: there are as many partial results as it has ranges
 };
 template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kernel(JoinArgs a) {
   typedef vec<float, 4> v4;
@@ -257,9 +264,10 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kern
   const int c = (int)(i - r * per) * 4, rank = a.rank == nullptr ? (int)r : a.rank[r];
   v4 v = {0.f, 0.f, 0.f, 0.f};
   if (rank >= 0) {
+    const int splits = a.count != nullptr ? ranges((*a.count + kWideK - 1) / kWideK, a.splits) : a.splits;
     const float* p = a.parts + (int64_t)rank * a.D + c;
 #pragma unroll 4
-    for (int k = 0; k < a.splits; ++k) v += *reinterpret_cast<const v4*>(p + k * a.R * a.D);
+    for (int k = 0; k < splits; ++k) v += *reinterpret_cast<const v4*>(p + k * a.R * a.D);
     const int shift = *a.shift;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -shift);
@@ -277,7 +285,7 @@ struct ProductArgs {
   int64_t lda, ldb;
   int M, N, K;             // kWeightGrad: K is an upper bound, else M
   const int* count;        // rows that count
-  int splits;
+  int splits;              // ranges of the contraction, at most
   // kStats
   vec<float, 2>* parts;
   float* tl;
@@ -296,6 +304,35 @@ struct ProductArgs {
   const int* shift;
 };
 
+// d lies in blocks of 64 x 64, whole rows of blocks one behind the other: a step of either product that reads it fetches pieces of 8 KB.  (Rows of d as they are: 128 bytes here and
+// there, 64 KB and more apart; dx of 16384 rows over 32000 503 us, dweight 468.)
+constexpr int kBlock = 64;
+template <typename T, bool KC, int FREE> struct BlockOperand : WideOperand<T, KC, FREE> {
+  typedef WideOperand<T, KC, FREE> W;
+  // p: [row of blocks][ldc / 64][64][64]
+  __device__ __forceinline__ void start(const T* p, int64_t ldc, int free0, int free_end, int k0) {
+    const int lane = lane_id(), first = wave_id() * W::N;
+    W::left = free_end - free0;
+    W::at = KC ? p + free0 * ldc + k0 * kBlock : p + k0 * ldc + free0 * kBlock;
+#pragma unroll
+    for (int q = 0; q < W::N; ++q) {
+      if constexpr (KC) {
+        const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7), there = min(row, W::left - 1);
+        W::off[q] = 2 * (uint32_t)(there / kBlock * kBlock * (int)ldc + there % kBlock * kBlock + 8 * piece);
+      } else {
+        constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
+        const int k = ROWS * (first + q) + lane / PIECES, p = lane % PIECES ^ 4 * (k & 3), piece = 8 * p < W::left ? p : 0;
+        W::off[q] = 2 * (uint32_t)(piece / 8 * kBlock * kBlock + k * kBlock + 8 * (piece % 8));
+      }
+    }
+  }
+  __device__ __forceinline__ void load(int64_t ldc, uint32_t lds) {
+#pragma unroll
+    for (int q = 0; q < W::N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * W::N + q));
+    W::at += kBlock * (KC ? (int64_t)kBlock : ldc);
+  }
+};
+
 // Eight waves over BM x BN: four by two of them for 256 rows, else two by four.
 template <int MODE, int BM, int BN> struct Shape {
   static constexpr int WM = BM == 256 ? 4 : 2, WN = 8 / WM, FM = BM / 32 / WM, FN = BN / 32 / WN;
@@ -303,6 +340,7 @@ template <int MODE, int BM, int BN> struct Shape {
   static constexpr int kStage = (BM + BN) * kWideK * 2, kTurnBytes = kTurn ? 4096 * 8 : 0;
   static constexpr int kFit = (kMaxLds - kTurnBytes) / kStage, kStages = kFit < 3 ? kFit : 3;
   static constexpr int kLoads = kStage / 1024 / 8, kLds = kStages * kStage + kTurnBytes;
+  static constexpr int kStores = MODE == kStats ? FM : MODE == kRowGrad ? 4 * FM * FN : 2 * FM * FN;   // of a wave and tile (kWeightGrad: partial results are twice as many)
   static_assert(kStages >= 2 && FM >= 1 && FN >= 1, "");
 };
 extern __shared__ __attribute__((aligned(16))) unsigned char castle_vocab_lds[];
@@ -310,65 +348,98 @@ extern __shared__ __attribute__((aligned(16))) unsigned char castle_vocab_lds[];
 template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
   typedef Shape<MODE, BM, BN> S;
   constexpr bool AK = MODE != kWeightGrad, BKC = MODE == kStats || MODE == kGrad;
-  typedef WideOperand<T, AK, BM> OpA;
+  typedef std::conditional_t<MODE == kRowGrad || MODE == kWeightGrad, BlockOperand<T, AK, BM>, WideOperand<T, AK, BM>> OpA;
   typedef WideOperand<T, BKC, BN> OpB;
   typedef vec<T, 8> vt;
   const int lane = lane_id(), wave = wave_id(), c = lane & 31, g = lane >> 5;
   const int count = __builtin_amdgcn_readfirstlane(*a.count), M = MODE == kWeightGrad ? a.M : min(a.M, count), K = MODE == kWeightGrad ? (int)up(min(a.K, count), kWideK) : a.K;
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
-  // tiles in the order of an XCD's L2: all rows of a band of columns, then those of the next
+  if (tiles == 0) return;
+  // Items are tiles for each range of the contraction; XCD x takes the x-th eighth of them.  Tiles in the order of an XCD's L2: all rows of a band of columns, then those of the next.
   constexpr int kBand = 2048 / BN;
-  auto place = [&](int t, int& m0, int& n0) __attribute__((always_inline)) {
-    const int band = t / (tiles_m * kBand), rest = t - band * tiles_m * kBand, width = min(kBand, tiles_n - band * kBand);
-    m0 = rest / width * BM;
-    n0 = (band * kBand + rest % width) * BN;
-  };
-  const int share = (tiles + 7) / 8, begin = blockIdx.x % 8 * share, last = min(tiles, begin + share), stride = gridDim.x / 8;
-  const int wm = wave / S::WN * 32 * S::FM, wn = wave % S::WN * 32 * S::FN;
-  const int all_steps = (K + kWideK - 1) / kWideK, per_split = (all_steps + a.splits - 1) / a.splits;
-  const int step0 = blockIdx.y * per_split, steps = max(0, min(all_steps, step0 + per_split) - step0), k0 = step0 * kWideK;
-  int tile = begin + blockIdx.x / 8;
-  if (tile >= last) return;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)castle_vocab_lds;
-  // the step that is requested next runs ahead of the one that is multiplied, into the next tile
-  OpA ra;
-  OpB rb;
-  int next_tile = tile, next_step = 0, ahead = 0;   // ahead: steps requested and not waited for
-  auto start = [&]() __attribute__((always_inline)) {
-    int m0, n0;
-    place(next_tile, m0, n0);
-    ra.start(static_cast<const T*>(a.a), a.lda, m0, M, k0);
-    rb.start(static_cast<const T*>(a.b), a.ldb, n0, a.N, k0);
-  };
-  auto request = [&](int buffer) __attribute__((always_inline)) {
-    if (next_tile >= last) return;
-    ++ahead;
-    if constexpr (MODE != kWeightGrad)
-      if (k0 + (next_step + 1) * kWideK > K) rb.place((int)a.ldb, K - k0 - next_step * kWideK);
-    ra.load(a.lda, lds0 + buffer);
-    rb.load(a.ldb, lds0 + buffer + BM * kWideK * 2);
-    if (++next_step == steps) {
-      next_step = 0;
-      next_tile += stride;
-      if (next_tile < last) start();
+  const int all_steps = (K + kWideK - 1) / kWideK, per_range = steps_of_range(all_steps, a.splits);
+  const int items = tiles * max(1, ranges(all_steps, a.splits));
+  // The place of an item, moved on by additions: divisions by the sizes took a tenth of what 16384 x 32000 logits of 512 take.
+  struct Walk { int band, rest, range; };   // rest: tile of the band
+  const int bands = (tiles_n + kBand - 1) / kBand;
+  auto advance = [&](Walk& w, int by) __attribute__((always_inline)) {
+    w.rest += by;
+    while (true) {
+      const int size = tiles_m * min(kBand, tiles_n - w.band * kBand);
+      if (w.rest < size) break;
+      w.rest -= size;
+      if (++w.band == bands) {
+        w.band = 0;
+        ++w.range;
+      }
     }
   };
-  if (steps > 0) {
+  struct Item { int m0, n0, range, k0, steps; };
+  auto item_at = [&](const Walk& w) __attribute__((always_inline)) {
+    const int width = min(kBand, tiles_n - w.band * kBand), m = width == kBand ? w.rest / kBand : w.rest / width;
+    return Item{m * BM, (w.band * kBand + w.rest - m * width) * BN, w.range, w.range * per_range * kWideK, min(per_range, all_steps - w.range * per_range)};
+  };
+  const int share = (items + 7) / 8, begin = blockIdx.x % 8 * share, last = min(items, begin + share), stride = gridDim.x / 8;
+  const int wm = wave / S::WN * 32 * S::FM, wn = wave % S::WN * 32 * S::FN;
+  int item = begin + blockIdx.x / 8;
+  if (item >= last) return;
+  const bool any = all_steps > 0;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)castle_vocab_lds;
+  // the step that is requested next runs ahead of the one that is multiplied, into the next item
+  OpA ra;
+  OpB rb;
+  Walk at = {0, 0, 0};
+  advance(at, item);
+  Walk next_at = at;
+  int next_item = item, next_steps = 0, next_k = 0, ahead = 0;   // ahead: steps requested and not waited for
+  auto start = [&]() __attribute__((always_inline)) {
+    const Item t = item_at(next_at);
+    next_steps = t.steps;
+    next_k = t.k0;
+    ra.start(static_cast<const T*>(a.a), a.lda, t.m0, M, t.k0);
+    rb.start(static_cast<const T*>(a.b), a.ldb, t.n0, a.N, t.k0);
+  };
+  auto request = [&](int buffer) __attribute__((always_inline)) {
+    if (next_item >= last) return;
+    ++ahead;
+    if constexpr (MODE != kWeightGrad)
+      if (next_k + kWideK > K) rb.place((int)a.ldb, K - next_k);
+    ra.load(a.lda, lds0 + buffer);
+    rb.load(a.ldb, lds0 + buffer + BM * kWideK * 2);
+    next_k += kWideK;
+    if (--next_steps == 0) {
+      next_item += stride;
+      if (next_item < last) {
+        advance(next_at, stride);
+        start();
+      }
+    }
+  };
+  if (any) {
     start();
     request(0);
     request(S::kStage);
     if constexpr (S::kStages == 3) request(2 * S::kStage);
   }
-  // The step behind the current one is in LDS, from every wave, and all have read the current one.  Waits are for all but the last so many requests; loads and stores of the
-  // end of a tile only make them stricter.
+  // The step behind the current one is in LDS, from every wave, and all have read the current one.  Waits are for all but the last so many requests; the stores of a
+  // tile inside the output, kStores at least, come behind those and are not waited for (`stored`).
+  bool stored = false;
   auto arrive = [&]() __attribute__((always_inline)) {
     auto wait = [&](auto n) __attribute__((always_inline)) {
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(n)::value) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(n)::value < 63 ? decltype(n)::value : 63) : "memory");
     };
     const int newer = ahead - 1;   // steps
-    if (newer > 1) wait(std::integral_constant<int, 2 * S::kLoads>());
-    else if (newer == 1) wait(std::integral_constant<int, S::kLoads>());
-    else wait(std::integral_constant<int, 0>());
+    if (newer > 1) {
+      if (stored) wait(std::integral_constant<int, 2 * S::kLoads + S::kStores>());
+      else wait(std::integral_constant<int, 2 * S::kLoads>());
+    } else if (newer == 1) {
+      if (stored) wait(std::integral_constant<int, S::kLoads + S::kStores>());
+      else wait(std::integral_constant<int, S::kLoads>());
+    } else {
+      if (stored) wait(std::integral_constant<int, S::kStores>());
+      else wait(std::integral_constant<int, 0>());
+    }
+    stored = false;
     --ahead;
   };
   int buffer = 0;
@@ -379,13 +450,35 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
     OpB::read(la + BM * kWideK, fb[slot], wn, s, c, g);
     __builtin_amdgcn_sched_barrier(0);   // these reads, then the products of the fragments before
   };
-  if (steps > 0) {
-    arrive();
-    read(0, 0);
-  }
-  while (tile < last) {
-    int m0, n0;
-    place(tile, m0, n0);
+  if (any) arrive();
+  while (item < last) {
+    const auto [m0, n0, range, k0, steps] = item_at(at);
+    // What the end of a tile needs of its rows: requested here, there behind the last wait for operands, and the next operands only behind that (the wait for these would
+    // include them).
+    float l[S::FM], f[S::FM];
+    int t[S::FM];
+    auto fetch_rows = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i) {
+        const int m = min(m0 + wm + 32 * i + c, M - 1);
+        t[i] = a.tc[m];
+        if constexpr (MODE == kGrad) {
+          l[i] = a.lse[m];
+          f[i] = a.factor[m];
+        }
+      }
+    };
+    auto rows_are_there = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i) {
+        asm volatile("" : "+v"(t[i]));
+        if constexpr (MODE == kGrad) asm volatile("" : "+v"(l[i]), "+v"(f[i]));
+      }
+    };
+    constexpr bool ROWS = MODE == kStats || MODE == kGrad;
+    if constexpr (ROWS) fetch_rows();
+    if (any) read(0, 0);
+    int done = 0;   // buffer of the step that ends
     acc_t acc[S::FM][S::FN];   // [n rows, m lanes]
 #pragma unroll
     for (int i = 0; i < S::FM; ++i)
@@ -404,78 +497,96 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
         multiply(s % 2);
       }
       arrive();
-      const int done = buffer;
+      done = buffer;
       buffer = buffer == (S::kStages - 1) * S::kStage ? 0 : buffer + S::kStage;
-      request(done);
-      read(0, 0);   // (behind the last step of all: what is there, for nothing)
+      if (it + 1 < steps) request(done);
+      read(0, 0);   // (behind the last step: for nothing)
       multiply(1);
     }
     asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");   // the loop may end right behind a product
     __builtin_amdgcn_sched_barrier(0);
-    tile += stride;
+    if constexpr (ROWS) rows_are_there();
+    if (any) request(done);
+    item += stride;
+    if (item < last) advance(at, stride);
+    const bool inside = m0 + BM <= M && n0 + BN <= a.N;
     if constexpr (MODE == kStats) {
       // this wave's columns of the row of lane c: 16 FN of them here, as many in lane c + 32
+      const int here = n0 + wn + 4 * g;   // column of element (j, r) of this lane, less 32 j + acc_row(r, 0)
 #pragma unroll
       for (int i = 0; i < S::FM; ++i) {
         const int m = m0 + wm + 32 * i + c;
-        const int here = n0 + wn + 4 * g;   // column of element (j, r) of this lane, less 32 j + acc_row(r, 0)
+        t[i] -= here;
+        acc_t z[S::FN];
+        const int end = n0 + BN > a.N ? a.N - here : 32 * S::FN;   // columns of this lane that are there
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) z[j] = acc[i][j];
         if (n0 + BN > a.N) {
 #pragma unroll
           for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 32 * j + acc_row(r, 0) < a.N - here ? acc[i][j][r] : -INFINITY;
+            for (int r = 0; r < 16; ++r) z[j][r] = 32 * j + acc_row(r, 0) < end ? z[j][r] : -INFINITY;
         }
-        const int t = (m < M ? a.tc[m] : -1) - here;
-        const bool mine = t >= 0 && t < 32 * S::FN && (t & 4) == 0;
+        const bool mine = m < M && t[i] >= 0 && t[i] < 32 * S::FN && (t[i] & 4) == 0;
         if (__ballot(mine) != 0) {
-          float z = 0.f;
+          float zt = 0.f;
 #pragma unroll
           for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z = t == 32 * j + acc_row(r, 0) ? acc[i][j][r] : z;
-          if (mine) a.tl[m] = z;
+            for (int r = 0; r < 16; ++r) zt = t[i] == 32 * j + acc_row(r, 0) ? z[j][r] : zt;
+          if (mine) a.tl[m] = zt;
         }
         float most = kLeast;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) most = fmaxf(most, acc[i][j][r]);   // fmaxf drops NaNs
+          for (int r = 0; r < 16; r += 2) most = fmaxf(fmaxf(most, z[j][r]), z[j][r + 1]);   // fmaxf drops NaNs
         most = fmaxf(most, __shfl_xor(most, 32));
         const float shift = most * kLog2e;
-        float sum = 0.f;
+        float sum[4] = {};
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum += fast_exp2(__builtin_fmaf(acc[i][j][r], kLog2e, -shift));
-        sum += __shfl_xor(sum, 32);
-        if (g == 0 && m < M) a.parts[(int64_t)(n0 / BN * S::WN + wave % S::WN) * a.Rp + m] = vec<float, 2>{most, sum};
+          for (int r = 0; r < 16; ++r) sum[r % 4] += fast_exp2(__builtin_fmaf(z[j][r], kLog2e, -shift));
+        float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        s += __shfl_xor(s, 32);
+        if (g == 0 && m < M) a.parts[(int64_t)(n0 / BN * S::WN + wave % S::WN) * a.Rp + m] = vec<float, 2>{most, s};
+        __builtin_amdgcn_sched_barrier(0);
       }
+      stored = inside;
     } else if constexpr (MODE == kRowGrad) {
-      float* out = a.out + (int64_t)blockIdx.y * a.part_rows * a.N;
+      float* out = a.out + (int64_t)range * a.part_rows * a.N;
 #pragma unroll
-      for (int i = 0; i < S::FM; ++i)
+      for (int i = 0; i < S::FM; ++i) {
+        const int m = m0 + wm + 32 * i + c;
+        float* row = out + (int64_t)m * a.N + n0 + wn + 4 * g;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int m = m0 + wm + 32 * i + c, n = n0 + wn + 32 * j + 8 * q + 4 * g;
-            if (m >= M || n >= a.N) continue;
-            vec<float, 4>* p = reinterpret_cast<vec<float, 4>*>(out + (int64_t)m * a.N + n);
+            if (m >= M || n0 + wn + 32 * j + 8 * q + 4 * g >= a.N) continue;
+            vec<float, 4>* p = reinterpret_cast<vec<float, 4>*>(row + 32 * j + 8 * q);
             vec<float, 4> v = pack4<float>(acc[i][j], q);
             if (a.add) v += *p;
             *p = v;
           }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      stored = inside && !a.add;
     } else if (MODE == kWeightGrad && a.splits > 1) {
-      float* out = a.out + (int64_t)blockIdx.y * a.M * a.N;
+      float* out = a.out + (int64_t)range * a.M * a.N;
 #pragma unroll
-      for (int i = 0; i < S::FM; ++i)
+      for (int i = 0; i < S::FM; ++i) {
+        const int m = m0 + wm + 32 * i + c;
+        float* row = out + (int64_t)m * a.N + n0 + wn + 4 * g;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int m = m0 + wm + 32 * i + c, n = n0 + wn + 32 * j + 8 * q + 4 * g;
-            if (m < M && n < a.N) *reinterpret_cast<vec<float, 4>*>(out + (int64_t)m * a.N + n) = pack4<float>(acc[i][j], q);
-          }
+          for (int q = 0; q < 4; ++q)
+            if (m < M && n0 + wn + 32 * j + 8 * q + 4 * g < a.N) *reinterpret_cast<vec<float, 4>*>(row + 32 * j + 8 * q) = pack4<float>(acc[i][j], q);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      stored = inside;
     } else {
       // to whole rows through LDS, 32 rows of up to 64 columns at a time, each wave in a part of its own; pieces placed as in the operands
       T* turn = reinterpret_cast<T*>(castle_vocab_lds + S::kStages * S::kStage + wave * 4096);
@@ -484,30 +595,43 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
       const int row_end = MODE == kGrad ? min((int)up(count, 64), (int)a.Rp) : M;
 #pragma unroll
       for (int i = 0; i < S::FM; ++i) {
-        const int m = m0 + wm + 32 * i + c;
-        float l = 0.f, f = 0.f;
-        int t = -1;
+        acc_t z[S::FN];
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) z[j] = acc[i][j];
         if constexpr (MODE == kGrad) {
-          if (m < M) {
-            l = a.lse[m] * kLog2e;
-            f = a.factor[m];
-            t = a.tc[m] - a.first - n0 - wn;
-          }
-          const bool here = __ballot(t >= 0 && t < 32 * S::FN) != 0, edge = n0 + BN > a.N;
+          const float shift = l[i] * kLog2e;
+          t[i] -= a.first + n0 + wn + 4 * g;
+          // g exp(z - lse), a factor that is not negative in the exponent; less the factor at the target
+          auto form = [&](auto target) __attribute__((always_inline)) {
+            const float up = __builtin_amdgcn_logf(f[i]) - shift;
 #pragma unroll
-          for (int j = 0; j < S::FN; ++j)
+            for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int n = 32 * j + acc_row(r, g);
-              float p = fast_exp2(__builtin_fmaf(acc[i][j][r], kLog2e, -l));
-              if (here) p -= t == n ? 1.f : 0.f;
-              acc[i][j][r] = m >= M || (edge && n0 + wn + n >= a.N) ? 0.f : p * f;
-            }
+              for (int r = 0; r < 16; ++r) {
+                float p = fast_exp2(__builtin_fmaf(z[j][r], kLog2e, up));
+                if constexpr (decltype(target)::value) p -= t[i] == 32 * j + acc_row(r, 0) ? f[i] : 0.f;
+                z[j][r] = p;
+              }
+          };
+          auto form_any = [&]() __attribute__((always_inline)) {
+            const int end = m0 + wm + 32 * i + c < M ? a.N - n0 - wn - 4 * g : 0;
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const int n = 32 * j + acc_row(r, 0);
+                const float p = fast_exp2(__builtin_fmaf(z[j][r], kLog2e, -shift)) - (t[i] == n ? 1.f : 0.f);
+                z[j][r] = n < end ? p * f[i] : 0.f;
+              }
+          };
+          if (!inside || __ballot(f[i] < 0.f) != 0) form_any();
+          else if (__ballot(t[i] >= 0 && t[i] < 32 * S::FN) != 0) form(std::true_type());
+          else form(std::false_type());
         } else {
 #pragma unroll
           for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = ldexpf(acc[i][j][r], -shift);
+            for (int r = 0; r < 16; ++r) z[j][r] = ldexpf(z[j][r], -shift);
         }
 #pragma unroll
         for (int h = 0; h < S::FN / FJ; ++h) {
@@ -516,18 +640,21 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
 #pragma unroll
           for (int j = 0; j < FJ; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) st4<T>(turn + c * 8 * CP + 8 * ((4 * j + q) ^ (c >> 1 & (CP - 1))) + 4 * g, pack4<T>(acc[i][FJ * h + j], q));
+            for (int q = 0; q < 4; ++q) st4<T>(turn + c * 8 * CP + 8 * ((4 * j + q) ^ (c >> 1 & (CP - 1))) + 4 * g, pack4<T>(z[FJ * h + j], q));
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           __builtin_amdgcn_wave_barrier();
 #pragma unroll
           for (int k = 0; k < 32 / RP; ++k) {
             const int row = RP * k + lane / CP, piece = lane % CP, mm = m0 + wm + 32 * i + row, n = n0 + wn + 32 * FJ * h + 8 * piece;
             const vt v = *reinterpret_cast<const vt*>(turn + row * 8 * CP + 8 * (piece ^ (row >> 1 & (CP - 1))));
-            if (mm < row_end && n < (MODE == kGrad ? (int)a.ldc : a.N)) *reinterpret_cast<vt*>(static_cast<T*>(a.c) + (int64_t)mm * a.ldc + n) = v;
+            T* to = static_cast<T*>(a.c) + (MODE == kGrad ? (int64_t)(mm / kBlock * kBlock) * a.ldc + n / kBlock * (kBlock * kBlock) + mm % kBlock * kBlock + n % kBlock
+                                                          : (int64_t)mm * a.ldc + n);
+            if (mm < row_end && n < (MODE == kGrad ? (int)a.ldc : a.N)) *reinterpret_cast<vt*>(to) = v;
           }
         }
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      stored = inside;
     }
   }
 }
@@ -540,8 +667,8 @@ template <typename T, int MODE, int BM, int BN> int launch_product_t(const Produ
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&vocab_product_kernel<T, MODE, BM, BN>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
     configured = true;
   }
-  const int64_t tiles = up(a.M, BM) / BM * (up(a.N, BN) / BN);
-  hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN>), dim3((unsigned)std::min<int64_t>(up(tiles, 8), 256), a.splits), dim3(kWideThreads), S::kLds, stream, a);
+  const int64_t items = up(a.M, BM) / BM * (up(a.N, BN) / BN) * a.splits;
+  hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -3;
 }
 // rows and columns of a workgroup's tile
@@ -572,8 +699,20 @@ struct Plan {
   int row_splits, weight_splits;
 };
 int64_t tiles(int64_t m, int64_t n, Tile t) { return up(m, t.rows) / t.rows * (up(n, t.columns) / t.columns); }
-// ranges of a contraction of `steps` for `n` tiles: as many as fill the CUs, of four steps at least
-int splits_for(int64_t n, int64_t steps) { return (int)std::max<int64_t>(1, std::min<int64_t>(256 / std::max<int64_t>(1, n), steps / 4)); }
+// Ranges of a contraction of `steps` for m x n outputs, from what it takes roughly (us): 1.5 a step and 5 an end for each of the items of the fullest CU, and for several ranges their partial
+// results, written and read at 4 TB/s.
+int splits_for(int64_t m, int64_t n, Tile t, int64_t steps) {
+  int best = 1;
+  double best_cost = 1e30;
+  for (int s = 1; s <= 128 && s <= std::max<int64_t>(1, steps / 2); ++s) {
+    const double cost = (tiles(m, n, t) * s + 255) / 256 * (1.5 * steps_of_range((int)steps, s) + 5) + (s > 1 ? 8e-6 / 4 * s * m * n : 0);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
 Plan plan(const VocabArgs& a, int es) {
   Plan p = {};
   p.Rp = up(a.R, 64);
@@ -589,8 +728,8 @@ Plan plan(const VocabArgs& a, int es) {
   } else {
     p.P = p.pieces;
   }
-  p.row_splits = splits_for(tiles(a.R, a.D, row_grad_tile(a.R, a.D)), p.ldc / kWideK);
-  p.weight_splits = splits_for(tiles(p.ldc, a.D, weight_grad_tile(a.D)), p.Rp / kWideK);
+  p.row_splits = splits_for(a.R, a.D, row_grad_tile(a.R, a.D), p.ldc / kWideK);
+  p.weight_splits = splits_for(p.ldc, a.D, weight_grad_tile(a.D), p.Rp / kWideK);
   return p;
 }
 // what the fp32 products of `bytes(columns)` need: of a whole piece of the vocabulary, and of the last one
@@ -657,7 +796,7 @@ int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 template <bool FIRST> int launch_gather(const RowArgs& a, int dtype, hipStream_t stream) {
   return by_tensor_type(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((gather_rows_kernel<T, FIRST>), dim3((unsigned)(up(a.v.R, kGatherRows) / kGatherRows)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((gather_rows_kernel<T, FIRST>), dim3((unsigned)(up(a.v.R, 64) / kGatherRows)), dim3(kThreads), 0, stream, a);
     return launched();
   });
 }
@@ -863,7 +1002,7 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
       if (e == 0 && dx != nullptr) e = launch_row_grad<T>(gx, stream);
       if (e == 0 && dw != nullptr) e = launch_weight_grad<T>(gw, stream);
       if (e == 0 && dw != nullptr && gw.splits > 1) {
-        const JoinArgs j = {b.weight_parts, nullptr, b.shift, gw.c, gw.splits, a.D, n};
+        const JoinArgs j = {b.weight_parts, nullptr, b.shift, gw.c, gw.splits, a.D, n, &s.head->count};
         hipLaunchKernelGGL((join_rows_kernel<T>), dim3((unsigned)(up((int64_t)n * a.D / 4, kThreads) / kThreads)), dim3(kThreads), 0, stream, j);
         e = launched();
       }
@@ -892,7 +1031,7 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
     }
   }
   if (dx == nullptr) return 0;
-  const JoinArgs j = {b.row_parts, s.rank, b.shift, dx, es == 2 ? p.row_splits : 1, a.D, a.R};
+  const JoinArgs j = {b.row_parts, s.rank, b.shift, dx, es == 2 ? ranges((int)up(std::min(a.V, p.columns), kWideK) / kWideK, p.row_splits) : 1, a.D, a.R, nullptr};
   return by_tensor_type(dtype, [&](auto t) {
     hipLaunchKernelGGL((join_rows_kernel<decltype(t)>), dim3((unsigned)(up((int64_t)a.R * a.D / 4, kThreads) / kThreads)), dim3(kThreads), 0, stream, j);
     return launched();
