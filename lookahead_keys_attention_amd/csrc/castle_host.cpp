@@ -987,38 +987,6 @@ Tensor cross_entropy(const Tensor& logits, const Tensor& target) {
   return CrossEntropyFn::apply(logits, target, true);
 }
 
-// the token embedding, with a gradient that needs neither a sort nor the host where the vocabulary is small
-struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& index) {
-    const at::AutoDispatchBelowADInplaceOrView below;
-    ctx->save_for_backward({index});
-    ctx->saved_data["vocabulary"] = weight.size(0);
-    return at::embedding(weight, index);
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
-    return once_differentiable([&] { return gradients(ctx, g); });
-  }
-  static variable_list gradients(AutogradContext* ctx, const variable_list& g) {
-    const Tensor index = token_rows(ctx->get_saved_variables()[0]);
-    const c10::DeviceGuard guard(index.device());
-    const int64_t V = ctx->saved_data["vocabulary"].toInt(), D = g[0].size(-1), R = index.numel();
-    const int64_t nbytes = castle_embedding_grad_workspace_bytes(R, (int)V, (int)D, dtype_code(g[0]));
-    if (nbytes < 0 || V * D % 8 != 0) return {at::embedding_dense_backward(g[0], index, V, -1, false), Tensor()};
-    const Tensor dy = row_major(g[0]);
-    Tensor dw = at::empty({V, D}, dy.options()), ws = bytes(nbytes, dy);
-    check(castle_embedding_grad(dy.data_ptr(), static_cast<const int64_t*>(index.data_ptr()), index.size(1), index.stride(0), R, (int)V, (int)D, dw.data_ptr(),
-                                dtype_code(dy), ws.data_ptr(), nbytes, stream_of(dy)),
-          "castle_embedding_grad");
-    return {dw, Tensor()};
-  }
-};
-
-Tensor embedding(const Tensor& weight, const Tensor& index) {
-  const c10::DeviceGuard guard(weight.device());
-  if (!wants_graph({weight}) || index.numel() == 0) return at::embedding(weight, index);
-  return EmbeddingFn::apply(weight, index);
-}
-
 // token numbers as the kernels address them: the rows of a matrix, a distance apart
 struct TokenRows {
   Tensor t;
@@ -1217,6 +1185,83 @@ Tensor embedding_autograd(const Tensor& weight, const Tensor& index, double scal
     return op.call(weight, index, scale, padding_idx);
   }
   return ScaledEmbeddingFn::apply(weight, index, scale, padding_idx);
+}
+
+// the token embedding of a model, its gradient without a sort where the vocabulary is small: up to kFewTokens tokens times vocabulary rows (us of
+// both by GPU and host, without / with the sort: 16384 tokens of 512 bf16 over 1024 43 / 52, over 4096 124 / 50, 65536 over 1024 128 / 52)
+constexpr int64_t kFewTokens = (int64_t)1 << 24;
+struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& index, double scale) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({index});
+    ctx->saved_data["vocabulary"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    return embedding_op(weight, index, scale, -1);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    return once_differentiable([&] { return gradients(ctx, g); });
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& g) {
+    const Tensor index = token_rows(ctx->get_saved_variables()[0]);
+    const c10::DeviceGuard guard(index.device());
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const int64_t V = ctx->saved_data["vocabulary"].toInt(), D = g[0].size(-1), R = index.numel();
+    const int64_t nbytes = castle_embedding_grad_workspace_bytes(R, (int)V, (int)D, dtype_code(g[0]));
+    if (scale != 1 || nbytes < 0 || V * D % 8 != 0 || R * V > kFewTokens) return {embedding_bwd_op(g[0], index, V, scale, -1), Tensor(), Tensor()};
+    const Tensor dy = row_major(g[0]);
+    Tensor dw = at::empty({V, D}, dy.options()), ws = bytes(nbytes, dy);
+    check(castle_embedding_grad(dy.data_ptr(), static_cast<const int64_t*>(index.data_ptr()), index.size(1), index.stride(0), R, (int)V, (int)D, dw.data_ptr(),
+                                dtype_code(dy), ws.data_ptr(), nbytes, stream_of(dy)),
+          "castle_embedding_grad");
+    return {dw, Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& weight, const Tensor& index, double scale) {
+  const c10::DeviceGuard guard(weight.device());
+  if (!wants_graph({weight}) || index.numel() == 0) return embedding_op(weight, index, scale, -1);
+  return EmbeddingFn::apply(weight, index, scale);
+}
+
+// The end of a residual stream and its loss: the mean cross entropy of norm(x + delta) w^T, without the logits
+struct HeadLossFn : torch::autograd::Function<HeadLossFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& delta, const Tensor& norm_w, const Tensor& w, const Tensor& target, std::optional<double> eps,
+                        bool want_graph) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t R = target.numel(), dim = x.size(-1);
+    const Normed n = norm_rows(x.reshape({R, dim}), delta.reshape({R, dim}), norm_w, eps, want_graph);
+    const Tensor rows = target.reshape({R});
+    auto [loss, state] = linear_cross_entropy_op(n.h, w, rows, CASTLE_LOSS_MEAN, -100);
+    if (want_graph) {
+      ctx->save_for_backward({n.sum, norm_w, w, n.h, n.rstd, rows, state});
+      ctx->saved_data["shape"] = x.sizes().vec();
+    }
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    return once_differentiable([&] { return gradients(ctx, g); });
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& g) {
+    variable_list grads(7);
+    const auto s = ctx->get_saved_variables();
+    const Tensor &sum = s[0], &norm_w = s[1], &w = s[2], &h = s[3], &rstd = s[4];
+    const c10::DeviceGuard guard(h.device());
+    const bool need_x = ctx->needs_input_grad(0) || ctx->needs_input_grad(1), need_norm = ctx->needs_input_grad(2), need_w = ctx->needs_input_grad(3);
+    auto [dh, dw] = linear_cross_entropy_bwd_op(g[0], h, w, s[5], s[6], CASTLE_LOSS_MEAN, -100, need_x || need_norm, need_w);
+    if (need_w) grads[3] = dw;
+    if (need_x || need_norm) {
+      auto [dx, dn] = norm_rows_bwd(dh, sum, rstd, norm_w, Tensor(), need_x, need_norm);
+      if (need_norm) grads[2] = dn;
+      if (need_x) grads[0] = grads[1] = dx.view(ctx->saved_data["shape"].toIntVector());
+    }
+    return grads;
+  }
+};
+
+Tensor head_loss(const Tensor& x, const Tensor& delta, const Tensor& norm_w, std::optional<double> eps, const Tensor& w, const Tensor& target) {
+  const c10::DeviceGuard guard(x.device());
+  if (!wants_graph({x, delta, norm_w, w})) return HeadLossFn::forward(nullptr, x, delta, norm_w, w, target, eps, false);
+  return HeadLossFn::apply(x, delta, norm_w, w, target, eps, true);
 }
 
 Tensor dropout_op(const Tensor& x_, const std::optional<Tensor>& residual_, double p, const Tensor& seed_) {
@@ -1517,7 +1562,8 @@ PYBIND11_MODULE(_castle_host, m) {
   m.def("feed_forward", &feed_forward, unlocked());
   m.def("head", &head, unlocked());
   m.def("cross_entropy", &cross_entropy, unlocked());
-  m.def("embedding", &embedding, unlocked());
+  m.def("head_loss", &head_loss, unlocked());
+  m.def("embedding", &embedding, py::arg("weight"), py::arg("index"), py::arg("scale") = 1.0, unlocked());
   m.def("small_linear", &small_linear, unlocked());
   m.def("sample_tokens", &sample_tokens, unlocked());
   m.def("gather_rows", &gather_rows, unlocked());

@@ -10,7 +10,10 @@ step, one `Cache` per layer.
 
 Differences a user can switch: `tie_embedding=True` shares the token embedding with the logits
 projection (the reference keeps them separate, train_triton.py:86,111); `rotary_emb` / `prenorm`
-default to the reference's choice (both on, train_triton.py:99-100).
+default to the reference's choice (both on, train_triton.py:99-100); `embedding_scale` multiplies the
+embedded tokens; `dropout` is the probability with which an element of the embedded tokens and of every
+block's output is dropped in training, on passes that neither take nor return caches.  Vocabularies of any size:
+from LINEAR_LOSS_MIN_VOCABULARY on, `return_loss` of a native model forms no logits.
 """
 from __future__ import annotations
 
@@ -32,6 +35,10 @@ READ_ONCE_BYTES = 320_000_000
 # 64, logits of one leading digit last: 256 11 / 72 and 12 / 72; 8192 35 / 95 and 39 / 131; 20480 80 / 101 and 82 / 145,
 # 88 / 102; 28672 107 / 103 and 110 / 168, 122 / 102; 131072 462 / 108 and 533 / 777).
 SAMPLER_MAX_VOCABULARY = 20480
+
+
+# From this vocabulary on the loss of a native model is formed without its logits (ops.linear_cross_entropy).
+LINEAR_LOSS_MIN_VOCABULARY = 16384
 
 
 # -- sampling helpers (train_triton.py:56-71) ------------------------------------------------
@@ -214,7 +221,10 @@ class GraphedDecoder:
         model = self.model
         embedding = model.token_emb
         plain = _unmodified(embedding, nn.Embedding) and embedding.max_norm is None
-        h = _native.host().gather_rows(embedding.weight, self.token) if plain else embedding(self.token)
+        if plain:
+            h = _native.host().gather_rows(embedding.weight, self.token) if model.embedding_scale == 1 else ops.embedding(embedding.weight, self.token, model.embedding_scale)
+        else:
+            h = model._embed(self.token, False)
         for (attention, feed_forward), store in zip(model.layers, self.stores):
             h = attention.graph_step(h, store, self.t_device, self.base_device, residual=h)
             h = token_feed_forward(feed_forward, h)
@@ -243,9 +253,13 @@ class GraphedDecoder:
 
 class CastleLM(nn.Module):
     def __init__(self, *, num_tokens, dim, depth, max_seq_len=512, dim_head=64, heads=8, use_triton=True,
-                 rotary_emb=True, prenorm=True, tie_embedding=False):
+                 rotary_emb=True, prenorm=True, tie_embedding=False, embedding_scale=1.0, dropout=0.0):
         super().__init__()
+        if not 0 <= dropout <= 1:
+            raise ValueError(f"CastleLM: dropout is a probability, got {dropout}")
         self.max_seq_len = max_seq_len
+        self.embedding_scale = float(embedding_scale)
+        self.dropout = float(dropout)
         self.token_emb = nn.Embedding(num_tokens, dim)
         self.layers = nn.ModuleList()
         for _ in range(depth):
@@ -271,11 +285,13 @@ class CastleLM(nn.Module):
             x, target = x[:, :-1], x[:, 1:]
         if cache is None and x.dim() == 2 and x.shape[1] > 1 and self._plain(x):
             return self._forward_plain(x, target if return_loss else None, return_next_cache)
-        h = self.token_emb(x)
+        native = self._native_on_gpu(x.device)
+        h = self._embed(x, native)
+        drop = self._dropout(x.device, native, cache is None and not return_next_cache)
+        h = drop(h, None)
         # one token per sequence, no graph to record: the few rows of every projection go through the small-M kernel
         # (only for a model whose layers run the native kernels: one built with use_triton=False stays on
         # the PyTorch layers throughout, so it remains an independent baseline for the native one)
-        native = self._native_on_gpu(h.device)
         token_step = h.shape[1] == 1 and not torch.is_grad_enabled() and native
         next_cache = []
         for index, (attention, feed_forward) in enumerate(self.layers):
@@ -285,12 +301,30 @@ class CastleLM(nn.Module):
                 next_cache.append(layer_next)
             else:
                 attended = attention(h, cache=layer_cache, return_next_cache=False)
-            h = h + attended
-            h = token_feed_forward(feed_forward, h) if token_step else h + block_feed_forward(feed_forward, h, native)
+            h = drop(attended, h)
+            h = token_feed_forward(feed_forward, h) if token_step else drop(block_feed_forward(feed_forward, h, native), h)
         logits = Castle._project(self.to_logits, h, token_step, norm=self.final_norm, native=native)
         if return_loss:
             return F.cross_entropy(logits.transpose(1, 2), target)
         return (logits, next_cache) if return_next_cache else logits
+
+    def _embed(self, x, native):
+        embedding = self.token_emb
+        if self.embedding_scale == 1:
+            return embedding(x)
+        if native and _unmodified(embedding, nn.Embedding) and embedding.max_norm is None and not embedding.scale_grad_by_freq and not embedding.sparse:
+            return ops.embedding(embedding.weight, x, self.embedding_scale, embedding.padding_idx)
+        return embedding(x) * self.embedding_scale
+
+    def _dropout(self, device, native, training):
+        """f(x, residual) -> residual + dropout(x), or x without a residual, with another mask at every call; their numbers are
+        drawn in one go from the generator of the device."""
+        if not (training and self.training and self.dropout > 0):
+            return lambda x, residual: x if residual is None else residual + x
+        if not native:
+            return lambda x, residual: F.dropout(x, self.dropout) if residual is None else residual + F.dropout(x, self.dropout)
+        seeds = iter(torch.randint(-2 ** 63, 2 ** 63 - 1, (1 + 2 * len(self.layers), 2), device=device))
+        return lambda x, residual: ops.dropout_add(x, residual, self.dropout, next(seeds))
 
     def _plain(self, x) -> bool:
         """True if whole sequences may run as one native call per block: native layers, unmodified modules, nothing
@@ -322,7 +356,8 @@ class CastleLM(nn.Module):
         """`forward` over whole sequences, one native call per block: the sum of a residual stream is formed by the
         norm that reads it next.  `stores`: where the layers' caches go, one for each."""
         host = _native.host()
-        h, delta, next_cache = host.embedding(self.token_emb.weight, x), None, []
+        drop = self._dropout(x.device, True, not return_next_cache)
+        h, delta, next_cache = drop(host.embedding(self.token_emb.weight, x, self.embedding_scale), None), None, []
         for index, (attention, feed_forward) in enumerate(self.layers):
             results = attention._layer_native(h, return_next_cache, delta, stores[index] if stores is not None else None)
             if return_next_cache:
@@ -332,7 +367,12 @@ class CastleLM(nn.Module):
                 results = (results,)
             attended, h = results if delta is not None else (results[0], h)
             norm, up, _, down = feed_forward
-            delta, h = host.feed_forward(h, attended, norm.weight, norm.eps, up.weight, down.weight)
+            delta, h = host.feed_forward(h, drop(attended, None), norm.weight, norm.eps, up.weight, down.weight)
+            delta = drop(delta, None)
+        weight = self.to_logits.weight
+        if (target is not None and LINEAR_LOSS_MIN_VOCABULARY <= weight.shape[0] <= 1 << 22 and weight.shape[1] % 8 == 0 and weight.shape[1] <= 1 << 16
+                and 0 < target.numel() <= 1 << 24):
+            return host.head_loss(h, delta, self.final_norm.weight, self.final_norm.eps, weight, target)
         logits = host.head(h, delta, self.final_norm.weight, self.final_norm.eps, self.to_logits.weight)
         if target is not None:
             return host.cross_entropy(logits, target)
