@@ -25,7 +25,6 @@ struct GemmArgs {
   float eps;
   void* h;
   float* rstd;
-  int whole;   // 1: the contraction is not split (N need not be whole pieces then, as long as rows of c are)
 };
 // Weight gradient w (both operands contraction-strided) and input gradient x (the second one) of a projection in one launch: w_groups workgroups in rows of w_row,
 // then x_groups in rows of x_row.

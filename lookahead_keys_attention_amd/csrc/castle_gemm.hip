@@ -713,7 +713,7 @@ bool gemm_norm_ok(int M, int N, int K, int elem_size) {
 
 int launch_gemm(GemmArgs a, bool a_kc, bool b_kc, int dtype, float* workspace, hipStream_t stream) {
   const int es = dtype == 0 ? 4 : 2, step = dtype == 0 ? 32 : kStep16;
-  Plan p = plan(a.M, a.N, a.K, (a.epilogue == kGemmPlain && !a.whole) || a.amax != nullptr, es);   // (the slots of the maxima follow from the plain plan)
+  Plan p = plan(a.M, a.N, a.K, a.epilogue == kGemmPlain || a.amax != nullptr, es);   // (the slots of the maxima follow from the plain plan)
   a.k_per_split = ((a.K + p.splits - 1) / p.splits + step - 1) / step * step;
   p.splits = (a.K + a.k_per_split - 1) / a.k_per_split;   // rounding up may leave the last ones empty
   a.part = p.splits > 1 ? workspace : nullptr;

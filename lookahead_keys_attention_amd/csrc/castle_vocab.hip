@@ -10,11 +10,12 @@
 // Rows that do not count (target = ignore) are left out at the start: the others are copied together, and what the products cost goes with their number, which the kernels
 // read from device memory.  So whatever a row that does not count holds, infinities and NaNs too, goes nowhere.
 //
-// fp32: the products are those of castle_gemm32.hip, the logits of a piece lie in memory, and kernels over rows do the rest.
+// fp32: an element times a power of two, which brings the largest of its tensor to 2^14 ... 2^15, is the sum of two fp16 numbers that hold 22 bits of it, or what lies above 2^-40 of
+// the largest; a product of two elements is ac' + ca' + aa', three matrix instructions, and what is left out of it is below 2^-22 of the product.  Operands lie as such pairs, 32
+// first parts and the 32 second ones behind them, so a step of 64 numbers is 32 of the contraction, and everything else is that of the 16-bit types.  (The fp32 products of
+// castle_gemm32.hip, of three bf16 parts and six instructions, convert inside the product: 2048 rows of 512 over 32000, logits in memory, 1832 us.)
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
-#include "castle_gemm.h"
-#include "castle_rows.h"
 #include "castle_vocab.h"
 #include "castle_wide.h"
 #include <algorithm>
@@ -39,10 +40,10 @@ struct RowArgs {
   int* block_counts;   // [R / kCountRows]
   VocabHead* head;
   int32_t* rank;
-  void* xc;            // [Rp][Dp]: rows that count, then zero rows up to `zero_to` of them (a multiple of 64, or all)
+  void* xc;            // [Rp][Dp]: rows that count, then zero rows up to a multiple of 64 of them; fp32: pairs, see split_rows_kernel
   int32_t* tc;         // [Rp] their targets, -1 outside of the vocabulary
   float* tl;           // [Rp] logits of the targets: NaN until they are found
-  int Dp, zero_all;
+  int Dp;
   void* loss;          // kEachLoss: zeros for the rows that do not count
 };
 __device__ __forceinline__ int64_t class_of(const VocabArgs& a, int64_t r) {
@@ -72,7 +73,25 @@ __global__ __launch_bounds__(kThreads) void count_rows_kernel(RowArgs a) {
   }
   n = sum_over_threads<kWaves>(n, s);
   if (threadIdx.x == 0) a.block_counts[blockIdx.x] = n;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.head->most[0] = a.head->most[1] = 0;
 }
+// The largest of a workgroup's finite |x|, kept as the bits of a float, which are in the order of the numbers (of any order of arrival the same).  Only one that is larger than what
+// is there goes by the atomic: all of 8192 waves took 100 us, one behind the other.
+__device__ __forceinline__ void keep_most(float most, uint32_t* to) {
+  __shared__ float s[kWaves];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+  if (lane_id() == 0) s[wave_id()] = most;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) most = fmaxf(most, s[w]);
+  const uint32_t bits = __builtin_bit_cast(uint32_t, most);
+  if (bits > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(to, bits);
+}
+__device__ __forceinline__ float finite_abs(float x) { return fabsf(x) <= __FLT_MAX__ ? fabsf(x) : 0.f; }
+// the power of two that brings it to 2^14 ... 2^15
+__device__ __forceinline__ int shift_of(uint32_t most) { return most != 0 ? 15 - __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, most)) : 0; }
 // FIRST: ranks and targets are formed here, else (backward pass) the ranks are there
 template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void gather_rows_kernel(RowArgs a) {
   constexpr int V = elem_traits<T>::vec16;
@@ -106,7 +125,10 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
       }
       if (a.v.reduction == kEachLoss && there && !counts) static_cast<T*>(a.loss)[r] = (T)0.f;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.head = {all, 1.f / (float)all};
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      a.head->count = all;
+      a.head->inv_count = 1.f / (float)all;
+    }
   } else {
     all = a.head->count;
     if (threadIdx.x < kGatherRows) {
@@ -121,22 +143,87 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
   }
   __syncthreads();
   const int pieces = a.Dp / V, have = a.v.D / V;
-  const vt none = {};
-  const int zero_end = a.zero_all ? a.v.R : (int)up(all, 64);
-  for (int k = wave_id(); k < kGatherRows; k += kWaves) {
-    const int rank = s_rank[k];
-    if (rank >= 0) {
-      const T* from = static_cast<const T*>(a.v.x) + (first + k) * a.v.ld_x;
-      T* to = static_cast<T*>(a.xc) + (int64_t)rank * a.Dp;
-#pragma unroll 4
-      for (int i = lane_id(); i < pieces; i += 64) *reinterpret_cast<vt*>(to + i * V) = i < have ? *reinterpret_cast<const vt*>(from + i * V) : none;
+  if constexpr (sizeof(T) == 4) {   // (copied as pairs by a launch of its own, once the largest is known)
+    if constexpr (FIRST) {
+      float most = 0.f;
+      for (int k = wave_id(); k < kGatherRows; k += kWaves) {
+        if (s_rank[k] < 0) continue;
+        const T* from = static_cast<const T*>(a.v.x) + (first + k) * a.v.ld_x;
+        for (int i = lane_id(); i < have; i += 64) {
+          const vt x = *reinterpret_cast<const vt*>(from + i * V);
+#pragma unroll
+          for (int e = 0; e < V; ++e) most = fmaxf(most, finite_abs(x[e]));
+        }
+      }
+      keep_most(most, &a.head->most[0]);
     }
-    const int64_t r = first + k;   // (the workgroups reach to the next multiple of 64)
-    if (r >= all && r < zero_end) {
-      T* to = static_cast<T*>(a.xc) + r * a.Dp;
-      for (int i = lane_id(); i < pieces; i += 64) *reinterpret_cast<vt*>(to + i * V) = none;
+  } else {
+    const vt none = {};
+    for (int k = wave_id(); k < kGatherRows; k += kWaves) {
+      const int rank = s_rank[k];
+      if (rank >= 0) {
+        const T* from = static_cast<const T*>(a.v.x) + (first + k) * a.v.ld_x;
+        T* to = static_cast<T*>(a.xc) + (int64_t)rank * a.Dp;
+#pragma unroll 4
+        for (int i = lane_id(); i < pieces; i += 64) *reinterpret_cast<vt*>(to + i * V) = i < have ? *reinterpret_cast<const vt*>(from + i * V) : none;
+      }
+      const int64_t r = first + k;   // (the workgroups reach to the next multiple of 64)
+      if (r >= all && r < up(all, 64)) {
+        T* to = static_cast<T*>(a.xc) + r * a.Dp;
+        for (int i = lane_id(); i < pieces; i += 64) *reinterpret_cast<vt*>(to + i * V) = none;
+      }
     }
   }
+}
+
+// fp32: the largest |w|, and rows as pairs: 32 first parts, the 32 second ones, the next 32 columns
+struct SplitArgs {
+  const float* from;       // rows of ld
+  int64_t ld;
+  int rows, D, Dp;
+  const int32_t* rank;     // nullptr, or where a row goes (-1: nowhere) and `count`, behind which rows up to a multiple of 64 are zero
+  const int* count;
+  uint32_t* most;
+  fp16_t* to;              // [rows][2 Dp]
+};
+__global__ __launch_bounds__(kThreads) void most_kernel(SplitArgs a) {
+  typedef vec<float, 4> v4;
+  float most = 0.f;
+  for (int64_t r = (int64_t)blockIdx.x * kWaves + wave_id(); r < a.rows; r += (int64_t)gridDim.x * kWaves) {
+#pragma unroll 4
+    for (int i = lane_id(); i < a.D / 4; i += 64) {
+      const v4 x = *reinterpret_cast<const v4*>(a.from + r * a.ld + i * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = fmaxf(most, finite_abs(x[e]));
+    }
+  }
+  keep_most(most, a.most);
+}
+__device__ __forceinline__ void split_in_two(vec<float, 8> x, frag<fp16_t>& h, frag<fp16_t>& l) {
+  h = __builtin_convertvector(x, frag<fp16_t>);
+  l = __builtin_convertvector(x - __builtin_convertvector(h, vec<float, 8>), frag<fp16_t>);
+}
+__global__ __launch_bounds__(kThreads) void split_rows_kernel(SplitArgs a) {
+  const int shift = shift_of(*a.most), per = a.Dp / 8;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, r = i / per;
+  if (r >= (a.rank != nullptr ? up(a.rows, 64) : a.rows)) return;
+  const int c = (int)(i - r * per) * 8;
+  auto put = [&](int64_t row, frag<fp16_t> h, frag<fp16_t> l) __attribute__((always_inline)) {
+    fp16_t* to = a.to + row * 2 * a.Dp + c / 32 * 64 + c % 32;
+    *reinterpret_cast<frag_mem<fp16_t>*>(to) = h;
+    *reinterpret_cast<frag_mem<fp16_t>*>(to + 32) = l;
+  };
+  if (a.rank != nullptr && r >= *a.count && r < up(*a.count, 64)) put(r, zero_frag<fp16_t>(), zero_frag<fp16_t>());
+  const int64_t row = a.rank == nullptr ? r : r < a.rows ? a.rank[r] : -1;
+  if (row < 0) return;
+  frag<fp16_t> h = zero_frag<fp16_t>(), l = h;
+  if (c < a.D) {
+    vec<float, 8> x = *reinterpret_cast<const frag_mem<float>*>(a.from + r * a.ld + c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], shift);
+    split_in_two(x, h, l);
+  }
+  put(row, h, l);
 }
 
 // maxima and sums of the P column ranges -> log-sum-exp of a row, its loss; partial sums of the losses, one of each workgroup
@@ -204,40 +291,43 @@ template <typename T> __global__ __launch_bounds__(kThreads) void loss_kernel(Lo
   }
 }
 
-// Factors of the rows of d.  d lies in the 16-bit type, so the largest factor is brought to 2^14 ... 2^15 by a power of two, 2^shift, which the gradients lose again: softmax
-// values down to 2^-29 are then normal numbers of fp16 (without it, a mean over 16384 rows would leave nothing of any below 2^-1), and d stays below 2^15.
+// Factors of the rows of d.  d lies in the 16-bit type (fp32: in pairs of fp16), so the largest factor is 2^14 ... 2^15, which the gradients lose again (Gain): softmax
+// values down to 2^-29 are then normal numbers of fp16 (without it, a mean over 16384 rows would leave nothing of any below 2^-1), and d stays below 2^15.  Where all rows have one
+// factor it is 2^15 itself, and the factor goes to the gradients in 32 bits: most rows have -1 or nearly that at their target, and times a factor that
+// is no power of two all of these would be rounded the same way, 2^-9 of bf16 at worst.
+struct Gain {
+  int shift;    // of d, to be taken back
+  float gain;   // of the gradients
+};
 struct FactorArgs {
   const void* dloss;
   const VocabHead* head;
   const int32_t *rank, *tc;
   float* factor;   // [Rp] by rank
-  int* shift;
-  int R, reduction, scaled;
+  Gain* gain;
+  int R, reduction;
 };
 template <typename T> __global__ __launch_bounds__(1024) void factor_kernel(FactorArgs a) {
   __shared__ float s[16];
   const bool each = a.reduction == kEachLoss;
   const T* g = static_cast<const T*>(a.dloss);
-  float most = 0.f;
+  int shift = 15;
   if (each) {
+    float most = 0.f;
     for (int r = threadIdx.x; r < a.R; r += 1024)
       if (a.rank[r] >= 0) most = fmaxf(most, fabsf((float)g[r]));   // fmaxf drops NaNs
-  } else {
-    most = fabsf(a.reduction == kMeanLoss ? (float)*g * a.head->inv_count : (float)*g);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+    if (lane_id() == 0) s[wave_id()] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 16; ++w) most = fmaxf(most, s[w]);
+    shift = most > 0.f && most <= __FLT_MAX__ ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-  if (lane_id() == 0) s[wave_id()] = most;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 16; ++w) most = fmaxf(most, s[w]);
-  const int shift = a.scaled && most > 0.f && most <= __FLT_MAX__ ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
-  if (threadIdx.x == 0 && blockIdx.x == 0) *a.shift = shift;
+  if (threadIdx.x == 0 && blockIdx.x == 0) *a.gain = {shift, a.head->count == 0 ? 0.f : each ? 1.f : a.reduction == kMeanLoss ? (float)*g * a.head->inv_count : (float)*g};
   for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < a.R; r += (int64_t)gridDim.x * 1024) {
     const int rank = a.rank[r];
-    if (rank < 0) continue;
-    const float f = each ? (float)g[r] : a.reduction == kMeanLoss ? (float)*g * a.head->inv_count : (float)*g;
-    a.factor[rank] = a.tc[rank] >= 0 ? ldexpf(f, shift) : NAN;
+    if (rank >= 0) a.factor[rank] = a.tc[rank] >= 0 ? ldexpf(each ? (float)g[r] : 1.f, shift) : NAN;
   }
 }
 
@@ -245,15 +335,17 @@ template <typename T> __global__ __launch_bounds__(1024) void factor_kernel(Fact
 __host__ __device__ constexpr int steps_of_range(int steps, int splits) { return steps > 0 ? (steps + splits - 1) / splits : 1; }
 __host__ __device__ constexpr int ranges(int steps, int splits) { return (steps + steps_of_range(steps, splits) - 1) / steps_of_range(steps, splits); }
 
-// dx[r] = 2^-shift times the sum of its partial results, zeros where it does not count
+// dx[r] (or dw[v]) = gain 2^-shift times the sum of its partial results, zeros where it does not count
 struct JoinArgs {
   const float* parts;   // [splits][R][D]
   const int32_t* rank;
-  const int* shift;
+  const Gain* gain;
   void* out;
   int splits, D;
   int64_t R;
   const int* count;     // nullptr, or the contraction: there are as many partial results as it has ranges
+  int step;             // of the contraction
+  const uint32_t* most; // fp32: of the other operand, whose power of two goes as well; else nullptr
 };
 template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kernel(JoinArgs a) {
   typedef vec<float, 4> v4;
@@ -264,13 +356,14 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kern
   const int c = (int)(i - r * per) * 4, rank = a.rank == nullptr ? (int)r : a.rank[r];
   v4 v = {0.f, 0.f, 0.f, 0.f};
   if (rank >= 0) {
-    const int splits = a.count != nullptr ? ranges((*a.count + kWideK - 1) / kWideK, a.splits) : a.splits;
+    const int splits = a.count != nullptr ? ranges((*a.count + a.step - 1) / a.step, a.splits) : a.splits;
     const float* p = a.parts + (int64_t)rank * a.D + c;
 #pragma unroll 4
     for (int k = 0; k < splits; ++k) v += *reinterpret_cast<const v4*>(p + k * a.R * a.D);
-    const int shift = *a.shift;
+    const int shift = a.gain->shift + (a.most != nullptr ? shift_of(*a.most) : 0);
+    const float gain = a.gain->gain;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -shift);
+    for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -shift) * gain;
   }
   *reinterpret_cast<vec4_mem<T>*>(static_cast<T*>(a.out) + r * a.D + c) = __builtin_convertvector(v, vec<T, 4>);
 }
@@ -301,63 +394,91 @@ struct ProductArgs {
   float* out;
   int64_t part_rows;
   int add;
-  const int* shift;
+  const Gain* gain;
+  const VocabHead* head;   // fp32: the largest elements of x and w
 };
 
-// d lies in blocks of 64 x 64, whole rows of blocks one behind the other: a step of either product that reads it fetches pieces of 8 KB.  (Rows of d as they are: 128 bytes here and
-// there, 64 KB and more apart; dx of 16384 rows over 32000 503 us, dweight 468.)
-constexpr int kBlock = 64;
-template <typename T, bool KC, int FREE> struct BlockOperand : WideOperand<T, KC, FREE> {
-  typedef WideOperand<T, KC, FREE> W;
-  // p: [row of blocks][ldc / 64][64][64]
-  __device__ __forceinline__ void start(const T* p, int64_t ldc, int free0, int free_end, int k0) {
-    const int lane = lane_id(), first = wave_id() * W::N;
+// Pairs of fp16 numbers instead of single ones, K of them a step: the second parts lie 32 places behind the first ones, in a row as in LDS.
+// an operand that is not contraction-contiguous: rows k and k + 32 in LDS are the two parts of row k
+template <typename T, int FREE> struct PairOperand : WideOperand<T, false, FREE> {
+  typedef WideOperand<T, false, FREE> W;
+  __device__ __forceinline__ void start(const T* p, int64_t ld, int free0, int free_end, int k0) {
+    W::at = p + k0 * ld + 2 * free0;
     W::left = free_end - free0;
-    W::at = KC ? p + free0 * ldc + k0 * kBlock : p + k0 * ldc + free0 * kBlock;
+    place((int)ld, kWideK / 2);
+  }
+  __device__ __forceinline__ void place(int ld, int steps) {
+    constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
+    const int lane = lane_id(), first = wave_id() * W::N;
+#pragma unroll
+    for (int q = 0; q < W::N; ++q) {
+      const int k = ROWS * (first + q) + lane / PIECES, p = lane % PIECES ^ 4 * (k & 3), piece = 8 * p < W::left ? p : 0;
+      W::off[q] = 2 * (uint32_t)(min(k % 32, steps - 1) * ld + piece / 4 * 64 + k / 32 * 32 + 8 * (piece % 4));
+    }
+  }
+  __device__ __forceinline__ void load(int64_t ld, uint32_t lds) {
+#pragma unroll
+    for (int q = 0; q < W::N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * W::N + q));
+    W::at += kWideK / 2 * ld;
+  }
+};
+
+// d lies in blocks of 64 x 64 (pairs: 32 x 32 pairs), whole rows of blocks one behind the other, so a step of either product that reads it fetches pieces of 4 or 8 KB.  (As rows
+// of V, 128 bytes here and there, 64 KB and more apart: the same time where the caches hold a band of columns.)
+template <bool PAIRS> constexpr int kBlock = PAIRS ? 32 : 64;   // rows; a row of a block is 64 numbers
+template <typename T, bool KC, int FREE, bool PAIRS> struct BlockOperand : WideOperand<T, KC, FREE> {
+  typedef WideOperand<T, KC, FREE> W;
+  static constexpr int B = kBlock<PAIRS>;
+  // p: [row of blocks][ldc / B][B][64]
+  __device__ __forceinline__ void start(const T* p, int64_t ldc, int free0, int free_end, int k0) {
+    const int lane = lane_id(), first = wave_id() * W::N, row_of_blocks = 64 * (int)ldc;
+    W::left = free_end - free0;
+    W::at = p + (KC ? free0 : k0) / B * (int64_t)row_of_blocks + (KC ? k0 : free0) / B * (B * 64);
 #pragma unroll
     for (int q = 0; q < W::N; ++q) {
       if constexpr (KC) {
         const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7), there = min(row, W::left - 1);
-        W::off[q] = 2 * (uint32_t)(there / kBlock * kBlock * (int)ldc + there % kBlock * kBlock + 8 * piece);
+        W::off[q] = 2 * (uint32_t)(there / B * row_of_blocks + there % B * 64 + 8 * piece);
       } else {
-        constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
+        constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES, P = B / 8;   // P: pieces of a row of a block, of one part
         const int k = ROWS * (first + q) + lane / PIECES, p = lane % PIECES ^ 4 * (k & 3), piece = 8 * p < W::left ? p : 0;
-        W::off[q] = 2 * (uint32_t)(piece / 8 * kBlock * kBlock + k * kBlock + 8 * (piece % 8));
+        W::off[q] = 2 * (uint32_t)(piece / P * (B * 64) + k % B * 64 + k / B * 32 + 8 * (piece % P));
       }
     }
   }
   __device__ __forceinline__ void load(int64_t ldc, uint32_t lds) {
 #pragma unroll
     for (int q = 0; q < W::N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * W::N + q));
-    W::at += kBlock * (KC ? (int64_t)kBlock : ldc);
+    W::at += KC ? (int64_t)B * 64 : 64 * ldc;
   }
 };
 
 // Eight waves over BM x BN: four by two of them for 256 rows, else two by four.
-template <int MODE, int BM, int BN> struct Shape {
+template <int MODE, int BM, int BN, bool PAIRS> struct Shape {
   static constexpr int WM = BM == 256 ? 4 : 2, WN = 8 / WM, FM = BM / 32 / WM, FN = BN / 32 / WN;
-  static constexpr bool kTurn = MODE == kGrad || MODE == kWeightGrad;   // a tile goes through LDS to whole rows, 4 KB of each wave
+  static constexpr bool kTurn = MODE == kGrad || (MODE == kWeightGrad && !PAIRS);   // a tile goes through LDS to whole rows, 4 KB of each wave
   static constexpr int kStage = (BM + BN) * kWideK * 2, kTurnBytes = kTurn ? 4096 * 8 : 0;
   static constexpr int kFit = (kMaxLds - kTurnBytes) / kStage, kStages = kFit < 3 ? kFit : 3;
   static constexpr int kLoads = kStage / 1024 / 8, kLds = kStages * kStage + kTurnBytes;
-  static constexpr int kStores = MODE == kStats ? FM : MODE == kRowGrad ? 4 * FM * FN : 2 * FM * FN;   // of a wave and tile (kWeightGrad: partial results are twice as many)
+  static constexpr int kStores = MODE == kStats ? FM : MODE == kRowGrad || PAIRS ? 4 * FM * FN : 2 * FM * FN;   // of a wave and tile (kWeightGrad: partial results are twice as many)
   static_assert(kStages >= 2 && FM >= 1 && FN >= 1, "");
 };
 extern __shared__ __attribute__((aligned(16))) unsigned char castle_vocab_lds[];
 
-template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
-  typedef Shape<MODE, BM, BN> S;
+template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
+  typedef Shape<MODE, BM, BN, PAIRS> S;
   constexpr bool AK = MODE != kWeightGrad, BKC = MODE == kStats || MODE == kGrad;
-  typedef std::conditional_t<MODE == kRowGrad || MODE == kWeightGrad, BlockOperand<T, AK, BM>, WideOperand<T, AK, BM>> OpA;
-  typedef WideOperand<T, BKC, BN> OpB;
+  constexpr int kStep = PAIRS ? kWideK / 2 : kWideK;   // of the contraction
+  typedef std::conditional_t<MODE == kRowGrad || MODE == kWeightGrad, BlockOperand<T, AK, BM, PAIRS>, WideOperand<T, AK, BM>> OpA;
+  typedef std::conditional_t<PAIRS && !BKC, PairOperand<T, BN>, WideOperand<T, BKC, BN>> OpB;
   typedef vec<T, 8> vt;
   const int lane = lane_id(), wave = wave_id(), c = lane & 31, g = lane >> 5;
-  const int count = __builtin_amdgcn_readfirstlane(*a.count), M = MODE == kWeightGrad ? a.M : min(a.M, count), K = MODE == kWeightGrad ? (int)up(min(a.K, count), kWideK) : a.K;
+  const int count = __builtin_amdgcn_readfirstlane(*a.count), M = MODE == kWeightGrad ? a.M : min(a.M, count), K = MODE == kWeightGrad ? (int)up(min(a.K, count), kStep) : a.K;
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
   if (tiles == 0) return;
   // Items are tiles for each range of the contraction; XCD x takes the x-th eighth of them.  Tiles in the order of an XCD's L2: all rows of a band of columns, then those of the next.
   constexpr int kBand = 2048 / BN;
-  const int all_steps = (K + kWideK - 1) / kWideK, per_range = steps_of_range(all_steps, a.splits);
+  const int all_steps = (K + kStep - 1) / kStep, per_range = steps_of_range(all_steps, a.splits);
   const int items = tiles * max(1, ranges(all_steps, a.splits));
   // The place of an item, moved on by additions: divisions by the sizes took a tenth of what 16384 x 32000 logits of 512 take.
   struct Walk { int band, rest, range; };   // rest: tile of the band
@@ -377,7 +498,7 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
   struct Item { int m0, n0, range, k0, steps; };
   auto item_at = [&](const Walk& w) __attribute__((always_inline)) {
     const int width = min(kBand, tiles_n - w.band * kBand), m = width == kBand ? w.rest / kBand : w.rest / width;
-    return Item{m * BM, (w.band * kBand + w.rest - m * width) * BN, w.range, w.range * per_range * kWideK, min(per_range, all_steps - w.range * per_range)};
+    return Item{m * BM, (w.band * kBand + w.rest - m * width) * BN, w.range, w.range * per_range * kStep, min(per_range, all_steps - w.range * per_range)};
   };
   const int share = (items + 7) / 8, begin = blockIdx.x % 8 * share, last = min(items, begin + share), stride = gridDim.x / 8;
   const int wm = wave / S::WN * 32 * S::FM, wn = wave % S::WN * 32 * S::FN;
@@ -396,17 +517,19 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
     const Item t = item_at(next_at);
     next_steps = t.steps;
     next_k = t.k0;
-    ra.start(static_cast<const T*>(a.a), a.lda, t.m0, M, t.k0);
-    rb.start(static_cast<const T*>(a.b), a.ldb, t.n0, a.N, t.k0);
+    constexpr int N = PAIRS ? 2 : 1;   // numbers of an element
+    ra.start(static_cast<const T*>(a.a), a.lda, t.m0, M, MODE == kStats || MODE == kGrad ? N * t.k0 : t.k0);
+    rb.start(static_cast<const T*>(a.b), a.ldb, t.n0, a.N, BKC ? N * t.k0 : t.k0);
   };
   auto request = [&](int buffer) __attribute__((always_inline)) {
     if (next_item >= last) return;
     ++ahead;
-    if constexpr (MODE != kWeightGrad)
-      if (next_k + kWideK > K) rb.place((int)a.ldb, K - next_k);
+    // (rows of pairs are padded to whole steps)
+    if constexpr (MODE == kRowGrad || (BKC && !PAIRS))
+      if (next_k + kStep > K) rb.place((int)a.ldb, K - next_k);
     ra.load(a.lda, lds0 + buffer);
     rb.load(a.ldb, lds0 + buffer + BM * kWideK * 2);
-    next_k += kWideK;
+    next_k += kStep;
     if (--next_steps == 0) {
       next_item += stride;
       if (next_item < last) {
@@ -443,13 +566,17 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
     --ahead;
   };
   int buffer = 0;
-  frag<T> fa[2][S::FM], fb[2][S::FN];
+  frag<T> fa[PAIRS ? 3 : 2][S::FM], fb[2][S::FN];
+  auto read_a = [&](int slot, int s) __attribute__((always_inline)) { OpA::read(reinterpret_cast<const T*>(castle_vocab_lds + buffer), fa[slot], wm, s, c, g); };
+  auto read_b = [&](int slot, int s) __attribute__((always_inline)) { OpB::read(reinterpret_cast<const T*>(castle_vocab_lds + buffer) + BM * kWideK, fb[slot], wn, s, c, g); };
+  auto then = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };   // these reads, then the products of the fragments before
   auto read = [&](int slot, int s) __attribute__((always_inline)) {
-    const T* la = reinterpret_cast<const T*>(castle_vocab_lds + buffer);
-    OpA::read(la, fa[slot], wm, s, c, g);
-    OpB::read(la + BM * kWideK, fb[slot], wn, s, c, g);
-    __builtin_amdgcn_sched_barrier(0);   // these reads, then the products of the fragments before
+    read_a(slot, s);
+    read_b(slot, s);
+    then();
   };
+  // logits of pairs: times this
+  const float unit = PAIRS && BKC ? ldexpf(1.f, -(shift_of(__builtin_amdgcn_readfirstlane(a.head->most[0])) + shift_of(__builtin_amdgcn_readfirstlane(a.head->most[1])))) : 1.f;
   if (any) arrive();
   while (item < last) {
     const auto [m0, n0, range, k0, steps] = item_at(at);
@@ -484,24 +611,43 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
       for (int j = 0; j < S::FN; ++j) zero(acc[i][j]);
-    auto multiply = [&](int slot) __attribute__((always_inline)) {
+    auto multiply = [&](int sa, int sb) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-        for (int j = 0; j < S::FN; ++j) mma(acc[i][j], fb[slot][j], fa[slot][i]);
+        for (int j = 0; j < S::FN; ++j) mma(acc[i][j], fb[sb][j], fa[sa][i]);
     };
     for (int it = 0; it < steps; ++it) {
+      if constexpr (PAIRS) {   // 16 of the contraction: first parts at s = 0, their second ones at s = 2; the others at 1 and 3
+        read_a(1, 2);
+        then();
+        multiply(0, 0);
+        read_b(1, 2);
+        then();
+        multiply(1, 0);
+        read_a(2, 1);
+        read_b(0, 1);
+        then();
+        multiply(0, 1);
+        read_a(1, 3);
+        then();
+        multiply(2, 0);
+        read_b(1, 3);
+        then();
+        multiply(1, 0);
+      } else {
 #pragma unroll
-      for (int s = 0; s < kWideK / 16 - 1; ++s) {
-        read(1 - s % 2, s + 1);
-        multiply(s % 2);
+        for (int s = 0; s < kWideK / 16 - 1; ++s) {
+          read(1 - s % 2, s + 1);
+          multiply(s % 2, s % 2);
+        }
       }
       arrive();
       done = buffer;
       buffer = buffer == (S::kStages - 1) * S::kStage ? 0 : buffer + S::kStage;
       if (it + 1 < steps) request(done);
       read(0, 0);   // (behind the last step: for nothing)
-      multiply(1);
+      multiply(PAIRS ? 2 : 1, 1);
     }
     asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");   // the loop may end right behind a product
     __builtin_amdgcn_sched_barrier(0);
@@ -534,7 +680,7 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
           for (int j = 0; j < S::FN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) zt = t[i] == 32 * j + acc_row(r, 0) ? z[j][r] : zt;
-          if (mine) a.tl[m] = zt;
+          if (mine) a.tl[m] = zt * unit;
         }
         float most = kLeast;
 #pragma unroll
@@ -542,15 +688,15 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
 #pragma unroll
           for (int r = 0; r < 16; r += 2) most = fmaxf(fmaxf(most, z[j][r]), z[j][r + 1]);   // fmaxf drops NaNs
         most = fmaxf(most, __shfl_xor(most, 32));
-        const float shift = most * kLog2e;
+        const float log2e = kLog2e * unit, shift = most * log2e;
         float sum[4] = {};
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum[r % 4] += fast_exp2(__builtin_fmaf(z[j][r], kLog2e, -shift));
+          for (int r = 0; r < 16; ++r) sum[r % 4] += fast_exp2(__builtin_fmaf(z[j][r], log2e, -shift));
         float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         s += __shfl_xor(s, 32);
-        if (g == 0 && m < M) a.parts[(int64_t)(n0 / BN * S::WN + wave % S::WN) * a.Rp + m] = vec<float, 2>{most, s};
+        if (g == 0 && m < M) a.parts[(int64_t)(n0 / BN * S::WN + wave % S::WN) * a.Rp + m] = vec<float, 2>{most * unit, s};
         __builtin_amdgcn_sched_barrier(0);
       }
       stored = inside;
@@ -573,8 +719,11 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
         __builtin_amdgcn_sched_barrier(0);
       }
       stored = inside && !a.add;
-    } else if (MODE == kWeightGrad && a.splits > 1) {
+    } else if (MODE == kWeightGrad && (PAIRS || a.splits > 1)) {   // (of pairs, the result itself where the contraction is whole)
       float* out = a.out + (int64_t)range * a.M * a.N;
+      const bool result = PAIRS && a.splits == 1;
+      const int shift = result ? __builtin_amdgcn_readfirstlane(a.gain->shift) + shift_of(__builtin_amdgcn_readfirstlane(a.head->most[0])) : 0;
+      const float gain = result ? a.gain->gain : 1.f;
 #pragma unroll
       for (int i = 0; i < S::FM; ++i) {
         const int m = m0 + wm + 32 * i + c;
@@ -583,15 +732,23 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
         for (int j = 0; j < S::FN; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if (m < M && n0 + wn + 32 * j + 8 * q + 4 * g < a.N) *reinterpret_cast<vec<float, 4>*>(row + 32 * j + 8 * q) = pack4<float>(acc[i][j], q);
+            if (m < M && n0 + wn + 32 * j + 8 * q + 4 * g < a.N) {
+              vec<float, 4> v = pack4<float>(acc[i][j], q);
+              if constexpr (PAIRS) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -shift) * gain;
+              }
+              *reinterpret_cast<vec<float, 4>*>(row + 32 * j + 8 * q) = v;
+            }
         __builtin_amdgcn_sched_barrier(0);
       }
       stored = inside;
     } else {
       // to whole rows through LDS, 32 rows of up to 64 columns at a time, each wave in a part of its own; pieces placed as in the operands
       T* turn = reinterpret_cast<T*>(castle_vocab_lds + S::kStages * S::kStage + wave * 4096);
-      constexpr int FJ = S::FN < 2 ? 1 : 2, CP = 4 * FJ, RP = 64 / CP;   // CP: pieces of a row; RP: rows of a store
-      const int shift = MODE == kWeightGrad ? __builtin_amdgcn_readfirstlane(*a.shift) : 0;
+      constexpr int FJ = PAIRS ? 1 : 2, RP = 8;   // RP: rows of a store, 64 numbers each
+      const int shift = MODE == kWeightGrad ? __builtin_amdgcn_readfirstlane(a.gain->shift) : 0;
+      const float gain = MODE == kWeightGrad ? a.gain->gain : 0.f;
       const int row_end = MODE == kGrad ? min((int)up(count, 64), (int)a.Rp) : M;
 #pragma unroll
       for (int i = 0; i < S::FM; ++i) {
@@ -599,7 +756,7 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) z[j] = acc[i][j];
         if constexpr (MODE == kGrad) {
-          const float shift = l[i] * kLog2e;
+          const float log2e = kLog2e * unit, shift = l[i] * kLog2e;
           t[i] -= a.first + n0 + wn + 4 * g;
           // g exp(z - lse), a factor that is not negative in the exponent; less the factor at the target
           auto form = [&](auto target) __attribute__((always_inline)) {
@@ -608,7 +765,7 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
             for (int j = 0; j < S::FN; ++j)
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
-                float p = fast_exp2(__builtin_fmaf(z[j][r], kLog2e, up));
+                float p = fast_exp2(__builtin_fmaf(z[j][r], log2e, up));
                 if constexpr (decltype(target)::value) p -= t[i] == 32 * j + acc_row(r, 0) ? f[i] : 0.f;
                 z[j][r] = p;
               }
@@ -620,7 +777,7 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 const int n = 32 * j + acc_row(r, 0);
-                const float p = fast_exp2(__builtin_fmaf(z[j][r], kLog2e, -shift)) - (t[i] == n ? 1.f : 0.f);
+                const float p = fast_exp2(__builtin_fmaf(z[j][r], log2e, -shift)) - (t[i] == n ? 1.f : 0.f);
                 z[j][r] = n < end ? p * f[i] : 0.f;
               }
           };
@@ -631,24 +788,29 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
 #pragma unroll
           for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z[j][r] = ldexpf(z[j][r], -shift);
+            for (int r = 0; r < 16; ++r) z[j][r] = ldexpf(z[j][r], -shift) * gain;
         }
 #pragma unroll
         for (int h = 0; h < S::FN / FJ; ++h) {
+          auto put = [&](int p, vec<T, 4> v) __attribute__((always_inline)) { st4<T>(turn + c * 64 + 8 * (p ^ (c >> 1 & 7)) + 4 * g, v); };
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           __builtin_amdgcn_wave_barrier();
 #pragma unroll
           for (int j = 0; j < FJ; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) st4<T>(turn + c * 8 * CP + 8 * ((4 * j + q) ^ (c >> 1 & (CP - 1))) + 4 * g, pack4<T>(z[FJ * h + j], q));
+            for (int q = 0; q < 4; ++q) {
+              const vec<T, 4> first = pack4<T>(z[FJ * h + j], q);
+              put(4 * j + q, first);
+              if constexpr (PAIRS) put(4 + q, __builtin_convertvector(pack4<float>(z[h], q) - __builtin_convertvector(first, vec<float, 4>), vec<T, 4>));
+            }
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           __builtin_amdgcn_wave_barrier();
 #pragma unroll
           for (int k = 0; k < 32 / RP; ++k) {
-            const int row = RP * k + lane / CP, piece = lane % CP, mm = m0 + wm + 32 * i + row, n = n0 + wn + 32 * FJ * h + 8 * piece;
-            const vt v = *reinterpret_cast<const vt*>(turn + row * 8 * CP + 8 * (piece ^ (row >> 1 & (CP - 1))));
-            T* to = static_cast<T*>(a.c) + (MODE == kGrad ? (int64_t)(mm / kBlock * kBlock) * a.ldc + n / kBlock * (kBlock * kBlock) + mm % kBlock * kBlock + n % kBlock
-                                                          : (int64_t)mm * a.ldc + n);
+            const int row = RP * k + lane / 8, piece = lane % 8, mm = m0 + wm + 32 * i + row, n = n0 + wn + 32 * FJ * h + 8 * (PAIRS ? piece % 4 : piece);
+            const vt v = *reinterpret_cast<const vt*>(turn + row * 64 + 8 * (piece ^ (row >> 1 & 7)));
+            constexpr int B = kBlock<PAIRS>;
+            T* to = static_cast<T*>(a.c) + (MODE == kGrad ? mm / B * 64 * a.ldc + n / B * (B * 64) + mm % B * 64 + (PAIRS ? 8 * piece : n % B) : mm * a.ldc + n);
             if (mm < row_end && n < (MODE == kGrad ? (int)a.ldc : a.N)) *reinterpret_cast<vt*>(to) = v;
           }
         }
@@ -659,16 +821,16 @@ template <typename T, int MODE, int BM, int BN> __global__ __launch_bounds__(kWi
   }
 }
 
-template <typename T, int MODE, int BM, int BN> int launch_product_t(const ProductArgs& a, hipStream_t stream) {
-  typedef Shape<MODE, BM, BN> S;
+template <typename T, int MODE, int BM, int BN, bool PAIRS> int launch_product_t(const ProductArgs& a, hipStream_t stream) {
+  typedef Shape<MODE, BM, BN, PAIRS> S;
   static PerDeviceOnce once;
   bool& configured = once.flag();
   if (!configured) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&vocab_product_kernel<T, MODE, BM, BN>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&vocab_product_kernel<T, MODE, BM, BN, PAIRS>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
     configured = true;
   }
   const int64_t items = up(a.M, BM) / BM * (up(a.N, BN) / BN) * a.splits;
-  hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
+  hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN, PAIRS>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -3;
 }
 // rows and columns of a workgroup's tile
@@ -676,16 +838,26 @@ struct Tile { int rows, columns; };
 Tile logits_tile(int R) { return {R <= 64 ? 64 : 256, 256}; }
 Tile row_grad_tile(int R, int D) { return {R <= 64 ? 64 : 256, D <= 128 ? 128 : 256}; }
 Tile weight_grad_tile(int D) { return {256, D <= 128 ? 128 : 256}; }
-template <typename T, int MODE> int launch_logits(const ProductArgs& a, hipStream_t stream) {
-  return logits_tile(a.M).rows == 64 ? launch_product_t<T, MODE, 64, 256>(a, stream) : launch_product_t<T, MODE, 256, 256>(a, stream);
-}
-template <typename T> int launch_row_grad(const ProductArgs& a, hipStream_t stream) {
-  const Tile t = row_grad_tile(a.M, a.N);
-  if (t.rows == 64) return t.columns == 128 ? launch_product_t<T, kRowGrad, 64, 128>(a, stream) : launch_product_t<T, kRowGrad, 64, 256>(a, stream);
-  return t.columns == 128 ? launch_product_t<T, kRowGrad, 256, 128>(a, stream) : launch_product_t<T, kRowGrad, 256, 256>(a, stream);
-}
-template <typename T> int launch_weight_grad(const ProductArgs& a, hipStream_t stream) {
-  return weight_grad_tile(a.N).columns == 128 ? launch_product_t<T, kWeightGrad, 256, 128>(a, stream) : launch_product_t<T, kWeightGrad, 256, 256>(a, stream);
+template <int MODE> int launch_product(const ProductArgs& a, int dtype, hipStream_t stream) {
+  auto of_type = [&](auto t, auto pairs) {
+    using T = decltype(t);
+    constexpr bool P = decltype(pairs)::value;
+    if constexpr (MODE == kStats || MODE == kGrad) {
+      return logits_tile(a.M).rows == 64 ? launch_product_t<T, MODE, 64, 256, P>(a, stream) : launch_product_t<T, MODE, 256, 256, P>(a, stream);
+    } else if constexpr (MODE == kRowGrad) {
+      const Tile tile = row_grad_tile(a.M, a.N);
+      if (tile.rows == 64) return tile.columns == 128 ? launch_product_t<T, MODE, 64, 128, P>(a, stream) : launch_product_t<T, MODE, 64, 256, P>(a, stream);
+      return tile.columns == 128 ? launch_product_t<T, MODE, 256, 128, P>(a, stream) : launch_product_t<T, MODE, 256, 256, P>(a, stream);
+    } else {
+      return weight_grad_tile(a.N).columns == 128 ? launch_product_t<T, MODE, 256, 128, P>(a, stream) : launch_product_t<T, MODE, 256, 256, P>(a, stream);
+    }
+  };
+  switch (dtype) {
+    case 0: return of_type(fp16_t(), std::true_type());
+    case 1: return of_type(bf16_t(), std::false_type());
+    case 2: return of_type(fp16_t(), std::false_type());
+    default: return -1;
+  }
 }
 
 // ---- sizes ----------------------------------------------------------------------------------------------------------
@@ -695,8 +867,9 @@ struct Plan {
   int Dp;                  // width of a copied row
   int P;                   // column ranges of a row's maxima and sums
   int columns, pieces;     // of the vocabulary at a time
-  int64_t ldc;             // of d (fp32: of the logits)
+  int64_t ldc;             // of d
   int row_splits, weight_splits;
+  int step;                // of a contraction
 };
 int64_t tiles(int64_t m, int64_t n, Tile t) { return up(m, t.rows) / t.rows * (up(n, t.columns) / t.columns); }
 // Ranges of a contraction of `steps` for m x n outputs, from what it takes roughly (us): 1.5 a step and 5 an end for each of the items of the fullest CU, and for several ranges their partial
@@ -713,27 +886,23 @@ int splits_for(int64_t m, int64_t n, Tile t, int64_t steps) {
   }
   return best;
 }
+// es: bytes of an element, also of a pair
 Plan plan(const VocabArgs& a, int es) {
   Plan p = {};
+  p.step = es == 4 ? kWideK / 2 : kWideK;
   p.Rp = up(a.R, 64);
-  p.Dp = es == 2 ? (int)up(a.D, kWideK) : a.D;
-  const int64_t fit = kPieceBytes / (p.Rp * es) / 256 * 256, width = up(a.V, 64);
-  p.pieces = (int)((width + std::max<int64_t>(256, fit) - 1) / std::max<int64_t>(256, fit));
+  p.Dp = (int)up(a.D, p.step);
+  const int64_t fit = std::max<int64_t>(256, kPieceBytes / (p.Rp * es) / 256 * 256), width = up(a.V, 64);
+  p.pieces = (int)((width + fit - 1) / fit);
   p.columns = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (a.V + p.columns - 1) / p.columns;
   p.ldc = std::min<int64_t>(p.columns, width);
-  if (es == 2) {
-    const Tile t = logits_tile(a.R);
-    p.P = (int)(up(a.V, t.columns) / t.columns * (t.rows == 256 ? 2 : 4));
-  } else {
-    p.P = p.pieces;
-  }
-  p.row_splits = splits_for(a.R, a.D, row_grad_tile(a.R, a.D), p.ldc / kWideK);
-  p.weight_splits = splits_for(p.ldc, a.D, weight_grad_tile(a.D), p.Rp / kWideK);
+  const Tile t = logits_tile(a.R);
+  p.P = (int)(up(a.V, t.columns) / t.columns * (t.rows == 256 ? 2 : 4));
+  p.row_splits = splits_for(a.R, a.D, row_grad_tile(a.R, a.D), p.ldc / p.step);
+  p.weight_splits = splits_for(p.ldc, a.D, weight_grad_tile(a.D), p.Rp / p.step);
   return p;
 }
-// what the fp32 products of `bytes(columns)` need: of a whole piece of the vocabulary, and of the last one
-template <typename F> int64_t products32(const VocabArgs& a, const Plan& p, F&& bytes) { return std::max(bytes(std::min(a.V, p.columns)), bytes(a.V - (p.pieces - 1) * p.columns)); }
 struct Carve {
   char* at;
   int64_t used = 0;
@@ -745,41 +914,37 @@ struct Carve {
 };
 struct Fwd {
   int* block_counts;
-  char* xc;
+  char *xc, *wc;   // wc: fp32, the pairs of w
   int32_t* tc;
   float *tl, *loss_c, *sums;
   vec<float, 2>* parts;
-  char* logits;
   Fwd(const VocabArgs& a, const Plan& p, int es, Carve& c) {
     block_counts = c.take<int>(up(a.R, kCountRows) / kCountRows);
     xc = c.take<char>(p.Rp * p.Dp * es);
+    wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * 4 : 0);
     tc = c.take<int32_t>(p.Rp);
     tl = c.take<float>(p.Rp);
     loss_c = c.take<float>(p.Rp);
     sums = c.take<float>(pieces_of_row(a.R));
     parts = c.take<vec<float, 2>>(p.P * p.Rp);
-    logits = c.take<char>(es == 4 ? a.R * p.ldc * 4 : 0);
   }
 };
 struct Bwd {
-  char* xc;
+  char *xc, *wc;
   int32_t* tc;
   float* factor;
-  int* shift;
+  Gain* gain;
   char* d;
   float *row_parts, *weight_parts;
-  char* products;
   Bwd(const VocabArgs& a, const Plan& p, int es, bool need_x, bool need_w, Carve& c) {
     xc = c.take<char>(p.Rp * p.Dp * es);
+    wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * 4 : 0);
     tc = c.take<int32_t>(p.Rp);
     factor = c.take<float>(p.Rp);
-    shift = c.take<int>(1);
+    gain = c.take<Gain>(1);
     d = c.take<char>(p.Rp * p.ldc * es);
-    row_parts = c.take<float>(need_x ? (int64_t)(es == 2 ? p.row_splits : p.pieces > 1 ? 2 : 1) * a.R * a.D : 0);
-    weight_parts = c.take<float>(need_w && es == 2 && p.weight_splits > 1 ? p.weight_splits * p.ldc * a.D : 0);
-    products = c.take<char>(es == 2 ? 0 : products32(a, p, [&](int n) {
-      return std::max(gemm_workspace(a.R, a.D, n, 4, false), gemm_workspace(n, a.D, a.R, 4, false));
-    }));
+    row_parts = c.take<float>(need_x ? (int64_t)p.row_splits * a.R * a.D : 0);
+    weight_parts = c.take<float>(need_w && p.weight_splits > 1 ? p.weight_splits * p.ldc * a.D : 0);
   }
 };
 struct State {
@@ -801,79 +966,14 @@ template <bool FIRST> int launch_gather(const RowArgs& a, int dtype, hipStream_t
   });
 }
 
-// ---- fp32: logits of a piece in memory -------------------------------------------------------------------------------
-struct Rows32 {
-  float* z;                // [R][ld]
-  int64_t ld, Rp;
-  int columns, first;      // of the vocabulary
-  const int* count;
-  const int32_t* tc;
-  float* tl;
-  vec<float, 2>* parts;    // of this piece, by rank
-  const float *lse, *factor;
-};
-// a wave to a row
-__global__ __launch_bounds__(kThreads) void row_stats32_kernel(Rows32 a) {
-  typedef vec<float, 4> v4;
-  const int row = blockIdx.x * kWaves + wave_id(), lane = lane_id();
-  if (row >= *a.count) return;
-  const float* z = a.z + row * a.ld;
-  float m = kLeast, s = 0.f;
-  for (int i = lane * 4; i < a.columns; i += 256) {
-    v4 v = *reinterpret_cast<const v4*>(z + i);   // (rows are padded to whole pieces)
-    float mn = m;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (i + e >= a.columns) v[e] = -INFINITY;
-      mn = fmaxf(mn, v[e]);
-    }
-    s *= fast_exp2((m - mn) * kLog2e);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s += fast_exp2((v[e] - mn) * kLog2e);
-    m = mn;
-  }
-  float M = m;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
-  s *= fast_exp2((m - M) * kLog2e);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
-  const int t = a.tc[row] - a.first;
-  if (lane == 0) {
-    a.parts[row] = vec<float, 2>{M, s};
-    if (a.tc[row] >= 0 && t >= 0 && t < a.columns) a.tl[row] = z[t];
-  }
-}
-// z -> d in place; zeros in the rows behind the last
-__global__ __launch_bounds__(kThreads) void row_grad32_kernel(Rows32 a, int R) {
-  typedef vec<float, 4> v4;
-  const int row = blockIdx.x * kWaves + wave_id(), lane = lane_id();
-  if (row >= R) return;
-  const bool counts = row < *a.count;
-  float* z = a.z + row * a.ld;
-  const float l = counts ? a.lse[row] : 0.f, f = counts ? a.factor[row] : 0.f;
-  const int t = counts ? a.tc[row] - a.first : -1;
-  for (int i = lane * 4; i < a.columns; i += 256) {
-    v4 v = *reinterpret_cast<const v4*>(z + i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = counts && i + e < a.columns ? f * (fast_exp2((v[e] - l) * kLog2e) - (t == i + e ? 1.f : 0.f)) : 0.f;
-    *reinterpret_cast<v4*>(z + i) = v;
-  }
-}
-GemmArgs product32(const void* a, int64_t lda, const void* b, int64_t ldb, void* c, int64_t ldc, int M, int N, int K, bool whole = false) {
-  GemmArgs g = {};
-  g.a = a;
-  g.b = b;
-  g.c = c;
-  g.M = M;
-  g.N = N;
-  g.K = K;
-  g.lda = lda;
-  g.ldb = ldb;
-  g.ldc = ldc;
-  g.epilogue = kGemmPlain;
-  g.whole = whole;
-  return g;
+// fp32: the rows of x that count, and w, as pairs
+int launch_split(const VocabArgs& a, const Plan& p, VocabHead* head, const int32_t* rank, void* xc, void* wc, bool first, hipStream_t stream) {
+  const SplitArgs x = {static_cast<const float*>(a.x), a.ld_x, a.R, a.D, p.Dp, rank, &head->count, &head->most[0], static_cast<fp16_t*>(xc)};
+  const SplitArgs w = {static_cast<const float*>(a.w), a.ld_w, a.V, a.D, p.Dp, nullptr, nullptr, &head->most[1], static_cast<fp16_t*>(wc)};
+  if (first) hipLaunchKernelGGL(most_kernel, dim3((unsigned)std::min<int64_t>(1024, up(a.V, kWaves) / kWaves)), dim3(kThreads), 0, stream, w);
+  hipLaunchKernelGGL(split_rows_kernel, dim3((unsigned)(up(p.Rp * (p.Dp / 8), kThreads) / kThreads)), dim3(kThreads), 0, stream, x);
+  hipLaunchKernelGGL(split_rows_kernel, dim3((unsigned)(up((int64_t)a.V * (p.Dp / 8), kThreads) / kThreads)), dim3(kThreads), 0, stream, w);
+  return launched();
 }
 
 }  // namespace
@@ -900,37 +1000,28 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   Carve cs = {static_cast<char*>(state)}, cw = {static_cast<char*>(workspace)};
   const State s(a.R, cs);
   const Fwd f(a, p, es, cw);
-  const RowArgs rows = {a, f.block_counts, s.head, s.rank, f.xc, f.tc, f.tl, p.Dp, es == 4, loss};
+  const RowArgs rows = {a, f.block_counts, s.head, s.rank, f.xc, f.tc, f.tl, p.Dp, loss};
   hipLaunchKernelGGL(count_rows_kernel, dim3((unsigned)(up(a.R, kCountRows) / kCountRows)), dim3(kThreads), 0, stream, rows);
   int rc = launch_gather<true>(rows, dtype, stream);
+  if (rc == 0 && es == 4) rc = launch_split(a, p, s.head, s.rank, f.xc, f.wc, true, stream);
   if (rc != 0) return rc;
-  if (es == 2) {
-    ProductArgs g = {};
-    g.a = f.xc;
-    g.b = a.w;
-    g.lda = p.Dp;
-    g.ldb = a.ld_w;
-    g.M = a.R;
-    g.N = a.V;
-    g.K = a.D;
-    g.count = &s.head->count;
-    g.splits = 1;
-    g.parts = f.parts;
-    g.tl = f.tl;
-    g.Rp = p.Rp;
-    g.tc = f.tc;
-    rc = by_type16(dtype, true, [&](auto t, auto) { return launch_logits<decltype(t), kStats>(g, stream); });
-    if (rc != 0) return rc;
-  } else {
-    for (int i = 0; i < p.pieces; ++i) {
-      const int v0 = i * p.columns, n = std::min(p.columns, a.V - v0);
-      rc = launch_gemm(product32(f.xc, p.Dp, static_cast<const float*>(a.w) + v0 * a.ld_w, a.ld_w, f.logits, p.ldc, a.R, n, a.D, true), true, true, 0, nullptr, stream);
-      if (rc != 0) return rc;
-      const Rows32 r = {reinterpret_cast<float*>(f.logits), p.ldc, p.Rp, n, v0, &s.head->count, f.tc, f.tl, f.parts + i * p.Rp, nullptr, nullptr};
-      hipLaunchKernelGGL(row_stats32_kernel, dim3((a.R + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, r);
-      if (launched() != 0) return -3;
-    }
-  }
+  ProductArgs g = {};
+  g.a = f.xc;
+  g.b = es == 4 ? f.wc : a.w;
+  g.lda = es == 4 ? 2 * p.Dp : p.Dp;
+  g.ldb = es == 4 ? 2 * p.Dp : a.ld_w;
+  g.M = a.R;
+  g.N = a.V;
+  g.K = a.D;
+  g.count = &s.head->count;
+  g.splits = 1;
+  g.parts = f.parts;
+  g.tl = f.tl;
+  g.Rp = p.Rp;
+  g.tc = f.tc;
+  g.head = s.head;
+  rc = launch_product<kStats>(g, dtype, stream);
+  if (rc != 0) return rc;
   const int groups = pieces_of_row(a.R);
   const LossArgs l = {f.parts, s.head, s.rank, f.tl, s.lse, f.loss_c, f.sums, loss, a.R, p.P, a.reduction, p.Rp};
   hipLaunchKernelGGL(row_loss_kernel, dim3(groups), dim3(kThreads), 0, stream, l);
@@ -946,23 +1037,29 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
   Carve cs = {static_cast<char*>(const_cast<void*>(state))}, cw = {static_cast<char*>(workspace)};
   const State s(a.R, cs);
   const Bwd b(a, p, es, dx != nullptr, dw != nullptr, cw);
-  const RowArgs rows = {a, nullptr, s.head, s.rank, b.xc, b.tc, nullptr, p.Dp, es == 4, nullptr};
+  const RowArgs rows = {a, nullptr, s.head, s.rank, b.xc, b.tc, nullptr, p.Dp, nullptr};
   int rc = launch_gather<false>(rows, dtype, stream);
+  if (rc == 0 && es == 4) rc = launch_split(a, p, s.head, s.rank, b.xc, b.wc, false, stream);
   if (rc != 0) return rc;
-  const FactorArgs fa = {dloss, s.head, s.rank, b.tc, b.factor, b.shift, a.R, a.reduction, es == 2};
+  const FactorArgs fa = {dloss, s.head, s.rank, b.tc, b.factor, b.gain, a.R, a.reduction};
   rc = by_tensor_type(dtype, [&](auto t) {
     hipLaunchKernelGGL((factor_kernel<decltype(t)>), dim3(std::min<unsigned>(64, (unsigned)(up(a.R, 1024) / 1024))), dim3(1024), 0, stream, fa);
     return launched();
   });
-  if (rc != 0) return rc;
-  for (int i = 0; i < p.pieces && es == 2; ++i) {
+  auto join = [&](const JoinArgs& j) {
+    return by_tensor_type(dtype, [&](auto t) {
+      hipLaunchKernelGGL((join_rows_kernel<decltype(t)>), dim3((unsigned)(up(j.R * j.D / 4, kThreads) / kThreads)), dim3(kThreads), 0, stream, j);
+      return launched();
+    });
+  };
+  const int64_t ld_x = es == 4 ? 2 * p.Dp : p.Dp, ld_w = es == 4 ? 2 * p.Dp : a.ld_w;   // numbers, as es is 2 bytes or two of them
+  for (int i = 0; i < p.pieces && rc == 0; ++i) {
     const int v0 = i * p.columns, n = std::min(p.columns, a.V - v0);
-    const char* w = static_cast<const char*>(a.w) + v0 * a.ld_w * es;
     ProductArgs g = {};
     g.a = b.xc;
-    g.b = w;
-    g.lda = p.Dp;
-    g.ldb = a.ld_w;
+    g.b = (es == 4 ? b.wc : static_cast<const char*>(a.w)) + v0 * ld_w * 2;
+    g.lda = ld_x;
+    g.ldb = ld_w;
     g.M = a.R;
     g.N = n;
     g.K = a.D;
@@ -975,67 +1072,42 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
     g.factor = b.factor;
     g.c = b.d;
     g.ldc = p.ldc;
-    g.shift = b.shift;
-    ProductArgs gx = g, gw = g;
-    gx.a = b.d;
-    gx.lda = p.ldc;
-    gx.N = a.D;
-    gx.K = n;
-    gx.splits = p.row_splits;
-    gx.out = b.row_parts;
-    gx.part_rows = a.R;
-    gx.add = i > 0;
-    gw.a = b.d;
-    gw.lda = p.ldc;
-    gw.b = b.xc;
-    gw.ldb = p.Dp;
-    gw.M = n;
-    gw.N = a.D;
-    gw.K = a.R;
-    gw.splits = p.weight_splits;
-    gw.c = static_cast<char*>(dw) + (int64_t)v0 * a.D * es;
-    gw.ldc = a.D;
-    gw.out = b.weight_parts;
-    rc = by_type16(dtype, true, [&](auto t, auto) {
-      using T = decltype(t);
-      int e = launch_logits<T, kGrad>(g, stream);
-      if (e == 0 && dx != nullptr) e = launch_row_grad<T>(gx, stream);
-      if (e == 0 && dw != nullptr) e = launch_weight_grad<T>(gw, stream);
-      if (e == 0 && dw != nullptr && gw.splits > 1) {
-        const JoinArgs j = {b.weight_parts, nullptr, b.shift, gw.c, gw.splits, a.D, n, &s.head->count};
-        hipLaunchKernelGGL((join_rows_kernel<T>), dim3((unsigned)(up((int64_t)n * a.D / 4, kThreads) / kThreads)), dim3(kThreads), 0, stream, j);
-        e = launched();
-      }
-      return e;
-    });
-    if (rc != 0) return rc;
-  }
-  for (int i = 0; i < p.pieces && es == 4; ++i) {
-    const int v0 = i * p.columns, n = std::min(p.columns, a.V - v0);
-    const float* w = static_cast<const float*>(a.w) + v0 * a.ld_w;
-    float* const more = reinterpret_cast<float*>(b.products);
-    rc = launch_gemm(product32(b.xc, p.Dp, w, a.ld_w, b.d, p.ldc, a.R, n, a.D, true), true, true, 0, nullptr, stream);
-    if (rc != 0) return rc;
-    const Rows32 r = {reinterpret_cast<float*>(b.d), p.ldc, p.Rp, n, v0, &s.head->count, b.tc, nullptr, nullptr, s.lse, b.factor};
-    hipLaunchKernelGGL(row_grad32_kernel, dim3((a.R + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, r, a.R);
-    if (launched() != 0) return -3;
-    if (dx != nullptr) {
-      float* const out = b.row_parts + (i > 0 ? (int64_t)a.R * a.D : 0);
-      rc = launch_gemm(product32(b.d, p.ldc, w, a.ld_w, out, a.D, a.R, a.D, n), true, false, 0, more, stream);
-      if (rc == 0 && i > 0) rc = launch_part_sum(b.row_parts, 2, (int64_t)a.R * a.D, b.row_parts, 0, stream);
-      if (rc != 0) return rc;
+    g.gain = b.gain;
+    g.head = s.head;
+    rc = launch_product<kGrad>(g, dtype, stream);
+    if (rc == 0 && dx != nullptr) {
+      ProductArgs x = g;
+      x.a = b.d;
+      x.lda = p.ldc;
+      x.N = a.D;
+      x.K = n;
+      x.splits = p.row_splits;
+      x.out = b.row_parts;
+      x.part_rows = a.R;
+      x.add = i > 0;
+      rc = launch_product<kRowGrad>(x, dtype, stream);
     }
-    if (dw != nullptr) {
-      rc = launch_gemm(product32(b.d, p.ldc, b.xc, p.Dp, static_cast<float*>(dw) + (int64_t)v0 * a.D, a.D, n, a.D, a.R), false, false, 0, more, stream);
-      if (rc != 0) return rc;
+    if (rc == 0 && dw != nullptr) {
+      ProductArgs w = g;
+      w.a = b.d;
+      w.lda = p.ldc;
+      w.b = b.xc;
+      w.ldb = ld_x;
+      w.M = n;
+      w.N = a.D;
+      w.K = a.R;
+      w.splits = p.weight_splits;
+      w.c = static_cast<char*>(dw) + (int64_t)v0 * a.D * es;
+      w.ldc = a.D;
+      w.out = w.splits > 1 ? b.weight_parts : static_cast<float*>(w.c);
+      rc = launch_product<kWeightGrad>(w, dtype, stream);
+      if (rc == 0 && w.splits > 1)
+        rc = join({b.weight_parts, nullptr, b.gain, w.c, w.splits, a.D, n, &s.head->count, p.step, es == 4 ? &s.head->most[0] : nullptr});
     }
   }
-  if (dx == nullptr) return 0;
-  const JoinArgs j = {b.row_parts, s.rank, b.shift, dx, es == 2 ? ranges((int)up(std::min(a.V, p.columns), kWideK) / kWideK, p.row_splits) : 1, a.D, a.R, nullptr};
-  return by_tensor_type(dtype, [&](auto t) {
-    hipLaunchKernelGGL((join_rows_kernel<decltype(t)>), dim3((unsigned)(up((int64_t)a.R * a.D / 4, kThreads) / kThreads)), dim3(kThreads), 0, stream, j);
-    return launched();
-  });
+  if (rc != 0 || dx == nullptr) return rc;
+  return join({b.row_parts, s.rank, b.gain, dx, ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.row_splits), a.D, a.R, nullptr, p.step,
+               es == 4 ? &s.head->most[1] : nullptr});
 }
 
 }  // namespace castle

@@ -1,11 +1,12 @@
 """Cross entropy against a vocabulary without the logits (ops.linear_cross_entropy): refusals and shapes without a GPU, results against the definition in 64 bits on one.
 
 Tolerances, element by element, u = 2^-23 (twice the rounding of a 32-bit operation, since the order of the 16 products inside a matrix instruction is its own):
-  logits     products of 16-bit numbers are exact; D of them are added 16 at a time: ez = (D / 16 + 32) u (|x| . |w|).  fp32: an element goes as three parts that hold all of it,
-             six products for one: the same with six times as many additions.
+  logits     products of 16-bit numbers are exact; D of them are added 16 at a time: ez = (D / 16 + 32) u (|x| . |w|).  fp32: an element goes as two parts that hold 2^-22 of it
+             (twice a rounding to 11 bits), three products for one and a fourth left out that is below 2^-22 of it: 3 2^-22 = 6 u of each product, and three times as many additions;
+             six times the bound above covers both.
   loss       twice the largest ez of the row (its log-sum-exp and its own logit), exp and log of 32 bits (16 u (1 + |log-sum-exp|)), and the rounding to the type
   d          a softmax value p is off by p (2 ez + 16 u (1 + |log-sum-exp|)); d = g (p - [target]) is rounded to the type, eps / 2 of it, or to the step 2^-25 below the
-             type's normal numbers, under a factor that brings the largest |g| to 2^14 at least; the sums over blocks of 16 of it as above
+             type's normal numbers, under a factor that brings the largest |g| to 2^14 at least (fp32: its second part, of fp16); the sums over blocks of 16 of it as above
   gradients  that times |w| (or |x|), summed, and the last rounding to the type, of a value or of the smallest normal number"""
 import ctypes
 
@@ -40,8 +41,8 @@ def reference(x, w, target, reduction, dloss, ignore, dtype):
     p[r, t] -= 1
     d = g[:, None] * p
     most = g.abs().max().item() if len(t) else 0.0
-    # (fp32 has neither the rounding nor the factor)
-    off_d = g.abs()[:, None] * off_p + (0 if dtype is torch.float32 else half) * d.abs() + (2.0 ** -25 / 2.0 ** 14 * most if dtype is torch.float16 else 0)
+    # (fp32: the two parts of d are among its sums' bound below)
+    off_d = g.abs()[:, None] * off_p + (0 if dtype is torch.float32 else half) * d.abs() + (2.0 ** -25 / 2.0 ** 14 * most if dtype is not torch.bfloat16 else 0)
     del z, ez, p, off_p
     w_a, x_a, d_a = w.abs(), xk.abs(), d.abs()
     V, six = w.shape[0], 6 if dtype is torch.float32 else 1
