@@ -34,17 +34,32 @@ constexpr float kLeast = -0.5f * __FLT_MAX__;
 
 __host__ __device__ constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+// Factors of the rows of d.  d lies in the 16-bit type (fp32: in pairs of fp16), so the largest factor is 2^14 ... 2^15, which the gradients lose again (Gain): softmax
+// values down to 2^-29 are then normal numbers of fp16 (without it, a mean over 16384 rows would leave nothing of any below 2^-1), and d stays below 2^15.  Where all rows have one
+// factor it is 2^15 itself, and the factor goes to the gradients in 32 bits: most rows have -1 or nearly that at their target, and times a factor that
+// is no power of two all of these would be rounded the same way, 2^-9 of bf16 at worst.
+struct Gain {
+  int shift;    // of d, to be taken back
+  float gain;   // of the gradients
+};
+constexpr int kDShift = 15;
+
 // ---- rows that count -----------------------------------------------------------------------------------------------
 struct RowArgs {
   VocabArgs v;
-  int* block_counts;   // [R / kCountRows]
+  int* block_counts;   // [R / kCountRows], or nullptr: every workgroup counts for itself
   VocabHead* head;
   int32_t* rank;
   void* xc;            // [Rp][Dp]: rows that count, then zero rows up to a multiple of 64 of them; fp32: pairs, see split_rows_kernel
   int32_t* tc;         // [Rp] their targets, -1 outside of the vocabulary
   float* tl;           // [Rp] logits of the targets: NaN until they are found
+  int32_t* row_of;     // [Rp] the row
   int Dp;
   void* loss;          // kEachLoss: zeros for the rows that do not count
+  // backward pass: the factor of each row, and what goes to the gradients (kEachLoss: factor_kernel)
+  const void* dloss;
+  float* factor;
+  Gain* gain;
 };
 __device__ __forceinline__ int64_t class_of(const VocabArgs& a, int64_t r) {
   if (a.n == a.R) return a.target[r];
@@ -100,14 +115,23 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
   const int64_t first = (int64_t)blockIdx.x * kGatherRows;
   int all;
   if constexpr (FIRST) {
-    const int blocks = (a.v.R + kCountRows - 1) / kCountRows, mine = (int)(first / kCountRows);
     int before = 0, total = 0;
-    for (int b = threadIdx.x; b < blocks; b += kThreads) {
-      const int n = a.block_counts[b];
-      total += n;
-      before += b < mine ? n : 0;
+    if (a.block_counts != nullptr) {
+      const int blocks = (a.v.R + kCountRows - 1) / kCountRows, mine = (int)(first / kCountRows);
+      for (int b = threadIdx.x; b < blocks; b += kThreads) {
+        const int n = a.block_counts[b];
+        total += n;
+        before += b < mine ? n : 0;
+      }
+      for (int64_t r = (int64_t)mine * kCountRows + threadIdx.x; r < first; r += kThreads) before += class_of(a.v, r) != a.v.ignore;
+    } else {
+#pragma unroll 4
+      for (int r = threadIdx.x; r < a.v.R; r += kThreads) {
+        const int n = class_of(a.v, r) != a.v.ignore;
+        total += n;
+        before += r < first ? n : 0;
+      }
     }
-    for (int64_t r = (int64_t)mine * kCountRows + threadIdx.x; r < first; r += kThreads) before += class_of(a.v, r) != a.v.ignore;
     before = sum_over_threads<kWaves>(before, s);
     all = sum_over_threads<kWaves>(total, s);
     if (wave_id() == 0) {
@@ -122,12 +146,14 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
       if (counts) {
         a.tc[rank] = t >= 0 && t < a.v.V ? (int32_t)t : -1;
         a.tl[rank] = NAN;
+        a.row_of[rank] = (int32_t)r;
       }
       if (a.v.reduction == kEachLoss && there && !counts) static_cast<T*>(a.loss)[r] = (T)0.f;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) {
       a.head->count = all;
       a.head->inv_count = 1.f / (float)all;
+      a.head->arrived = 0;
     }
   } else {
     all = a.head->count;
@@ -137,8 +163,14 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
       s_rank[lane_id()] = rank;
       if (rank >= 0) {
         const int64_t t = class_of(a.v, r);
-        a.tc[rank] = t >= 0 && t < a.v.V ? (int32_t)t : -1;
+        const bool there = t >= 0 && t < a.v.V;
+        a.tc[rank] = there ? (int32_t)t : -1;
+        if (a.v.reduction != kEachLoss) a.factor[rank] = there ? ldexpf(1.f, kDShift) : NAN;
       }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.v.reduction != kEachLoss) {
+      const float g = (float)*static_cast<const T*>(a.dloss);
+      *a.gain = {kDShift, all == 0 ? 0.f : a.v.reduction == kMeanLoss ? g * a.head->inv_count : g};
     }
   }
   __syncthreads();
@@ -226,18 +258,19 @@ __global__ __launch_bounds__(kThreads) void split_rows_kernel(SplitArgs a) {
   put(row, h, l);
 }
 
-// maxima and sums of the P column ranges -> log-sum-exp of a row, its loss; partial sums of the losses, one of each workgroup
+// Maxima and sums of the P column ranges -> log-sum-exp of a row, its loss.  Sums of the losses of a workgroup's rows; the workgroup that arrives last adds them all, in their
+// order (a launch of its own took 3 to 5 us).
 struct LossArgs {
   const vec<float, 2>* parts;   // [P][Rp]
-  const VocabHead* head;
-  const int32_t* rank;
+  VocabHead* head;
+  const int32_t* row_of;
   const float* tl;
-  float *lse, *loss_c, *sums;   // loss_c: [Rp] by rank
+  float *lse, *sums;
   void* loss;
-  int R, P, reduction;
+  int P, reduction;
   int64_t Rp;
 };
-__global__ __launch_bounds__(kThreads) void row_loss_kernel(LossArgs a) {
+template <typename T> __global__ __launch_bounds__(kThreads) void row_loss_kernel(LossArgs a) {
   typedef vec<float, 2> v2;
   __shared__ float s_m[kLossRows][kThreads / kLossRows + 1], s_s[kLossRows][kThreads / kLossRows + 1];
   const int c = threadIdx.x % kLossRows, q = threadIdx.x / kLossRows, row = blockIdx.x * kLossRows + c, count = a.head->count;
@@ -264,70 +297,59 @@ __global__ __launch_bounds__(kThreads) void row_loss_kernel(LossArgs a) {
     const float lse = m + logf(s);
     a.lse[row] = lse;
     loss = lse - a.tl[row];
-    a.loss_c[row] = loss;
+    if (a.reduction == kEachLoss) static_cast<T*>(a.loss)[a.row_of[row]] = (T)loss;
   }
+  if (a.reduction == kEachLoss) return;
+  __shared__ int s_last;
+  __shared__ float s_sum[kWaves];
   if (threadIdx.x < 64) {
 #pragma unroll
     for (int o = 1; o < kLossRows; o <<= 1) loss += __shfl_xor(loss, o);
-    if (threadIdx.x == 0) a.sums[blockIdx.x] = loss;
+    if (threadIdx.x == 0) {
+      __hip_atomic_store(a.sums + blockIdx.x, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the sum is where every XCD sees it before the count is; release and acquire would write caches back: 1024 workgroups 28 us)
+      s_last = __hip_atomic_fetch_add(&a.head->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
   }
-}
-template <typename T> __global__ __launch_bounds__(kThreads) void loss_kernel(LossArgs a, int groups) {
-  if (a.reduction == kEachLoss) {
-    const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (r < a.R && a.rank[r] >= 0) static_cast<T*>(a.loss)[r] = (T)a.loss_c[a.rank[r]];
-    return;
-  }
-  __shared__ float s[kWaves];
+  __syncthreads();
+  if (!s_last) return;
   float v = 0.f;
-  for (int i = threadIdx.x; i < groups; i += kThreads) v += a.sums[i];
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) v += __hip_atomic_load(a.sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  if (lane_id() == 0) s[wave_id()] = v;
+  if (lane_id() == 0) s_sum[wave_id()] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kWaves; ++w) v += s[w];
-    *static_cast<T*>(a.loss) = (T)(a.reduction == kMeanLoss ? v / (float)a.head->count : v);
+    for (int w = 1; w < kWaves; ++w) v += s_sum[w];
+    *static_cast<T*>(a.loss) = (T)(a.reduction == kMeanLoss ? v / (float)count : v);
   }
 }
 
-// Factors of the rows of d.  d lies in the 16-bit type (fp32: in pairs of fp16), so the largest factor is 2^14 ... 2^15, which the gradients lose again (Gain): softmax
-// values down to 2^-29 are then normal numbers of fp16 (without it, a mean over 16384 rows would leave nothing of any below 2^-1), and d stays below 2^15.  Where all rows have one
-// factor it is 2^15 itself, and the factor goes to the gradients in 32 bits: most rows have -1 or nearly that at their target, and times a factor that
-// is no power of two all of these would be rounded the same way, 2^-9 of bf16 at worst.
-struct Gain {
-  int shift;    // of d, to be taken back
-  float gain;   // of the gradients
-};
+// kEachLoss: factors of the rows, the largest of them at 2^14 ... 2^15
 struct FactorArgs {
-  const void* dloss;
-  const VocabHead* head;
+  const void* dloss;       // [R]
   const int32_t *rank, *tc;
-  float* factor;   // [Rp] by rank
+  float* factor;           // [Rp] by rank
   Gain* gain;
-  int R, reduction;
+  int R;
 };
 template <typename T> __global__ __launch_bounds__(1024) void factor_kernel(FactorArgs a) {
   __shared__ float s[16];
-  const bool each = a.reduction == kEachLoss;
   const T* g = static_cast<const T*>(a.dloss);
-  int shift = 15;
-  if (each) {
-    float most = 0.f;
-    for (int r = threadIdx.x; r < a.R; r += 1024)
-      if (a.rank[r] >= 0) most = fmaxf(most, fabsf((float)g[r]));   // fmaxf drops NaNs
+  float most = 0.f;
+  for (int r = threadIdx.x; r < a.R; r += 1024)
+    if (a.rank[r] >= 0) most = fmaxf(most, fabsf((float)g[r]));   // fmaxf drops NaNs
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-    if (lane_id() == 0) s[wave_id()] = most;
-    __syncthreads();
+  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+  if (lane_id() == 0) s[wave_id()] = most;
+  __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 16; ++w) most = fmaxf(most, s[w]);
-    shift = most > 0.f && most <= __FLT_MAX__ ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
-  }
-  if (threadIdx.x == 0 && blockIdx.x == 0) *a.gain = {shift, a.head->count == 0 ? 0.f : each ? 1.f : a.reduction == kMeanLoss ? (float)*g * a.head->inv_count : (float)*g};
+  for (int w = 0; w < 16; ++w) most = fmaxf(most, s[w]);
+  const int shift = most > 0.f && most <= __FLT_MAX__ ? kDShift - __builtin_amdgcn_frexp_expf(most) : 0;
+  if (threadIdx.x == 0 && blockIdx.x == 0) *a.gain = {shift, 1.f};
   for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < a.R; r += (int64_t)gridDim.x * 1024) {
     const int rank = a.rank[r];
-    if (rank >= 0) a.factor[rank] = a.tc[rank] >= 0 ? ldexpf(each ? (float)g[r] : 1.f, shift) : NAN;
+    if (rank >= 0) a.factor[rank] = a.tc[rank] >= 0 ? ldexpf((float)g[r], shift) : NAN;
   }
 }
 
@@ -833,24 +855,30 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> int launch_product_t
   hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN, PAIRS>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -3;
 }
-// rows and columns of a workgroup's tile
+// Rows and columns of a workgroup's tile.  64 rows for that few; else 128 where 256 leave CUs idle: by what the fullest CU takes (us), 1.4 a step and 5 an end of 256 x 256, 0.85 and
+// 3 of 128 x 256.
 struct Tile { int rows, columns; };
-Tile logits_tile(int R) { return {R <= 64 ? 64 : 256, 256}; }
-Tile row_grad_tile(int R, int D) { return {R <= 64 ? 64 : 256, D <= 128 ? 128 : 256}; }
-Tile weight_grad_tile(int D) { return {256, D <= 128 ? 128 : 256}; }
-template <int MODE> int launch_product(const ProductArgs& a, int dtype, hipStream_t stream) {
+int64_t tiles(int64_t m, int64_t n, Tile t) { return up(m, t.rows) / t.rows * (up(n, t.columns) / t.columns); }
+Tile tile_of(int R, int n, int steps, int splits = 1) {
+  if (R <= 64) return {64, 256};
+  auto cost = [&](Tile t, double step, double end) { return (tiles(R, n, t) * splits + 255) / 256 * (step * steps + end); };
+  return cost({128, 256}, 0.85, 3) < cost({256, 256}, 1.4, 5) ? Tile{128, 256} : Tile{256, 256};
+}
+template <int MODE> int launch_product(const ProductArgs& a, Tile tile, int dtype, hipStream_t stream) {
   auto of_type = [&](auto t, auto pairs) {
     using T = decltype(t);
     constexpr bool P = decltype(pairs)::value;
-    if constexpr (MODE == kStats || MODE == kGrad) {
-      return logits_tile(a.M).rows == 64 ? launch_product_t<T, MODE, 64, 256, P>(a, stream) : launch_product_t<T, MODE, 256, 256, P>(a, stream);
-    } else if constexpr (MODE == kRowGrad) {
-      const Tile tile = row_grad_tile(a.M, a.N);
-      if (tile.rows == 64) return tile.columns == 128 ? launch_product_t<T, MODE, 64, 128, P>(a, stream) : launch_product_t<T, MODE, 64, 256, P>(a, stream);
-      return tile.columns == 128 ? launch_product_t<T, MODE, 256, 128, P>(a, stream) : launch_product_t<T, MODE, 256, 256, P>(a, stream);
-    } else {
-      return weight_grad_tile(a.N).columns == 128 ? launch_product_t<T, MODE, 256, 128, P>(a, stream) : launch_product_t<T, MODE, 256, 256, P>(a, stream);
+    if constexpr (MODE != kWeightGrad) {
+      if (tile.rows == 64) {
+        if constexpr (MODE == kRowGrad)
+          if (tile.columns == 128) return launch_product_t<T, MODE, 64, 128, P>(a, stream);
+        return launch_product_t<T, MODE, 64, 256, P>(a, stream);
+      }
+      if (tile.rows == 128) return launch_product_t<T, MODE, 128, 256, P>(a, stream);
     }
+    if constexpr (MODE == kRowGrad || MODE == kWeightGrad)
+      if (tile.columns == 128) return launch_product_t<T, MODE, 256, 128, P>(a, stream);
+    return launch_product_t<T, MODE, 256, 256, P>(a, stream);
   };
   switch (dtype) {
     case 0: return of_type(fp16_t(), std::true_type());
@@ -861,27 +889,32 @@ template <int MODE> int launch_product(const ProductArgs& a, int dtype, hipStrea
 }
 
 // ---- sizes ----------------------------------------------------------------------------------------------------------
-int pieces_of_row(int R) { return (R + kLossRows - 1) / kLossRows; }
+int loss_groups(int R) { return (R + kLossRows - 1) / kLossRows; }
+struct Split { Tile tile; int ranges; };   // of a contraction
 struct Plan {
   int64_t Rp;              // rows, a multiple of 64
   int Dp;                  // width of a copied row
   int P;                   // column ranges of a row's maxima and sums
   int columns, pieces;     // of the vocabulary at a time
   int64_t ldc;             // of d
-  int row_splits, weight_splits;
+  Tile logits;
+  Split rows, weights;
   int step;                // of a contraction
 };
-int64_t tiles(int64_t m, int64_t n, Tile t) { return up(m, t.rows) / t.rows * (up(n, t.columns) / t.columns); }
-// Ranges of a contraction of `steps` for m x n outputs, from what it takes roughly (us): 1.5 a step and 5 an end for each of the items of the fullest CU, and for several ranges their partial
-// results, written and read at 4 TB/s.
-int splits_for(int64_t m, int64_t n, Tile t, int64_t steps) {
-  int best = 1;
+// Tile and ranges of a contraction of `steps` for m x n outputs, from what it takes roughly (us): so much a step and an end for each of the items of the fullest CU, and for
+// several ranges their partial results, written and read at 4 TB/s.
+Split split_of(int64_t m, int64_t n, int64_t steps, std::initializer_list<Tile> kinds) {
+  Split best = {};
   double best_cost = 1e30;
-  for (int s = 1; s <= 128 && s <= std::max<int64_t>(1, steps / 2); ++s) {
-    const double cost = (tiles(m, n, t) * s + 255) / 256 * (1.5 * steps_of_range((int)steps, s) + 5) + (s > 1 ? 8e-6 / 4 * s * m * n : 0);
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = s;
+  for (const Tile t : kinds) {
+    const bool large = t.rows * t.columns > 128 * 256;
+    const double step = large ? 1.5 : t.rows * t.columns > 64 * 128 ? 1.05 : 0.6, end = large ? 5 : 3;
+    for (int s = 1; s <= 128 && s <= std::max<int64_t>(1, steps / 2); ++s) {
+      const double cost = (tiles(m, n, t) * s + 255) / 256 * (step * steps_of_range((int)steps, s) + end) + (s > 1 ? 8e-6 / 4 * s * m * n : 0);
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = {t, s};
+      }
     }
   }
   return best;
@@ -897,10 +930,12 @@ Plan plan(const VocabArgs& a, int es) {
   p.columns = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (a.V + p.columns - 1) / p.columns;
   p.ldc = std::min<int64_t>(p.columns, width);
-  const Tile t = logits_tile(a.R);
-  p.P = (int)(up(a.V, t.columns) / t.columns * (t.rows == 256 ? 2 : 4));
-  p.row_splits = splits_for(a.R, a.D, row_grad_tile(a.R, a.D), p.ldc / p.step);
-  p.weight_splits = splits_for(p.ldc, a.D, weight_grad_tile(a.D), p.Rp / p.step);
+  p.logits = tile_of(a.R, a.V, p.Dp / p.step);
+  p.P = (int)(up(a.V, 256) / 256 * (p.logits.rows == 256 ? 2 : 4));
+  const int wide = a.D <= 128 ? 128 : 256;
+  p.rows = a.R <= 64 ? split_of(a.R, a.D, p.ldc / p.step, {{64, wide}}) : wide == 128 ? split_of(a.R, a.D, p.ldc / p.step, {{256, 128}})
+                                                                                      : split_of(a.R, a.D, p.ldc / p.step, {{256, 256}, {128, 256}});
+  p.weights = split_of(p.ldc, a.D, p.Rp / p.step, {{256, wide}});
   return p;
 }
 struct Carve {
@@ -915,8 +950,8 @@ struct Carve {
 struct Fwd {
   int* block_counts;
   char *xc, *wc;   // wc: fp32, the pairs of w
-  int32_t* tc;
-  float *tl, *loss_c, *sums;
+  int32_t *tc, *row_of;
+  float *tl, *sums;
   vec<float, 2>* parts;
   Fwd(const VocabArgs& a, const Plan& p, int es, Carve& c) {
     block_counts = c.take<int>(up(a.R, kCountRows) / kCountRows);
@@ -924,8 +959,8 @@ struct Fwd {
     wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * 4 : 0);
     tc = c.take<int32_t>(p.Rp);
     tl = c.take<float>(p.Rp);
-    loss_c = c.take<float>(p.Rp);
-    sums = c.take<float>(pieces_of_row(a.R));
+    row_of = c.take<int32_t>(p.Rp);
+    sums = c.take<float>(loss_groups(a.R));
     parts = c.take<vec<float, 2>>(p.P * p.Rp);
   }
 };
@@ -943,8 +978,8 @@ struct Bwd {
     factor = c.take<float>(p.Rp);
     gain = c.take<Gain>(1);
     d = c.take<char>(p.Rp * p.ldc * es);
-    row_parts = c.take<float>(need_x ? (int64_t)p.row_splits * a.R * a.D : 0);
-    weight_parts = c.take<float>(need_w && p.weight_splits > 1 ? p.weight_splits * p.ldc * a.D : 0);
+    row_parts = c.take<float>(need_x ? (int64_t)p.rows.ranges * a.R * a.D : 0);
+    weight_parts = c.take<float>(need_w && p.weights.ranges > 1 ? p.weights.ranges * p.ldc * a.D : 0);
   }
 };
 struct State {
@@ -1000,8 +1035,10 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   Carve cs = {static_cast<char*>(state)}, cw = {static_cast<char*>(workspace)};
   const State s(a.R, cs);
   const Fwd f(a, p, es, cw);
-  const RowArgs rows = {a, f.block_counts, s.head, s.rank, f.xc, f.tc, f.tl, p.Dp, loss};
-  hipLaunchKernelGGL(count_rows_kernel, dim3((unsigned)(up(a.R, kCountRows) / kCountRows)), dim3(kThreads), 0, stream, rows);
+  // up to 4096 rows the copying workgroups count for themselves, which is less than a launch (fp32 needs the launch for its first zeros)
+  const bool count = es == 4 || a.R > 4096;
+  const RowArgs rows = {a, count ? f.block_counts : nullptr, s.head, s.rank, f.xc, f.tc, f.tl, f.row_of, p.Dp, loss, nullptr, nullptr, nullptr};
+  if (count) hipLaunchKernelGGL(count_rows_kernel, dim3((unsigned)(up(a.R, kCountRows) / kCountRows)), dim3(kThreads), 0, stream, rows);
   int rc = launch_gather<true>(rows, dtype, stream);
   if (rc == 0 && es == 4) rc = launch_split(a, p, s.head, s.rank, f.xc, f.wc, true, stream);
   if (rc != 0) return rc;
@@ -1020,13 +1057,11 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   g.Rp = p.Rp;
   g.tc = f.tc;
   g.head = s.head;
-  rc = launch_product<kStats>(g, dtype, stream);
+  rc = launch_product<kStats>(g, p.logits, dtype, stream);
   if (rc != 0) return rc;
-  const int groups = pieces_of_row(a.R);
-  const LossArgs l = {f.parts, s.head, s.rank, f.tl, s.lse, f.loss_c, f.sums, loss, a.R, p.P, a.reduction, p.Rp};
-  hipLaunchKernelGGL(row_loss_kernel, dim3(groups), dim3(kThreads), 0, stream, l);
+  const LossArgs l = {f.parts, s.head, f.row_of, f.tl, s.lse, f.sums, loss, p.P, a.reduction, p.Rp};
   return by_tensor_type(dtype, [&](auto t) {
-    hipLaunchKernelGGL((loss_kernel<decltype(t)>), dim3(a.reduction == kEachLoss ? (unsigned)(up(a.R, kThreads) / kThreads) : 1), dim3(kThreads), 0, stream, l, groups);
+    hipLaunchKernelGGL((row_loss_kernel<decltype(t)>), dim3(loss_groups(a.R)), dim3(kThreads), 0, stream, l);
     return launched();
   });
 }
@@ -1037,15 +1072,16 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
   Carve cs = {static_cast<char*>(const_cast<void*>(state))}, cw = {static_cast<char*>(workspace)};
   const State s(a.R, cs);
   const Bwd b(a, p, es, dx != nullptr, dw != nullptr, cw);
-  const RowArgs rows = {a, nullptr, s.head, s.rank, b.xc, b.tc, nullptr, p.Dp, nullptr};
+  const RowArgs rows = {a, nullptr, s.head, s.rank, b.xc, b.tc, nullptr, nullptr, p.Dp, nullptr, dloss, b.factor, b.gain};
   int rc = launch_gather<false>(rows, dtype, stream);
   if (rc == 0 && es == 4) rc = launch_split(a, p, s.head, s.rank, b.xc, b.wc, false, stream);
-  if (rc != 0) return rc;
-  const FactorArgs fa = {dloss, s.head, s.rank, b.tc, b.factor, b.gain, a.R, a.reduction};
-  rc = by_tensor_type(dtype, [&](auto t) {
-    hipLaunchKernelGGL((factor_kernel<decltype(t)>), dim3(std::min<unsigned>(64, (unsigned)(up(a.R, 1024) / 1024))), dim3(1024), 0, stream, fa);
-    return launched();
-  });
+  if (rc == 0 && a.reduction == kEachLoss) {
+    const FactorArgs f = {dloss, s.rank, b.tc, b.factor, b.gain, a.R};
+    rc = by_tensor_type(dtype, [&](auto t) {
+      hipLaunchKernelGGL((factor_kernel<decltype(t)>), dim3(std::min<unsigned>(64, (unsigned)(up(a.R, 1024) / 1024))), dim3(1024), 0, stream, f);
+      return launched();
+    });
+  }
   auto join = [&](const JoinArgs& j) {
     return by_tensor_type(dtype, [&](auto t) {
       hipLaunchKernelGGL((join_rows_kernel<decltype(t)>), dim3((unsigned)(up(j.R * j.D / 4, kThreads) / kThreads)), dim3(kThreads), 0, stream, j);
@@ -1074,18 +1110,18 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
     g.ldc = p.ldc;
     g.gain = b.gain;
     g.head = s.head;
-    rc = launch_product<kGrad>(g, dtype, stream);
+    rc = launch_product<kGrad>(g, p.logits, dtype, stream);
     if (rc == 0 && dx != nullptr) {
       ProductArgs x = g;
       x.a = b.d;
       x.lda = p.ldc;
       x.N = a.D;
       x.K = n;
-      x.splits = p.row_splits;
+      x.splits = p.rows.ranges;
       x.out = b.row_parts;
       x.part_rows = a.R;
       x.add = i > 0;
-      rc = launch_product<kRowGrad>(x, dtype, stream);
+      rc = launch_product<kRowGrad>(x, p.rows.tile, dtype, stream);
     }
     if (rc == 0 && dw != nullptr) {
       ProductArgs w = g;
@@ -1096,17 +1132,17 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
       w.M = n;
       w.N = a.D;
       w.K = a.R;
-      w.splits = p.weight_splits;
+      w.splits = p.weights.ranges;
       w.c = static_cast<char*>(dw) + (int64_t)v0 * a.D * es;
       w.ldc = a.D;
       w.out = w.splits > 1 ? b.weight_parts : static_cast<float*>(w.c);
-      rc = launch_product<kWeightGrad>(w, dtype, stream);
+      rc = launch_product<kWeightGrad>(w, p.weights.tile, dtype, stream);
       if (rc == 0 && w.splits > 1)
         rc = join({b.weight_parts, nullptr, b.gain, w.c, w.splits, a.D, n, &s.head->count, p.step, es == 4 ? &s.head->most[0] : nullptr});
     }
   }
   if (rc != 0 || dx == nullptr) return rc;
-  return join({b.row_parts, s.rank, b.gain, dx, ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.row_splits), a.D, a.R, nullptr, p.step,
+  return join({b.row_parts, s.rank, b.gain, dx, ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.rows.ranges), a.D, a.R, nullptr, p.step,
                es == 4 ? &s.head->most[1] : nullptr});
 }
 
