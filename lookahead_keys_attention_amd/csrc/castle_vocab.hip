@@ -27,7 +27,7 @@ constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 constexpr int kWaves = kThreads / 64;
 constexpr int kCountRows = 1024;   // rows of a workgroup that counts
 constexpr int kGatherRows = 16;    // rows of a workgroup that copies
-constexpr int kLossRows = 16;      // rows of a workgroup that joins maxima and sums
+constexpr int kLossRows = 16, kManyLossRows = 64;   // rows of a workgroup that joins maxima and sums: few, and of more than 4096 (one atomic of each: 1024 of them 22 us)
 
 // Where maxima start: a score of -inf has weight 0 behind it wherever it stands, and log2(e) times it is finite.
 constexpr float kLeast = -0.5f * __FLT_MAX__;
@@ -270,14 +270,14 @@ struct LossArgs {
   int P, reduction;
   int64_t Rp;
 };
-template <typename T> __global__ __launch_bounds__(kThreads) void row_loss_kernel(LossArgs a) {
+template <typename T, int ROWS> __global__ __launch_bounds__(kThreads) void row_loss_kernel(LossArgs a) {
   typedef vec<float, 2> v2;
-  __shared__ float s_m[kLossRows][kThreads / kLossRows + 1], s_s[kLossRows][kThreads / kLossRows + 1];
-  const int c = threadIdx.x % kLossRows, q = threadIdx.x / kLossRows, row = blockIdx.x * kLossRows + c, count = a.head->count;
+  __shared__ float s_m[ROWS][kThreads / ROWS + 1], s_s[ROWS][kThreads / ROWS + 1];
+  const int c = threadIdx.x % ROWS, q = threadIdx.x / ROWS, row = blockIdx.x * ROWS + c, count = a.head->count;
   float m = kLeast, s = 0.f;
   if (row < count) {
 #pragma unroll 8
-    for (int p = q; p < a.P; p += kThreads / kLossRows) {
+    for (int p = q; p < a.P; p += kThreads / ROWS) {
       const v2 x = a.parts[p * a.Rp + row];
       const float mn = fmaxf(m, x[0]);
       s = s * fast_exp2((m - mn) * kLog2e) + x[1] * fast_exp2((x[0] - mn) * kLog2e);
@@ -289,7 +289,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void row_loss_kerne
   __syncthreads();
   float loss = 0.f;
   if (q == 0 && row < count) {
-    for (int k = 1; k < kThreads / kLossRows; ++k) {
+    for (int k = 1; k < kThreads / ROWS; ++k) {
       const float mn = fmaxf(m, s_m[c][k]);
       s = s * fast_exp2((m - mn) * kLog2e) + s_s[c][k] * fast_exp2((s_m[c][k] - mn) * kLog2e);
       m = mn;
@@ -304,7 +304,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void row_loss_kerne
   __shared__ float s_sum[kWaves];
   if (threadIdx.x < 64) {
 #pragma unroll
-    for (int o = 1; o < kLossRows; o <<= 1) loss += __shfl_xor(loss, o);
+    for (int o = 1; o < ROWS; o <<= 1) loss += __shfl_xor(loss, o);
     if (threadIdx.x == 0) {
       __hip_atomic_store(a.sums + blockIdx.x, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the sum is where every XCD sees it before the count is; release and acquire would write caches back: 1024 workgroups 28 us)
@@ -696,13 +696,13 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
             for (int r = 0; r < 16; ++r) z[j][r] = 32 * j + acc_row(r, 0) < end ? z[j][r] : -INFINITY;
         }
         const bool mine = m < M && t[i] >= 0 && t[i] < 32 * S::FN && (t[i] & 4) == 0;
-        if (__ballot(mine) != 0) {
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {   // (32 columns at a time: of few waves one has a target there, and all wait for it)
+          if (__ballot(mine && t[i] / 32 == j) == 0) continue;
           float zt = 0.f;
 #pragma unroll
-          for (int j = 0; j < S::FN; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) zt = t[i] == 32 * j + acc_row(r, 0) ? z[j][r] : zt;
-          if (mine) a.tl[m] = zt * unit;
+          for (int r = 0; r < 16; ++r) zt = t[i] == 32 * j + acc_row(r, 0) ? z[j][r] : zt;
+          if (mine && t[i] / 32 == j) a.tl[m] = zt * unit;
         }
         float most = kLeast;
 #pragma unroll
@@ -780,32 +780,26 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
         if constexpr (MODE == kGrad) {
           const float log2e = kLog2e * unit, shift = l[i] * kLog2e;
           t[i] -= a.first + n0 + wn + 4 * g;
-          // g exp(z - lse), a factor that is not negative in the exponent; less the factor at the target
-          auto form = [&](auto target) __attribute__((always_inline)) {
+          if (!inside || __ballot(f[i] < 0.f) != 0) {
+            const int end = m0 + wm + 32 * i + c < M ? a.N - n0 - wn - 4 * g : 0;
+            if (end == 0) t[i] = -1;
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) z[j][r] = 32 * j + acc_row(r, 0) < end ? f[i] * fast_exp2(__builtin_fmaf(z[j][r], log2e, -shift)) : 0.f;
+          } else {   // a factor that is not negative goes to the exponent
             const float up = __builtin_amdgcn_logf(f[i]) - shift;
 #pragma unroll
             for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                float p = fast_exp2(__builtin_fmaf(z[j][r], log2e, up));
-                if constexpr (decltype(target)::value) p -= t[i] == 32 * j + acc_row(r, 0) ? f[i] : 0.f;
-                z[j][r] = p;
-              }
-          };
-          auto form_any = [&]() __attribute__((always_inline)) {
-            const int end = m0 + wm + 32 * i + c < M ? a.N - n0 - wn - 4 * g : 0;
+              for (int r = 0; r < 16; ++r) z[j][r] = fast_exp2(__builtin_fmaf(z[j][r], log2e, up));
+          }
 #pragma unroll
-            for (int j = 0; j < S::FN; ++j)
+          for (int j = 0; j < S::FN; ++j) {
+            if (__ballot(t[i] >= 0 && t[i] / 32 == j) == 0) continue;
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const int n = 32 * j + acc_row(r, 0);
-                const float p = fast_exp2(__builtin_fmaf(z[j][r], log2e, -shift)) - (t[i] == n ? 1.f : 0.f);
-                z[j][r] = n < end ? p * f[i] : 0.f;
-              }
-          };
-          if (!inside || __ballot(f[i] < 0.f) != 0) form_any();
-          else if (__ballot(t[i] >= 0 && t[i] < 32 * S::FN) != 0) form(std::true_type());
-          else form(std::false_type());
+            for (int r = 0; r < 16; ++r) z[j][r] -= t[i] == 32 * j + acc_row(r, 0) ? f[i] : 0.f;
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < S::FN; ++j)
@@ -889,7 +883,8 @@ template <int MODE> int launch_product(const ProductArgs& a, Tile tile, int dtyp
 }
 
 // ---- sizes ----------------------------------------------------------------------------------------------------------
-int loss_groups(int R) { return (R + kLossRows - 1) / kLossRows; }
+int loss_rows(int R) { return R > 4096 ? kManyLossRows : kLossRows; }
+int loss_groups(int R) { return (R + loss_rows(R) - 1) / loss_rows(R); }
 struct Split { Tile tile; int ranges; };   // of a contraction
 struct Plan {
   int64_t Rp;              // rows, a multiple of 64
@@ -1061,7 +1056,8 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   if (rc != 0) return rc;
   const LossArgs l = {f.parts, s.head, f.row_of, f.tl, s.lse, f.sums, loss, p.P, a.reduction, p.Rp};
   return by_tensor_type(dtype, [&](auto t) {
-    hipLaunchKernelGGL((row_loss_kernel<decltype(t)>), dim3(loss_groups(a.R)), dim3(kThreads), 0, stream, l);
+    if (loss_rows(a.R) == kLossRows) hipLaunchKernelGGL((row_loss_kernel<decltype(t), kLossRows>), dim3(loss_groups(a.R)), dim3(kThreads), 0, stream, l);
+    else hipLaunchKernelGGL((row_loss_kernel<decltype(t), kManyLossRows>), dim3(loss_groups(a.R)), dim3(kThreads), 0, stream, l);
     return launched();
   });
 }
