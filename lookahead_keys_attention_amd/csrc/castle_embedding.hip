@@ -84,7 +84,7 @@ __global__ __launch_bounds__(kThreads) void sort_count_kernel(SortArgs a) {
 // From the counts of all workgroups to the place of each digit's first key of each wave here, then the keys to their places: equal digits in the order they came.
 __global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
   const int digits = 1 << a.bits, wave = wave_id(), lane = lane_id();
-  uint32_t* const s_sum = castle_digits + kWaves * digits;   // [kThreads]
+  __shared__ uint32_t s_sum[kWaves];
   for (int d = threadIdx.x; d < kWaves * digits; d += kThreads) castle_digits[d] = 0;
   __syncthreads();
   const int64_t first = ((int64_t)blockIdx.x * kWaves + wave) * a.wave_tokens, last = min(a.tokens.rows, first + a.wave_tokens);
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
 #pragma unroll
     for (int p = 0; p < kMaxPer; ++p) {
       if (p >= per) break;
-#pragma unroll 8
+#pragma unroll 16
       for (int g = 0; g < (int)gridDim.x; ++g) {
         const uint32_t n = a.counts[(int64_t)g * digits + d0 + p];
         all[p] += n;
@@ -107,16 +107,18 @@ __global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
       sum += all[p];
     }
   }
-  s_sum[threadIdx.x] = sum;
-  __syncthreads();
-  for (int o = 1; o < kThreads; o <<= 1) {
-    const uint32_t left = (int)threadIdx.x >= o ? s_sum[threadIdx.x - o] : 0;
-    __syncthreads();
-    s_sum[threadIdx.x] += left;
-    __syncthreads();
+  uint32_t up = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t left = __shfl_up(up, o);
+    up += lane >= o ? left : 0;
   }
+  if (lane == 63) s_sum[wave] = up;
+  __syncthreads();
   if (d0 < digits) {
-    uint32_t at = s_sum[threadIdx.x] - sum;
+    uint32_t at = up - sum;
+#pragma unroll
+    for (int w = 0; w < kWaves - 1; ++w) at += w < wave ? s_sum[w] : 0;
 #pragma unroll
     for (int p = 0; p < kMaxPer; ++p) {
       if (p >= per) break;
@@ -152,6 +154,94 @@ __global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
       a.keys[at] = key;
       a.places[at] = a.places_in != nullptr ? a.places_in[i] : (uint32_t)i;
     }
+  }
+}
+
+// Up to 8192 tokens and 2^18 keys: all in one workgroup of sixteen waves, a pair in one word, eight of them in the registers of a thread, from there to their places in LDS and
+// back.  Lanes of equal digits are found once a pass: a pair's rank among the digits of its wave is kept until the places are known (32000 rows of 512 bf16, the
+// whole gradient: 8192 tokens 42 us, 8256 by four launches 49; the 16384 of which four launches sort in 25 us take a workgroup 34).
+constexpr int kSortRounds = 8, kSortThreads = 1024, kSortTokens = kSortRounds * kSortThreads, kPlaceBits = 13;
+template <int BITS> __global__ __launch_bounds__(kSortThreads) void sort_all_kernel(SortArgs a, int passes) {
+  constexpr int W = kSortThreads / 64, DIGITS = 1 << BITS;
+  const int wave = wave_id(), lane = lane_id(), n = (int)a.tokens.rows;
+  uint32_t* const s_pairs = castle_digits;                  // [kSortTokens]
+  uint32_t* const s_digits = s_pairs + kSortTokens;         // [wave][digit]
+  uint32_t* const mine = s_digits + wave * DIGITS;
+  __shared__ uint32_t s_sum[W];
+  // of each wave a range in order, 64 at a time
+  const int per_wave = ((n + W - 1) / W + 63) / 64 * 64, first = wave * per_wave, last = min(n, first + per_wave);
+  uint32_t e[kSortRounds], rank[kSortRounds];
+#pragma unroll
+  for (int i = 0; i < kSortRounds; ++i) {
+    const int at = first + 64 * i + lane;
+    e[i] = at < last ? key_of(a, at) << kPlaceBits | (uint32_t)at : 0;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = kPlaceBits + pass * BITS;
+    for (int d = threadIdx.x; d < W * DIGITS; d += kSortThreads) s_digits[d] = 0;
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < kSortRounds; ++i) {
+      if (first + 64 * i >= last) break;
+      const bool there = first + 64 * i + lane < last;
+      const uint32_t d = e[i] >> shift & (DIGITS - 1);
+      uint64_t same = __ballot(there);   // lanes of the same digit
+#pragma unroll
+      for (int b = 0; b < BITS; ++b) {
+        const uint64_t ones = __ballot(d >> b & 1);
+        same &= d >> b & 1 ? ones : ~ones;
+      }
+      const uint32_t before = mine[d];
+      rank[i] = before + __popcll(same & below);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (there && (same & below) == 0) mine[d] = before + __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    // the place of each digit's first pair of each wave: a thread has one digit (there are at most as many as threads)
+    const bool digit = (int)threadIdx.x < DIGITS;
+    uint32_t count[W], sum = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      count[w] = digit ? s_digits[w * DIGITS + threadIdx.x] : 0;
+      sum += count[w];
+    }
+    uint32_t up = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t left = __shfl_up(up, o);
+      up += lane >= o ? left : 0;
+    }
+    if (lane == 63) s_sum[wave] = up;
+    __syncthreads();
+    uint32_t at = up - sum;
+    for (int w = 0; w < wave; ++w) at += s_sum[w];
+    if (digit) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        s_digits[w * DIGITS + threadIdx.x] = at;
+        at += count[w];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSortRounds; ++i)
+      if (first + 64 * i + lane < last) s_pairs[mine[e[i] >> shift & (DIGITS - 1)] + rank[i]] = e[i];
+    __syncthreads();
+    if (pass + 1 < passes) {
+#pragma unroll
+      for (int i = 0; i < kSortRounds; ++i) {
+        const int k = first + 64 * i + lane;
+        if (k < last) e[i] = s_pairs[k];
+      }
+    }
+  }
+  for (int k = threadIdx.x; k < n; k += kSortThreads) {
+    a.keys[k] = s_pairs[k] >> kPlaceBits;
+    a.places[k] = s_pairs[k] & ((1u << kPlaceBits) - 1);
   }
 }
 
@@ -202,7 +292,8 @@ template <typename T, int N> __global__ __launch_bounds__(kThreads) void run_sum
                 [&](int i, vec<float, N> v) { *reinterpret_cast<vec<float, N>*>(a.parts + (int64_t)blockIdx.x * a.D + i * N) = v; });
 }
 
-// first sorted place whose key is not below `key`
+// First sorted place whose key is not below `key` (64 lanes that look at 64 places at a time for it make three trips to memory instead of
+// 14, but over 14 times the lines: 16384 tokens, 32000 rows of 512 bf16, 22 -> 37 us).
 __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
   int64_t lo = 0, hi = n;
   while (lo < hi) {
@@ -212,8 +303,9 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, 
   }
   return lo;
 }
-constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that one wave sums by itself
-template <typename T, int N> __global__ __launch_bounds__(kThreads) void table_grad_kernel(SumArgs a) {
+constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that one wave, or part of one, sums by itself
+// LPR: lanes to a row of few tokens
+template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) void table_grad_kernel(SumArgs a) {
   __shared__ int64_t s_bound[2 * kMaxRowsPerGroup];   // first place of a row and of the next one
   __shared__ float s_acc[(kWaves - 1) * N * 64];
   // Rows gridDim.x apart: the frequent tokens of a vocabulary stand together (a workgroup to 31 rows in a row: 162 us for 16384 tokens of 512 bf16 over 32000, the one of
@@ -222,10 +314,10 @@ template <typename T, int N> __global__ __launch_bounds__(kThreads) void table_g
   if ((int)threadIdx.x < 2 * rows) s_bound[threadIdx.x] = lower_bound(a.keys, a.rows, (uint32_t)(blockIdx.x + threadIdx.x / 2 * G + threadIdx.x % 2));
   __syncthreads();
   auto write = [&](int v, int i, vec<float, N> acc) { store_n<T, N>(static_cast<T*>(a.dw) + (int64_t)v * a.D + i * N, acc * a.scale); };
-  for (int k = wave; k < rows; k += kWaves) {
+  for (int k = threadIdx.x / LPR; k < rows; k += kThreads / LPR) {
     const int64_t s = s_bound[2 * k], e = s_bound[2 * k + 1];
     if (e - s > kFew) continue;
-    for (int i = lane; i < pieces; i += 64) write(blockIdx.x + k * G, i, sum_places<T, N>(a, s, e, 1, i));
+    for (int i = threadIdx.x % LPR; i < pieces; i += LPR) write(blockIdx.x + k * G, i, sum_places<T, N>(a, s, e, 1, i));
   }
   for (int k = 0; k < rows; ++k) {   // by all waves: places in front of the first whole piece, whole pieces, places behind
     const int64_t s = s_bound[2 * k], e = s_bound[2 * k + 1];
@@ -280,6 +372,11 @@ SortedGradPlan sorted_grad_plan(int64_t rows, int V, int D) {
   while (bits < 31 && (int64_t)V >> bits != 0) ++bits;   // the keys are 0 .. V
   p.passes = (bits + 9) / 10;
   p.bits = (bits + p.passes - 1) / p.passes;
+  p.together = rows <= kSortTokens && bits <= 18;
+  if (p.together) {   // (the counts of sixteen waves lie in LDS)
+    p.passes = bits <= 9 ? 1 : 2;
+    p.bits = bits > 9 && bits <= 16 ? 8 : 9;
+  }
   // 256 tokens to a wave until there are 256 workgroups, whose counts each of them adds up
   const int64_t waves = std::min<int64_t>(256 * kWaves, std::max<int64_t>(1, (rows + 255) / 256));
   p.wave_tokens = ((rows + waves - 1) / waves + 63) / 64 * 64;
@@ -294,6 +391,17 @@ SortedGradPlan sorted_grad_plan(int64_t rows, int V, int D) {
   return p;
 }
 
+template <int BITS> static int launch_sort_all(const SortArgs& a, int passes, hipStream_t stream) {
+  static PerDeviceOnce once;
+  bool& configured = once.flag();
+  constexpr int kBytes = (kSortTokens + (kSortThreads / 64 << BITS)) * 4;
+  if (!configured) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&sort_all_kernel<BITS>), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes) != hipSuccess) return -3;
+    configured = true;
+  }
+  hipLaunchKernelGGL((sort_all_kernel<BITS>), dim3(1), dim3(kSortThreads), kBytes, stream, a, passes);
+  return launched();
+}
 int launch_sorted_grad(const SortedGradArgs& g, int dtype, hipStream_t stream) {
   const SortedGradPlan& p = g.plan;
   char* at = static_cast<char*>(g.workspace);
@@ -305,19 +413,29 @@ int launch_sorted_grad(const SortedGradArgs& g, int dtype, hipStream_t stream) {
     places[i] = reinterpret_cast<uint32_t*>(take(p.places));
   }
   float* const parts = reinterpret_cast<float*>(take(p.parts));
-  for (int pass = 0; pass < p.passes; ++pass) {
+  if (p.together) {
+    const int last = (p.passes - 1) % 2;
+    const SortArgs a = {g.tokens, g.V, g.padding, 0, p.bits, 0, nullptr, nullptr, keys[last], places[last], nullptr};
+    const int rc = p.bits == 8 ? launch_sort_all<8>(a, p.passes, stream) : launch_sort_all<9>(a, p.passes, stream);
+    if (rc != 0) return rc;
+  }
+  for (int pass = 0; pass < p.passes && !p.together; ++pass) {
     const int to = pass % 2;
     const SortArgs a = {g.tokens, g.V, g.padding, pass * p.bits, p.bits, p.wave_tokens, pass > 0 ? keys[1 - to] : nullptr, pass > 0 ? places[1 - to] : nullptr,
                         keys[to], places[to], counts};
     hipLaunchKernelGGL(sort_count_kernel, dim3(p.groups), dim3(kThreads), 4 << p.bits, stream, a);
-    hipLaunchKernelGGL(sort_place_kernel, dim3(p.groups), dim3(kThreads), (kWaves * 4 << p.bits) + kThreads * 4, stream, a);
+    hipLaunchKernelGGL(sort_place_kernel, dim3(p.groups), dim3(kThreads), kWaves * 4 << p.bits, stream, a);
   }
   const int sorted = (p.passes - 1) % 2;
   const SumArgs s = {keys[sorted], places[sorted], g.tokens.rows, g.dy, g.dw, parts, g.V, g.D, p.rows_per_group, g.scale};
   return by_pieces(dtype, whole_pieces(g.D, g.D, dtype, {g.dy, g.dw}), [&](auto t, auto n) {
     using T = decltype(t);
     if (s.rows >= kRun) hipLaunchKernelGGL((run_sum_kernel<T, n.value>), dim3((unsigned)(s.rows / kRun)), dim3(kThreads), 0, stream, s);
-    hipLaunchKernelGGL((table_grad_kernel<T, n.value>), dim3((unsigned)((g.V + p.rows_per_group - 1) / p.rows_per_group)), dim3(kThreads), 0, stream, s);
+    const dim3 grid((unsigned)((g.V + p.rows_per_group - 1) / p.rows_per_group));
+    const int pieces = g.D / n.value;
+    if (pieces <= 16) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 16>), grid, dim3(kThreads), 0, stream, s);
+    else if (pieces <= 32) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 32>), grid, dim3(kThreads), 0, stream, s);
+    else hipLaunchKernelGGL((table_grad_kernel<T, n.value, 64>), grid, dim3(kThreads), 0, stream, s);
     return launched();
   });
 }

@@ -33,6 +33,7 @@ int launch_embedding(const EmbeddingArgs& a, int dtype, hipStream_t stream);
 // Gradient of the embedding by sorted tokens: sizes of what lies in the workspace, in this order
 struct SortedGradPlan {
   int passes, bits;        // of a digit
+  bool together;           // the sort in one workgroup
   int groups;              // workgroups of a sorting pass
   int64_t wave_tokens;     // tokens of a wave of them
   int rows_per_group;      // vocabulary rows of a workgroup of the sums

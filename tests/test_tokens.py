@@ -174,6 +174,21 @@ def test_gradient_of_one_token_again_and_again(n):
 
 
 @gpu
+@pytest.mark.parametrize("V", [255, 256, 511, 512, 65535, 65536, (1 << 18) - 1, 1 << 18])
+@pytest.mark.parametrize("n", [1, 1023, 8191, 8192, 8193, 16385])
+def test_gradient_where_the_sorting_changes(n, V):
+    """Whole numbers, whose sums are exact in 32 bits: every token in its row, at the digits and numbers of tokens where another way of sorting begins."""
+    g = torch.Generator().manual_seed(n + V)
+    w = torch.zeros(V, 4)
+    ids = (torch.rand(n, generator=g, dtype=torch.float64) * np.log(V + 1)).exp().long().sub(1).clamp(0, V - 1)
+    ids[-1] = V - 1
+    dy = torch.randint(-8, 9, (n, 4), generator=g).float()
+    leaf = w.to(DEV).requires_grad_()
+    ops.embedding(leaf, ids.to(DEV)).backward(dy.to(DEV))
+    assert torch.equal(leaf.grad.cpu(), w.index_add(0, ids, dy))
+
+
+@gpu
 def test_embedding_tokens_that_are_not_there_and_masked_values():
     g = torch.Generator().manual_seed(1)
     w, ids = torch.randn(100, 16, generator=g), torch.randint(0, 100, (4, 50), generator=g)
