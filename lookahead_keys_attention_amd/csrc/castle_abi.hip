@@ -843,7 +843,7 @@ int castle_embedding_grad(const void* dy, const int64_t* index, int64_t index_n,
 
 static int token_rows(castle::TokenRows& t, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows) {
   if (rows <= 0 || rows > kMaxRows || index_n <= 0 || rows % index_n != 0) return CASTLE_ERR_SHAPE;
-  if (index == nullptr || reinterpret_cast<uintptr_t>(index) % 8 != 0) return CASTLE_ERR_ARG;
+  if (index == nullptr || reinterpret_cast<uintptr_t>(index) % 8 != 0 || index_ld < 0) return CASTLE_ERR_ARG;
   t = {index, rows, index_n, index_ld};
   return CASTLE_OK;
 }
@@ -915,7 +915,7 @@ static int vocab_args(castle::VocabArgs& a, const void* x, int64_t ld_x, const v
                       int64_t ignore_index, int rows, int vocabulary, int width, int reduction, int dtype) {
   if (elem_size(dtype) == 0) return CASTLE_ERR_DTYPE;
   if (!vocab_sizes_ok(rows, vocabulary, width) || target_n <= 0 || rows % target_n != 0) return CASTLE_ERR_SHAPE;
-  if (x == nullptr || w == nullptr || target == nullptr || !aligned16({x, w}) || reinterpret_cast<uintptr_t>(target) % 8 != 0 || ld_x < 0 || ld_x % 8 != 0 || ld_w < 0 ||
+  if (x == nullptr || w == nullptr || target == nullptr || !aligned16({x, w}) || reinterpret_cast<uintptr_t>(target) % 8 != 0 || target_ld < 0 || ld_x < 0 || ld_x % 8 != 0 || ld_w < 0 ||
       ld_w % 8 != 0 || ld_w > 1 << 22 || reduction < CASTLE_LOSS_MEAN || reduction > CASTLE_LOSS_EACH)
     return CASTLE_ERR_ARG;
   a = {x, w, ld_x, ld_w, target, target_n, target_ld, ignore_index, rows, vocabulary, width, reduction};

@@ -1131,6 +1131,7 @@ Tensor embedding_op(const Tensor& weight, const Tensor& index, double scale, int
   Tensor y = at::empty(with_width(index, weight.size(1)), weight.options());
   if (y.numel() == 0) return y;
   TORCH_CHECK_VALUE(weight.size(0) > 0, "embedding: tokens, but no vocabulary");
+  TORCH_CHECK_VALUE(weight.size(0) < INT32_MAX && weight.size(1) <= INT32_MAX, "embedding: vocabulary and width below 2^31, got ", weight.sizes());
   const Tensor table = weight.stride(1) == 1 && weight.stride(0) >= 0 ? weight : weight.contiguous();
   const TokenRows tokens(index);
   check(castle_embedding(table.data_ptr(), table.stride(0), (int)table.size(0), (int)table.size(1), tokens.ptr(), tokens.n, tokens.ld, index.numel(), (float)scale,
@@ -1145,6 +1146,8 @@ Tensor embedding_bwd_op(const Tensor& dy_, const Tensor& index, int64_t vocabula
   TORCH_CHECK_VALUE(dy_.dim() == index.dim() + 1 && dy_.sizes().slice(0, index.dim()) == index.sizes(), "embedding_bwd: a row for each token");
   const c10::DeviceGuard guard(dy_.device());
   const int64_t rows = index.numel(), width = dy_.size(-1);
+  TORCH_CHECK_VALUE(vocabulary >= 0 && vocabulary < INT32_MAX && width <= INT32_MAX && padding_idx >= -1 && padding_idx < std::max<int64_t>(vocabulary, 1),
+                    "embedding_bwd: a vocabulary of ", vocabulary, ", a width of ", width, " and padding ", padding_idx);
   if (dy_.numel() == 0 || vocabulary == 0) return at::zeros({vocabulary, width}, dy_.options());
   const Tensor dy = row_major(dy_);
   const TokenRows tokens(index);

@@ -37,8 +37,21 @@ READ_ONCE_BYTES = 320_000_000
 SAMPLER_MAX_VOCABULARY = 20480
 
 
-# From this vocabulary on the loss of a native model is formed without its logits (ops.linear_cross_entropy).
+# From this vocabulary on the loss of a native model is formed without its logits (ops.linear_cross_entropy).  Training in 16 bits, where that takes four products
+# and logits in memory three, forms the logits of more than 2048 rows wider than 512 as long as they take no more than LOGITS_MAX_BYTES.  Measured, us with the logits / without them,
+# loss and gradients, then the loss alone: bf16 2048 x 512 over 16384 233 / 218 and 71 / 57, over 8192 151 / 156 and 43 / 39; 16384 x 512 over 32000 2282 / 2286 and 904 / 596;
+# 2048 x 1024 over 32000 625 / 561, 8192 x 1024 1704 / 2056, and 575 / 518; 8192 x 2048 over 131072 11780 / 15095 and 3698 / 3788; fp32 2048 x 512 over 32000 1455 / 879, 511 / 235.
 LINEAR_LOSS_MIN_VOCABULARY = 16384
+LOGITS_MAX_BYTES = 4 << 30
+
+
+def linear_loss_is_ahead(rows: int, weight: torch.Tensor) -> bool:
+    """Whether the cross entropy of `rows` hidden rows against `weight` is taken without their logits; False where ops.linear_cross_entropy would refuse them."""
+    V, D = weight.shape
+    if not (LINEAR_LOSS_MIN_VOCABULARY <= V <= 1 << 22 and D % 8 == 0 and D <= 1 << 16 and 0 < rows <= 1 << 24):
+        return False
+    kept = weight.element_size() * rows * V
+    return weight.element_size() == 4 or not torch.is_grad_enabled() or rows <= 2048 or D <= 512 or kept > LOGITS_MAX_BYTES
 
 
 # -- sampling helpers (train_triton.py:56-71) ------------------------------------------------
@@ -370,8 +383,7 @@ class CastleLM(nn.Module):
             delta, h = host.feed_forward(h, drop(attended, None), norm.weight, norm.eps, up.weight, down.weight)
             delta = drop(delta, None)
         weight = self.to_logits.weight
-        if (target is not None and LINEAR_LOSS_MIN_VOCABULARY <= weight.shape[0] <= 1 << 22 and weight.shape[1] % 8 == 0 and weight.shape[1] <= 1 << 16
-                and 0 < target.numel() <= 1 << 24):
+        if target is not None and linear_loss_is_ahead(target.numel(), weight):
             return host.head_loss(h, delta, self.final_norm.weight, self.final_norm.eps, weight, target)
         logits = host.head(h, delta, self.final_norm.weight, self.final_norm.eps, self.to_logits.weight)
         if target is not None:

@@ -45,6 +45,19 @@ def test_scale_and_dropout_of_the_dense_model():
             make(False, dropout=bad)
 
 
+def test_where_the_loss_is_taken_without_logits():
+    def ahead(rows, V, D, dtype=torch.bfloat16):
+        return LM.linear_loss_is_ahead(rows, torch.empty(V, D, dtype=dtype, device="meta"))
+
+    assert ahead(2048, 16384, 512) and not ahead(2048, 16383, 512) and ahead(1 << 24, 1 << 22, 512) and ahead(1, 16384, 1 << 16)
+    assert not any(ahead(*bad) for bad in ((2048, (1 << 22) + 1, 512), (2048, 16384, 516), (2048, 16384, (1 << 16) + 8), (0, 16384, 512), ((1 << 24) + 1, 16384, 512)))
+    # in 16 bits with gradients, wide rows go by the logits' memory
+    assert ahead(2048, 32000, 520) and not ahead(2049, 32000, 520) and ahead(2049, 32000, 520, torch.float32)
+    assert not ahead(1 << 14, 1 << 17, 1024) and ahead((1 << 14) + 1, 1 << 17, 1024)
+    with torch.no_grad():
+        assert ahead(2049, 32000, 520)
+
+
 # ---- on a GPU -------------------------------------------------------------------------------------------------------
 def train(model, x):
     model.zero_grad()
@@ -73,6 +86,19 @@ def test_training_step_equals_the_dense_model(tie, dtype):
             handle.remove()
     with torch.no_grad():   # (short sequences of 16 bits go another way without gradients: the same loss, not the same bits)
         assert (native(x, return_loss=True).double() - want[0]).abs() <= tol * want[0].abs()
+
+
+@gpu
+def test_wide_rows_with_and_without_logits(monkeypatch):
+    """Training in bf16 on either side of the rule: the same loss and gradients within what the rounding of logits and of bf16 allows, 2e-2 of the norm."""
+    model = make(True, dim=520, depth=1).bfloat16().to(DEV)
+    x = ids(53, 41).to(DEV)
+    assert not LM.linear_loss_is_ahead(53 * 40, model.to_logits.weight)
+    want = train(model, x)
+    monkeypatch.setattr(LM, "LOGITS_MAX_BYTES", 0)
+    assert LM.linear_loss_is_ahead(53 * 40, model.to_logits.weight)
+    for k, (a, b) in enumerate(zip(train(model, x), want, strict=True)):
+        assert (a.float() - b.float()).norm() <= 2e-2 * b.float().norm(), k
 
 
 @gpu

@@ -114,14 +114,14 @@ def test_entry_points_check_their_arguments_on_the_host():
     emb = lib.castle_embedding
     emb.argtypes = [vp, i64, i, i, vp, i64, i64, i64, f, vp, i, vp]
     good = [p, 8, 10, 8, p, 6, 6, 6, 1.0, p, 1, None]
-    for at, bad, code in ((10, 3, -1), (2, 0, -2), (3, 0, -2), (5, 4, -2), (7, 0, -2), (7, (1 << 30) + 6, -2), (0, None, -5), (0, p + 1, -5), (4, p + 4, -5), (9, p + 1, -5), (1, -8, -5)):
+    for at, bad, code in ((10, 3, -1), (2, 0, -2), (3, 0, -2), (5, 4, -2), (7, 0, -2), (7, (1 << 30) + 6, -2), (0, None, -5), (0, p + 1, -5), (4, p + 4, -5), (9, p + 1, -5), (1, -8, -5), (6, -6, -5)):
         args = list(good)
         args[at] = bad
         assert emb(*args) == code, (at, bad)
     grad = lib.castle_embedding_sorted_grad
     grad.argtypes = [vp, vp, i64, i64, i64, i, i, f, i, vp, i, vp, i64, vp]
     good = [p, p, 6, 6, 6, 10, 8, 1.0, -1, p, 1, p, 1 << 30, None]
-    for at, bad, code in ((10, 7, -1), (2, 4, -2), (4, 0, -2), (5, 0, -2), (0, p + 1, -5), (1, None, -5), (9, None, -5), (8, 10, -5), (8, -2, -5), (11, None, -4), (11, p + 16, -4), (12, 100, -4)):
+    for at, bad, code in ((10, 7, -1), (2, 4, -2), (4, 0, -2), (5, 0, -2), (0, p + 1, -5), (1, None, -5), (9, None, -5), (8, 10, -5), (8, -2, -5), (3, -1, -5), (11, None, -4), (11, p + 16, -4), (12, 100, -4)):
         args = list(good)
         args[at] = bad
         assert grad(*args) == code, (at, bad)
@@ -252,6 +252,25 @@ def test_embedding_gradient_is_the_same_every_time_in_graphs_and_on_other_stream
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, eager)
+
+
+@gpu
+def test_embedding_of_a_table_past_32_bits_of_elements():
+    V, D = 70001, 65536
+    w = torch.zeros(V, D, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator().manual_seed(4)
+    few = torch.tensor([0, 1, 32768, 65535, 65536, 65537, V - 1])
+    rows = torch.randn(len(few), D, generator=g).bfloat16().to(DEV)
+    w[few.to(DEV)] = rows
+    ids = torch.randint(0, len(few), (90,), generator=g)
+    dy = torch.randint(-8, 9, (90, D), generator=g).bfloat16().to(DEV)   # (whole numbers: exact sums)
+    y = ops.embedding(w.requires_grad_(), few[ids].to(DEV), 2.0)
+    assert torch.equal(y, 2 * rows[ids.to(DEV)])
+    grad, = torch.autograd.grad(y, w, dy)
+    want = torch.zeros(len(few), D, device=DEV).index_add_(0, ids.to(DEV), 2 * dy.float())
+    assert torch.equal(grad[few.to(DEV)], want.bfloat16())
+    grad[few.to(DEV)] = 0
+    assert grad.count_nonzero() == 0
 
 
 # ---- dropout --------------------------------------------------------------------------------------------------------

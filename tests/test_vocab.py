@@ -140,7 +140,7 @@ def test_entry_points_check_their_arguments_on_the_host():
     fwd.argtypes = [vp, i64, vp, i64, vp, i64, i64, i64, i, i, i, i, vp, vp, i64, i, vp, i64, vp]
     good = [p, 8, p, 8, p, 6, 6, -100, 6, 10, 8, 0, p, p, 1 << 20, 1, p, 1 << 24, None]
     wrong = [(15, 4, -1), (8, 0, -2), (9, 0, -2), (10, 4, -2), (5, 4, -2), (5, 0, -2), (0, None, -5), (0, p + 8, -5), (2, p + 2, -5), (4, p + 4, -5), (1, 12, -5), (3, 12, -5),
-             (1, -8, -5), (3, 1 << 23, -5), (11, 3, -5), (11, -1, -5), (12, p + 1, -5), (12, None, -5), (13, None, -4), (13, p + 16, -4), (14, 100, -4), (16, None, -4), (16, p + 64, -4),
+             (1, -8, -5), (6, -1, -5), (3, 1 << 23, -5), (11, 3, -5), (11, -1, -5), (12, p + 1, -5), (12, None, -5), (13, None, -4), (13, p + 16, -4), (14, 100, -4), (16, None, -4), (16, p + 64, -4),
              (17, 100, -4)]
     for at, bad, code in wrong:
         args = list(good)
@@ -149,7 +149,7 @@ def test_entry_points_check_their_arguments_on_the_host():
     bwd = lib.castle_linear_cross_entropy_bwd
     bwd.argtypes = [vp, i64, vp, i64, vp, i64, i64, i64, i, i, i, i, vp, vp, i64, vp, vp, i, vp, i64, vp]
     good = [p, 8, p, 8, p, 6, 6, -100, 6, 10, 8, 0, p, p, 1 << 20, p, p, 1, p, 1 << 24, None]
-    for at, bad, code in wrong[1:17] + [(17, 4, -1), (12, None, -5), (12, p + 1, -5), (15, p + 8, -5), (16, p + 8, -5), (13, None, -4), (14, 100, -4), (18, None, -4), (19, 100, -4)]:
+    for at, bad, code in wrong[1:18] + [(17, 4, -1), (12, None, -5), (12, p + 1, -5), (15, p + 8, -5), (16, p + 8, -5), (13, None, -4), (14, 100, -4), (18, None, -4), (19, 100, -4)]:
         args = list(good)
         args[at] = bad
         assert bwd(*args) == code, (at, bad)
@@ -329,6 +329,79 @@ def test_the_same_every_time_in_graphs_and_on_other_streams(dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
+
+
+@gpu
+def test_rows_past_32_bits_of_elements():
+    """Hidden rows of more than 2^32 elements: the last ones have a loss, a gradient and a part in the weight's."""
+    R, D, V, few, dtype = 65600, 65536, 40, 30, torch.bfloat16
+    g = torch.Generator().manual_seed(14)
+    x = torch.zeros(R, D, dtype=dtype, device=DEV)
+    x[-few:] = torch.randn(few, D, generator=g).to(dtype).to(DEV)
+    w = (torch.randn(V, D, generator=g) * D ** -0.5).to(dtype).to(DEV)
+    target = torch.randint(0, V, (R,), generator=g).to(DEV)
+    dloss = torch.zeros(R, dtype=dtype, device=DEV)
+    dloss[-few:] = 0.75
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    each = ops.linear_cross_entropy(*leaves, target, "none")
+    dx, dw = torch.autograd.grad(each, leaves, dloss)
+    ref = reference(x[-few:].detach(), w.detach(), target[-few:], "none", dloss[-few:], -100, dtype)
+    for got, (r, bound), what in zip((each[-few:].detach(), dx[-few:], dw), ref, ("loss", "dx", "dw")):
+        within(got, r, bound, dtype, what)
+    assert not dx[:-few].any()
+
+
+@gpu
+def test_a_vocabulary_past_32_bits_of_elements():
+    """Rows of zeros but for the last ones: their logits are 0, their softmax values one number of each row."""
+    R, D, V, few, dtype = 5, 65536, 65600, 30, torch.bfloat16
+    g = torch.Generator().manual_seed(15)
+    x = torch.randn(R, D, generator=g).to(dtype).to(DEV)
+    w = torch.zeros(V, D, dtype=dtype, device=DEV)
+    w[-few:] = (torch.randn(few, D, generator=g) * D ** -0.5).to(dtype).to(DEV)
+    target = torch.tensor([V - 1, V - 30, V - 31, 0, V - 2], device=DEV)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    each = ops.linear_cross_entropy(*leaves, target, "none")
+    dx, dw = torch.autograd.grad(each, leaves, torch.ones_like(each))
+    z = torch.zeros(R, V, dtype=torch.float64, device=DEV)
+    z[:, -few:] = x.detach().double() @ w[-few:].detach().double().T
+    d = torch.softmax(z, 1)
+    d[range(R), target] -= 1
+    # as for the other sizes: logits off by ez, softmax values by 2 ez, d and the result by half a step
+    x64, w64 = x.detach().double(), w[-few:].detach().double()
+    ez = (D / 16 + 32) * U * (x64.abs() @ w64.abs().T).max()
+    for got, ref, most in ((each.detach(), torch.logsumexp(z, 1) - z[range(R), target], 1.0), (dx, d[:, -few:] @ w64, d[:, -few:].abs() @ w64.abs()),
+                           (dw[-few:], d[:, -few:].T @ x64, d[:, -few:].T.abs() @ x64.abs()), (dw[:3], d[:, :3].T @ x64, d[:, :3].T.abs() @ x64.abs()),
+                           (dw[32768:32771], d[:, 32768:32771].T @ x64, d[:, 32768:32771].T.abs() @ x64.abs())):
+        assert ((got.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (1.02 * 2.0 ** -8 + 2 * ez) * most).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_calls_that_run_at_once(dtype):
+    """Two streams with inputs of their own, and a leaf and a gradient of the loss that are not at 16 bytes."""
+    calls = [inputs(500 + 100 * k, 700, 64, dtype, 16 + k) for k in range(2)]
+    want = [check(*c)[1] for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [None, None]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for k, (x, w, target) in enumerate(calls):
+            with torch.cuda.stream(streams[k]):
+                leaves = [x.detach().requires_grad_(), w.detach().requires_grad_()]
+                got[k] = torch.autograd.grad(ops.linear_cross_entropy(*leaves, target), leaves, torch.tensor(1.25, dtype=dtype, device=DEV))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    x, w, target = calls[0]
+    odd = torch.cat((x.new_zeros(1), x.flatten()))[1:].view(x.shape)
+    dloss = torch.arange(1, len(target) + 2, device=DEV).to(dtype)[1:]
+    leaves = [odd.requires_grad_(), w.requires_grad_()]
+    a = torch.autograd.grad(ops.linear_cross_entropy(*leaves, target, "none"), leaves, dloss)
+    leaves[0] = x.detach().requires_grad_()
+    b = torch.autograd.grad(ops.linear_cross_entropy(*leaves, target, "none"), leaves, dloss.clone())
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 @gpu
