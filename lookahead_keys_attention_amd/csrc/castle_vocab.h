@@ -19,7 +19,6 @@ struct VocabHead {
   int32_t count;
   float inv_count;
   uint32_t arrived;   // workgroups of the forward pass that have their sums there
-  uint32_t most[2];   // fp32: the largest finite |x| of the rows that count, and |w|, as bits
 };
 int64_t vocab_state_bytes(int64_t R);
 int64_t vocab_fwd_bytes(const VocabArgs& a, int es);

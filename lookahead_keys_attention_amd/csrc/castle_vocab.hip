@@ -10,10 +10,11 @@
 // Rows that do not count (target = ignore) are left out at the start: the others are copied together, and what the products cost goes with their number, which the kernels
 // read from device memory.  So whatever a row that does not count holds, infinities and NaNs too, goes nowhere.
 //
-// fp32: an element times a power of two, which brings the largest of its tensor to 2^14 ... 2^15, is the sum of two fp16 numbers that hold 22 bits of it, or what lies above 2^-40 of
-// the largest; a product of two elements is ac' + ca' + aa', three matrix instructions, and what is left out of it is below 2^-22 of the product.  Operands lie as such pairs, 32
-// first parts and the 32 second ones behind them, so a step of 64 numbers is 32 of the contraction, and everything else is that of the 16-bit types.  (The fp32 products of
-// castle_gemm32.hip, of three bf16 parts and six instructions, convert inside the product: 2048 rows of 512 over 32000, logits in memory, 1832 us.)
+// fp32: an element is the sum of three bf16 numbers, 8 bits in each, of any exponent (below 2^-110 it keeps what lies above 2^-134); of the products of two elements' parts the six
+// are formed that are not below 2^-24 of the whole.  Operands lie as such parts, 16 first ones, the 16 second ones and the 16 third ones, so a step is 16 of the contraction, and
+// everything else is that of the 16-bit types.  (Pairs of fp16 numbers with a power of two for each tensor, three products, took 845 us for 2048 rows of 512 over 32000, but
+// what is far below the largest element loses its digits: the gradient of a class whose softmax values are 2^-40 was gone.  The fp32 products of castle_gemm32.hip convert
+// inside the product: logits in memory, 1832 us.)
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
 #include "castle_vocab.h"
@@ -34,7 +35,7 @@ constexpr float kLeast = -0.5f * __FLT_MAX__;
 
 __host__ __device__ constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Factors of the rows of d.  d lies in the 16-bit type (fp32: in pairs of fp16), so the largest factor is 2^14 ... 2^15, which the gradients lose again (Gain): softmax
+// Factors of the rows of d.  d lies in the 16-bit type, so the largest factor is 2^14 ... 2^15, which the gradients lose again (Gain): softmax
 // values down to 2^-29 are then normal numbers of fp16 (without it, a mean over 16384 rows would leave nothing of any below 2^-1), and d stays below 2^15.  Where all rows have one
 // factor it is 2^15 itself, and the factor goes to the gradients in 32 bits: most rows have -1 or nearly that at their target, and times a factor that
 // is no power of two all of these would be rounded the same way, 2^-9 of bf16 at worst.
@@ -43,6 +44,8 @@ struct Gain {
   float gain;   // of the gradients
 };
 constexpr int kDShift = 15;
+// fp32: d is of any size, and the factors are those of the loss, unless the largest is below 2^-20, where the last parts of what is far below it would be lost.
+__device__ __forceinline__ int small_factor_shift(float most) { return most > 0.f && most < 0x1p-20f ? -__builtin_amdgcn_frexp_expf(most) : 0; }
 
 // ---- rows that count -----------------------------------------------------------------------------------------------
 struct RowArgs {
@@ -50,7 +53,7 @@ struct RowArgs {
   int* block_counts;   // [R / kCountRows], or nullptr: every workgroup counts for itself
   VocabHead* head;
   int32_t* rank;
-  void* xc;            // [Rp][Dp]: rows that count, then zero rows up to a multiple of 64 of them; fp32: pairs, see split_rows_kernel
+  void* xc;            // [Rp][Dp]: rows that count, then zero rows up to a multiple of 64 of them; fp32: parts, see split_rows_kernel
   int32_t* tc;         // [Rp] their targets, -1 outside of the vocabulary
   float* tl;           // [Rp] logits of the targets: NaN until they are found
   int32_t* row_of;     // [Rp] the row
@@ -88,25 +91,7 @@ __global__ __launch_bounds__(kThreads) void count_rows_kernel(RowArgs a) {
   }
   n = sum_over_threads<kWaves>(n, s);
   if (threadIdx.x == 0) a.block_counts[blockIdx.x] = n;
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.head->most[0] = a.head->most[1] = 0;
 }
-// The largest of a workgroup's finite |x|, kept as the bits of a float, which are in the order of the numbers (of any order of arrival the same).  Only one that is larger than what
-// is there goes by the atomic: all of 8192 waves took 100 us, one behind the other.
-__device__ __forceinline__ void keep_most(float most, uint32_t* to) {
-  __shared__ float s[kWaves];
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-  if (lane_id() == 0) s[wave_id()] = most;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) most = fmaxf(most, s[w]);
-  const uint32_t bits = __builtin_bit_cast(uint32_t, most);
-  if (bits > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(to, bits);
-}
-__device__ __forceinline__ float finite_abs(float x) { return fabsf(x) <= __FLT_MAX__ ? fabsf(x) : 0.f; }
-// the power of two that brings it to 2^14 ... 2^15
-__device__ __forceinline__ int shift_of(uint32_t most) { return most != 0 ? 15 - __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, most)) : 0; }
 // FIRST: ranks and targets are formed here, else (backward pass) the ranks are there
 template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void gather_rows_kernel(RowArgs a) {
   constexpr int V = elem_traits<T>::vec16;
@@ -157,6 +142,8 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
     }
   } else {
     all = a.head->count;
+    float g = 0.f;   // of every row
+    if (a.v.reduction != kEachLoss && all > 0) g = (float)*static_cast<const T*>(a.dloss) * (a.v.reduction == kMeanLoss ? a.head->inv_count : 1.f);
     if (threadIdx.x < kGatherRows) {
       const int64_t r = first + lane_id();
       const int rank = r < a.v.R ? a.rank[r] : -1;
@@ -165,31 +152,14 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
         const int64_t t = class_of(a.v, r);
         const bool there = t >= 0 && t < a.v.V;
         a.tc[rank] = there ? (int32_t)t : -1;
-        if (a.v.reduction != kEachLoss) a.factor[rank] = there ? ldexpf(1.f, kDShift) : NAN;
+        if (a.v.reduction != kEachLoss) a.factor[rank] = !there ? NAN : sizeof(T) == 4 ? ldexpf(g, small_factor_shift(fabsf(g))) : ldexpf(1.f, kDShift);
       }
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.v.reduction != kEachLoss) {
-      const float g = (float)*static_cast<const T*>(a.dloss);
-      *a.gain = {kDShift, all == 0 ? 0.f : a.v.reduction == kMeanLoss ? g * a.head->inv_count : g};
-    }
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.v.reduction != kEachLoss) *a.gain = sizeof(T) == 4 ? Gain{small_factor_shift(fabsf(g)), 1.f} : Gain{kDShift, g};
   }
   __syncthreads();
   const int pieces = a.Dp / V, have = a.v.D / V;
-  if constexpr (sizeof(T) == 4) {   // (copied as pairs by a launch of its own, once the largest is known)
-    if constexpr (FIRST) {
-      float most = 0.f;
-      for (int k = wave_id(); k < kGatherRows; k += kWaves) {
-        if (s_rank[k] < 0) continue;
-        const T* from = static_cast<const T*>(a.v.x) + (first + k) * a.v.ld_x;
-        for (int i = lane_id(); i < have; i += 64) {
-          const vt x = *reinterpret_cast<const vt*>(from + i * V);
-#pragma unroll
-          for (int e = 0; e < V; ++e) most = fmaxf(most, finite_abs(x[e]));
-        }
-      }
-      keep_most(most, &a.head->most[0]);
-    }
-  } else {
+  if constexpr (sizeof(T) == 2) {   // (fp32: as parts, by a launch of its own)
     const vt none = {};
     for (int k = wave_id(); k < kGatherRows; k += kWaves) {
       const int rank = s_rank[k];
@@ -208,54 +178,50 @@ template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void ga
   }
 }
 
-// fp32: the largest |w|, and rows as pairs: 32 first parts, the 32 second ones, the next 32 columns
+// fp32: rows as parts, of 16 columns the first ones, the second and the third ones
 struct SplitArgs {
   const float* from;       // rows of ld
   int64_t ld;
   int rows, D, Dp;
   const int32_t* rank;     // nullptr, or where a row goes (-1: nowhere) and `count`, behind which rows up to a multiple of 64 are zero
   const int* count;
-  uint32_t* most;
-  fp16_t* to;              // [rows][2 Dp]
+  bf16_t* to;              // [rows][3 Dp]
 };
-__global__ __launch_bounds__(kThreads) void most_kernel(SplitArgs a) {
-  typedef vec<float, 4> v4;
-  float most = 0.f;
-  for (int64_t r = (int64_t)blockIdx.x * kWaves + wave_id(); r < a.rows; r += (int64_t)gridDim.x * kWaves) {
-#pragma unroll 4
-    for (int i = lane_id(); i < a.D / 4; i += 64) {
-      const v4 x = *reinterpret_cast<const v4*>(a.from + r * a.ld + i * 4);
+constexpr int kPart = 16;   // columns
+template <int N> struct Parts { vec<bf16_t, N> p[3]; };
+// ANY: a finite number that bf16 rounds to infinity has its largest one as first part
+template <bool ANY, int N> __device__ __forceinline__ Parts<N> split_in_three(vec<float, N> x) {
+  constexpr float kMost = 0x1.fep127f;
+  Parts<N> r;
+  vec<float, N> first = x;
+  if constexpr (ANY)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) most = fmaxf(most, finite_abs(x[e]));
-    }
+    for (int e = 0; e < N; ++e) first[e] = fabsf(x[e]) > kMost && fabsf(x[e]) <= __FLT_MAX__ ? copysignf(kMost, x[e]) : x[e];
+  r.p[0] = __builtin_convertvector(first, vec<bf16_t, N>);
+#pragma unroll
+  for (int k = 1; k < 3; ++k) {
+    x -= __builtin_convertvector(r.p[k - 1], vec<float, N>);
+    r.p[k] = __builtin_convertvector(x, vec<bf16_t, N>);
   }
-  keep_most(most, a.most);
-}
-__device__ __forceinline__ void split_in_two(vec<float, 8> x, frag<fp16_t>& h, frag<fp16_t>& l) {
-  h = __builtin_convertvector(x, frag<fp16_t>);
-  l = __builtin_convertvector(x - __builtin_convertvector(h, vec<float, 8>), frag<fp16_t>);
+  return r;
 }
 __global__ __launch_bounds__(kThreads) void split_rows_kernel(SplitArgs a) {
-  const int shift = shift_of(*a.most), per = a.Dp / 8;
+  const int per = a.Dp / 8;
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, r = i / per;
   if (r >= (a.rank != nullptr ? up(a.rows, 64) : a.rows)) return;
   const int c = (int)(i - r * per) * 8;
-  auto put = [&](int64_t row, frag<fp16_t> h, frag<fp16_t> l) __attribute__((always_inline)) {
-    fp16_t* to = a.to + row * 2 * a.Dp + c / 32 * 64 + c % 32;
-    *reinterpret_cast<frag_mem<fp16_t>*>(to) = h;
-    *reinterpret_cast<frag_mem<fp16_t>*>(to + 32) = l;
+  auto put = [&](int64_t row, vec<float, 8> x) __attribute__((always_inline)) {
+    const Parts<8> parts = split_in_three<true>(x);
+    bf16_t* to = a.to + row * 3 * a.Dp + c / kPart * (3 * kPart) + c % kPart;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<frag_mem<bf16_t>*>(to + k * kPart) = parts.p[k];
   };
-  if (a.rank != nullptr && r >= *a.count && r < up(*a.count, 64)) put(r, zero_frag<fp16_t>(), zero_frag<fp16_t>());
+  vec<float, 8> x = {};
+  if (a.rank != nullptr && r >= *a.count && r < up(*a.count, 64)) put(r, x);
   const int64_t row = a.rank == nullptr ? r : r < a.rows ? a.rank[r] : -1;
   if (row < 0) return;
-  frag<fp16_t> h = zero_frag<fp16_t>(), l = h;
-  if (c < a.D) {
-    vec<float, 8> x = *reinterpret_cast<const frag_mem<float>*>(a.from + r * a.ld + c);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], shift);
-    split_in_two(x, h, l);
-  }
-  put(row, h, l);
+  if (c < a.D) x = *reinterpret_cast<const frag_mem<float>*>(a.from + r * a.ld + c);
+  put(row, x);
 }
 
 // Maxima and sums of the P column ranges -> log-sum-exp of a row, its loss.  Sums of the losses of a workgroup's rows; the workgroup that arrives last adds them all, in their
@@ -325,7 +291,7 @@ template <typename T, int ROWS> __global__ __launch_bounds__(kThreads) void row_
   }
 }
 
-// kEachLoss: factors of the rows, the largest of them at 2^14 ... 2^15
+// kEachLoss: factors of the rows, the largest of them at 2^14 ... 2^15 (fp32: see small_factor_shift)
 struct FactorArgs {
   const void* dloss;       // [R]
   const int32_t *rank, *tc;
@@ -345,7 +311,7 @@ template <typename T> __global__ __launch_bounds__(1024) void factor_kernel(Fact
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 16; ++w) most = fmaxf(most, s[w]);
-  const int shift = most > 0.f && most <= __FLT_MAX__ ? kDShift - __builtin_amdgcn_frexp_expf(most) : 0;
+  const int shift = sizeof(T) == 4 ? small_factor_shift(most) : most > 0.f && most <= __FLT_MAX__ ? kDShift - __builtin_amdgcn_frexp_expf(most) : 0;
   if (threadIdx.x == 0 && blockIdx.x == 0) *a.gain = {shift, 1.f};
   for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < a.R; r += (int64_t)gridDim.x * 1024) {
     const int rank = a.rank[r];
@@ -367,7 +333,6 @@ struct JoinArgs {
   int64_t R;
   const int* count;     // nullptr, or the contraction: there are as many partial results as it has ranges
   int step;             // of the contraction
-  const uint32_t* most; // fp32: of the other operand, whose power of two goes as well; else nullptr
 };
 template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kernel(JoinArgs a) {
   typedef vec<float, 4> v4;
@@ -382,7 +347,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kern
     const float* p = a.parts + (int64_t)rank * a.D + c;
 #pragma unroll 4
     for (int k = 0; k < splits; ++k) v += *reinterpret_cast<const v4*>(p + k * a.R * a.D);
-    const int shift = a.gain->shift + (a.most != nullptr ? shift_of(*a.most) : 0);
+    const int shift = a.gain->shift;
     const float gain = a.gain->gain;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -shift) * gain;
@@ -417,82 +382,88 @@ struct ProductArgs {
   int64_t part_rows;
   int add;
   const Gain* gain;
-  const VocabHead* head;   // fp32: the largest elements of x and w
 };
 
-// Pairs of fp16 numbers instead of single ones, K of them a step: the second parts lie 32 places behind the first ones, in a row as in LDS.
-// an operand that is not contraction-contiguous: rows k and k + 32 in LDS are the two parts of row k
-template <typename T, int FREE> struct PairOperand : WideOperand<T, false, FREE> {
-  typedef WideOperand<T, false, FREE> W;
+// PARTS: a step is 16 of the contraction, its first parts at s = 0 of what is in LDS, the second and third ones at 1 and 2; the last quarter of the place is not used (there the
+// third ones lie again)
+template <typename T, bool KC, int FREE> struct PartsOperand : WideOperand<T, KC, FREE> {
+  typedef WideOperand<T, KC, FREE> W;
   __device__ __forceinline__ void start(const T* p, int64_t ld, int free0, int free_end, int k0) {
-    W::at = p + k0 * ld + 2 * free0;
+    W::at = KC ? p + free0 * ld + 3 * k0 : p + k0 * ld + 3 * free0;
     W::left = free_end - free0;
-    place((int)ld, kWideK / 2);
+    place((int)ld, kPart);
   }
+  // steps: what is left of the contraction, behind whose end (rows, not contraction-contiguous) the last one is read again
   __device__ __forceinline__ void place(int ld, int steps) {
-    constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
     const int lane = lane_id(), first = wave_id() * W::N;
 #pragma unroll
     for (int q = 0; q < W::N; ++q) {
-      const int k = ROWS * (first + q) + lane / PIECES, p = lane % PIECES ^ 4 * (k & 3), piece = 8 * p < W::left ? p : 0;
-      W::off[q] = 2 * (uint32_t)(min(k % 32, steps - 1) * ld + piece / 4 * 64 + k / 32 * 32 + 8 * (piece % 4));
+      if constexpr (KC) {
+        const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7);
+        W::off[q] = 2 * (uint32_t)(ld * min(row, W::left - 1) + 8 * min(piece, 5));
+      } else {
+        constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
+        const int k = ROWS * (first + q) + lane / PIECES, p = lane % PIECES ^ 4 * (k & 3), piece = 8 * p < W::left ? p : 0;
+        W::off[q] = 2 * (uint32_t)(min(k % kPart, steps - 1) * ld + piece / 2 * (3 * kPart) + min(k / kPart, 2) * kPart + 8 * (piece % 2));
+      }
     }
   }
   __device__ __forceinline__ void load(int64_t ld, uint32_t lds) {
 #pragma unroll
     for (int q = 0; q < W::N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * W::N + q));
-    W::at += kWideK / 2 * ld;
+    W::at += KC ? 3 * kPart : kPart * ld;
   }
 };
 
-// d lies in blocks of 64 x 64 (pairs: 32 x 32 pairs), whole rows of blocks one behind the other, so a step of either product that reads it fetches pieces of 4 or 8 KB.  (As rows
-// of V, 128 bytes here and there, 64 KB and more apart: the same time where the caches hold a band of columns.)
-template <bool PAIRS> constexpr int kBlock = PAIRS ? 32 : 64;   // rows; a row of a block is 64 numbers
-template <typename T, bool KC, int FREE, bool PAIRS> struct BlockOperand : WideOperand<T, KC, FREE> {
+// d lies in blocks of 64 x 64 (parts: 16 x 16), whole rows of blocks one behind the other, so a step of either product that reads it fetches pieces of 8 KB (parts: 1.5, or whole rows
+// of blocks).  (As rows of V, 128 bytes here and there, 64 KB and more apart: the same time where the caches hold a band of columns.)
+template <bool PARTS> constexpr int kBlock = PARTS ? kPart : 64;          // rows and columns
+template <bool PARTS> constexpr int kBlockRow = PARTS ? 3 * kPart : 64;   // numbers of a row
+template <typename T, bool KC, int FREE, bool PARTS> struct BlockOperand : WideOperand<T, KC, FREE> {
   typedef WideOperand<T, KC, FREE> W;
-  static constexpr int B = kBlock<PAIRS>;
-  // p: [row of blocks][ldc / B][B][64]
+  static constexpr int B = kBlock<PARTS>, BR = kBlockRow<PARTS>;
+  // p: [row of blocks][ldc / B][B][BR]
   __device__ __forceinline__ void start(const T* p, int64_t ldc, int free0, int free_end, int k0) {
-    const int lane = lane_id(), first = wave_id() * W::N, row_of_blocks = 64 * (int)ldc;
+    const int lane = lane_id(), first = wave_id() * W::N, row_of_blocks = BR * (int)ldc;
     W::left = free_end - free0;
-    W::at = p + (KC ? free0 : k0) / B * (int64_t)row_of_blocks + (KC ? k0 : free0) / B * (B * 64);
+    W::at = p + (KC ? free0 : k0) / B * (int64_t)row_of_blocks + (KC ? k0 : free0) / B * (B * BR);
 #pragma unroll
     for (int q = 0; q < W::N; ++q) {
       if constexpr (KC) {
         const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7), there = min(row, W::left - 1);
-        W::off[q] = 2 * (uint32_t)(there / B * row_of_blocks + there % B * 64 + 8 * piece);
+        W::off[q] = 2 * (uint32_t)(there / B * row_of_blocks + there % B * BR + 8 * (PARTS ? min(piece, 5) : piece));
       } else {
         constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES, P = B / 8;   // P: pieces of a row of a block, of one part
         const int k = ROWS * (first + q) + lane / PIECES, p = lane % PIECES ^ 4 * (k & 3), piece = 8 * p < W::left ? p : 0;
-        W::off[q] = 2 * (uint32_t)(piece / P * (B * 64) + k % B * 64 + k / B * 32 + 8 * (piece % P));
+        W::off[q] = 2 * (uint32_t)(piece / P * (B * BR) + k % B * BR + min(k / B, 2) * B + 8 * (piece % P));
       }
     }
   }
   __device__ __forceinline__ void load(int64_t ldc, uint32_t lds) {
 #pragma unroll
     for (int q = 0; q < W::N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * W::N + q));
-    W::at += KC ? (int64_t)B * 64 : 64 * ldc;
+    W::at += KC ? (int64_t)B * BR : BR * ldc;
   }
 };
 
 // Eight waves over BM x BN: four by two of them for 256 rows, else two by four.
-template <int MODE, int BM, int BN, bool PAIRS> struct Shape {
+template <int MODE, int BM, int BN, bool PARTS> struct Shape {
   static constexpr int WM = BM == 256 ? 4 : 2, WN = 8 / WM, FM = BM / 32 / WM, FN = BN / 32 / WN;
-  static constexpr bool kTurn = MODE == kGrad || (MODE == kWeightGrad && !PAIRS);   // a tile goes through LDS to whole rows, 4 KB of each wave
+  static constexpr bool kTurn = MODE == kGrad || (MODE == kWeightGrad && !PARTS);   // a tile goes through LDS to whole rows, 4 KB of each wave
   static constexpr int kStage = (BM + BN) * kWideK * 2, kTurnBytes = kTurn ? 4096 * 8 : 0;
   static constexpr int kFit = (kMaxLds - kTurnBytes) / kStage, kStages = kFit < 3 ? kFit : 3;
   static constexpr int kLoads = kStage / 1024 / 8, kLds = kStages * kStage + kTurnBytes;
-  static constexpr int kStores = MODE == kStats ? FM : MODE == kRowGrad || PAIRS ? 4 * FM * FN : 2 * FM * FN;   // of a wave and tile (kWeightGrad: partial results are twice as many)
+  static constexpr int kStores = MODE == kStats ? FM : PARTS && MODE == kGrad ? 6 * FM * FN : MODE == kRowGrad || PARTS ? 4 * FM * FN : 2 * FM * FN;   // of a wave and tile (kWeightGrad: partial results are twice as many)
   static_assert(kStages >= 2 && FM >= 1 && FN >= 1, "");
 };
 extern __shared__ __attribute__((aligned(16))) unsigned char castle_vocab_lds[];
 
-template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
-  typedef Shape<MODE, BM, BN, PAIRS> S;
+template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
+  typedef Shape<MODE, BM, BN, PARTS> S;
   constexpr bool AK = MODE != kWeightGrad, BKC = MODE == kStats || MODE == kGrad;
-  constexpr int kStep = PAIRS ? kWideK / 2 : kWideK;   // of the contraction
-  typedef std::conditional_t<MODE == kRowGrad || MODE == kWeightGrad, BlockOperand<T, AK, BM, PAIRS>, WideOperand<T, AK, BM>> OpA;
-  typedef std::conditional_t<PAIRS && !BKC, PairOperand<T, BN>, WideOperand<T, BKC, BN>> OpB;
+  constexpr int kStep = PARTS ? kPart : kWideK;   // of the contraction
+  typedef std::conditional_t<MODE == kRowGrad || MODE == kWeightGrad, BlockOperand<T, AK, BM, PARTS>, std::conditional_t<PARTS, PartsOperand<T, AK, BM>, WideOperand<T, AK, BM>>> OpA;
+  typedef std::conditional_t<PARTS, PartsOperand<T, BKC, BN>, WideOperand<T, BKC, BN>> OpB;
   typedef vec<T, 8> vt;
   const int lane = lane_id(), wave = wave_id(), c = lane & 31, g = lane >> 5;
   const int count = __builtin_amdgcn_readfirstlane(*a.count), M = MODE == kWeightGrad ? a.M : min(a.M, count), K = MODE == kWeightGrad ? (int)up(min(a.K, count), kStep) : a.K;
@@ -539,15 +510,14 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
     const Item t = item_at(next_at);
     next_steps = t.steps;
     next_k = t.k0;
-    constexpr int N = PAIRS ? 2 : 1;   // numbers of an element
-    ra.start(static_cast<const T*>(a.a), a.lda, t.m0, M, MODE == kStats || MODE == kGrad ? N * t.k0 : t.k0);
-    rb.start(static_cast<const T*>(a.b), a.ldb, t.n0, a.N, BKC ? N * t.k0 : t.k0);
+    ra.start(static_cast<const T*>(a.a), a.lda, t.m0, M, t.k0);
+    rb.start(static_cast<const T*>(a.b), a.ldb, t.n0, a.N, t.k0);
   };
   auto request = [&](int buffer) __attribute__((always_inline)) {
     if (next_item >= last) return;
     ++ahead;
-    // (rows of pairs are padded to whole steps)
-    if constexpr (MODE == kRowGrad || (BKC && !PAIRS))
+    // (rows of parts are padded to whole steps)
+    if constexpr (MODE == kRowGrad || (BKC && !PARTS))
       if (next_k + kStep > K) rb.place((int)a.ldb, K - next_k);
     ra.load(a.lda, lds0 + buffer);
     rb.load(a.ldb, lds0 + buffer + BM * kWideK * 2);
@@ -588,7 +558,7 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
     --ahead;
   };
   int buffer = 0;
-  frag<T> fa[PAIRS ? 3 : 2][S::FM], fb[2][S::FN];
+  frag<T> fa[PARTS ? 3 : 2][S::FM], fb[2][S::FN];
   auto read_a = [&](int slot, int s) __attribute__((always_inline)) { OpA::read(reinterpret_cast<const T*>(castle_vocab_lds + buffer), fa[slot], wm, s, c, g); };
   auto read_b = [&](int slot, int s) __attribute__((always_inline)) { OpB::read(reinterpret_cast<const T*>(castle_vocab_lds + buffer) + BM * kWideK, fb[slot], wn, s, c, g); };
   auto then = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };   // these reads, then the products of the fragments before
@@ -597,8 +567,6 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
     read_b(slot, s);
     then();
   };
-  // logits of pairs: times this
-  const float unit = PAIRS && BKC ? ldexpf(1.f, -(shift_of(__builtin_amdgcn_readfirstlane(a.head->most[0])) + shift_of(__builtin_amdgcn_readfirstlane(a.head->most[1])))) : 1.f;
   if (any) arrive();
   while (item < last) {
     const auto [m0, n0, range, k0, steps] = item_at(at);
@@ -640,23 +608,20 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
         for (int j = 0; j < S::FN; ++j) mma(acc[i][j], fb[sb][j], fa[sa][i]);
     };
     for (int it = 0; it < steps; ++it) {
-      if constexpr (PAIRS) {   // 16 of the contraction: first parts at s = 0, their second ones at s = 2; the others at 1 and 3
+      if constexpr (PARTS) {   // a a', c a', a c', b a', a b', and b b' below
         read_a(1, 2);
-        then();
-        multiply(0, 0);
         read_b(1, 2);
         then();
-        multiply(1, 0);
+        multiply(0, 0);
         read_a(2, 1);
-        read_b(0, 1);
         then();
+        multiply(1, 0);
         multiply(0, 1);
-        read_a(1, 3);
+        then();
+        read_b(1, 1);
         then();
         multiply(2, 0);
-        read_b(1, 3);
-        then();
-        multiply(1, 0);
+        multiply(0, 1);
       } else {
 #pragma unroll
         for (int s = 0; s < kWideK / 16 - 1; ++s) {
@@ -669,7 +634,7 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
       buffer = buffer == (S::kStages - 1) * S::kStage ? 0 : buffer + S::kStage;
       if (it + 1 < steps) request(done);
       read(0, 0);   // (behind the last step: for nothing)
-      multiply(PAIRS ? 2 : 1, 1);
+      multiply(PARTS ? 2 : 1, 1);
     }
     asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");   // the loop may end right behind a product
     __builtin_amdgcn_sched_barrier(0);
@@ -702,7 +667,7 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
           float zt = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) zt = t[i] == 32 * j + acc_row(r, 0) ? z[j][r] : zt;
-          if (mine && t[i] / 32 == j) a.tl[m] = zt * unit;
+          if (mine && t[i] / 32 == j) a.tl[m] = zt;
         }
         float most = kLeast;
 #pragma unroll
@@ -710,15 +675,15 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
 #pragma unroll
           for (int r = 0; r < 16; r += 2) most = fmaxf(fmaxf(most, z[j][r]), z[j][r + 1]);   // fmaxf drops NaNs
         most = fmaxf(most, __shfl_xor(most, 32));
-        const float log2e = kLog2e * unit, shift = most * log2e;
+        const float shift = most * kLog2e;
         float sum[4] = {};
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum[r % 4] += fast_exp2(__builtin_fmaf(z[j][r], log2e, -shift));
+          for (int r = 0; r < 16; ++r) sum[r % 4] += fast_exp2(__builtin_fmaf(z[j][r], kLog2e, -shift));
         float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         s += __shfl_xor(s, 32);
-        if (g == 0 && m < M) a.parts[(int64_t)(n0 / BN * S::WN + wave % S::WN) * a.Rp + m] = vec<float, 2>{most * unit, s};
+        if (g == 0 && m < M) a.parts[(int64_t)(n0 / BN * S::WN + wave % S::WN) * a.Rp + m] = vec<float, 2>{most, s};
         __builtin_amdgcn_sched_barrier(0);
       }
       stored = inside;
@@ -741,10 +706,10 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
         __builtin_amdgcn_sched_barrier(0);
       }
       stored = inside && !a.add;
-    } else if (MODE == kWeightGrad && (PAIRS || a.splits > 1)) {   // (of pairs, the result itself where the contraction is whole)
+    } else if (MODE == kWeightGrad && (PARTS || a.splits > 1)) {   // (of parts, the result itself where the contraction is whole)
       float* out = a.out + (int64_t)range * a.M * a.N;
-      const bool result = PAIRS && a.splits == 1;
-      const int shift = result ? __builtin_amdgcn_readfirstlane(a.gain->shift) + shift_of(__builtin_amdgcn_readfirstlane(a.head->most[0])) : 0;
+      const bool result = PARTS && a.splits == 1;
+      const int shift = result ? __builtin_amdgcn_readfirstlane(a.gain->shift) : 0;
       const float gain = result ? a.gain->gain : 1.f;
 #pragma unroll
       for (int i = 0; i < S::FM; ++i) {
@@ -756,7 +721,7 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
           for (int q = 0; q < 4; ++q)
             if (m < M && n0 + wn + 32 * j + 8 * q + 4 * g < a.N) {
               vec<float, 4> v = pack4<float>(acc[i][j], q);
-              if constexpr (PAIRS) {
+              if constexpr (PARTS) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -shift) * gain;
               }
@@ -766,9 +731,8 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
       }
       stored = inside;
     } else {
-      // to whole rows through LDS, 32 rows of up to 64 columns at a time, each wave in a part of its own; pieces placed as in the operands
+      // to whole rows through LDS, 32 rows of 64 columns (parts: of 16) at a time, each wave in a place of its own; pieces placed as in the operands
       T* turn = reinterpret_cast<T*>(castle_vocab_lds + S::kStages * S::kStage + wave * 4096);
-      constexpr int FJ = PAIRS ? 1 : 2, RP = 8;   // RP: rows of a store, 64 numbers each
       const int shift = MODE == kWeightGrad ? __builtin_amdgcn_readfirstlane(a.gain->shift) : 0;
       const float gain = MODE == kWeightGrad ? a.gain->gain : 0.f;
       const int row_end = MODE == kGrad ? min((int)up(count, 64), (int)a.Rp) : M;
@@ -778,7 +742,7 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) z[j] = acc[i][j];
         if constexpr (MODE == kGrad) {
-          const float log2e = kLog2e * unit, shift = l[i] * kLog2e;
+          const float shift = l[i] * kLog2e;
           t[i] -= a.first + n0 + wn + 4 * g;
           if (!inside || __ballot(f[i] < 0.f) != 0) {
             const int end = m0 + wm + 32 * i + c < M ? a.N - n0 - wn - 4 * g : 0;
@@ -786,13 +750,13 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
 #pragma unroll
             for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) z[j][r] = 32 * j + acc_row(r, 0) < end ? f[i] * fast_exp2(__builtin_fmaf(z[j][r], log2e, -shift)) : 0.f;
+              for (int r = 0; r < 16; ++r) z[j][r] = 32 * j + acc_row(r, 0) < end ? f[i] * fast_exp2(__builtin_fmaf(z[j][r], kLog2e, -shift)) : 0.f;
           } else {   // a factor that is not negative goes to the exponent
             const float up = __builtin_amdgcn_logf(f[i]) - shift;
 #pragma unroll
             for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) z[j][r] = fast_exp2(__builtin_fmaf(z[j][r], log2e, up));
+              for (int r = 0; r < 16; ++r) z[j][r] = fast_exp2(__builtin_fmaf(z[j][r], kLog2e, up));
           }
 #pragma unroll
           for (int j = 0; j < S::FN; ++j) {
@@ -807,26 +771,32 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
             for (int r = 0; r < 16; ++r) z[j][r] = ldexpf(z[j][r], -shift) * gain;
         }
 #pragma unroll
-        for (int h = 0; h < S::FN / FJ; ++h) {
+        for (int h = 0; h < (PARTS ? 2 * S::FN : S::FN / 2); ++h) {
           auto put = [&](int p, vec<T, 4> v) __attribute__((always_inline)) { st4<T>(turn + c * 64 + 8 * (p ^ (c >> 1 & 7)) + 4 * g, v); };
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           __builtin_amdgcn_wave_barrier();
+          if constexpr (PARTS) {
 #pragma unroll
-          for (int j = 0; j < FJ; ++j)
+            for (int q = 0; q < 2; ++q) {
+              const Parts<4> parts = split_in_three<false>(pack4<float>(z[h / 2], 2 * (h % 2) + q));
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const vec<T, 4> first = pack4<T>(z[FJ * h + j], q);
-              put(4 * j + q, first);
-              if constexpr (PAIRS) put(4 + q, __builtin_convertvector(pack4<float>(z[h], q) - __builtin_convertvector(first, vec<float, 4>), vec<T, 4>));
+              for (int k = 0; k < 3; ++k) put(2 * k + q, parts.p[k]);
             }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) put(4 * j + q, pack4<T>(z[2 * h + j], q));
+          }
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           __builtin_amdgcn_wave_barrier();
+          constexpr int PIECES = PARTS ? 6 : 8;   // of a row
 #pragma unroll
-          for (int k = 0; k < 32 / RP; ++k) {
-            const int row = RP * k + lane / 8, piece = lane % 8, mm = m0 + wm + 32 * i + row, n = n0 + wn + 32 * FJ * h + 8 * (PAIRS ? piece % 4 : piece);
+          for (int k = 0; k < 32 * PIECES / 64; ++k) {
+            const int at = 64 * k + lane, row = at / PIECES, piece = at % PIECES, mm = m0 + wm + 32 * i + row, n = n0 + wn + (PARTS ? 16 * h : 64 * h + 8 * piece);
             const vt v = *reinterpret_cast<const vt*>(turn + row * 64 + 8 * (piece ^ (row >> 1 & 7)));
-            constexpr int B = kBlock<PAIRS>;
-            T* to = static_cast<T*>(a.c) + (MODE == kGrad ? mm / B * 64 * a.ldc + n / B * (B * 64) + mm % B * 64 + (PAIRS ? 8 * piece : n % B) : mm * a.ldc + n);
+            constexpr int B = kBlock<PARTS>, BR = kBlockRow<PARTS>;
+            T* to = static_cast<T*>(a.c) + (MODE == kGrad ? mm / B * BR * a.ldc + n / B * (B * BR) + mm % B * BR + (PARTS ? 8 * piece : n % B) : mm * a.ldc + n);
             if (mm < row_end && n < (MODE == kGrad ? (int)a.ldc : a.N)) *reinterpret_cast<vt*>(to) = v;
           }
         }
@@ -837,16 +807,16 @@ template <typename T, int MODE, int BM, int BN, bool PAIRS> __global__ __launch_
   }
 }
 
-template <typename T, int MODE, int BM, int BN, bool PAIRS> int launch_product_t(const ProductArgs& a, hipStream_t stream) {
-  typedef Shape<MODE, BM, BN, PAIRS> S;
+template <typename T, int MODE, int BM, int BN, bool PARTS> int launch_product_t(const ProductArgs& a, hipStream_t stream) {
+  typedef Shape<MODE, BM, BN, PARTS> S;
   static PerDeviceOnce once;
   bool& configured = once.flag();
   if (!configured) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&vocab_product_kernel<T, MODE, BM, BN, PAIRS>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&vocab_product_kernel<T, MODE, BM, BN, PARTS>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
     configured = true;
   }
   const int64_t items = up(a.M, BM) / BM * (up(a.N, BN) / BN) * a.splits;
-  hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN, PAIRS>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
+  hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN, PARTS>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -3;
 }
 // Rows and columns of a workgroup's tile.  64 rows for that few; else 128 where 256 leave CUs idle: by what the fullest CU takes (us), 1.4 a step and 5 an end of 256 x 256, 0.85 and
@@ -859,9 +829,9 @@ Tile tile_of(int R, int n, int steps, int splits = 1) {
   return cost({128, 256}, 0.85, 3) < cost({256, 256}, 1.4, 5) ? Tile{128, 256} : Tile{256, 256};
 }
 template <int MODE> int launch_product(const ProductArgs& a, Tile tile, int dtype, hipStream_t stream) {
-  auto of_type = [&](auto t, auto pairs) {
+  auto of_type = [&](auto t, auto parts) {
     using T = decltype(t);
-    constexpr bool P = decltype(pairs)::value;
+    constexpr bool P = decltype(parts)::value;
     if constexpr (MODE != kWeightGrad) {
       if (tile.rows == 64) {
         if constexpr (MODE == kRowGrad)
@@ -875,7 +845,7 @@ template <int MODE> int launch_product(const ProductArgs& a, Tile tile, int dtyp
     return launch_product_t<T, MODE, 256, 256, P>(a, stream);
   };
   switch (dtype) {
-    case 0: return of_type(fp16_t(), std::true_type());
+    case 0: return of_type(bf16_t(), std::true_type());
     case 1: return of_type(bf16_t(), std::false_type());
     case 2: return of_type(fp16_t(), std::false_type());
     default: return -1;
@@ -914,13 +884,14 @@ Split split_of(int64_t m, int64_t n, int64_t steps, std::initializer_list<Tile> 
   }
   return best;
 }
-// es: bytes of an element, also of a pair
+// bytes of an element of an operand of the products; es: of one of the tensors
+constexpr int operand_bytes(int es) { return es == 4 ? 6 : 2; }
 Plan plan(const VocabArgs& a, int es) {
   Plan p = {};
-  p.step = es == 4 ? kWideK / 2 : kWideK;
+  p.step = es == 4 ? kPart : kWideK;
   p.Rp = up(a.R, 64);
   p.Dp = (int)up(a.D, p.step);
-  const int64_t fit = std::max<int64_t>(256, kPieceBytes / (p.Rp * es) / 256 * 256), width = up(a.V, 64);
+  const int64_t fit = std::max<int64_t>(256, kPieceBytes / (p.Rp * operand_bytes(es)) / 256 * 256), width = up(a.V, 64);
   p.pieces = (int)((width + fit - 1) / fit);
   p.columns = (int)up((a.V + p.pieces - 1) / p.pieces, 256);
   p.pieces = (a.V + p.columns - 1) / p.columns;
@@ -944,14 +915,14 @@ struct Carve {
 };
 struct Fwd {
   int* block_counts;
-  char *xc, *wc;   // wc: fp32, the pairs of w
+  char *xc, *wc;   // wc: fp32, the parts of w
   int32_t *tc, *row_of;
   float *tl, *sums;
   vec<float, 2>* parts;
   Fwd(const VocabArgs& a, const Plan& p, int es, Carve& c) {
     block_counts = c.take<int>(up(a.R, kCountRows) / kCountRows);
-    xc = c.take<char>(p.Rp * p.Dp * es);
-    wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * 4 : 0);
+    xc = c.take<char>(p.Rp * p.Dp * operand_bytes(es));
+    wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * operand_bytes(es) : 0);
     tc = c.take<int32_t>(p.Rp);
     tl = c.take<float>(p.Rp);
     row_of = c.take<int32_t>(p.Rp);
@@ -967,12 +938,12 @@ struct Bwd {
   char* d;
   float *row_parts, *weight_parts;
   Bwd(const VocabArgs& a, const Plan& p, int es, bool need_x, bool need_w, Carve& c) {
-    xc = c.take<char>(p.Rp * p.Dp * es);
-    wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * 4 : 0);
+    xc = c.take<char>(p.Rp * p.Dp * operand_bytes(es));
+    wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * operand_bytes(es) : 0);
     tc = c.take<int32_t>(p.Rp);
     factor = c.take<float>(p.Rp);
     gain = c.take<Gain>(1);
-    d = c.take<char>(p.Rp * p.ldc * es);
+    d = c.take<char>(p.Rp * p.ldc * operand_bytes(es));
     row_parts = c.take<float>(need_x ? (int64_t)p.rows.ranges * a.R * a.D : 0);
     weight_parts = c.take<float>(need_w && p.weights.ranges > 1 ? p.weights.ranges * p.ldc * a.D : 0);
   }
@@ -996,11 +967,10 @@ template <bool FIRST> int launch_gather(const RowArgs& a, int dtype, hipStream_t
   });
 }
 
-// fp32: the rows of x that count, and w, as pairs
-int launch_split(const VocabArgs& a, const Plan& p, VocabHead* head, const int32_t* rank, void* xc, void* wc, bool first, hipStream_t stream) {
-  const SplitArgs x = {static_cast<const float*>(a.x), a.ld_x, a.R, a.D, p.Dp, rank, &head->count, &head->most[0], static_cast<fp16_t*>(xc)};
-  const SplitArgs w = {static_cast<const float*>(a.w), a.ld_w, a.V, a.D, p.Dp, nullptr, nullptr, &head->most[1], static_cast<fp16_t*>(wc)};
-  if (first) hipLaunchKernelGGL(most_kernel, dim3((unsigned)std::min<int64_t>(1024, up(a.V, kWaves) / kWaves)), dim3(kThreads), 0, stream, w);
+// fp32: the rows of x that count, and w, as parts
+int launch_split(const VocabArgs& a, const Plan& p, const int* count, const int32_t* rank, void* xc, void* wc, hipStream_t stream) {
+  const SplitArgs x = {static_cast<const float*>(a.x), a.ld_x, a.R, a.D, p.Dp, rank, count, static_cast<bf16_t*>(xc)};
+  const SplitArgs w = {static_cast<const float*>(a.w), a.ld_w, a.V, a.D, p.Dp, nullptr, nullptr, static_cast<bf16_t*>(wc)};
   hipLaunchKernelGGL(split_rows_kernel, dim3((unsigned)(up(p.Rp * (p.Dp / 8), kThreads) / kThreads)), dim3(kThreads), 0, stream, x);
   hipLaunchKernelGGL(split_rows_kernel, dim3((unsigned)(up((int64_t)a.V * (p.Dp / 8), kThreads) / kThreads)), dim3(kThreads), 0, stream, w);
   return launched();
@@ -1030,18 +1000,17 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   Carve cs = {static_cast<char*>(state)}, cw = {static_cast<char*>(workspace)};
   const State s(a.R, cs);
   const Fwd f(a, p, es, cw);
-  // up to 4096 rows the copying workgroups count for themselves, which is less than a launch (fp32 needs the launch for its first zeros)
-  const bool count = es == 4 || a.R > 4096;
+  const bool count = a.R > 4096;   // (up to there the copying workgroups count for themselves, which is less than a launch)
   const RowArgs rows = {a, count ? f.block_counts : nullptr, s.head, s.rank, f.xc, f.tc, f.tl, f.row_of, p.Dp, loss, nullptr, nullptr, nullptr};
   if (count) hipLaunchKernelGGL(count_rows_kernel, dim3((unsigned)(up(a.R, kCountRows) / kCountRows)), dim3(kThreads), 0, stream, rows);
   int rc = launch_gather<true>(rows, dtype, stream);
-  if (rc == 0 && es == 4) rc = launch_split(a, p, s.head, s.rank, f.xc, f.wc, true, stream);
+  if (rc == 0 && es == 4) rc = launch_split(a, p, &s.head->count, s.rank, f.xc, f.wc, stream);
   if (rc != 0) return rc;
   ProductArgs g = {};
   g.a = f.xc;
   g.b = es == 4 ? f.wc : a.w;
-  g.lda = es == 4 ? 2 * p.Dp : p.Dp;
-  g.ldb = es == 4 ? 2 * p.Dp : a.ld_w;
+  g.lda = es == 4 ? 3 * p.Dp : p.Dp;
+  g.ldb = es == 4 ? 3 * p.Dp : a.ld_w;
   g.M = a.R;
   g.N = a.V;
   g.K = a.D;
@@ -1051,7 +1020,6 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   g.tl = f.tl;
   g.Rp = p.Rp;
   g.tc = f.tc;
-  g.head = s.head;
   rc = launch_product<kStats>(g, p.logits, dtype, stream);
   if (rc != 0) return rc;
   const LossArgs l = {f.parts, s.head, f.row_of, f.tl, s.lse, f.sums, loss, p.P, a.reduction, p.Rp};
@@ -1070,7 +1038,7 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
   const Bwd b(a, p, es, dx != nullptr, dw != nullptr, cw);
   const RowArgs rows = {a, nullptr, s.head, s.rank, b.xc, b.tc, nullptr, nullptr, p.Dp, nullptr, dloss, b.factor, b.gain};
   int rc = launch_gather<false>(rows, dtype, stream);
-  if (rc == 0 && es == 4) rc = launch_split(a, p, s.head, s.rank, b.xc, b.wc, false, stream);
+  if (rc == 0 && es == 4) rc = launch_split(a, p, &s.head->count, s.rank, b.xc, b.wc, stream);
   if (rc == 0 && a.reduction == kEachLoss) {
     const FactorArgs f = {dloss, s.rank, b.tc, b.factor, b.gain, a.R};
     rc = by_tensor_type(dtype, [&](auto t) {
@@ -1084,7 +1052,7 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
       return launched();
     });
   };
-  const int64_t ld_x = es == 4 ? 2 * p.Dp : p.Dp, ld_w = es == 4 ? 2 * p.Dp : a.ld_w;   // numbers, as es is 2 bytes or two of them
+  const int64_t ld_x = es == 4 ? 3 * p.Dp : p.Dp, ld_w = es == 4 ? 3 * p.Dp : a.ld_w;   // numbers of 2 bytes
   for (int i = 0; i < p.pieces && rc == 0; ++i) {
     const int v0 = i * p.columns, n = std::min(p.columns, a.V - v0);
     ProductArgs g = {};
@@ -1105,7 +1073,6 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
     g.c = b.d;
     g.ldc = p.ldc;
     g.gain = b.gain;
-    g.head = s.head;
     rc = launch_product<kGrad>(g, p.logits, dtype, stream);
     if (rc == 0 && dx != nullptr) {
       ProductArgs x = g;
@@ -1134,12 +1101,11 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
       w.out = w.splits > 1 ? b.weight_parts : static_cast<float*>(w.c);
       rc = launch_product<kWeightGrad>(w, p.weights.tile, dtype, stream);
       if (rc == 0 && w.splits > 1)
-        rc = join({b.weight_parts, nullptr, b.gain, w.c, w.splits, a.D, n, &s.head->count, p.step, es == 4 ? &s.head->most[0] : nullptr});
+        rc = join({b.weight_parts, nullptr, b.gain, w.c, w.splits, a.D, n, &s.head->count, p.step});
     }
   }
   if (rc != 0 || dx == nullptr) return rc;
-  return join({b.row_parts, s.rank, b.gain, dx, ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.rows.ranges), a.D, a.R, nullptr, p.step,
-               es == 4 ? &s.head->most[1] : nullptr});
+  return join({b.row_parts, s.rank, b.gain, dx, ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.rows.ranges), a.D, a.R, nullptr, p.step});
 }
 
 }  // namespace castle

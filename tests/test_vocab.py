@@ -1,12 +1,13 @@
 """Cross entropy against a vocabulary without the logits (ops.linear_cross_entropy): refusals and shapes without a GPU, results against the definition in 64 bits on one.
 
 Tolerances, element by element, u = 2^-23 (twice the rounding of a 32-bit operation, since the order of the 16 products inside a matrix instruction is its own):
-  logits     products of 16-bit numbers are exact; D of them are added 16 at a time: ez = (D / 16 + 32) u (|x| . |w|).  fp32: an element goes as two parts that hold 2^-22 of it
-             (twice a rounding to 11 bits), three products for one and a fourth left out that is below 2^-22 of it: 3 2^-22 = 6 u of each product, and three times as many additions;
-             six times the bound above covers both.
+  logits     products of 16-bit numbers are exact; D of them are added 16 at a time: ez = (D / 16 + 32) u (|x| . |w|).  fp32: an element goes as three parts, exactly, six products for
+             one, six times as many additions; the three that are left out are below 2^-24 of the product together, which the 32 u cover.
   loss       twice the largest ez of the row (its log-sum-exp and its own logit), exp and log of 32 bits (16 u (1 + |log-sum-exp|)), and the rounding to the type
   d          a softmax value p is off by p (2 ez + 16 u (1 + |log-sum-exp|)); d = g (p - [target]) is rounded to the type, eps / 2 of it, or to the step 2^-25 below the
-             type's normal numbers, under a factor that brings the largest |g| to 2^14 at least (fp32: its second part, of fp16); the sums over blocks of 16 of it as above
+             type's normal numbers, under a factor that brings the largest |g| to 2^14 at least; fp32: no rounding, but values below 2^-125 of the largest |g| may be
+             taken for zero; the sums over blocks of 16 of it as above
+             (u of what was added, or of 2^-126, below which fp32 has steps of 2^-149)
   gradients  that times |w| (or |x|), summed, and the last rounding to the type, of a value or of the smallest normal number"""
 import ctypes
 
@@ -41,13 +42,12 @@ def reference(x, w, target, reduction, dloss, ignore, dtype):
     p[r, t] -= 1
     d = g[:, None] * p
     most = g.abs().max().item() if len(t) else 0.0
-    # (fp32: the two parts of d are among its sums' bound below)
-    off_d = g.abs()[:, None] * off_p + (0 if dtype is torch.float32 else half) * d.abs() + (2.0 ** -25 / 2.0 ** 14 * most if dtype is not torch.bfloat16 else 0)
+    off_d = g.abs()[:, None] * off_p + (0 if dtype is torch.float32 else half) * d.abs() + {torch.float16: 2.0 ** -25 / 2.0 ** 14, torch.float32: 2.0 ** -125}.get(dtype, 0) * most
     del z, ez, p, off_p
     w_a, x_a, d_a = w.abs(), xk.abs(), d.abs()
     V, six = w.shape[0], 6 if dtype is torch.float32 else 1
-    dx_k, off_dx = d @ w, off_d @ w_a + (V / 16 + 32) * U * six * (d_a @ w_a)
-    dw, off_dw = d.T @ xk, off_d.T @ x_a + (n / 16 + 32) * U * six * (d_a.T @ x_a)
+    dx_k, off_dx = d @ w, off_d @ w_a + (V / 16 + 32) * U * six * (d_a @ w_a + 2.0 ** -126)
+    dw, off_dw = d.T @ xk, off_d.T @ x_a + (n / 16 + 32) * U * six * (d_a.T @ x_a + 2.0 ** -126)
     dx, bound_dx = torch.zeros_like(x), torch.zeros_like(x)
     dx[keep], bound_dx[keep] = dx_k, off_dx
     if reduction == "none":
@@ -241,6 +241,35 @@ def test_small_and_large_gradients_of_the_loss(dtype):
         check(x, w, target, "mean", dloss=torch.tensor(scale, dtype=dtype, device=DEV), tell=scale)
     zero = check(x, w, target, dloss=torch.tensor(0.0, dtype=dtype, device=DEV))[1]
     assert not any(g.any() for g in zero)
+
+
+@gpu
+def test_fp32_keeps_what_is_far_below_the_largest():
+    """Rows, classes and columns of very different sizes, rows whose losses count very differently, and classes that are as good as impossible: each gradient is as exact as its own sums."""
+    g = torch.Generator().manual_seed(17)
+
+    def power(low, high, n):
+        return 2.0 ** torch.randint(low, high + 1, (n,), generator=g).float()
+
+    R, V, D = 150, 700, 96
+    x, w, target = (t.cpu() for t in inputs(R, V, D, torch.float32, 17, spread=1.0))
+    channels = power(-30, 30, D)
+    for rows, classes in ((power(-40, 2, R), torch.ones(V)), (torch.ones(R), power(-40, 2, V)), (power(3, 5, R), power(-20, 1, V))):
+        xs, ws = (x * rows[:, None] * channels).to(DEV), (w * classes[:, None] / channels).to(DEV)
+        check(xs, ws, target.to(DEV))
+        check(xs, ws, target.to(DEV), "none", dloss=power(-60, 20, R).to(DEV))
+    # a class of softmax values below 2^-60 in every row: its gradient is not zero, and right
+    ws = w.clone()
+    ws[5] = 0
+    xs = x + 64 * torch.eye(D)[0]
+    ws[:, 0] = 1
+    ws[5, 0] = 0
+    _, (_, dw) = check(xs.to(DEV), ws.to(DEV), (target.clamp(min=6)).to(DEV))
+    assert 0 < dw[5].abs().max() < 2.0 ** -60
+    # the largest numbers of the type as elements: logits beyond it, and far below
+    xs, ws = x.clone(), w.clone()
+    xs[:, 0], ws[:, 0] = 2.0 ** -130, torch.finfo(torch.float32).max * (1 - 2 * (torch.arange(V) % 2))
+    check(xs.to(DEV), ws.to(DEV), target.to(DEV), tell="largest")
 
 
 @gpu
