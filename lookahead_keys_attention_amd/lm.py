@@ -37,10 +37,11 @@ READ_ONCE_BYTES = 320_000_000
 SAMPLER_MAX_VOCABULARY = 20480
 
 
-# From this vocabulary on the loss of a native model is formed without its logits (ops.linear_cross_entropy).  Training in 16 bits, where that takes four products
-# and logits in memory three, forms the logits of more than 2048 rows wider than 512 as long as they take no more than LOGITS_MAX_BYTES.  Measured, us with the logits / without them,
-# loss and gradients, then the loss alone: bf16 2048 x 512 over 16384 233 / 218 and 71 / 57, over 8192 151 / 156 and 43 / 39; 16384 x 512 over 32000 2282 / 2286 and 904 / 596;
-# 2048 x 1024 over 32000 625 / 561, 8192 x 1024 1704 / 2056, and 575 / 518; 8192 x 2048 over 131072 11780 / 15095 and 3698 / 3788; fp32 2048 x 512 over 32000 1455 / 879, 511 / 235.
+# From this vocabulary on the loss of a native model is formed without its logits (ops.linear_cross_entropy), which takes four products and logits in memory three: in training in
+# 16 bits, more than 2048 rows wider than 512 keep the logits as long as these take no more than LOGITS_MAX_BYTES, in 32 bits those below 2^24 logits.  Measured, us with the
+# logits / without them, loss and gradients, then the loss alone: bf16 2048 x 512 over 8192 151 / 156 and 43 / 39, over 16384 233 / 218 and 71 / 57; 16384 x 512 over 32000
+# 2282 / 2286 and 904 / 596; 2048 x 1024 over 32000 625 / 561, 8192 x 1024 1704 / 2056 and 575 / 518; 8192 x 2048 over 131072 11780 / 15095 and 3698 / 3788; fp32 256 x 512 over
+# 16384 179 / 241, over 65536 597 / 579; 2048 x 512 over 32000 1469 / 1468 and 519 / 365; 16384 x 512 over 32000 11494 / 11083 and 3856 / 2544.
 LINEAR_LOSS_MIN_VOCABULARY = 16384
 LOGITS_MAX_BYTES = 4 << 30
 
@@ -50,8 +51,11 @@ def linear_loss_is_ahead(rows: int, weight: torch.Tensor) -> bool:
     V, D = weight.shape
     if not (LINEAR_LOSS_MIN_VOCABULARY <= V <= 1 << 22 and D % 8 == 0 and D <= 1 << 16 and 0 < rows <= 1 << 24):
         return False
-    kept = weight.element_size() * rows * V
-    return weight.element_size() == 4 or not torch.is_grad_enabled() or rows <= 2048 or D <= 512 or kept > LOGITS_MAX_BYTES
+    if not torch.is_grad_enabled():
+        return True
+    if weight.element_size() == 4:
+        return rows * V >= 1 << 24
+    return rows <= 2048 or D <= 512 or weight.element_size() * rows * V > LOGITS_MAX_BYTES
 
 
 # -- sampling helpers (train_triton.py:56-71) ------------------------------------------------

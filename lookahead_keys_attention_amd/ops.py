@@ -356,7 +356,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     Sums and the loss are formed in 32 bits from unrounded logits; the result has the type of x.  reduction: "mean" over the rows that count,
     "sum", or "none" for the loss of each row, shaped like `target`.  Rows of class `ignore_index` cost nothing and have no part in anything, whatever they
     hold.  A class outside 0 .. V - 1 makes the loss and the gradients NaN.  Differentiable in x and weight, once; D is a multiple of 8.
-    float32: products of two parts of each element, which hold 22 bits of it if it lies above 2^-18 of the largest of its tensor, and fewer below."""
+    float32: by three bf16 parts of each element, which hold all of its 24 bits down to 2^-110; an infinite element makes what it enters NaN."""
     if N._host is None:
         N.host()
     if reduction not in LOSS_REDUCTIONS:

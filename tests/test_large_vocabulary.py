@@ -53,9 +53,10 @@ def test_where_the_loss_is_taken_without_logits():
     assert not any(ahead(*bad) for bad in ((2048, (1 << 22) + 1, 512), (2048, 16384, 516), (2048, 16384, (1 << 16) + 8), (0, 16384, 512), ((1 << 24) + 1, 16384, 512)))
     # in 16 bits with gradients, wide rows go by the logits' memory
     assert ahead(2048, 32000, 520) and not ahead(2049, 32000, 520) and ahead(2049, 32000, 520, torch.float32)
+    assert not ahead(1023, 16384, 64, torch.float32) and ahead(1024, 16384, 64, torch.float32)
     assert not ahead(1 << 14, 1 << 17, 1024) and ahead((1 << 14) + 1, 1 << 17, 1024)
     with torch.no_grad():
-        assert ahead(2049, 32000, 520)
+        assert ahead(2049, 32000, 520) and ahead(1, 16384, 8, torch.float32)
 
 
 # ---- on a GPU -------------------------------------------------------------------------------------------------------
@@ -69,13 +70,14 @@ def train(model, x):
 @gpu
 @pytest.mark.parametrize("tie", [False, True])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_training_step_equals_the_dense_model(tie, dtype):
-    """Loss and every gradient; with a hook the model runs module by module and forms logits, without one it does not.  bf16: the rule of the package, 2e-2 of the norm."""
+def test_training_step_equals_the_dense_model(tie, dtype, monkeypatch):
+    """Loss and every gradient; with a hook the model runs module by module and forms logits, without one it does not, whatever the rule says.  bf16: the rule of the package, 2e-2 of the norm."""
     native = make(True, tie_embedding=tie, embedding_scale=8.0).to(dtype).to(DEV)
     dense = make(False, tie_embedding=tie, embedding_scale=8.0).double().to(DEV)
     dense.load_state_dict({k: v.double() for k, v in native.state_dict().items()})
     x = ids().to(DEV)
     assert native._plain(x)
+    monkeypatch.setattr(LM, "linear_loss_is_ahead", lambda rows, weight: True)
     want = train(dense, x)
     tol = 1e-4 if dtype is torch.float32 else 2e-2
     for hooked in (False, True):
