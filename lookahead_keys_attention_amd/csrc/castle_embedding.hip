@@ -4,7 +4,7 @@
 //
 // Both are bound by HBM: the forward pass reads a row and writes one, the gradient reads dy and writes the whole table once.  The gradient needs the rows of
 // each token together, in an order of their own (atomic additions would leave the order, and with it the last bits, to chance): (token, place) pairs are sorted, stable, by
-// digits of up to ten bits, a counting and a placing launch for each.  Pieces of 64 sorted places that hold one token alone are summed first, so that a token that takes a tenth of a text
+// digits of up to ten bits, a counting and a placing launch for each.  Where each token's places begin and end is noted, and pieces of 64 sorted places that hold one token alone are summed first, so that a token that takes a tenth of a text
 // does not keep one workgroup busy when the rest is done; then every row of the table is summed and written once, zeros where there is no token.
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
@@ -53,6 +53,7 @@ template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) voi
 
 // ---- sorting -------------------------------------------------------------------------------------------------------
 // Every wave has a range of its own, in order; workgroup g has those of four waves.
+struct Range { uint32_t first, end; };   // sorted places of a token
 struct SortArgs {
   TokenRows tokens;
   int V, padding;
@@ -61,7 +62,15 @@ struct SortArgs {
   const uint32_t *keys_in, *places_in;   // nullptr: the tokens themselves
   uint32_t *keys, *places;
   uint32_t* counts;                      // [workgroup][digit]
+  // workgroups behind the `groups` that sort clear ranges of sorted places in passing, where there are any
+  Range* ranges;
+  int groups;
 };
+constexpr int kClear = 4096;   // ranges of a workgroup that clears
+__device__ __forceinline__ void clear_ranges(const SortArgs& a, int threads) {
+  const int64_t first = (int64_t)(blockIdx.x - a.groups) * kClear;
+  for (int64_t v = first + threadIdx.x; v < min((int64_t)a.V, first + kClear); v += threads) a.ranges[v] = {0, 0};
+}
 __device__ __forceinline__ uint32_t key_of(const SortArgs& a, int64_t i) {
   if (a.keys_in != nullptr) return a.keys_in[i];
   const int64_t t = token_of(a.tokens, i);
@@ -74,6 +83,7 @@ __device__ __forceinline__ void wave_counts(const SortArgs& a, uint32_t* mine, i
 }
 __global__ __launch_bounds__(kThreads) void sort_count_kernel(SortArgs a) {
   const int digits = 1 << a.bits;
+  if ((int)blockIdx.x >= a.groups) return clear_ranges(a, kThreads);
   for (int d = threadIdx.x; d < digits; d += kThreads) castle_digits[d] = 0;
   __syncthreads();
   const int64_t first = ((int64_t)blockIdx.x * kWaves + wave_id()) * a.wave_tokens;
@@ -99,7 +109,7 @@ __global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
     for (int p = 0; p < kMaxPer; ++p) {
       if (p >= per) break;
 #pragma unroll 16
-      for (int g = 0; g < (int)gridDim.x; ++g) {
+      for (int g = 0; g < a.groups; ++g) {
         const uint32_t n = a.counts[(int64_t)g * digits + d0 + p];
         all[p] += n;
         before[p] += g < (int)blockIdx.x ? n : 0;
@@ -159,10 +169,11 @@ __global__ __launch_bounds__(kThreads) void sort_place_kernel(SortArgs a) {
 
 // Up to 8192 tokens and 2^18 keys: all in one workgroup of sixteen waves, a pair in one word, eight of them in the registers of a thread, from there to their places in LDS and
 // back.  Lanes of equal digits are found once a pass: a pair's rank among the digits of its wave is kept until the places are known (32000 rows of 512 bf16, the
-// whole gradient: 8192 tokens 42 us, 8256 by four launches 49; the 16384 of which four launches sort in 25 us take a workgroup 34).
+// whole gradient: 8192 tokens 38 us, 8256 by four launches 45; the 16384 of which four launches sort in 25 us take a workgroup 34).
 constexpr int kSortRounds = 8, kSortThreads = 1024, kSortTokens = kSortRounds * kSortThreads, kPlaceBits = 13;
 template <int BITS> __global__ __launch_bounds__(kSortThreads) void sort_all_kernel(SortArgs a, int passes) {
   constexpr int W = kSortThreads / 64, DIGITS = 1 << BITS;
+  if ((int)blockIdx.x >= a.groups) return clear_ranges(a, kSortThreads);
   const int wave = wave_id(), lane = lane_id(), n = (int)a.tokens.rows;
   uint32_t* const s_pairs = castle_digits;                  // [kSortTokens]
   uint32_t* const s_digits = s_pairs + kSortTokens;         // [wave][digit]
@@ -248,6 +259,7 @@ template <int BITS> __global__ __launch_bounds__(kSortThreads) void sort_all_ker
 // ---- sums ----------------------------------------------------------------------------------------------------------
 struct SumArgs {
   const uint32_t *keys, *places;
+  Range* ranges;   // [V], zeros
   int64_t rows;
   const void* dy;
   void* dw;
@@ -285,42 +297,41 @@ template <int N, typename F, typename G> __device__ __forceinline__ void over_wa
 }
 template <typename T, int N> __global__ __launch_bounds__(kThreads) void run_sum_kernel(SumArgs a) {
   __shared__ float s_acc[(kWaves - 1) * N * 64];
-  const int64_t first = (int64_t)blockIdx.x * kRun;
+  const int64_t first = (int64_t)blockIdx.x * kRun, i = first + threadIdx.x;
+  if (threadIdx.x < kRun && i < a.rows) {   // where a token ends and the next one begins
+    const uint32_t k = a.keys[i], before = i > 0 ? a.keys[i - 1] : k + 1;
+    if (k != before) {
+      if (k < (uint32_t)a.V) a.ranges[k].first = (uint32_t)i;
+      if (i > 0) a.ranges[before].end = (uint32_t)i;   // (keys behind the vocabulary are the last ones)
+    }
+    if (i == a.rows - 1 && k < (uint32_t)a.V) a.ranges[k].end = (uint32_t)a.rows;
+  }
+  if (first + kRun > a.rows) return;
   const uint32_t key = a.keys[first];
   if (key >= (uint32_t)a.V || a.keys[first + kRun - 1] != key) return;
   over_waves<N>(s_acc, a.D / N, [&](int i) { return sum_places<T, N>(a, first + wave_id(), first + kRun, kWaves, i); },
                 [&](int i, vec<float, N> v) { *reinterpret_cast<vec<float, N>*>(a.parts + (int64_t)blockIdx.x * a.D + i * N) = v; });
 }
 
-// First sorted place whose key is not below `key` (64 lanes that look at 64 places at a time for it make three trips to memory instead of
-// 14, but over 14 times the lines: 16384 tokens, 32000 rows of 512 bf16, 22 -> 37 us).
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
-  int64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (keys[mid] < key) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
 constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that one wave, or part of one, sums by itself
 // LPR: lanes to a row of few tokens
 template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) void table_grad_kernel(SumArgs a) {
-  __shared__ int64_t s_bound[2 * kMaxRowsPerGroup];   // first place of a row and of the next one
+  __shared__ Range s_range[kMaxRowsPerGroup];
   __shared__ float s_acc[(kWaves - 1) * N * 64];
   // Rows gridDim.x apart: the frequent tokens of a vocabulary stand together (a workgroup to 31 rows in a row: 162 us for 16384 tokens of 512 bf16 over 32000, the one of
   // the first tokens alone with all of it).
   const int G = gridDim.x, rows = ((int)a.V - (int)blockIdx.x + G - 1) / G, wave = wave_id(), lane = lane_id(), pieces = a.D / N;
-  if ((int)threadIdx.x < 2 * rows) s_bound[threadIdx.x] = lower_bound(a.keys, a.rows, (uint32_t)(blockIdx.x + threadIdx.x / 2 * G + threadIdx.x % 2));
+  // (Bounds by a search of each workgroup among the keys: 14 trips to memory for 16384 tokens, 21 us instead of 16.)
+  if ((int)threadIdx.x < rows) s_range[threadIdx.x] = a.ranges[blockIdx.x + threadIdx.x * G];
   __syncthreads();
   auto write = [&](int v, int i, vec<float, N> acc) { store_n<T, N>(static_cast<T*>(a.dw) + (int64_t)v * a.D + i * N, acc * a.scale); };
   for (int k = threadIdx.x / LPR; k < rows; k += kThreads / LPR) {
-    const int64_t s = s_bound[2 * k], e = s_bound[2 * k + 1];
+    const int64_t s = s_range[k].first, e = s_range[k].end;
     if (e - s > kFew) continue;
     for (int i = threadIdx.x % LPR; i < pieces; i += LPR) write(blockIdx.x + k * G, i, sum_places<T, N>(a, s, e, 1, i));
   }
   for (int k = 0; k < rows; ++k) {   // by all waves: places in front of the first whole piece, whole pieces, places behind
-    const int64_t s = s_bound[2 * k], e = s_bound[2 * k + 1];
+    const int64_t s = s_range[k].first, e = s_range[k].end;
     if (e - s <= kFew) continue;
     const int64_t c0 = (s + kRun - 1) / kRun, c1 = e / kRun;
     over_waves<N>(s_acc, pieces, [&](int i) {
@@ -387,10 +398,12 @@ SortedGradPlan sorted_grad_plan(int64_t rows, int V, int D) {
   p.keys = bytes(4 * rows);
   p.places = bytes(4 * rows);
   p.parts = bytes(rows / kRun * D * 4);
-  p.total = p.counts + 2 * (p.keys + p.places) + p.parts;
+  p.ranges = bytes((int64_t)V * sizeof(Range));
+  p.total = p.counts + 2 * (p.keys + p.places) + p.parts + p.ranges;
   return p;
 }
 
+static int clearing_groups(int V) { return (int)(((int64_t)V + kClear - 1) / kClear); }
 template <int BITS> static int launch_sort_all(const SortArgs& a, int passes, hipStream_t stream) {
   static PerDeviceOnce once;
   bool& configured = once.flag();
@@ -399,7 +412,7 @@ template <int BITS> static int launch_sort_all(const SortArgs& a, int passes, hi
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&sort_all_kernel<BITS>), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes) != hipSuccess) return -3;
     configured = true;
   }
-  hipLaunchKernelGGL((sort_all_kernel<BITS>), dim3(1), dim3(kSortThreads), kBytes, stream, a, passes);
+  hipLaunchKernelGGL((sort_all_kernel<BITS>), dim3(1 + clearing_groups(a.V)), dim3(kSortThreads), kBytes, stream, a, passes);
   return launched();
 }
 int launch_sorted_grad(const SortedGradArgs& g, int dtype, hipStream_t stream) {
@@ -413,24 +426,25 @@ int launch_sorted_grad(const SortedGradArgs& g, int dtype, hipStream_t stream) {
     places[i] = reinterpret_cast<uint32_t*>(take(p.places));
   }
   float* const parts = reinterpret_cast<float*>(take(p.parts));
+  Range* const ranges = reinterpret_cast<Range*>(take(p.ranges));
   if (p.together) {
     const int last = (p.passes - 1) % 2;
-    const SortArgs a = {g.tokens, g.V, g.padding, 0, p.bits, 0, nullptr, nullptr, keys[last], places[last], nullptr};
+    const SortArgs a = {g.tokens, g.V, g.padding, 0, p.bits, 0, nullptr, nullptr, keys[last], places[last], nullptr, ranges, 1};
     const int rc = p.bits == 8 ? launch_sort_all<8>(a, p.passes, stream) : launch_sort_all<9>(a, p.passes, stream);
     if (rc != 0) return rc;
   }
   for (int pass = 0; pass < p.passes && !p.together; ++pass) {
     const int to = pass % 2;
     const SortArgs a = {g.tokens, g.V, g.padding, pass * p.bits, p.bits, p.wave_tokens, pass > 0 ? keys[1 - to] : nullptr, pass > 0 ? places[1 - to] : nullptr,
-                        keys[to], places[to], counts};
-    hipLaunchKernelGGL(sort_count_kernel, dim3(p.groups), dim3(kThreads), 4 << p.bits, stream, a);
+                        keys[to], places[to], counts, ranges, p.groups};
+    hipLaunchKernelGGL(sort_count_kernel, dim3(p.groups + (pass == 0 ? clearing_groups(g.V) : 0)), dim3(kThreads), 4 << p.bits, stream, a);
     hipLaunchKernelGGL(sort_place_kernel, dim3(p.groups), dim3(kThreads), kWaves * 4 << p.bits, stream, a);
   }
   const int sorted = (p.passes - 1) % 2;
-  const SumArgs s = {keys[sorted], places[sorted], g.tokens.rows, g.dy, g.dw, parts, g.V, g.D, p.rows_per_group, g.scale};
+  const SumArgs s = {keys[sorted], places[sorted], ranges, g.tokens.rows, g.dy, g.dw, parts, g.V, g.D, p.rows_per_group, g.scale};
   return by_pieces(dtype, whole_pieces(g.D, g.D, dtype, {g.dy, g.dw}), [&](auto t, auto n) {
     using T = decltype(t);
-    if (s.rows >= kRun) hipLaunchKernelGGL((run_sum_kernel<T, n.value>), dim3((unsigned)(s.rows / kRun)), dim3(kThreads), 0, stream, s);
+    hipLaunchKernelGGL((run_sum_kernel<T, n.value>), dim3((unsigned)((s.rows + kRun - 1) / kRun)), dim3(kThreads), 0, stream, s);
     const dim3 grid((unsigned)((g.V + p.rows_per_group - 1) / p.rows_per_group));
     const int pieces = g.D / n.value;
     if (pieces <= 16) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 16>), grid, dim3(kThreads), 0, stream, s);

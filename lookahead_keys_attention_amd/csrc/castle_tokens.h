@@ -37,7 +37,7 @@ struct SortedGradPlan {
   int groups;              // workgroups of a sorting pass
   int64_t wave_tokens;     // tokens of a wave of them
   int rows_per_group;      // vocabulary rows of a workgroup of the sums
-  int64_t counts, keys, places, parts, total;   // bytes
+  int64_t counts, keys, places, parts, ranges, total;   // bytes
 };
 struct SortedGradArgs {
   TokenRows tokens;
