@@ -416,7 +416,8 @@ int castle_embedding_grad(const void* dy, const int64_t* index, int64_t index_n,
  *
  * _bwd: dx (rows x width) and dweight (vocabulary x width), contiguous, either may be NULL; dloss is one element, or `rows` of them.  All in a fixed order.  The logits are formed
  * again, as many columns of the vocabulary at a time as a workspace of about 1 GB holds; 16-bit types: what is multiplied with w and x is rounded to the type, under a power of two that
- * keeps it among its normal numbers.  gradients of _workspace_bytes: 0 for the forward pass, else the sum of 1 (dx) and 2 (dweight). */
+ * keeps it among its normal numbers; fp32: products by three bf16 parts of each element, all of whose 24 bits count down to 2^-110, an infinite one makes what it enters NaN,
+ * and the parts of x and w lie in the workspace, 6 bytes an element.  gradients of _workspace_bytes: 0 for the forward pass, else the sum of 1 (dx) and 2 (dweight). */
 #define CASTLE_LOSS_MEAN 0
 #define CASTLE_LOSS_SUM 1
 #define CASTLE_LOSS_EACH 2
@@ -430,9 +431,9 @@ int castle_linear_cross_entropy_bwd(const void* x, int64_t ld_x, const void* w, 
                                     int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* y[r] = scale * table[token r] in the type `dtype`, rounded once: rows of `width` elements, `ld` apart in the table, contiguous in y; the token of row r is
- * index[(r / index_n) * index_ld + r % index_n].  A token outside 0 .. vocabulary - 1 gives a row of NaNs.  Any width and vocabulary; whole 16-byte pieces are faster.
+ * index[(r / index_n) * index_ld + r % index_n].  A token outside 0 .. vocabulary - 1 gives a row of NaNs.  Any width, vocabulary and alignment.
  *
- * Its gradient for vocabularies of any size: dtable[v] = scale * the sum of the dy rows whose token is v, in the order of the rows (the same sum every time), rounded once;
+ * Its gradient for vocabularies of any size: dtable[v] = scale * the sum of the dy rows whose token is v, in a fixed order, rounded once;
  * zeros where there is none.  Rows whose token is `padding` (-1: none) or outside of the vocabulary have no part in it. */
 int castle_embedding(const void* table, int64_t ld, int vocabulary, int width, const int64_t* index, int64_t index_n, int64_t index_ld, int64_t rows, float scale,
                      void* y, int dtype, void* stream);

@@ -4,8 +4,11 @@
 //
 // Both are bound by HBM: the forward pass reads a row and writes one, the gradient reads dy and writes the whole table once.  The gradient needs the rows of
 // each token together, in an order of their own (atomic additions would leave the order, and with it the last bits, to chance): (token, place) pairs are sorted, stable, by
-// digits of up to ten bits, a counting and a placing launch for each.  Where each token's places begin and end is noted, and pieces of 64 sorted places that hold one token alone are summed first, so that a token that takes a tenth of a text
-// does not keep one workgroup busy when the rest is done; then every row of the table is summed and written once, zeros where there is no token.
+// digits of up to ten bits, a counting and a placing launch for each.  Where each token's places begin and end is noted, and pieces of 64 sorted places that hold one
+// token alone are summed first, so that a token that takes a tenth of a text does not keep one workgroup busy when the rest is done; then every row of the
+// table is summed and written once, zeros where there is no token.
+// Measured, bf16: 65536 tokens over 131072 rows of 2048, forward 86 us (5.5 TB/s), gradient 243 (3.3 TB/s of what it has to move, 33 of it the sort); 16384 over 32000 of 512, 7 and
+// 44 us, of which 24 are the four launches of the sort, each little more than its start and two trips to memory.
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
 #include "castle_tokens.h"
@@ -23,11 +26,16 @@ __device__ __forceinline__ int64_t token_of(const TokenRows& t, int64_t r) {
   return t.index[q * t.index_ld + ((uint32_t)r - q * (uint32_t)t.n)];
 }
 
-// N elements at a time: a 16-byte piece, or one where rows are no whole pieces
+// N elements at a time: 16 bytes, wherever they begin, or one element where a row has fewer.  Piece i of a row: the last one ends with the row, and reads and writes what the
+// one before it does as well (single elements where rows are no whole pieces: 5569 tokens of 828 bf16 over 6556, forward and gradient, 121 us, so 58).
+template <int N> __device__ __forceinline__ int column(int i, int D) { return min(i * N, D - N); }
+template <int N> __device__ __forceinline__ int pieces_of(int D) { return (D + N - 1) / N; }
+template <typename T, int N> struct Anywhere { typedef vec<T, N> type __attribute__((aligned(sizeof(T)))); };
 template <typename T, int N> __device__ __forceinline__ vec<float, N> load_n(const T* p) {
-  return __builtin_convertvector(*reinterpret_cast<const vec<T, N>*>(p), vec<float, N>);
+  const vec<T, N> v = *reinterpret_cast<const typename Anywhere<T, N>::type*>(p);
+  return __builtin_convertvector(v, vec<float, N>);
 }
-template <typename T, int N> __device__ __forceinline__ void store_n(T* p, vec<float, N> v) { *reinterpret_cast<vec<T, N>*>(p) = __builtin_convertvector(v, vec<T, N>); }
+template <typename T, int N> __device__ __forceinline__ void store_n(T* p, vec<float, N> v) { *reinterpret_cast<typename Anywhere<T, N>::type*>(p) = __builtin_convertvector(v, vec<T, N>); }
 template <int N> __device__ __forceinline__ vec<float, N> fill_n(float x) {
   vec<float, N> v;
 #pragma unroll
@@ -45,9 +53,10 @@ template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) voi
   const T* row = static_cast<const T*>(a.table) + (there ? t : 0) * a.ld;
   T* y = static_cast<T*>(a.y) + r * a.D;
 #pragma unroll 4
-  for (int i = threadIdx.x % LPR; i < a.D / N; i += LPR) {
-    const vec<float, N> v = load_n<T, N>(row + i * N) * a.scale;
-    store_n<T, N>(y + i * N, there ? v : fill_n<N>(NAN));
+  for (int i = threadIdx.x % LPR; i < pieces_of<N>(a.D); i += LPR) {
+    const int c = column<N>(i, a.D);
+    const vec<float, N> v = load_n<T, N>(row + c) * a.scale;
+    store_n<T, N>(y + c, there ? v : fill_n<N>(NAN));
   }
 }
 
@@ -267,20 +276,20 @@ struct SumArgs {
   int V, D, rows_per_group;
   float scale;
 };
-// dy rows of the sorted places first, first + step, ...
-template <typename T, int N> __device__ __forceinline__ vec<float, N> sum_places(const SumArgs& a, int64_t first, int64_t last, int step, int i) {
+// N columns from c of the dy rows of the sorted places first, first + step, ...
+template <typename T, int N> __device__ __forceinline__ vec<float, N> sum_places(const SumArgs& a, int64_t first, int64_t last, int step, int c) {
   vec<float, N> acc = fill_n<N>(0.f);
 #pragma unroll 8
-  for (int64_t k = first; k < last; k += step) acc += load_n<T, N>(static_cast<const T*>(a.dy) + (int64_t)a.places[k] * a.D + i * N);
+  for (int64_t k = first; k < last; k += step) acc += load_n<T, N>(static_cast<const T*>(a.dy) + (int64_t)a.places[k] * a.D + c);
   return acc;
 }
-// f(wave's sum of column piece i) added over the waves, in their order, handed to `out` in wave 0
-template <int N, typename F, typename G> __device__ __forceinline__ void over_waves(float* s_acc, int pieces, F&& f, G&& out) {
-  const int wave = wave_id(), lane = lane_id();
+// f(first column of a piece), a wave's sum of it, added over the waves, in their order, handed to `out` in wave 0
+template <int N, typename F, typename G> __device__ __forceinline__ void over_waves(float* s_acc, int D, F&& f, G&& out) {
+  const int wave = wave_id(), lane = lane_id(), pieces = pieces_of<N>(D);
   for (int p0 = 0; p0 < pieces; p0 += 64) {
-    const int i = p0 + lane;
+    const int i = p0 + lane, c = column<N>(i, D);
     vec<float, N> acc = fill_n<N>(0.f);
-    if (i < pieces) acc = f(i);
+    if (i < pieces) acc = f(c);
     if (wave > 0)
 #pragma unroll
       for (int e = 0; e < N; ++e) s_acc[((wave - 1) * N + e) * 64 + lane] = acc[e];
@@ -290,7 +299,7 @@ template <int N, typename F, typename G> __device__ __forceinline__ void over_wa
       for (int w = 0; w < kWaves - 1; ++w)
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] += s_acc[(w * N + e) * 64 + lane];
-      out(i, acc);
+      out(c, acc);
     }
     __syncthreads();
   }
@@ -309,8 +318,8 @@ template <typename T, int N> __global__ __launch_bounds__(kThreads) void run_sum
   if (first + kRun > a.rows) return;
   const uint32_t key = a.keys[first];
   if (key >= (uint32_t)a.V || a.keys[first + kRun - 1] != key) return;
-  over_waves<N>(s_acc, a.D / N, [&](int i) { return sum_places<T, N>(a, first + wave_id(), first + kRun, kWaves, i); },
-                [&](int i, vec<float, N> v) { *reinterpret_cast<vec<float, N>*>(a.parts + (int64_t)blockIdx.x * a.D + i * N) = v; });
+  over_waves<N>(s_acc, a.D, [&](int c) { return sum_places<T, N>(a, first + wave_id(), first + kRun, kWaves, c); },
+                [&](int c, vec<float, N> v) { store_n<float, N>(a.parts + (int64_t)blockIdx.x * a.D + c, v); });
 }
 
 constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that one wave, or part of one, sums by itself
@@ -320,57 +329,55 @@ template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) voi
   __shared__ float s_acc[(kWaves - 1) * N * 64];
   // Rows gridDim.x apart: the frequent tokens of a vocabulary stand together (a workgroup to 31 rows in a row: 162 us for 16384 tokens of 512 bf16 over 32000, the one of
   // the first tokens alone with all of it).
-  const int G = gridDim.x, rows = ((int)a.V - (int)blockIdx.x + G - 1) / G, wave = wave_id(), lane = lane_id(), pieces = a.D / N;
+  const int G = gridDim.x, rows = ((int)a.V - (int)blockIdx.x + G - 1) / G, wave = wave_id();
   // (Bounds by a search of each workgroup among the keys: 14 trips to memory for 16384 tokens, 21 us instead of 16.)
   if ((int)threadIdx.x < rows) s_range[threadIdx.x] = a.ranges[blockIdx.x + threadIdx.x * G];
   __syncthreads();
-  auto write = [&](int v, int i, vec<float, N> acc) { store_n<T, N>(static_cast<T*>(a.dw) + (int64_t)v * a.D + i * N, acc * a.scale); };
+  auto write = [&](int v, int c, vec<float, N> acc) { store_n<T, N>(static_cast<T*>(a.dw) + (int64_t)v * a.D + c, acc * a.scale); };
   for (int k = threadIdx.x / LPR; k < rows; k += kThreads / LPR) {
     const int64_t s = s_range[k].first, e = s_range[k].end;
     if (e - s > kFew) continue;
-    for (int i = threadIdx.x % LPR; i < pieces; i += LPR) write(blockIdx.x + k * G, i, sum_places<T, N>(a, s, e, 1, i));
+    for (int i = threadIdx.x % LPR; i < pieces_of<N>(a.D); i += LPR) {
+      const int c = column<N>(i, a.D);
+      write(blockIdx.x + k * G, c, sum_places<T, N>(a, s, e, 1, c));
+    }
   }
   for (int k = 0; k < rows; ++k) {   // by all waves: places in front of the first whole piece, whole pieces, places behind
     const int64_t s = s_range[k].first, e = s_range[k].end;
     if (e - s <= kFew) continue;
     const int64_t c0 = (s + kRun - 1) / kRun, c1 = e / kRun;
-    over_waves<N>(s_acc, pieces, [&](int i) {
-      if (c1 <= c0) return sum_places<T, N>(a, s + wave, e, kWaves, i);
-      vec<float, N> acc = sum_places<T, N>(a, s + wave, c0 * kRun, kWaves, i);
+    over_waves<N>(s_acc, a.D, [&](int c) {
+      if (c1 <= c0) return sum_places<T, N>(a, s + wave, e, kWaves, c);
+      vec<float, N> acc = sum_places<T, N>(a, s + wave, c0 * kRun, kWaves, c);
 #pragma unroll 4
-      for (int64_t c = c0 + wave; c < c1; c += kWaves) acc += *reinterpret_cast<const vec<float, N>*>(a.parts + c * a.D + i * N);
-      return acc + sum_places<T, N>(a, c1 * kRun + wave, e, kWaves, i);
-    }, [&](int i, vec<float, N> acc) { write(blockIdx.x + k * G, i, acc); });
+      for (int64_t p = c0 + wave; p < c1; p += kWaves) acc += load_n<float, N>(a.parts + p * a.D + c);
+      return acc + sum_places<T, N>(a, c1 * kRun + wave, e, kWaves, c);
+    }, [&](int c, vec<float, N> acc) { write(blockIdx.x + k * G, c, acc); });
   }
 }
 
 // f(type, std::integral_constant elements at a time)
-template <typename F> int by_pieces(int dtype, bool whole, F&& f) {
+template <typename F> int by_pieces(int dtype, int D, F&& f) {
   return by_tensor_type(dtype, [&](auto t) {
     using T = decltype(t);
-    if (whole) return f(t, std::integral_constant<int, elem_traits<T>::vec16>());
+    constexpr int N = elem_traits<T>::vec16;
+    if (D >= N) return f(t, std::integral_constant<int, N>());
     return f(t, std::integral_constant<int, 1>());
   });
-}
-bool whole_pieces(int D, int64_t ld, int dtype, std::initializer_list<const void*> ps) {
-  const int es = dtype == 0 ? 4 : 2;
-  bool whole = (int64_t)D * es % 16 == 0 && ld * es % 16 == 0;
-  for (const void* p : ps) whole = whole && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  return whole;
 }
 int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
 
 }  // namespace
 
 int launch_embedding(const EmbeddingArgs& a, int dtype, hipStream_t stream) {
-  return by_pieces(dtype, whole_pieces(a.D, a.ld, dtype, {a.table, a.y}), [&](auto t, auto n) {
+  return by_pieces(dtype, a.D, [&](auto t, auto n) {
     using T = decltype(t);
     auto go = [&](auto lpr) {
       constexpr int LPR = decltype(lpr)::value, rows = kThreads / LPR;
       hipLaunchKernelGGL((embedding_kernel<T, n.value, LPR>), dim3((unsigned)((a.tokens.rows + rows - 1) / rows)), dim3(kThreads), 0, stream, a);
       return launched();
     };
-    const int pieces = a.D / n.value;
+    const int pieces = (a.D + n.value - 1) / n.value;
     if (pieces <= 16) return go(std::integral_constant<int, 16>());
     if (pieces <= 32) return go(std::integral_constant<int, 32>());
     return go(std::integral_constant<int, 64>());
@@ -442,11 +449,11 @@ int launch_sorted_grad(const SortedGradArgs& g, int dtype, hipStream_t stream) {
   }
   const int sorted = (p.passes - 1) % 2;
   const SumArgs s = {keys[sorted], places[sorted], ranges, g.tokens.rows, g.dy, g.dw, parts, g.V, g.D, p.rows_per_group, g.scale};
-  return by_pieces(dtype, whole_pieces(g.D, g.D, dtype, {g.dy, g.dw}), [&](auto t, auto n) {
+  return by_pieces(dtype, g.D, [&](auto t, auto n) {
     using T = decltype(t);
     hipLaunchKernelGGL((run_sum_kernel<T, n.value>), dim3((unsigned)((s.rows + kRun - 1) / kRun)), dim3(kThreads), 0, stream, s);
     const dim3 grid((unsigned)((g.V + p.rows_per_group - 1) / p.rows_per_group));
-    const int pieces = g.D / n.value;
+    const int pieces = (g.D + n.value - 1) / n.value;
     if (pieces <= 16) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 16>), grid, dim3(kThreads), 0, stream, s);
     else if (pieces <= 32) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 32>), grid, dim3(kThreads), 0, stream, s);
     else hipLaunchKernelGGL((table_grad_kernel<T, n.value, 64>), grid, dim3(kThreads), 0, stream, s);
