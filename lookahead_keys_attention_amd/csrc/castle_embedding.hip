@@ -7,7 +7,7 @@
 // digits of up to ten bits, a counting and a placing launch for each.  Where each token's places begin and end is noted, and pieces of 64 sorted places that hold one
 // token alone are summed first, so that a token that takes a tenth of a text does not keep one workgroup busy when the rest is done; then every row of the
 // table is summed and written once, zeros where there is no token.
-// Measured, bf16: 65536 tokens over 131072 rows of 2048, forward 86 us (5.5 TB/s), gradient 243 (3.3 TB/s of what it has to move, 33 of it the sort); 16384 over 32000 of 512, 7 and
+// Measured, bf16: 65536 tokens over 131072 rows of 2048, forward 86 us (5.5 TB/s), gradient 212 (3.8 TB/s of what it has to move, 33 of it the sort); 16384 over 32000 of 512, 7 and
 // 44 us, of which 24 are the four launches of the sort, each little more than its start and two trips to memory.
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
@@ -284,9 +284,9 @@ template <typename T, int N> __device__ __forceinline__ vec<float, N> sum_places
   return acc;
 }
 // f(first column of a piece), a wave's sum of it, added over the waves, in their order, handed to `out` in wave 0
-template <int N, typename F, typename G> __device__ __forceinline__ void over_waves(float* s_acc, int D, F&& f, G&& out) {
+template <int N, typename F, typename G> __device__ __forceinline__ void over_waves(float* s_acc, int D, int first, int step, F&& f, G&& out) {   // pieces from `first`, 64 and then `step` on
   const int wave = wave_id(), lane = lane_id(), pieces = pieces_of<N>(D);
-  for (int p0 = 0; p0 < pieces; p0 += 64) {
+  for (int p0 = first; p0 < pieces; p0 += step) {
     const int i = p0 + lane, c = column<N>(i, D);
     vec<float, N> acc = fill_n<N>(0.f);
     if (i < pieces) acc = f(c);
@@ -307,7 +307,7 @@ template <int N, typename F, typename G> __device__ __forceinline__ void over_wa
 template <typename T, int N> __global__ __launch_bounds__(kThreads) void run_sum_kernel(SumArgs a) {
   __shared__ float s_acc[(kWaves - 1) * N * 64];
   const int64_t first = (int64_t)blockIdx.x * kRun, i = first + threadIdx.x;
-  if (threadIdx.x < kRun && i < a.rows) {   // where a token ends and the next one begins
+  if (blockIdx.y == 0 && threadIdx.x < kRun && i < a.rows) {   // where a token ends and the next one begins
     const uint32_t k = a.keys[i], before = i > 0 ? a.keys[i - 1] : k + 1;
     if (k != before) {
       if (k < (uint32_t)a.V) a.ranges[k].first = (uint32_t)i;
@@ -318,13 +318,13 @@ template <typename T, int N> __global__ __launch_bounds__(kThreads) void run_sum
   if (first + kRun > a.rows) return;
   const uint32_t key = a.keys[first];
   if (key >= (uint32_t)a.V || a.keys[first + kRun - 1] != key) return;
-  over_waves<N>(s_acc, a.D, [&](int c) { return sum_places<T, N>(a, first + wave_id(), first + kRun, kWaves, c); },
+  over_waves<N>(s_acc, a.D, 64 * blockIdx.y, 64 * gridDim.y, [&](int c) { return sum_places<T, N>(a, first + wave_id(), first + kRun, kWaves, c); },
                 [&](int c, vec<float, N> v) { store_n<float, N>(a.parts + (int64_t)blockIdx.x * a.D + c, v); });
 }
 
 constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that one wave, or part of one, sums by itself
-// LPR: lanes to a row of few tokens
-template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) void table_grad_kernel(SumArgs a) {
+// LPR: lanes to a row of few tokens, AT: pieces of each side by side, whose loads are on their way together (65536 tokens over 131072 rows of 2048 bf16: one by one 185 us, four 150)
+template <typename T, int N, int LPR, int AT> __global__ __launch_bounds__(kThreads) void table_grad_kernel(SumArgs a) {
   __shared__ Range s_range[kMaxRowsPerGroup];
   __shared__ float s_acc[(kWaves - 1) * N * 64];
   // Rows gridDim.x apart: the frequent tokens of a vocabulary stand together (a workgroup to 31 rows in a row: 162 us for 16384 tokens of 512 bf16 over 32000, the one of
@@ -337,16 +337,30 @@ template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) voi
   for (int k = threadIdx.x / LPR; k < rows; k += kThreads / LPR) {
     const int64_t s = s_range[k].first, e = s_range[k].end;
     if (e - s > kFew) continue;
-    for (int i = threadIdx.x % LPR; i < pieces_of<N>(a.D); i += LPR) {
-      const int c = column<N>(i, a.D);
-      write(blockIdx.x + k * G, c, sum_places<T, N>(a, s, e, 1, c));
+    for (int i = threadIdx.x % LPR; i < pieces_of<N>(a.D); i += AT * LPR) {
+      vec<float, N> acc[AT];
+      int c[AT];
+#pragma unroll
+      for (int u = 0; u < AT; ++u) {
+        acc[u] = fill_n<N>(0.f);
+        c[u] = column<N>(min(i + u * LPR, pieces_of<N>(a.D) - 1), a.D);
+      }
+#pragma unroll AT == 1 ? 8 : 2
+      for (int64_t p = s; p < e; ++p) {
+        const T* row = static_cast<const T*>(a.dy) + (int64_t)a.places[p] * a.D;
+#pragma unroll
+        for (int u = 0; u < AT; ++u) acc[u] += load_n<T, N>(row + c[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < AT; ++u)
+        if (u == 0 || i + u * LPR < pieces_of<N>(a.D)) write(blockIdx.x + k * G, c[u], acc[u]);
     }
   }
   for (int k = 0; k < rows; ++k) {   // by all waves: places in front of the first whole piece, whole pieces, places behind
     const int64_t s = s_range[k].first, e = s_range[k].end;
     if (e - s <= kFew) continue;
     const int64_t c0 = (s + kRun - 1) / kRun, c1 = e / kRun;
-    over_waves<N>(s_acc, a.D, [&](int c) {
+    over_waves<N>(s_acc, a.D, 0, 64, [&](int c) {
       if (c1 <= c0) return sum_places<T, N>(a, s + wave, e, kWaves, c);
       vec<float, N> acc = sum_places<T, N>(a, s + wave, c0 * kRun, kWaves, c);
 #pragma unroll 4
@@ -451,12 +465,13 @@ int launch_sorted_grad(const SortedGradArgs& g, int dtype, hipStream_t stream) {
   const SumArgs s = {keys[sorted], places[sorted], ranges, g.tokens.rows, g.dy, g.dw, parts, g.V, g.D, p.rows_per_group, g.scale};
   return by_pieces(dtype, g.D, [&](auto t, auto n) {
     using T = decltype(t);
-    hipLaunchKernelGGL((run_sum_kernel<T, n.value>), dim3((unsigned)((s.rows + kRun - 1) / kRun)), dim3(kThreads), 0, stream, s);
-    const dim3 grid((unsigned)((g.V + p.rows_per_group - 1) / p.rows_per_group));
     const int pieces = (g.D + n.value - 1) / n.value;
-    if (pieces <= 16) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 16>), grid, dim3(kThreads), 0, stream, s);
-    else if (pieces <= 32) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 32>), grid, dim3(kThreads), 0, stream, s);
-    else hipLaunchKernelGGL((table_grad_kernel<T, n.value, 64>), grid, dim3(kThreads), 0, stream, s);
+    hipLaunchKernelGGL((run_sum_kernel<T, n.value>), dim3((unsigned)((s.rows + kRun - 1) / kRun), std::min(8, (pieces + 63) / 64)), dim3(kThreads), 0, stream, s);
+    const dim3 grid((unsigned)((g.V + p.rows_per_group - 1) / p.rows_per_group));
+    if (pieces <= 16) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 16, 1>), grid, dim3(kThreads), 0, stream, s);
+    else if (pieces <= 32) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 32, 1>), grid, dim3(kThreads), 0, stream, s);
+    else if (pieces <= 64) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 64, 1>), grid, dim3(kThreads), 0, stream, s);
+    else hipLaunchKernelGGL((table_grad_kernel<T, n.value, 64, 4>), grid, dim3(kThreads), 0, stream, s);
     return launched();
   });
 }
