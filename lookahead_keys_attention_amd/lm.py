@@ -341,7 +341,13 @@ class CastleLM(nn.Module):
         if not native:
             return lambda x, residual: F.dropout(x, self.dropout) if residual is None else residual + F.dropout(x, self.dropout)
         seeds = iter(torch.randint(-2 ** 63, 2 ** 63 - 1, (1 + 2 * len(self.layers), 2), device=device))
-        return lambda x, residual: ops.dropout_add(x, residual, self.dropout, next(seeds))
+
+        def drop(x, residual):
+            if residual is not None and residual.dtype != x.dtype:   # (under autocast: the sum has the wider type)
+                return residual + ops.dropout_add(x, None, self.dropout, next(seeds))
+            return ops.dropout_add(x, residual, self.dropout, next(seeds))
+
+        return drop
 
     def _plain(self, x) -> bool:
         """True if whole sequences may run as one native call per block: native layers, unmodified modules, nothing

@@ -162,6 +162,53 @@ def test_dropout_in_training(hooked):
 
 
 @gpu
+def test_dropout_under_autocast():
+    """The blocks' outputs have 16 bits then, what they are added to 32: the loss without dropout to within 2e-2, gradients of everything."""
+    model = make(True, dropout=0.2, embedding_scale=2.0).to(DEV)
+    x = ids().to(DEV)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = train(model, x)
+    assert len(got) == 1 + sum(p.requires_grad for p in model.parameters()) and all(t.isfinite().all() for t in got)
+    model.eval()
+    with torch.no_grad():
+        want = model(x, return_loss=True)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            assert (model(x, return_loss=True) - want).abs() <= 2e-2 * want
+
+
+@gpu
+def test_training_step_in_a_graph(monkeypatch):
+    """Loss and gradients of a model, captured; each replay draws the masks that the device's generator has next, as an eager step does, and sees the tokens that are there then."""
+    monkeypatch.setattr(LM, "linear_loss_is_ahead", lambda rows, weight: True)
+    model = make(True, dropout=0.25, embedding_scale=2.0).bfloat16().to(DEV)
+    x, leaves = ids().to(DEV), [p for p in model.parameters() if p.requires_grad]
+
+    def step():
+        loss = model(x, return_loss=True)
+        return loss.detach(), *torch.autograd.grad(loss, leaves)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    seen = []
+    for k in range(3):
+        x.copy_(ids(seed=k))
+        torch.manual_seed(k // 2)
+        want = step()
+        torch.manual_seed(k // 2)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        seen.append(got[1].clone())   # (a loss of 16 bits may well be the same)
+    assert not any(torch.equal(seen[a], seen[b]) for a, b in ((0, 1), (0, 2), (1, 2)))
+
+
+@gpu
 @pytest.mark.parametrize("graph", [False, True])
 def test_sampling_with_a_scaled_embedding(graph):
     """Greedy tokens of the native model, also one that is in training and has dropout, are those of the parallel pass over what it has written."""
