@@ -822,14 +822,14 @@ template <typename T, int MODE, int BM, int BN, bool PARTS> int launch_product_t
   hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN, PARTS>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -3;
 }
-// Rows and columns of a workgroup's tile.  64 rows for that few; else 128 where 256 leave CUs idle: by what the fullest CU takes (us), 1.4 a step and 5 an end of 256 x 256, 0.85 and
-// 3 of 128 x 256.
+// Rows and columns of a workgroup's tile.  Of 64, 128 or 256 rows those with which the fullest CU is done first (us): 1.4 a step and 5 an end of 256 x 256, 0.85 and 3 of 128,
+// 0.56 and 1.6 of 64.  (The loss alone of 128 rows over 32000, 512 wide in bf16, with tiles of 64 rows / 128: 28 / 30 us, 2048 wide 46 / 52; 256 rows 34 / 32, since 500 tiles take two rounds.)
 struct Tile { int rows, columns; };
 int64_t tiles(int64_t m, int64_t n, Tile t) { return up(m, t.rows) / t.rows * (up(n, t.columns) / t.columns); }
-Tile tile_of(int R, int n, int steps, int splits = 1) {
-  if (R <= 64) return {64, 256};
-  auto cost = [&](Tile t, double step, double end) { return (tiles(R, n, t) * splits + 255) / 256 * (step * steps + end); };
-  return cost({128, 256}, 0.85, 3) < cost({256, 256}, 1.4, 5) ? Tile{128, 256} : Tile{256, 256};
+Tile tile_of(int R, int n, int steps) {
+  auto cost = [&](Tile t, double step, double end) { return (tiles(R, n, t) + 255) / 256 * (step * steps + end); };
+  const double large = cost({256, 256}, 1.4, 5), middle = cost({128, 256}, 0.85, 3), small = cost({64, 256}, 0.56, 1.6);
+  return R <= 64 || small < std::min(middle, large) ? Tile{64, 256} : middle < large ? Tile{128, 256} : Tile{256, 256};
 }
 template <int MODE> int launch_product(const ProductArgs& a, Tile tile, int dtype, hipStream_t stream) {
   auto of_type = [&](auto t, auto parts) {
@@ -870,13 +870,14 @@ struct Plan {
   int step;                // of a contraction
 };
 // Tile and ranges of a contraction of `steps` for m x n outputs, from what it takes roughly (us): so much a step and an end for each of the items of the fullest CU, and for
-// several ranges their partial results, written and read at 4 TB/s.
+// several ranges their partial results, written and read at 4 TB/s.  (Forward pass and the gradient of the rows over 32000, 512 wide in bf16, without tiles of 64 rows / with them:
+// 64 rows 67 / 61 us, 128 76 / 68, 256 81 / 78; over 4000 256 61 / 56, 1000 69 / 65.)
 Split split_of(int64_t m, int64_t n, int64_t steps, std::initializer_list<Tile> kinds) {
   Split best = {};
   double best_cost = 1e30;
   for (const Tile t : kinds) {
-    const bool large = t.rows * t.columns > 128 * 256;
-    const double step = large ? 1.5 : t.rows * t.columns > 64 * 128 ? 1.05 : 0.6, end = large ? 5 : 3;
+    const int area = t.rows * t.columns;
+    const double step = area > 128 * 256 ? 1.5 : area > 64 * 256 ? 1.05 : area > 64 * 128 ? 0.8 : 0.6, end = area > 128 * 256 ? 5 : 3;
     for (int s = 1; s <= 128 && s <= std::max<int64_t>(1, steps / 2); ++s) {
       const double cost = (tiles(m, n, t) * s + 255) / 256 * (step * steps_of_range((int)steps, s) + end) + (s > 1 ? 8e-6 / 4 * s * m * n : 0);
       if (cost < best_cost) {
@@ -902,8 +903,9 @@ Plan plan(const VocabArgs& a, int es) {
   p.logits = tile_of(a.R, a.V, p.Dp / p.step);
   p.P = (int)(up(a.V, 256) / 256 * (p.logits.rows == 256 ? 2 : 4));
   const int wide = a.D <= 128 ? 128 : 256;
-  p.rows = a.R <= 64 ? split_of(a.R, a.D, p.ldc / p.step, {{64, wide}}) : wide == 128 ? split_of(a.R, a.D, p.ldc / p.step, {{256, 128}})
-                                                                                      : split_of(a.R, a.D, p.ldc / p.step, {{256, 256}, {128, 256}});
+  p.rows = wide == 128 ? (a.R <= 64 ? split_of(a.R, a.D, p.ldc / p.step, {{64, 128}}) : split_of(a.R, a.D, p.ldc / p.step, {{64, 128}, {256, 128}}))
+         : a.R <= 64   ? split_of(a.R, a.D, p.ldc / p.step, {{64, 128}, {64, 256}})
+                       : split_of(a.R, a.D, p.ldc / p.step, {{64, 128}, {64, 256}, {128, 256}, {256, 256}});
   p.weights = split_of(p.ldc, a.D, p.Rp / p.step, {{256, wide}});
   return p;
 }
