@@ -878,8 +878,10 @@ Split split_of(int64_t m, int64_t n, int64_t steps, std::initializer_list<Tile> 
   for (const Tile t : kinds) {
     const int area = t.rows * t.columns;
     const double step = area > 128 * 256 ? 1.5 : area > 64 * 256 ? 1.05 : area > 64 * 128 ? 0.8 : 0.6, end = area > 128 * 256 ? 5 : 3;
-    for (int s = 1; s <= 128 && s <= std::max<int64_t>(1, steps / 2); ++s) {
-      const double cost = (tiles(m, n, t) * s + 255) / 256 * (step * steps_of_range((int)steps, s) + end) + (s > 1 ? 8e-6 / 4 * s * m * n : 0);
+    const int most = (int)std::min<int64_t>(128, std::max<int64_t>(1, steps / 2));
+    const int64_t items = tiles(m, n, t);
+    for (int s = 1; s <= most; ++s) {
+      const double cost = (items * s + 255) / 256 * (step * steps_of_range((int)steps, s) + end) + (s > 1 ? 8e-6 / 4 * s * m * n : 0);
       if (cost < best_cost) {
         best_cost = cost;
         best = {t, s};
@@ -890,7 +892,7 @@ Split split_of(int64_t m, int64_t n, int64_t steps, std::initializer_list<Tile> 
 }
 // bytes of an element of an operand of the products; es: of one of the tensors
 constexpr int operand_bytes(int es) { return es == 4 ? 6 : 2; }
-Plan plan(const VocabArgs& a, int es) {
+Plan make_plan(const VocabArgs& a, int es, bool gradients) {
   Plan p = {};
   p.step = es == 4 ? kPart : kWideK;
   p.Rp = up(a.R, 64);
@@ -902,12 +904,20 @@ Plan plan(const VocabArgs& a, int es) {
   p.ldc = std::min<int64_t>(p.columns, width);
   p.logits = tile_of(a.R, a.V, p.Dp / p.step);
   p.P = (int)(up(a.V, 256) / 256 * (p.logits.rows == 256 ? 2 : 4));
+  if (!gradients) return p;
   const int wide = a.D <= 128 ? 128 : 256;
   p.rows = wide == 128 ? (a.R <= 64 ? split_of(a.R, a.D, p.ldc / p.step, {{64, 128}}) : split_of(a.R, a.D, p.ldc / p.step, {{64, 128}, {256, 128}}))
          : a.R <= 64   ? split_of(a.R, a.D, p.ldc / p.step, {{64, 128}, {64, 256}})
                        : split_of(a.R, a.D, p.ldc / p.step, {{64, 128}, {64, 256}, {128, 256}, {256, 256}});
   p.weights = split_of(p.ldc, a.D, p.Rp / p.step, {{256, wide}});
   return p;
+}
+// A call asks three times for the plan of its sizes, 2 us each: a thread keeps the last one.
+Plan plan(const VocabArgs& a, int es, bool gradients) {
+  struct Last { int R, V, D, es, gradients; Plan p; };
+  static thread_local Last last = {};
+  if (last.R != a.R || last.V != a.V || last.D != a.D || last.es != es || last.gradients != (int)gradients) last = {a.R, a.V, a.D, es, gradients, make_plan(a, es, gradients)};
+  return last.p;
 }
 struct Carve {
   char* at;
@@ -990,18 +1000,18 @@ int64_t vocab_state_bytes(int64_t R) {
 }
 int64_t vocab_fwd_bytes(const VocabArgs& a, int es) {
   Carve c = {nullptr};
-  Fwd(a, plan(a, es), es, c);
+  Fwd(a, plan(a, es, false), es, c);
   return c.used;
 }
 int64_t vocab_bwd_bytes(const VocabArgs& a, int es, bool need_x, bool need_w) {
   Carve c = {nullptr};
-  Bwd(a, plan(a, es), es, need_x, need_w, c);
+  Bwd(a, plan(a, es, true), es, need_x, need_w, c);
   return c.used;
 }
 
 int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, void* workspace, hipStream_t stream) {
   const int es = dtype == 0 ? 4 : 2;
-  const Plan p = plan(a, es);
+  const Plan p = plan(a, es, false);
   Carve cs = {static_cast<char*>(state)}, cw = {static_cast<char*>(workspace)};
   const State s(a.R, cs);
   const Fwd f(a, p, es, cw);
@@ -1037,7 +1047,7 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
 
 int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const void* state, void* dx, void* dw, void* workspace, hipStream_t stream) {
   const int es = dtype == 0 ? 4 : 2;
-  const Plan p = plan(a, es);
+  const Plan p = plan(a, es, true);
   Carve cs = {static_cast<char*>(const_cast<void*>(state))}, cw = {static_cast<char*>(workspace)};
   const State s(a.R, cs);
   const Bwd b(a, p, es, dx != nullptr, dw != nullptr, cw);
