@@ -31,7 +31,7 @@ constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 constexpr int kWaves = kThreads / 64;
 constexpr int kCountRows = 1024;   // rows of a workgroup that counts
 constexpr int kGatherRows = 16;    // rows of a workgroup that copies
-constexpr int kLossRows = 16, kManyLossRows = 64;   // rows of a workgroup that joins maxima and sums: few, and of more than 4096 (one atomic of each: 1024 of them 22 us)
+constexpr int kFewLossRows = 4, kLossRows = 16, kManyLossRows = 64;   // rows of a workgroup that joins maxima and sums: of up to 512, of up to 4096 and of more (one atomic of each: 1024 of them 22 us)
 
 // Where maxima start: a score of -inf has weight 0 behind it wherever it stands, and log2(e) times it is finite.
 constexpr float kLeast = -0.5f * __FLT_MAX__;
@@ -241,28 +241,42 @@ struct LossArgs {
 };
 template <typename T, int ROWS> __global__ __launch_bounds__(kThreads) void row_loss_kernel(LossArgs a) {
   typedef vec<float, 2> v2;
-  __shared__ float s_m[ROWS][kThreads / ROWS + 1], s_s[ROWS][kThreads / ROWS + 1];
+  constexpr int Q = kThreads / ROWS, AT = 8;   // threads of a row, parts of a thread side by side
+  __shared__ float s_m[kWaves][ROWS], s_s[kWaves][ROWS];
   const int c = threadIdx.x % ROWS, q = threadIdx.x / ROWS, row = blockIdx.x * ROWS + c, count = a.head->count;
   float m = kLeast, s = 0.f;
-  if (row < count) {
-#pragma unroll 8
-    for (int p = q; p < a.P; p += kThreads / ROWS) {
-      const v2 x = a.parts[p * a.Rp + row];
-      const float mn = fmaxf(m, x[0]);
-      s = s * fast_exp2((m - mn) * kLog2e) + x[1] * fast_exp2((x[0] - mn) * kLog2e);
+  if (row < count)
+    for (int p0 = q; p0 < a.P; p0 += AT * Q) {
+      v2 x[AT];
+      float mn = m;
+#pragma unroll
+      for (int k = 0; k < AT; ++k) x[k] = p0 + k * Q < a.P ? a.parts[(p0 + k * Q) * a.Rp + row] : v2{kLeast, 0.f};
+#pragma unroll
+      for (int k = 0; k < AT; ++k) mn = fmaxf(mn, x[k][0]);
+      s *= fast_exp2((m - mn) * kLog2e);
+#pragma unroll
+      for (int k = 0; k < AT; ++k) s += x[k][1] * fast_exp2((x[k][0] - mn) * kLog2e);
       m = mn;
     }
+  auto join = [&](float m2, float s2) __attribute__((always_inline)) {
+    const float mn = fmaxf(m, m2);
+    s = s * fast_exp2((m - mn) * kLog2e) + s2 * fast_exp2((m2 - mn) * kLog2e);
+    m = mn;
+  };
+#pragma unroll
+  for (int o = ROWS; o < 64; o <<= 1) {
+    const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
+    join(m2, s2);
   }
-  s_m[c][q] = m;
-  s_s[c][q] = s;
+  if (lane_id() < ROWS) {
+    s_m[wave_id()][c] = m;
+    s_s[wave_id()][c] = s;
+  }
   __syncthreads();
   float loss = 0.f;
   if (q == 0 && row < count) {
-    for (int k = 1; k < kThreads / ROWS; ++k) {
-      const float mn = fmaxf(m, s_m[c][k]);
-      s = s * fast_exp2((m - mn) * kLog2e) + s_s[c][k] * fast_exp2((s_m[c][k] - mn) * kLog2e);
-      m = mn;
-    }
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) join(s_m[w][c], s_s[w][c]);
     const float lse = m + logf(s);
     a.lse[row] = lse;
     loss = lse - a.tl[row];
@@ -856,7 +870,7 @@ template <int MODE> int launch_product(const ProductArgs& a, Tile tile, int dtyp
 }
 
 // ---- sizes ----------------------------------------------------------------------------------------------------------
-int loss_rows(int R) { return R > 4096 ? kManyLossRows : kLossRows; }
+int loss_rows(int R) { return R > 4096 ? kManyLossRows : R > 512 ? kLossRows : kFewLossRows; }
 int loss_groups(int R) { return (R + loss_rows(R) - 1) / loss_rows(R); }
 struct Split { Tile tile; int ranges; };   // of a contraction
 struct Plan {
@@ -1039,8 +1053,12 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   if (rc != 0) return rc;
   const LossArgs l = {f.parts, s.head, f.row_of, f.tl, s.lse, f.sums, loss, p.P, a.reduction, p.Rp};
   return by_tensor_type(dtype, [&](auto t) {
-    if (loss_rows(a.R) == kLossRows) hipLaunchKernelGGL((row_loss_kernel<decltype(t), kLossRows>), dim3(loss_groups(a.R)), dim3(kThreads), 0, stream, l);
-    else hipLaunchKernelGGL((row_loss_kernel<decltype(t), kManyLossRows>), dim3(loss_groups(a.R)), dim3(kThreads), 0, stream, l);
+    auto go = [&](auto rows) { hipLaunchKernelGGL((row_loss_kernel<decltype(t), rows.value>), dim3(loss_groups(a.R)), dim3(kThreads), 0, stream, l); };
+    switch (loss_rows(a.R)) {
+      case kFewLossRows: go(std::integral_constant<int, kFewLossRows>()); break;
+      case kLossRows: go(std::integral_constant<int, kLossRows>()); break;
+      default: go(std::integral_constant<int, kManyLossRows>());
+    }
     return launched();
   });
 }
