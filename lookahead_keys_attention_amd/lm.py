@@ -269,6 +269,8 @@ class GraphedDecoder:
 
 
 class CastleLM(nn.Module):
+    embedding_scale, dropout = 1.0, 0.0   # (of models that were saved whole without them)
+
     def __init__(self, *, num_tokens, dim, depth, max_seq_len=512, dim_head=64, heads=8, use_triton=True,
                  rotary_emb=True, prenorm=True, tie_embedding=False, embedding_scale=1.0, dropout=0.0):
         super().__init__()

@@ -351,7 +351,7 @@ def small_linear(x: torch.Tensor, weight: torch.Tensor, norm=None, activation=No
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduction: str = "mean", ignore_index: int = -100) -> torch.Tensor:
     """F.cross_entropy(x @ weight.T, target) of hidden rows x (..., D), a vocabulary (V, D) and classes (...), without the logits in memory
-    (the end of a language model, train_triton.py:164-171): what it keeps for the backward pass is one number per row.
+    (the end of a language model, train_triton.py:164-171): what it keeps for the backward pass, beside its inputs, is two numbers per row.
 
     Sums and the loss are formed in 32 bits from unrounded logits; the result has the type of x.  reduction: "mean" over the rows that count,
     "sum", or "none" for the loss of each row, shaped like `target`.  Rows of class `ignore_index` cost nothing and have no part in anything, whatever they

@@ -43,6 +43,8 @@ def test_scale_and_dropout_of_the_dense_model():
     for bad in (-0.1, 1.1):
         with pytest.raises(ValueError):
             make(False, dropout=bad)
+    del plain.__dict__["dropout"], plain.__dict__["embedding_scale"]   # a model that was saved whole before it had them
+    assert plain(x).shape == (3, 41, V)
 
 
 def test_where_the_loss_is_taken_without_logits():
