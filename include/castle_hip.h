@@ -421,7 +421,7 @@ int castle_embedding_grad(const void* dy, const int64_t* index, int64_t index_n,
 #define CASTLE_LOSS_MEAN 0
 #define CASTLE_LOSS_SUM 1
 #define CASTLE_LOSS_EACH 2
-int64_t castle_linear_cross_entropy_state_bytes(int rows);
+int64_t castle_linear_cross_entropy_state_bytes(int rows, int width, int dtype);
 int64_t castle_linear_cross_entropy_workspace_bytes(int rows, int vocabulary, int width, int dtype, int gradients);
 int castle_linear_cross_entropy(const void* x, int64_t ld_x, const void* w, int64_t ld_w, const int64_t* target, int64_t target_n, int64_t target_ld, int64_t ignore_index,
                                 int rows, int vocabulary, int width, int reduction, void* loss, void* state, int64_t state_bytes, int dtype, void* workspace,

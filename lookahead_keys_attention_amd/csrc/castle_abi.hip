@@ -923,7 +923,11 @@ static int vocab_args(castle::VocabArgs& a, const void* x, int64_t ld_x, const v
 }
 static_assert(CASTLE_LOSS_MEAN == castle::kMeanLoss && CASTLE_LOSS_SUM == castle::kSumLoss && CASTLE_LOSS_EACH == castle::kEachLoss, "");
 
-int64_t castle_linear_cross_entropy_state_bytes(int rows) { return rows > 0 && rows <= 1 << 24 ? castle::vocab_state_bytes(rows) : CASTLE_ERR_SHAPE; }
+int64_t castle_linear_cross_entropy_state_bytes(int rows, int width, int dtype) {
+  const int es = elem_size(dtype);
+  if (es == 0) return CASTLE_ERR_DTYPE;
+  return vocab_sizes_ok(rows, 1, width) ? castle::vocab_state_bytes(rows, width, es) : CASTLE_ERR_SHAPE;
+}
 int64_t castle_linear_cross_entropy_workspace_bytes(int rows, int vocabulary, int width, int dtype, int gradients) {
   const int es = elem_size(dtype);
   if (es == 0) return CASTLE_ERR_DTYPE;
@@ -944,7 +948,7 @@ int castle_linear_cross_entropy(const void* x, int64_t ld_x, const void* w, int6
   const int rc = vocab_args(a, x, ld_x, w, ld_w, target, target_n, target_ld, ignore_index, rows, vocabulary, width, reduction, dtype);
   if (rc != CASTLE_OK) return rc;
   if (!aligned_to({loss}, elem_size(dtype))) return CASTLE_ERR_ARG;
-  if (!workspace_ok(state, state_bytes, castle::vocab_state_bytes(rows)) || !workspace_ok(workspace, workspace_bytes, castle::vocab_fwd_bytes(a, elem_size(dtype))))
+  if (!workspace_ok(state, state_bytes, castle::vocab_state_bytes(rows, width, elem_size(dtype))) || !workspace_ok(workspace, workspace_bytes, castle::vocab_fwd_bytes(a, elem_size(dtype))))
     return CASTLE_ERR_WORKSPACE;
   return castle::launch_vocab_fwd(a, dtype, loss, state, workspace, static_cast<hipStream_t>(stream));
 }
@@ -956,7 +960,7 @@ int castle_linear_cross_entropy_bwd(const void* x, int64_t ld_x, const void* w, 
   const int rc = vocab_args(a, x, ld_x, w, ld_w, target, target_n, target_ld, ignore_index, rows, vocabulary, width, reduction, dtype);
   if (rc != CASTLE_OK) return rc;
   if (!aligned_to({dloss}, elem_size(dtype)) || !aligned16({dx, dweight}) || (dx == nullptr && dweight == nullptr)) return CASTLE_ERR_ARG;
-  if (!workspace_ok(state, state_bytes, castle::vocab_state_bytes(rows)) ||
+  if (!workspace_ok(state, state_bytes, castle::vocab_state_bytes(rows, width, elem_size(dtype))) ||
       !workspace_ok(workspace, workspace_bytes, castle::vocab_bwd_bytes(a, elem_size(dtype), dx != nullptr, dweight != nullptr)))
     return CASTLE_ERR_WORKSPACE;
   return castle::launch_vocab_bwd(a, dtype, dloss, state, dx, dweight, workspace, static_cast<hipStream_t>(stream));

@@ -1043,7 +1043,7 @@ std::tuple<Tensor, Tensor> linear_cross_entropy_op(const Tensor& x, const Tensor
     if (reduction != CASTLE_LOSS_EACH) loss.fill_(reduction == CASTLE_LOSS_MEAN ? std::numeric_limits<double>::quiet_NaN() : 0.0);
     return {loss, bytes(0, x)};
   }
-  const int64_t sbytes = check(castle_linear_cross_entropy_state_bytes(c.rows), "castle_linear_cross_entropy_state_bytes");
+  const int64_t sbytes = check(castle_linear_cross_entropy_state_bytes(c.rows, c.width, c.dtype), "castle_linear_cross_entropy_state_bytes");
   const int64_t nbytes = check(castle_linear_cross_entropy_workspace_bytes(c.rows, c.vocabulary, c.width, c.dtype, 0), "castle_linear_cross_entropy_workspace_bytes");
   Tensor state = bytes(sbytes, x), ws = bytes(nbytes, x);
   check(castle_linear_cross_entropy(c.x.data_ptr(), c.x.stride(0), c.w.data_ptr(), c.w.stride(0), c.target.ptr(), c.target.n, c.target.ld, ignore_index, c.rows, c.vocabulary,

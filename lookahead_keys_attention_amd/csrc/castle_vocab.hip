@@ -10,7 +10,7 @@
 // either gradient, 1.1 to 1.2 PFLOP/s (the library's product of these sizes 1.36).  Where the contraction is short the ends of the tiles show, which nothing hides behind
 // with one workgroup to a CU: 16384 rows of 512 over 32000, 0.54 TFLOP a product, 0.63, 0.73 (1 GB of d written), 0.51 and 0.49 ms.  (Two workgroups of four waves with shorter steps: the same.)
 //
-// Rows that do not count (target = ignore) are left out at the start: the others are copied together, and what the products cost goes with their number, which the kernels
+// Rows that do not count (target = ignore) are left out at the start: the others are copied together (for both passes), and what the products cost goes with their number, which the kernels
 // read from device memory.  So whatever a row that does not count holds, infinities and NaNs too, goes nowhere.
 //
 // fp32: an element is the sum of three bf16 numbers, 8 bits in each, of any exponent (below 2^-110 it keeps what lies above 2^-134); of the products of two elements' parts the six
@@ -62,10 +62,6 @@ struct RowArgs {
   int32_t* row_of;     // [Rp] the row
   int Dp;
   void* loss;          // kEachLoss: zeros for the rows that do not count
-  // backward pass: the factor of each row, and what goes to the gradients (kEachLoss: factor_kernel)
-  const void* dloss;
-  float* factor;
-  Gain* gain;
 };
 __device__ __forceinline__ int64_t class_of(const VocabArgs& a, int64_t r) {
   if (a.n == a.R) return a.target[r];
@@ -95,70 +91,51 @@ __global__ __launch_bounds__(kThreads) void count_rows_kernel(RowArgs a) {
   n = sum_over_threads<kWaves>(n, s);
   if (threadIdx.x == 0) a.block_counts[blockIdx.x] = n;
 }
-// FIRST: ranks and targets are formed here, else (backward pass) the ranks are there
-template <typename T, bool FIRST> __global__ __launch_bounds__(kThreads) void gather_rows_kernel(RowArgs a) {
+// ranks, targets and (16 bits) rows in their order
+template <typename T> __global__ __launch_bounds__(kThreads) void gather_rows_kernel(RowArgs a) {
   constexpr int V = elem_traits<T>::vec16;
   typedef vec<T, V> vt;
   __shared__ int s[kWaves], s_rank[kGatherRows];
   const int64_t first = (int64_t)blockIdx.x * kGatherRows;
-  int all;
-  if constexpr (FIRST) {
-    int before = 0, total = 0;
-    if (a.block_counts != nullptr) {
-      const int blocks = (a.v.R + kCountRows - 1) / kCountRows, mine = (int)(first / kCountRows);
-      for (int b = threadIdx.x; b < blocks; b += kThreads) {
-        const int n = a.block_counts[b];
-        total += n;
-        before += b < mine ? n : 0;
-      }
-      for (int64_t r = (int64_t)mine * kCountRows + threadIdx.x; r < first; r += kThreads) before += class_of(a.v, r) != a.v.ignore;
-    } else {
-#pragma unroll 4
-      for (int r = threadIdx.x; r < a.v.R; r += kThreads) {
-        const int n = class_of(a.v, r) != a.v.ignore;
-        total += n;
-        before += r < first ? n : 0;
-      }
+  int before = 0, total = 0;
+  if (a.block_counts != nullptr) {
+    const int blocks = (a.v.R + kCountRows - 1) / kCountRows, mine = (int)(first / kCountRows);
+    for (int b = threadIdx.x; b < blocks; b += kThreads) {
+      const int n = a.block_counts[b];
+      total += n;
+      before += b < mine ? n : 0;
     }
-    before = sum_over_threads<kWaves>(before, s);
-    all = sum_over_threads<kWaves>(total, s);
-    if (wave_id() == 0) {
-      const int64_t r = first + lane_id();
-      const bool mine = lane_id() < kGatherRows, there = mine && r < a.v.R;
-      const int64_t t = there ? class_of(a.v, r) : a.v.ignore;
-      const bool counts = t != a.v.ignore;
-      const uint64_t mask = __ballot(counts);
-      const int rank = counts ? before + __popcll(mask & ((1ull << lane_id()) - 1)) : -1;
-      if (mine) s_rank[lane_id()] = rank;
-      if (there) a.rank[r] = rank;
-      if (counts) {
-        a.tc[rank] = t >= 0 && t < a.v.V ? (int32_t)t : -1;
-        a.tl[rank] = NAN;
-        a.row_of[rank] = (int32_t)r;
-      }
-      if (a.v.reduction == kEachLoss && there && !counts) static_cast<T*>(a.loss)[r] = (T)0.f;
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      a.head->count = all;
-      a.head->inv_count = 1.f / (float)all;
-      a.head->arrived = 0;
-    }
+    for (int64_t r = (int64_t)mine * kCountRows + threadIdx.x; r < first; r += kThreads) before += class_of(a.v, r) != a.v.ignore;
   } else {
-    all = a.head->count;
-    float g = 0.f;   // of every row
-    if (a.v.reduction != kEachLoss && all > 0) g = (float)*static_cast<const T*>(a.dloss) * (a.v.reduction == kMeanLoss ? a.head->inv_count : 1.f);
-    if (threadIdx.x < kGatherRows) {
-      const int64_t r = first + lane_id();
-      const int rank = r < a.v.R ? a.rank[r] : -1;
-      s_rank[lane_id()] = rank;
-      if (rank >= 0) {
-        const int64_t t = class_of(a.v, r);
-        const bool there = t >= 0 && t < a.v.V;
-        a.tc[rank] = there ? (int32_t)t : -1;
-        if (a.v.reduction != kEachLoss) a.factor[rank] = !there ? NAN : sizeof(T) == 4 ? ldexpf(g, small_factor_shift(fabsf(g))) : ldexpf(1.f, kDShift);
-      }
+#pragma unroll 4
+    for (int r = threadIdx.x; r < a.v.R; r += kThreads) {
+      const int n = class_of(a.v, r) != a.v.ignore;
+      total += n;
+      before += r < first ? n : 0;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.v.reduction != kEachLoss) *a.gain = sizeof(T) == 4 ? Gain{small_factor_shift(fabsf(g)), 1.f} : Gain{kDShift, g};
+  }
+  before = sum_over_threads<kWaves>(before, s);
+  const int all = sum_over_threads<kWaves>(total, s);
+  if (wave_id() == 0) {
+    const int64_t r = first + lane_id();
+    const bool mine = lane_id() < kGatherRows, there = mine && r < a.v.R;
+    const int64_t t = there ? class_of(a.v, r) : a.v.ignore;
+    const bool counts = t != a.v.ignore;
+    const uint64_t mask = __ballot(counts);
+    const int rank = counts ? before + __popcll(mask & ((1ull << lane_id()) - 1)) : -1;
+    if (mine) s_rank[lane_id()] = rank;
+    if (there) a.rank[r] = rank;
+    if (counts) {
+      a.tc[rank] = t >= 0 && t < a.v.V ? (int32_t)t : -1;
+      a.tl[rank] = NAN;
+      a.row_of[rank] = (int32_t)r;
+    }
+    if (a.v.reduction == kEachLoss && there && !counts) static_cast<T*>(a.loss)[r] = (T)0.f;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.head->count = all;
+    a.head->inv_count = 1.f / (float)all;
+    a.head->arrived = 0;
   }
   __syncthreads();
   const int pieces = a.Dp / V, have = a.v.D / V;
@@ -308,6 +285,18 @@ template <typename T, int ROWS> __global__ __launch_bounds__(kThreads) void row_
   }
 }
 
+// One factor for all rows: 2^15 and the gain (fp32: the factor itself)
+template <typename T> __device__ __forceinline__ float one_factor(const void* dloss, const VocabHead& head, int reduction, Gain& gain) {
+  float g = (float)*static_cast<const T*>(dloss);
+  if (head.count == 0) g = 0.f;
+  else if (reduction == kMeanLoss) g *= head.inv_count;
+  if constexpr (sizeof(T) == 4) {
+    gain = {small_factor_shift(fabsf(g)), 1.f};
+    return ldexpf(g, gain.shift);
+  }
+  gain = {kDShift, g};
+  return ldexpf(1.f, kDShift);
+}
 // kEachLoss: factors of the rows, the largest of them at 2^14 ... 2^15 (fp32: see small_factor_shift)
 struct FactorArgs {
   const void* dloss;       // [R]
@@ -391,14 +380,17 @@ struct ProductArgs {
   const int32_t* tc;
   int first;               // column of the vocabulary that n = 0 is
   // kGrad: d, rows of ldc; rows behind the last up to a multiple of 64 and columns N ... ldc - 1 are zero
-  const float *lse, *factor;
+  const float *lse, *factor;   // factor: nullptr, or of each row; else one of dloss
+  const void* dloss;
+  const VocabHead* head;
+  int reduction;
   void* c;
   int64_t ldc;
   // kRowGrad: partial results [splits][part_rows][N], added to those that are there; kWeightGrad: c, or partial results [splits][M][N] where there are several
   float* out;
   int64_t part_rows;
   int add;
-  const Gain* gain;
+  Gain* gain;              // kGrad writes it where there is one factor
 };
 
 // PARTS: a step is 16 of the contraction, its first parts at s = 0 of what is in LDS, the second and third ones at 1 and 2; the last quarter of the place is not used (there the
@@ -485,6 +477,14 @@ template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_
   const int lane = lane_id(), wave = wave_id(), c = lane & 31, g = lane >> 5;
   const int count = __builtin_amdgcn_readfirstlane(*a.count), M = MODE == kWeightGrad ? a.M : min(a.M, count), K = MODE == kWeightGrad ? (int)up(min(a.K, count), kStep) : a.K;
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  float factor = 0.f;
+  if constexpr (MODE == kGrad) {
+    if (a.factor == nullptr) {
+      Gain gain;
+      factor = one_factor<std::conditional_t<PARTS, float, T>>(a.dloss, *a.head, a.reduction, gain);
+      if (blockIdx.x == 0 && threadIdx.x == 0) *a.gain = gain;
+    }
+  }
   if (tiles == 0) return;
   // Items are tiles for each range of the contraction; XCD x takes the x-th eighth of them.  Tiles in the order of an XCD's L2: all rows of a band of columns, then those of the next.
   constexpr int kBand = 2048 / BN;
@@ -598,7 +598,7 @@ template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_
         t[i] = a.tc[m];
         if constexpr (MODE == kGrad) {
           l[i] = a.lse[m];
-          f[i] = a.factor[m];
+          f[i] = a.factor != nullptr ? a.factor[m] : factor;
         }
       }
     };
@@ -606,7 +606,10 @@ template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_
 #pragma unroll
       for (int i = 0; i < S::FM; ++i) {
         asm volatile("" : "+v"(t[i]));
-        if constexpr (MODE == kGrad) asm volatile("" : "+v"(l[i]), "+v"(f[i]));
+        if constexpr (MODE == kGrad) {
+          asm volatile("" : "+v"(l[i]), "+v"(f[i]));
+          if (t[i] < 0) f[i] = NAN;
+        }
       }
     };
     constexpr bool ROWS = MODE == kStats || MODE == kGrad;
@@ -944,15 +947,14 @@ struct Carve {
 };
 struct Fwd {
   int* block_counts;
-  char *xc, *wc;   // wc: fp32, the parts of w
-  int32_t *tc, *row_of;
+  char *xc, *wc;   // fp32: the parts of the rows that count and of w
+  int32_t* row_of;
   float *tl, *sums;
   vec<float, 2>* parts;
   Fwd(const VocabArgs& a, const Plan& p, int es, Carve& c) {
     block_counts = c.take<int>(up(a.R, kCountRows) / kCountRows);
-    xc = c.take<char>(p.Rp * p.Dp * operand_bytes(es));
+    xc = c.take<char>(es == 4 ? p.Rp * p.Dp * operand_bytes(es) : 0);
     wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * operand_bytes(es) : 0);
-    tc = c.take<int32_t>(p.Rp);
     tl = c.take<float>(p.Rp);
     row_of = c.take<int32_t>(p.Rp);
     sums = c.take<float>(loss_groups(a.R));
@@ -961,15 +963,13 @@ struct Fwd {
 };
 struct Bwd {
   char *xc, *wc;
-  int32_t* tc;
   float* factor;
   Gain* gain;
   char* d;
   float *row_parts, *weight_parts;
   Bwd(const VocabArgs& a, const Plan& p, int es, bool need_x, bool need_w, Carve& c) {
-    xc = c.take<char>(p.Rp * p.Dp * operand_bytes(es));
+    xc = c.take<char>(es == 4 ? p.Rp * p.Dp * operand_bytes(es) : 0);
     wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * operand_bytes(es) : 0);
-    tc = c.take<int32_t>(p.Rp);
     factor = c.take<float>(p.Rp);
     gain = c.take<Gain>(1);
     d = c.take<char>(p.Rp * p.ldc * operand_bytes(es));
@@ -979,19 +979,22 @@ struct Bwd {
 };
 struct State {
   VocabHead* head;
-  int32_t* rank;
+  int32_t *rank, *tc;
   float* lse;
-  State(int64_t R, Carve& c) {
+  char* xc;   // 16 bits: the rows that count
+  State(int64_t R, int D, int es, Carve& c) {
     head = c.take<VocabHead>(1);
     rank = c.take<int32_t>(R);
+    tc = c.take<int32_t>(R);
     lse = c.take<float>(R);
+    xc = c.take<char>(es == 2 ? up(R, 64) * up(D, kWideK) * 2 : 0);
   }
 };
 int launched() { return hipGetLastError() == hipSuccess ? 0 : -3; }
-template <bool FIRST> int launch_gather(const RowArgs& a, int dtype, hipStream_t stream) {
+int launch_gather(const RowArgs& a, int dtype, hipStream_t stream) {
   return by_tensor_type(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((gather_rows_kernel<T, FIRST>), dim3((unsigned)(up(a.v.R, 64) / kGatherRows)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((gather_rows_kernel<T>), dim3((unsigned)(up(a.v.R, 64) / kGatherRows)), dim3(kThreads), 0, stream, a);
     return launched();
   });
 }
@@ -1007,9 +1010,9 @@ int launch_split(const VocabArgs& a, const Plan& p, const int* count, const int3
 
 }  // namespace
 
-int64_t vocab_state_bytes(int64_t R) {
+int64_t vocab_state_bytes(int64_t R, int D, int es) {
   Carve c = {nullptr};
-  State(R, c);
+  State(R, D, es, c);
   return c.used;
 }
 int64_t vocab_fwd_bytes(const VocabArgs& a, int es) {
@@ -1027,16 +1030,17 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   const int es = dtype == 0 ? 4 : 2;
   const Plan p = plan(a, es, false);
   Carve cs = {static_cast<char*>(state)}, cw = {static_cast<char*>(workspace)};
-  const State s(a.R, cs);
+  const State s(a.R, a.D, es, cs);
   const Fwd f(a, p, es, cw);
+  char* const xc = es == 4 ? f.xc : s.xc;
   const bool count = a.R > 4096;   // (up to there the copying workgroups count for themselves, which is less than a launch)
-  const RowArgs rows = {a, count ? f.block_counts : nullptr, s.head, s.rank, f.xc, f.tc, f.tl, f.row_of, p.Dp, loss, nullptr, nullptr, nullptr};
+  const RowArgs rows = {a, count ? f.block_counts : nullptr, s.head, s.rank, xc, s.tc, f.tl, f.row_of, p.Dp, loss};
   if (count) hipLaunchKernelGGL(count_rows_kernel, dim3((unsigned)(up(a.R, kCountRows) / kCountRows)), dim3(kThreads), 0, stream, rows);
-  int rc = launch_gather<true>(rows, dtype, stream);
+  int rc = launch_gather(rows, dtype, stream);
   if (rc == 0 && es == 4) rc = launch_split(a, p, &s.head->count, s.rank, f.xc, f.wc, stream);
   if (rc != 0) return rc;
   ProductArgs g = {};
-  g.a = f.xc;
+  g.a = xc;
   g.b = es == 4 ? f.wc : a.w;
   g.lda = es == 4 ? 3 * p.Dp : p.Dp;
   g.ldb = es == 4 ? 3 * p.Dp : a.ld_w;
@@ -1048,7 +1052,7 @@ int launch_vocab_fwd(const VocabArgs& a, int dtype, void* loss, void* state, voi
   g.parts = f.parts;
   g.tl = f.tl;
   g.Rp = p.Rp;
-  g.tc = f.tc;
+  g.tc = s.tc;
   rc = launch_product<kStats>(g, p.logits, dtype, stream);
   if (rc != 0) return rc;
   const LossArgs l = {f.parts, s.head, f.row_of, f.tl, s.lse, f.sums, loss, p.P, a.reduction, p.Rp};
@@ -1067,13 +1071,12 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
   const int es = dtype == 0 ? 4 : 2;
   const Plan p = plan(a, es, true);
   Carve cs = {static_cast<char*>(const_cast<void*>(state))}, cw = {static_cast<char*>(workspace)};
-  const State s(a.R, cs);
+  const State s(a.R, a.D, es, cs);
   const Bwd b(a, p, es, dx != nullptr, dw != nullptr, cw);
-  const RowArgs rows = {a, nullptr, s.head, s.rank, b.xc, b.tc, nullptr, nullptr, p.Dp, nullptr, dloss, b.factor, b.gain};
-  int rc = launch_gather<false>(rows, dtype, stream);
-  if (rc == 0 && es == 4) rc = launch_split(a, p, &s.head->count, s.rank, b.xc, b.wc, stream);
+  char* const xc = es == 4 ? b.xc : s.xc;
+  int rc = es == 4 ? launch_split(a, p, &s.head->count, s.rank, b.xc, b.wc, stream) : 0;
   if (rc == 0 && a.reduction == kEachLoss) {
-    const FactorArgs f = {dloss, s.rank, b.tc, b.factor, b.gain, a.R};
+    const FactorArgs f = {dloss, s.rank, s.tc, b.factor, b.gain, a.R};
     rc = by_tensor_type(dtype, [&](auto t) {
       hipLaunchKernelGGL((factor_kernel<decltype(t)>), dim3(std::min<unsigned>(64, (unsigned)(up(a.R, 1024) / 1024))), dim3(1024), 0, stream, f);
       return launched();
@@ -1089,7 +1092,7 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
   for (int i = 0; i < p.pieces && rc == 0; ++i) {
     const int v0 = i * p.columns, n = std::min(p.columns, a.V - v0);
     ProductArgs g = {};
-    g.a = b.xc;
+    g.a = xc;
     g.b = (es == 4 ? b.wc : static_cast<const char*>(a.w)) + v0 * ld_w * 2;
     g.lda = ld_x;
     g.ldb = ld_w;
@@ -1099,10 +1102,13 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
     g.count = &s.head->count;
     g.splits = 1;
     g.Rp = p.Rp;
-    g.tc = b.tc;
+    g.tc = s.tc;
     g.first = v0;
     g.lse = s.lse;
-    g.factor = b.factor;
+    g.factor = a.reduction == kEachLoss ? b.factor : nullptr;
+    g.dloss = dloss;
+    g.head = s.head;
+    g.reduction = a.reduction;
     g.c = b.d;
     g.ldc = p.ldc;
     g.gain = b.gain;
@@ -1123,7 +1129,7 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
       ProductArgs w = g;
       w.a = b.d;
       w.lda = p.ldc;
-      w.b = b.xc;
+      w.b = xc;
       w.ldb = ld_x;
       w.M = n;
       w.N = a.D;

@@ -177,8 +177,10 @@ LOSS_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 def _fake_linear_cross_entropy(x, weight, target, reduction, ignore_index):
     rows = target.numel()
-    # three parts of whole 256 bytes: two numbers, and for each row its place among those that count and its log-sum-exp
-    nbytes = 256 + 2 * ((4 * rows + 255) // 256 * 256) if rows else 0
+    # parts of whole 256 bytes: two numbers, for each row its place among those that count, its class and its log-sum-exp, in 16 bits the rows that count
+    nbytes = 256 + 3 * ((4 * rows + 255) // 256 * 256) if rows else 0
+    if rows and x.element_size() == 2:
+        nbytes += (rows + 63) // 64 * 64 * ((x.shape[-1] + 63) // 64 * 64) * 2
     return (torch.empty(target.shape if reduction == LOSS_REDUCTIONS["none"] else (), dtype=x.dtype, device=x.device),
             torch.empty(nbytes, dtype=torch.uint8, device=x.device))
 
@@ -351,7 +353,7 @@ def small_linear(x: torch.Tensor, weight: torch.Tensor, norm=None, activation=No
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduction: str = "mean", ignore_index: int = -100) -> torch.Tensor:
     """F.cross_entropy(x @ weight.T, target) of hidden rows x (..., D), a vocabulary (V, D) and classes (...), without the logits in memory
-    (the end of a language model, train_triton.py:164-171): what it keeps for the backward pass, beside its inputs, is two numbers per row.
+    (the end of a language model, train_triton.py:164-171): what it keeps for the backward pass, beside its inputs, is three numbers per row and in 16 bits a copy of the rows.
 
     Sums and the loss are formed in 32 bits from unrounded logits; the result has the type of x.  reduction: "mean" over the rows that count,
     "sum", or "none" for the loss of each row, shaped like `target`.  Rows of class `ignore_index` cost nothing and have no part in anything, whatever they

@@ -123,11 +123,13 @@ def test_entry_points_check_their_arguments_on_the_host():
 
     lib, i, i64, vp = N.lib(), ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
     state, size = lib.castle_linear_cross_entropy_state_bytes, lib.castle_linear_cross_entropy_workspace_bytes
-    state.restype, state.argtypes, size.restype, size.argtypes = i64, [i], i64, [i] * 5
-    assert state(0) == state((1 << 24) + 1) == -2
+    state.restype, state.argtypes, size.restype, size.argtypes = i64, [i] * 3, i64, [i] * 5
+    assert state(0, 8, 1) == state((1 << 24) + 1, 8, 1) == state(5, 12, 1) == -2 and state(5, 8, 3) == -1
     for rows in (1, 64, 1000):   # what the operator's shape propagation says
-        _, fake = ops._fake_linear_cross_entropy(torch.empty(rows, 8), torch.empty(5, 8), torch.empty(rows, dtype=torch.long), 0, -100)
-        assert state(rows) == fake.numel()
+        for width in (8, 64, 72):
+            for code, dtype in ((0, torch.float32), (1, torch.bfloat16), (2, torch.float16)):
+                _, fake = ops._fake_linear_cross_entropy(torch.empty(rows, width, dtype=dtype), torch.empty(5, width, dtype=dtype), torch.empty(rows, dtype=torch.long), 0, -100)
+                assert state(rows, width, code) == fake.numel()
     assert size(5, 10, 8, 3, 0) == -1 and size(5, 10, 8, 1, 4) == size(5, 10, 8, 1, -1) == -5
     for bad in ((0, 10, 8), (5, 0, 8), (5, 10, 0), (5, 10, 12), ((1 << 24) + 1, 10, 8), (5, (1 << 22) + 1, 8), (5, 10, (1 << 16) + 8)):
         assert size(*bad, 1, 0) == -2
