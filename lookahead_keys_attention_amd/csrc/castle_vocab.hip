@@ -396,10 +396,14 @@ struct ProductArgs {
   Gain* gain;              // kGrad writes it where there is one factor
 };
 
+// Loads of a wave for a step.  Of operands that are not contraction-contiguous, parts leave out the quarter that is not used, where that is whole loads: three buffers fit
+// the products for dw (2048 rows of 512 over 32000 413 -> 395 us).
+template <bool KC, int FREE, bool PARTS> constexpr int kOperandLoads = PARTS && !KC && FREE == 256 ? 3 : FREE / 64;
 // PARTS: a step is 16 of the contraction, its first parts at s = 0 of what is in LDS, the second and third ones at 1 and 2; the last quarter of the place is not used (there the
 // third ones lie again)
 template <typename T, bool KC, int FREE> struct PartsOperand : WideOperand<T, KC, FREE> {
   typedef WideOperand<T, KC, FREE> W;
+  static constexpr int N = kOperandLoads<KC, FREE, true>;
   __device__ __forceinline__ void start(const T* p, int64_t ld, int free0, int free_end, int k0) {
     W::at = KC ? p + free0 * ld + 3 * k0 : p + k0 * ld + 3 * free0;
     W::left = free_end - free0;
@@ -407,9 +411,9 @@ template <typename T, bool KC, int FREE> struct PartsOperand : WideOperand<T, KC
   }
   // steps: what is left of the contraction, behind whose end (rows, not contraction-contiguous) the last one is read again
   __device__ __forceinline__ void place(int ld, int steps) {
-    const int lane = lane_id(), first = wave_id() * W::N;
+    const int lane = lane_id(), first = wave_id() * N;
 #pragma unroll
-    for (int q = 0; q < W::N; ++q) {
+    for (int q = 0; q < N; ++q) {
       if constexpr (KC) {
         const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7);
         W::off[q] = 2 * (uint32_t)(ld * min(row, W::left - 1) + 8 * min(piece, 5));
@@ -422,7 +426,7 @@ template <typename T, bool KC, int FREE> struct PartsOperand : WideOperand<T, KC
   }
   __device__ __forceinline__ void load(int64_t ld, uint32_t lds) {
 #pragma unroll
-    for (int q = 0; q < W::N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * W::N + q));
+    for (int q = 0; q < N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * N + q));
     W::at += KC ? 3 * kPart : kPart * ld;
   }
 };
@@ -433,14 +437,14 @@ template <bool PARTS> constexpr int kBlock = PARTS ? kPart : 64;          // row
 template <bool PARTS> constexpr int kBlockRow = PARTS ? 3 * kPart : 64;   // numbers of a row
 template <typename T, bool KC, int FREE, bool PARTS> struct BlockOperand : WideOperand<T, KC, FREE> {
   typedef WideOperand<T, KC, FREE> W;
-  static constexpr int B = kBlock<PARTS>, BR = kBlockRow<PARTS>;
+  static constexpr int N = kOperandLoads<KC, FREE, PARTS>, B = kBlock<PARTS>, BR = kBlockRow<PARTS>;
   // p: [row of blocks][ldc / B][B][BR]
   __device__ __forceinline__ void start(const T* p, int64_t ldc, int free0, int free_end, int k0) {
-    const int lane = lane_id(), first = wave_id() * W::N, row_of_blocks = BR * (int)ldc;
+    const int lane = lane_id(), first = wave_id() * N, row_of_blocks = BR * (int)ldc;
     W::left = free_end - free0;
     W::at = p + (KC ? free0 : k0) / B * (int64_t)row_of_blocks + (KC ? k0 : free0) / B * (B * BR);
 #pragma unroll
-    for (int q = 0; q < W::N; ++q) {
+    for (int q = 0; q < N; ++q) {
       if constexpr (KC) {
         const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7), there = min(row, W::left - 1);
         W::off[q] = 2 * (uint32_t)(there / B * row_of_blocks + there % B * BR + 8 * (PARTS ? min(piece, 5) : piece));
@@ -453,7 +457,7 @@ template <typename T, bool KC, int FREE, bool PARTS> struct BlockOperand : WideO
   }
   __device__ __forceinline__ void load(int64_t ldc, uint32_t lds) {
 #pragma unroll
-    for (int q = 0; q < W::N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * W::N + q));
+    for (int q = 0; q < N; ++q) load_to_lds(W::at, W::off[q], lds + 1024 * (wave_id() * N + q));
     W::at += KC ? (int64_t)B * BR : BR * ldc;
   }
 };
@@ -462,9 +466,10 @@ template <typename T, bool KC, int FREE, bool PARTS> struct BlockOperand : WideO
 template <int MODE, int BM, int BN, bool PARTS> struct Shape {
   static constexpr int WM = BM == 256 ? 4 : 2, WN = 8 / WM, FM = BM / 32 / WM, FN = BN / 32 / WN;
   static constexpr bool kTurn = MODE == kGrad || (MODE == kWeightGrad && !PARTS);   // a tile goes through LDS to whole rows, 4 KB of each wave
-  static constexpr int kStage = (BM + BN) * kWideK * 2, kTurnBytes = kTurn ? 4096 * 8 : 0;
-  static constexpr int kFit = (kMaxLds - kTurnBytes) / kStage, kStages = kFit < 3 ? kFit : 3;
-  static constexpr int kLoads = kStage / 1024 / 8, kLds = kStages * kStage + kTurnBytes;
+  static constexpr bool kContractA = MODE != kWeightGrad, kContractB = MODE == kStats || MODE == kGrad;   // operands that are contraction-contiguous
+  static constexpr int kLoadsA = kOperandLoads<kContractA, BM, PARTS>, kLoads = kLoadsA + kOperandLoads<kContractB, BN, PARTS>;
+  static constexpr int kBytesA = kLoadsA * 8 * 1024, kStage = kLoads * 8 * 1024, kTurnBytes = kTurn ? 4096 * 8 : 0;
+  static constexpr int kFit = (kMaxLds - kTurnBytes) / kStage, kStages = kFit < 3 ? kFit : 3, kLds = kStages * kStage + kTurnBytes;
   static constexpr int kStores = MODE == kStats ? FM : PARTS && MODE == kGrad ? 6 * FM * FN : MODE == kRowGrad || PARTS ? 4 * FM * FN : 2 * FM * FN;   // of a wave and tile (kWeightGrad: partial results are twice as many)
   static_assert(kStages >= 2 && FM >= 1 && FN >= 1, "");
 };
@@ -472,7 +477,7 @@ extern __shared__ __attribute__((aligned(16))) unsigned char castle_vocab_lds[];
 
 template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
   typedef Shape<MODE, BM, BN, PARTS> S;
-  constexpr bool AK = MODE != kWeightGrad, BKC = MODE == kStats || MODE == kGrad;
+  constexpr bool AK = S::kContractA, BKC = S::kContractB;
   constexpr int kStep = PARTS ? kPart : kWideK;   // of the contraction
   typedef std::conditional_t<MODE == kRowGrad || MODE == kWeightGrad, BlockOperand<T, AK, BM, PARTS>, std::conditional_t<PARTS, PartsOperand<T, AK, BM>, WideOperand<T, AK, BM>>> OpA;
   typedef std::conditional_t<PARTS, PartsOperand<T, BKC, BN>, WideOperand<T, BKC, BN>> OpB;
@@ -540,7 +545,7 @@ template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_
     if constexpr (MODE == kRowGrad || (BKC && !PARTS))
       if (next_k + kStep > K) rb.place((int)a.ldb, K - next_k);
     ra.load(a.lda, lds0 + buffer);
-    rb.load(a.ldb, lds0 + buffer + BM * kWideK * 2);
+    rb.load(a.ldb, lds0 + buffer + S::kBytesA);
     next_k += kStep;
     if (--next_steps == 0) {
       next_item += stride;
@@ -580,7 +585,7 @@ template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_
   int buffer = 0;
   frag<T> fa[PARTS ? 3 : 2][S::FM], fb[2][S::FN];
   auto read_a = [&](int slot, int s) __attribute__((always_inline)) { OpA::read(reinterpret_cast<const T*>(castle_vocab_lds + buffer), fa[slot], wm, s, c, g); };
-  auto read_b = [&](int slot, int s) __attribute__((always_inline)) { OpB::read(reinterpret_cast<const T*>(castle_vocab_lds + buffer) + BM * kWideK, fb[slot], wn, s, c, g); };
+  auto read_b = [&](int slot, int s) __attribute__((always_inline)) { OpB::read(reinterpret_cast<const T*>(castle_vocab_lds + buffer + S::kBytesA), fb[slot], wn, s, c, g); };
   auto then = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };   // these reads, then the products of the fragments before
   auto read = [&](int slot, int s) __attribute__((always_inline)) {
     read_a(slot, s);
