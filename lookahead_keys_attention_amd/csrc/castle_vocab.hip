@@ -15,7 +15,7 @@
 //
 // fp32: an element is the sum of three bf16 numbers, 8 bits in each, of any exponent (below 2^-110 it keeps what lies above 2^-134); of the products of two elements' parts the six
 // are formed that are not below 2^-24 of the whole.  Operands lie as such parts, 16 first ones, the 16 second ones and the 16 third ones, so a step is 16 of the contraction, and
-// everything else is that of the 16-bit types.  (Pairs of fp16 numbers with a power of two for each tensor, three products, took 845 us for 2048 rows of 512 over 32000, but
+// everything else is that of the 16-bit types.  (Pairs of fp16 numbers with a power of two for each tensor, three products, took 845 us for 2048 rows of 512 over 32000 instead of 1410, but
 // what is far below the largest element loses its digits: the gradient of a class whose softmax values are 2^-40 was gone.  The fp32 products of castle_gemm32.hip convert
 // inside the product: logits in memory, 1832 us.)
 #include "castle_tiles.h"
