@@ -194,8 +194,8 @@ class GraphedDecoder:
         self.counters.copy_(torch.tensor([self.length, self.base0], dtype=torch.int32), non_blocking=False)
 
     def _signature(self):
-        """What the captured graph has baked in: the addresses of the weights it reads."""
-        return tuple(p.data_ptr() for p in self.model.parameters())
+        """What the captured graph has baked in: the scale of the embedding, the addresses of the weights it reads."""
+        return (self.model.embedding_scale, *(p.data_ptr() for p in self.model.parameters()))
 
     def fits(self, caches, max_len: int) -> bool:
         """True if `load(caches)` can reuse this graph for a generation of up to max_len rows."""

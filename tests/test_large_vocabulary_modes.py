@@ -1,0 +1,36 @@
+"""A language model's scaled embedding, dropout and loss over a large vocabulary on the passes beside plain training: a decoder that is kept between samples, sequences of one token, frozen
+models, empty batches."""
+import pytest
+import torch
+
+from lookahead_keys_attention_amd import CastleLM, ops
+
+DEV = "cuda:0"
+gpu = pytest.mark.gpu
+
+
+def make(native=True, **kw):
+    torch.manual_seed(3)
+    return CastleLM(use_triton=native, **{"num_tokens": 300, "dim": 64, "depth": 2, "heads": 2, "dim_head": 32, **kw}).to(DEV)
+
+
+@gpu
+def test_a_kept_decoder_follows_the_scale_of_the_embedding():
+    """The scale is set between two samples: the steps of the second one are those of a decoder captured anew, with the new scale."""
+    model = make()
+    prompt = torch.randint(0, 300, (2, 9), generator=torch.Generator().manual_seed(5)).to(DEV)
+
+    def sample():
+        return model.sample(prompt, 40, temperature=0, graph=True)
+
+    want = {}
+    for scale in (1.0, 6.0, 0.25):
+        model.embedding_scale = scale
+        model.release_decoder()
+        want[scale] = sample()
+    assert not torch.equal(want[1.0], want[6.0]) and not torch.equal(want[6.0], want[0.25])
+    for scale in (6.0, 1.0, 0.25, 0.25, 1.0):
+        model.embedding_scale = scale
+        assert torch.equal(sample(), want[scale]), scale
+        kept = model.__dict__["_kept_decoder"]
+        assert torch.equal(sample(), want[scale]) and model.__dict__["_kept_decoder"] is kept   # (and the same scale again needs no other graph)
