@@ -306,12 +306,13 @@ class CastleLM(nn.Module):
             return self._forward_plain(x, target if return_loss else None, return_next_cache)
         native = self._native_on_gpu(x.device)
         h = self._embed(x, native)
-        drop = self._dropout(x.device, native, cache is None and not return_next_cache)
+        training = cache is None and not return_next_cache
+        drop = self._dropout(x.device, native, training)
         h = drop(h, None)
-        # one token per sequence, no graph to record: the few rows of every projection go through the small-M kernel
+        # one token per sequence, no graph to record, nothing to drop (the residual is added in the same launch): the few rows of every projection go through the small-M kernel
         # (only for a model whose layers run the native kernels: one built with use_triton=False stays on
         # the PyTorch layers throughout, so it remains an independent baseline for the native one)
-        token_step = h.shape[1] == 1 and not torch.is_grad_enabled() and native
+        token_step = h.shape[1] == 1 and not torch.is_grad_enabled() and native and not self._drops(training)
         next_cache = []
         for index, (attention, feed_forward) in enumerate(self.layers):
             layer_cache = cache[index] if cache is not None and index < len(cache) else None
@@ -335,10 +336,13 @@ class CastleLM(nn.Module):
             return ops.embedding(embedding.weight, x, self.embedding_scale, embedding.padding_idx)
         return embedding(x) * self.embedding_scale
 
+    def _drops(self, training):
+        return training and self.training and self.dropout > 0
+
     def _dropout(self, device, native, training):
         """f(x, residual) -> residual + dropout(x), or x without a residual, with another mask at every call; their numbers are
         drawn in one go from the generator of the device."""
-        if not (training and self.training and self.dropout > 0):
+        if not self._drops(training):
             return lambda x, residual: x if residual is None else residual + x
         if not native:
             return lambda x, residual: F.dropout(x, self.dropout) if residual is None else residual + F.dropout(x, self.dropout)

@@ -34,3 +34,29 @@ def test_a_kept_decoder_follows_the_scale_of_the_embedding():
         assert torch.equal(sample(), want[scale]), scale
         kept = model.__dict__["_kept_decoder"]
         assert torch.equal(sample(), want[scale]) and model.__dict__["_kept_decoder"] is kept   # (and the same scale again needs no other graph)
+
+
+@gpu
+def test_one_token_a_sequence_drops_every_branch():
+    """A model in training, sequences of one token: the outputs of all blocks are dropped.  The dense model of 64 bits with the masks of the same numbers; 1e-4 of
+    the norm, as for longer sequences."""
+    p = 0.5
+    model = make(dropout=p, embedding_scale=2.0)
+    x = torch.randint(0, 300, (7, 1), generator=torch.Generator().manual_seed(6)).to(DEV)
+    torch.manual_seed(9)
+    with torch.no_grad():
+        got = model(x)
+    dense = make(False, embedding_scale=2.0).double()
+    dense.load_state_dict({k: v.double() for k, v in model.state_dict().items()})
+    torch.manual_seed(9)
+    seeds = iter(torch.randint(-2 ** 63, 2 ** 63 - 1, (5, 2), device=DEV))
+    with torch.no_grad():
+        def drop(t):
+            return t * ops.dropout_add(torch.ones(t.shape, device=DEV), None, p, next(seeds)).double()
+
+        h = drop(dense.token_emb(x) * 2)
+        for attention, feed_forward in dense.layers:
+            h = h + drop(attention(h, return_next_cache=False))
+            h = h + drop(feed_forward(h))
+        want = dense.to_logits(dense.final_norm(h))
+    assert (got.double() - want).norm() <= 1e-4 * want.norm()
