@@ -367,7 +367,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kern
 // ---- products of 16-bit operands ------------------------------------------------------------------------------------
 // The frame is that of gemm_wide_kernel (castle_gemm.hip): tiles of the output by workgroups of eight waves, steps of 64 of the contraction straight from memory to LDS into
 // two or three buffers, requested over the end of a tile.  What differs: sizes that are read from device memory, contractions of any length (d and the copied rows are padded with
-// zeros, and behind the end of w's rows or of a row of it what is there is read again), and what becomes of a tile:
+// zeros, behind the end of a row of w zeros are read, and behind the last row that one again), and what becomes of a tile:
 enum { kStats = 0, kGrad = 1, kRowGrad = 2, kWeightGrad = 3 };
 struct ProductArgs {
   const void *a, *b;
@@ -475,7 +475,8 @@ template <int MODE, int BM, int BN, bool PARTS> struct Shape {
 };
 extern __shared__ __attribute__((aligned(16))) unsigned char castle_vocab_lds[];
 
-template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
+// END: rows of w end inside a step (kernels of their own: with the test for it in each, 3000 rows of 256 over 50257 took 392 us instead of 383)
+template <typename T, int MODE, int BM, int BN, bool PARTS, bool END> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
   typedef Shape<MODE, BM, BN, PARTS> S;
   constexpr bool AK = S::kContractA, BKC = S::kContractB;
   constexpr int kStep = PARTS ? kPart : kWideK;   // of the contraction
@@ -541,11 +542,14 @@ template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_
   auto request = [&](int buffer) __attribute__((always_inline)) {
     if (next_item >= last) return;
     ++ahead;
-    // (rows of parts are padded to whole steps)
-    if constexpr (MODE == kRowGrad || (BKC && !PARTS))
+    // behind the end of the contraction d and the copied rows are zeros, and so are those of parts, to whole steps
+    if constexpr (MODE == kRowGrad)
       if (next_k + kStep > K) rb.place((int)a.ldb, K - next_k);
     ra.load(a.lda, lds0 + buffer);
-    rb.load(a.ldb, lds0 + buffer + S::kBytesA);
+    bool end = false;
+    if constexpr (END)
+      if ((end = next_k + kStep > K)) rb.load_end(K - next_k, static_cast<const T*>(a.a) + K, lds0 + buffer + S::kBytesA);   // (what is behind the first copied row)
+    if (!end) rb.load(a.ldb, lds0 + buffer + S::kBytesA);
     next_k += kStep;
     if (--next_steps == 0) {
       next_item += stride;
@@ -835,17 +839,22 @@ template <typename T, int MODE, int BM, int BN, bool PARTS> __global__ __launch_
   }
 }
 
-template <typename T, int MODE, int BM, int BN, bool PARTS> int launch_product_t(const ProductArgs& a, hipStream_t stream) {
+template <typename T, int MODE, int BM, int BN, bool PARTS, bool END> int launch_product_as(const ProductArgs& a, hipStream_t stream) {
   typedef Shape<MODE, BM, BN, PARTS> S;
   static PerDeviceOnce once;
   bool& configured = once.flag();
   if (!configured) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&vocab_product_kernel<T, MODE, BM, BN, PARTS>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&vocab_product_kernel<T, MODE, BM, BN, PARTS, END>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
     configured = true;
   }
   const int64_t items = up(a.M, BM) / BM * (up(a.N, BN) / BN) * a.splits;
-  hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN, PARTS>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
+  hipLaunchKernelGGL((vocab_product_kernel<T, MODE, BM, BN, PARTS, END>), dim3((unsigned)std::min<int64_t>(up(items, 8), 256)), dim3(kWideThreads), S::kLds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -3;
+}
+template <typename T, int MODE, int BM, int BN, bool PARTS> int launch_product_t(const ProductArgs& a, hipStream_t stream) {
+  if constexpr (!PARTS && (MODE == kStats || MODE == kGrad))
+    if (a.K % kWideK != 0) return launch_product_as<T, MODE, BM, BN, PARTS, true>(a, stream);
+  return launch_product_as<T, MODE, BM, BN, PARTS, false>(a, stream);
 }
 // Rows and columns of a workgroup's tile.  Of 64, 128 or 256 rows those with which the fullest CU is done first (us): 1.4 a step and 5 an end of 256 x 256, 0.85 and 3 of 128,
 // 0.56 and 1.6 of 64.  (The loss alone of 128 rows over 32000, 512 wide in bf16, with tiles of 64 rows / 128: 28 / 30 us, 2048 wide 46 / 52; 256 rows 34 / 32, since 500 tiles take two rounds.)
