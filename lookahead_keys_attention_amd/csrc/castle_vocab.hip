@@ -300,11 +300,16 @@ template <typename T> __device__ __forceinline__ float one_factor(const void* dl
   gain = {kDShift, g};
   return ldexpf(1.f, kDShift);
 }
-// kEachLoss: factors of the rows, the largest of them at 2^14 ... 2^15 (fp32: see small_factor_shift)
+// kEachLoss: factors of the rows, the largest finite one at 2^14 ... 2^15 (fp32: see small_factor_shift).  fp16: a factor more than 2^kNear below that has a power of two of its own in
+// d, which brings it there too, until the gradients of the rows have read it: below 2^-14 of d a number of fp16 loses digits, and over a vocabulary most softmax values of a row are about 2^-15.
+// For the gradient of w, which adds over the rows, d then goes to the common power (lower_rows_kernel): what is lost there is 2^-40 of the largest factor.
+// (16384 rows of 512 over 32000, forward and backward: 2360 us, with nine of ten rows to be brought there 2640; without the launch 2380.)
+constexpr int kNear = 4;
 struct FactorArgs {
   const void* dloss;       // [R]
   const int32_t *rank, *tc;
   float* factor;           // [Rp] by rank
+  int32_t* own;            // [Rp] by rank, or nullptr: none has a power of its own
   Gain* gain;
   int R;
 };
@@ -313,18 +318,25 @@ template <typename T> __global__ __launch_bounds__(1024) void factor_kernel(Fact
   const T* g = static_cast<const T*>(a.dloss);
   float most = 0.f;
   for (int r = threadIdx.x; r < a.R; r += 1024)
-    if (a.rank[r] >= 0) most = fmaxf(most, fabsf((float)g[r]));   // fmaxf drops NaNs
+    if (a.rank[r] >= 0 && fabsf((float)g[r]) <= __FLT_MAX__) most = fmaxf(most, fabsf((float)g[r]));   // (not NaN or infinite)
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
   if (lane_id() == 0) s[wave_id()] = most;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 16; ++w) most = fmaxf(most, s[w]);
-  const int shift = sizeof(T) == 4 ? small_factor_shift(most) : most > 0.f && most <= __FLT_MAX__ ? kDShift - __builtin_amdgcn_frexp_expf(most) : 0;
+  const int shift = sizeof(T) == 4 ? small_factor_shift(most) : most > 0.f ? kDShift - __builtin_amdgcn_frexp_expf(most) : 0;
   if (threadIdx.x == 0 && blockIdx.x == 0) *a.gain = {shift, 1.f};
   for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < a.R; r += (int64_t)gridDim.x * 1024) {
     const int rank = a.rank[r];
-    if (rank >= 0) a.factor[rank] = a.tc[rank] >= 0 ? ldexpf((float)g[r], shift) : NAN;
+    if (rank < 0) continue;
+    float f = a.tc[rank] >= 0 ? ldexpf((float)g[r], shift) : NAN;
+    if (a.own != nullptr) {
+      const int below = fabsf(f) > 0.f && fabsf(f) <= __FLT_MAX__ ? kDShift - __builtin_amdgcn_frexp_expf(f) : 0, own = below > kNear ? below : 0;
+      a.own[rank] = own;
+      f = ldexpf(f, own);
+    }
+    a.factor[rank] = f;
   }
 }
 
@@ -337,6 +349,7 @@ struct JoinArgs {
   const float* parts;   // [splits][R][D]
   const int32_t* rank;
   const Gain* gain;
+  const int32_t* own;   // nullptr, or by rank (FactorArgs)
   void* out;
   int splits, D;
   int64_t R;
@@ -356,7 +369,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kern
     const float* p = a.parts + (int64_t)rank * a.D + c;
 #pragma unroll 4
     for (int k = 0; k < splits; ++k) v += *reinterpret_cast<const v4*>(p + k * a.R * a.D);
-    const int shift = a.gain->shift;
+    const int shift = a.gain->shift + (a.own != nullptr ? a.own[rank] : 0);
     const float gain = a.gain->gain;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -shift) * gain;
@@ -435,6 +448,35 @@ template <typename T, bool KC, int FREE> struct PartsOperand : WideOperand<T, KC
 // of blocks).  (As rows of V, 128 bytes here and there, 64 KB and more apart: the same time where the caches hold a band of columns.)
 template <bool PARTS> constexpr int kBlock = PARTS ? kPart : 64;          // rows and columns
 template <bool PARTS> constexpr int kBlockRow = PARTS ? 3 * kPart : 64;   // numbers of a row
+// Rows of d from a power of two of their own to the common one; workgroups to each row of blocks, most of which have none to do.
+struct LowerArgs {
+  fp16_t* d;   // [row of blocks][ldc / 64][64][64]
+  const int32_t* own;
+  const int* count;
+  int64_t ldc;
+};
+__global__ __launch_bounds__(kThreads) void lower_rows_kernel(LowerArgs a) {
+  constexpr int B = kBlock<false>, PIECES = B * B / 8, EACH = PIECES / kThreads;   // of a thread, the same rows in every block
+  const int64_t first = (int64_t)blockIdx.x * B;
+  const int count = *a.count, blocks = (int)(a.ldc / B);
+  int own[EACH];
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int64_t r = first + (k * kThreads + threadIdx.x) / (B / 8);
+    own[k] = r < count ? a.own[r] : 0;
+  }
+  for (int b = blockIdx.y; b < blocks; b += gridDim.y)
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      if (own[k] == 0) continue;
+      frag_mem<fp16_t>* p = reinterpret_cast<frag_mem<fp16_t>*>(a.d + first * a.ldc + (int64_t)b * (B * B) + 8 * (k * kThreads + threadIdx.x));
+      vec<float, 8> v = __builtin_convertvector((frag<fp16_t>)*p, vec<float, 8>);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], -own[k]);
+      *p = __builtin_convertvector(v, frag<fp16_t>);
+    }
+}
+
 template <typename T, bool KC, int FREE, bool PARTS> struct BlockOperand : WideOperand<T, KC, FREE> {
   typedef WideOperand<T, KC, FREE> W;
   static constexpr int N = kOperandLoads<KC, FREE, PARTS>, B = kBlock<PARTS>, BR = kBlockRow<PARTS>;
@@ -981,6 +1023,7 @@ struct Fwd {
 struct Bwd {
   char *xc, *wc;
   float* factor;
+  int32_t* own;
   Gain* gain;
   char* d;
   float *row_parts, *weight_parts;
@@ -988,6 +1031,7 @@ struct Bwd {
     xc = c.take<char>(es == 4 ? p.Rp * p.Dp * operand_bytes(es) : 0);
     wc = c.take<char>(es == 4 ? (int64_t)a.V * p.Dp * operand_bytes(es) : 0);
     factor = c.take<float>(p.Rp);
+    own = c.take<int32_t>(p.Rp);
     gain = c.take<Gain>(1);
     d = c.take<char>(p.Rp * p.ldc * operand_bytes(es));
     row_parts = c.take<float>(need_x ? (int64_t)p.rows.ranges * a.R * a.D : 0);
@@ -1092,8 +1136,9 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
   const Bwd b(a, p, es, dx != nullptr, dw != nullptr, cw);
   char* const xc = es == 4 ? b.xc : s.xc;
   int rc = es == 4 ? launch_split(a, p, &s.head->count, s.rank, b.xc, b.wc, stream) : 0;
+  int32_t* const own = dtype == 2 && a.reduction == kEachLoss ? b.own : nullptr;
   if (rc == 0 && a.reduction == kEachLoss) {
-    const FactorArgs f = {dloss, s.rank, s.tc, b.factor, b.gain, a.R};
+    const FactorArgs f = {dloss, s.rank, s.tc, b.factor, own, b.gain, a.R};
     rc = by_tensor_type(dtype, [&](auto t) {
       hipLaunchKernelGGL((factor_kernel<decltype(t)>), dim3(std::min<unsigned>(64, (unsigned)(up(a.R, 1024) / 1024))), dim3(1024), 0, stream, f);
       return launched();
@@ -1142,6 +1187,12 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
       x.add = i > 0;
       rc = launch_product<kRowGrad>(x, p.rows.tile, dtype, stream);
     }
+    if (rc == 0 && dw != nullptr && own != nullptr) {
+      const int64_t rows = p.Rp / kBlock<false>;
+      hipLaunchKernelGGL(lower_rows_kernel, dim3((unsigned)rows, (unsigned)std::max<int64_t>(1, std::min(p.ldc / kBlock<false>, 1024 / rows))), dim3(kThreads), 0, stream,
+                         LowerArgs{reinterpret_cast<fp16_t*>(b.d), own, &s.head->count, p.ldc});
+      rc = launched();
+    }
     if (rc == 0 && dw != nullptr) {
       ProductArgs w = g;
       w.a = b.d;
@@ -1157,11 +1208,11 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
       w.out = w.splits > 1 ? b.weight_parts : static_cast<float*>(w.c);
       rc = launch_product<kWeightGrad>(w, p.weights.tile, dtype, stream);
       if (rc == 0 && w.splits > 1)
-        rc = join({b.weight_parts, nullptr, b.gain, w.c, w.splits, a.D, n, &s.head->count, p.step});
+        rc = join({b.weight_parts, nullptr, b.gain, nullptr, w.c, w.splits, a.D, n, &s.head->count, p.step});
     }
   }
   if (rc != 0 || dx == nullptr) return rc;
-  return join({b.row_parts, s.rank, b.gain, dx, ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.rows.ranges), a.D, a.R, nullptr, p.step});
+  return join({b.row_parts, s.rank, b.gain, own, dx, ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.rows.ranges), a.D, a.R, nullptr, p.step});
 }
 
 }  // namespace castle

@@ -27,3 +27,70 @@ def test_a_class_of_minus_infinity_has_no_weight(D, dtype):
     within(loss.detach(), *ref[0], dtype, "loss")
     within(dw[rest], *ref[2], dtype, "dw")
     assert not dw[gone].any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_whose_losses_count_very_differently(dtype):
+    """Each row's gradient is as exact as the row's own factor allows, however small that is beside the others', an infinite one among them; a table of one sign, so that what many unlikely
+    classes add is a large part of it.  d of a row lies in the type under a factor of 2^10 at least (fp16), so what is below its normal numbers is off by 2^-25 / 2^10 of the row's own
+    factor; the table's gradient has that of the largest, twice: d is rounded again where it goes to the common factor."""
+    R, V, D = 150, 9000, 64
+    g = torch.Generator().manual_seed(21)
+    x, w, target = inputs(R, V, D, dtype, 21)
+    w = (w.float().abs() + 0.25).to(dtype)
+    x = (x.float() / 16).to(dtype)
+    low, high = (-9, 14) if dtype is torch.float16 else (-60, 30)
+    dloss = (2.0 ** torch.randint(low, high + 1, (R,), generator=g).double() * (1 + torch.rand(R, generator=g).double())).to(dtype).to(DEV)
+    dloss[:2] = torch.tensor([2.0 ** low, 2.0 ** high])
+    target[5] = -100
+    keep = target != -100
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    each = ops.linear_cross_entropy(*leaves, target, "none")
+    dx, dw = torch.autograd.grad(each, leaves, dloss, retain_graph=True)
+    for r in range(R):   # a row by itself: its factor is the largest
+        if keep[r]:
+            (_, _), (ref, bound), _ = reference(x[r:r + 1].detach(), w.detach(), target[r:r + 1], "none", dloss[r:r + 1], -100, dtype)
+            if dtype is torch.float16:
+                bound = bound + 2.0 ** -35 * dloss[r].double().abs() * w.detach().double().abs().sum(0)
+            within(dx[r:r + 1], ref, bound, dtype, (r, dloss[r].item()))
+    assert not dx[5].any()
+    (_, _), _, (ref, bound) = reference(x.detach(), w.detach(), target, "none", dloss, -100, dtype)
+    if dtype is torch.float16:
+        bound = bound + 2.0 ** -25 / 2.0 ** 14 * dloss[keep].double().abs().max() * x.detach()[keep].double().abs().sum(0)
+    within(dw, ref, bound, dtype, "dw")
+    # alone of all, one gradient without the other: the same bits
+    assert torch.equal(torch.autograd.grad(each, leaves[1], dloss, retain_graph=True)[0], dw)
+    assert torch.equal(torch.autograd.grad(each, leaves[0], dloss, retain_graph=True)[0], dx)
+    # an infinite factor is its row's alone, as far as the rows' gradients go
+    dloss[3] = float("inf")
+    again, = torch.autograd.grad(each, leaves[0], dloss)
+    others = torch.arange(R, device=DEV) != 3
+    assert not again[3].isfinite().any()
+    for r in (0, 1, 40, 149):
+        (_, _), (ref, bound), _ = reference(x[r:r + 1].detach(), w.detach(), target[r:r + 1], "none", dloss[r:r + 1], -100, dtype)
+        if dtype is torch.float16:
+            bound = bound + 2.0 ** -35 * dloss[r].double().abs() * w.detach().double().abs().sum(0)
+        within(again[r:r + 1], ref, bound, dtype, (r, "beside an infinite one"))
+    assert again[others].isfinite().all()
+
+
+@gpu
+def test_rows_whose_losses_count_very_differently_in_several_pieces():
+    """The same in fp16 over a vocabulary of two pieces of d."""
+    R, V, D, dtype = 4200, 140001, 16, torch.float16
+    g = torch.Generator().manual_seed(22)
+    x, w, target = inputs(R, V, D, dtype, 22)
+    w = (w.float().abs() + 0.25).to(dtype)
+    dloss = (2.0 ** torch.randint(-9, 15, (R,), generator=g).double()).to(dtype).to(DEV)
+    dloss[::3] = 0
+    target[::7] = -100
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(*leaves, target, "none"), leaves, dloss)
+    x, w = x.detach(), w.detach()
+    for r in [int(dloss[r] != 0) and r for r in (1, 2, 4, 64, 100, 2000, 4199)]:
+        _, (ref, bound), _ = reference(x[r:r + 1], w, target[r:r + 1], "none", dloss[r:r + 1], -100, dtype)
+        within(dx[r:r + 1], ref, bound + 2.0 ** -35 * dloss[r].double().abs() * w.double().abs().sum(0), dtype, (r, dloss[r].item()))
+    assert not dx[::3].any() and not dx[::7].any()
+    _, _, (ref, bound) = reference(x, w, target, "none", dloss, -100, dtype)
+    within(dw, ref, bound + 2.0 ** -25 / 2.0 ** 14 * dloss.double().abs().max() * x[target != -100].double().abs().sum(0), dtype, "dw")
