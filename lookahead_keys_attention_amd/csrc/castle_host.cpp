@@ -1222,7 +1222,7 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
 
 Tensor embedding(const Tensor& weight, const Tensor& index, double scale) {
   const c10::DeviceGuard guard(weight.device());
-  if (!wants_graph({weight}) || index.numel() == 0) return embedding_op(weight, index, scale, -1);
+  if (!wants_graph({weight}) || index.numel() == 0) return embedding_autograd(weight, index, scale, -1);
   return EmbeddingFn::apply(weight, index, scale);
 }
 

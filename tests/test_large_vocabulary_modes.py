@@ -3,7 +3,7 @@ models, empty batches."""
 import pytest
 import torch
 
-from lookahead_keys_attention_amd import CastleLM, ops
+from lookahead_keys_attention_amd import CastleLM, _native, ops
 
 DEV = "cuda:0"
 gpu = pytest.mark.gpu
@@ -60,3 +60,15 @@ def test_one_token_a_sequence_drops_every_branch():
             h = h + drop(feed_forward(h))
         want = dense.to_logits(dense.final_norm(h))
     assert (got.double() - want).norm() <= 1e-4 * want.norm()
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1.0, 3.0])
+def test_no_tokens_at_all_still_record_a_graph(scale):
+    """The embedding of an empty batch hangs on its table, whose gradient is zeros."""
+    table = torch.randn(30, 16, device=DEV, requires_grad=True)
+    for shape in ((0, 5), (4, 0)):
+        y = _native.host().embedding(table, torch.zeros(shape, dtype=torch.long, device=DEV), scale)
+        assert y.shape == (*shape, 16) and y.requires_grad
+        grad, = torch.autograd.grad(y.sum(), table)
+        assert grad.shape == table.shape and not grad.any()
