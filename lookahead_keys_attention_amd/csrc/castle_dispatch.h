@@ -5,6 +5,13 @@
 
 namespace castle {
 
+// Grid of n workgroups (y of them each) whose kernel asks block_of_many() for its number.  A dispatch counts the threads of a dimension in 32 bits, and those past 2^32 are left out
+// without an error: more than 2^21 workgroups stand in x and z, some behind the last one among them.
+inline dim3 many_blocks(int64_t n, unsigned y = 1) {
+  constexpr int64_t kMost = 1 << 21;
+  return n <= kMost ? dim3((unsigned)n, y) : dim3((unsigned)kMost, y, (unsigned)((n + kMost - 1) / kMost));
+}
+
 // f(compute type, tensor type): bf16 tensors are converted to fp16 on load (exact inside the fp16 range) and every
 // operand produced inside the kernels is fp16, unless bf16_operands asks for bf16 MFMA operands
 template <typename F> int by_type(int dtype, bool bf16_operands, F&& f) {

@@ -40,7 +40,7 @@ template <typename T, bool RESIDUAL> __global__ __launch_bounds__(kThreads) void
   const uint64_t key = (uint64_t)a.seed[0], at = (uint64_t)a.seed[1];
   const T *x = static_cast<const T*>(a.x), *res = static_cast<const T*>(a.residual);
   T* y = static_cast<T*>(a.y);
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, first = i * 8;
+  const int64_t i = block_of_many() * kThreads + threadIdx.x, first = i * 8;
   if (first >= a.n) return;
   if (first + 8 <= a.n) {
     const frag<T> v = *reinterpret_cast<const frag_mem<T>*>(x + first);
@@ -70,8 +70,8 @@ int launch_dropout(const DropoutArgs& a, int dtype, hipStream_t stream) {
   const int64_t blocks = ((a.n + 7) / 8 + kThreads - 1) / kThreads;
   return by_tensor_type(dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.residual != nullptr) hipLaunchKernelGGL((dropout_kernel<T, true>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+    if (a.residual != nullptr) hipLaunchKernelGGL((dropout_kernel<T, true>), many_blocks(blocks), dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((dropout_kernel<T, false>), many_blocks(blocks), dim3(kThreads), 0, stream, a);
     return hipGetLastError() == hipSuccess ? 0 : -3;
   });
 }

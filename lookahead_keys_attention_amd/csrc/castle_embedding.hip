@@ -28,8 +28,9 @@ __device__ __forceinline__ int64_t token_of(const TokenRows& t, int64_t r) {
 
 // N elements at a time: 16 bytes, wherever they begin, or one element where a row has fewer.  Piece i of a row: the last one ends with the row, and reads and writes what the
 // one before it does as well (single elements where rows are no whole pieces: 5569 tokens of 828 bf16 over 6556, forward and gradient, 121 us, so 58).
-template <int N> __device__ __forceinline__ int column(int i, int D) { return min(i * N, D - N); }
-template <int N> __device__ __forceinline__ int pieces_of(int D) { return (D + N - 1) / N; }
+// (Widths and vocabularies reach 2^31 - 1: what is a little more than they are is formed in 32 bits without a sign, or in 64.)
+template <int N> __device__ __forceinline__ int column(int i, int D) { return (int)min((uint32_t)i * N, (uint32_t)D - N); }
+template <int N> __host__ __device__ __forceinline__ int pieces_of(int D) { return (int)(((uint32_t)D + N - 1) / N); }
 template <typename T, int N> struct Anywhere { typedef vec<T, N> type __attribute__((aligned(sizeof(T)))); };
 template <typename T, int N> __device__ __forceinline__ vec<float, N> load_n(const T* p) {
   const vec<T, N> v = *reinterpret_cast<const typename Anywhere<T, N>::type*>(p);
@@ -46,7 +47,7 @@ template <int N> __device__ __forceinline__ vec<float, N> fill_n(float x) {
 // LPR lanes to a row
 template <typename T, int N, int LPR> __global__ __launch_bounds__(kThreads) void embedding_kernel(EmbeddingArgs a) {
   constexpr int RPG = kThreads / LPR;
-  const int64_t r = (int64_t)blockIdx.x * RPG + threadIdx.x / LPR;
+  const int64_t r = block_of_many() * RPG + threadIdx.x / LPR;
   if (r >= a.tokens.rows) return;
   const int64_t t = token_of(a.tokens, r);
   const bool there = t >= 0 && t < a.V;
@@ -306,7 +307,7 @@ template <int N, typename F, typename G> __device__ __forceinline__ void over_wa
 }
 template <typename T, int N> __global__ __launch_bounds__(kThreads) void run_sum_kernel(SumArgs a) {
   __shared__ float s_acc[(kWaves - 1) * N * 64];
-  const int64_t first = (int64_t)blockIdx.x * kRun, i = first + threadIdx.x;
+  const int64_t piece = block_of_many(), first = piece * kRun, i = first + threadIdx.x;
   if (blockIdx.y == 0 && threadIdx.x < kRun && i < a.rows) {   // where a token ends and the next one begins
     const uint32_t k = a.keys[i], before = i > 0 ? a.keys[i - 1] : k + 1;
     if (k != before) {
@@ -319,7 +320,7 @@ template <typename T, int N> __global__ __launch_bounds__(kThreads) void run_sum
   const uint32_t key = a.keys[first];
   if (key >= (uint32_t)a.V || a.keys[first + kRun - 1] != key) return;
   over_waves<N>(s_acc, a.D, 64 * blockIdx.y, 64 * gridDim.y, [&](int c) { return sum_places<T, N>(a, first + wave_id(), first + kRun, kWaves, c); },
-                [&](int c, vec<float, N> v) { store_n<float, N>(a.parts + (int64_t)blockIdx.x * a.D + c, v); });
+                [&](int c, vec<float, N> v) { store_n<float, N>(a.parts + piece * a.D + c, v); });
 }
 
 constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that one wave, or part of one, sums by itself
@@ -327,11 +328,12 @@ constexpr int kMaxRowsPerGroup = 32, kFew = 8;   // kFew: tokens of a row that o
 template <typename T, int N, int LPR, int AT> __global__ __launch_bounds__(kThreads) void table_grad_kernel(SumArgs a) {
   __shared__ Range s_range[kMaxRowsPerGroup];
   __shared__ float s_acc[(kWaves - 1) * N * 64];
-  // Rows gridDim.x apart: the frequent tokens of a vocabulary stand together (a workgroup to 31 rows in a row: 162 us for 16384 tokens of 512 bf16 over 32000, the one of
+  // Rows G apart: the frequent tokens of a vocabulary stand together (a workgroup to 31 rows in a row: 162 us for 16384 tokens of 512 bf16 over 32000, the one of
   // the first tokens alone with all of it).
-  const int G = gridDim.x, rows = ((int)a.V - (int)blockIdx.x + G - 1) / G, wave = wave_id();
+  const uint32_t G = gridDim.x * gridDim.z, first = (uint32_t)block_of_many();
+  const int rows = (int)(((uint32_t)a.V - first + G - 1) / G), wave = wave_id();   // (none of a workgroup behind the last one)
   // (Bounds by a search of each workgroup among the keys: 14 trips to memory for 16384 tokens, 21 us instead of 16.)
-  if ((int)threadIdx.x < rows) s_range[threadIdx.x] = a.ranges[blockIdx.x + threadIdx.x * G];
+  if ((int)threadIdx.x < rows) s_range[threadIdx.x] = a.ranges[first + threadIdx.x * G];
   __syncthreads();
   auto write = [&](int v, int c, vec<float, N> acc) { store_n<T, N>(static_cast<T*>(a.dw) + (int64_t)v * a.D + c, acc * a.scale); };
   for (int k = threadIdx.x / LPR; k < rows; k += kThreads / LPR) {
@@ -353,7 +355,7 @@ template <typename T, int N, int LPR, int AT> __global__ __launch_bounds__(kThre
       }
 #pragma unroll
       for (int u = 0; u < AT; ++u)
-        if (u == 0 || i + u * LPR < pieces_of<N>(a.D)) write(blockIdx.x + k * G, c[u], acc[u]);
+        if (u == 0 || i + u * LPR < pieces_of<N>(a.D)) write(first + k * G, c[u], acc[u]);
     }
   }
   for (int k = 0; k < rows; ++k) {   // by all waves: places in front of the first whole piece, whole pieces, places behind
@@ -366,7 +368,7 @@ template <typename T, int N, int LPR, int AT> __global__ __launch_bounds__(kThre
 #pragma unroll 4
       for (int64_t p = c0 + wave; p < c1; p += kWaves) acc += load_n<float, N>(a.parts + p * a.D + c);
       return acc + sum_places<T, N>(a, c1 * kRun + wave, e, kWaves, c);
-    }, [&](int c, vec<float, N> acc) { write(blockIdx.x + k * G, c, acc); });
+    }, [&](int c, vec<float, N> acc) { write(first + k * G, c, acc); });
   }
 }
 
@@ -388,10 +390,10 @@ int launch_embedding(const EmbeddingArgs& a, int dtype, hipStream_t stream) {
     using T = decltype(t);
     auto go = [&](auto lpr) {
       constexpr int LPR = decltype(lpr)::value, rows = kThreads / LPR;
-      hipLaunchKernelGGL((embedding_kernel<T, n.value, LPR>), dim3((unsigned)((a.tokens.rows + rows - 1) / rows)), dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((embedding_kernel<T, n.value, LPR>), many_blocks((a.tokens.rows + rows - 1) / rows), dim3(kThreads), 0, stream, a);
       return launched();
     };
-    const int pieces = (a.D + n.value - 1) / n.value;
+    const int pieces = pieces_of<n.value>(a.D);
     if (pieces <= 16) return go(std::integral_constant<int, 16>());
     if (pieces <= 32) return go(std::integral_constant<int, 32>());
     return go(std::integral_constant<int, 64>());
@@ -465,9 +467,9 @@ int launch_sorted_grad(const SortedGradArgs& g, int dtype, hipStream_t stream) {
   const SumArgs s = {keys[sorted], places[sorted], ranges, g.tokens.rows, g.dy, g.dw, parts, g.V, g.D, p.rows_per_group, g.scale};
   return by_pieces(dtype, g.D, [&](auto t, auto n) {
     using T = decltype(t);
-    const int pieces = (g.D + n.value - 1) / n.value;
-    hipLaunchKernelGGL((run_sum_kernel<T, n.value>), dim3((unsigned)((s.rows + kRun - 1) / kRun), std::min(8, (pieces + 63) / 64)), dim3(kThreads), 0, stream, s);
-    const dim3 grid((unsigned)((g.V + p.rows_per_group - 1) / p.rows_per_group));
+    const int pieces = pieces_of<n.value>(g.D);
+    hipLaunchKernelGGL((run_sum_kernel<T, n.value>), many_blocks((s.rows + kRun - 1) / kRun, std::min(8, (pieces + 63) / 64)), dim3(kThreads), 0, stream, s);
+    const dim3 grid = many_blocks(((int64_t)g.V + p.rows_per_group - 1) / p.rows_per_group);
     if (pieces <= 16) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 16, 1>), grid, dim3(kThreads), 0, stream, s);
     else if (pieces <= 32) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 32, 1>), grid, dim3(kThreads), 0, stream, s);
     else if (pieces <= 64) hipLaunchKernelGGL((table_grad_kernel<T, n.value, 64, 1>), grid, dim3(kThreads), 0, stream, s);

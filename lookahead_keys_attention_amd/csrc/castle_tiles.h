@@ -60,6 +60,8 @@ template <typename T> __host__ __device__ constexpr int lds_ld_tr(int cols) {
   return sizeof(T) == 2 && cols == 128 ? 152 : lds_ld<T>(cols);
 }
 
+// number of this workgroup in a grid of many_blocks (castle_dispatch.h)
+__device__ __forceinline__ int64_t block_of_many() { return (int64_t)blockIdx.z * gridDim.x + blockIdx.x; }
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
 // The wave index is read through readfirstlane so that the compiler knows it is uniform:
 // every branch that depends on it then becomes a scalar branch.  This matters for

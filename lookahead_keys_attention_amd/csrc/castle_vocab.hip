@@ -186,11 +186,12 @@ template <bool ANY, int N> __device__ __forceinline__ Parts<N> split_in_three(ve
   return r;
 }
 // x in the first x_groups workgroups, w in the others
-__global__ __launch_bounds__(kThreads) void split_rows_kernel(SplitArgs x_args, SplitArgs w_args, int x_groups) {
-  const bool of_x = (int)blockIdx.x < x_groups;
+__global__ __launch_bounds__(kThreads) void split_rows_kernel(SplitArgs x_args, SplitArgs w_args, int64_t x_groups) {
+  const int64_t group = block_of_many();
+  const bool of_x = group < x_groups;
   const SplitArgs& a = of_x ? x_args : w_args;
   const int per = a.Dp / 8;
-  const int64_t i = (int64_t)(blockIdx.x - (of_x ? 0 : x_groups)) * kThreads + threadIdx.x, r = i / per;
+  const int64_t i = (group - (of_x ? 0 : x_groups)) * kThreads + threadIdx.x, r = i / per;
   if (r >= (a.rank != nullptr ? up(a.rows, 64) : a.rows)) return;
   const int c = (int)(i - r * per) * 8;
   auto put = [&](int64_t row, vec<float, 8> x) __attribute__((always_inline)) {
@@ -358,7 +359,7 @@ struct JoinArgs {
 };
 template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kernel(JoinArgs a) {
   typedef vec<float, 4> v4;
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t i = block_of_many() * kThreads + threadIdx.x;
   const int per = a.D / 4;
   if (i >= a.R * per) return;
   const int64_t r = i / per;
@@ -1064,8 +1065,8 @@ int launch_gather(const RowArgs& a, int dtype, hipStream_t stream) {
 int launch_split(const VocabArgs& a, const Plan& p, const int* count, const int32_t* rank, void* xc, void* wc, hipStream_t stream) {
   const SplitArgs x = {static_cast<const float*>(a.x), a.ld_x, a.R, a.D, p.Dp, rank, count, static_cast<bf16_t*>(xc)};
   const SplitArgs w = {static_cast<const float*>(a.w), a.ld_w, a.V, a.D, p.Dp, nullptr, nullptr, static_cast<bf16_t*>(wc)};
-  auto groups = [&](int64_t rows) { return up(rows * (p.Dp / 8), kThreads) / kThreads; };   // (at most 2^29 of x and 2^27 of w)
-  hipLaunchKernelGGL(split_rows_kernel, dim3((unsigned)(groups(p.Rp) + groups(a.V))), dim3(kThreads), 0, stream, x, w, (int)groups(p.Rp));
+  auto groups = [&](int64_t rows) { return up(rows * (p.Dp / 8), kThreads) / kThreads; };
+  hipLaunchKernelGGL(split_rows_kernel, many_blocks(groups(p.Rp) + groups(a.V)), dim3(kThreads), 0, stream, x, w, groups(p.Rp));
   return launched();
 }
 
@@ -1146,7 +1147,7 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
   }
   auto join = [&](const JoinArgs& j) {
     return by_tensor_type(dtype, [&](auto t) {
-      hipLaunchKernelGGL((join_rows_kernel<decltype(t)>), dim3((unsigned)(up(j.R * j.D / 4, kThreads) / kThreads)), dim3(kThreads), 0, stream, j);
+      hipLaunchKernelGGL((join_rows_kernel<decltype(t)>), many_blocks(up(j.R * j.D / 4, kThreads) / kThreads), dim3(kThreads), 0, stream, j);
       return launched();
     });
   };
