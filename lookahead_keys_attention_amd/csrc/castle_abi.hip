@@ -164,7 +164,7 @@ castle::FwdWorkspace carve(void* base, void* state, const Geometry& g) {
 
 }  // namespace
 
-constexpr int64_t kMaxRows = (int64_t)1 << 30;   // rows of a launch: the grids stay below 2^31 workgroups
+constexpr int64_t kMaxRows = (int64_t)1 << 30;   // rows of a launch: their numbers stay within 31 bits
 
 extern "C" {
 

@@ -32,7 +32,7 @@ template <typename T, int LPR, int NP> __global__ __launch_bounds__(kThreads) vo
   typedef vec<T, V> vt;
   typedef vec<float, V> vf;
   const int lane = lane_id(), sub = lane % LPR, pieces = a.D / V;
-  const int64_t row = ((int64_t)blockIdx.x * kRowWaves + wave_id()) * RPW + lane / LPR;
+  const int64_t row = (block_of_many() * kRowWaves + wave_id()) * RPW + lane / LPR;
   if (row >= a.rows) return;
   const int64_t at = row * a.D;
   vf x[NP], w[NP];
@@ -249,7 +249,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void ce_bwd_kernel(
   typedef vec<T, V> vt;
   typedef vec<float, V> vf;
   const int lane = lane_id(), pieces = a.V / V;
-  const int64_t row = (int64_t)blockIdx.x * kRowWaves + wave_id();
+  const int64_t row = block_of_many() * kRowWaves + wave_id();
   if (row >= a.rows) return;
   const int64_t t = target_of(a, row), at = row * a.V;
   const bool counts = t != -100;
@@ -274,7 +274,8 @@ template <typename T> __global__ __launch_bounds__(kThreads) void embedding_grad
   typedef vec<float, V> vf;
   __shared__ int s_list[kChunk], s_wave[kRowWaves];
   extern __shared__ float s_row[];   // [D]
-  const int lane = lane_id(), wave = wave_id(), v = blockIdx.x, pieces = a.D / V;
+  const int lane = lane_id(), wave = wave_id(), v = (int)block_of_many(), pieces = a.D / V;
+  if (v >= a.V) return;
   const int64_t r0 = (int64_t)blockIdx.y * kChunk, r1 = r0 + kChunk < a.rows ? r0 + kChunk : a.rows;
   int found = 0;
   for (int64_t base = r0; base < r1; base += kThreads) {
@@ -335,7 +336,7 @@ int launch_norm(const NormArgs& a, int dtype, hipStream_t stream) {
     using T = decltype(t);
     return by_row_length(a.D / elem_traits<T>::vec16, [&](auto lpr, auto np) {
       constexpr int rows = kRowWaves * (64 / lpr.value);
-      hipLaunchKernelGGL((norm_kernel<T, lpr.value, np.value>), dim3((unsigned)((a.rows + rows - 1) / rows)), dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((norm_kernel<T, lpr.value, np.value>), many_blocks((a.rows + rows - 1) / rows), dim3(kThreads), 0, stream, a);
       return launched();
     });
   });
@@ -400,7 +401,7 @@ int launch_cross_entropy(const CrossEntropyArgs& a, void* loss, float* inv_count
 int launch_cross_entropy_bwd(const CrossEntropyArgs& a, const void* grad, const float* inv_count, void* dlogits, int dtype, hipStream_t stream) {
   return by_tensor_type(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((ce_bwd_kernel<T>), dim3((unsigned)((a.rows + kRowWaves - 1) / kRowWaves)), dim3(kThreads), 0, stream, a, static_cast<const T*>(grad),
+    hipLaunchKernelGGL((ce_bwd_kernel<T>), many_blocks((a.rows + kRowWaves - 1) / kRowWaves), dim3(kThreads), 0, stream, a, static_cast<const T*>(grad),
                        inv_count, static_cast<T*>(dlogits));
     return launched();
   });
@@ -411,7 +412,7 @@ int launch_embedding_grad(const EmbeddingGradArgs& a, void* dw, int dtype, hipSt
   return by_tensor_type(dtype, [&](auto t) {
     using T = decltype(t);
     const int chunks = embedding_grad_chunks(a.rows);
-    hipLaunchKernelGGL((embedding_grad_kernel<T>), dim3(a.V, chunks), dim3(kThreads), a.D * sizeof(float), stream, a);
+    hipLaunchKernelGGL((embedding_grad_kernel<T>), many_blocks(a.V, chunks), dim3(kThreads), a.D * sizeof(float), stream, a);
     if (launched() != 0) return -3;
     return launch_part_sum(a.part, chunks, (int64_t)a.V * a.D, dw, dtype, stream);
   });

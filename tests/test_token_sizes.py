@@ -1,8 +1,10 @@
-"""Token embedding and dropout (ops.embedding, ops.dropout_add) at the ends of their ranges of sizes."""
+"""Token embedding, dropout and the operators on rows at the ends of their ranges of sizes."""
+import ctypes
+
 import pytest
 import torch
 
-from lookahead_keys_attention_amd import ops
+from lookahead_keys_attention_amd import _native, ops
 from test_tokens import kept
 
 DEV = "cuda:0"
@@ -65,3 +67,49 @@ def test_dropout_of_more_elements_than_a_launch_has_threads_for(room):
         assert torch.equal(y[first:first + count].cpu(), want), first
     for part in y.split(1 << 30):
         assert abs(part.count_nonzero().item() / len(part) - (1 - p)) <= 8 * (p * (1 - p) / len(part)) ** 0.5
+
+
+@gpu
+def test_norm_of_more_rows_than_a_launch_has_threads_for(room):
+    """2^28 rows of sixteen lanes each: those behind them are normalised as well."""
+    room(16)
+    few = torch.randn(1 << 10, 8, generator=torch.Generator().manual_seed(2)).bfloat16().to(DEV)
+    x, weight = few.repeat((1 << 18) + 1, 1), torch.full((8,), 0.5, dtype=torch.bfloat16, device=DEV)
+    _native.host()
+    want = torch.ops.castle_hip.rms_norm(few, weight, 1e-6)
+    got = torch.ops.castle_hip.rms_norm(x, weight, 1e-6)
+    for a, b in zip(got, want):
+        assert bool((a.view(-1, *b.shape) == b).all())
+
+
+@gpu
+def test_gradient_of_the_loss_of_more_rows_than_a_launch_has_threads_for(room):
+    """2^26 rows of a wave each."""
+    room(12)
+    few = torch.randn(1 << 10, 8, generator=torch.Generator().manual_seed(3)).to(DEV)
+    logits, n = few.repeat((1 << 16) + 1, 1)[None].requires_grad_(), (1 << 26) + (1 << 10)
+    target = torch.arange(n, device=DEV)[None] % 8
+    grad, = torch.autograd.grad(_native.host().cross_entropy(logits, target), logits, torch.tensor(float(n), device=DEV))
+    want = torch.softmax(few.double(), 1)
+    want[range(1 << 10), torch.arange(1 << 10) % 8] -= 1
+    # (softmax, the factor and their product in 32 bits, exp with what its argument is off by: 32 steps of 2^-24)
+    assert bool(((grad.view(-1, 1 << 10, 8) - want.float()).abs() <= 32 * 2.0 ** -24).all())
+
+
+@gpu
+def test_gradient_without_a_sort_of_a_vocabulary_beyond_the_threads_of_a_launch(room):
+    """2^24 rows of the table, a workgroup to each, are 2^32 threads."""
+    room(4)
+    V, D, tokens = (1 << 24) + 8, 8, torch.tensor([0, 1 << 24, (1 << 24) + 7], device=DEV)
+    lib, i, i64, vp = _native.lib(), ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
+    size, call = lib.castle_embedding_grad_workspace_bytes, lib.castle_embedding_grad
+    size.restype, size.argtypes = i64, [i64, i, i, i]
+    call.argtypes = [vp, vp, i64, i64, i64, i, i, vp, i, vp, i64, vp]
+    dy, dw = torch.randn(3, D, device=DEV).bfloat16(), torch.ones(V, D, dtype=torch.bfloat16, device=DEV)
+    nbytes = size(3, V, D, 1)
+    ws = torch.full((nbytes,), 0x3F, dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    assert call(dy.data_ptr(), tokens.data_ptr(), 3, 3, 3, V, D, dw.data_ptr(), 1, ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream) == 0
+    want = torch.zeros_like(dw)
+    want[tokens] = dy
+    assert torch.equal(dw, want)
