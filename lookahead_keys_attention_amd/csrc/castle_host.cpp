@@ -1190,9 +1190,12 @@ Tensor embedding_autograd(const Tensor& weight, const Tensor& index, double scal
   return ScaledEmbeddingFn::apply(weight, index, scale, padding_idx);
 }
 
-// the token embedding of a model, its gradient without a sort where the vocabulary is small: up to kFewTokens tokens times vocabulary rows (us of
-// both by GPU and host, without / with the sort: 16384 tokens of 512 bf16 over 1024 43 / 52, over 4096 124 / 50, 65536 over 1024 128 / 52)
-constexpr int64_t kFewTokens = (int64_t)1 << 24;
+// The token embedding of a model, its gradient without a sort where the vocabulary is small: that kernel goes over tokens times vocabulary, and writes and reads a table of partial sums
+// in 32 bits.  Forward and gradient by GPU and host, us, without / with the sort: 16384 tokens of 512 bf16 over 1024 rows 43 / 52, over 4096 124 / 50, 65536 over 1024 128 / 52; few tokens over
+// many rows: 512 over 4096 50 / 56, 1024 over 16384 54 / 54 (fp32 56 / 37), 128 over 131072 292 / 54; 2048 wide, 512 over 4096 53 / 56, 4096 over 4096 85 / 57, 128 over 131072 1103 / 132,
+// with 1 GB of partial sums.
+constexpr int64_t kFewTokens = (int64_t)1 << 24;   // tokens times rows
+constexpr int64_t kFewTableRows = 4096, kSmallTable = (int64_t)1 << 21;   // elements
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& index, double scale) {
     const at::AutoDispatchBelowADInplaceOrView below;
@@ -1210,7 +1213,8 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t V = ctx->saved_data["vocabulary"].toInt(), D = g[0].size(-1), R = index.numel();
     const int64_t nbytes = castle_embedding_grad_workspace_bytes(R, (int)V, (int)D, dtype_code(g[0]));
-    if (scale != 1 || nbytes < 0 || V * D % 8 != 0 || R * V > kFewTokens) return {embedding_bwd_op(g[0], index, V, scale, -1), Tensor(), Tensor()};
+    if (scale != 1 || nbytes < 0 || V * D % 8 != 0 || R * V > kFewTokens || V > kFewTableRows || V * D > kSmallTable)
+      return {embedding_bwd_op(g[0], index, V, scale, -1), Tensor(), Tensor()};
     const Tensor dy = row_major(g[0]);
     Tensor dw = at::empty({V, D}, dy.options()), ws = bytes(nbytes, dy);
     check(castle_embedding_grad(dy.data_ptr(), static_cast<const int64_t*>(index.data_ptr()), index.size(1), index.stride(0), R, (int)V, (int)D, dw.data_ptr(),

@@ -72,3 +72,19 @@ def test_no_tokens_at_all_still_record_a_graph(scale):
         assert y.shape == (*shape, 16) and y.requires_grad
         grad, = torch.autograd.grad(y.sum(), table)
         assert grad.shape == table.shape and not grad.any()
+
+
+@gpu
+def test_gradient_of_few_tokens_over_a_large_vocabulary_takes_no_second_table():
+    """The model's embedding of 128 tokens over 131072 rows: beside the gradient itself there is no table of partial sums in memory."""
+    table = torch.randn(131072, 256, device=DEV).bfloat16().requires_grad_()
+    index = torch.randint(0, 131072, (2, 64), device=DEV)
+    y = _native.host().embedding(table, index)
+    dy = torch.randn_like(y)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grad, = torch.autograd.grad(y, table, dy)
+    assert torch.cuda.max_memory_allocated() - before < 1.1 * grad.numel() * grad.element_size()
+    want = torch.zeros(table.shape, dtype=torch.float64, device=DEV).index_add_(0, index.flatten(), dy.double().flatten(0, 1))
+    assert ((grad.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5).all()
