@@ -398,10 +398,13 @@ class CastleLM(nn.Module):
             norm, up, _, down = feed_forward
             delta, h = host.feed_forward(h, drop(attended, None), norm.weight, norm.eps, up.weight, down.weight)
             delta = drop(delta, None)
-        weight = self.to_logits.weight
-        if target is not None and linear_loss_is_ahead(target.numel(), weight):
-            return host.head_loss(h, delta, self.final_norm.weight, self.final_norm.eps, weight, target)
-        logits = host.head(h, delta, self.final_norm.weight, self.final_norm.eps, self.to_logits.weight)
+        norm, weight = self.final_norm.weight, self.to_logits.weight
+        if target is not None:
+            with torch.set_grad_enabled(torch.is_grad_enabled() and any(t.requires_grad for t in (h, delta, norm, weight))):   # (frozen parameters: no gradients to be ahead in)
+                ahead = linear_loss_is_ahead(target.numel(), weight)
+            if ahead:
+                return host.head_loss(h, delta, norm, self.final_norm.eps, weight, target)
+        logits = host.head(h, delta, norm, self.final_norm.eps, weight)
         if target is not None:
             return host.cross_entropy(logits, target)
         return (logits, next_cache) if return_next_cache else logits

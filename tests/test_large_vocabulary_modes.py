@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from lookahead_keys_attention_amd import CastleLM, _native, ops
+from lookahead_keys_attention_amd import lm as LM
 
 DEV = "cuda:0"
 gpu = pytest.mark.gpu
@@ -88,3 +89,20 @@ def test_gradient_of_few_tokens_over_a_large_vocabulary_takes_no_second_table():
     assert torch.cuda.max_memory_allocated() - before < 1.1 * grad.numel() * grad.element_size()
     want = torch.zeros(table.shape, dtype=torch.float64, device=DEV).index_add_(0, index.flatten(), dy.double().flatten(0, 1))
     assert ((grad.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5).all()
+
+
+@gpu
+def test_a_model_without_gradients_takes_the_loss_of_inference(monkeypatch):
+    """Frozen parameters record no graph, whether gradients are switched off or not: the rule is asked as for inference; one parameter that is not frozen, and it is asked as for training."""
+    model = make(num_tokens=16400).bfloat16()
+    x, asked = torch.randint(0, 16400, (3, 20), device=DEV), []
+    monkeypatch.setattr(LM, "linear_loss_is_ahead", lambda rows, weight: asked.append(torch.is_grad_enabled()) or True)
+    loss = model(x, return_loss=True)
+    assert asked == [True] and loss.requires_grad
+    model.requires_grad_(False)
+    assert not model(x, return_loss=True).requires_grad and asked == [True, False]
+    model.final_norm.weight.requires_grad_(True)
+    assert model(x, return_loss=True).requires_grad and asked == [True, False, True]
+    with torch.no_grad():
+        model(x, return_loss=True)
+    assert asked == [True, False, True, False]
