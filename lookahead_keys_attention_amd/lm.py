@@ -37,25 +37,30 @@ READ_ONCE_BYTES = 320_000_000
 SAMPLER_MAX_VOCABULARY = 20480
 
 
-# From this vocabulary on the loss of a native model is formed without its logits (ops.linear_cross_entropy), which takes four products and logits in memory three: in training in
-# 16 bits, more than 2048 rows wider than 512 keep the logits as long as these take no more than LOGITS_MAX_BYTES, in 32 bits those below 2^24 logits.  Measured, us with the
-# logits / without them, loss and gradients, then the loss alone: bf16 2048 x 512 over 8192 151 / 156 and 43 / 39, over 16384 233 / 218 and 71 / 57; 16384 x 512 over 32000
-# 2282 / 2286 and 904 / 596; 2048 x 1024 over 32000 625 / 561, 8192 x 1024 1704 / 2056 and 575 / 518; 8192 x 2048 over 131072 11780 / 15095 and 3698 / 3788; fp32 256 x 512 over
-# 16384 179 / 241, over 65536 597 / 579; 2048 x 512 over 32000 1469 / 1468 and 519 / 365; 16384 x 512 over 32000 11494 / 11083 and 3856 / 2544.
+# From this vocabulary on the loss of a native model may be formed without its logits (ops.linear_cross_entropy): four products where logits in memory take three, and in 32 bits a copy of
+# the table in three parts, against passes over the logits.  Logits of more than LOGITS_MAX_BYTES are never formed; smaller ones are where they are ahead.  Measured, us with the logits / without
+# them, rows x width over the vocabulary, loss and gradients:
+#   16 bits  2048 x 512 over 16384 235 / 214, over 131072 1812 / 1202; 2048 x 1024 over 16384 329 / 319, over 32000 621 / 565; 1024 x 2048 over 16384 329 / 325, over 131072 2493 / 2149;
+#            512 x 4096 353 / 362, 2476 / 2260; 2048 x 2048 463 / 547, 3901 / 3954; 2048 x 4096 828 / 1023, 5881 / 7580; 8192 x 1024 over 32000 1704 / 2056; 16384 x 512 2282 / 2286
+#   32 bits  256 x 512 over 16384 179 / 241, over 131072 1212 / 1072; 1024 x 512 over 16384 411 / 448, 512 x 1024 over 131072 3211 / 3289, 128 x 2048 1989 / 2868, 1024 x 2048 10789 / 11572
+# and the loss alone:
+#   16 bits  1 x 512 over 16384 30 / 18, 2048 x 512 70 / 54; 8192 x 2048 490 / 505, over 131072 3803 / 3830; 1024 x 4096 140 / 143, 1029 / 974; 2048 x 4096 235 / 259, 1782 / 1883; 8192 x 4096 850 / 982
+#   32 bits  1 x 128 over 16384 35 / 28, 16 x 512 41 / 52, 128 x 512 56 / 54; 1 x 2048 56 / 184, 256 x 2048 150 / 221, 512 x 2048 274 / 254, over 131072 1953 / 1746
 LINEAR_LOSS_MIN_VOCABULARY = 16384
 LOGITS_MAX_BYTES = 4 << 30
 
 
 def linear_loss_is_ahead(rows: int, weight: torch.Tensor) -> bool:
-    """Whether the cross entropy of `rows` hidden rows against `weight` is taken without their logits; False where ops.linear_cross_entropy would refuse them."""
+    """Whether the cross entropy of `rows` hidden rows against `weight` is taken without their logits, where a graph is recorded (gradients are switched on) or not; False where
+    ops.linear_cross_entropy would refuse them."""
     V, D = weight.shape
     if not (LINEAR_LOSS_MIN_VOCABULARY <= V <= 1 << 22 and D % 8 == 0 and D <= 1 << 16 and 0 < rows <= 1 << 24):
         return False
-    if not torch.is_grad_enabled():
+    if weight.element_size() * rows * V > LOGITS_MAX_BYTES:
         return True
-    if weight.element_size() == 4:
-        return rows * V >= 1 << 24
-    return rows <= 2048 or D <= 512 or weight.element_size() * rows * V > LOGITS_MAX_BYTES
+    if torch.is_grad_enabled():
+        return rows * V >= 1 << 24 and 2 * rows >= D if weight.element_size() == 4 else D <= 512 or rows <= 2048 and rows * D <= 1 << 21
+    return D <= 128 or 4 * rows >= D if weight.element_size() == 4 else D <= 2048 or rows * D <= 1 << 22
 
 
 # -- sampling helpers (train_triton.py:56-71) ------------------------------------------------

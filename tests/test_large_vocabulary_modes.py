@@ -106,3 +106,21 @@ def test_a_model_without_gradients_takes_the_loss_of_inference(monkeypatch):
     with torch.no_grad():
         model(x, return_loss=True)
     assert asked == [True, False, True, False]
+
+
+def test_where_logits_in_memory_are_ahead():
+    """Sizes on either side of each bound, in training and without gradients; logits of more than LOGITS_MAX_BYTES are never formed."""
+    def ahead(rows, V, D, dtype):
+        return LM.linear_loss_is_ahead(rows, torch.empty(V, D, dtype=dtype, device="meta"))
+
+    half, full, most = torch.bfloat16, torch.float32, LM.LOGITS_MAX_BYTES
+    for grad, yes, no in ((True, [(2048, 16384, 1024, half), (1024, 131072, 2048, half), (512, 16384, 4096, half), (1 << 14, 32000, 512, half), (256, 131072, 512, full),
+                                  (1024, 131072, 2048, full)],
+                           [(2048, 16384, 1032, half), (1025, 131072, 2048, half), (2048, 131072, 4096, half), (255, 131072, 512, full), (1023, 131072, 2048, full), (128, 131072, 2048, full)]),
+                          (False, [(1, 16384, 2048, half), (1 << 14, 16384, 2048, half), (1024, 16384, 4096, half), (1, 16384, 128, full), (128, 16384, 512, full), (512, 16384, 2048, full)],
+                           [(1025, 16384, 4096, half), (8192, 32000, 4096, half), (1, 16384, 136, full), (127, 16384, 512, full), (511, 131072, 2048, full)])):
+        with torch.set_grad_enabled(grad):
+            assert all(ahead(*case) for case in yes) and not any(ahead(*case) for case in no), grad
+            for dtype in (half, full):
+                rows = most // dtype.itemsize // (1 << 18)
+                assert ahead(rows + 1, 1 << 18, 1 << 16, dtype) and not ahead(rows, 1 << 18, 1 << 16, dtype)
