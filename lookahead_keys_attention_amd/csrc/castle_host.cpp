@@ -1059,6 +1059,8 @@ std::tuple<Tensor, Tensor> linear_cross_entropy_bwd_op(const Tensor& dloss_, con
   const VocabCall c(x, weight, target, reduction);
   TORCH_CHECK_VALUE(dloss_.scalar_type() == x.scalar_type() && dloss_.device() == x.device() && dloss_.numel() == (reduction == CASTLE_LOSS_EACH ? c.rows : 1),
                     "linear_cross_entropy_bwd: the loss has another shape, type or device");
+  TORCH_CHECK_VALUE(state.scalar_type() == at::kByte && state.dim() == 1 && state.is_contiguous() && state.device() == x.device(),
+                    "linear_cross_entropy_bwd: the state is what the forward pass has returned, on ", x.device());
   Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
   Tensor dw = need_w ? at::empty(weight.sizes(), weight.options()) : at::empty({0}, weight.options());
   if (c.rows == 0 && need_w) dw.zero_();

@@ -94,3 +94,18 @@ def test_rows_whose_losses_count_very_differently_in_several_pieces():
     assert not dx[::3].any() and not dx[::7].any()
     _, _, (ref, bound) = reference(x, w, target, "none", dloss, -100, dtype)
     within(dw, ref, bound + 2.0 ** -25 / 2.0 ** 14 * dloss.double().abs().max() * x[target != -100].double().abs().sum(0), dtype, "dw")
+
+
+@gpu
+def test_the_backward_operator_refuses_what_no_forward_pass_has_returned():
+    x, w, target = inputs(20, 30, 16, torch.bfloat16, 23)
+    forward, backward = torch.ops.castle_hip.linear_cross_entropy, torch.ops.castle_hip.linear_cross_entropy_bwd
+    loss, state = forward(x, w, target, 0, -100)
+    good = backward(loss, x, w, target, state, 0, -100)
+    for bad in (state.cpu(), state.view(torch.int32), state[None], state.repeat_interleave(2)[::2]):
+        with pytest.raises(ValueError, match="state"):
+            backward(loss, x, w, target, bad, 0, -100)
+    for bad in (state[:-256], torch.cat((state[:16], state))[16:], state[:0]):   # too short, not at 256 bytes
+        with pytest.raises(RuntimeError):
+            backward(loss, x, w, target, bad, 0, -100)
+    assert all(torch.equal(a, b) for a, b in zip(backward(loss, x, w, target, state.clone(), 0, -100), good))
