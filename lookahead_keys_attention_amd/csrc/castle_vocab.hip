@@ -378,6 +378,96 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kern
   *reinterpret_cast<vec4_mem<T>*>(static_cast<T*>(a.out) + r * a.D + c) = __builtin_convertvector(v, vec<T, 4>);
 }
 
+// The gradients of up to kFewRows rows of 16 bits, where d's rounding at the targets shows: -(1 - p) of a row is its largest element, often by far, and what is lost of it is lost of dx[r] and
+// of dw[target] alike (over many rows these errors are as one of the result's own roundings; of four rows of 200 over 904 they were 2.3 times that).  A workgroup to a row, and to 1024
+// columns of it: that element again in 32 bits; dx from its partial results and what d has lost there; the row of dw that belongs to the first row of each target once more, all of it,
+// with these elements.
+constexpr int kFewRows = 64;
+struct FewArgs {
+  VocabArgs v;
+  const VocabHead* head;
+  const int32_t *rank, *tc;
+  const float *lse, *factor;   // factor, own: by rank, or nullptr
+  const int32_t* own;
+  const Gain* gain;
+  const void *xc, *d;          // d: one row of blocks
+  const float* parts;          // of dx, [splits][R][D]
+  void *dx, *dw;
+  int Dp, splits;
+};
+template <typename T> __global__ __launch_bounds__(kThreads) void few_rows_kernel(FewArgs a) {
+  constexpr int B = 64;   // rows and columns of a block of d
+  typedef vec<float, 4> v4;
+  __shared__ float s_sum[kWaves], s_coef[kFewRows];
+  const int rank = a.rank[blockIdx.x], lane = lane_id(), wave = wave_id(), D = a.v.D, c = 4 * (blockIdx.y * kThreads + threadIdx.x);
+  T* const dx = a.dx != nullptr ? static_cast<T*>(a.dx) + (int64_t)blockIdx.x * D + c : nullptr;
+  if (rank < 0) {
+    if (dx != nullptr && c < D) st4<T>(dx, vec<T, 4>{});
+    return;
+  }
+  const int target = a.tc[rank], count = min(a.head->count, kFewRows), shift = a.gain->shift;
+  const float gain = a.gain->gain;
+  const T *x = static_cast<const T*>(a.xc), *w = static_cast<const T*>(a.v.w) + (int64_t)max(target, 0) * a.v.ld_w;
+  const T* const d = static_cast<const T*>(a.d) + (int64_t)max(target, 0) / B * (B * B) + max(target, 0) % B;   // of this class, rows B apart
+  auto own_of = [&](int k) { return a.own != nullptr ? a.own[k] : 0; };
+  // d of row k, whose target this is, by all threads
+  auto at_target = [&](int k) {
+    float z = 0.f;
+    for (int i = 8 * threadIdx.x; i < D; i += 8 * kThreads) {
+      const frag<T> p = *reinterpret_cast<const frag_mem<T>*>(x + (int64_t)k * a.Dp + i), q = *reinterpret_cast<const frag_mem<T>*>(w + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z = __builtin_fmaf((float)p[e], (float)q[e], z);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) z += __shfl_xor(z, o);
+    __syncthreads();   // (the sums before have been read)
+    if (lane == 0) s_sum[wave] = z;
+    __syncthreads();
+    z = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) z += s_sum[i];
+    return (a.factor != nullptr ? a.factor[k] : ldexpf(1.f, kDShift)) * (fast_exp2((z - a.lse[k]) * kLog2e) - 1.f);
+  };
+  const int own = own_of(rank);
+  float here = 0.f, lost = 0.f;
+  if (target >= 0) {
+    here = at_target(rank);
+    lost = here - (own != 0 ? (float)(T)here : (float)d[rank * B]);   // (a row with a power of its own may have been lowered)
+  }
+  if (dx != nullptr && c < D) {
+    v4 v = {0.f, 0.f, 0.f, 0.f};
+    const float* p = a.parts + (int64_t)rank * D + c;
+#pragma unroll 4
+    for (int k = 0; k < a.splits; ++k) v += *reinterpret_cast<const v4*>(p + (int64_t)k * a.v.R * D);
+    const vec<T, 4> there = *reinterpret_cast<const vec4_mem<T>*>(w + c);
+    vec<T, 4> out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float sum = lost != 0.f ? __builtin_fmaf(lost, (float)there[e], v[e]) : v[e];
+      out[e] = (T)(ldexpf(sum, -shift - own) * gain);
+    }
+    st4<T>(dx, out);
+  }
+  if (a.dw == nullptr || target < 0) return;
+  uint64_t same = __ballot(lane < count && a.tc[lane] == target);
+  if (same & ((1ull << rank) - 1)) return;   // (another row's)
+  if ((int)threadIdx.x < count) s_coef[threadIdx.x] = (float)d[threadIdx.x * B];
+  __syncthreads();
+  for (; same != 0; same &= same - 1) {
+    const int k = __builtin_ctzll(same);
+    const float f = ldexpf(k == rank ? here : at_target(k), -own_of(k));
+    if (threadIdx.x == 0) s_coef[k] = f;
+  }
+  __syncthreads();
+  if (c >= D) return;
+  v4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int k = 0; k < count; ++k) v += s_coef[k] * __builtin_convertvector(*reinterpret_cast<const vec4_mem<T>*>(x + (int64_t)k * a.Dp + c), v4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -shift) * gain;
+  st4<T>(static_cast<T*>(a.dw) + (int64_t)target * D + c, __builtin_convertvector(v, vec<T, 4>));
+}
+
 // ---- products of 16-bit operands ------------------------------------------------------------------------------------
 // The frame is that of gemm_wide_kernel (castle_gemm.hip): tiles of the output by workgroups of eight waves, steps of 64 of the contraction straight from memory to LDS into
 // two or three buffers, requested over the end of a tile.  What differs: sizes that are read from device memory, contractions of any length (d and the copied rows are padded with
@@ -1212,7 +1302,16 @@ int launch_vocab_bwd(const VocabArgs& a, int dtype, const void* dloss, const voi
         rc = join({b.weight_parts, nullptr, b.gain, nullptr, w.c, w.splits, a.D, n, &s.head->count, p.step});
     }
   }
-  if (rc != 0 || dx == nullptr) return rc;
+  if (rc != 0) return rc;
+  if (es == 2 && a.R <= kFewRows) {   // (of so few rows d is one piece for any vocabulary, and its contraction for dw is one range)
+    const FewArgs f = {a, s.head, s.rank, s.tc, s.lse, a.reduction == kEachLoss ? b.factor : nullptr, own, b.gain, xc, b.d, b.row_parts, dx, dw, p.Dp,
+                       ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.rows.ranges)};
+    const dim3 grid((unsigned)a.R, (unsigned)(up(a.D, 4 * kThreads) / (4 * kThreads)));
+    if (dtype == 1) hipLaunchKernelGGL((few_rows_kernel<bf16_t>), grid, dim3(kThreads), 0, stream, f);
+    else hipLaunchKernelGGL((few_rows_kernel<fp16_t>), grid, dim3(kThreads), 0, stream, f);
+    return launched();
+  }
+  if (dx == nullptr) return rc;
   return join({b.row_parts, s.rank, b.gain, own, dx, ranges((int)up(std::min(a.V, p.columns), p.step) / p.step, p.rows.ranges), a.D, a.R, nullptr, p.step});
 }
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from lookahead_keys_attention_amd import ops
-from test_vocab import DEV, TYPES, gpu, inputs, reference, within
+from test_vocab import DEV, TYPES, U, gpu, inputs, reference, within
 
 
 @gpu
@@ -109,3 +109,50 @@ def test_the_backward_operator_refuses_what_no_forward_pass_has_returned():
         with pytest.raises(RuntimeError):
             backward(loss, x, w, target, bad, 0, -100)
     assert all(torch.equal(a, b) for a, b in zip(backward(loss, x, w, target, state.clone(), 0, -100), good))
+
+
+@gpu
+@pytest.mark.parametrize("R", [1, 2, 7, 33, 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_few_rows_lose_nothing_of_their_targets(R, dtype, reduction):
+    """Each row has eight columns of its own, in it and in the class it aims at, and other classes are zero: in these columns both gradients are the target's part alone, which is p - 1 of
+    32 bits times the factor, the logit off by ez as everywhere, and is rounded once.  Some rows have the same target, one does not count, one's is not there."""
+    D, V = 8 * max(R, 3), 5000
+    g = torch.Generator().manual_seed(R)
+    target = torch.randint(0, V, (R,), generator=g)
+    target[3::5] = target[0]
+    own = torch.arange(D)[None] // 8 == torch.arange(R)[:, None]
+    x = torch.where(own, torch.randn(R, D, generator=g), 0.0).to(dtype)
+    w = torch.zeros(V, D)
+    for r in range(R):   # (logits of 4 to 12: softmax values of the target from 0.01 to 0.97)
+        v = torch.randn(8, generator=g)
+        part = x[r, own[r]].float()
+        w[target[r], own[r]] = v + (4 + 8 * torch.rand(1, generator=g) - v @ part) * part / (part @ part)
+    w = w.to(dtype)
+    counts = torch.ones(R, dtype=torch.bool)
+    if R > 8:
+        counts[5] = False
+    given = torch.where(counts, target, -100)
+    dloss = torch.tensor(0.8125, dtype=dtype) if reduction == "mean" else (0.5 + torch.rand(R, generator=g)).to(dtype)
+    if reduction == "none" and dtype is torch.float16:
+        dloss[R // 2] *= 2.0 ** -9   # (a power of two of its own)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w)]
+    loss = ops.linear_cross_entropy(*leaves, given.to(DEV), reduction)
+    dx, dw = (t.cpu().double() for t in torch.autograd.grad(loss, leaves, dloss.to(DEV), retain_graph=True))
+    assert torch.equal(torch.autograd.grad(loss, leaves[0], dloss.to(DEV), retain_graph=True)[0].cpu().double(), dx)
+    assert torch.equal(torch.autograd.grad(loss, leaves[1], dloss.to(DEV))[0].cpu().double(), dw)
+    x, w = x.double(), w.double()
+    z, half = x @ w.T, torch.finfo(dtype).eps / 2
+    lse = torch.logsumexp(z, 1)
+    for r in range(R):
+        if not counts[r]:
+            assert not dx[r].any()
+            continue
+        factor, p = dloss.double().expand(R)[r] / (counts.sum() if reduction == "mean" else 1), torch.exp(z[r, target[r]] - lse[r])
+        ez = (D / 16 + 32) * U * (x[r].abs() @ w[target[r]].abs())
+        off = abs(factor) * (p * (2 * ez + 16 * U * (1 + lse[r].abs())) + 8 * U)
+        for got, other in ((dx[r, own[r]], w[target[r], own[r]]), (dw[target[r], own[r]], x[r, own[r]])):
+            ref = factor * (p - 1) * other
+            most = off * other.abs() + half * (ref.abs() + off * other.abs()).clamp(min=torch.finfo(dtype).tiny)
+            assert ((got - ref).abs() <= most).all(), (r, ((got - ref).abs() / most).max())
