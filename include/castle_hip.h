@@ -415,10 +415,11 @@ int castle_embedding_grad(const void* dy, const int64_t* index, int64_t index_n,
  * loss.  loss: one element of the type, or `rows` of them.  `state`: castle_linear_cross_entropy_state_bytes for the backward pass.
  *
  * _bwd: dx (rows x width) and dweight (vocabulary x width), contiguous, either may be NULL; dloss is one element, or `rows` of them.  All in a fixed order.  The logits are formed
- * again, as many columns of the vocabulary at a time as a workspace of about 1 GB holds; 16-bit types: what is multiplied with w and x is rounded to the type, under a power of two that
- * keeps it among its normal numbers (fp16 and each row's loss: for dx one of the row's own where its dloss is less than 2^-4 of the largest, for dweight the same for all rows: steps of 2^-40 of the
- * largest dloss); fp32: products by three bf16 parts of each element, all of whose 24 bits count down to 2^-110, an infinite one makes what it enters NaN,
- * and the parts of x and w lie in the workspace, 6 bytes an element.  gradients of _workspace_bytes: 0 for the forward pass, else the sum of 1 (dx) and 2 (dweight). */
+ * again, as many columns of the vocabulary at a time as 1 GiB of the workspace holds at two bytes (fp32: six) a row and column, 256 at least (of 2^24 rows 8 GiB, fp32 24); beside that dx takes
+ * 4 bytes an element for each range that its sums are split into, and in fp32 x and w 6 bytes an element in three bf16 parts.  16-bit types: what is multiplied with w and x is rounded to the
+ * type, under a power of two that keeps it among its normal numbers (fp16 and each row's loss: for dx one of the row's own where its dloss is less than 2^-4 of the largest, for dweight the
+ * same for all rows: steps of 2^-40 of the largest dloss); of up to 64 rows what is lost of it at the targets is taken up again.  fp32: products by three bf16 parts of each element, all of
+ * whose 24 bits count down to 2^-110; an infinite one makes what it enters NaN.  gradients of _workspace_bytes: 0 for the forward pass, else the sum of 1 (dx) and 2 (dweight). */
 #define CASTLE_LOSS_MEAN 0
 #define CASTLE_LOSS_SUM 1
 #define CASTLE_LOSS_EACH 2

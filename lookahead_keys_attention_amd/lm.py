@@ -12,8 +12,13 @@ Differences a user can switch: `tie_embedding=True` shares the token embedding w
 projection (the reference keeps them separate, train_triton.py:86,111); `rotary_emb` / `prenorm`
 default to the reference's choice (both on, train_triton.py:99-100); `embedding_scale` multiplies the
 embedded tokens; `dropout` is the probability with which an element of the embedded tokens and of every
-block's output is dropped in training, on passes that neither take nor return caches.  Vocabularies of any size:
-from LINEAR_LOSS_MIN_VOCABULARY on, `return_loss` of a native model forms no logits.
+block's output is dropped in training, on passes that neither take nor return caches.
+
+Vocabularies of any size.  From LINEAR_LOSS_MIN_VOCABULARY on, `return_loss` of a native model whose modules run as they are (no
+hooks, no autocast, no torch.compile) forms no logits where they would take more than LOGITS_MAX_BYTES or be slower
+(`linear_loss_is_ahead`); a larger LINEAR_LOSS_MIN_VOCABULARY keeps them.  Without them, in float32, an infinite element of the
+last rows or of the projection makes the loss NaN, and of elements below 2^-110 the last digits do not count
+(ops.linear_cross_entropy).  On the native path a token outside of the vocabulary is embedded as NaNs.
 """
 from __future__ import annotations
 
