@@ -381,7 +381,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_rows_kern
 // The gradients of up to kFewRows rows of 16 bits, where d's rounding at the targets shows: -(1 - p) of a row is its largest element, often by far, and what is lost of it is lost of dx[r] and
 // of dw[target] alike (over many rows these errors are as one of the result's own roundings; of four rows of 200 over 904 they were 2.3 times that).  A workgroup to a row, and to 1024
 // columns of it: that element again in 32 bits; dx from its partial results and what d has lost there; the row of dw that belongs to the first row of each target once more, all of it,
-// with these elements.
+// with these elements.  (Bound by the trips to memory one behind the other: 64 rows of 512 over 32000, forward and backward in a captured graph, 71 us, with the plain join 66.)
 constexpr int kFewRows = 64;
 struct FewArgs {
   VocabArgs v;
