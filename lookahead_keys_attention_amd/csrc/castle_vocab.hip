@@ -608,7 +608,7 @@ template <int MODE, int BM, int BN, bool PARTS> struct Shape {
 };
 extern __shared__ __attribute__((aligned(16))) unsigned char castle_vocab_lds[];
 
-// END: rows of w end inside a step (kernels of their own: with the test for it in each, 3000 rows of 256 over 50257 took 392 us instead of 383)
+// END: rows of w end inside a step (kernels of their own: with the test for it in each, 3000 rows of 256 over 50257 took 392 us instead of 383; of 264 636, where reading the row's last piece again took 620)
 template <typename T, int MODE, int BM, int BN, bool PARTS, bool END> __global__ __launch_bounds__(kWideThreads, 2) void vocab_product_kernel(ProductArgs a) {
   typedef Shape<MODE, BM, BN, PARTS> S;
   constexpr bool AK = S::kContractA, BKC = S::kContractB;
