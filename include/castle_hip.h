@@ -448,6 +448,72 @@ int castle_embedding_sorted_grad(const void* dy, const int64_t* index, int64_t i
  * stay where theirs is at least t.  seed: two numbers in device memory.  The backward pass is the same call on dy without a residual: nothing is kept. */
 int castle_dropout(const void* x, const void* residual, void* y, int64_t n, double p, const int64_t* seed, int dtype, void* stream);
 
+/* Gated feed-forward block: u = x w_in^T, (g, v) the halves of u's columns, h = act(g) v, y = h w_out^T, for rows x (rows x dim, ld_x apart), w_in (2 hidden x dim) and w_out
+ * (dim x hidden); y is contiguous.  dim and hidden are multiples of 8, leading dimensions too, everything 16-byte aligned, operands within 2^31 elements (castle_gemm_operand_ok; [g v] of
+ * rows x 2 hidden is one).  state: NULL, or castle_gated_state_bytes for the backward pass.
+ * _bwd: dx (rows x dim), dw_in and dw_out, contiguous, each may be NULL.  gradients of _bwd_workspace_bytes: the sum of 1 (dx), 2 (dw_in) and 4 (dw_out). */
+#define CASTLE_GATE_SILU 0
+#define CASTLE_GATE_GELU 1   /* erf form */
+typedef struct castle_gated {
+  const void *x, *w_in, *w_out;
+  int64_t ld_x, ld_in, ld_out;
+  int32_t rows, dim, hidden, activation;
+} castle_gated;
+int64_t castle_gated_state_bytes(int rows, int dim, int hidden, int dtype);
+int64_t castle_gated_workspace_bytes(int rows, int dim, int hidden, int dtype, int with_state);
+int64_t castle_gated_bwd_workspace_bytes(int rows, int dim, int hidden, int dtype, int gradients);
+int castle_gated_feed_forward(const castle_gated* args, void* y, void* state, int64_t state_bytes, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int castle_gated_feed_forward_bwd(const castle_gated* args, const void* dy, const void* state, int64_t state_bytes, void* dx, void* dw_in, void* dw_out, int dtype,
+                                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The norms on both sides of a residual sum: y = residual + scale gate (x / sqrt(mean(x^2) + eps) weight), h = y / sqrt(mean(y^2) + eps) next_weight, each rounded once.  Rows of `width`
+ * elements, contiguous, of any alignment, up to CASTLE_RESIDUAL_MAX_WIDTH.  weight, scale and next_weight (width), gate (rows / span x width: row r has that of r / span) may be NULL: without
+ * weight x is not normalised, without next_weight there is no h.  rstd, next_rstd: NULL, or one float per row for the backward pass (where there is the norm).
+ * _bwd: of the gradients dy and dh, either of which may be NULL (not both); any of the results may be NULL. */
+#define CASTLE_RESIDUAL_MAX_WIDTH 8192
+typedef struct castle_residual {
+  const void *x, *residual, *weight, *scale, *gate, *next_weight;
+  int64_t rows, span;
+  int32_t width;
+  float eps;
+  float *rstd, *next_rstd;
+} castle_residual;
+typedef struct castle_residual_grads {
+  const void *dy, *dh;
+  void *dx, *dresidual, *dweight, *dscale, *dgate, *dnext_weight;
+} castle_residual_grads;
+int castle_residual_norm(const castle_residual* args, void* y, void* h, int dtype, void* stream);
+int64_t castle_residual_norm_bwd_workspace_bytes(const castle_residual* args, const castle_residual_grads* grads, int dtype);
+int castle_residual_norm_bwd(const castle_residual* args, const castle_residual_grads* grads, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A step of AdamW over `count` tensors (descriptions in host memory, everything that they point to in device memory), in place, and the 2-norm of their gradients:
+ *   g' = c g, c = min(1, max_norm / (norm + 1e-6));  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * param and grad have n elements of the type `dtype`, of any alignment; no tensor twice.  exp_avg and exp_avg_sq: n floats (m, v), or where the exponents are given (for all tensors or none) n e4m3
+ * numbers each, which times 2^exponent of their 256 elements are m and sqrt(v): E is the least power with which the largest finite one is at most 448, between -126 and 120.  Those are rounded to
+ * the next number towards zero of the number plus u steps, 0 <= u < 1 a multiple of 2^-16; a second moment that is not zero stays above zero.  So are 16-bit parameters where there is a seed (else
+ * to the nearest).  u: elements 8 i .. 8 i + 7 of a tensor take the eight 16-bit halves, low half first, of the four words that Philox4x32-10 makes of the counter 4 i + kind (64 bits; kind 0 second
+ * moment, 1 first, 2 parameter), the low 32 bits of t, the tensor's place in the call, and the key *seed.  step: the number of steps taken, t - 1, one more behind the call.  lr_device: NULL, or a
+ * float that stands for lr.  max_norm < 0: no clipping, norm is not read; else norm_given says whether *norm is there or formed here.  The elements of a call are at most 2^36.
+ * castle_gradient_norm reads grad and n alone. */
+typedef struct castle_optim_tensor {
+  void* param;
+  const void* grad;
+  void *exp_avg, *exp_avg_sq;
+  int8_t *exp_avg_exponents, *exp_avg_sq_exponents;
+  int64_t n;
+} castle_optim_tensor;
+typedef struct castle_adamw_options {
+  double lr, b1, b2, eps, weight_decay, max_norm;
+  const float* lr_device;
+  int64_t* step;
+  const int64_t* seed;
+  float* norm;
+  int32_t norm_given;
+} castle_adamw_options;
+int64_t castle_optim_workspace_bytes(int count);
+int castle_gradient_norm(const castle_optim_tensor* tensors, int count, float* norm, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int castle_adamw(const castle_optim_tensor* tensors, int count, const castle_adamw_options* options, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Per-kernel timing (no counterpart in the reference; for benchmarks).  While enabled, every
  * kernel launched by the entry points above is bracketed by a HIP event pair on its stream.
  * castle_profile_enable(on) also discards pending records.  castle_profile_read waits for the

@@ -83,6 +83,17 @@ EXPORTED_SYMBOLS = (
     "castle_embedding_sorted_grad_workspace_bytes",
     "castle_embedding_sorted_grad",
     "castle_dropout",
+    "castle_gated_state_bytes",
+    "castle_gated_workspace_bytes",
+    "castle_gated_bwd_workspace_bytes",
+    "castle_gated_feed_forward",
+    "castle_gated_feed_forward_bwd",
+    "castle_residual_norm",
+    "castle_residual_norm_bwd_workspace_bytes",
+    "castle_residual_norm_bwd",
+    "castle_optim_workspace_bytes",
+    "castle_gradient_norm",
+    "castle_adamw",
     "castle_profile_enable",
     "castle_profile_read",
 )

@@ -1,6 +1,7 @@
 // extern "C" surface of libcastle_hip.so (declared in include/castle_hip.h): argument
 // validation, workspace carving and dispatch to the kernel launchers.  No torch types.
 #include <hip/hip_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include "../../include/castle_hip.h"
@@ -9,8 +10,11 @@
 #include <stdlib.h>
 #include <initializer_list>
 #include "castle_params.h"
+#include "castle_gated.h"
 #include "castle_gemm.h"
+#include "castle_optim.h"
 #include "castle_profile.h"
+#include "castle_residual.h"
 #include "castle_rows.h"
 #include "castle_tokens.h"
 #include "castle_vocab.h"
@@ -964,6 +968,158 @@ int castle_linear_cross_entropy_bwd(const void* x, int64_t ld_x, const void* w, 
       !workspace_ok(workspace, workspace_bytes, castle::vocab_bwd_bytes(a, elem_size(dtype), dx != nullptr, dweight != nullptr)))
     return CASTLE_ERR_WORKSPACE;
   return castle::launch_vocab_bwd(a, dtype, dloss, state, dx, dweight, workspace, static_cast<hipStream_t>(stream));
+}
+
+static_assert(CASTLE_GATE_SILU == castle::kSilu && CASTLE_GATE_GELU == castle::kGeluGate, "");
+static int gated_sizes_ok(int rows, int dim, int hidden) {
+  return rows > 0 && dim > 0 && hidden > 0 && dim % 8 == 0 && hidden % 8 == 0 && dim <= 1 << 20 && hidden <= 1 << 20 && castle_gemm_operand_ok(rows, 2 * (int64_t)hidden) &&
+         castle_gemm_operand_ok(rows, dim) && castle_gemm_operand_ok(2 * (int64_t)hidden, dim) && castle_gemm_operand_ok(dim, hidden);
+}
+static int gated_args(castle::GatedArgs& g, const castle_gated* a, int dtype) {
+  if (elem_size(dtype) == 0) return CASTLE_ERR_DTYPE;
+  if (a == nullptr || a->x == nullptr || a->w_in == nullptr || a->w_out == nullptr || !aligned16({a->x, a->w_in, a->w_out}) || a->activation < CASTLE_GATE_SILU || a->activation > CASTLE_GATE_GELU)
+    return CASTLE_ERR_ARG;
+  if (!gated_sizes_ok(a->rows, a->dim, a->hidden) || a->ld_x < a->dim || a->ld_in < a->dim || a->ld_out < a->hidden || a->ld_x % 8 != 0 || a->ld_in % 8 != 0 || a->ld_out % 8 != 0 ||
+      !castle_gemm_operand_ok(a->rows, a->ld_x) || !castle_gemm_operand_ok(2 * (int64_t)a->hidden, a->ld_in) || !castle_gemm_operand_ok(a->dim, a->ld_out))
+    return CASTLE_ERR_SHAPE;
+  g = {a->x, a->w_in, a->w_out, a->ld_x, a->ld_in, a->ld_out, a->rows, a->dim, a->hidden, a->activation};
+  return CASTLE_OK;
+}
+
+int64_t castle_gated_state_bytes(int rows, int dim, int hidden, int dtype) {
+  if (elem_size(dtype) == 0) return CASTLE_ERR_DTYPE;
+  return gated_sizes_ok(rows, dim, hidden) ? castle::gated_state(rows, dim, hidden, dtype) : CASTLE_ERR_SHAPE;
+}
+
+int64_t castle_gated_workspace_bytes(int rows, int dim, int hidden, int dtype, int with_state) {
+  if (elem_size(dtype) == 0) return CASTLE_ERR_DTYPE;
+  return gated_sizes_ok(rows, dim, hidden) ? castle::gated_workspace(rows, dim, hidden, dtype, with_state != 0) : CASTLE_ERR_SHAPE;
+}
+
+int64_t castle_gated_bwd_workspace_bytes(int rows, int dim, int hidden, int dtype, int gradients) {
+  if (elem_size(dtype) == 0) return CASTLE_ERR_DTYPE;
+  if (gradients <= 0 || gradients > 7) return CASTLE_ERR_ARG;
+  return gated_sizes_ok(rows, dim, hidden) ? castle::gated_bwd_workspace(rows, dim, hidden, dtype, gradients) : CASTLE_ERR_SHAPE;
+}
+
+int castle_gated_feed_forward(const castle_gated* args, void* y, void* state, int64_t state_bytes, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  castle::GatedArgs g;
+  if (const int rc = gated_args(g, args, dtype)) return rc;
+  if (y == nullptr || !aligned16({y})) return CASTLE_ERR_ARG;
+  if ((state != nullptr && !workspace_ok(state, state_bytes, castle::gated_state(g.R, g.D, g.F, dtype))) ||
+      !workspace_ok(workspace, workspace_bytes, castle::gated_workspace(g.R, g.D, g.F, dtype, state != nullptr)))
+    return CASTLE_ERR_WORKSPACE;
+  return castle::launch_gated(g, y, state, dtype, workspace, static_cast<hipStream_t>(stream));
+}
+
+int castle_gated_feed_forward_bwd(const castle_gated* args, const void* dy, const void* state, int64_t state_bytes, void* dx, void* dw_in, void* dw_out, int dtype,
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
+  castle::GatedArgs g;
+  if (const int rc = gated_args(g, args, dtype)) return rc;
+  const int gradients = (dx != nullptr) + 2 * (dw_in != nullptr) + 4 * (dw_out != nullptr);
+  if (dy == nullptr || gradients == 0 || !aligned16({dy, dx, dw_in, dw_out})) return CASTLE_ERR_ARG;
+  if (!workspace_ok(state, state_bytes, castle::gated_state(g.R, g.D, g.F, dtype)) || !workspace_ok(workspace, workspace_bytes, castle::gated_bwd_workspace(g.R, g.D, g.F, dtype, gradients)))
+    return CASTLE_ERR_WORKSPACE;
+  return castle::launch_gated_bwd(g, dy, state, dx, dw_in, dw_out, dtype, workspace, static_cast<hipStream_t>(stream));
+}
+
+static_assert(CASTLE_RESIDUAL_MAX_WIDTH == castle::kResidualMaxWidth, "");
+static int residual_args(castle::ResidualArgs& r, const castle_residual* a, int dtype) {
+  const int es = elem_size(dtype);
+  if (es == 0) return CASTLE_ERR_DTYPE;
+  if (a == nullptr || a->x == nullptr || a->residual == nullptr || !(a->eps >= 0.f) || reinterpret_cast<uintptr_t>(a->rstd) % 4 != 0 || reinterpret_cast<uintptr_t>(a->next_rstd) % 4 != 0) return CASTLE_ERR_ARG;
+  for (const void* p : {a->x, a->residual, a->weight, a->scale, a->gate, a->next_weight})
+    if (reinterpret_cast<uintptr_t>(p) % es != 0) return CASTLE_ERR_ARG;
+  if (a->rows <= 0 || a->rows > (int64_t)1 << 40 || a->width <= 0 || a->width > CASTLE_RESIDUAL_MAX_WIDTH || (a->gate != nullptr && (a->span <= 0 || a->rows % a->span != 0))) return CASTLE_ERR_SHAPE;
+  r = {a->x, a->residual, a->weight, a->scale, a->next_weight, a->gate, a->rows, a->gate != nullptr ? a->span : 1, a->width, a->eps, a->weight != nullptr ? a->rstd : nullptr,
+       a->next_weight != nullptr ? a->next_rstd : nullptr, nullptr, nullptr};
+  return CASTLE_OK;
+}
+static int residual_grad_args(castle::ResidualBwdArgs& b, const castle_residual* a, const castle_residual_grads* g, int dtype) {
+  if (const int rc = residual_args(b.f, a, dtype)) return rc;
+  if (g == nullptr || (g->dy == nullptr && g->dh == nullptr) || (g->dh != nullptr && (a->next_weight == nullptr || a->next_rstd == nullptr)) || (a->weight != nullptr && a->rstd == nullptr) ||
+      (g->dweight != nullptr && a->weight == nullptr) || (g->dscale != nullptr && a->scale == nullptr) || (g->dgate != nullptr && a->gate == nullptr) ||
+      (g->dnext_weight != nullptr && g->dh == nullptr))
+    return CASTLE_ERR_ARG;
+  for (const void* p : {g->dy, g->dh, (const void*)g->dx, (const void*)g->dresidual, (const void*)g->dweight, (const void*)g->dscale, (const void*)g->dgate, (const void*)g->dnext_weight})
+    if (reinterpret_cast<uintptr_t>(p) % elem_size(dtype) != 0) return CASTLE_ERR_ARG;
+  b.dy = g->dy;
+  b.dh = g->dh;
+  b.dx = g->dx;
+  b.dresidual = g->dresidual;
+  b.dgate = g->dgate;
+  b.dw = g->dweight;
+  b.dscale = g->dscale;
+  b.dnext = g->dnext_weight;
+  return CASTLE_OK;
+}
+
+int castle_residual_norm(const castle_residual* args, void* y, void* h, int dtype, void* stream) {
+  castle::ResidualArgs r;
+  if (const int rc = residual_args(r, args, dtype)) return rc;
+  if (y == nullptr || (args->next_weight != nullptr && h == nullptr) || !aligned_to({y, h}, elem_size(dtype))) return CASTLE_ERR_ARG;
+  r.y = y;
+  r.h = h;
+  return castle::launch_residual(r, dtype, static_cast<hipStream_t>(stream));
+}
+
+int64_t castle_residual_norm_bwd_workspace_bytes(const castle_residual* args, const castle_residual_grads* grads, int dtype) {
+  castle::ResidualBwdArgs b = {};
+  if (const int rc = residual_grad_args(b, args, grads, dtype)) return rc;
+  return align_up(castle::residual_bwd_workspace(b), 256);
+}
+
+int castle_residual_norm_bwd(const castle_residual* args, const castle_residual_grads* grads, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  castle::ResidualBwdArgs b = {};
+  if (const int rc = residual_grad_args(b, args, grads, dtype)) return rc;
+  const int64_t need = align_up(castle::residual_bwd_workspace(b), 256);
+  if (need > 0 && !workspace_ok(workspace, workspace_bytes, need)) return CASTLE_ERR_WORKSPACE;
+  return castle::launch_residual_bwd(b, dtype, workspace, static_cast<hipStream_t>(stream));
+}
+
+static_assert(sizeof(castle_optim_tensor) == sizeof(castle::OptimTensor) && offsetof(castle_optim_tensor, n) == offsetof(castle::OptimTensor, n) &&
+              offsetof(castle_optim_tensor, exp_avg_exponents) == offsetof(castle::OptimTensor, em), "");
+constexpr int64_t kOptimElements = (int64_t)1 << 36;
+int64_t castle_optim_workspace_bytes(int count) { return count >= 0 && count <= 1 << 20 ? castle::optim_workspace(count) : CASTLE_ERR_SHAPE; }
+
+// step: a whole step, else the norm of the gradients alone
+static int optim_tensors_ok(const castle_optim_tensor* tensors, int count, int dtype, bool step) {
+  const int es = elem_size(dtype);
+  if (es == 0) return CASTLE_ERR_DTYPE;
+  if (count < 0 || count > 1 << 20) return CASTLE_ERR_SHAPE;
+  if (count > 0 && tensors == nullptr) return CASTLE_ERR_ARG;
+  int64_t all = 0;
+  for (int i = 0; i < count; ++i) {
+    const castle_optim_tensor& t = tensors[i];
+    if (t.n < 0 || t.n > kOptimElements || (all += t.n) > kOptimElements) return CASTLE_ERR_SHAPE;
+    const bool small = tensors[0].exp_avg_exponents != nullptr;
+    if (t.n > 0 && (t.grad == nullptr || reinterpret_cast<uintptr_t>(t.grad) % es != 0)) return CASTLE_ERR_ARG;
+    if (!step) continue;
+    if ((t.exp_avg_exponents != nullptr) != small || (t.exp_avg_sq_exponents != nullptr) != small) return CASTLE_ERR_ARG;
+    if (t.n > 0 && (t.param == nullptr || t.exp_avg == nullptr || t.exp_avg_sq == nullptr || reinterpret_cast<uintptr_t>(t.param) % es != 0 ||
+                    (!small && (reinterpret_cast<uintptr_t>(t.exp_avg) % 4 != 0 || reinterpret_cast<uintptr_t>(t.exp_avg_sq) % 4 != 0))))
+      return CASTLE_ERR_ARG;
+  }
+  return CASTLE_OK;
+}
+
+int castle_gradient_norm(const castle_optim_tensor* tensors, int count, float* norm, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = optim_tensors_ok(tensors, count, dtype, false)) return rc;
+  if (norm == nullptr || reinterpret_cast<uintptr_t>(norm) % 4 != 0) return CASTLE_ERR_ARG;
+  if (!workspace_ok(workspace, workspace_bytes, castle::optim_workspace(count))) return CASTLE_ERR_WORKSPACE;
+  return castle::launch_grad_norm(reinterpret_cast<const castle::OptimTensor*>(tensors), count, norm, dtype, workspace, static_cast<hipStream_t>(stream));
+}
+
+int castle_adamw(const castle_optim_tensor* tensors, int count, const castle_adamw_options* o, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = optim_tensors_ok(tensors, count, dtype, true)) return rc;
+  if (o == nullptr || o->step == nullptr || reinterpret_cast<uintptr_t>(o->step) % 8 != 0 || reinterpret_cast<uintptr_t>(o->seed) % 8 != 0 || reinterpret_cast<uintptr_t>(o->lr_device) % 4 != 0 ||
+      !(o->b1 >= 0 && o->b1 < 1) || !(o->b2 >= 0 && o->b2 < 1) || !(o->eps >= 0) || std::isnan(o->max_norm) || (o->max_norm >= 0 && (o->norm == nullptr || reinterpret_cast<uintptr_t>(o->norm) % 4 != 0)) ||
+      (count > 0 && tensors[0].exp_avg_exponents != nullptr && o->seed == nullptr))
+    return CASTLE_ERR_ARG;
+  if (!workspace_ok(workspace, workspace_bytes, castle::optim_workspace(count))) return CASTLE_ERR_WORKSPACE;
+  const castle::StepOptions s = {o->lr, o->b1, o->b2, o->eps, o->weight_decay, o->max_norm, o->lr_device, o->step, o->seed};
+  return castle::launch_adamw(reinterpret_cast<const castle::OptimTensor*>(tensors), count, s, o->max_norm >= 0 ? o->norm : nullptr, o->max_norm >= 0 && !o->norm_given, dtype, workspace,
+                              static_cast<hipStream_t>(stream));
 }
 
 int castle_profile_enable(int on) { return castle::profile_enable(on); }

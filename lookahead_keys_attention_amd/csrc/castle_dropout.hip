@@ -8,31 +8,15 @@
 // Bound by HBM, one pass: 65536 rows of 2048 bf16 with a residual 144 us (5.6 TB/s), the backward pass without one 83 us (6.5 TB/s).
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
+#include "castle_philox.h"
 #include "castle_tokens.h"
 
 namespace castle {
 namespace {
 
-struct Words { uint32_t w[4]; };
-__device__ __forceinline__ Words philox(uint64_t counter, uint64_t key, uint64_t at) {
-  uint32_t a = (uint32_t)counter, b = (uint32_t)(counter >> 32), c = (uint32_t)at, d = (uint32_t)(at >> 32), k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
-#pragma unroll
-  for (int round = 0; round < 10; ++round) {
-    const uint64_t p = (uint64_t)0xD2511F53u * a, q = (uint64_t)0xCD9E8D57u * c;
-    a = (uint32_t)(q >> 32) ^ b ^ k0;
-    c = (uint32_t)(p >> 32) ^ d ^ k1;
-    b = (uint32_t)q;
-    d = (uint32_t)p;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-  return {{a, b, c, d}};
-}
-
 // A dropped element is zero whatever x holds there: selected, not multiplied.
 template <typename T> __device__ __forceinline__ float kept(T x, const Words& r, int e, uint32_t threshold, float scale) {
-  const uint32_t u = r.w[e >> 1] >> (e & 1 ? 16 : 0) & 0xffffu;
-  return u >= threshold ? (float)x * scale : 0.f;
+  return half_of(r, e) >= threshold ? (float)x * scale : 0.f;
 }
 
 template <typename T, bool RESIDUAL> __global__ __launch_bounds__(kThreads) void dropout_kernel(DropoutArgs a) {

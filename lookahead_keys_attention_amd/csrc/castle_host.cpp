@@ -16,6 +16,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <limits>
 #include <optional>
 #include <tuple>
@@ -1316,6 +1317,358 @@ Tensor dropout_autograd(const Tensor& x, const std::optional<Tensor>& residual, 
   return DropoutFn::apply(x, residual, p, seed);
 }
 
+// ---- gated feed-forward block ---------------------------------------------------------------------------------------
+struct GatedCall {
+  Tensor x, w_in, w_out;
+  castle_gated a;
+  int dtype;
+  GatedCall(const Tensor& x_, const Tensor& w_in_, const Tensor& w_out_, int64_t activation) {
+    dtype = dtype_code(x_);
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && w_in_.dim() == 2 && w_out_.dim() == 2 && w_in_.size(1) == x_.size(-1) && w_out_.size(0) == x_.size(-1) && w_in_.size(0) == 2 * w_out_.size(1),
+                      "gated_feed_forward: x is (..., D), weight_in (2 F, D) and weight_out (D, F), got ", x_.sizes(), ", ", w_in_.sizes(), " and ", w_out_.sizes());
+    for (const Tensor* t : {&w_in_, &w_out_})
+      TORCH_CHECK_VALUE(t->scalar_type() == x_.scalar_type() && t->device() == x_.device(), "gated_feed_forward: x and the weights are of one type on one device");
+    TORCH_CHECK_VALUE(activation == CASTLE_GATE_SILU || activation == CASTLE_GATE_GELU, "gated_feed_forward: unknown activation");
+    const int64_t D = x_.size(-1), F = w_out_.size(1), R = D ? x_.numel() / D : 0;
+    TORCH_CHECK_VALUE(D > 0 && D % 8 == 0 && F > 0 && F % 8 == 0 && D <= 1 << 20 && F <= 1 << 20, "gated_feed_forward: widths are multiples of 8 up to 2^20, got D = ", D, " and F = ", F);
+    TORCH_CHECK_VALUE(R <= INT32_MAX && castle_gemm_operand_ok(R, 2 * F) && castle_gemm_operand_ok(R, D) && castle_gemm_operand_ok(2 * F, D) && castle_gemm_operand_ok(D, F),
+                      "gated_feed_forward: operands of less than 2^31 elements, (rows + 192) x 2 F among them, got ", R, " rows, D = ", D, " and F = ", F);
+    x = rows_of_eight(x_.reshape({R, D}));
+    w_in = rows_of_eight(w_in_);
+    w_out = rows_of_eight(w_out_);
+    auto near = [](Tensor& t) { if (!castle_gemm_operand_ok(t.size(0), t.stride(0)) || t.stride(0) < t.size(1)) t = t.clone(at::MemoryFormat::Contiguous); };
+    near(x);
+    near(w_in);
+    near(w_out);
+    a = {x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), x.stride(0), w_in.stride(0), w_out.stride(0), (int32_t)R, (int32_t)D, (int32_t)F, (int32_t)activation};
+  }
+};
+std::tuple<Tensor, Tensor> gated_op(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t activation, bool keep_state) {
+  require_gpu(x, "gated_feed_forward");
+  const c10::DeviceGuard guard(x.device());
+  const GatedCall c(x, w_in, w_out, activation);
+  Tensor y = at::empty(x.sizes(), x.options());
+  if (c.a.rows == 0) return {y, bytes(0, x)};
+  const int64_t sbytes = keep_state ? check(castle_gated_state_bytes(c.a.rows, c.a.dim, c.a.hidden, c.dtype), "castle_gated_state_bytes") : 0;
+  const int64_t nbytes = check(castle_gated_workspace_bytes(c.a.rows, c.a.dim, c.a.hidden, c.dtype, keep_state), "castle_gated_workspace_bytes");
+  Tensor state = bytes(sbytes, x), ws = bytes(nbytes, x);
+  check(castle_gated_feed_forward(&c.a, y.data_ptr(), keep_state ? state.data_ptr() : nullptr, sbytes, c.dtype, ws.data_ptr(), nbytes, stream_of(x)), "castle_gated_feed_forward");
+  return {y, state};
+}
+// (a gradient that is not asked for comes back empty)
+std::tuple<Tensor, Tensor, Tensor> gated_bwd_op(const Tensor& dy_, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const Tensor& state, int64_t activation, bool need_x,
+                                                bool need_in, bool need_out) {
+  require_gpu(x, "gated_feed_forward_bwd");
+  const c10::DeviceGuard guard(x.device());
+  const GatedCall c(x, w_in, w_out, activation);
+  TORCH_CHECK_VALUE(dy_.sizes() == x.sizes() && dy_.scalar_type() == x.scalar_type() && dy_.device() == x.device(), "gated_feed_forward_bwd: the gradient has another shape, type or device");
+  TORCH_CHECK_VALUE(state.scalar_type() == at::kByte && state.dim() == 1 && state.is_contiguous() && state.device() == x.device(),
+                    "gated_feed_forward_bwd: the state is what the forward pass has returned, on ", x.device());
+  auto result = [&](bool need, const Tensor& like) { return need ? at::empty(like.sizes(), like.options()) : at::empty({0}, like.options()); };
+  Tensor dx = result(need_x, x), din = result(need_in, w_in), dout = result(need_out, w_out);
+  if (c.a.rows == 0) {
+    din.zero_();
+    dout.zero_();
+  }
+  if (c.a.rows == 0 || !(need_x || need_in || need_out)) return {dx, din, dout};
+  const Tensor dy = row_major(dy_);
+  const int64_t nbytes = check(castle_gated_bwd_workspace_bytes(c.a.rows, c.a.dim, c.a.hidden, c.dtype, need_x + 2 * need_in + 4 * need_out), "castle_gated_bwd_workspace_bytes");
+  Tensor ws = bytes(nbytes, x);
+  check(castle_gated_feed_forward_bwd(&c.a, dy.data_ptr(), state.data_ptr(), state.numel(), need_x ? dx.data_ptr() : nullptr, need_in ? din.data_ptr() : nullptr,
+                                      need_out ? dout.data_ptr() : nullptr, c.dtype, ws.data_ptr(), nbytes, stream_of(x)),
+        "castle_gated_feed_forward_bwd");
+  return {dx, din, dout};
+}
+struct GatedFn : torch::autograd::Function<GatedFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t activation) {
+    static const auto op = op_handle<decltype(gated_op)>("castle_hip::gated_feed_forward");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, state] = op.call(x, w_in, w_out, activation, true);
+    ctx->save_for_backward({x, w_in, w_out, state});
+    ctx->saved_data["activation"] = activation;
+    ctx->mark_non_differentiable({state});
+    ctx->set_materialize_grads(false);
+    return {y, state};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    static const auto op = op_handle<decltype(gated_bwd_op)>("castle_hip::gated_feed_forward_bwd");
+    if (!g[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto s = ctx->get_saved_variables();
+    const bool need_x = ctx->needs_input_grad(0), need_in = ctx->needs_input_grad(1), need_out = ctx->needs_input_grad(2);
+    auto [dx, din, dout] = op.call(g[0], s[0], s[1], s[2], s[3], ctx->saved_data["activation"].toInt(), need_x, need_in, need_out);
+    return {need_x ? dx : Tensor(), need_in ? din : Tensor(), need_out ? dout : Tensor(), Tensor()};
+  }
+};
+std::tuple<Tensor, Tensor, Tensor> gated_bwd_autograd(const Tensor& dy, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const Tensor& state, int64_t activation, bool need_x,
+                                                      bool need_in, bool need_out) {
+  static const auto op = op_handle<decltype(gated_bwd_op)>("castle_hip::gated_feed_forward_bwd");
+  const bool graph = wants_graph({dy, x, w_in, w_out});
+  const at::AutoDispatchBelowADInplaceOrView below;
+  const auto [dx, din, dout] = op.call(dy, x, w_in, w_out, state, activation, need_x, need_in, need_out);
+  if (!graph) return {dx, din, dout};
+  const auto r = no_second_derivatives({dx, din, dout});
+  return {r[0], r[1], r[2]};
+}
+std::tuple<Tensor, Tensor> gated_autograd(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t activation, bool keep_state) {
+  if (!wants_graph({x, w_in, w_out})) {
+    static const auto op = op_handle<decltype(gated_op)>("castle_hip::gated_feed_forward");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(x, w_in, w_out, activation, keep_state);
+  }
+  auto r = GatedFn::apply(x, w_in, w_out, activation);
+  return {r[0], r[1]};
+}
+
+// ---- norms on both sides of a residual sum ----------------------------------------------------------------------------
+using OptTensor = std::optional<Tensor>;
+struct ResidualCall {
+  Tensor x, residual, w, scale, gate, next;
+  castle_residual a;
+  int dtype;
+  ResidualCall(const Tensor& x_, const Tensor& residual_, const OptTensor& w_, const OptTensor& scale_, const OptTensor& gate_, const OptTensor& next_, double eps) {
+    dtype = dtype_code(x_);
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && residual_.sizes() == x_.sizes(), "residual_norm: x and the residual have one shape (..., D), got ", x_.sizes(), " and ", residual_.sizes());
+    TORCH_CHECK_VALUE(eps >= 0, "residual_norm: eps is not negative, got ", eps);
+    const int64_t n = x_.dim(), D = x_.size(-1);
+    TORCH_CHECK_VALUE(D > 0 && D <= CASTLE_RESIDUAL_MAX_WIDTH, "residual_norm: rows of 1 to ", CASTLE_RESIDUAL_MAX_WIDTH, " elements, got ", D);
+    auto take = [&](const OptTensor& t) -> Tensor {
+      if (!t) return Tensor();
+      TORCH_CHECK_VALUE(t->scalar_type() == x_.scalar_type() && t->device() == x_.device(), "residual_norm: all tensors are of one type on one device");
+      return t->contiguous();
+    };
+    for (const OptTensor* t : {&w_, &scale_, &next_})
+      TORCH_CHECK_VALUE(!*t || ((*t)->dim() == 1 && (*t)->size(0) == D), "residual_norm: weights and scale have one number for each of ", D, " columns");
+    int64_t span = 1;
+    if (gate_) {
+      // the leading axes of x, then ones: a gate of each row, of each sequence, of all
+      const Tensor& g = *gate_;
+      bool ok = g.dim() == n && g.size(-1) == D, shared = false;
+      if (g.dim() == 1 && n > 1 && g.size(0) == D) {
+        ok = true;
+        for (int64_t i = 0; i < n - 1; ++i) span *= x_.size(i);
+      } else {
+        for (int64_t i = 0; ok && i < n - 1; ++i) {
+          if (!shared && g.size(i) == x_.size(i)) continue;
+          shared = true;
+          ok = g.size(i) == 1;
+          span *= x_.size(i);
+        }
+      }
+      TORCH_CHECK_VALUE(ok, "residual_norm: the gate has the shape of x, or ones behind some of its leading axes, then D; got ", g.sizes(), " for ", x_.sizes());
+    }
+    x = take(x_);
+    residual = take(residual_);
+    w = take(w_);
+    scale = take(scale_);
+    gate = take(gate_);
+    next = take(next_);
+    auto ptr = [](const Tensor& t) -> const void* { return t.defined() ? t.data_ptr() : nullptr; };
+    a = {ptr(x), ptr(residual), ptr(w), ptr(scale), ptr(gate), ptr(next), x.numel() / D, span, (int32_t)D, (float)eps, nullptr, nullptr};
+  }
+};
+Tensor row_numbers(const Tensor& like, int64_t n) { return at::empty({n}, like.options().dtype(at::kFloat)); }
+std::tuple<Tensor, Tensor, Tensor, Tensor> residual_norm_op(const Tensor& x, const Tensor& residual, const OptTensor& w, const OptTensor& scale, const OptTensor& gate, const OptTensor& next,
+                                                            double eps, bool keep) {
+  require_gpu(x, "residual_norm");
+  const c10::DeviceGuard guard(x.device());
+  ResidualCall c(x, residual, w, scale, gate, next, eps);
+  const int64_t R = c.a.rows;
+  Tensor y = at::empty(x.sizes(), x.options()), h = next ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  Tensor rstd = row_numbers(x, keep && w ? R : 0), next_rstd = row_numbers(x, keep && next ? R : 0);
+  if (R == 0) return {y, h, rstd, next_rstd};
+  if (keep && w) c.a.rstd = static_cast<float*>(rstd.data_ptr());
+  if (keep && next) c.a.next_rstd = static_cast<float*>(next_rstd.data_ptr());
+  check(castle_residual_norm(&c.a, y.data_ptr(), next ? h.data_ptr() : nullptr, c.dtype, stream_of(x)), "castle_residual_norm");
+  return {y, h, rstd, next_rstd};
+}
+using SixTensors = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+// need: a bit for each of x, residual, weight, scale, gate, next_weight, from the lowest on; what is not asked for comes back empty
+SixTensors residual_norm_bwd_op(const OptTensor& dy_, const OptTensor& dh_, const Tensor& x, const Tensor& residual, const OptTensor& w, const OptTensor& scale, const OptTensor& gate,
+                                const OptTensor& next, const Tensor& rstd, const Tensor& next_rstd, double eps, int64_t need) {
+  require_gpu(x, "residual_norm_bwd");
+  const c10::DeviceGuard guard(x.device());
+  ResidualCall c(x, residual, w, scale, gate, next, eps);
+  const int64_t R = c.a.rows;
+  for (const OptTensor* d : {&dy_, &dh_})
+    TORCH_CHECK_VALUE(!*d || ((*d)->sizes() == x.sizes() && (*d)->scalar_type() == x.scalar_type() && (*d)->device() == x.device()), "residual_norm_bwd: a gradient has another shape, type or device");
+  TORCH_CHECK_VALUE(dy_ || (dh_ && next), "residual_norm_bwd: no gradient");
+  auto rows_ok = [&](const Tensor& t, bool there) { return t.scalar_type() == at::kFloat && t.is_contiguous() && t.device() == x.device() && (!there || t.numel() == R); };
+  TORCH_CHECK_VALUE(rows_ok(rstd, w.has_value()) && rows_ok(next_rstd, dh_ && next), "residual_norm_bwd: the rows' factors are what the forward pass has returned");
+  const Tensor dy = dy_ ? dy_->contiguous() : Tensor(), dh = dh_ && next ? dh_->contiguous() : Tensor();
+  const OptTensor like[6] = {x, residual, w, scale, gate, next};
+  Tensor d[6];
+  void* p[6];
+  for (int i = 0; i < 6; ++i) {
+    const bool there = need >> i & 1 && like[i];
+    d[i] = there ? at::empty(like[i]->sizes(), like[i]->options()) : at::empty({0}, x.options());
+    p[i] = there ? d[i].data_ptr() : nullptr;
+    if (there && (R == 0 || (i == 5 && !dh.defined()))) {
+      d[i].zero_();
+      p[i] = nullptr;
+    }
+  }
+  if (R > 0) {
+    if (w) c.a.rstd = static_cast<float*>(rstd.data_ptr());
+    if (dh.defined()) c.a.next_rstd = static_cast<float*>(next_rstd.data_ptr());
+    const castle_residual_grads g = {dy.defined() ? dy.data_ptr() : nullptr, dh.defined() ? dh.data_ptr() : nullptr, p[0], p[1], p[2], p[3], p[4], p[5]};
+    const int64_t nbytes = check(castle_residual_norm_bwd_workspace_bytes(&c.a, &g, c.dtype), "castle_residual_norm_bwd_workspace_bytes");
+    const Tensor ws = nbytes ? bytes(nbytes, x) : Tensor();
+    check(castle_residual_norm_bwd(&c.a, &g, c.dtype, nbytes ? ws.data_ptr() : nullptr, nbytes, stream_of(x)), "castle_residual_norm_bwd");
+  }
+  return {d[0], d[1], d[2], d[3], d[4], d[5]};
+}
+struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const OptTensor& w, const OptTensor& scale, const OptTensor& gate, const OptTensor& next, double eps) {
+    static const auto op = op_handle<decltype(residual_norm_op)>("castle_hip::residual_norm");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, h, rstd, next_rstd] = op.call(x, residual, w, scale, gate, next, eps, true);
+    ctx->save_for_backward({x, residual, w.value_or(Tensor()), scale.value_or(Tensor()), gate.value_or(Tensor()), next.value_or(Tensor()), rstd, next_rstd});
+    ctx->saved_data["eps"] = eps;
+    if (next) ctx->mark_non_differentiable({rstd, next_rstd});
+    else ctx->mark_non_differentiable({h, rstd, next_rstd});
+    ctx->set_materialize_grads(false);
+    return {y, h, rstd, next_rstd};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    static const auto op = op_handle<decltype(residual_norm_bwd_op)>("castle_hip::residual_norm_bwd");
+    variable_list grads(7);
+    if (!g[0].defined() && !g[1].defined()) return grads;
+    const auto s = ctx->get_saved_variables();
+    auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    int64_t need = 0;
+    size_t seen = 0;   // (needs_input_grad counts the tensors that were there)
+    for (int i = 0; i < 6; ++i)
+      if (s[i].defined() && ctx->needs_input_grad(seen++)) need |= 1 << i;
+    const auto [dx, dr, dw, ds, dg, dn] =
+        op.call(opt(g[0]), opt(g[1]), s[0], s[1], opt(s[2]), opt(s[3]), opt(s[4]), opt(s[5]), s[6], s[7], ctx->saved_data["eps"].toDouble(), need);
+    const Tensor d[6] = {dx, dr, dw, ds, dg, dn};
+    for (int i = 0; i < 6; ++i)
+      if (need >> i & 1) grads[i] = d[i];
+    return grads;
+  }
+};
+SixTensors residual_norm_bwd_autograd(const OptTensor& dy, const OptTensor& dh, const Tensor& x, const Tensor& residual, const OptTensor& w, const OptTensor& scale, const OptTensor& gate,
+                                      const OptTensor& next, const Tensor& rstd, const Tensor& next_rstd, double eps, int64_t need) {
+  static const auto op = op_handle<decltype(residual_norm_bwd_op)>("castle_hip::residual_norm_bwd");
+  const auto t = [](const OptTensor& o) { return o.value_or(Tensor()); };
+  const bool graph = wants_graph({t(dy), t(dh), x, residual, t(w), t(scale), t(gate), t(next)});
+  const at::AutoDispatchBelowADInplaceOrView below;
+  const auto d = op.call(dy, dh, x, residual, w, scale, gate, next, rstd, next_rstd, eps, need);
+  if (!graph) return d;
+  const auto r = no_second_derivatives({std::get<0>(d), std::get<1>(d), std::get<2>(d), std::get<3>(d), std::get<4>(d), std::get<5>(d)});
+  return {r[0], r[1], r[2], r[3], r[4], r[5]};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> residual_norm_autograd(const Tensor& x, const Tensor& residual, const OptTensor& w, const OptTensor& scale, const OptTensor& gate,
+                                                                  const OptTensor& next, double eps, bool keep) {
+  const auto t = [](const OptTensor& o) { return o.value_or(Tensor()); };
+  if (!wants_graph({x, residual, t(w), t(scale), t(gate), t(next)})) {
+    static const auto op = op_handle<decltype(residual_norm_op)>("castle_hip::residual_norm");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(x, residual, w, scale, gate, next, eps, keep);
+  }
+  auto r = ResidualNormFn::apply(x, residual, w, scale, gate, next, eps);
+  return {r[0], r[1], r[2], r[3]};
+}
+
+// ---- AdamW over many tensors ----------------------------------------------------------------------------------------
+void check_gradients(const std::vector<Tensor>& grads, const char* what) {
+  TORCH_CHECK_VALUE(!grads.empty(), what, ": no tensors");
+  for (const Tensor& g : grads) {
+    require_gpu(g, what);
+    TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.scalar_type() == grads[0].scalar_type() && g.device() == grads[0].device(), what, ": dense tensors of one type on one device");
+  }
+  dtype_code(grads[0]);
+}
+Tensor gradient_norm(const std::vector<Tensor>& grads) {
+  check_gradients(grads, "gradient_norm");
+  const c10::DeviceGuard guard(grads[0].device());
+  std::vector<Tensor> keep;
+  std::vector<castle_optim_tensor> t(grads.size());
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor g = grads[i].is_non_overlapping_and_dense() ? grads[i] : grads[i].contiguous();
+    keep.push_back(g);
+    t[i] = {nullptr, g.data_ptr(), nullptr, nullptr, nullptr, nullptr, g.numel()};
+  }
+  const int64_t nbytes = check(castle_optim_workspace_bytes((int)t.size()), "castle_optim_workspace_bytes");
+  const Tensor ws = bytes(nbytes, grads[0]);
+  Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+  check(castle_gradient_norm(t.data(), (int)t.size(), static_cast<float*>(norm.data_ptr()), dtype_code(grads[0]), ws.data_ptr(), nbytes, stream_of(ws)), "castle_gradient_norm");
+  return norm;
+}
+
+// in place; -> the norm of the gradients where they are clipped
+OptTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& avgs, const std::vector<Tensor>& sqs,
+                     const std::optional<std::vector<Tensor>>& avg_exponents, const std::optional<std::vector<Tensor>>& sq_exponents, const Tensor& step, double lr, const OptTensor& lr_device,
+                     double b1, double b2, double eps, double weight_decay, std::optional<double> max_norm, const OptTensor& norm_given, const OptTensor& seed) {
+  const char* what = "adamw_step";
+  check_gradients(params, what);
+  check_gradients(grads, what);
+  const size_t n = params.size();
+  const bool small = avg_exponents.has_value();
+  const at::Device device = params[0].device();
+  TORCH_CHECK_VALUE(grads.size() == n && avgs.size() == n && sqs.size() == n && sq_exponents.has_value() == small && (!small || (avg_exponents->size() == n && sq_exponents->size() == n)),
+                    "adamw_step: a gradient and two states for each parameter, exponents for both states or for none");
+  TORCH_CHECK_VALUE(grads[0].scalar_type() == params[0].scalar_type() && grads[0].device() == device, "adamw_step: gradients have the type and the device of their parameters");
+  TORCH_CHECK_VALUE(b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1 && eps >= 0 && weight_decay >= 0, "adamw_step: betas in [0, 1), eps and weight_decay not negative");
+  TORCH_CHECK_VALUE(!max_norm || *max_norm >= 0, "adamw_step: max_norm is not negative");
+  TORCH_CHECK_VALUE(!small || seed, "adamw_step: states of 8 bits are rounded by chance, which takes a seed");
+  auto one = [&](const Tensor& t, at::ScalarType type) { return t.scalar_type() == type && t.numel() == 1 && t.device() == device; };
+  TORCH_CHECK_VALUE(one(step, at::kLong) && (!seed || one(*seed, at::kLong)), "adamw_step: step and seed are int64 tensors of one element on ", device);
+  TORCH_CHECK_VALUE((!lr_device || one(*lr_device, at::kFloat)) && (!norm_given || one(*norm_given, at::kFloat)), "adamw_step: a learning rate or norm in a tensor is one float32 number on ", device);
+  const c10::DeviceGuard guard(device);
+  std::vector<Tensor> keep;
+  std::vector<castle_optim_tensor> t(n);
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  written.reserve(3 * n);
+  const at::ScalarType state_type = small ? at::kFloat8_e4m3fn : at::kFloat;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &p = params[i], &m = avgs[i], &v = sqs[i];
+    TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense(), "adamw_step: parameter ", i, " has gaps or elements that share memory");
+    TORCH_CHECK_VALUE(grads[i].sizes() == p.sizes(), "adamw_step: gradient ", i, " has another shape than its parameter");
+    auto fits = [&](const Tensor& s) { return s.sizes() == p.sizes() && (s.strides() == p.strides() || p.numel() <= 1) && s.scalar_type() == state_type && s.device() == device; };
+    TORCH_CHECK_VALUE(fits(m) && fits(v), "adamw_step: states ", i, " are ", state_type, " tensors with the shape and strides of their parameter on ", device);
+    Tensor g = grads[i];
+    if (g.strides() != p.strides() && p.numel() > 1) {
+      g = at::empty_strided(p.sizes(), p.strides(), g.options());
+      g.copy_(grads[i]);
+      keep.push_back(g);
+    }
+    t[i] = {p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), nullptr, nullptr, p.numel()};
+    if (small) {
+      const Tensor &em = (*avg_exponents)[i], &ev = (*sq_exponents)[i];
+      auto exponents = [&](const Tensor& e) { return e.scalar_type() == at::kChar && e.is_contiguous() && e.numel() == (p.numel() + 255) / 256 && e.device() == device; };
+      TORCH_CHECK_VALUE(exponents(em) && exponents(ev), "adamw_step: exponents ", i, " are contiguous int8 tensors, one number for 256 elements, on ", device);
+      t[i].exp_avg_exponents = static_cast<int8_t*>(em.data_ptr());
+      t[i].exp_avg_sq_exponents = static_cast<int8_t*>(ev.data_ptr());
+      if (p.numel() == 0) t[i].exp_avg_exponents = t[i].exp_avg_sq_exponents = reinterpret_cast<int8_t*>(1);   // (nothing is read or written)
+    }
+    for (const Tensor* w : {&p, &m, &v})
+      if (w->numel() > 0) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(w->data_ptr());
+        written.emplace_back(at, at + w->numel() * w->element_size());
+      }
+  }
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i) TORCH_CHECK_VALUE(written[i - 1].second <= written[i].first, "adamw_step: two parameters or states share memory");
+  OptTensor norm = norm_given;
+  if (max_norm && !norm) norm = at::empty({}, params[0].options().dtype(at::kFloat).requires_grad(false));
+  const castle_adamw_options o = {lr, b1, b2, eps, weight_decay, max_norm.value_or(-1), lr_device ? static_cast<const float*>(lr_device->data_ptr()) : nullptr,
+                                  static_cast<int64_t*>(step.data_ptr()), seed ? static_cast<const int64_t*>(seed->data_ptr()) : nullptr,
+                                  max_norm ? static_cast<float*>(norm->data_ptr()) : nullptr, norm_given.has_value()};
+  const int64_t nbytes = check(castle_optim_workspace_bytes((int)n), "castle_optim_workspace_bytes");
+  const Tensor ws = bytes(nbytes, params[0]);
+  check(castle_adamw(t.data(), (int)n, &o, dtype_code(params[0]), ws.data_ptr(), nbytes, stream_of(ws)), "castle_adamw");
+  // whoever keeps one of these for a backward pass is told that it has changed
+  auto changed = [](const Tensor& x) { if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version(); };
+  for (size_t i = 0; i < n; ++i) {
+    changed(params[i]);
+    changed(avgs[i]);
+    changed(sqs[i]);
+  }
+  changed(step);
+  return max_norm ? norm : OptTensor();
+}
+
 // ---- the cached single-token step ------------------------------------------------------------------------------
 // rows of a matrix that the kernels can read 16 bytes at a time
 bool rows_readable(const Tensor& t) {
@@ -1519,6 +1872,12 @@ TORCH_LIBRARY(castle_hip, m) {
   m.def("embedding(Tensor weight, Tensor index, float scale, int padding_idx) -> Tensor", tags);
   m.def("embedding_bwd(Tensor dy, Tensor index, int vocabulary, float scale, int padding_idx) -> Tensor", tags);
   m.def("dropout_add(Tensor x, Tensor? residual, float p, Tensor seed) -> Tensor", tags);
+  m.def("gated_feed_forward(Tensor x, Tensor weight_in, Tensor weight_out, int activation, bool keep_state) -> (Tensor, Tensor)", tags);
+  m.def("gated_feed_forward_bwd(Tensor dy, Tensor x, Tensor weight_in, Tensor weight_out, Tensor state, int activation, bool need_x=True, bool need_in=True, bool need_out=True) "
+        "-> (Tensor, Tensor, Tensor)", tags);
+  m.def("residual_norm(Tensor x, Tensor residual, Tensor? weight, Tensor? scale, Tensor? gate, Tensor? next_weight, float eps, bool keep) -> (Tensor, Tensor, Tensor, Tensor)", tags);
+  m.def("residual_norm_bwd(Tensor? dy, Tensor? dh, Tensor x, Tensor residual, Tensor? weight, Tensor? scale, Tensor? gate, Tensor? next_weight, Tensor rstd, Tensor next_rstd, float eps, "
+        "int need) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", tags);
 }
 TORCH_LIBRARY_IMPL(castle_hip, CUDA, m) {
   m.impl("attention", &attention);
@@ -1534,6 +1893,10 @@ TORCH_LIBRARY_IMPL(castle_hip, CUDA, m) {
   m.impl("embedding", &embedding_op);
   m.impl("embedding_bwd", &embedding_bwd_op);
   m.impl("dropout_add", &dropout_op);
+  m.impl("gated_feed_forward", &gated_op);
+  m.impl("gated_feed_forward_bwd", &gated_bwd_op);
+  m.impl("residual_norm", &residual_norm_op);
+  m.impl("residual_norm_bwd", &residual_norm_bwd_op);
 }
 // CPU tensors: an error that says what is wrong
 TORCH_LIBRARY_IMPL(castle_hip, CPU, m) {
@@ -1542,6 +1905,8 @@ TORCH_LIBRARY_IMPL(castle_hip, CPU, m) {
   m.impl("linear_cross_entropy", &linear_cross_entropy_op);
   m.impl("embedding", &embedding_op);
   m.impl("dropout_add", &dropout_op);
+  m.impl("gated_feed_forward", &gated_op);
+  m.impl("residual_norm", &residual_norm_op);
 }
 TORCH_LIBRARY_IMPL(castle_hip, Autograd, m) {
   m.impl("attention", &attention_autograd);
@@ -1557,6 +1922,10 @@ TORCH_LIBRARY_IMPL(castle_hip, Autograd, m) {
   m.impl("embedding", &embedding_autograd);
   m.impl("embedding_bwd", &embedding_bwd_autograd);
   m.impl("dropout_add", &dropout_autograd);
+  m.impl("gated_feed_forward", &gated_autograd);
+  m.impl("gated_feed_forward_bwd", &gated_bwd_autograd);
+  m.impl("residual_norm", &residual_norm_autograd);
+  m.impl("residual_norm_bwd", &residual_norm_bwd_autograd);
 }
 
 PYBIND11_MODULE(_castle_host, m) {
@@ -1575,6 +1944,8 @@ PYBIND11_MODULE(_castle_host, m) {
   m.def("embedding", &embedding, py::arg("weight"), py::arg("index"), py::arg("scale") = 1.0, unlocked());
   m.def("small_linear", &small_linear, unlocked());
   m.def("sample_tokens", &sample_tokens, unlocked());
+  m.def("gradient_norm", &gradient_norm, unlocked());
+  m.def("adamw_step", &adamw_step, unlocked());
   m.def("gather_rows", &gather_rows, unlocked());
   py::class_<StepPlan>(m, "StepPlan")
       .def(py::init<std::vector<Tensor>, Tensor, Tensor, Tensor, bool>())

@@ -1,0 +1,331 @@
+// A step of AdamW over many tensors and the norm of their gradients.
+//
+//   g' = c g, c = min(1, max_norm / (norm + 1e-6))      m = b1 m + (1 - b1) g'        v = b2 v + (1 - b2) g'^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// States of 8 bits: 256 elements share 2^E, the least power of two with which the largest of them is at most 448, and are e4m3 numbers times that: m, and r = sqrt(v), whose
+// range is half of v's in octaves.  They are rounded up or down by chance, so that the mean is kept.  To the nearest, a state would stay where it is: a step with b2 = 0.999 moves r by
+// 0.05 %, steps of e4m3 are 6 to 12 %.  A second moment that is not zero stays above zero (2^-18 of the largest): as zero its element would move by lr m / eps.  16-bit
+// parameters are rounded by chance too where there is a seed: lr = 1e-4 moves none of bf16 to the nearest.
+// Every number is formed by single 32-bit operations, rounded each (no contraction), in the order of the formulas.
+//
+// Bound by HBM: per element of 16 bits 10 bytes with states of 8 bits, 22 with 32, 28 of fp32, and the gradients once more for their norm, which has to be there before the first element.
+// Tensors go 64 to a launch, their addresses in its arguments: a table in memory would have to be written anew for every step, as gradients move.
+#include "castle_tiles.h"
+#include "castle_dispatch.h"
+#include "castle_optim.h"
+#include "castle_philox.h"
+#include <algorithm>
+
+namespace castle {
+namespace {
+
+constexpr int kGroup = kThreads * 8;      // elements of a workgroup's turn, eight a thread
+constexpr int kTurns = 4;                 // turns of a workgroup
+constexpr int kWaves = kThreads / 64;
+
+// rows of any alignment (gfx950 reads and writes them at the speed of aligned ones where they are aligned)
+template <typename T> using any8 = vec<T, 8> __attribute__((aligned(1)));
+
+struct LaunchTensors {
+  OptimTensor t[kTensorsOfLaunch];
+  uint32_t first[kTensorsOfLaunch];   // piece (kGroup * kTurns elements) that each begins with; behind the last tensor the number of pieces
+  int count, number;                  // number: of the first tensor, in the whole call
+};
+static_assert(sizeof(LaunchTensors) + 64 <= 4096, "arguments of a launch");
+
+// the tensor that a piece lies in: every lane looks at one of them
+__device__ __forceinline__ int tensor_of(const LaunchTensors& a, uint32_t piece) {
+  const int i = min(lane_id(), a.count - 1);
+  const uint64_t begun = __ballot(lane_id() < a.count && a.first[i] <= piece);
+  return 63 - __builtin_clzll(begun);   // (sizes of zero are left out on the host, so firsts grow)
+}
+
+template <typename T> __device__ __forceinline__ vec<float, 8> read8(const T* p, int left) {
+  vec<float, 8> x = {};
+  if (left >= 8) {
+    x = __builtin_convertvector((frag<T>)*reinterpret_cast<const any8<T>*>(p), decltype(x));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) x[e] = (float)p[e];
+  }
+  return x;
+}
+template <typename T> __device__ __forceinline__ void write8(T* p, vec<T, 8> x, int left) {
+  if (left >= 8) {
+    *reinterpret_cast<any8<T>*>(p) = x;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) p[e] = x[e];
+  }
+}
+
+// ---- norm ----------------------------------------------------------------------------------------------------------
+// Sums of squares in double: of the largest floats they do not overflow, of the smallest they do not vanish, and the adds (two instructions an element) hide behind the reads.
+template <typename T> __global__ __launch_bounds__(kThreads) void norm_parts_kernel(LaunchTensors a, uint32_t pieces, double* parts) {
+  __shared__ double s[kWaves];
+  double sum[2] = {0, 0};
+  for (uint32_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+    const int k = __builtin_amdgcn_readfirstlane(tensor_of(a, piece));
+    const OptimTensor& t = a.t[k];
+    const T* g = static_cast<const T*>(t.g);
+    const int64_t begin = (int64_t)(piece - a.first[k]) * (kGroup * kTurns) + threadIdx.x * 8;
+    vec<float, 8> x[kTurns];
+#pragma unroll
+    for (int j = 0; j < kTurns; ++j) {
+      const int64_t at = begin + j * kGroup;
+      x[j] = at < t.n ? read8(g + at, (int)min((int64_t)8, t.n - at)) : vec<float, 8>{};
+    }
+#pragma unroll
+    for (int j = 0; j < kTurns; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e & 1] = __builtin_fma((double)x[j][e], (double)x[j][e], sum[e & 1]);
+  }
+  double v = sum[0] + sum[1];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  if (lane_id() == 0) s[wave_id()] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += s[w];
+    parts[blockIdx.x] = v;
+  }
+}
+
+// One workgroup: the norm of `parts` partial sums (if there are any), and the numbers of a step (if one follows)
+__global__ __launch_bounds__(1024) void begin_kernel(const double* parts, int count, float* norm, StepOptions o, StepNumbers* numbers) {
+#pragma clang fp contract(off)
+  __shared__ double s[16];
+  double v = 0;
+  for (int i = threadIdx.x; i < count; i += 1024) v += parts[i];
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) v += __shfl_xor(v, k);
+  if (lane_id() == 0) s[wave_id()] = v;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  float n = 0.f;
+  if (parts != nullptr) {
+    for (int w = 1; w < 16; ++w) v += s[w];
+    n = (float)sqrt(v);
+    *norm = n;
+  } else if (norm != nullptr) {
+    n = *norm;
+  }
+  if (numbers == nullptr) return;
+  StepNumbers r = {};
+  const int64_t t = *o.step + 1;
+  *o.step = t;
+  const double lr = o.lr_device != nullptr ? (double)*o.lr_device : o.lr;
+  r.clip = 1.f;
+  if (o.max_norm >= 0) {
+    const float c = (float)o.max_norm / (n + 1e-6f);
+    r.clip = c > 1.f ? 1.f : c;   // (a NaN stays one)
+  }
+  r.rate = (float)(lr / (1 - pow(o.b1, (double)t)));
+  r.root = (float)(1 / sqrt(1 - pow(o.b2, (double)t)));
+  r.keep = (float)(1 - lr * o.weight_decay);
+  r.step = (uint32_t)t;
+  *numbers = r;
+}
+
+// ---- step ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+
+__device__ __forceinline__ float from_e4m3(uint32_t code) {
+  const uint32_t mag = code & 0x7f;
+  const float normal = __builtin_bit_cast(float, (mag << 20) + (120u << 23)), low = (float)mag * 0x1p-9f;
+  const float x = mag == 0x7f ? NAN : mag < 8 ? low : normal;
+  return code & 0x80 ? -x : x;
+}
+// |s| <= 448 (or it is infinite or NaN); u: 16 random bits
+template <bool POSITIVE> __device__ __forceinline__ uint32_t to_e4m3(float s, uint32_t u) {
+#pragma clang fp contract(off)
+  const uint32_t bits = __builtin_bit_cast(uint32_t, s), mag = bits & 0x7fffffff;
+  const float a = fabsf(s);
+  uint32_t code = a < 0x1p-6f ? (uint32_t)(a * 512.f + (float)u * 0x1p-16f) : ((mag + (u << 4)) >> 20) - 960;
+  if (POSITIVE && mag != 0) code = max(code, 1u);
+  if (mag >= 0x7f800000u) code = 0x7f;
+  return code | (bits >> 31) << 7;
+}
+// E of 256 elements, 32 lanes of them, from the largest |x| that is finite
+__device__ __forceinline__ int exponent_of(const vec<float, 8>& x) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, (float)x[e]) & 0x7fffffff;
+    most = max(most, b < 0x7f800000u ? b : 0u);
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
+  const int power = (int)(most >> 23) - 135 + ((most & 0x7fffff) > 0x600000);
+  return min(max(power, -126), 120);
+}
+
+template <typename T> __device__ __forceinline__ T by_chance(float p, uint32_t u) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, p);
+  if ((bits & 0x7f800000u) == 0x7f800000u) return (T)p;
+  if constexpr (__is_same(T, bf16_t)) {
+    return __builtin_bit_cast(bf16_t, (uint16_t)((bits + u) >> 16));
+  } else {
+#pragma clang fp contract(off)
+    const float up = __builtin_bit_cast(float, (bits + (u >> 3)) & 0xffffe000u);
+    const float low = copysignf(floorf(fabsf(p) * 0x1p24f + (float)u * 0x1p-16f) * 0x1p-24f, p);
+    return (T)(fabsf(p) < 0x1p-14f ? low : up);
+  }
+}
+
+// SMALL: states of 8 bits; CHANCE: 16-bit parameters are rounded by chance
+template <typename T, bool SMALL, bool CHANCE> __global__ __launch_bounds__(kThreads) void adamw_kernel(LaunchTensors a, const StepNumbers* numbers, const int64_t* seed,
+                                                                                                       float b1, float c1, float b2, float c2, float eps) {
+#pragma clang fp contract(off)
+  typedef vec<float, 8> vf;
+  typedef vec<uint8_t, 8> v8;
+  const int k = __builtin_amdgcn_readfirstlane(tensor_of(a, blockIdx.x));
+  const OptimTensor t = a.t[k];
+  const StepNumbers s = *numbers;
+  const uint64_t key = SMALL || CHANCE ? (uint64_t)*seed : 0, at_step = (uint64_t)(uint32_t)(a.number + k) << 32 | s.step;
+  const int64_t begin = (int64_t)(blockIdx.x - a.first[k]) * (kGroup * kTurns) + threadIdx.x * 8;
+#pragma unroll 1
+  for (int j = 0; j < kTurns; ++j) {
+    const int64_t at = begin + j * kGroup, wave_at = at - 8 * lane_id();
+    if (wave_at >= t.n) return;   // (of a wave: 256 elements exchange their maximum)
+    const int left = (int)max((int64_t)0, min((int64_t)8, t.n - at));
+    T* p = static_cast<T*>(t.p) + at;
+    vf x = read8(static_cast<const T*>(t.g) + at, left), q = read8(p, left), m, v;
+    uint8_t *m8 = static_cast<uint8_t*>(t.m) + at, *v8p = static_cast<uint8_t*>(t.v) + at;
+    if constexpr (SMALL) {
+      v8 cm = {}, cv = {};
+      if (left == 8) {
+        cm = *reinterpret_cast<const any8<uint8_t>*>(m8);
+        cv = *reinterpret_cast<const any8<uint8_t>*>(v8p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) { cm[e] = m8[e]; cv[e] = v8p[e]; }
+      }
+      const float pm = left > 0 ? power_of_two(t.em[at / kScaleBlock]) : 1.f, pv = left > 0 ? power_of_two(t.ev[at / kScaleBlock]) : 1.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] = from_e4m3(cm[e]) * pm;
+        const float r = from_e4m3(cv[e]) * pv;
+        v[e] = r * r;
+      }
+    } else {
+      m = read8(static_cast<const float*>(t.m) + at, left);
+      v = read8(static_cast<const float*>(t.v) + at, left);
+    }
+    vf r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float g = x[e] * s.clip;
+      m[e] = b1 * m[e] + c1 * g;
+      v[e] = b2 * v[e] + c2 * (g * g);
+      r[e] = sqrtf(v[e]);
+      q[e] = q[e] * s.keep - s.rate * m[e] / (r[e] * s.root + eps);
+    }
+    const uint64_t counter = 4 * (uint64_t)(at >> 3);
+    if constexpr (SMALL) {
+      const int em = exponent_of(m), ev = exponent_of(r);
+      const float im = power_of_two(-em), iv = power_of_two(-ev);
+      const Words wv = philox(counter, key, at_step), wm = philox(counter + 1, key, at_step);
+      v8 cm, cv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        cv[e] = (uint8_t)to_e4m3<true>(r[e] * iv, half_of(wv, e));
+        cm[e] = (uint8_t)to_e4m3<false>(m[e] * im, half_of(wm, e));
+      }
+      write8<uint8_t>(m8, cm, left);
+      write8<uint8_t>(v8p, cv, left);
+      if (left > 0 && at % kScaleBlock == 0) {
+        t.em[at / kScaleBlock] = (int8_t)em;
+        t.ev[at / kScaleBlock] = (int8_t)ev;
+      }
+    } else {
+      write8<float>(static_cast<float*>(t.m) + at, m, left);
+      write8<float>(static_cast<float*>(t.v) + at, v, left);
+    }
+    vec<T, 8> y;
+    if constexpr (CHANCE) {
+      const Words w = philox(counter + 2, key, at_step);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = by_chance<T>(q[e], half_of(w, e));
+    } else {
+      y = __builtin_convertvector(q, decltype(y));
+    }
+    write8<T>(p, y, left);
+  }
+}
+
+// f(tensors of a launch, their pieces) for 64 of them at a time.  A tensor's number is its place in the call; one without elements has a piece in which there is nothing to do.
+template <typename F> int for_launches(const OptimTensor* tensors, int count, F&& f) {
+  for (int from = 0; from < count; from += kTensorsOfLaunch) {
+    LaunchTensors a = {};
+    a.count = std::min(count - from, kTensorsOfLaunch);
+    a.number = from;
+    uint32_t pieces = 0;   // (all elements of a call are at most 2^36: of 256 threads a piece, 2^31 threads)
+    for (int i = 0; i < a.count; ++i) {
+      a.t[i] = tensors[from + i];
+      a.first[i] = pieces;
+      pieces += (uint32_t)std::max<int64_t>(1, (a.t[i].n + kGroup * kTurns - 1) / (kGroup * kTurns));
+    }
+    if (const int rc = f(a, pieces)) return rc;
+  }
+  return 0;
+}
+
+}  // namespace
+
+int64_t optim_workspace(int count) { return 256 + (int64_t)((count + kTensorsOfLaunch - 1) / kTensorsOfLaunch) * kNormGroups * 8; }
+
+static int norm_parts(const OptimTensor* tensors, int count, int dtype, double* parts, int* made, hipStream_t stream) {
+  *made = 0;
+  return for_launches(tensors, count, [&](const LaunchTensors& a, uint32_t pieces) {
+    const int groups = (int)std::min<uint32_t>(pieces, kNormGroups);
+    const int rc = by_tensor_type(dtype, [&](auto t) {
+      hipLaunchKernelGGL((norm_parts_kernel<decltype(t)>), dim3(groups), dim3(kThreads), 0, stream, a, pieces, parts + *made);
+      return hipGetLastError() == hipSuccess ? 0 : -3;
+    });
+    *made += groups;
+    return rc;
+  });
+}
+
+int launch_grad_norm(const OptimTensor* tensors, int count, float* norm, int dtype, void* workspace, hipStream_t stream) {
+  double* parts = reinterpret_cast<double*>(static_cast<char*>(workspace) + 256);
+  int made = 0;
+  if (const int rc = norm_parts(tensors, count, dtype, parts, &made, stream)) return rc;
+  hipLaunchKernelGGL(begin_kernel, dim3(1), dim3(1024), 0, stream, parts, made, norm, StepOptions{}, nullptr);
+  return hipGetLastError() == hipSuccess ? 0 : -3;
+}
+
+int launch_adamw(const OptimTensor* tensors, int count, const StepOptions& o, float* norm, bool clip_here, int dtype, void* workspace, hipStream_t stream) {
+  StepNumbers* numbers = static_cast<StepNumbers*>(workspace);
+  double* parts = nullptr;
+  int made = 0;
+  if (clip_here) {
+    parts = reinterpret_cast<double*>(static_cast<char*>(workspace) + 256);
+    if (const int rc = norm_parts(tensors, count, dtype, parts, &made, stream)) return rc;
+  }
+  hipLaunchKernelGGL(begin_kernel, dim3(1), dim3(1024), 0, stream, parts, made, norm, o, numbers);
+  if (hipGetLastError() != hipSuccess) return -3;
+  const float b1 = (float)o.b1, c1 = (float)(1 - o.b1), b2 = (float)o.b2, c2 = (float)(1 - o.b2), eps = (float)o.eps;
+  return for_launches(tensors, count, [&](const LaunchTensors& a, uint32_t pieces) {
+    return by_tensor_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      auto go = [&](auto small, auto chance) {
+        hipLaunchKernelGGL((adamw_kernel<T, decltype(small)::value, decltype(chance)::value>), dim3(pieces), dim3(kThreads), 0, stream, a, numbers, o.seed, b1, c1, b2, c2, eps);
+        return hipGetLastError() == hipSuccess ? 0 : -3;
+      };
+      const std::true_type yes;
+      const std::false_type no;
+      const bool small = tensors[0].em != nullptr;
+      if constexpr (sizeof(T) == 4) return small ? go(yes, no) : go(no, no);
+      else return small ? go(yes, yes) : o.seed != nullptr ? go(no, yes) : go(no, no);
+    });
+  });
+}
+
+}  // namespace castle

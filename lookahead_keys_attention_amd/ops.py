@@ -87,6 +87,8 @@ def _as_readable(t: torch.Tensor) -> torch.Tensor:
 #   castle_hip::linear_cross_entropy   rows, weight, classes -> (loss, what its backward pass needs back)
 #   castle_hip::embedding        table, token numbers, scale -> rows
 #   castle_hip::dropout_add      x, a residual or None, p, seed -> residual + what stays of x
+#   castle_hip::gated_feed_forward   rows, two weights -> (rows, what its backward pass needs back)
+#   castle_hip::residual_norm    x, residual, weights, scale, gate -> (sum, its norm, factors of the rows)
 #   castle_hip::attention_bwd / attention_packed_bwd / rms_norm_bwd / linear_bwd / linear_cross_entropy_bwd / embedding_bwd   their backward passes
 #                                 (rms_norm_bwd, linear_bwd, linear_cross_entropy_bwd: a gradient that is not asked for comes back empty; dropout_add is its own)
 # `U` is an empty tensor when the lookahead keys are not asked for.  The workspace output is what
@@ -201,6 +203,27 @@ def _fake_dropout_add(x, residual, p, seed):
     return torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+def _fake_gated(x, weight_in, weight_out, activation, keep_state):
+    rows, D, F = x.numel() // x.shape[-1], x.shape[-1], weight_out.shape[1]
+    nbytes = N.check(N.lib().castle_gated_state_bytes(int(rows), int(D), int(F), N.dtype_code(x.dtype)), "castle_gated_state_bytes") if keep_state and rows else 0
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+
+
+def _fake_gated_bwd(dy, x, weight_in, weight_out, state, activation, need_x=True, need_in=True, need_out=True):
+    return tuple(torch.empty(t.shape if need else (0,), dtype=t.dtype, device=t.device) for t, need in ((x, need_x), (weight_in, need_in), (weight_out, need_out)))
+
+
+def _fake_residual_norm(x, residual, weight, scale, gate, next_weight, eps, keep):
+    rows = x.numel() // x.shape[-1]
+    factors = [torch.empty(rows if keep and w is not None else 0, dtype=torch.float32, device=x.device) for w in (weight, next_weight)]
+    return (torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape if next_weight is not None else (0,), dtype=x.dtype, device=x.device), *factors)
+
+
+def _fake_residual_norm_bwd(dy, dh, x, residual, weight, scale, gate, next_weight, rstd, next_rstd, eps, need):
+    like = (x, residual, weight, scale, gate, next_weight)
+    return tuple(torch.empty(t.shape if t is not None and need >> i & 1 else (0,), dtype=x.dtype, device=x.device) for i, t in enumerate(like))
+
+
 def _register_fakes():
     """Called once, when _castle_host.so has defined the operators."""
     for name, fake in (("attention", _fake_attention), ("attention_bwd", _fake_attention_bwd),
@@ -208,7 +231,9 @@ def _register_fakes():
                        ("rms_norm", _fake_rms_norm), ("rms_norm_bwd", _fake_rms_norm_bwd),
                        ("linear", _fake_linear), ("linear_bwd", _fake_linear_bwd),
                        ("linear_cross_entropy", _fake_linear_cross_entropy), ("linear_cross_entropy_bwd", _fake_linear_cross_entropy_bwd),
-                       ("embedding", _fake_embedding), ("embedding_bwd", _fake_embedding_bwd), ("dropout_add", _fake_dropout_add)):
+                       ("embedding", _fake_embedding), ("embedding_bwd", _fake_embedding_bwd), ("dropout_add", _fake_dropout_add),
+                       ("gated_feed_forward", _fake_gated), ("gated_feed_forward_bwd", _fake_gated_bwd),
+                       ("residual_norm", _fake_residual_norm), ("residual_norm_bwd", _fake_residual_norm_bwd)):
         if hasattr(torch.ops.castle_hip, name):   # (an older build, until it is built again: the package is imported for that)
             torch.library.register_fake("castle_hip::" + name, fake)
 
@@ -389,6 +414,66 @@ def dropout_add(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: 
     if N._host is None:
         N.host()
     return torch.ops.castle_hip.dropout_add(x, residual, float(p), seed)
+
+
+GATE_ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def gated_feed_forward(x: torch.Tensor, weight_in: torch.Tensor, weight_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """(act(x G^T) * (x U^T)) weight_out^T: the feed-forward block with a gate, x (..., D), weight_in (2 F, D) the rows of G above those of U, weight_out (D, F);
+    the counterpart of nn.Linear, nn.GELU, nn.Linear in train_triton.py:102-107.  activation: "silu" or "gelu" (erf form).
+
+    Sums in 32 bits; in 16-bit types the hidden rows act(..) * (..) are rounded once on their way to the second product, and so are their gradients.  Differentiable
+    in all three, once: it keeps what the backward pass needs of the hidden rows (about 6 bytes an element in 16-bit types).  D and F are multiples of 8, any number of rows of
+    which (rows + 192) 2 F is below 2^31."""
+    if N._host is None:
+        N.host()
+    if activation not in GATE_ACTIVATIONS:
+        raise ValueError(f"gated_feed_forward: unknown activation {activation!r}")
+    return torch.ops.castle_hip.gated_feed_forward(x, weight_in, weight_out, GATE_ACTIVATIONS[activation], False)[0]
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None, scale: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                  next_weight: torch.Tensor | None = None, eps: float | None = None):
+    """y = residual + scale * gate * norm(x) * weight, and with `next_weight` also h = norm(y) * next_weight: -> y, or (y, h).  norm(t) = t / sqrt(mean(t^2) + eps) over the last
+    axis, eps that of nn.RMSNorm in 32 bits where none is given: what stands between two blocks of a residual stream (train_triton.py:161-164), with a norm behind the block and a
+    learned scale of its branch.
+
+    x and residual (..., D); weight, scale, next_weight (D,), each of which may be left out (without weight x is taken as it is).  gate: the shape of x, or ones behind some of its leading axes, then
+    D: (B, 1, D) is a gate of each sequence, (D,) one of all.  All results are rounded once, h from the sum in 32 bits.  Differentiable in all tensors, once.  D is at most 8192."""
+    if N._host is None:
+        N.host()
+    y, h, _, _ = torch.ops.castle_hip.residual_norm(x, residual, weight, scale, gate, next_weight, torch.finfo(torch.float32).eps if eps is None else float(eps), False)
+    return y if next_weight is None else (y, h)
+
+
+@torch.no_grad()
+def gradient_norm(grads) -> torch.Tensor:
+    """The 2-norm of all elements of the tensors (one type, one GPU) as a float32 number on the GPU: squares are summed in 64 bits, in a fixed order."""
+    if N._host is None:
+        N.host()
+    return N.host().gradient_norm(list(grads))
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step: torch.Tensor, *, lr, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, max_norm: float | None = None,
+               norm: torch.Tensor | None = None, seed: torch.Tensor | None = None, exp_avg_exponents=None, exp_avg_sq_exponents=None) -> torch.Tensor | None:
+    """One step of AdamW over all parameters of a list, in place, in a few launches (the optimiser of train_triton.py:219-259, with its clipping):
+    g' = c g, c = min(1, max_norm / (norm + 1e-6));  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;
+    p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+
+    params, grads: lists of tensors of one type (float32, bfloat16, float16) on one GPU, no two with memory in common.  step: an int64 tensor of one element on the GPU, the steps taken so far; it
+    is one more afterwards (t).  lr: a number, or a float32 tensor of one element on the GPU, which a captured step reads anew.  max_norm: gradients are clipped by
+    their norm over all of the list, or by `norm`, a float32 tensor of one element; the norm is returned.
+
+    States, with the shapes and strides of their parameters: float32 tensors (m, v), or torch.float8_e4m3fn ones of m and sqrt(v) with int8 exponents, contiguous, one of each 256 elements in
+    memory, which are the numbers times 2^exponent.  Those are rounded by chance, such that the mean is kept, by numbers drawn from `seed` (int64, one element), step, tensor and place; with a seed
+    so are 16-bit parameters, without one they are rounded to the nearest.  castle_adamw in include/castle_hip.h says how.  A state that is infinite or NaN is NaN in 8 bits."""
+    if N._host is None:
+        N.host()
+    rate, rate_device = (0.0, lr) if isinstance(lr, torch.Tensor) else (float(lr), None)
+    lists = [None if t is None else list(t) for t in (params, grads, exp_avgs, exp_avg_sqs, exp_avg_exponents, exp_avg_sq_exponents)]
+    return N.host().adamw_step(*lists, step, rate, rate_device, float(betas[0]), float(betas[1]), float(eps), float(weight_decay), None if max_norm is None else float(max_norm), norm, seed)
 
 
 @torch.no_grad()
