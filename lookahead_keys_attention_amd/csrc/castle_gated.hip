@@ -6,6 +6,7 @@
 #include "castle_gelu.h"
 #include "castle_gemm.h"
 #include "castle_rows.h"
+#include "castle_wide.h"
 #include <algorithm>
 
 namespace castle {
@@ -29,34 +30,342 @@ template <typename T, int ACT> struct Gate {
   }
 };
 
-// h of u = [R][2 F]; BWD: [dg dv] of dh and u, in place of u or not, and h
-template <typename T, int ACT> __global__ __launch_bounds__(kThreads) void gate_kernel(const T* u, int64_t n, int F, T* h) {
-  const int64_t i = (block_of_many() * kThreads + threadIdx.x) * 8, row = i / F, col = i - row * F;
+// ---- fp32: u in memory ----------------------------------------------------------------------------------------------
+__device__ __forceinline__ vf load8(const float* p) { return *reinterpret_cast<const frag_mem<float>*>(p); }
+__device__ __forceinline__ void store8(float* p, vf v) { *reinterpret_cast<frag_mem<float>*>(p) = v; }
+// h of u = [R][2 F]
+template <int ACT> __global__ __launch_bounds__(kThreads) void gate_kernel(const float* u, int64_t n, int F, float* h) {
+  const int64_t i = (block_of_many() * kThreads + threadIdx.x) * 8, row = i / F, at = row * 2 * F + i - row * F;
   if (i >= n) return;
-  const vf g = __builtin_convertvector((frag<T>)*reinterpret_cast<const frag_mem<T>*>(u + row * 2 * F + col), vf);
-  const vf v = __builtin_convertvector((frag<T>)*reinterpret_cast<const frag_mem<T>*>(u + row * 2 * F + F + col), vf);
+  const vf g = load8(u + at), v = load8(u + at + F);
   vf y;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = Gate<T, ACT>(g[e]).act * v[e];
-  *reinterpret_cast<frag_mem<T>*>(h + i) = __builtin_convertvector(y, frag<T>);
+  for (int e = 0; e < 8; ++e) y[e] = Gate<float, ACT>(g[e]).act * v[e];
+  store8(h + i, y);
 }
-template <typename T, int ACT> __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const T* u, const T* dh, int64_t n, int F, T* du, T* h) {
-  const int64_t i = (block_of_many() * kThreads + threadIdx.x) * 8, row = i / F, col = i - row * F;
+// [dg dv] of dh and u, and h; dh or h may be nullptr
+template <int ACT> __global__ __launch_bounds__(kThreads) void gate_bwd_kernel(const float* u, const float* dh, int64_t n, int F, float* du, float* h) {
+  const int64_t i = (block_of_many() * kThreads + threadIdx.x) * 8, row = i / F, at = row * 2 * F + i - row * F;
   if (i >= n) return;
-  const vf g = __builtin_convertvector((frag<T>)*reinterpret_cast<const frag_mem<T>*>(u + row * 2 * F + col), vf);
-  const vf v = __builtin_convertvector((frag<T>)*reinterpret_cast<const frag_mem<T>*>(u + row * 2 * F + F + col), vf);
-  const vf d = __builtin_convertvector((frag<T>)*reinterpret_cast<const frag_mem<T>*>(dh + i), vf);
+  const vf g = load8(u + at), v = load8(u + at + F), d = dh != nullptr ? load8(dh + i) : vf{};
   vf dg, dv, y;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const Gate<T, ACT> a(g[e]);
+    const Gate<float, ACT> a(g[e]);
     dg[e] = d[e] * (v[e] * a.slope);
     dv[e] = d[e] * a.act;
     y[e] = a.act * v[e];
   }
-  *reinterpret_cast<frag_mem<T>*>(du + row * 2 * F + col) = __builtin_convertvector(dg, frag<T>);
-  *reinterpret_cast<frag_mem<T>*>(du + row * 2 * F + F + col) = __builtin_convertvector(dv, frag<T>);
-  if (h != nullptr) *reinterpret_cast<frag_mem<T>*>(h + i) = __builtin_convertvector(y, frag<T>);
+  if (dh != nullptr) {
+    store8(du + at, dg);
+    store8(du + at + F, dv);
+  }
+  if (h != nullptr) store8(h + i, y);
+}
+
+// ---- 16-bit types: the gate inside the products ---------------------------------------------------------------------
+// Tiles of BM rows by 128 hidden columns.  Forward: of a step of the contraction both halves of w_in lie in LDS, 32 of its rows and 32 of the other half in turn, so that a wave holds g and v of the
+// same elements in its accumulators and u never leaves them: h goes to memory and, for the backward pass, a = act(g) and b = v act'(g), in the order of the registers.  Backward: the tile of dh = dy w_out
+// meets a and b in the same order, and [dg dv] = [dh b, dh a] goes to memory.  a and b keep 24 of their 32 bits (one part of 16 and one of 8): as 16-bit numbers each would be
+// rounded twice on the way to dg and dv, and the gradients were twice as far from the formula as rounded once; with h and [dg dv] alone rounded it is 1.4 times.
+enum { kForward = 0, kForwardKeep = 1, kBackward = 2 };
+struct GatedProductArgs {
+  const void *a, *b;       // x and w_in; dy and w_out
+  int64_t lda, ldb;
+  int R, F, K;             // K: of the contraction
+  void* out;               // h [R][F]; [dg dv] [R][2 F]
+  unsigned char* planes;   // a and b: [tile][wave][piece of 32 x 32] of kPlaneBytes
+};
+constexpr int kTileF = 128;             // hidden columns of a tile
+constexpr int kPlaneBytes = 6 * 1024;   // 16 numbers a lane of a and of b: 32 bytes of each of their first parts, 16 of the others
+template <int MODE, int BM> struct GatedShape {
+  static constexpr int BN = MODE == kBackward ? kTileF : 2 * kTileF;
+  static constexpr int WM = BM == 256 ? 4 : 2, WN = 8 / WM, FM = BM / 32 / WM, FN = BN / 32 / WN, FH = kTileF / 32 / WN;   // pieces of a wave: rows, columns of the product, hidden columns
+  static constexpr int kLoadsA = BM / 64, kLoads = kLoadsA + BN / 64, kBytesA = kLoadsA * 8 * 1024, kStage = kLoads * 8 * 1024;
+  static constexpr int kTurn = 2048, kFit = (kMaxLds - 8 * kTurn) / kStage, kStages = kFit < 3 ? kFit : 3, kLds = kStages * kStage + 8 * kTurn;
+  static constexpr int kStores = FM * FH * (MODE == kForward ? 2 : MODE == kForwardKeep ? 8 : 4);   // of a wave and tile
+  static_assert(kStages >= 2 && FM >= 1 && FH >= 1, "");
+};
+__device__ const uint32_t castle_gated_zeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
+extern __shared__ __attribute__((aligned(16))) unsigned char castle_gated_lds[];
+
+// PAIRS: rows 64 k .. 64 k + 31 of the tile are rows 32 k .. of the first half of the matrix, the next 32 the same of its second half, `half` elements further on
+template <typename T, bool KC, int FREE, bool PAIRS> struct GatedOperand : WideOperand<T, KC, FREE> {
+  typedef WideOperand<T, KC, FREE> W;
+  static constexpr int N = W::N;
+  __device__ __forceinline__ void start(const T* p, int64_t ld, int free0, int free_end, uint32_t half) {
+    W::start(p, ld, free0, free_end, 0);
+    if constexpr (PAIRS) {
+      const int lane = lane_id(), first = wave_id() * N;
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7), there = min(row / 64 * 32 + row % 32, W::left - 1);
+        W::off[q] = 2 * ((uint32_t)((int)ld * there + 8 * piece) + (row & 32 ? half : 0u));
+      }
+    }
+  }
+  // the last step, `steps` of it left: zeros behind the contraction's end
+  __device__ __forceinline__ void load_end(int steps, uint32_t lds) {
+    const T* zeros = reinterpret_cast<const T*>(castle_gated_zeros);
+    if constexpr (KC) {
+      W::load_end(steps, zeros, lds);
+    } else {
+      constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
+      const int first = wave_id() * N, k = ROWS * first + lane_id() / PIECES;
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        if (k + ROWS * q < steps) load_to_lds(W::at, W::off[q], lds + 1024 * (first + q));
+        else load_to_lds(zeros, 0, lds + 1024 * (first + q));
+      }
+    }
+  }
+};
+
+typedef vec<uint32_t, 4> u4;
+// sixteen numbers of a lane as their upper 24 bits: [0], [1] upper halves, [2] the bytes behind them
+__device__ __forceinline__ void to_parts(const vec<float, 16>& x, u4 (&p)[3]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t lo = __builtin_bit_cast(uint32_t, (float)x[2 * k]), hi = __builtin_bit_cast(uint32_t, (float)x[2 * k + 1]);
+    p[k / 4][k % 4] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+    if (k % 2 == 0) {
+      const uint32_t lo2 = __builtin_bit_cast(uint32_t, (float)x[2 * k + 2]), hi2 = __builtin_bit_cast(uint32_t, (float)x[2 * k + 3]);
+      const uint32_t first = __builtin_amdgcn_perm(hi, lo, 0x0c0c0501), second = __builtin_amdgcn_perm(hi2, lo2, 0x0c0c0501);
+      p[2][k / 2] = first | second << 16;
+    }
+  }
+}
+__device__ __forceinline__ vec<float, 16> from_parts(const u4& p0, const u4& p1, const u4& p2) {
+  vec<float, 16> x;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t upper = k < 4 ? p0[k % 4] : p1[k % 4], lower = p2[k / 2];   // byte 1 of the number from byte k % 2 * 2 (+ 1) of `lower`
+    x[2 * k] = __builtin_bit_cast(float, __builtin_amdgcn_perm(upper, lower, k % 2 ? 0x0504020c : 0x0504000c));
+    x[2 * k + 1] = __builtin_bit_cast(float, __builtin_amdgcn_perm(upper, lower, k % 2 ? 0x0706030c : 0x0706010c));
+  }
+  return x;
+}
+
+// The frame is that of gemm_wide_kernel (castle_gemm.hip): eight waves, one workgroup to a CU, steps of 64 of the contraction straight from memory to LDS into two or three buffers, requested over the
+// end of a tile.  END: the contraction ends inside a step.
+template <typename T, int MODE, int ACT, int BM, bool END> __global__ __launch_bounds__(kWideThreads, 2) void gated_product_kernel(GatedProductArgs a) {
+  typedef GatedShape<MODE, BM> S;
+  typedef GatedOperand<T, true, BM, false> OpA;
+  typedef GatedOperand<T, MODE != kBackward, S::BN, MODE != kBackward> OpB;
+  typedef vec<T, 8> vt;
+  typedef vec<float, 16> v16;
+  const int lane = lane_id(), wave = wave_id(), c = lane & 31, g = lane >> 5;
+  // tiles in the order of an XCD's L2: all rows of a band of columns, then those of the next; XCD x takes the x-th eighth
+  constexpr int kBand = 2048 / S::BN;
+  const int tiles_m = (a.R + BM - 1) / BM, tiles_n = (a.F + kTileF - 1) / kTileF, tiles = tiles_m * tiles_n;
+  auto place = [&](int t, int& m, int& n) __attribute__((always_inline)) {
+    const int band = t / (tiles_m * kBand), rest = t - band * tiles_m * kBand, width = min(kBand, tiles_n - band * kBand);
+    m = rest / width;
+    n = band * kBand + rest % width;
+  };
+  const int share = (tiles + 7) / 8, first = blockIdx.x % 8 * share, last = min(tiles, first + share), stride = gridDim.x / 8;
+  const int wm = wave / S::WN * 32 * S::FM, wn = wave % S::WN * 32 * S::FN, wh = wave % S::WN * 32 * S::FH;
+  const int steps = (a.K + kWideK - 1) / kWideK;
+  int tile = first + blockIdx.x / 8;
+  if (tile >= last) return;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)castle_gated_lds, half = (uint32_t)a.F * (uint32_t)a.ldb;
+  // the step that is requested next runs ahead of the one that is multiplied, into the next tile
+  OpA ra;
+  OpB rb;
+  int next_tile = tile, next_step = 0, ahead = 0;   // ahead: steps requested and not waited for
+  auto start = [&]() __attribute__((always_inline)) {
+    int m, n;
+    place(next_tile, m, n);
+    ra.start(static_cast<const T*>(a.a), a.lda, m * BM, a.R, 0);
+    rb.start(static_cast<const T*>(a.b), a.ldb, n * kTileF, a.F, half);
+  };
+  auto request = [&](int buffer) __attribute__((always_inline)) {
+    if (next_tile >= last) return;
+    ++ahead;
+    if (END && next_step == steps - 1) {
+      const int left = a.K - next_step * kWideK;
+      ra.load_end(left, lds0 + buffer);
+      rb.load_end(left, lds0 + buffer + S::kBytesA);
+    } else {
+      ra.load(a.lda, lds0 + buffer);
+      rb.load(a.ldb, lds0 + buffer + S::kBytesA);
+    }
+    if (++next_step == steps) {
+      next_step = 0;
+      next_tile += stride;
+      if (next_tile < last) start();
+    }
+  };
+  start();
+  request(0);
+  request(S::kStage);
+  if constexpr (S::kStages == 3) request(2 * S::kStage);
+  // The step behind the current one is in LDS, from every wave, and all have read the current one.  Waits are for all but the last so many requests; the stores of a tile inside the output come
+  // behind those and are not waited for (`stored`).
+  bool stored = false;
+  auto arrive = [&]() __attribute__((always_inline)) {
+    auto wait = [&](auto n) __attribute__((always_inline)) {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(n)::value < 63 ? decltype(n)::value : 63) : "memory");
+    };
+    const int newer = ahead - 1;   // steps
+    if (newer > 1) {
+      if (stored) wait(std::integral_constant<int, 2 * S::kLoads + S::kStores>());
+      else wait(std::integral_constant<int, 2 * S::kLoads>());
+    } else if (newer == 1) {
+      if (stored) wait(std::integral_constant<int, S::kLoads + S::kStores>());
+      else wait(std::integral_constant<int, S::kLoads>());
+    } else {
+      if (stored) wait(std::integral_constant<int, S::kStores>());
+      else wait(std::integral_constant<int, 0>());
+    }
+    stored = false;
+    --ahead;
+  };
+  int buffer = 0;
+  frag<T> fa[2][S::FM], fb[2][S::FN];
+  auto read = [&](int slot, int s) __attribute__((always_inline)) {
+    OpA::read(reinterpret_cast<const T*>(castle_gated_lds + buffer), fa[slot], wm, s, c, g);
+    OpB::read(reinterpret_cast<const T*>(castle_gated_lds + buffer + S::kBytesA), fb[slot], wn, s, c, g);
+    __builtin_amdgcn_sched_barrier(0);   // these reads, then the products of the fragments before
+  };
+  T* const turn = reinterpret_cast<T*>(castle_gated_lds + S::kStages * S::kStage + wave * S::kTurn);
+  arrive();
+  while (tile < last) {
+    int tm, tn;
+    place(tile, tm, tn);
+    const int m0 = tm * BM, n0 = tn * kTileF;
+    const bool inside = m0 + BM <= a.R && n0 + kTileF <= a.F;
+    u4* const planes = reinterpret_cast<u4*>(a.planes + (((int64_t)tm * tiles_n + tn) * 8 + wave) * (S::FM * S::FH * kPlaneBytes)) + lane;
+    // (backward: requested before the tile's products, which hide them)
+    u4 kept[MODE == kBackward ? S::FM * S::FH : 1][6];
+    if constexpr (MODE == kBackward) {
+#pragma unroll
+      for (int p = 0; p < S::FM * S::FH; ++p)
+#pragma unroll
+        for (int k = 0; k < 6; ++k) kept[p][k] = __builtin_nontemporal_load(planes + (p * 6 + k) * 64);
+    }
+    read(0, 0);
+    int done = 0;   // buffer of the step that ends
+    acc_t acc[S::FM][S::FN];   // [columns, m lanes]
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) zero(acc[i][j]);
+    auto multiply = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) mma(acc[i][j], fb[slot][j], fa[slot][i]);
+    };
+    for (int it = 0; it < steps; ++it) {
+#pragma unroll
+      for (int s = 0; s < kWideK / 16 - 1; ++s) {
+        read(1 - s % 2, s + 1);
+        multiply(s % 2);
+      }
+      arrive();
+      done = buffer;
+      buffer = buffer == (S::kStages - 1) * S::kStage ? 0 : buffer + S::kStage;
+      if (it + 1 < steps) request(done);
+      read(0, 0);   // (behind the last step: for nothing)
+      multiply(1);
+    }
+    asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");   // the loop may end right behind a product
+    __builtin_amdgcn_sched_barrier(0);
+    request(done);
+    tile += stride;
+    // 32 x 32 numbers to whole rows, 64 bytes of each, through the wave's own place in LDS (piece p of row r at p ^ (r / 4 % 4))
+    auto to_rows = [&](const v16& z, T* out, int64_t ld, int m, int n) __attribute__((always_inline)) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) st4<T>(turn + c * 32 + 8 * (q ^ (c >> 2 & 3)) + 4 * g, pack4<T>(z, q));
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = 16 * k + (lane >> 2), piece = lane & 3;
+        const vt v = *reinterpret_cast<const vt*>(turn + row * 32 + 8 * (piece ^ (row >> 2 & 3)));
+        if (m + row < a.R && n + 8 * piece < a.F) *reinterpret_cast<vt*>(out + (m + row) * ld + n + 8 * piece) = v;
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FH; ++j) {
+        const int m = m0 + wm + 32 * i, n = n0 + wh + 32 * j;
+        v16 x, y;
+        if constexpr (MODE == kBackward) {
+          const u4(&p)[6] = kept[i * S::FH + j];
+          x = from_parts(p[0], p[1], p[2]) * acc[i][j];   // dv
+          y = from_parts(p[3], p[4], p[5]) * acc[i][j];   // dg
+          T* out = static_cast<T*>(a.out);
+          to_rows(y, out, 2 * (int64_t)a.F, m, n);
+          to_rows(x, out + a.F, 2 * (int64_t)a.F, m, n);
+        } else {
+          v16 h;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const Gate<T, ACT> gate(acc[i][2 * j][r]);
+            x[r] = gate.act;
+            y[r] = acc[i][2 * j + 1][r] * gate.slope;
+            h[r] = acc[i][2 * j + 1][r] * gate.act;
+          }
+          if constexpr (MODE == kForwardKeep) {
+            u4 p[3];
+            u4* to = planes + (i * S::FH + j) * 6 * 64;
+            to_parts(x, p);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) __builtin_nontemporal_store(p[k], to + k * 64);
+            to_parts(y, p);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) __builtin_nontemporal_store(p[k], to + (3 + k) * 64);
+          }
+          to_rows(h, static_cast<T*>(a.out), a.F, m, n);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    stored = inside;
+  }
+}
+
+template <typename T, int MODE, int ACT, int BM, bool END> int launch_product_as(const GatedProductArgs& a, hipStream_t stream) {
+  typedef GatedShape<MODE, BM> S;
+  static PerDeviceOnce once;
+  bool& configured = once.flag();
+  if (!configured) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gated_product_kernel<T, MODE, ACT, BM, END>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
+    configured = true;
+  }
+  const int64_t tiles = (int64_t)((a.R + BM - 1) / BM) * ((a.F + kTileF - 1) / kTileF);
+  hipLaunchKernelGGL((gated_product_kernel<T, MODE, ACT, BM, END>), dim3((unsigned)std::min<int64_t>((tiles + 7) / 8 * 8, 256)), dim3(kWideThreads), S::kLds, stream, a);
+  return hipGetLastError() == hipSuccess ? 0 : -3;
+}
+// Rows of a tile: those with which the fullest CU is done first (us a step of the contraction, and at a tile's end); of both passes, which share the order of a and b.
+int tile_rows(int R, int D, int F) {
+  const int steps = (D + kWideK - 1) / kWideK;
+  auto cost = [&](int rows, double step, double end) {
+    const int64_t tiles = (int64_t)((R + rows - 1) / rows) * ((F + kTileF - 1) / kTileF);
+    return (double)((tiles + 255) / 256) * (steps * step + end);
+  };
+  const double large = cost(256, 1.4, 5), middle = cost(128, 0.85, 3), small = cost(64, 0.56, 1.6);
+  return small < std::min(middle, large) ? 64 : middle < large ? 128 : 256;
+}
+template <int MODE> int launch_product(const GatedProductArgs& a, int rows, int act, int dtype, hipStream_t stream) {
+  return by_type16(dtype, true, [&](auto t, auto) {
+    using T = decltype(t);
+    auto of_end = [&](auto bm, auto ac) {
+      constexpr int BM = decltype(bm)::value, ACT = decltype(ac)::value;
+      return a.K % kWideK != 0 ? launch_product_as<T, MODE, ACT, BM, true>(a, stream) : launch_product_as<T, MODE, ACT, BM, false>(a, stream);
+    };
+    auto of_act = [&](auto bm) {
+      if constexpr (MODE != kBackward)
+        if (act == kGeluGate) return of_end(bm, std::integral_constant<int, kGeluGate>());
+      return of_end(bm, std::integral_constant<int, kSilu>());   // (the backward pass has a and b)
+    };
+    return rows == 64 ? of_act(std::integral_constant<int, 64>()) : rows == 128 ? of_act(std::integral_constant<int, 128>()) : of_act(std::integral_constant<int, 256>());
+  });
 }
 
 int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
@@ -90,58 +399,87 @@ int grads(const Operand2& dy, const Operand2& x, const Operand2& w, void* dw, vo
   return dw == nullptr ? 0 : product({dy.p, dy.ld, false}, {x.p, x.ld, false}, dw, N, K, R, dtype, workspace, stream);
 }
 
-template <typename F> int by_type_and_act(int dtype, int act, F&& f) {
-  return by_tensor_type(dtype, [&](auto t) {
-    return act == kSilu ? f(t, std::integral_constant<int, kSilu>()) : f(t, std::integral_constant<int, kGeluGate>());
-  });
+// f(activation)
+template <typename F> int by_act(int act, F&& f) { return act == kSilu ? f(std::integral_constant<int, kSilu>()) : f(std::integral_constant<int, kGeluGate>()); }
+
+int64_t hidden_bytes(int R, int F, int dtype) { return up((int64_t)R * F * elem_size(dtype)); }
+int64_t planes_bytes(int R, int D, int F) {
+  const int rows = tile_rows(R, D, F);
+  return (int64_t)((R + rows - 1) / rows) * ((F + kTileF - 1) / kTileF) * rows * kTileF * 6;
 }
 
 }  // namespace
 
-// state: u
-int64_t gated_state(int R, int D, int F, int dtype) { return up((int64_t)R * 2 * F * elem_size(dtype)); }
+// What the backward pass needs: fp32 u, [R][2 F]; else h, [R][F], and a and b
+int64_t gated_state(int R, int D, int F, int dtype) { return dtype == 0 ? 2 * hidden_bytes(R, F, 0) : hidden_bytes(R, F, dtype) + planes_bytes(R, D, F); }
 int64_t gated_workspace(int R, int D, int F, int dtype, bool keeps) {
-  return up((int64_t)R * F * elem_size(dtype)) + (keeps ? 0 : gated_state(R, D, F, dtype)) + std::max(product_workspace(R, 2 * F, D, dtype), product_workspace(R, D, F, dtype));
+  const int64_t h = hidden_bytes(R, F, dtype), down = product_workspace(R, D, F, dtype);
+  if (dtype != 0) return std::max<int64_t>(256, (keeps ? 0 : h) + down);
+  return h + (keeps ? 0 : 2 * h) + std::max(product_workspace(R, 2 * F, D, 0), down);
 }
 int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* workspace, hipStream_t stream) {
   char* at = static_cast<char*>(workspace);
-  void* h = at;
-  at += up((int64_t)a.R * a.F * elem_size(dtype));
-  void* u = state;
-  if (u == nullptr) {
-    u = at;
-    at += gated_state(a.R, a.D, a.F, dtype);
+  const int64_t hidden = hidden_bytes(a.R, a.F, dtype);
+  auto take = [&](int64_t bytes) { char* p = at; at += bytes; return p; };
+  void* h;
+  int rc;
+  if (dtype != 0) {
+    h = state != nullptr ? state : take(hidden);
+    const GatedProductArgs p = {a.x, a.w_in, a.ld_x, a.ld_in, a.R, a.F, a.D, h, state != nullptr ? static_cast<unsigned char*>(state) + hidden : nullptr};
+    const int rows = tile_rows(a.R, a.D, a.F);
+    rc = state != nullptr ? launch_product<kForwardKeep>(p, rows, a.act, dtype, stream) : launch_product<kForward>(p, rows, a.act, dtype, stream);
+  } else {
+    h = take(hidden);
+    float* u = static_cast<float*>(state != nullptr ? state : take(2 * hidden));
+    const int64_t n = (int64_t)a.R * a.F;
+    rc = product({a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, u, a.R, 2 * a.F, a.D, dtype, at, stream);
+    if (rc == 0)
+      rc = by_act(a.act, [&](auto act) {
+        hipLaunchKernelGGL((gate_kernel<decltype(act)::value>), many_blocks((n / 8 + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, u, n, a.F, static_cast<float*>(h));
+        return hipGetLastError() == hipSuccess ? 0 : -3;
+      });
   }
-  if (const int rc = product({a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, u, a.R, 2 * a.F, a.D, dtype, at, stream)) return rc;
-  const int64_t n = (int64_t)a.R * a.F;
-  const int rc = by_type_and_act(dtype, a.act, [&](auto t, auto act) {
-    using T = decltype(t);
-    hipLaunchKernelGGL((gate_kernel<T, decltype(act)::value>), many_blocks((n / 8 + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, static_cast<const T*>(u), n, a.F, static_cast<T*>(h));
-    return hipGetLastError() == hipSuccess ? 0 : -3;
-  });
   return rc != 0 ? rc : product({h, a.F, true}, {a.w_out, a.ld_out, true}, y, a.R, a.D, a.F, dtype, at, stream);
 }
 
 int64_t gated_bwd_workspace(int R, int D, int F, int dtype, int gradients) {
-  const bool dx = gradients & 1, dw_in = gradients & 2, dw_out = gradients & 4;
-  const int64_t hidden = up((int64_t)R * F * elem_size(dtype));
-  return (dw_out ? hidden : 0) + hidden + gated_state(R, D, F, dtype) +
-         std::max({product_workspace(R, F, D, dtype), dw_out ? product_workspace(D, F, R, dtype) : 0, grads_bytes(R, 2 * F, D, dtype, dw_in, dx)});
+  const bool dx = gradients & 1, dw_in = gradients & 2, dw_out = gradients & 4, below = dx || dw_in;
+  const int64_t hidden = hidden_bytes(R, F, dtype), products = std::max(dw_out ? product_workspace(D, F, R, dtype) : 0, below ? grads_bytes(R, 2 * F, D, dtype, dw_in, dx) : 0);
+  if (dtype != 0) return std::max<int64_t>(256, (below ? 2 * hidden : 0) + products);
+  return (dw_out ? hidden : 0) + (below ? 3 * hidden + std::max(products, product_workspace(R, F, D, 0)) : products);
 }
 int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void* dx, void* dw_in, void* dw_out, int dtype, void* workspace, hipStream_t stream) {
   char* at = static_cast<char*>(workspace);
-  const int64_t hidden = up((int64_t)a.R * a.F * elem_size(dtype)), n = (int64_t)a.R * a.F;
+  const int64_t hidden = hidden_bytes(a.R, a.F, dtype), n = (int64_t)a.R * a.F;
+  const bool below = dx != nullptr || dw_in != nullptr;
   auto take = [&](int64_t bytes) { char* p = at; at += bytes; return p; };
-  void *h = dw_out != nullptr ? take(hidden) : nullptr, *dh = take(hidden), *du = take(gated_state(a.R, a.D, a.F, dtype));
-  if (const int rc = product({dy, a.D, true}, {a.w_out, a.ld_out, false}, dh, a.R, a.F, a.D, dtype, at, stream)) return rc;
-  int rc = by_type_and_act(dtype, a.act, [&](auto t, auto act) {
-    using T = decltype(t);
-    hipLaunchKernelGGL((gate_bwd_kernel<T, decltype(act)::value>), many_blocks((n / 8 + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, static_cast<const T*>(state),
-                       static_cast<const T*>(dh), n, a.F, static_cast<T*>(du), static_cast<T*>(h));
-    return hipGetLastError() == hipSuccess ? 0 : -3;
-  });
-  if (rc != 0) return rc;
-  if (dw_out != nullptr && (rc = product({dy, a.D, false}, {h, a.F, false}, dw_out, a.D, a.F, a.R, dtype, at, stream)) != 0) return rc;
+  const void* h = state;
+  void* du = nullptr;
+  int rc = 0;
+  if (dtype != 0) {
+    if (below) {
+      du = take(2 * hidden);
+      const GatedProductArgs p = {dy, a.w_out, a.D, a.ld_out, a.R, a.F, a.D, du, const_cast<unsigned char*>(static_cast<const unsigned char*>(state)) + hidden};
+      rc = launch_product<kBackward>(p, tile_rows(a.R, a.D, a.F), a.act, dtype, stream);
+    }
+  } else {
+    float* h32 = dw_out != nullptr ? reinterpret_cast<float*>(take(hidden)) : nullptr;
+    const float* dh = nullptr;
+    h = h32;
+    if (below) {
+      dh = reinterpret_cast<const float*>(take(hidden));
+      du = take(2 * hidden);
+      rc = product({dy, a.D, true}, {a.w_out, a.ld_out, false}, const_cast<float*>(dh), a.R, a.F, a.D, dtype, at, stream);
+    }
+    if (rc == 0)
+      rc = by_act(a.act, [&](auto act) {
+        hipLaunchKernelGGL((gate_bwd_kernel<decltype(act)::value>), many_blocks((n / 8 + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, static_cast<const float*>(state), dh, n, a.F,
+                           static_cast<float*>(du), h32);
+        return hipGetLastError() == hipSuccess ? 0 : -3;
+      });
+  }
+  if (rc == 0 && dw_out != nullptr) rc = product({dy, a.D, false}, {h, a.F, false}, dw_out, a.D, a.F, a.R, dtype, at, stream);
+  if (rc != 0 || !below) return rc;
   return grads({du, 2 * a.F, true}, {a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, dw_in, dx, a.R, 2 * a.F, a.D, dtype, at, stream);
 }
 

@@ -1,0 +1,261 @@
+"""Gated feed-forward block (ops.gated_feed_forward): refusals and shapes without a GPU, results against the formula in 64 bits on one.
+
+Tolerances, from the formula with every error that the kernels may make.  E = 2^-23 is what an addition of a matrix product may lose (2^-24 rounded, twice that cut off), H half a step of the
+type.  A hidden sum of n products of exact 16-bit numbers (fp32: of three parts, 2^-22 more) is off by (n + 8) E of the sum of its magnitudes.  act moves by 1.13 of what its argument does, its
+slope by 0.8; both are evaluated to 2^-18 of themselves (gelu: 3e-6 where it counts), and next to zero to 2^-24.  In 16 bits a = act(g) and b = v act'(g) lose what lies below 24 bits, 2^-16,
+h, dg and dv are rounded once, H.  Each product adds up what its operands are off by and its own sum's error, and the result is rounded: H."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from lookahead_keys_attention_amd import ops
+
+DEV = "cuda:0"
+gpu = pytest.mark.gpu
+E = 2.0 ** -23
+
+
+def inputs(R, D, F, dtype, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g)
+    return [t.to(dtype) for t in (n(R, D) * spread, n(2 * F, D) * D ** -0.5, n(D, F) * F ** -0.5, n(R, D))]
+
+
+def act_of(g, activation):
+    """act, its slope"""
+    if activation == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s + g * s * (1 - s)
+    cdf = 0.5 * torch.erfc(-g * 0.5 ** 0.5)
+    return g * cdf, cdf + g * torch.exp(-g * g / 2) * 0.3989422804014327
+
+
+def reference(x, win, wout, dy, activation, dtype):
+    """{name: (value, what the result may be off by before it is rounded)} in 64 bits."""
+    H = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    more = 2.0 ** -22 if dtype == torch.float32 else 0.0
+    x, win, wout, dy = (t.double() for t in (x, win, wout, dy))
+    R, D, F = x.shape[0], x.shape[1], wout.shape[1]
+
+    def product(a, b, da, db):
+        """a b and its error, of operands that are off by da and db (or exact)"""
+        off = ((a.shape[1] + 8) * E + more) * (a.abs() @ b.abs())
+        if da is not None:
+            off = off + da @ b.abs()
+        if db is not None:
+            off = off + a.abs() @ db
+        return a @ b, off
+
+    u, du_off = product(x, win.T, None, None)
+    g, v = u.chunk(2, 1)
+    g_off, v_off = du_off.chunk(2, 1)
+    act, slope = act_of(g, activation)
+    act_off = 1.13 * g_off + 2.0 ** -18 * act.abs() + 2.0 ** -24
+    slope_off = 0.8 * g_off + 2.0 ** -18 * slope.abs() + 2.0 ** -24
+    h = act * v
+    h_off = act_off * v.abs() + act.abs() * v_off + act_off * v_off + H * h.abs() + (2.0 ** -24 * h.abs())
+    y = product(h, wout.T, h_off, None)
+    dh, dh_off = product(dy, wout, None, None)
+    cut = 2.0 ** -16 if H else 2.0 ** -23
+    a_off, b = act_off + cut * act.abs(), v * slope
+    b_off = slope_off * v.abs() + slope.abs() * v_off + slope_off * v_off + cut * b.abs()
+    d = torch.cat((dh * b, dh * act), 1)
+    d_off = torch.cat((dh_off * (b.abs() + b_off) + dh.abs() * b_off, dh_off * (act.abs() + a_off) + dh.abs() * a_off), 1)
+    d_off = d_off + (H + 2.0 ** -23) * (d.abs() + d_off)
+    return {"y": y, "dx": product(d, win, d_off, None), "dwin": product(d.T, x, d_off.T, None), "dwout": product(dy.T, h, None, h_off)}
+
+
+def within(got, ref, dtype, what):
+    value, off = ref
+    got = got.detach().cpu().double()
+    most = off + torch.finfo(dtype).eps / 2 * (value.abs() + off).clamp(min=torch.finfo(dtype).tiny)
+    assert got.shape == value.shape, what
+    assert got.isfinite().all(), what
+    worst = ((got - value).abs() - most).max() if got.numel() else 0.0
+    assert worst <= 0, (what, float(worst))
+
+
+def run(x, win, wout, dy, activation):
+    leaves = [t.to(DEV).requires_grad_() for t in (x, win, wout)]
+    y = ops.gated_feed_forward(*leaves, activation=activation)
+    grads = torch.autograd.grad(y, leaves, dy.to(DEV))
+    return dict(zip(("y", "dx", "dwin", "dwout"), (y, *grads)))
+
+
+# ---- without a GPU --------------------------------------------------------------------------------------------------
+def test_traces_and_keeps_shapes():
+    with FakeTensorMode():
+        for dtype in (torch.bfloat16, torch.float32):
+            x, win, wout = (torch.empty(*s, dtype=dtype, requires_grad=True) for s in ((2, 3, 16), (80, 16), (16, 40)))
+            y = ops.gated_feed_forward(x, win, wout)
+            assert y.shape == x.shape and y.dtype == dtype
+            y.sum().backward()
+            assert all(t.grad.shape == t.shape for t in (x, win, wout))
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(x=torch.zeros(2, 12)), ValueError),                                    # another width
+    (dict(win=torch.zeros(24, 16)), ValueError),                                 # not twice the hidden width
+    (dict(x=torch.zeros(2, 12), win=torch.zeros(32, 12), wout=torch.zeros(12, 16)), ValueError),   # widths of no whole pieces
+    (dict(wout=torch.zeros(16, 16, dtype=torch.bfloat16)), ValueError),
+    (dict(activation="relu"), ValueError),
+    (dict(), RuntimeError),                                                      # tensors on the CPU
+])
+def test_refusals_on_the_host(change, error):
+    args = dict(x=torch.zeros(2, 16), win=torch.zeros(32, 16), wout=torch.zeros(16, 16), activation="silu") | change
+    with pytest.raises((error, RuntimeError)):
+        ops.gated_feed_forward(args["x"], args["win"], args["wout"], activation=args["activation"])
+
+
+# ---- on a GPU -------------------------------------------------------------------------------------------------------
+SIZES = [(1, 8, 8), (3, 64, 128), (64, 72, 136), (65, 136, 40), (200, 512, 680), (513, 256, 264), (129, 1024, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("R, D, F", SIZES)
+def test_values_and_gradients(R, D, F, dtype, activation):
+    t = inputs(R, D, F, dtype, seed=R)
+    ref = reference(*t, activation, dtype)
+    for name, got in run(*t, activation).items():
+        within(got, ref[name], dtype, name)
+
+
+# one, two and four rows of waves to a tile; tiles that end inside in both directions; a contraction that ends inside a step
+@gpu
+@pytest.mark.parametrize("R, D, F", [(4090, 64, 1016), (8190, 64, 1016), (8200, 200, 1032), (300, 1000, 2048)])
+def test_sizes_of_tiles(R, D, F):
+    t = inputs(R, D, F, torch.bfloat16, seed=1)
+    t_gpu = [x.to(DEV) for x in t]   # (the reference of these sizes is formed on the GPU)
+    ref = {k: (v.cpu(), off.cpu()) for k, (v, off) in reference(*t_gpu, "silu", torch.bfloat16).items()}
+    for name, got in run(*t, "silu").items():
+        within(got, ref[name], torch.bfloat16, name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 2, 16, 17, 32, 50, 64])
+def test_tokens_without_gradients(rows, dtype):
+    for D, F in ((64, 24), (512, 1408), (1040, 72)):
+        x, win, wout, dy = inputs(rows, D, F, dtype, seed=rows)
+        with torch.no_grad():
+            y = ops.gated_feed_forward(*(t.to(DEV) for t in (x[:, None], win, wout)))
+        within(y[:, 0], reference(x, win, wout, dy, "silu", dtype)["y"], dtype, (D, F))
+
+
+@gpu
+@pytest.mark.parametrize("need", range(1, 8))
+def test_gradients_that_are_asked_for(need):
+    for dtype in (torch.bfloat16, torch.float32):
+        t = inputs(70, 64, 72, dtype)
+        ref = reference(*t, "silu", dtype)
+        leaves = [x.to(DEV).requires_grad_(bool(need >> i & 1)) for i, x in enumerate(t[:3])]
+        y = ops.gated_feed_forward(*leaves)
+        y.backward(t[3].to(DEV))
+        for i, (leaf, name) in enumerate(zip(leaves, ("dx", "dwin", "dwout"))):
+            if need >> i & 1:
+                within(leaf.grad, ref[name], dtype, name)
+            else:
+                assert leaf.grad is None
+
+
+@gpu
+def test_strides_of_all_operands():
+    for dtype in (torch.bfloat16, torch.float32):
+        x, win, wout, dy = inputs(40, 64, 72, dtype)
+        ref = reference(x, win, wout, dy, "silu", dtype)
+        wide = lambda t: torch.cat((t, t.new_full((t.shape[0], 24), float("nan"))), 1).to(DEV)[:, :t.shape[1]]   # rows apart
+        turned = lambda t: t.t().contiguous().to(DEV).t()                                                        # columns apart
+        odd = lambda t: torch.cat((t.flatten(), t.new_zeros(1))).to(DEV).roll(1)[1:].view(t.shape)               # not 16-byte aligned
+        for f in (wide, turned, odd):
+            leaves = [f(t).detach().requires_grad_() for t in (x, win, wout)]
+            y = ops.gated_feed_forward(*leaves)
+            grads = torch.autograd.grad(y, leaves, f(dy))
+            for name, got in zip(("y", "dx", "dwin", "dwout"), (y, *grads)):
+                within(got, ref[name], dtype, name)
+
+
+@gpu
+def test_shapes_and_empty_calls():
+    x, win, wout, dy = (t.to(DEV) for t in inputs(24, 64, 72, torch.bfloat16))
+    flat = ops.gated_feed_forward(x, win, wout)
+    assert torch.equal(ops.gated_feed_forward(x.view(2, 3, 4, 64), win, wout).view(24, 64), flat)
+    assert torch.equal(ops.gated_feed_forward(x[0], win, wout), ops.gated_feed_forward(x[:1], win, wout)[0])
+    leaves = [t.clone().requires_grad_() for t in (x[:0], win, wout)]
+    y = ops.gated_feed_forward(*leaves)
+    assert y.shape == (0, 64)
+    y.backward(dy[:0])
+    assert leaves[0].grad.shape == (0, 64) and not leaves[1].grad.any() and not leaves[2].grad.any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_far_arguments_and_what_is_not_finite(dtype):
+    """Gates of +-1000 are one and zero; a NaN or an infinity of a row stays in that row.  (Not in fp16, which ends at 65504: hidden numbers are 1000 times 1000 here, and infinite in it.)"""
+    D, F = 64, 72
+    x, win, wout, dy = inputs(66, D, F, dtype, spread=1000.0)
+    ref = reference(x, win, wout, dy, "silu", dtype)
+    for name, got in run(x, win, wout, dy, "silu").items():
+        within(got, ref[name], dtype, name)
+    ref = reference(x, win, wout, dy, "gelu", dtype)
+    x[5, 3], x[7, 60] = float("nan"), float("inf")
+    bad = run(x, win, wout, dy, "gelu")
+    keep = [r for r in range(66) if r not in (5, 7)]
+    for name in ("y", "dx"):
+        # (not the same bits in fp32: a tile of a product in which something is not finite goes to other instructions)
+        within(bad[name][keep], tuple(t[keep] for t in ref[name]), dtype, name)
+        assert bad[name][5].isnan().all(), name
+
+
+@gpu
+def test_the_same_bits_every_time_on_any_stream_and_in_a_graph():
+    t = [x.to(DEV) for x in inputs(700, 136, 264, torch.bfloat16)]
+    leaves = [x.clone().requires_grad_() for x in t[:3]]
+
+    def step():
+        y = ops.gated_feed_forward(*leaves)
+        return (y.detach(), *torch.autograd.grad(y, leaves, t[3]))
+
+    first = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = step()
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(t[0] * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want)), k
+
+
+@gpu
+def test_refusals_on_the_gpu():
+    x, win, wout, dy = (t.to(DEV) for t in inputs(4, 64, 72, torch.bfloat16))
+    with pytest.raises(ValueError):
+        ops.gated_feed_forward(x, win.float(), wout)
+    with pytest.raises(ValueError):
+        ops.gated_feed_forward(x, win.cpu(), wout)
+    with pytest.raises((TypeError, RuntimeError)):
+        ops.gated_feed_forward(x.double(), win.double(), wout.double())
+    big = torch.empty(1, dtype=torch.bfloat16, device=DEV).expand(1 << 24, 64)   # hidden rows of 2^24 x 144 elements
+    with pytest.raises(ValueError):
+        ops.gated_feed_forward(big, win, wout)
+    w = win.clone().requires_grad_()
+    y = ops.gated_feed_forward(x, w, wout)
+    dw, = torch.autograd.grad(y, w, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dw.sum().backward()
+    y = ops.gated_feed_forward(x, w, wout)
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
