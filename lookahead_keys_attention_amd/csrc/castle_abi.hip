@@ -1057,7 +1057,7 @@ static int residual_grad_args(castle::ResidualBwdArgs& b, const castle_residual*
 int castle_residual_norm(const castle_residual* args, void* y, void* h, int dtype, void* stream) {
   castle::ResidualArgs r;
   if (const int rc = residual_args(r, args, dtype)) return rc;
-  if (y == nullptr || (args->next_weight != nullptr && h == nullptr) || !aligned_to({y, h}, elem_size(dtype))) return CASTLE_ERR_ARG;
+  if (!aligned_to({y}, elem_size(dtype)) || (args->next_weight != nullptr && !aligned_to({h}, elem_size(dtype)))) return CASTLE_ERR_ARG;
   r.y = y;
   r.h = h;
   return castle::launch_residual(r, dtype, static_cast<hipStream_t>(stream));
