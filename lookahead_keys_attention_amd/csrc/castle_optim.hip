@@ -25,6 +25,7 @@ constexpr int kTurns = 4;                 // turns of a workgroup
 constexpr int kWaves = kThreads / 64;
 
 // rows of any alignment (gfx950 reads and writes them at the speed of aligned ones where they are aligned)
+typedef vec<float, 8> vf8;
 template <typename T> using any8 = vec<T, 8> __attribute__((aligned(1)));
 
 struct LaunchTensors {
@@ -41,17 +42,18 @@ __device__ __forceinline__ int tensor_of(const LaunchTensors& a, uint32_t piece)
   return 63 - __builtin_clzll(begun);   // (sizes of zero are left out on the host, so firsts grow)
 }
 
-template <typename T> __device__ __forceinline__ vec<float, 8> read8(const T* p, int left) {
-  vec<float, 8> x = {};
+template <typename T> __device__ __forceinline__ vec<T, 8> raw8(const T* p, int left) {
+  vec<T, 8> x = {};
   if (left >= 8) {
-    x = __builtin_convertvector((frag<T>)*reinterpret_cast<const any8<T>*>(p), decltype(x));
+    x = *reinterpret_cast<const any8<T>*>(p);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < left) x[e] = (float)p[e];
+      if (e < left) x[e] = p[e];
   }
   return x;
 }
+template <typename T> __device__ __forceinline__ vec<float, 8> read8(const T* p, int left) { return __builtin_convertvector(raw8(p, left), vf8); }
 template <typename T> __device__ __forceinline__ void write8(T* p, vec<T, 8> x, int left) {
   if (left >= 8) {
     *reinterpret_cast<any8<T>*>(p) = x;
@@ -133,48 +135,81 @@ __global__ __launch_bounds__(1024) void begin_kernel(const double* parts, int co
 
 // ---- step ----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
 
-__device__ __forceinline__ float from_e4m3(uint32_t code) {
-  const uint32_t mag = code & 0x7f;
-  const float normal = __builtin_bit_cast(float, (mag << 20) + (120u << 23)), low = (float)mag * 0x1p-9f;
-  const float x = mag == 0x7f ? NAN : mag < 8 ? low : normal;
-  return code & 0x80 ? -x : x;
+// sqrt and quotient to an ulp or two (correctly rounded ones took a fifth of the kernel with states of 8 bits); below 2^-96 the instruction's argument is scaled, whose denormal numbers count as zero
+__device__ __forceinline__ float fast_sqrt(float x) {
+  const bool low = x < 0x1p-96f;
+  return __builtin_amdgcn_sqrtf(low ? x * 0x1p64f : x) * (low ? 0x1p-32f : 1.f);
 }
-// |s| <= 448 (or it is infinite or NaN); u: 16 random bits
-template <bool POSITIVE> __device__ __forceinline__ uint32_t to_e4m3(float s, uint32_t u) {
-#pragma clang fp contract(off)
-  const uint32_t bits = __builtin_bit_cast(uint32_t, s), mag = bits & 0x7fffffff;
-  const float a = fabsf(s);
-  uint32_t code = a < 0x1p-6f ? (uint32_t)(a * 512.f + (float)u * 0x1p-16f) : ((mag + (u << 4)) >> 20) - 960;
-  if (POSITIVE && mag != 0) code = max(code, 1u);
-  if (mag >= 0x7f800000u) code = 0x7f;
-  return code | (bits >> 31) << 7;
+
+// Eight numbers to e4m3, up or down by chance: the instruction adds the upper bits of its last operand to what it cuts off, below the normal numbers too, which is what castle_hip.h says (its results
+// are those of that formula for 1.7e7 numbers from 2^-20 to 448 and all that is not finite).
+__device__ __forceinline__ vec<uint8_t, 8> to_e4m3(const vec<float, 8>& x, const Words& u) {
+  vec<uint32_t, 2> c = {};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    int w = 0;
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * k], u.w[2 * k] << 16, w, 0);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * k + 1], u.w[2 * k] & 0xffff0000u, w, 1);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * k + 2], u.w[2 * k + 1] << 16, w, 2);
+    c[k] = __builtin_amdgcn_cvt_sr_fp8_f32(x[4 * k + 3], u.w[2 * k + 1] & 0xffff0000u, w, 3);
+  }
+  typedef vec<uint8_t, 8> v8;
+  return __builtin_bit_cast(v8, c);
 }
-// E of 256 elements, 32 lanes of them, from the largest |x| that is finite
-__device__ __forceinline__ int exponent_of(const vec<float, 8>& x) {
+__device__ __forceinline__ vec<float, 8> from_e4m3(vec<uint8_t, 8> codes, float power) {
+  typedef vec<uint32_t, 2> v2;
+  const v2 c = __builtin_bit_cast(v2, codes);
+  vec<float, 8> x;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[k], true);
+    x[4 * k] = lo[0] * power;
+    x[4 * k + 1] = lo[1] * power;
+    x[4 * k + 2] = hi[0] * power;
+    x[4 * k + 3] = hi[1] * power;
+  }
+  return x;
+}
+// the largest |x| of 256 elements, 32 lanes of them, as bits; FINITE: of those that are finite
+template <bool FINITE> __device__ __forceinline__ uint32_t largest(const vec<float, 8>& x) {
   uint32_t most = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, (float)x[e]) & 0x7fffffff;
-    most = max(most, b < 0x7f800000u ? b : 0u);
+    const uint32_t b = bits_of(x[e]) & 0x7fffffff;
+    most = max(most, !FINITE || b < 0x7f800000u ? b : 0u);
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
-  const int power = (int)(most >> 23) - 135 + ((most & 0x7fffff) > 0x600000);
-  return min(max(power, -126), 120);
+  return most;
 }
+__device__ __forceinline__ uint32_t largest_finite(const vec<float, 8>& x) {
+  uint32_t most = largest<false>(x);
+  if (__ballot(most >= 0x7f800000u) != 0) most = largest<true>(x);   // (of the whole wave: its lanes exchange)
+  return most;
+}
+// E for the bits of the largest
+__device__ __forceinline__ int exponent_of(uint32_t most) { return min(max((int)(most >> 23) - 135 + ((most & 0x7fffff) > 0x600000), -126), 120); }
 
-template <typename T> __device__ __forceinline__ T by_chance(float p, uint32_t u) {
-  const uint32_t bits = __builtin_bit_cast(uint32_t, p);
-  if ((bits & 0x7f800000u) == 0x7f800000u) return (T)p;
-  if constexpr (__is_same(T, bf16_t)) {
-    return __builtin_bit_cast(bf16_t, (uint16_t)((bits + u) >> 16));
-  } else {
+// eight 16-bit parameters by chance
+template <typename T> __device__ __forceinline__ vec<T, 8> by_chance(const vec<float, 8>& q, const Words& r) {
+  vec<T, 8> y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float p = q[e];
+    const bool finite = __builtin_isfinite(p);
+    const uint32_t bits = bits_of(p), u = finite ? half_of(r, e) : 0;   // (what is not finite has nothing to be cut off)
+    if constexpr (__is_same(T, bf16_t)) {
+      y[e] = __builtin_bit_cast(bf16_t, (uint16_t)((bits + u) >> 16));
+    } else {
 #pragma clang fp contract(off)
-    const float up = __builtin_bit_cast(float, (bits + (u >> 3)) & 0xffffe000u);
-    const float low = copysignf(floorf(fabsf(p) * 0x1p24f + (float)u * 0x1p-16f) * 0x1p-24f, p);
-    return (T)(fabsf(p) < 0x1p-14f ? low : up);
+      const float up = __builtin_bit_cast(float, (bits + (u >> 3)) & 0xffffe000u);
+      const float low = copysignf(floorf(fabsf(p) * 0x1p24f + (float)u * 0x1p-16f) * 0x1p-24f, p);
+      y[e] = (T)(finite ? fabsf(p) < 0x1p-14f ? low : up : p);
+    }
   }
+  return y;
 }
 
 // SMALL: states of 8 bits; CHANCE: 16-bit parameters are rounded by chance
@@ -182,63 +217,70 @@ template <typename T, bool SMALL, bool CHANCE> __global__ __launch_bounds__(kThr
                                                                                                        float b1, float c1, float b2, float c2, float eps) {
 #pragma clang fp contract(off)
   typedef vec<float, 8> vf;
-  typedef vec<uint8_t, 8> v8;
+  typedef std::conditional_t<SMALL, uint8_t, float> State;
   const int k = __builtin_amdgcn_readfirstlane(tensor_of(a, blockIdx.x));
   const OptimTensor t = a.t[k];
   const StepNumbers s = *numbers;
   const uint64_t key = SMALL || CHANCE ? (uint64_t)*seed : 0, at_step = (uint64_t)(uint32_t)(a.number + k) << 32 | s.step;
   const int64_t begin = (int64_t)(blockIdx.x - a.first[k]) * (kGroup * kTurns) + threadIdx.x * 8;
+  // what a turn reads is requested a turn ahead
+  struct Turn {
+    vec<T, 8> g, p;
+    vec<State, 8> m, v;
+    float pm, pv;
+  };
+  auto left_at = [&](int64_t at) __attribute__((always_inline)) { return (int)max((int64_t)0, min((int64_t)8, t.n - at)); };
+  auto fetch = [&](int64_t at) __attribute__((always_inline)) {
+    const int left = left_at(at);
+    Turn r;
+    r.g = raw8(static_cast<const T*>(t.g) + at, left);
+    r.p = raw8(static_cast<const T*>(t.p) + at, left);
+    r.m = raw8(static_cast<const State*>(t.m) + at, left);
+    r.v = raw8(static_cast<const State*>(t.v) + at, left);
+    if constexpr (SMALL) {
+      r.pm = left > 0 ? power_of_two(t.em[at / kScaleBlock]) : 1.f;
+      r.pv = left > 0 ? power_of_two(t.ev[at / kScaleBlock]) : 1.f;
+    }
+    return r;
+  };
+  if (begin - 8 * lane_id() >= t.n) return;   // (of a wave: 256 elements exchange their maximum)
+  Turn next = fetch(begin);
 #pragma unroll 1
   for (int j = 0; j < kTurns; ++j) {
-    const int64_t at = begin + j * kGroup, wave_at = at - 8 * lane_id();
-    if (wave_at >= t.n) return;   // (of a wave: 256 elements exchange their maximum)
-    const int left = (int)max((int64_t)0, min((int64_t)8, t.n - at));
-    T* p = static_cast<T*>(t.p) + at;
-    vf x = read8(static_cast<const T*>(t.g) + at, left), q = read8(p, left), m, v;
-    uint8_t *m8 = static_cast<uint8_t*>(t.m) + at, *v8p = static_cast<uint8_t*>(t.v) + at;
+    const int64_t at = begin + j * kGroup;
+    const int left = left_at(at);
+    const Turn now = next;
+    const bool more = j + 1 < kTurns && at + kGroup - 8 * lane_id() < t.n;
+    if (more) next = fetch(at + kGroup);
+    const vf x = __builtin_convertvector(now.g, vf), p = __builtin_convertvector(now.p, vf);
+    vf m, v, r, q;
     if constexpr (SMALL) {
-      v8 cm = {}, cv = {};
-      if (left == 8) {
-        cm = *reinterpret_cast<const any8<uint8_t>*>(m8);
-        cv = *reinterpret_cast<const any8<uint8_t>*>(v8p);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < left) { cm[e] = m8[e]; cv[e] = v8p[e]; }
-      }
-      const float pm = left > 0 ? power_of_two(t.em[at / kScaleBlock]) : 1.f, pv = left > 0 ? power_of_two(t.ev[at / kScaleBlock]) : 1.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        m[e] = from_e4m3(cm[e]) * pm;
-        const float r = from_e4m3(cv[e]) * pv;
-        v[e] = r * r;
-      }
+      m = from_e4m3(now.m, now.pm);
+      v = from_e4m3(now.v, now.pv);
+      v *= v;
     } else {
-      m = read8(static_cast<const float*>(t.m) + at, left);
-      v = read8(static_cast<const float*>(t.v) + at, left);
+      m = now.m;
+      v = now.v;
     }
-    vf r;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float g = x[e] * s.clip;
       m[e] = b1 * m[e] + c1 * g;
       v[e] = b2 * v[e] + c2 * (g * g);
-      r[e] = sqrtf(v[e]);
-      q[e] = q[e] * s.keep - s.rate * m[e] / (r[e] * s.root + eps);
+      r[e] = fast_sqrt(v[e]);
+      q[e] = p[e] * s.keep - s.rate * m[e] * fast_rcp(r[e] * s.root + eps);
     }
     const uint64_t counter = 4 * (uint64_t)(at >> 3);
     if constexpr (SMALL) {
-      const int em = exponent_of(m), ev = exponent_of(r);
-      const float im = power_of_two(-em), iv = power_of_two(-ev);
-      const Words wv = philox(counter, key, at_step), wm = philox(counter + 1, key, at_step);
-      v8 cm, cv;
+      // (the largest root is that of the largest square: the exponent goes by the correctly rounded one)
+      const int em = exponent_of(largest_finite(m)), ev = exponent_of(bits_of(sqrtf(__builtin_bit_cast(float, largest_finite(v)))));
+      m *= power_of_two(-em);
+      r *= power_of_two(-ev);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        cv[e] = (uint8_t)to_e4m3<true>(r[e] * iv, half_of(wv, e));
-        cm[e] = (uint8_t)to_e4m3<false>(m[e] * im, half_of(wm, e));
-      }
-      write8<uint8_t>(m8, cm, left);
-      write8<uint8_t>(v8p, cv, left);
+      for (int e = 0; e < 8; ++e) r[e] = bits_of(r[e]) - 1 < bits_of(0x1p-9f) - 1 ? 0x1p-9f : r[e];   // what is not zero stays above it
+      const vec<uint8_t, 8> cv = to_e4m3(r, philox(counter, key, at_step)), cm = to_e4m3(m, philox(counter + 1, key, at_step));
+      write8<uint8_t>(static_cast<uint8_t*>(t.m) + at, cm, left);
+      write8<uint8_t>(static_cast<uint8_t*>(t.v) + at, cv, left);
       if (left > 0 && at % kScaleBlock == 0) {
         t.em[at / kScaleBlock] = (int8_t)em;
         t.ev[at / kScaleBlock] = (int8_t)ev;
@@ -248,14 +290,10 @@ template <typename T, bool SMALL, bool CHANCE> __global__ __launch_bounds__(kThr
       write8<float>(static_cast<float*>(t.v) + at, v, left);
     }
     vec<T, 8> y;
-    if constexpr (CHANCE) {
-      const Words w = philox(counter + 2, key, at_step);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = by_chance<T>(q[e], half_of(w, e));
-    } else {
-      y = __builtin_convertvector(q, decltype(y));
-    }
-    write8<T>(p, y, left);
+    if constexpr (CHANCE) y = by_chance<T>(q, philox(counter + 2, key, at_step));
+    else y = __builtin_convertvector(q, decltype(y));
+    write8<T>(static_cast<T*>(t.p) + at, y, left);
+    if (!more) return;
   }
 }
 
