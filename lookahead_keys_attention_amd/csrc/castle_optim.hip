@@ -25,7 +25,6 @@ constexpr int kTurns = 4;                 // turns of a workgroup
 constexpr int kWaves = kThreads / 64;
 
 // rows of any alignment (gfx950 reads and writes them at the speed of aligned ones where they are aligned)
-typedef vec<float, 8> vf8;
 template <typename T> using any8 = vec<T, 8> __attribute__((aligned(1)));
 
 struct LaunchTensors {
@@ -53,7 +52,6 @@ template <typename T> __device__ __forceinline__ vec<T, 8> raw8(const T* p, int 
   }
   return x;
 }
-template <typename T> __device__ __forceinline__ vec<float, 8> read8(const T* p, int left) { return __builtin_convertvector(raw8(p, left), vf8); }
 template <typename T> __device__ __forceinline__ void write8(T* p, vec<T, 8> x, int left) {
   if (left >= 8) {
     *reinterpret_cast<any8<T>*>(p) = x;
@@ -65,25 +63,51 @@ template <typename T> __device__ __forceinline__ void write8(T* p, vec<T, 8> x, 
 }
 
 // ---- norm ----------------------------------------------------------------------------------------------------------
-// Sums of squares in double: of the largest floats they do not overflow, of the smallest they do not vanish, and the adds (two instructions an element) hide behind the reads.
-template <typename T> __global__ __launch_bounds__(kThreads) void norm_parts_kernel(LaunchTensors a, uint32_t pieces, double* parts) {
+// Sums of squares in double: of the largest floats they do not overflow, of the smallest they do not vanish, and the adds (two instructions an element) hide behind the reads.  The next piece is
+// requested before the one that is there is added up.
+constexpr int kGradsOfLaunch = 192;
+struct LaunchGrads {
+  const void* g[kGradsOfLaunch];
+  int64_t n[kGradsOfLaunch];
+  uint32_t first[kGradsOfLaunch];   // piece that each begins with
+  int count;
+};
+static_assert(sizeof(LaunchGrads) + 64 <= 4096, "arguments of a launch");
+template <typename T> __global__ __launch_bounds__(kThreads) void norm_parts_kernel(LaunchGrads a, uint32_t pieces, double* parts) {
   __shared__ double s[kWaves];
   double sum[2] = {0, 0};
-  for (uint32_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
-    const int k = __builtin_amdgcn_readfirstlane(tensor_of(a, piece));
-    const OptimTensor& t = a.t[k];
-    const T* g = static_cast<const T*>(t.g);
+  vec<T, 8> x[2][kTurns];
+  auto fetch = [&](int slot, uint32_t piece) __attribute__((always_inline)) {
+    const int lane = lane_id();
+    int k = 0;
+#pragma unroll
+    for (int i = 0; i < kGradsOfLaunch; i += 64) k += __popcll(__ballot(i + lane < a.count && a.first[min(i + lane, a.count - 1)] <= piece));
+    k = __builtin_amdgcn_readfirstlane(k - 1);
     const int64_t begin = (int64_t)(piece - a.first[k]) * (kGroup * kTurns) + threadIdx.x * 8;
-    vec<float, 8> x[kTurns];
 #pragma unroll
     for (int j = 0; j < kTurns; ++j) {
-      const int64_t at = begin + j * kGroup;
-      x[j] = at < t.n ? read8(g + at, (int)min((int64_t)8, t.n - at)) : vec<float, 8>{};
+      const int64_t left = a.n[k] - begin - j * kGroup;
+      x[slot][j] = raw8(static_cast<const T*>(a.g[k]) + begin + j * kGroup, (int)max((int64_t)0, min((int64_t)8, left)));
     }
+  };
+  auto add = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < kTurns; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e & 1] = __builtin_fma((double)x[j][e], (double)x[j][e], sum[e & 1]);
+      for (int e = 0; e < 8; ++e) {
+        const double g = (double)(float)x[slot][j][e];
+        sum[e & 1] = __builtin_fma(g, g, sum[e & 1]);
+      }
+  };
+  uint32_t piece = blockIdx.x;
+  fetch(0, piece);
+  while (true) {
+    if (piece + gridDim.x < pieces) fetch(1, piece + gridDim.x);
+    add(0);
+    if ((piece += gridDim.x) >= pieces) break;
+    if (piece + gridDim.x < pieces) fetch(0, piece + gridDim.x);
+    add(1);
+    if ((piece += gridDim.x) >= pieces) break;
   }
   double v = sum[0] + sum[1];
 #pragma unroll
@@ -137,11 +161,9 @@ __global__ __launch_bounds__(1024) void begin_kernel(const double* parts, int co
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 __device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
 
-// sqrt and quotient to an ulp or two (correctly rounded ones took a fifth of the kernel with states of 8 bits); below 2^-96 the instruction's argument is scaled, whose denormal numbers count as zero
-__device__ __forceinline__ float fast_sqrt(float x) {
-  const bool low = x < 0x1p-96f;
-  return __builtin_amdgcn_sqrtf(low ? x * 0x1p64f : x) * (low ? 0x1p-32f : 1.f);
-}
+// Roots and quotients to an ulp or two: correctly rounded ones took a fifth of the kernel with states of 8 bits.  The instruction takes denormal numbers for zero: x below 2^-126, or zero, has the
+// root 2^-63 here (compared as whole numbers, of which a NaN is among the largest).
+__device__ __forceinline__ float fast_sqrt(float x) { return __builtin_amdgcn_sqrtf(__builtin_bit_cast(float, max(bits_of(x), bits_of(0x1p-126f)))); }
 
 // Eight numbers to e4m3, up or down by chance: the instruction adds the upper bits of its last operand to what it cuts off, below the normal numbers too, which is what castle_hip.h says (its results
 // are those of that formula for 1.7e7 numbers from 2^-20 to 448 and all that is not finite).
@@ -172,21 +194,21 @@ __device__ __forceinline__ vec<float, 8> from_e4m3(vec<uint8_t, 8> codes, float 
   }
   return x;
 }
-// the largest |x| of 256 elements, 32 lanes of them, as bits; FINITE: of those that are finite
-template <bool FINITE> __device__ __forceinline__ uint32_t largest(const vec<float, 8>& x) {
+// the largest |x| of 256 elements, 32 lanes of them, as bits; SIGNED: some may be negative, FINITE: of those that are finite
+template <bool SIGNED, bool FINITE> __device__ __forceinline__ uint32_t largest(const vec<float, 8>& x) {
   uint32_t most = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const uint32_t b = bits_of(x[e]) & 0x7fffffff;
+    const uint32_t b = SIGNED || FINITE ? bits_of(x[e]) & 0x7fffffff : bits_of(x[e]);
     most = max(most, !FINITE || b < 0x7f800000u ? b : 0u);
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
   return most;
 }
-__device__ __forceinline__ uint32_t largest_finite(const vec<float, 8>& x) {
-  uint32_t most = largest<false>(x);
-  if (__ballot(most >= 0x7f800000u) != 0) most = largest<true>(x);   // (of the whole wave: its lanes exchange)
+template <bool SIGNED> __device__ __forceinline__ uint32_t largest_finite(const vec<float, 8>& x) {
+  uint32_t most = largest<SIGNED, false>(x);
+  if (__ballot(most >= 0x7f800000u) != 0) most = largest<SIGNED, true>(x);   // (of the whole wave: its lanes exchange)
   return most;
 }
 // E for the bits of the largest
@@ -273,11 +295,11 @@ template <typename T, bool SMALL, bool CHANCE> __global__ __launch_bounds__(kThr
     const uint64_t counter = 4 * (uint64_t)(at >> 3);
     if constexpr (SMALL) {
       // (the largest root is that of the largest square: the exponent goes by the correctly rounded one)
-      const int em = exponent_of(largest_finite(m)), ev = exponent_of(bits_of(sqrtf(__builtin_bit_cast(float, largest_finite(v)))));
+      const int em = exponent_of(largest_finite<true>(m)), ev = exponent_of(bits_of(sqrtf(__builtin_bit_cast(float, largest_finite<false>(v)))));
       m *= power_of_two(-em);
       r *= power_of_two(-ev);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = bits_of(r[e]) - 1 < bits_of(0x1p-9f) - 1 ? 0x1p-9f : r[e];   // what is not zero stays above it
+      for (int e = 0; e < 8; ++e) r[e] = v[e] == 0.f ? 0.f : __builtin_bit_cast(float, max(bits_of(r[e]), bits_of(0x1p-9f)));   // what is not zero stays above it
       const vec<uint8_t, 8> cv = to_e4m3(r, philox(counter, key, at_step)), cm = to_e4m3(m, philox(counter + 1, key, at_step));
       write8<uint8_t>(static_cast<uint8_t*>(t.m) + at, cm, left);
       write8<uint8_t>(static_cast<uint8_t*>(t.v) + at, cv, left);
@@ -297,17 +319,19 @@ template <typename T, bool SMALL, bool CHANCE> __global__ __launch_bounds__(kThr
   }
 }
 
-// f(tensors of a launch, their pieces) for 64 of them at a time.  A tensor's number is its place in the call; one without elements has a piece in which there is nothing to do.
+// One without elements has a piece in which there is nothing to do.  (All elements of a call are at most 2^36: of 256 threads a piece, 2^31 threads.)
+uint32_t pieces_of(int64_t n) { return (uint32_t)std::max<int64_t>(1, (n + kGroup * kTurns - 1) / (kGroup * kTurns)); }
+// f(tensors of a launch, their pieces) for 64 of them at a time; a tensor's number is its place in the call.
 template <typename F> int for_launches(const OptimTensor* tensors, int count, F&& f) {
   for (int from = 0; from < count; from += kTensorsOfLaunch) {
     LaunchTensors a = {};
     a.count = std::min(count - from, kTensorsOfLaunch);
     a.number = from;
-    uint32_t pieces = 0;   // (all elements of a call are at most 2^36: of 256 threads a piece, 2^31 threads)
+    uint32_t pieces = 0;
     for (int i = 0; i < a.count; ++i) {
       a.t[i] = tensors[from + i];
       a.first[i] = pieces;
-      pieces += (uint32_t)std::max<int64_t>(1, (a.t[i].n + kGroup * kTurns - 1) / (kGroup * kTurns));
+      pieces += pieces_of(a.t[i].n);
     }
     if (const int rc = f(a, pieces)) return rc;
   }
@@ -316,19 +340,29 @@ template <typename F> int for_launches(const OptimTensor* tensors, int count, F&
 
 }  // namespace
 
-int64_t optim_workspace(int count) { return 256 + (int64_t)((count + kTensorsOfLaunch - 1) / kTensorsOfLaunch) * kNormGroups * 8; }
+int64_t optim_workspace(int count) { return 256 + (int64_t)((count + kGradsOfLaunch - 1) / kGradsOfLaunch) * kNormGroups * 8; }
 
 static int norm_parts(const OptimTensor* tensors, int count, int dtype, double* parts, int* made, hipStream_t stream) {
   *made = 0;
-  return for_launches(tensors, count, [&](const LaunchTensors& a, uint32_t pieces) {
+  for (int from = 0; from < count; from += kGradsOfLaunch) {
+    LaunchGrads a = {};
+    a.count = std::min(count - from, kGradsOfLaunch);
+    uint32_t pieces = 0;
+    for (int i = 0; i < a.count; ++i) {
+      a.g[i] = tensors[from + i].g;
+      a.n[i] = tensors[from + i].n;
+      a.first[i] = pieces;
+      pieces += pieces_of(a.n[i]);
+    }
     const int groups = (int)std::min<uint32_t>(pieces, kNormGroups);
     const int rc = by_tensor_type(dtype, [&](auto t) {
       hipLaunchKernelGGL((norm_parts_kernel<decltype(t)>), dim3(groups), dim3(kThreads), 0, stream, a, pieces, parts + *made);
       return hipGetLastError() == hipSuccess ? 0 : -3;
     });
+    if (rc != 0) return rc;
     *made += groups;
-    return rc;
-  });
+  }
+  return 0;
 }
 
 int launch_grad_norm(const OptimTensor* tensors, int count, float* norm, int dtype, void* workspace, hipStream_t stream) {
