@@ -21,13 +21,20 @@ namespace {
 template <typename T> using any8 = vec<T, 8> __attribute__((aligned(1)));
 typedef vec<float, 8> vf;
 
-constexpr int kForwardGroups = 2048, kBackwardGroups = 1024;   // workgroups, at most
+constexpr int kForwardGroups = 1024;  // workgroups of the forward pass, at most
 constexpr int kGateRows = 8;          // rows of a unit under a gate that several rows have
 
 // LPR lanes of WPR waves have a row, NP pieces of 8 elements a lane
 template <int LPR_, int WPR_, int NP_> struct Layout {
   static constexpr int LPR = LPR_, WPR = WPR_, NP = NP_, kBlock = WPR == 1 ? kThreads : 64 * WPR, kRows = kBlock / (LPR * WPR);
+  // workgroups that a CU holds of the backward pass, and waves of a SIMD: all of a launch run at once, each over several rows (1024 workgroups of which 768 ran at once: 396 us, see below)
+  static constexpr int kHeld = WPR == 8 ? 1 : NP == 1 ? 3 : 2, kWavesPerSimd = WPR == 8 ? 2 : kHeld;
 };
+// workgroups for n turns, `most` at once, with as many turns each as they can have alike
+int even_groups(int64_t n, int64_t most) {
+  const int64_t turns = (n + most - 1) / most;
+  return (int)((n + turns - 1) / turns);
+}
 
 template <typename T> __device__ __forceinline__ vec<T, 8> read8(const T* p, int left) {
   vec<T, 8> x = {};
@@ -49,6 +56,12 @@ template <typename T> __device__ __forceinline__ void write8(T* p, vf v, int lef
 }
 template <typename T> __device__ __forceinline__ vf wide(vec<T, 8> x) { return __builtin_convertvector(x, vf); }
 
+// which of the workgroup's rows a lane has a part in: the same for a wave where a row is a wave's or more, and known to be
+template <typename L> __device__ __forceinline__ int row_of_lane() {
+  if constexpr (L::WPR > 1) return 0;
+  else if constexpr (L::LPR == 64) return wave_id();
+  else return threadIdx.x / L::LPR;
+}
 // sums over the lanes of a row, N at a time; `turn` alternates between two places in LDS, so that one barrier is enough
 template <typename L, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* s, int& turn) {
 #pragma unroll
@@ -94,17 +107,30 @@ template <typename T, typename L> __global__ __launch_bounds__(L::kBlock) void r
   vec<T, 8> next[L::NP];
   columns<T, L>(a, sub, c, next);
   const int64_t step = (int64_t)gridDim.x * L::kRows;
-  for (int64_t row = (int64_t)blockIdx.x * L::kRows + threadIdx.x / TPR; row < a.rows; row += step) {
+  // the next row is requested before the one that is there is summed over
+  vec<T, 8> nx[L::NP], nr[L::NP], ng[L::NP];
+  auto fetch = [&](int64_t row) __attribute__((always_inline)) {
     const int64_t at = row * a.D;
-    vf x[L::NP], y[L::NP], g[L::NP];
-    const T* gate = a.gate == nullptr ? nullptr : static_cast<const T*>(a.gate) + row / a.span * a.D;
 #pragma unroll
     for (int p = 0; p < L::NP; ++p) {
       const int i = 8 * (p * TPR + sub), left = a.D - i;
-      x[p] = wide<T>(read8(static_cast<const T*>(a.x) + at + i, left));
-      y[p] = wide<T>(read8(static_cast<const T*>(a.residual) + at + i, left));
-      if (gate != nullptr) g[p] = wide<T>(read8(gate + i, left));
+      nx[p] = read8(static_cast<const T*>(a.x) + at + i, left);
+      nr[p] = read8(static_cast<const T*>(a.residual) + at + i, left);
+      if (a.gate != nullptr) ng[p] = read8(static_cast<const T*>(a.gate) + row / a.span * a.D + i, left);
     }
+  };
+  int64_t row = (int64_t)blockIdx.x * L::kRows + row_of_lane<L>();
+  if (row < a.rows) fetch(row);
+  for (; row < a.rows; row += step) {
+    const int64_t at = row * a.D;
+    vf x[L::NP], y[L::NP], g[L::NP];
+#pragma unroll
+    for (int p = 0; p < L::NP; ++p) {
+      x[p] = wide<T>(nx[p]);
+      y[p] = wide<T>(nr[p]);
+      g[p] = wide<T>(ng[p]);
+    }
+    if (row + step < a.rows) fetch(row + step);
     float inv = 1.f;
     if (a.w != nullptr) {
       float sum[1] = {0.f};
@@ -119,7 +145,7 @@ template <typename T, typename L> __global__ __launch_bounds__(L::kBlock) void r
 #pragma unroll
     for (int p = 0; p < L::NP; ++p) {
       vf q = x[p] * inv * c[p];
-      if (gate != nullptr) q *= g[p];
+      if (a.gate != nullptr) q *= g[p];
       y[p] += q;
       const int i = 8 * (p * TPR + sub);
       write8<T>(static_cast<T*>(a.y) + at + i, y[p], a.D - i);
@@ -151,7 +177,7 @@ struct BwdKernelArgs {
   float* unit_sums;   // [unit][D], or nullptr: a unit has a whole span
 };
 // GATES: 0 none, 1 each row one of its own, 2 one of several rows
-template <typename T, typename L, int GATES> __global__ __launch_bounds__(L::kBlock) void residual_bwd_kernel(BwdKernelArgs k) {
+template <typename T, typename L, int GATES> __global__ __launch_bounds__(L::kBlock, L::kWavesPerSimd) void residual_bwd_kernel(BwdKernelArgs k) {
   const ResidualBwdArgs& b = k.b;
   const ResidualArgs& a = b.f;
   __shared__ float s[8 * L::WPR];
@@ -160,80 +186,108 @@ template <typename T, typename L, int GATES> __global__ __launch_bounds__(L::kBl
   const int sub = threadIdx.x % TPR;
   int turn = 0;
   vf c[L::NP], sum_p[L::NP], sum_next[L::NP], sum_unit[GATES == 2 ? L::NP : 1];
-  vec<T, 8> next[L::NP];
-  columns<T, L>(a, sub, c, next);
+  vec<T, 8> next_w[L::NP];
+  columns<T, L>(a, sub, c, next_w);
 #pragma unroll
   for (int p = 0; p < L::NP; ++p) sum_p[p] = sum_next[p] = vf{};
   const float per = 1.f / (float)a.D;
   const int64_t step = (int64_t)gridDim.x * L::kRows;
-  for (int64_t unit = (int64_t)blockIdx.x * L::kRows + threadIdx.x / TPR; unit < k.u.units; unit += step) {
-    const int64_t span = unit / k.u.per_span, first = span * a.span + unit % k.u.per_span * k.u.rows, last = min(first + k.u.rows, (span + 1) * a.span);
-    vec<T, 8> g[GATES ? L::NP : 1];
-    if constexpr (GATES == 2) {
+  // a row of a unit; rows are requested one ahead
+  struct Place { int64_t unit, row, last; };
+  auto begin = [&](int64_t unit) __attribute__((always_inline)) {
+    if constexpr (GATES != 2) return Place{unit, unit, unit + 1};
+    const int64_t span = unit / k.u.per_span, first = span * a.span + unit % k.u.per_span * k.u.rows;
+    return Place{unit, first, min(first + k.u.rows, (span + 1) * a.span)};
+  };
+  struct Row {
+    vec<T, 8> x[L::NP], r[L::NP], dy[L::NP], dh[L::NP], g[GATES == 1 ? L::NP : 1];
+    float inv, inv_y;
+  };
+  auto fetch = [&](int64_t row) __attribute__((always_inline)) {
+    Row f;
+    const int64_t at = row * a.D;
 #pragma unroll
-      for (int p = 0; p < L::NP; ++p) {
-        const int i = 8 * (p * TPR + sub);
-        g[p] = read8(static_cast<const T*>(a.gate) + span * a.D + i, a.D - i);
-        sum_unit[p] = vf{};
-      }
+    for (int p = 0; p < L::NP; ++p) {
+      const int i = 8 * (p * TPR + sub), left = a.D - i;
+      f.x[p] = read8(static_cast<const T*>(a.x) + at + i, left);
+      f.r[p] = read8(static_cast<const T*>(a.residual) + at + i, left);
+      f.dy[p] = f.dh[p] = {};
+      if (b.dy != nullptr) f.dy[p] = read8(static_cast<const T*>(b.dy) + at + i, left);
+      if (b.dh != nullptr) f.dh[p] = read8(static_cast<const T*>(b.dh) + at + i, left);
+      if constexpr (GATES == 1) f.g[p] = read8(static_cast<const T*>(a.gate) + at + i, left);
     }
-    for (int64_t row = first; row < last; ++row) {
-      const int64_t at = row * a.D;
-      vec<T, 8> x[L::NP], r[L::NP], dy[L::NP], dh[L::NP];
+    f.inv = a.w != nullptr ? a.rstd[row] : 1.f;
+    f.inv_y = b.dh != nullptr ? a.next_rstd[row] : 0.f;
+    return f;
+  };
+  Place now = {(int64_t)blockIdx.x * L::kRows + row_of_lane<L>(), 0, 0};
+  Row ahead;
+  bool new_unit = true;
+  vec<T, 8> unit_g[GATES == 2 ? L::NP : 1];
+  if (now.unit < k.u.units) {
+    now = begin(now.unit);
+    ahead = fetch(now.row);
+  }
+  while (now.unit < k.u.units) {
+    const int64_t row = now.row, unit = now.unit, at = row * a.D;
+    const bool unit_ends = row + 1 == now.last;
+    const Row f = ahead;
+    if constexpr (GATES == 2)
+      if (new_unit) {
 #pragma unroll
-      for (int p = 0; p < L::NP; ++p) {
-        const int i = 8 * (p * TPR + sub), left = a.D - i;
-        x[p] = read8(static_cast<const T*>(a.x) + at + i, left);
-        r[p] = read8(static_cast<const T*>(a.residual) + at + i, left);
-        dy[p] = dh[p] = {};
-        if (b.dy != nullptr) dy[p] = read8(static_cast<const T*>(b.dy) + at + i, left);
-        if (b.dh != nullptr) dh[p] = read8(static_cast<const T*>(b.dh) + at + i, left);
-        if constexpr (GATES == 1) g[p] = read8(static_cast<const T*>(a.gate) + at + i, left);
-      }
-      const float inv = a.w != nullptr ? a.rstd[row] : 1.f, inv_y = b.dh != nullptr ? a.next_rstd[row] : 0.f;
-      float sum[4] = {};   // of dn yh, dy q, dn q, yh q
-#pragma unroll
-      for (int p = 0; p < L::NP; ++p) {
-        vf q = wide<T>(x[p]) * inv * c[p];
-        if constexpr (GATES != 0) q *= wide<T>(g[p]);
-        const vf yh = (wide<T>(r[p]) + q) * inv_y, dn = wide<T>(dh[p]) * wide<T>(next[p]), d = wide<T>(dy[p]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sum[0] = __builtin_fmaf(dn[e], yh[e], sum[0]);
-          sum[1] = __builtin_fmaf(d[e], q[e], sum[1]);
-          sum[2] = __builtin_fmaf(dn[e], q[e], sum[2]);
-          sum[3] = __builtin_fmaf(yh[e], q[e], sum[3]);
+        for (int p = 0; p < L::NP; ++p) {
+          const int i = 8 * (p * TPR + sub);
+          unit_g[p] = read8(static_cast<const T*>(a.gate) + row / a.span * a.D + i, a.D - i);
+          sum_unit[p] = vf{};
         }
       }
-      row_sums<L>(sum, s, turn);
-      const float m2 = sum[0] * per, m1 = a.w != nullptr ? (sum[1] + inv_y * (sum[2] - m2 * sum[3])) * per : 0.f;
+    if (unit_ends) {
+      now.unit += step;
+      if (now.unit < k.u.units) now = begin(now.unit);
+    } else {
+      ++now.row;
+    }
+    new_unit = unit_ends;
+    if (now.unit < k.u.units) ahead = fetch(now.row);
+    const vec<T, 8>* g = GATES == 1 ? f.g : unit_g;
+    float sum[4] = {};   // of dn yh, dy q, dn q, yh q
 #pragma unroll
-      for (int p = 0; p < L::NP; ++p) {
-        const int i = 8 * (p * TPR + sub), left = a.D - i;
-        const vf xh = wide<T>(x[p]) * inv;
-        vf cg = c[p];
-        if constexpr (GATES != 0) cg *= wide<T>(g[p]);
-        const vf yh = (wide<T>(r[p]) + xh * cg) * inv_y, dhp = wide<T>(dh[p]), dn = dhp * wide<T>(next[p]);
-        const vf d = wide<T>(dy[p]) + (dn - yh * m2) * inv_y, t = d * xh;
-        sum_next[p] += dhp * yh;
-        if constexpr (GATES == 2) sum_unit[p] += t;
-        else if constexpr (GATES == 1) sum_p[p] += t * wide<T>(g[p]);
-        else sum_p[p] += t;
-        if (b.dresidual != nullptr) write8<T>(static_cast<T*>(b.dresidual) + at + i, d, left);
-        if (b.dx != nullptr) write8<T>(static_cast<T*>(b.dx) + at + i, (d * cg - xh * m1) * inv, left);
-        if constexpr (GATES == 1)
-          if (b.dgate != nullptr) write8<T>(static_cast<T*>(b.dgate) + at + i, t * c[p], left);
+    for (int p = 0; p < L::NP; ++p) {
+      vf q = wide<T>(f.x[p]) * f.inv * c[p];
+      if constexpr (GATES != 0) q *= wide<T>(g[p]);
+      const vf yh = (wide<T>(f.r[p]) + q) * f.inv_y, dn = wide<T>(f.dh[p]) * wide<T>(next_w[p]), d = wide<T>(f.dy[p]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sum[0] = __builtin_fmaf(dn[e], yh[e], sum[0]);
+        sum[1] = __builtin_fmaf(d[e], q[e], sum[1]);
+        sum[2] = __builtin_fmaf(dn[e], q[e], sum[2]);
+        sum[3] = __builtin_fmaf(yh[e], q[e], sum[3]);
       }
     }
-    if constexpr (GATES == 2) {
+    row_sums<L>(sum, s, turn);
+    const float m2 = sum[0] * per, m1 = a.w != nullptr ? (sum[1] + f.inv_y * (sum[2] - m2 * sum[3])) * per : 0.f;
 #pragma unroll
-      for (int p = 0; p < L::NP; ++p) {
-        const int i = 8 * (p * TPR + sub), left = a.D - i;
-        sum_p[p] += sum_unit[p] * wide<T>(g[p]);
-        if (b.dgate == nullptr) continue;
-        if (k.unit_sums == nullptr) write8<T>(static_cast<T*>(b.dgate) + span * a.D + i, sum_unit[p] * c[p], left);
-        else write8<float>(k.unit_sums + unit * a.D + i, sum_unit[p], left);
-      }
+    for (int p = 0; p < L::NP; ++p) {
+      const int i = 8 * (p * TPR + sub), left = a.D - i;
+      const vf xh = wide<T>(f.x[p]) * f.inv;
+      vf cg = c[p];
+      if constexpr (GATES != 0) cg *= wide<T>(g[p]);
+      const vf yh = (wide<T>(f.r[p]) + xh * cg) * f.inv_y, dhp = wide<T>(f.dh[p]), dn = dhp * wide<T>(next_w[p]);
+      const vf d = wide<T>(f.dy[p]) + (dn - yh * m2) * f.inv_y, t = d * xh;
+      sum_next[p] += dhp * yh;
+      if constexpr (GATES == 2) sum_unit[p] += t;
+      else if constexpr (GATES == 1) sum_p[p] += t * wide<T>(g[p]);
+      else sum_p[p] += t;
+      if (b.dresidual != nullptr) write8<T>(static_cast<T*>(b.dresidual) + at + i, d, left);
+      if (b.dx != nullptr) write8<T>(static_cast<T*>(b.dx) + at + i, (d * cg - xh * m1) * f.inv, left);
+      if constexpr (GATES == 1)
+        if (b.dgate != nullptr) write8<T>(static_cast<T*>(b.dgate) + at + i, t * c[p], left);
+      if constexpr (GATES == 2)
+        if (unit_ends) {
+          sum_p[p] += sum_unit[p] * wide<T>(g[p]);
+          if (b.dgate != nullptr && k.unit_sums == nullptr) write8<T>(static_cast<T*>(b.dgate) + row / a.span * a.D + i, sum_unit[p] * c[p], left);
+          if (b.dgate != nullptr && k.unit_sums != nullptr) write8<float>(k.unit_sums + unit * a.D + i, sum_unit[p], left);
+        }
     }
   }
   if (k.parts == nullptr) return;
@@ -338,17 +392,18 @@ template <typename F> int by_width(int D, F&& f) {
   if (D <= 4096) return f(Layout<64, 8, 1>());
   return D <= kResidualMaxWidth ? f(Layout<64, 8, 2>()) : -2;
 }
-int rows_of_group(int D) { return D <= 128 ? 16 : D <= 256 ? 8 : D <= 1024 ? 4 : 1; }
+int rows_of_group(int D) { return by_width(D, [](auto l) { return decltype(l)::kRows; }); }
+int groups_at_once(int D) { return by_width(D, [](auto l) { return 256 * decltype(l)::kHeld; }); }
 Units units_of(const ResidualBwdArgs& b) {
   const ResidualArgs& a = b.f;
   if (a.gate == nullptr || a.span == 1) return {a.rows, a.rows, 1};
-  const int64_t lanes = (int64_t)kBackwardGroups * rows_of_group(a.D);
+  const int64_t lanes = (int64_t)groups_at_once(a.D) * rows_of_group(a.D);
   const int64_t rows = std::min(a.span, std::max<int64_t>(kGateRows, (a.rows + lanes - 1) / lanes)), per_span = (a.span + rows - 1) / rows;
   return {a.rows / a.span * per_span, per_span, rows};
 }
 int groups_of(const ResidualBwdArgs& b, const Units& u) {
   const int per = rows_of_group(b.f.D);
-  return (int)std::min<int64_t>((u.units + per - 1) / per, kBackwardGroups);
+  return even_groups((u.units + per - 1) / per, groups_at_once(b.f.D));
 }
 bool wants_columns(const ResidualBwdArgs& b) { return b.dw != nullptr || b.dscale != nullptr || b.dnext != nullptr; }
 bool wants_units(const ResidualBwdArgs& b, const Units& u) { return b.dgate != nullptr && b.f.span > 1 && u.per_span > 1; }
@@ -366,7 +421,7 @@ int launch_residual(const ResidualArgs& a, int dtype, hipStream_t stream) {
     using T = decltype(t);
     return by_width(a.D, [&](auto l) {
       using L = decltype(l);
-      const int groups = (int)std::min<int64_t>((a.rows + L::kRows - 1) / L::kRows, kForwardGroups);
+      const int groups = even_groups((a.rows + L::kRows - 1) / L::kRows, kForwardGroups);
       hipLaunchKernelGGL((residual_kernel<T, L>), dim3(groups), dim3(L::kBlock), 0, stream, a);
       return hipGetLastError() == hipSuccess ? 0 : -3;
     });
