@@ -368,6 +368,152 @@ template <int MODE> int launch_product(const GatedProductArgs& a, int rows, int 
   });
 }
 
+// ---- 16-bit types, few rows (tokens) ---------------------------------------------------------------------------------
+// What bounds them is reading the weights once, and how many bytes the busiest CU draws (about 50 a ns): its rows of x and of the weights.  So every workgroup takes all rows and as many columns as let
+// all CUs have one, both halves of them side by side, and its eight waves split the contraction, straight from memory to the matrix instructions, a few steps in flight at a time.  The second product,
+// whose contraction is the long one, goes in ranges of it too, joined by a launch of its own.
+// 32 rows of 2048 through 5504: 28.3 us with the tiles above and products in ranges, of which 19 and 11.5 on the GPU; now FIRST and SECOND.
+constexpr int kFewRows = 64, kRowWaves = 8, kRowDepth = 32;   // rows at most, waves, contraction of a step
+struct RowsArgs {
+  const void *x, *w;
+  int64_t ld_x, ld_w;
+  int R, N, K, cols;     // cols: of a workgroup
+  int64_t half;          // gate: elements from a row of w to the row of its other half
+  int k_per_range;       // a multiple of kRowDepth
+  void* out;             // [R][N]
+  float* part;           // or partial results [range][R][N]
+};
+typedef vec<float, 4> acc4_t;
+__device__ __forceinline__ void mma16(acc4_t& c, const vec<bf16_t, 8>& a, const vec<bf16_t, 8>& b) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ void mma16(acc4_t& c, const vec<fp16_t, 8>& a, const vec<fp16_t, 8>& b) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+constexpr int kNoGate = -1;
+// ACT: kNoGate, or tiles of 16 columns are 8 of either half.  MT: 16 rows each, NT: tiles of 16 columns
+template <typename T, int ACT, int MT, int NT> __global__ __launch_bounds__(64 * kRowWaves, 2) void gated_rows_kernel(RowsArgs a) {
+  extern __shared__ float s_sums[];   // [wave][16 MT][16 NT + 1]
+  constexpr int LD = 16 * NT + 1, PER = ACT == kNoGate ? 16 : 8;   // columns of a tile
+  constexpr int kRowSteps = MT + NT <= 5 ? 8 : 4;                  // in flight at a time: 160 registers
+  typedef vec<T, 8> vt;
+  const int lane = lane_id(), wave = wave_id(), c = lane & 15, g = lane >> 4, n0 = blockIdx.x * a.cols, n_end = min(a.N, n0 + a.cols);
+  const int k0 = blockIdx.y * a.k_per_range, k1 = min(a.K, k0 + a.k_per_range), steps = (k1 - k0 + kRowDepth - 1) / kRowDepth, per = (steps + kRowWaves - 1) / kRowWaves;
+  const int s_end = min(steps, (wave + 1) * per);
+  const T *x = static_cast<const T*>(a.x) + k0 + 8 * g, *w = static_cast<const T*>(a.w) + k0 + 8 * g;
+  const T* wr[NT];
+  bool there[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = n0 + PER * j + (c & (PER - 1));
+    there[j] = n < n_end;
+    wr[j] = w + (int64_t)min(n, a.N - 1) * a.ld_w + (ACT != kNoGate && c >= 8 ? a.half : 0);
+  }
+  acc4_t acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = acc4_t{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = wave * per; s0 < s_end; s0 += kRowSteps) {
+    vt fa[kRowSteps][MT], fb[kRowSteps][NT];
+#pragma unroll
+    for (int u = 0; u < kRowSteps; ++u) {
+      const int k = kRowDepth * (s0 + u);
+      const bool in = s0 + u < s_end && k0 + k + 8 * g < k1;   // (whole pieces: K is a multiple of 8)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        fb[u][j] = vt{};
+        if (in && there[j]) fb[u][j] = *reinterpret_cast<const vt*>(wr[j] + k);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        fa[u][i] = vt{};
+        if (in && 16 * i + c < a.R) fa[u][i] = *reinterpret_cast<const vt*>(x + (16 * i + c) * a.ld_x + k);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRowSteps; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma16(acc[i][j], fa[u][i], fb[u][j]);
+  }
+  settle();
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s_sums[(wave * 16 * MT + 16 * i + 4 * g + r) * LD + 16 * j + c] = acc[i][j][r];
+  __syncthreads();
+  auto sum = [&](int row, int col) __attribute__((always_inline)) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRowWaves; ++k) v += s_sums[(k * 16 * MT + row) * LD + col];
+    return v;
+  };
+  for (int o = threadIdx.x; o < 16 * MT * PER * NT; o += 64 * kRowWaves) {
+    const int row = o / (PER * NT), col = o % (PER * NT), n = n0 + col;
+    if (row >= a.R || n >= n_end) continue;
+    if constexpr (ACT != kNoGate) {
+      const int at = col / 8 * 16 + col % 8;
+      static_cast<T*>(a.out)[(int64_t)row * a.N + n] = (T)(Gate<T, ACT>(sum(row, at)).act * sum(row, at + 8));
+    } else if (a.part != nullptr) {
+      a.part[((int64_t)blockIdx.y * a.R + row) * a.N + n] = sum(row, col);
+    } else {
+      static_cast<T*>(a.out)[(int64_t)row * a.N + n] = (T)sum(row, col);
+    }
+  }
+}
+// Columns of a workgroup and ranges of the contraction: the least of what the busiest CU draws, and a launch to join ranges
+struct RowsPlan { int cols, ranges; };
+RowsPlan rows_plan(int R, int N, int K, bool gate) {
+  const int halves = gate ? 2 : 1, most = 48 / halves;   // (three tiles of 16)
+  RowsPlan best = {most, 1};
+  double best_cost = 1e30;
+  for (int ranges = 1; ranges <= (gate ? 1 : 8); ++ranges) {
+    if (ranges > 1 && K / ranges < 2 * kRowDepth * kRowWaves) break;
+    for (int cols = 4; cols <= most; ++cols) {
+      const int64_t groups = (int64_t)((N + cols - 1) / cols) * ranges, turns = (groups + 255) / 256;
+      const double cost = turns * (R + halves * cols) * (2.0 * K / ranges) / 50e3 + (ranges > 1 ? 3.0 + ranges * 8.0 * R * N / 4e6 : 0);
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = {cols, ranges};
+      }
+    }
+  }
+  return best;
+}
+template <typename T, int ACT> int launch_rows_as(const RowsArgs& a, int ranges, hipStream_t stream) {
+  const int nt = (a.cols * (ACT == kNoGate ? 1 : 2) + 15) / 16;
+  auto go = [&](auto m, auto n) {
+    constexpr int MT = decltype(m)::value, NT = decltype(n)::value, kLds = kRowWaves * 16 * MT * (16 * NT + 1) * 4;
+    static PerDeviceOnce once;
+    bool& configured = once.flag();
+    if (!configured) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gated_rows_kernel<T, ACT, MT, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) return -3;
+      configured = true;
+    }
+    hipLaunchKernelGGL((gated_rows_kernel<T, ACT, MT, NT>), dim3((a.N + a.cols - 1) / a.cols, ranges), dim3(64 * kRowWaves), kLds, stream, a);
+    return hipGetLastError() == hipSuccess ? 0 : -3;
+  };
+  auto of_rows = [&](auto m) {
+    return nt == 1 ? go(m, std::integral_constant<int, 1>()) : nt == 2 ? go(m, std::integral_constant<int, 2>()) : go(m, std::integral_constant<int, 3>());
+  };
+  return a.R <= 16 ? of_rows(std::integral_constant<int, 1>()) : a.R <= 32 ? of_rows(std::integral_constant<int, 2>()) : of_rows(std::integral_constant<int, 4>());
+}
+int64_t rows_bytes(int R, int N, int K) {
+  const RowsPlan p = rows_plan(R, N, K, false);
+  return p.ranges > 1 ? ((int64_t)p.ranges * R * N * 4 + 255) / 256 * 256 : 0;
+}
+// act: kNoGate, or that of the gate between the two halves of w, N rows each
+int launch_rows(const void* x, int64_t ld_x, const void* w, int64_t ld_w, void* out, int R, int N, int K, int act, int dtype, void* workspace, hipStream_t stream) {
+  const RowsPlan p = rows_plan(R, N, K, act != kNoGate);
+  const int per = ((K + p.ranges - 1) / p.ranges + kRowDepth - 1) / kRowDepth * kRowDepth, ranges = (K + per - 1) / per;
+  const RowsArgs a = {x, w, ld_x, ld_w, R, N, K, p.cols, (int64_t)N * ld_w, per, out, ranges > 1 ? static_cast<float*>(workspace) : nullptr};
+  const int rc = by_type16(dtype, true, [&](auto t, auto) {
+    using T = decltype(t);
+    return act == kNoGate ? launch_rows_as<T, kNoGate>(a, ranges, stream) : act == kSilu ? launch_rows_as<T, kSilu>(a, 1, stream) : launch_rows_as<T, kGeluGate>(a, 1, stream);
+  });
+  return rc != 0 || ranges == 1 ? rc : launch_part_sum(a.part, ranges, (int64_t)R * N, out, dtype, stream);
+}
+
 int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
 int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
@@ -402,6 +548,7 @@ int grads(const Operand2& dy, const Operand2& x, const Operand2& w, void* dw, vo
 // f(activation)
 template <typename F> int by_act(int act, F&& f) { return act == kSilu ? f(std::integral_constant<int, kSilu>()) : f(std::integral_constant<int, kGeluGate>()); }
 
+bool few_rows(int R, int dtype) { return R <= kFewRows && dtype != 0; }
 int64_t hidden_bytes(int R, int F, int dtype) { return up((int64_t)R * F * elem_size(dtype)); }
 int64_t planes_bytes(int R, int D, int F) {
   const int rows = tile_rows(R, D, F);
@@ -413,7 +560,7 @@ int64_t planes_bytes(int R, int D, int F) {
 // What the backward pass needs: fp32 u, [R][2 F]; else h, [R][F], and a and b
 int64_t gated_state(int R, int D, int F, int dtype) { return dtype == 0 ? 2 * hidden_bytes(R, F, 0) : hidden_bytes(R, F, dtype) + planes_bytes(R, D, F); }
 int64_t gated_workspace(int R, int D, int F, int dtype, bool keeps) {
-  const int64_t h = hidden_bytes(R, F, dtype), down = product_workspace(R, D, F, dtype);
+  const int64_t h = hidden_bytes(R, F, dtype), down = few_rows(R, dtype) ? rows_bytes(R, D, F) : product_workspace(R, D, F, dtype);
   if (dtype != 0) return std::max<int64_t>(256, (keeps ? 0 : h) + down);
   return h + (keeps ? 0 : 2 * h) + std::max(product_workspace(R, 2 * F, D, 0), down);
 }
@@ -427,7 +574,9 @@ int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* work
     h = state != nullptr ? state : take(hidden);
     const GatedProductArgs p = {a.x, a.w_in, a.ld_x, a.ld_in, a.R, a.F, a.D, h, state != nullptr ? static_cast<unsigned char*>(state) + hidden : nullptr};
     const int rows = tile_rows(a.R, a.D, a.F);
-    rc = state != nullptr ? launch_product<kForwardKeep>(p, rows, a.act, dtype, stream) : launch_product<kForward>(p, rows, a.act, dtype, stream);
+    if (state != nullptr) rc = launch_product<kForwardKeep>(p, rows, a.act, dtype, stream);
+    else if (few_rows(a.R, dtype)) rc = launch_rows(a.x, a.ld_x, a.w_in, a.ld_in, h, a.R, a.F, a.D, a.act, dtype, nullptr, stream);
+    else rc = launch_product<kForward>(p, rows, a.act, dtype, stream);
   } else {
     h = take(hidden);
     float* u = static_cast<float*>(state != nullptr ? state : take(2 * hidden));
@@ -439,7 +588,9 @@ int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* work
         return hipGetLastError() == hipSuccess ? 0 : -3;
       });
   }
-  return rc != 0 ? rc : product({h, a.F, true}, {a.w_out, a.ld_out, true}, y, a.R, a.D, a.F, dtype, at, stream);
+  if (rc != 0) return rc;
+  if (few_rows(a.R, dtype)) return launch_rows(h, a.F, a.w_out, a.ld_out, y, a.R, a.D, a.F, kNoGate, dtype, at, stream);
+  return product({h, a.F, true}, {a.w_out, a.ld_out, true}, y, a.R, a.D, a.F, dtype, at, stream);
 }
 
 int64_t gated_bwd_workspace(int R, int D, int F, int dtype, int gradients) {
