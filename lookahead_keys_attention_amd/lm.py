@@ -12,7 +12,10 @@ Differences a user can switch: `tie_embedding=True` shares the token embedding w
 projection (the reference keeps them separate, train_triton.py:86,111); `rotary_emb` / `prenorm`
 default to the reference's choice (both on, train_triton.py:99-100); `embedding_scale` multiplies the
 embedded tokens; `dropout` is the probability with which an element of the embedded tokens and of every
-block's output is dropped in training, on passes that neither take nor return caches.
+block's output is dropped in training, on passes that neither take nor return caches; `gated` has gated feed-forward blocks of
+two thirds of the hidden width (blocks.GatedFeedForward, `activation` "silu" or "gelu"); `post_norm` puts a norm behind every
+block too, and `residual_scale` a learned scale of its branch that begins there (blocks.ResidualBranch: sum and norms are one
+launch then).
 
 Vocabularies of any size.  From LINEAR_LOSS_MIN_VOCABULARY on, `return_loss` of a native model whose modules run as they are (no
 hooks, no autocast, no torch.compile) forms no logits where they would take more than LOGITS_MAX_BYTES or be slower
@@ -29,8 +32,10 @@ import math
 import torch
 import torch.nn.functional as F
 from torch import nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import _native, ops
+from .blocks import GatedFeedForward, ResidualBranch, _native_tensors
 from .castle import Castle, _linear, _unmodified
 
 
@@ -252,6 +257,12 @@ class GraphedDecoder:
             h = _native.host().gather_rows(embedding.weight, self.token) if model.embedding_scale == 1 else ops.embedding(embedding.weight, self.token, model.embedding_scale)
         else:
             h = model._embed(self.token, False)
+        if model.has_branches:
+            n = model.first_norm(h)
+            for index, ((attention, feed_forward), store) in enumerate(zip(model.layers, self.stores)):
+                h, n = model._branch(2 * index, attention.graph_step(n, store, self.t_device, self.base_device), h)
+                h, n = model._branch(2 * index + 1, feed_forward(n), h)
+            return Castle._project(model.to_logits, n, True)
         for (attention, feed_forward), store in zip(model.layers, self.stores):
             h = attention.graph_step(h, store, self.t_device, self.base_device, residual=h)
             h = token_feed_forward(feed_forward, h)
@@ -279,28 +290,35 @@ class GraphedDecoder:
 
 
 class CastleLM(nn.Module):
-    embedding_scale, dropout = 1.0, 0.0   # (of models that were saved whole without them)
+    embedding_scale, dropout, gated = 1.0, 0.0, False   # (of models that were saved whole without them)
 
     def __init__(self, *, num_tokens, dim, depth, max_seq_len=512, dim_head=64, heads=8, use_triton=True,
-                 rotary_emb=True, prenorm=True, tie_embedding=False, embedding_scale=1.0, dropout=0.0):
+                 rotary_emb=True, prenorm=True, tie_embedding=False, embedding_scale=1.0, dropout=0.0, gated=False, activation="silu", post_norm=False, residual_scale=None):
         super().__init__()
+        branches = post_norm or residual_scale is not None
+        if branches and not prenorm:
+            raise ValueError("CastleLM: post_norm and residual_scale stand beside the norms in front of the blocks (prenorm)")
         if not 0 <= dropout <= 1:
             raise ValueError(f"CastleLM: dropout is a probability, got {dropout}")
         self.max_seq_len = max_seq_len
         self.embedding_scale = float(embedding_scale)
         self.dropout = float(dropout)
+        self.gated = bool(gated)
         self.token_emb = nn.Embedding(num_tokens, dim)
         self.layers = nn.ModuleList()
         for _ in range(depth):
             attention = Castle(dim=dim, heads=heads, dim_head=dim_head, use_triton=use_triton,
-                               rotary_emb=rotary_emb, prenorm=prenorm)
-            feed_forward = nn.Sequential(
-                nn.RMSNorm(dim),
-                nn.Linear(dim, 4 * dim, bias=False),
-                nn.GELU(),
-                nn.Linear(4 * dim, dim, bias=False),
-            )
+                               rotary_emb=rotary_emb, prenorm=prenorm and not branches)
+            if gated:
+                parts = [GatedFeedForward(dim, activation=activation, use_triton=use_triton)]
+            else:
+                parts = [nn.Linear(dim, 4 * dim, bias=False), nn.GELU(), nn.Linear(4 * dim, dim, bias=False)]
+            feed_forward = nn.Sequential(*([] if branches else [nn.RMSNorm(dim)]), *parts)
             self.layers.append(nn.ModuleList([attention, feed_forward]))
+        if branches:   # the norm in front of a block is that of the branch before it, the last one's the final norm
+            self.first_norm = nn.RMSNorm(dim)
+            self.branches = nn.ModuleList(ResidualBranch(dim, post_norm, residual_scale, use_triton) for _ in range(2 * depth))
+            self.next_norms = nn.ModuleList(nn.RMSNorm(dim) for _ in range(2 * depth - 1))
         self.final_norm = nn.RMSNorm(dim)
         self.to_logits = nn.Linear(dim, num_tokens, bias=False)
         if tie_embedding:
@@ -324,19 +342,42 @@ class CastleLM(nn.Module):
         # the PyTorch layers throughout, so it remains an independent baseline for the native one)
         token_step = h.shape[1] == 1 and not torch.is_grad_enabled() and native and not self._drops(training)
         next_cache = []
-        for index, (attention, feed_forward) in enumerate(self.layers):
+
+        def attend(index, attention, t):
             layer_cache = cache[index] if cache is not None and index < len(cache) else None
-            if return_next_cache:
-                attended, layer_next = attention(h, cache=layer_cache, return_next_cache=True)
-                next_cache.append(layer_next)
-            else:
-                attended = attention(h, cache=layer_cache, return_next_cache=False)
-            h = drop(attended, h)
-            h = token_feed_forward(feed_forward, h) if token_step else drop(block_feed_forward(feed_forward, h, native), h)
-        logits = Castle._project(self.to_logits, h, token_step, norm=self.final_norm, native=native)
+            if not return_next_cache:
+                return attention(t, cache=layer_cache, return_next_cache=False)
+            attended, layer_next = attention(t, cache=layer_cache, return_next_cache=True)
+            next_cache.append(layer_next)
+            return attended
+
+        if self.has_branches:
+            n = self.first_norm(h)
+            for index, (attention, feed_forward) in enumerate(self.layers):
+                h, n = self._branch(2 * index, drop(attend(index, attention, n), None), h)
+                h, n = self._branch(2 * index + 1, drop(feed_forward(n), None), h)
+        else:
+            for index, (attention, feed_forward) in enumerate(self.layers):
+                h = drop(attend(index, attention, h), h)
+                h = token_feed_forward(feed_forward, h) if token_step else drop(block_feed_forward(feed_forward, h, native), h)
+            n = None   # (the norm goes with the projection)
+        to_logits = self.to_logits
+        # (models without the newer blocks come here for their hooks, and keep their logits)
+        if (return_loss and native and (self.gated or n is not None) and _unmodified(to_logits, nn.Linear) and to_logits.bias is None and not _has_any_global_hook()
+                and _native_tensors(None, h, to_logits.weight) and linear_loss_is_ahead(target.numel(), to_logits.weight)):
+            return ops.linear_cross_entropy(self.final_norm(h) if n is None else n, to_logits.weight, target)
+        logits = Castle._project(to_logits, h if n is None else n, token_step, norm=self.final_norm if n is None else None, native=native)
         if return_loss:
             return F.cross_entropy(logits.transpose(1, 2), target)
         return (logits, next_cache) if return_next_cache else logits
+
+    @property
+    def has_branches(self):
+        return "branches" in self._modules
+
+    def _branch(self, index, x, residual):
+        """The end of block `index`: (sum, the norm in front of what comes next)."""
+        return self.branches[index](x, residual, self.next_norms[index] if index < len(self.next_norms) else self.final_norm)
 
     def _embed(self, x, native):
         embedding = self.token_emb

@@ -417,6 +417,7 @@ def dropout_add(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: 
 
 
 GATE_ACTIVATIONS = {"silu": 0, "gelu": 1}
+RESIDUAL_NORM_MAX_WIDTH = 8192   # CASTLE_RESIDUAL_MAX_WIDTH
 
 
 def gated_feed_forward(x: torch.Tensor, weight_in: torch.Tensor, weight_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
