@@ -6,6 +6,7 @@
 #include "castle_gelu.h"
 #include "castle_gemm.h"
 #include "castle_rows.h"
+#include "castle_weights.h"
 #include "castle_wide.h"
 #include <algorithm>
 
@@ -104,21 +105,7 @@ template <typename T, bool KC, int FREE, bool PAIRS> struct GatedOperand : WideO
       }
     }
   }
-  // the last step, `steps` of it left: zeros behind the contraction's end
-  __device__ __forceinline__ void load_end(int steps, uint32_t lds) {
-    const T* zeros = reinterpret_cast<const T*>(castle_gated_zeros);
-    if constexpr (KC) {
-      W::load_end(steps, zeros, lds);
-    } else {
-      constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
-      const int first = wave_id() * N, k = ROWS * first + lane_id() / PIECES;
-#pragma unroll
-      for (int q = 0; q < N; ++q) {
-        if (k + ROWS * q < steps) load_to_lds(W::at, W::off[q], lds + 1024 * (first + q));
-        else load_to_lds(zeros, 0, lds + 1024 * (first + q));
-      }
-    }
-  }
+  __device__ __forceinline__ void load_end(int steps, uint32_t lds) { W::load_end(steps, reinterpret_cast<const T*>(castle_gated_zeros), lds); }
 };
 
 typedef vec<uint32_t, 4> u4;
@@ -372,7 +359,7 @@ template <int MODE> int launch_product(const GatedProductArgs& a, int rows, int 
 // What bounds them is reading the weights once, and how many bytes the busiest CU draws (about 50 a ns): its rows of x and of the weights.  So every workgroup takes all rows and as many columns as let
 // all CUs have one, both halves of them side by side, and its eight waves split the contraction, straight from memory to the matrix instructions, a few steps in flight at a time.  The second product,
 // whose contraction is the long one, goes in ranges of it too, joined by a launch of its own.
-// 32 rows of 2048 through 5504: 28.3 us with the tiles above and products in ranges, of which 19 and 11.5 on the GPU; now FIRST and SECOND.
+// 32 rows of 2048 through 5504: 28.3 us with the tiles above and products in ranges, of which 19 and 11.5 on the GPU; here 24.9, of which 13.8 the first and 8.5 + 3.8 the second with its join.
 constexpr int kFewRows = 64, kRowWaves = 8, kRowDepth = 32;   // rows at most, waves, contraction of a step
 struct RowsArgs {
   const void *x, *w;
@@ -548,6 +535,13 @@ int grads(const Operand2& dy, const Operand2& x, const Operand2& w, void* dw, vo
 // f(activation)
 template <typename F> int by_act(int act, F&& f) { return act == kSilu ? f(std::integral_constant<int, kSilu>()) : f(std::integral_constant<int, kGeluGate>()); }
 
+// Both weight gradients in one launch, where that is ahead of one for each (the second of which may be that of dx too)
+bool both_weights(int R, int D, int F, int dtype, bool dx, WeightsPlan& p) {
+  if (dtype == 0 || (dx && grads_workspace(R, 2 * F, D, 2, kGemmPlain, false) >= 0)) return false;
+  p = weights_plan(R, 2 * F, D, D, F);
+  return p.cost < gemm_cost(2 * F, D, R, 2) + gemm_cost(D, F, R, 2);
+}
+
 bool few_rows(int R, int dtype) { return R <= kFewRows && dtype != 0; }
 int64_t hidden_bytes(int R, int F, int dtype) { return up((int64_t)R * F * elem_size(dtype)); }
 int64_t planes_bytes(int R, int D, int F) {
@@ -595,7 +589,10 @@ int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* work
 
 int64_t gated_bwd_workspace(int R, int D, int F, int dtype, int gradients) {
   const bool dx = gradients & 1, dw_in = gradients & 2, dw_out = gradients & 4, below = dx || dw_in;
-  const int64_t hidden = hidden_bytes(R, F, dtype), products = std::max(dw_out ? product_workspace(D, F, R, dtype) : 0, below ? grads_bytes(R, 2 * F, D, dtype, dw_in, dx) : 0);
+  const int64_t hidden = hidden_bytes(R, F, dtype);
+  int64_t products = std::max(dw_out ? product_workspace(D, F, R, dtype) : 0, below ? grads_bytes(R, 2 * F, D, dtype, dw_in, dx) : 0);
+  WeightsPlan p;
+  if (dw_in && dw_out && both_weights(R, D, F, dtype, dx, p)) products = std::max(up(weights_workspace(p)), dx ? product_workspace(R, D, 2 * F, dtype) : 0);
   if (dtype != 0) return std::max<int64_t>(256, (below ? 2 * hidden : 0) + products);
   return (dw_out ? hidden : 0) + (below ? 3 * hidden + std::max(products, product_workspace(R, F, D, 0)) : products);
 }
@@ -628,6 +625,11 @@ int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void
                            static_cast<float*>(du), h32);
         return hipGetLastError() == hipSuccess ? 0 : -3;
       });
+  }
+  WeightsPlan plan;
+  if (rc == 0 && dw_in != nullptr && dw_out != nullptr && both_weights(a.R, a.D, a.F, dtype, dx != nullptr, plan)) {
+    rc = launch_weights({du, a.x, dw_in, 2 * a.F, a.D, 2 * a.F, a.ld_x}, {dy, h, dw_out, a.D, a.F, a.D, a.F}, a.R, plan, dtype, reinterpret_cast<float*>(at), stream);
+    return rc != 0 || dx == nullptr ? rc : product({du, 2 * a.F, true}, {a.w_in, a.ld_in, false}, dx, a.R, a.D, 2 * a.F, dtype, at, stream);
   }
   if (rc == 0 && dw_out != nullptr) rc = product({dy, a.D, false}, {h, a.F, false}, dw_out, a.D, a.F, a.R, dtype, at, stream);
   if (rc != 0 || !below) return rc;

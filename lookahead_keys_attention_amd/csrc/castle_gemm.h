@@ -36,6 +36,7 @@ constexpr int kNormBytes = 2048;   // longest row that a product normalises
 bool gemm_norm_ok(int M, int N, int K, int elem_size);
 bool gemm_amax_ok(int M, int N, int K, int elem_size, int amax_from, int amax_to);
 void gemm_plan(int M, int N, int K, int elem_size, bool epilogue, int (&out)[4]);
+float gemm_cost(int M, int N, int K, int elem_size);   // what a plain product takes, us
 int64_t gemm_workspace(int M, int N, int K, int elem_size, bool epilogue);
 // fp32, castle_gemm32.hip
 int launch_gemm32(const GemmArgs& a, bool a_kc, bool b_kc, int tile, int splits, int waves, hipStream_t stream);

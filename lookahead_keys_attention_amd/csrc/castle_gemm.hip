@@ -686,6 +686,8 @@ template <typename T, bool AK, bool BKC> int launch_t(GemmArgs a, const Plan& p,
 
 }  // namespace
 
+float gemm_cost(int M, int N, int K, int elem_size) { return plan(M, N, K, true, elem_size).cost; }
+
 int64_t gemm_workspace(int M, int N, int K, int elem_size, bool epilogue) {
   const Plan p = plan(M, N, K, !epilogue, elem_size);
   return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;

@@ -20,7 +20,7 @@ template <typename T, bool KC, int FREE> struct WideOperand {
     left = free_end - free0;
     place((int)ld, kWideK);
   }
-  // steps: what is left of the contraction; behind its end the last row is read again (KC: load_end)
+  // steps: what is left of the contraction; behind its end the last row is read again (or load_end)
   __device__ __forceinline__ void place(int ld, int steps) {
     const int lane = lane_id(), first = wave_id() * N;
 #pragma unroll
@@ -40,15 +40,21 @@ template <typename T, bool KC, int FREE> struct WideOperand {
     for (int q = 0; q < N; ++q) load_to_lds(at, off[q], lds + 1024 * (wave_id() * N + q));
     at += KC ? kWideK : kWideK * ld;
   }
-  // KC, the last step of a contraction, `steps` of it left: the pieces behind its end are those 16 bytes of zeros.  (Read again, whatever is not finite there would meet the zeros of
+  // The last step of a contraction, `steps` of it left: the pieces behind its end are those 16 bytes of zeros.  (Read again, whatever is not finite there would meet the zeros of
   // the other operand's rows.)
   __device__ __forceinline__ void load_end(int steps, const T* zeros, uint32_t lds) {
-    static_assert(KC, "");
     const int lane = lane_id(), first = wave_id() * N;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7);
-      if (8 * piece < steps) load_to_lds(at, off[q], lds + 1024 * (first + q));
+      bool there;
+      if constexpr (KC) {
+        const int row = 8 * (first + q) + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7);
+        there = 8 * piece < steps;
+      } else {
+        constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
+        there = ROWS * (first + q) + lane / PIECES < steps;
+      }
+      if (there) load_to_lds(at, off[q], lds + 1024 * (first + q));
       else load_to_lds(zeros, 0, lds + 1024 * (first + q));
     }
   }

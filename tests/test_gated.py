@@ -134,6 +134,22 @@ def test_sizes_of_tiles(R, D, F):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R, D, F", [(199, 1024, 4096), (3000, 768, 2048), (12345, 200, 520), (1000, 2048, 4096), (2048, 2048, 3000)])
+def test_weight_gradients_of_one_launch(R, D, F, dtype):
+    """Tiles taken whole, in ranges, both; contractions that end inside a step, with rows behind the end that are not finite; ragged tiles; the same bits again."""
+    x, win, wout, dy = (t.to(DEV) for t in inputs(R, D, F, dtype, seed=R))
+    ref = {k: (v.cpu(), off.cpu()) for k, (v, off) in reference(x, win, wout, dy, "silu", dtype).items()}
+    longer = [torch.cat((t, torch.full((64, D), float("nan"), device=DEV, dtype=dtype))) for t in (x, dy)]
+    x, dy = (t[:R] for t in longer)
+    got = run(x, win, wout, dy, "silu")
+    for k in ref:
+        within(got[k], ref[k], dtype, k)
+    again = run(x, win, wout, dy, "silu")
+    assert all(torch.equal(got[k], again[k]) for k in got)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows", [1, 2, 16, 17, 32, 50, 64])
 def test_tokens_without_gradients(rows, dtype):

@@ -208,8 +208,7 @@ def test_a_training_step_of_all_of_it(bits):
         assert ((p.detach().double() - want).abs() <= most * 1.01).all()
     # two steps outside, two replayed
     state = copy.deepcopy(optimizer.state_dict()), [p.detach().clone() for p in params]
-    losses = [step(), step()]
-    after = [p.detach().clone() for p in params]
+    eager = [(step(), [p.detach().clone() for p in params]) for _ in range(2)]
     optimizer.load_state_dict(state[0])
     with torch.no_grad():
         for p, old in zip(params, state[1]):
@@ -228,8 +227,10 @@ def test_a_training_step_of_all_of_it(bits):
         for p, g in zip(params, torch.autograd.grad(loss, params)):
             p.grad.copy_(g)
         optimizer.step()
-    for want in losses:
+    # The library's loss over (batch, classes, positions) adds its partial sums, one for each of the 4 sequences, to a bf16 number in any order: after each of 4 additions and the division
+    # half a step, so two orders are up to 2 (4 + 1) 2^-9 of it apart.  Nothing else depends on that number.
+    for want, after in eager:
         graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(loss.detach(), want)
-    assert all(torch.equal(p, q) for p, q in zip(params, after))
+        assert abs(float(loss.detach()) - float(want)) <= 10 * 2.0 ** -9 * float(want)
+        assert all(torch.equal(p, q) for p, q in zip(params, after))
