@@ -23,6 +23,10 @@ def _native_tensors(use_triton, *tensors) -> bool:
             and all(t is None or t.dtype == first.dtype and t.device == first.device for t in tensors))
 
 
+def _norm_of_rows(norm, width) -> bool:
+    return _unmodified(norm, nn.RMSNorm) and norm.weight is not None and norm.weight.shape == (width,)
+
+
 class GatedFeedForward(nn.Module):
     """to_out(act(g) * v) with (g, v) the halves of to_hidden(x); two thirds of the hidden width of a block without a gate give it the same number of parameters."""
 
@@ -57,11 +61,10 @@ class ResidualBranch(nn.Module):
 
     def forward(self, x, residual, next_norm):
         norm = self.norm
-        weight = None if norm is None else norm.weight
-        alike = norm is None or norm.eps == next_norm.eps
-        if (alike and _native_tensors(self.use_triton, x, residual, weight, self.scale, next_norm.weight) and _unmodified(next_norm, nn.RMSNorm) and (norm is None or _unmodified(norm, nn.RMSNorm))
-                and x.shape[-1] <= ops.RESIDUAL_NORM_MAX_WIDTH):
-            return ops.residual_norm(x, residual, weight=weight, scale=self.scale, next_weight=next_norm.weight, eps=next_norm.eps)
+        width = x.shape[-1]
+        if (_norm_of_rows(next_norm, width) and (norm is None or _norm_of_rows(norm, width) and norm.eps == next_norm.eps) and width <= ops.RESIDUAL_NORM_MAX_WIDTH
+                and _native_tensors(self.use_triton, x, residual, None if norm is None else norm.weight, self.scale, next_norm.weight)):
+            return ops.residual_norm(x, residual, weight=None if norm is None else norm.weight, scale=self.scale, next_weight=next_norm.weight, eps=next_norm.eps)
         if norm is not None:
             x = norm(x)
         if self.scale is not None:

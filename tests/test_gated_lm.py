@@ -154,6 +154,21 @@ def test_what_goes_through_the_kernels(monkeypatch):
 
 
 @gpu
+@pytest.mark.parametrize("next_norm", [torch.nn.RMSNorm(16, elementwise_affine=False), torch.nn.RMSNorm((3, 16)), torch.nn.RMSNorm(16)])
+@pytest.mark.parametrize("own", [torch.nn.RMSNorm(16, elementwise_affine=False), torch.nn.RMSNorm((3, 16)), None])
+def test_branches_with_other_norms(next_norm, own):
+    """Norms without weights or over more than a row: the formulation."""
+    branch = ResidualBranch(16, False, 0.3, use_triton=True)
+    branch.norm = own
+    branch, next_norm = branch.to(DEV), copy.deepcopy(next_norm).to(DEV)
+    x, r = torch.randn(2, 3, 16, device=DEV), torch.randn(2, 3, 16, device=DEV)
+    y, h = branch(x, r, next_norm)
+    want = r + 0.3 * (x if own is None else own.to(DEV)(x))
+    near(y, want, 1e-6, "sum")
+    near(h, next_norm(want), 1e-5, "norm")
+
+
+@gpu
 def test_loss_over_a_large_vocabulary_and_dropout():
     kind = dict(gated=True, post_norm=True, residual_scale=0.4, num_tokens=20000, embedding_scale=8.0)
     native, dense = models(kind, torch.bfloat16)
