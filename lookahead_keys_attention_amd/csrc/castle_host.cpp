@@ -1642,14 +1642,19 @@ OptTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor
       t[i].exp_avg_sq_exponents = static_cast<int8_t*>(ev.data_ptr());
       if (p.numel() == 0) t[i].exp_avg_exponents = t[i].exp_avg_sq_exponents = reinterpret_cast<int8_t*>(1);   // (nothing is read or written)
     }
-    for (const Tensor* w : {&p, &m, &v})
-      if (w->numel() > 0) {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(w->data_ptr());
-        written.emplace_back(at, at + w->numel() * w->element_size());
-      }
+    auto write = [&](const Tensor& w) {
+      if (w.numel() == 0) return;
+      const uintptr_t at = reinterpret_cast<uintptr_t>(w.data_ptr());
+      written.emplace_back(at, at + w.numel() * w.element_size());
+    };
+    for (const Tensor* w : {&p, &m, &v}) write(*w);
+    if (small) {
+      write((*avg_exponents)[i]);
+      write((*sq_exponents)[i]);
+    }
   }
   std::sort(written.begin(), written.end());
-  for (size_t i = 1; i < written.size(); ++i) TORCH_CHECK_VALUE(written[i - 1].second <= written[i].first, "adamw_step: two parameters or states share memory");
+  for (size_t i = 1; i < written.size(); ++i) TORCH_CHECK_VALUE(written[i - 1].second <= written[i].first, "adamw_step: two parameters, states or their exponents share memory");
   OptTensor norm = norm_given;
   if (max_norm && !norm) norm = at::empty({}, params[0].options().dtype(at::kFloat).requires_grad(false));
   const castle_adamw_options o = {lr, b1, b2, eps, weight_decay, max_norm.value_or(-1), lr_device ? static_cast<const float*>(lr_device->data_ptr()) : nullptr,

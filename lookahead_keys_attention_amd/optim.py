@@ -19,6 +19,11 @@ from . import ops
 _MOMENTS = ("exp_avg", "exp_avg_sq")
 
 
+def _order(t):
+    """The steps of a dense tensor's axes, but for those of one element, which say nothing."""
+    return [(n, s) for n, s in zip(t.shape, t.stride()) if n != 1] if t.numel() else []
+
+
 class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32, stochastic_rounding=True):
         if isinstance(lr, torch.Tensor):
@@ -55,7 +60,7 @@ class AdamW(torch.optim.Optimizer):
             chance = small or (group["stochastic_rounding"] and params[0].dtype != torch.float32)
             states = {k: [self.state[p][k] for p in params] for k in first if k not in ("step", "seed")}
             got = ops.adamw_step(params, [p.grad for p in params], states["exp_avg"], states["exp_avg_sq"], first["step"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                                 weight_decay=group["weight_decay"], max_norm=self.max_norm, norm=norm, seed=first["seed"] if chance else None,
+                                 weight_decay=group["weight_decay"], max_norm=self.max_norm, norm=None if norm is None else norm.to(params[0].device), seed=first["seed"] if chance else None,
                                  exp_avg_exponents=states.get("exp_avg_exponents"), exp_avg_sq_exponents=states.get("exp_avg_sq_exponents"))
             self.grad_norm = got
         return loss
@@ -66,7 +71,7 @@ class AdamW(torch.optim.Optimizer):
         kinds = {}
         for g in grads:
             kinds.setdefault((g.dtype, g.device), []).append(g)
-        norms = [ops.gradient_norm(k) for k in kinds.values()]
+        norms = [ops.gradient_norm(k).to(grads[0].device) for k in kinds.values()]
         return norms[0] if len(norms) == 1 else torch.linalg.vector_norm(torch.stack(norms).double()).float()
 
     def _calls(self, group):
@@ -107,9 +112,18 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """States come back in the types that they were saved in (torch.optim.Optimizer casts them to their parameters'); those that counted alike share one count again."""
-        super().load_state_dict(state_dict)
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
+        if any("state_bits" not in group for group in state_dict["param_groups"]):
+            raise ValueError("AdamW: these states were not saved by this optimizer")
+        for i, p in zip(saved, params):
+            for key in _MOMENTS if i in state_dict["state"] else ():
+                value = state_dict["state"][i][key]
+                if value.shape != p.shape:
+                    raise ValueError("AdamW: a saved state has another shape than its parameter")
+                if value.dtype != torch.float32 and _order(value) != _order(torch.empty_like(p, device="meta")):
+                    raise ValueError("AdamW: a saved state of 8 bits has another order in memory than its parameter, and its exponents go by that")
+        super().load_state_dict(state_dict)
         shared = {}
         for i, p in zip(saved, params):
             if i not in state_dict["state"]:
@@ -117,8 +131,6 @@ class AdamW(torch.optim.Optimizer):
             state = {}
             for key, value in state_dict["state"][i].items():
                 if key in _MOMENTS:
-                    if value.shape != p.shape:
-                        raise ValueError("AdamW: a saved state has another shape than its parameter")
                     state[key] = torch.empty_like(p, dtype=value.dtype)
                     # (numbers of 8 bits are copied as bytes)
                     same = value.dtype if value.dtype == torch.float32 else torch.uint8

@@ -434,6 +434,35 @@ def test_optimizer_goes_on_from_a_saved_state(bits, dtype):
         assert s["exp_avg"].element_size() == s["exp_avg_sq"].element_size() == 1 and s["exp_avg_exponents"].numel() == (24 * 40 + 255) // 256
 
 
+def test_saved_states_that_do_not_fit():
+    w = torch.nn.Parameter(torch.randn(24, 40))
+    optimizer = AdamW([w], state_bits=8)
+    small = lambda *shape: torch.zeros(*shape, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    numbers = dict(step=torch.ones(1, dtype=torch.int64), seed=torch.zeros(1, dtype=torch.int64), exp_avg_exponents=torch.zeros(4, dtype=torch.int8), exp_avg_sq_exponents=torch.zeros(4, dtype=torch.int8))
+    saved = lambda m, v: dict(optimizer.state_dict(), state={0: dict(numbers, exp_avg=m, exp_avg_sq=v)})
+    optimizer.load_state_dict(saved(small(24, 40), small(24, 40)))
+    assert optimizer.state[w]["exp_avg"].dtype == torch.float8_e4m3fn
+    for m, v in ((small(40, 24).T, small(24, 40)), (small(24, 40), small(40, 24).T), (small(40, 24), small(40, 24))):
+        with pytest.raises(ValueError):
+            optimizer.load_state_dict(saved(m, v))
+    with pytest.raises(ValueError):
+        optimizer.load_state_dict(torch.optim.AdamW([torch.nn.Parameter(torch.randn(24, 40))]).state_dict())
+    one = torch.nn.Parameter(torch.randn(1, 40).T)   # an axis of one element says nothing about the order
+    AdamW([one], state_bits=8).load_state_dict(saved(small(40, 1), small(40, 1)))
+
+
+@gpu
+def test_exponents_that_share_memory_are_refused():
+    params = [torch.zeros(512, device=DEV) for _ in range(2)]
+    state = lambda: [torch.zeros(512, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2)]
+    e = lambda: [torch.zeros(2, dtype=torch.int8, device=DEV) for _ in range(2)]
+    one, step, seed = e(), torch.zeros(1, dtype=torch.int64, device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV)
+    for em, ev in (([one[0], one[0]], e()), (one, [one[1], one[0]])):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.adamw_step(params, [torch.ones_like(p) for p in params], state(), state(), step, lr=1e-3, seed=seed, exp_avg_exponents=em, exp_avg_sq_exponents=ev)
+    assert int(step) == 0
+
+
 @gpu
 def test_optimizer_with_parameters_that_join_later_and_several_types():
     net = torch.nn.ModuleList([torch.nn.Linear(8, 8, device=DEV), torch.nn.Linear(8, 8, device=DEV, dtype=torch.bfloat16), torch.nn.Linear(8, 8, device=DEV)])
