@@ -514,22 +514,39 @@ int product(const Operand2& a, const Operand2& b, void* c, int M, int N, int K, 
   const GemmArgs g = {a.p, b.p, c, nullptr, M, N, K, a.ld, b.ld, N, kGemmPlain, 0, nullptr, nullptr, nullptr, 0, 1, nullptr, 0.f, nullptr, nullptr};
   return launch_gemm(g, a.kc, b.kc, dtype, static_cast<float*>(workspace), stream);
 }
-// Both gradients of a projection y = x w^T, dy [R][N], x [R][K], in one launch where that is ahead
-int64_t grads_bytes(int R, int N, int K, int dtype, bool dw, bool dx) {
-  const int64_t both = dw && dx ? grads_workspace(R, N, K, elem_size(dtype), kGemmPlain, false) : -1;
-  if (both >= 0) return up(both);
-  return std::max(dw ? product_workspace(N, K, R, dtype) : 0, dx ? product_workspace(R, K, N, dtype) : 0);
+// Gradients of a projection y = x w^T, dy [R][N], x [R][K], and `more`, the weight gradient of another one of as many rows: of what is asked for (c not nullptr) as much in one launch as is ahead so
+struct More {
+  Operand2 a, b;
+  void* c;
+  int M, N;
+};
+int64_t grads_bytes(int R, int N, int K, int dtype, bool dw, bool dx, int more_m, int more_n) {
+  const int64_t more = more_m > 0 ? product_workspace(more_m, more_n, R, dtype) : 0, both = dw && dx ? grads_workspace(R, N, K, elem_size(dtype), kGemmPlain, false) : -1;
+  if (both < 0) return std::max({dw ? product_workspace(N, K, R, dtype) : 0, dx ? product_workspace(R, K, N, dtype) : 0, more});
+  const int64_t third = more_m > 0 ? grads_more(R, N, K, elem_size(dtype), more_m, more_n) : -1;
+  return third >= 0 ? up(both + third) : std::max(up(both), more);
 }
-int grads(const Operand2& dy, const Operand2& x, const Operand2& w, void* dw, void* dx, int R, int N, int K, int dtype, void* workspace, hipStream_t stream) {
+int grads(const Operand2& dy, const Operand2& x, const Operand2& w, void* dw, void* dx, int R, int N, int K, const More& more, int dtype, void* workspace, hipStream_t stream) {
+  const auto args = [](const Operand2& a, const Operand2& b, void* c, int M, int N, int K) {
+    return GemmArgs{a.p, b.p, c, nullptr, M, N, K, a.ld, b.ld, N, kGemmPlain, 0, nullptr, nullptr, nullptr, 0, 1, nullptr, 0.f, nullptr, nullptr};
+  };
   if (dw != nullptr && dx != nullptr && grads_workspace(R, N, K, elem_size(dtype), kGemmPlain, false) >= 0) {
-    GradsArgs p = {};
-    p.w = {dy.p, x.p, dw, nullptr, N, K, R, dy.ld, x.ld, K, kGemmPlain, 0, nullptr, nullptr, nullptr, 0, 1, nullptr, 0.f, nullptr, nullptr};
-    p.x = {dy.p, w.p, dx, nullptr, R, K, N, dy.ld, w.ld, K, kGemmPlain, 0, nullptr, nullptr, nullptr, 0, 1, nullptr, 0.f, nullptr, nullptr};
-    return launch_grads(p, dtype, static_cast<float*>(workspace), nullptr, stream);
+    MoreGradsArgs p = {};
+    p.w = args(dy, x, dw, N, K, R);
+    p.x = args(dy, w, dx, R, K, N);
+    if (more.c == nullptr) return launch_grads(p, dtype, static_cast<float*>(workspace), nullptr, stream);
+    if (grads_more(R, N, K, elem_size(dtype), more.M, more.N) >= 0) {
+      p.v = args(more.a, more.b, more.c, more.M, more.N, R);
+      return launch_more_grads(p, dtype, static_cast<float*>(workspace), stream);
+    }
+    const int rc = product(more.a, more.b, more.c, more.M, more.N, R, dtype, workspace, stream);
+    return rc != 0 ? rc : launch_grads(p, dtype, static_cast<float*>(workspace), nullptr, stream);
   }
-  if (dx != nullptr)
-    if (const int rc = product({dy.p, dy.ld, true}, {w.p, w.ld, false}, dx, R, K, N, dtype, workspace, stream)) return rc;
-  return dw == nullptr ? 0 : product({dy.p, dy.ld, false}, {x.p, x.ld, false}, dw, N, K, R, dtype, workspace, stream);
+  int rc = 0;
+  if (more.c != nullptr) rc = product(more.a, more.b, more.c, more.M, more.N, R, dtype, workspace, stream);
+  if (rc == 0 && dx != nullptr) rc = product({dy.p, dy.ld, true}, {w.p, w.ld, false}, dx, R, K, N, dtype, workspace, stream);
+  if (rc == 0 && dw != nullptr) rc = product({dy.p, dy.ld, false}, {x.p, x.ld, false}, dw, N, K, R, dtype, workspace, stream);
+  return rc;
 }
 
 // f(activation)
@@ -590,7 +607,7 @@ int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* work
 int64_t gated_bwd_workspace(int R, int D, int F, int dtype, int gradients) {
   const bool dx = gradients & 1, dw_in = gradients & 2, dw_out = gradients & 4, below = dx || dw_in;
   const int64_t hidden = hidden_bytes(R, F, dtype);
-  int64_t products = std::max(dw_out ? product_workspace(D, F, R, dtype) : 0, below ? grads_bytes(R, 2 * F, D, dtype, dw_in, dx) : 0);
+  int64_t products = grads_bytes(R, 2 * F, D, dtype, dw_in, dx, dw_out ? D : 0, F);
   WeightsPlan p;
   if (dw_in && dw_out && both_weights(R, D, F, dtype, dx, p)) products = std::max(up(weights_workspace(p)), dx ? product_workspace(R, D, 2 * F, dtype) : 0);
   if (dtype != 0) return std::max<int64_t>(256, (below ? 2 * hidden : 0) + products);
@@ -631,9 +648,8 @@ int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void
     rc = launch_weights({du, a.x, dw_in, 2 * a.F, a.D, 2 * a.F, a.ld_x}, {dy, h, dw_out, a.D, a.F, a.D, a.F}, a.R, plan, dtype, reinterpret_cast<float*>(at), stream);
     return rc != 0 || dx == nullptr ? rc : product({du, 2 * a.F, true}, {a.w_in, a.ld_in, false}, dx, a.R, a.D, 2 * a.F, dtype, at, stream);
   }
-  if (rc == 0 && dw_out != nullptr) rc = product({dy, a.D, false}, {h, a.F, false}, dw_out, a.D, a.F, a.R, dtype, at, stream);
-  if (rc != 0 || !below) return rc;
-  return grads({du, 2 * a.F, true}, {a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, dw_in, dx, a.R, 2 * a.F, a.D, dtype, at, stream);
+  if (rc != 0) return rc;
+  return grads({du, 2 * a.F, true}, {a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, dw_in, dx, a.R, 2 * a.F, a.D, {{dy, a.D, false}, {h, a.F, false}, dw_out, a.D, a.F}, dtype, at, stream);
 }
 
 }  // namespace castle

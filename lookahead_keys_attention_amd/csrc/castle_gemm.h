@@ -32,6 +32,11 @@ struct GradsArgs {
   GemmArgs w, x;
   int w_groups, w_row, x_groups, x_row;
 };
+// And between them another weight gradient v of as many rows, in as many ranges.  (By itself: longer arguments cost every launch 0.1 to 0.2 us.)
+struct MoreGradsArgs : GradsArgs {
+  GemmArgs v;
+  int v_groups, v_row;
+};
 constexpr int kNormBytes = 2048;   // longest row that a product normalises
 bool gemm_norm_ok(int M, int N, int K, int elem_size);
 bool gemm_amax_ok(int M, int N, int K, int elem_size, int amax_from, int amax_to);
@@ -41,10 +46,13 @@ int64_t gemm_workspace(int M, int N, int K, int elem_size, bool epilogue);
 // fp32, castle_gemm32.hip
 int launch_gemm32(const GemmArgs& a, bool a_kc, bool b_kc, int tile, int splits, int waves, hipStream_t stream);
 int launch_grads32(const GradsArgs& p, int tile, int waves, hipStream_t stream);
+int launch_grads32(const MoreGradsArgs& p, int tile, int waves, hipStream_t stream);
 struct GradsPlan { int tile, waves, w_splits, x_splits; };   // tile 0: two launches
 GradsPlan grads_plan(int R, int N, int K, int elem_size, int epilogue, bool amax);
 int64_t grads_workspace(int R, int N, int K, int elem_size, int epilogue, bool amax);   // -1: two launches are ahead
+int64_t grads_more(int R, int N, int K, int elem_size, int M2, int N2);   // further workspace for a v of M2 x N2; -1: a launch of its own is ahead
 struct PartSum;
+int launch_more_grads(MoreGradsArgs p, int dtype, float* workspace, hipStream_t stream);
 int launch_grads(GradsArgs p, int dtype, float* workspace, PartSum* later, hipStream_t stream);   // later: dw's sum is left to launch_sums, if it has one (parts > 0)
 int launch_gemm(GemmArgs a, bool a_kc, bool b_kc, int dtype, float* workspace, hipStream_t stream);
 

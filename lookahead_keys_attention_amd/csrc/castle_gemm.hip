@@ -19,6 +19,7 @@
 #include "castle_waves.h"
 #include "castle_wide.h"
 #include <algorithm>
+#include <type_traits>
 #include <cmath>
 #include "castle_rows.h"
 
@@ -320,10 +321,18 @@ __global__ __launch_bounds__(kThreads * G, BM == 128 ? 2 : 4) void gemm_kernel(G
 // (w.k_per_split rows of the contraction each), then those of the input gradient.
 // Each by itself is bound by its start, trips to memory and CUs that stay idle; together they fill them (3000 rows 256 -> 1536, us: 16.8 and 11.4, both 19.0; the rule and
 // more figures at grads_plan).  Tiles of 64 x 64 for both, by one or two groups: larger ones do not leave a CU room for a workgroup of the other.
-template <typename T, int G> __global__ __launch_bounds__(kThreads * G, 4) void grads_kernel(GradsArgs p) {
+template <typename T, int G, typename Args> __global__ __launch_bounds__(kThreads * G, 4) void grads_kernel(Args p) {
   constexpr int kElems = max2(tile_elems<T, false, false, 64, 64, kStep16, G>(), tile_elems<T, true, false, 64, 64, kStep16, G>());
   __shared__ __attribute__((aligned(16))) T smem[kElems];
   int b = blockIdx.x;
+  if constexpr (std::is_same_v<Args, MoreGradsArgs>) {
+    if (b >= p.w_groups && b < p.w_groups + p.v_groups) {
+      b -= p.w_groups;
+      gemm_tiles<T, false, false, 64, 64, kStep16, G, false>(p.v, smem, b % p.v_row, b / p.v_row, p.v_row);
+      return;
+    }
+    if (b >= p.w_groups) b -= p.v_groups;
+  }
   if (b < p.w_groups) {
     gemm_tiles<T, false, false, 64, 64, kStep16, G, false>(p.w, smem, b % p.w_row, b / p.w_row, p.w_row);
   } else {
@@ -785,7 +794,18 @@ int64_t grads_workspace(int R, int N, int K, int elem_size, int epilogue, bool a
   if (g.tile == 0) return -1;
   return ((g.w_splits > 1 ? (int64_t)g.w_splits * N * K : 0) + (g.x_splits > 1 ? (int64_t)g.x_splits * R * K : 0)) * 4;
 }
-int launch_grads(GradsArgs p, int dtype, float* workspace, PartSum* later, hipStream_t stream) {
+// A third product takes what the CUs are not busy with: 256 rows of 512 through 1408, with their gate's gradient, 24.6 us in three launches and 21.7 in two; fp32 3000 rows of 256 through 680 93.5 and
+// 78.6.  Workgroups of eight waves (two to a CU) that need another round for it do not: bf16 777 rows of 768 through 2048 53.4 and 57.6, fp32 128 rows of 768 through 768 32.0 and 34.4.
+int64_t grads_more(int R, int N, int K, int elem_size, int M2, int N2) {
+  const GradsPlan g = grads_plan(R, N, K, elem_size, kGemmPlain, false);
+  const auto tiles = [&](int m, int n) { return (int64_t)((m + g.tile - 1) / g.tile) * ((n + g.tile - 1) / g.tile); };
+  const int64_t two = tiles(N, K) * g.w_splits + tiles(R, K) * g.x_splits, more = tiles(M2, N2) * g.w_splits;
+  if (g.waves == 8 && (two + more + 511) / 512 > (two + 511) / 512) return -1;
+  return g.w_splits > 1 ? (int64_t)g.w_splits * M2 * N2 * 4 : 0;
+}
+namespace {
+template <typename Args> int launch_grads_as(Args& p, int dtype, float* workspace, PartSum* later, hipStream_t stream) {
+  constexpr bool MORE = std::is_same_v<Args, MoreGradsArgs>;
   const int step = dtype == 0 ? 32 : kStep16;
   const GradsPlan g = grads_plan(p.x.M, p.x.K, p.x.N, dtype == 0 ? 4 : 2, p.x.epilogue, p.x.amax != nullptr);
   auto place = [&](GemmArgs& a, int splits, int& groups, int& row) {
@@ -798,23 +818,34 @@ int launch_grads(GradsArgs p, int dtype, float* workspace, PartSum* later, hipSt
   };
   place(p.w, g.w_splits, p.w_groups, p.w_row);
   place(p.x, g.x_splits, p.x_groups, p.x_row);
+  int all = p.w_groups + p.x_groups;
+  if constexpr (MORE) {
+    place(p.v, g.w_splits, p.v_groups, p.v_row);
+    all += p.v_groups;
+  }
   int rc = dtype == 0 ? launch_grads32(p, g.tile, g.waves, stream) : by_type16(dtype, true, [&](auto t, auto) {
     using T = decltype(t);
-    if (g.waves == 8) hipLaunchKernelGGL((grads_kernel<T, 2>), dim3(p.w_groups + p.x_groups), dim3(2 * kThreads), 0, stream, p);
-    else hipLaunchKernelGGL((grads_kernel<T, 1>), dim3(p.w_groups + p.x_groups), dim3(kThreads), 0, stream, p);
+    if (g.waves == 8) hipLaunchKernelGGL((grads_kernel<T, 2, Args>), dim3(all), dim3(2 * kThreads), 0, stream, p);
+    else hipLaunchKernelGGL((grads_kernel<T, 1, Args>), dim3(all), dim3(kThreads), 0, stream, p);
     return hipGetLastError() == hipSuccess ? 0 : -3;
   });
-  PartSum sums[2];
+  PartSum sums[3];
   int count = 0;
   if (later != nullptr) later->parts = 0;
-  for (const GemmArgs* a : {&p.w, &p.x}) {
-    if (a->part == nullptr) continue;
-    const PartSum sum = {a->part, (int64_t)a->M * a->N, a->c, (a->K + a->k_per_split - 1) / a->k_per_split, 0};
-    if (a == &p.w && later != nullptr) *later = sum;
+  auto sum_of = [&](const GemmArgs& a) {
+    if (a.part == nullptr) return;
+    const PartSum sum = {a.part, (int64_t)a.M * a.N, a.c, (a.K + a.k_per_split - 1) / a.k_per_split, 0};
+    if (&a == &p.w && later != nullptr) *later = sum;
     else sums[count++] = sum;
-  }
+  };
+  sum_of(p.w);
+  sum_of(p.x);
+  if constexpr (MORE) sum_of(p.v);
   if (rc == 0 && count > 0) rc = launch_sums(sums, count, dtype, stream);
   return rc;
 }
+}  // namespace
+int launch_grads(GradsArgs p, int dtype, float* workspace, PartSum* later, hipStream_t stream) { return launch_grads_as(p, dtype, workspace, later, stream); }
+int launch_more_grads(MoreGradsArgs p, int dtype, float* workspace, hipStream_t stream) { return launch_grads_as(p, dtype, workspace, nullptr, stream); }
 
 }  // namespace castle

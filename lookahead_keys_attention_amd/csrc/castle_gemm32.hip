@@ -359,15 +359,30 @@ __global__ __launch_bounds__(64 * W, W / 4 < 2 ? 2 : W / 4) void gemm32_kernel(G
 }
 // both gradients of a projection: workgroups of the weight gradient, then those of the input gradient (castle_gemm.hip; 256 rows 512 -> 3072, us: 12.9 and 16.1, both
 // 24.6, 512 -> 512 5.6 and 6.5, both 8.4)
-template <int TILE, int W> __global__ __launch_bounds__(64 * W, W / 4 < 2 ? 2 : W / 4) void grads32_kernel(GradsArgs p) {
+template <int TILE, int W, typename Args> __global__ __launch_bounds__(64 * W, W / 4 < 2 ? 2 : W / 4) void grads32_kernel(Args p) {
   __shared__ __attribute__((aligned(16))) vec<float, 4> s_sum[W * wave_bytes<TILE>() / 16];
   int b = blockIdx.x;
+  if constexpr (std::is_same_v<Args, MoreGradsArgs>) {
+    if (b >= p.w_groups && b < p.w_groups + p.v_groups) {
+      b -= p.w_groups;
+      gemm32_tile<false, false, TILE, W, false>(p.v, s_sum, b % p.v_row, b / p.v_row);
+      return;
+    }
+    if (b >= p.w_groups) b -= p.v_groups;
+  }
   if (b < p.w_groups) {
     gemm32_tile<false, false, TILE, W, false>(p.w, s_sum, b % p.w_row, b / p.w_row);
   } else {
     b -= p.w_groups;
     gemm32_tile<true, false, TILE, W, false>(p.x, s_sum, b % p.x_row, b / p.x_row);
   }
+}
+template <typename Args> int launch_grads32_as(const Args& p, int groups, int tile, int waves, hipStream_t stream) {
+  const dim3 grid(groups);
+  if (tile == 32 && waves == 8) hipLaunchKernelGGL((grads32_kernel<32, 8, Args>), grid, dim3(512), 0, stream, p);
+  else if (tile == 32) hipLaunchKernelGGL((grads32_kernel<32, 4, Args>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((grads32_kernel<64, 4, Args>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError() == hipSuccess ? 0 : -3;
 }
 
 }  // namespace
@@ -392,12 +407,7 @@ int launch_gemm32(const GemmArgs& a, bool a_kc, bool b_kc, int tile, int splits,
   return b_kc ? -2 : go(no, no, no);
 }
 
-int launch_grads32(const GradsArgs& p, int tile, int waves, hipStream_t stream) {
-  const dim3 grid(p.w_groups + p.x_groups);
-  if (tile == 32 && waves == 8) hipLaunchKernelGGL((grads32_kernel<32, 8>), grid, dim3(512), 0, stream, p);
-  else if (tile == 32) hipLaunchKernelGGL((grads32_kernel<32, 4>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((grads32_kernel<64, 4>), grid, dim3(256), 0, stream, p);
-  return hipGetLastError() == hipSuccess ? 0 : -3;
-}
+int launch_grads32(const GradsArgs& p, int tile, int waves, hipStream_t stream) { return launch_grads32_as(p, p.w_groups + p.x_groups, tile, waves, stream); }
+int launch_grads32(const MoreGradsArgs& p, int tile, int waves, hipStream_t stream) { return launch_grads32_as(p, p.w_groups + p.v_groups + p.x_groups, tile, waves, stream); }
 
 }  // namespace castle

@@ -151,6 +151,19 @@ def test_weight_gradients_of_one_launch(R, D, F, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("R, D, F", [(2048, 64, 64), (3000, 64, 128), (4096, 128, 320), (777, 768, 2048), (128, 768, 768)])
+def test_gradients_of_one_launch(R, D, F, dtype):
+    """All three products of the backward pass together, in ranges of the rows or not, and the two launches where a third does not fit."""
+    t = inputs(R, D, F, dtype, seed=R + F)
+    ref = {k: (v.cpu(), off.cpu()) for k, (v, off) in reference(*(x.to(DEV) for x in t), "silu", dtype).items()}
+    got, again = run(*t, "silu"), run(*t, "silu")
+    for name in ref:
+        within(got[name], ref[name], dtype, name)
+        assert torch.equal(got[name], again[name])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows", [1, 2, 16, 17, 32, 50, 64])
 def test_tokens_without_gradients(rows, dtype):
     for D, F in ((64, 24), (512, 1408), (1040, 72)):
