@@ -108,6 +108,27 @@ template <typename T, bool KC, int FREE, bool PAIRS> struct GatedOperand : WideO
   __device__ __forceinline__ void load_end(int steps, uint32_t lds) { W::load_end(steps, reinterpret_cast<const T*>(castle_gated_zeros), lds); }
 };
 
+// x as a number of 32 bits, whoever reads it: a product that is rounded to 16 bits in the same instruction would not be the one whose rest is taken
+__device__ __forceinline__ void in_32_bits(float& x) { asm("" : "+v"(x)); }
+__device__ __forceinline__ void in_32_bits(vec<float, 16>& x) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    float e = x[r];
+    in_32_bits(e);
+    x[r] = e;
+  }
+}
+// what x loses when it is rounded to T; of what becomes infinite nothing
+template <typename T> __device__ __forceinline__ float rest(float x) {
+  const float r = (float)(T)x;
+  return __builtin_fabsf(r) == __builtin_inff() ? 0.f : x - r;
+}
+template <typename T> __device__ __forceinline__ vec<float, 16> rest(const vec<float, 16>& x) {
+  vec<float, 16> y;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) y[r] = rest<T>((float)x[r]);
+  return y;
+}
 typedef vec<uint32_t, 4> u4;
 // sixteen numbers of a lane as their upper 24 bits: [0], [1] upper halves, [2] the bytes behind them
 __device__ __forceinline__ void to_parts(const vec<float, 16>& x, u4 (&p)[3]) {
@@ -134,8 +155,8 @@ __device__ __forceinline__ vec<float, 16> from_parts(const u4& p0, const u4& p1,
 }
 
 // The frame is that of gemm_wide_kernel (castle_gemm.hip): eight waves, one workgroup to a CU, steps of 64 of the contraction straight from memory to LDS into two or three buffers, requested over the
-// end of a tile.  END: the contraction ends inside a step.
-template <typename T, int MODE, int ACT, int BM, bool END> __global__ __launch_bounds__(kWideThreads, 2) void gated_product_kernel(GatedProductArgs a) {
+// end of a tile.  END: the contraction ends inside a step.  LOW: what the rounding of h and of [dg dv] leaves is kept too, in as many rows behind them.
+template <typename T, int MODE, int ACT, int BM, bool END, bool LOW> __global__ __launch_bounds__(kWideThreads, 2) void gated_product_kernel(GatedProductArgs a) {
   typedef GatedShape<MODE, BM> S;
   typedef GatedOperand<T, true, BM, false> OpA;
   typedef GatedOperand<T, MODE != kBackward, S::BN, MODE != kBackward> OpB;
@@ -287,8 +308,17 @@ template <typename T, int MODE, int ACT, int BM, bool END> __global__ __launch_b
           x = from_parts(p[0], p[1], p[2]) * acc[i][j];   // dv
           y = from_parts(p[3], p[4], p[5]) * acc[i][j];   // dg
           T* out = static_cast<T*>(a.out);
+          if constexpr (LOW) {
+            in_32_bits(x);
+            in_32_bits(y);
+          }
           to_rows(y, out, 2 * (int64_t)a.F, m, n);
           to_rows(x, out + a.F, 2 * (int64_t)a.F, m, n);
+          if constexpr (LOW) {
+            out += (int64_t)a.R * 2 * a.F;
+            to_rows(rest<T>(y), out, 2 * (int64_t)a.F, m, n);
+            to_rows(rest<T>(x), out + a.F, 2 * (int64_t)a.F, m, n);
+          }
         } else {
           v16 h;
 #pragma unroll
@@ -308,7 +338,9 @@ template <typename T, int MODE, int ACT, int BM, bool END> __global__ __launch_b
 #pragma unroll
             for (int k = 0; k < 3; ++k) __builtin_nontemporal_store(p[k], to + (3 + k) * 64);
           }
+          if constexpr (LOW) in_32_bits(h);
           to_rows(h, static_cast<T*>(a.out), a.F, m, n);
+          if constexpr (LOW) to_rows(rest<T>(h), static_cast<T*>(a.out) + (int64_t)a.R * a.F, a.F, m, n);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -317,20 +349,25 @@ template <typename T, int MODE, int ACT, int BM, bool END> __global__ __launch_b
   }
 }
 
-template <typename T, int MODE, int ACT, int BM, bool END> int launch_product_as(const GatedProductArgs& a, hipStream_t stream) {
+template <typename T, int MODE, int ACT, int BM, bool END, bool LOW = false> int launch_product_as(const GatedProductArgs& a, hipStream_t stream) {
   typedef GatedShape<MODE, BM> S;
   static PerDeviceOnce once;
   bool& configured = once.flag();
   if (!configured) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gated_product_kernel<T, MODE, ACT, BM, END>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&gated_product_kernel<T, MODE, ACT, BM, END, LOW>), hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) != hipSuccess) return -3;
     configured = true;
   }
   const int64_t tiles = (int64_t)((a.R + BM - 1) / BM) * ((a.F + kTileF - 1) / kTileF);
-  hipLaunchKernelGGL((gated_product_kernel<T, MODE, ACT, BM, END>), dim3((unsigned)std::min<int64_t>((tiles + 7) / 8 * 8, 256)), dim3(kWideThreads), S::kLds, stream, a);
+  hipLaunchKernelGGL((gated_product_kernel<T, MODE, ACT, BM, END, LOW>), dim3((unsigned)std::min<int64_t>((tiles + 7) / 8 * 8, 256)), dim3(kWideThreads), S::kLds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -3;
 }
+// Few numbers, 16-bit types: where h and [dg dv] alone are rounded on the way, results are 1.4 times as far from the formula as results rounded once, and of a few hundred numbers now and then twice as
+// far.  There what the roundings leave takes part in the products too, and launches bound them as before (backward pass, us, rounded / in parts: 8 rows of 24 through 192 13.2 / 10.5, 5770 of 16 through 24
+// 19.4 / 15.1, 40 of 96 through 4000 20.7 / 18.5; 1 of 1904 through 5048 51 / 61, whose gradients of 2 x 38 MB are written in pieces of 16 bytes).
+bool few_numbers(int R, int D, int F) { return std::min({(int64_t)R * D, (int64_t)D * F, (int64_t)R * F}) < 4096; }
 // Rows of a tile: those with which the fullest CU is done first (us a step of the contraction, and at a tile's end); of both passes, which share the order of a and b.
 int tile_rows(int R, int D, int F) {
+  if (few_numbers(R, D, F)) return 64;
   const int steps = (D + kWideK - 1) / kWideK;
   auto cost = [&](int rows, double step, double end) {
     const int64_t tiles = (int64_t)((R + rows - 1) / rows) * ((F + kTileF - 1) / kTileF);
@@ -339,9 +376,14 @@ int tile_rows(int R, int D, int F) {
   const double large = cost(256, 1.4, 5), middle = cost(128, 0.85, 3), small = cost(64, 0.56, 1.6);
   return small < std::min(middle, large) ? 64 : middle < large ? 128 : 256;
 }
-template <int MODE> int launch_product(const GatedProductArgs& a, int rows, int act, int dtype, hipStream_t stream) {
+template <int MODE> int launch_product(const GatedProductArgs& a, int rows, int act, bool low, int dtype, hipStream_t stream) {
   return by_type16(dtype, true, [&](auto t, auto) {
     using T = decltype(t);
+    if (low) {
+      if constexpr (MODE != kBackward)
+        if (act == kGeluGate) return launch_product_as<T, MODE, kGeluGate, 64, true, true>(a, stream);
+      return launch_product_as<T, MODE, kSilu, 64, true, true>(a, stream);
+    }
     auto of_end = [&](auto bm, auto ac) {
       constexpr int BM = decltype(bm)::value, ACT = decltype(ac)::value;
       return a.K % kWideK != 0 ? launch_product_as<T, MODE, ACT, BM, true>(a, stream) : launch_product_as<T, MODE, ACT, BM, false>(a, stream);
@@ -368,7 +410,9 @@ struct RowsArgs {
   int64_t half;          // gate: elements from a row of w to the row of its other half
   int k_per_range;       // a multiple of kRowDepth
   void* out;             // [R][N]
-  float* part;           // or partial results [range][R][N]
+  float* part;           // or partial results [range][out_R][N]
+  int out_R;             // R; half of it: the rows of x are what has been rounded and, behind it, what that has left, and their sums are added
+  bool low;              // gate: what the rounding of `out` leaves goes behind it
 };
 typedef vec<float, 4> acc4_t;
 __device__ __forceinline__ void mma16(acc4_t& c, const vec<bf16_t, 8>& a, const vec<bf16_t, 8>& b) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -437,14 +481,18 @@ template <typename T, int ACT, int MT, int NT> __global__ __launch_bounds__(64 *
   };
   for (int o = threadIdx.x; o < 16 * MT * PER * NT; o += 64 * kRowWaves) {
     const int row = o / (PER * NT), col = o % (PER * NT), n = n0 + col;
-    if (row >= a.R || n >= n_end) continue;
+    if (row >= a.out_R || n >= n_end) continue;
     if constexpr (ACT != kNoGate) {
       const int at = col / 8 * 16 + col % 8;
-      static_cast<T*>(a.out)[(int64_t)row * a.N + n] = (T)(Gate<T, ACT>(sum(row, at)).act * sum(row, at + 8));
-    } else if (a.part != nullptr) {
-      a.part[((int64_t)blockIdx.y * a.R + row) * a.N + n] = sum(row, col);
+      float h = Gate<T, ACT>(sum(row, at)).act * sum(row, at + 8);
+      in_32_bits(h);
+      static_cast<T*>(a.out)[(int64_t)row * a.N + n] = (T)h;
+      if (a.low) static_cast<T*>(a.out)[(int64_t)(a.R + row) * a.N + n] = (T)rest<T>(h);
     } else {
-      static_cast<T*>(a.out)[(int64_t)row * a.N + n] = (T)sum(row, col);
+      float v = sum(row, col);
+      if (a.out_R < a.R) v += sum(a.out_R + row, col);
+      if (a.part != nullptr) a.part[((int64_t)blockIdx.y * a.out_R + row) * a.N + n] = v;
+      else static_cast<T*>(a.out)[(int64_t)row * a.N + n] = (T)v;
     }
   }
 }
@@ -485,20 +533,193 @@ template <typename T, int ACT> int launch_rows_as(const RowsArgs& a, int ranges,
   };
   return a.R <= 16 ? of_rows(std::integral_constant<int, 1>()) : a.R <= 32 ? of_rows(std::integral_constant<int, 2>()) : of_rows(std::integral_constant<int, 4>());
 }
-int64_t rows_bytes(int R, int N, int K) {
-  const RowsPlan p = rows_plan(R, N, K, false);
+// low: h, rounded, and behind it what that has left, is written (gate) or read
+int64_t rows_bytes(int R, int N, int K, bool low) {
+  const RowsPlan p = rows_plan(low ? 2 * R : R, N, K, false);
   return p.ranges > 1 ? ((int64_t)p.ranges * R * N * 4 + 255) / 256 * 256 : 0;
 }
 // act: kNoGate, or that of the gate between the two halves of w, N rows each
-int launch_rows(const void* x, int64_t ld_x, const void* w, int64_t ld_w, void* out, int R, int N, int K, int act, int dtype, void* workspace, hipStream_t stream) {
-  const RowsPlan p = rows_plan(R, N, K, act != kNoGate);
+int launch_rows(const void* x, int64_t ld_x, const void* w, int64_t ld_w, void* out, int R, int N, int K, int act, bool low, int dtype, void* workspace, hipStream_t stream) {
+  const int rows = low && act == kNoGate ? 2 * R : R;
+  const RowsPlan p = rows_plan(rows, N, K, act != kNoGate);
   const int per = ((K + p.ranges - 1) / p.ranges + kRowDepth - 1) / kRowDepth * kRowDepth, ranges = (K + per - 1) / per;
-  const RowsArgs a = {x, w, ld_x, ld_w, R, N, K, p.cols, (int64_t)N * ld_w, per, out, ranges > 1 ? static_cast<float*>(workspace) : nullptr};
+  const RowsArgs a = {x, w, ld_x, ld_w, rows, N, K, p.cols, (int64_t)N * ld_w, per, out, ranges > 1 ? static_cast<float*>(workspace) : nullptr, R, low};
   const int rc = by_type16(dtype, true, [&](auto t, auto) {
     using T = decltype(t);
     return act == kNoGate ? launch_rows_as<T, kNoGate>(a, ranges, stream) : act == kSilu ? launch_rows_as<T, kSilu>(a, 1, stream) : launch_rows_as<T, kGeluGate>(a, 1, stream);
   });
   return rc != 0 || ranges == 1 ? rc : launch_part_sum(a.part, ranges, (int64_t)R * N, out, dtype, stream);
+}
+
+// ---- 16-bit types, few numbers ---------------------------------------------------------------------------------------
+// Products of an operand in two parts, rounded and what that has left, with one in one: tiles of 32 x 32, four waves that take steps of 16 of the contraction in turns, straight from memory (16 bytes
+// where the contraction is contiguous, else element by element, whose lanes lie side by side), in ranges that fill the card, summed in a launch of their own.
+struct PartsJob {
+  const void *a, *low, *b;   // a and low [M][lda] or [K][lda], b [N][ldb] or [K][ldb]
+  int64_t lda, ldb, cm, cn;  // element (m, n) of c at m cm + n cn; one of them is 1
+  int M, N, K, ranges, k_per_range;   // k_per_range: a multiple of 16
+  void* c;
+  float* part;               // [range], in c's order
+};
+struct PartsArgs {
+  PartsJob job[3];
+  int groups[3];
+};
+// eight steps of the contraction of one row or column.  LAST: those behind its end are zeros (none of what memory holds there meets anything).  All are requested, then looked at.
+template <typename T, bool KC> struct PartsPiece {
+  vec<uint32_t, KC ? 4 : 8> w;
+  template <bool LAST> __device__ __forceinline__ void load(const T* p, int64_t ld, int k, int k_end) {
+    if constexpr (KC) {
+      w = *reinterpret_cast<const vec<uint32_t, 4>*>(p + (LAST ? min(k, k_end - 8) : k));   // (the contraction is a multiple of 8)
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = reinterpret_cast<const uint16_t*>(p)[(int64_t)(LAST ? min(k + e, k_end - 1) : k + e) * ld];
+    }
+  }
+  template <bool LAST> __device__ __forceinline__ frag<T> get(int k, int k_end) {
+    if constexpr (LAST) {
+#pragma unroll
+      for (int e = 0; e < (KC ? 4 : 8); ++e) {
+        uint32_t v = w[e];
+        asm("" : "+v"(v));   // (a request by itself, not one behind a condition)
+        w[e] = (KC ? k : k + e) < k_end ? v : 0u;
+      }
+    }
+    if constexpr (KC) return __builtin_bit_cast(frag<T>, w);
+    vec<uint32_t, 4> pairs;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pairs[e] = w[(KC ? 0 : 2) * e] | w[(KC ? 0 : 2) * e + (KC ? 0 : 1)] << 16;
+    return __builtin_bit_cast(frag<T>, pairs);
+  }
+};
+constexpr int kPartsWaves = 4;
+// the waves of a workgroup share a tile, or, for short contractions, each has one
+__host__ __device__ __forceinline__ bool parts_shared(int K) { return K > 64; }
+template <typename T, bool AKC, bool BKC> __device__ __forceinline__ void parts_tile(const PartsJob& j, int group, vec<float, 4>* s_sum) {
+  constexpr int U = 4;   // steps in flight
+  const int lane = lane_id(), wave = wave_id(), c = lane & 31, g = lane >> 5;
+  const bool shared = parts_shared(j.K);
+  const int tiles_n = (j.N + 31) / 32, tiles = (j.M + 31) / 32 * tiles_n, range = shared ? group / tiles : 0, tile = shared ? group % tiles : group * kPartsWaves + wave;
+  if (tile >= tiles) return;   // (not of a tile that waves share)
+  const int m0 = tile / tiles_n * 32, n0 = tile % tiles_n * 32, m = min(m0 + c, j.M - 1), n = min(n0 + c, j.N - 1);   // (rows and columns behind the end: the last one's, not stored)
+  const int k_end = min(j.K, (range + 1) * j.k_per_range), step = shared ? 16 * kPartsWaves : 16;
+  const T *a = static_cast<const T*>(j.a) + (AKC ? m * j.lda : m), *low = static_cast<const T*>(j.low) + (AKC ? m * j.lda : m), *b = static_cast<const T*>(j.b) + (BKC ? n * j.ldb : n);
+  acc_t acc;   // [n rows, m lanes]
+  zero(acc);
+  int k = range * j.k_per_range + (shared ? 16 * wave : 0);
+  auto steps = [&](auto u_, auto last_) __attribute__((always_inline)) {
+    constexpr int N = decltype(u_)::value;
+    constexpr bool LAST = decltype(last_)::value;
+    PartsPiece<T, AKC> pa[N], pl[N];
+    PartsPiece<T, BKC> pb[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int at = k + step * u + 8 * g;
+      pa[u].template load<LAST>(a, j.lda, at, k_end);
+      pl[u].template load<LAST>(low, j.lda, at, k_end);
+      pb[u].template load<LAST>(b, j.ldb, at, k_end);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int at = k + step * u + 8 * g;
+      const frag<T> fb = pb[u].template get<LAST>(at, k_end);
+      mma(acc, fb, pl[u].template get<LAST>(at, k_end));
+      mma(acc, fb, pa[u].template get<LAST>(at, k_end));
+    }
+    k += step * N;
+  };
+  while (k + step * (U - 1) + 16 <= k_end) steps(std::integral_constant<int, U>(), std::false_type());
+  while (k < k_end) steps(std::integral_constant<int, 2>(), std::true_type());
+  settle();
+  auto store = [&](const vec<float, 4>& x, int q) __attribute__((always_inline)) {
+    const int64_t row = m0 + c, col = n0 + 8 * q + 4 * g, at = row * j.cm + col * j.cn;
+    if (row >= j.M || col >= j.N) return;   // (columns are multiples of 8)
+    auto to = [&](auto* out) __attribute__((always_inline)) {
+      using O = std::remove_reference_t<decltype(*out)>;
+      if (j.cn == 1) {
+        *reinterpret_cast<vec<O, 4>*>(out + at) = __builtin_convertvector(x, vec<O, 4>);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[at + e * j.cn] = (O)(float)x[e];
+      }
+    };
+    if (j.part != nullptr) to(j.part + (int64_t)range * j.M * j.N);
+    else to(static_cast<T*>(j.c));
+  };
+  if (!shared) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) store(pack4<float>(acc, q), q);
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) s_sum[(wave * 4 + q) * 64 + lane] = pack4<float>(acc, q);
+  __syncthreads();
+  vec<float, 4> x = s_sum[wave * 64 + lane];   // quad `wave` of all waves
+#pragma unroll
+  for (int w = 1; w < kPartsWaves; ++w) x += s_sum[(w * 4 + wave) * 64 + lane];
+  store(x, wave);
+}
+template <typename T> __global__ __launch_bounds__(64 * kPartsWaves) void parts_product_kernel(PartsArgs p) {
+  __shared__ vec<float, 4> s_sum[kPartsWaves * 4 * 64];
+  parts_tile<T, true, true>(p.job[0], blockIdx.x, s_sum);
+}
+// the first job: dx, the others: weight gradients
+template <typename T> __global__ __launch_bounds__(64 * kPartsWaves) void parts_grads_kernel(PartsArgs p) {
+  __shared__ vec<float, 4> s_sum[kPartsWaves * 4 * 64];
+  int group = blockIdx.x;
+  if (group < p.groups[0]) {
+    parts_tile<T, true, false>(p.job[0], group, s_sum);
+  } else {
+    group -= p.groups[0];
+    const bool last = group >= p.groups[1];
+    parts_tile<T, false, false>(p.job[last ? 2 : 1], last ? group - p.groups[1] : group, s_sum);
+  }
+}
+// ranges of a job, its workgroups; what its partial sums take
+int64_t parts_plan(PartsJob& j, int& groups) {
+  const int64_t tiles = (int64_t)((j.M + 31) / 32) * ((j.N + 31) / 32);
+  const int steps = (j.K + 15) / 16, most = (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, 128, steps / (4 * kPartsWaves)}));
+  if (!parts_shared(j.K)) {
+    j.k_per_range = 64;
+    j.ranges = 1;
+    groups = (int)((tiles + kPartsWaves - 1) / kPartsWaves);
+    return 0;
+  }
+  const int each = (steps + most - 1) / most;
+  j.k_per_range = 16 * each;
+  j.ranges = (steps + each - 1) / each;
+  groups = (int)(tiles * j.ranges);
+  return j.ranges > 1 ? ((int64_t)j.ranges * j.M * j.N * 4 + 255) / 256 * 256 : 0;
+}
+int64_t parts_bytes(int M, int N, int K) {
+  PartsJob j = {};
+  j.M = M;
+  j.N = N;
+  j.K = K;
+  int groups;
+  return parts_plan(j, groups);
+}
+template <typename Launch> int launch_parts(PartsArgs& p, int dtype, void* workspace, hipStream_t stream, Launch&& launch) {
+  char* at = static_cast<char*>(workspace);
+  PartSum sums[3];
+  int count = 0, groups = 0;
+  for (int i = 0; i < 3; ++i) {
+    PartsJob& j = p.job[i];
+    p.groups[i] = 0;
+    if (j.c == nullptr) continue;
+    const int64_t bytes = parts_plan(j, p.groups[i]);
+    groups += p.groups[i];
+    if (bytes == 0) continue;
+    j.part = reinterpret_cast<float*>(at);
+    at += bytes;
+    sums[count++] = {j.part, (int64_t)j.M * j.N, j.c, j.ranges, 0};
+  }
+  const int rc = by_type16(dtype, true, [&](auto t, auto) {
+    launch(t, groups);
+    return hipGetLastError() == hipSuccess ? 0 : -3;
+  });
+  return rc != 0 || count == 0 ? rc : launch_sums(sums, count, dtype, stream);
 }
 
 int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
@@ -560,7 +781,9 @@ bool both_weights(int R, int D, int F, int dtype, bool dx, WeightsPlan& p) {
 }
 
 bool few_rows(int R, int dtype) { return R <= kFewRows && dtype != 0; }
-int64_t hidden_bytes(int R, int F, int dtype) { return up((int64_t)R * F * elem_size(dtype)); }
+bool in_parts(int R, int D, int F, int dtype) { return dtype != 0 && few_numbers(R, D, F); }
+// of h; and, in parts, of what its rounding has left
+int64_t hidden_bytes(int R, int D, int F, int dtype) { return up((int64_t)R * F * elem_size(dtype) * (in_parts(R, D, F, dtype) ? 2 : 1)); }
 int64_t planes_bytes(int R, int D, int F) {
   const int rows = tile_rows(R, D, F);
   return (int64_t)((R + rows - 1) / rows) * ((F + kTileF - 1) / kTileF) * rows * kTileF * 6;
@@ -569,15 +792,19 @@ int64_t planes_bytes(int R, int D, int F) {
 }  // namespace
 
 // What the backward pass needs: fp32 u, [R][2 F]; else h, [R][F], and a and b
-int64_t gated_state(int R, int D, int F, int dtype) { return dtype == 0 ? 2 * hidden_bytes(R, F, 0) : hidden_bytes(R, F, dtype) + planes_bytes(R, D, F); }
+int64_t gated_state(int R, int D, int F, int dtype) { return dtype == 0 ? 2 * hidden_bytes(R, D, F, 0) : hidden_bytes(R, D, F, dtype) + planes_bytes(R, D, F); }
+// y is a product of all rows in a workgroup
+bool down_by_rows(int R, int D, int F, int dtype) { return few_rows(in_parts(R, D, F, dtype) ? 2 * R : R, dtype); }
 int64_t gated_workspace(int R, int D, int F, int dtype, bool keeps) {
-  const int64_t h = hidden_bytes(R, F, dtype), down = few_rows(R, dtype) ? rows_bytes(R, D, F) : product_workspace(R, D, F, dtype);
+  const bool parts = in_parts(R, D, F, dtype);
+  const int64_t h = hidden_bytes(R, D, F, dtype), down = down_by_rows(R, D, F, dtype) ? rows_bytes(R, D, F, parts) : parts ? parts_bytes(R, D, F) : product_workspace(R, D, F, dtype);
   if (dtype != 0) return std::max<int64_t>(256, (keeps ? 0 : h) + down);
   return h + (keeps ? 0 : 2 * h) + std::max(product_workspace(R, 2 * F, D, 0), down);
 }
 int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* workspace, hipStream_t stream) {
   char* at = static_cast<char*>(workspace);
-  const int64_t hidden = hidden_bytes(a.R, a.F, dtype);
+  const int64_t hidden = hidden_bytes(a.R, a.D, a.F, dtype);
+  const bool parts = in_parts(a.R, a.D, a.F, dtype), by_rows = down_by_rows(a.R, a.D, a.F, dtype);
   auto take = [&](int64_t bytes) { char* p = at; at += bytes; return p; };
   void* h;
   int rc;
@@ -585,9 +812,9 @@ int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* work
     h = state != nullptr ? state : take(hidden);
     const GatedProductArgs p = {a.x, a.w_in, a.ld_x, a.ld_in, a.R, a.F, a.D, h, state != nullptr ? static_cast<unsigned char*>(state) + hidden : nullptr};
     const int rows = tile_rows(a.R, a.D, a.F);
-    if (state != nullptr) rc = launch_product<kForwardKeep>(p, rows, a.act, dtype, stream);
-    else if (few_rows(a.R, dtype)) rc = launch_rows(a.x, a.ld_x, a.w_in, a.ld_in, h, a.R, a.F, a.D, a.act, dtype, nullptr, stream);
-    else rc = launch_product<kForward>(p, rows, a.act, dtype, stream);
+    if (state != nullptr) rc = launch_product<kForwardKeep>(p, rows, a.act, parts, dtype, stream);
+    else if (by_rows) rc = launch_rows(a.x, a.ld_x, a.w_in, a.ld_in, h, a.R, a.F, a.D, a.act, parts, dtype, nullptr, stream);
+    else rc = launch_product<kForward>(p, rows, a.act, parts, dtype, stream);
   } else {
     h = take(hidden);
     float* u = static_cast<float*>(state != nullptr ? state : take(2 * hidden));
@@ -600,23 +827,29 @@ int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* work
       });
   }
   if (rc != 0) return rc;
-  if (few_rows(a.R, dtype)) return launch_rows(h, a.F, a.w_out, a.ld_out, y, a.R, a.D, a.F, kNoGate, dtype, at, stream);
+  if (by_rows) return launch_rows(h, a.F, a.w_out, a.ld_out, y, a.R, a.D, a.F, kNoGate, parts, dtype, at, stream);
+  if (parts) {
+    PartsArgs p = {};
+    p.job[0] = {h, static_cast<const uint16_t*>(h) + (int64_t)a.R * a.F, a.w_out, a.F, a.ld_out, a.D, 1, a.R, a.D, a.F, 0, 0, y, nullptr};
+    return launch_parts(p, dtype, at, stream, [&](auto t, int groups) { hipLaunchKernelGGL((parts_product_kernel<decltype(t)>), dim3(groups), dim3(64 * kPartsWaves), 0, stream, p); });
+  }
   return product({h, a.F, true}, {a.w_out, a.ld_out, true}, y, a.R, a.D, a.F, dtype, at, stream);
 }
 
 int64_t gated_bwd_workspace(int R, int D, int F, int dtype, int gradients) {
   const bool dx = gradients & 1, dw_in = gradients & 2, dw_out = gradients & 4, below = dx || dw_in;
-  const int64_t hidden = hidden_bytes(R, F, dtype);
+  const int64_t hidden = hidden_bytes(R, D, F, dtype);
   int64_t products = grads_bytes(R, 2 * F, D, dtype, dw_in, dx, dw_out ? D : 0, F);
   WeightsPlan p;
   if (dw_in && dw_out && both_weights(R, D, F, dtype, dx, p)) products = std::max(up(weights_workspace(p)), dx ? product_workspace(R, D, 2 * F, dtype) : 0);
+  if (in_parts(R, D, F, dtype)) products = (dx ? parts_bytes(R, D, 2 * F) : 0) + (dw_in ? parts_bytes(2 * F, D, R) : 0) + (dw_out ? parts_bytes(F, D, R) : 0);
   if (dtype != 0) return std::max<int64_t>(256, (below ? 2 * hidden : 0) + products);
   return (dw_out ? hidden : 0) + (below ? 3 * hidden + std::max(products, product_workspace(R, F, D, 0)) : products);
 }
 int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void* dx, void* dw_in, void* dw_out, int dtype, void* workspace, hipStream_t stream) {
   char* at = static_cast<char*>(workspace);
-  const int64_t hidden = hidden_bytes(a.R, a.F, dtype), n = (int64_t)a.R * a.F;
-  const bool below = dx != nullptr || dw_in != nullptr;
+  const int64_t hidden = hidden_bytes(a.R, a.D, a.F, dtype), n = (int64_t)a.R * a.F;
+  const bool below = dx != nullptr || dw_in != nullptr, parts = in_parts(a.R, a.D, a.F, dtype);
   auto take = [&](int64_t bytes) { char* p = at; at += bytes; return p; };
   const void* h = state;
   void* du = nullptr;
@@ -625,7 +858,7 @@ int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void
     if (below) {
       du = take(2 * hidden);
       const GatedProductArgs p = {dy, a.w_out, a.D, a.ld_out, a.R, a.F, a.D, du, const_cast<unsigned char*>(static_cast<const unsigned char*>(state)) + hidden};
-      rc = launch_product<kBackward>(p, tile_rows(a.R, a.D, a.F), a.act, dtype, stream);
+      rc = launch_product<kBackward>(p, tile_rows(a.R, a.D, a.F), a.act, parts, dtype, stream);
     }
   } else {
     float* h32 = dw_out != nullptr ? reinterpret_cast<float*>(take(hidden)) : nullptr;
@@ -642,6 +875,16 @@ int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void
                            static_cast<float*>(du), h32);
         return hipGetLastError() == hipSuccess ? 0 : -3;
       });
+  }
+  if (parts) {
+    if (rc != 0) return rc;
+    const uint16_t *d = static_cast<const uint16_t*>(du), *hh = static_cast<const uint16_t*>(h);
+    const int64_t n2 = 2 * n;
+    PartsArgs p = {};
+    if (dx != nullptr) p.job[0] = {d, d + n2, a.w_in, 2 * (int64_t)a.F, a.ld_in, a.D, 1, a.R, a.D, 2 * a.F, 0, 0, dx, nullptr};
+    if (dw_in != nullptr) p.job[1] = {d, d + n2, a.x, 2 * (int64_t)a.F, a.ld_x, a.D, 1, 2 * a.F, a.D, a.R, 0, 0, dw_in, nullptr};
+    if (dw_out != nullptr) p.job[2] = {hh, hh + n, dy, a.F, a.D, 1, a.F, a.F, a.D, a.R, 0, 0, dw_out, nullptr};
+    return launch_parts(p, dtype, at, stream, [&](auto t, int groups) { hipLaunchKernelGGL((parts_grads_kernel<decltype(t)>), dim3(groups), dim3(64 * kPartsWaves), 0, stream, p); });
   }
   WeightsPlan plan;
   if (rc == 0 && dw_in != nullptr && dw_out != nullptr && both_weights(a.R, a.D, a.F, dtype, dx != nullptr, plan)) {

@@ -424,7 +424,8 @@ def gated_feed_forward(x: torch.Tensor, weight_in: torch.Tensor, weight_out: tor
     """(act(x G^T) * (x U^T)) weight_out^T: the feed-forward block with a gate, x (..., D), weight_in (2 F, D) the rows of G above those of U, weight_out (D, F);
     the counterpart of nn.Linear, nn.GELU, nn.Linear in train_triton.py:102-107.  activation: "silu" or "gelu" (erf form).
 
-    Sums in 32 bits; in 16-bit types the hidden rows act(..) * (..) are rounded once on their way to the second product, and so are their gradients.  Differentiable
+    Sums in 32 bits; in 16-bit types the hidden rows act(..) * (..) are rounded once on their way to the second product, and so are their gradients (not where rows x D, rows x F or D x F is below 4096:
+    there only results are rounded).  Differentiable
     in all three, once: it keeps what the backward pass needs of the hidden rows (about 6 bytes an element in 16-bit types).  D and F are multiples of 8, any number of rows of
     which (rows + 192) 2 F is below 2^31."""
     if N._host is None:
