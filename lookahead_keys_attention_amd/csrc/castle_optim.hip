@@ -289,7 +289,8 @@ template <typename T, bool SMALL, bool CHANCE> __global__ __launch_bounds__(kThr
       const float g = x[e] * s.clip;
       m[e] = b1 * m[e] + c1 * g;
       v[e] = b2 * v[e] + c2 * (g * g);
-      r[e] = fast_sqrt(v[e]);
+      // (correctly rounded beside parameters of 32 bits: a root that is one unit off is rounded to another state in one of 6 million cases, and those show where parameters keep their 24 bits)
+      r[e] = SMALL && sizeof(T) == 4 ? sqrtf(v[e]) : fast_sqrt(v[e]);
       q[e] = p[e] * s.keep - s.rate * m[e] * fast_rcp(r[e] * s.root + eps);
     }
     const uint64_t counter = 4 * (uint64_t)(at >> 3);
