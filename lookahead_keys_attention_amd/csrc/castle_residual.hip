@@ -10,6 +10,7 @@
 //
 // Bound by HBM: forward reads two tensors and writes two, backward reads four and writes two (the residual is read again rather than y: y is needed in 32 bits).  A row belongs to 16, 32 or
 // 64 lanes, of more than 1024 elements to four or eight waves; a lane owns 8 columns of each piece of a row, so column sums stay in its registers over all its rows.
+// us and TB/s: 65536 x 2048 with a gate of each sequence forward 213 and 5.0, backward 334 and 4.8, the join of the workgroups' column sums 9; 16384 x 512 14.6, 23.7 and 4.9 (4.6 and 4.2 TB/s).
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
 #include "castle_residual.h"
@@ -27,7 +28,7 @@ constexpr int kGateRows = 8;          // rows of a unit under a gate that severa
 // LPR lanes of WPR waves have a row, NP pieces of 8 elements a lane
 template <int LPR_, int WPR_, int NP_> struct Layout {
   static constexpr int LPR = LPR_, WPR = WPR_, NP = NP_, kBlock = WPR == 1 ? kThreads : 64 * WPR, kRows = kBlock / (LPR * WPR);
-  // workgroups that a CU holds of the backward pass, and waves of a SIMD: all of a launch run at once, each over several rows (1024 workgroups of which 768 ran at once: 396 us, see below)
+  // workgroups that a CU holds of the backward pass, and waves of a SIMD: all of a launch run at once, each over several rows (65536 x 2048 with a gate of each sequence: 1024 workgroups of which 768 ran at once 396 us, 764 of them 334)
   static constexpr int kHeld = WPR == 8 ? 1 : NP == 1 ? 3 : 2, kWavesPerSimd = WPR == 8 ? 2 : kHeld;
 };
 // workgroups for n turns, `most` at once, with as many turns each as they can have alike
