@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -222,6 +223,26 @@ bool wants_graph(std::initializer_list<Tensor> ts) {
     graph = graph || t.requires_grad();
   }
   return graph && at::GradMode::is_enabled();
+}
+
+// In a backward pass that is recorded into a graph: what the gradients go to next has to belong to the graph too.  Nodes that an earlier pass has left alive (a loss that is kept keeps those of its
+// leaves) belong to that pass's stream; autograd would make it wait for the one that records, which nothing ends, and the process ends with the recording.
+void refuse_nodes_outside(const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.is_valid()) continue;
+    const auto stream = edge.function->stream();
+    if (!stream || stream == node->stream()) continue;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;   // (the default stream is never recorded, and may not be asked)
+    if (stream->id() != 0) {
+      const c10::hip::HIPStreamMasqueradingAsCUDA other(c10::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *stream);
+      if (hipStreamIsCapturing(other.hip_stream().stream(), &status) != hipSuccess) status = hipStreamCaptureStatusNone;
+    }
+    TORCH_CHECK(status == hipStreamCaptureStatusActive, what, ": a graph records this backward pass, but an earlier pass over the same tensors is still alive outside of it (a loss or an output that is kept): "
+                "drop it before the recording begins");
+  }
 }
 
 // The gradients have no derivatives of their own.  Where a graph of the backward pass is recorded (create_graph) they hang on a
@@ -1393,6 +1414,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     static const auto op = op_handle<decltype(gated_bwd_op)>("castle_hip::gated_feed_forward_bwd");
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    refuse_nodes_outside("gated_feed_forward");
     const auto s = ctx->get_saved_variables();
     const bool need_x = ctx->needs_input_grad(0), need_in = ctx->needs_input_grad(1), need_out = ctx->needs_input_grad(2);
     auto [dx, din, dout] = op.call(g[0], s[0], s[1], s[2], s[3], ctx->saved_data["activation"].toInt(), need_x, need_in, need_out);
@@ -1533,6 +1555,7 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
     static const auto op = op_handle<decltype(residual_norm_bwd_op)>("castle_hip::residual_norm_bwd");
     variable_list grads(7);
     if (!g[0].defined() && !g[1].defined()) return grads;
+    refuse_nodes_outside("residual_norm");
     const auto s = ctx->get_saved_variables();
     auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     int64_t need = 0;

@@ -295,6 +295,61 @@ def test_the_same_bits_every_time_on_any_stream_and_in_a_graph():
 
 
 @gpu
+@pytest.mark.parametrize("R, D, F", [(3000, 768, 2048), (300, 64, 136), (6, 40, 1024)])
+def test_two_streams_at_once_and_a_graph(R, D, F):
+    """Weight gradients in whole tiles and ranges, in the launch of all three, in two parts: calls of two streams side by side, and replays among eager calls."""
+    sets = [[t.to(DEV) for t in inputs(R, D, F, torch.bfloat16, seed=k)] for k in range(2)]
+    want = [{k: v.detach() for k, v in run(*t, "gelu").items()} for t in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for t, stream, g in zip(sets, streams, got):
+            with torch.cuda.stream(stream):
+                g.append({k: v.detach() for k, v in run(*t, "gelu").items()})   # (no pass is kept alive: see below)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(r[k], w[k]) for r in g for k in w)
+    x, win, wout, dy = [t.detach().clone() for t in sets[0]]
+    leaves = [t.requires_grad_() for t in (x, win, wout)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.gated_feed_forward(*leaves, activation="gelu")
+        grads = torch.autograd.grad(y, leaves, dy)
+    for k in (1, 0, 1):
+        with torch.no_grad():
+            for t, new in zip((x, win, wout, dy), sets[k]):
+                t.copy_(new)
+        graph.replay()
+        other = run(*sets[1 - k], "gelu")
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, want[k][name]) for a, name in zip((y, *grads), ("y", "dx", "dwin", "dwout")))
+        assert all(torch.equal(other[name], want[1 - k][name]) for name in other)
+
+
+@gpu
+@pytest.mark.parametrize("leaves_of_its_own", [True, False])
+def test_a_recorded_backward_pass_beside_one_that_lives_is_refused(leaves_of_its_own):
+    x, win, wout, dy = (t.to(DEV) for t in inputs(64, 64, 128, torch.bfloat16))
+    leaves = [t.requires_grad_() for t in (x, win, wout)]
+    kept = ops.gated_feed_forward(*leaves)
+    inside = leaves if leaves_of_its_own else [t.clone() for t in leaves]   # (or what an earlier pass would reach)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(ops.gated_feed_forward(*inside), inside, dy)
+    torch.cuda.synchronize()
+    want = [t.clone() for t in torch.autograd.grad(kept, leaves, dy)]
+    del kept, inside
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = torch.autograd.grad(ops.gated_feed_forward(*leaves), leaves, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+@gpu
 def test_refusals_on_the_gpu():
     x, win, wout, dy = (t.to(DEV) for t in inputs(4, 64, 72, torch.bfloat16))
     with pytest.raises(ValueError):

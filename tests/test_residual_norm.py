@@ -264,3 +264,22 @@ def test_refusals_on_the_gpu():
     dw, = torch.autograd.grad(call(g | dict(weight=w))[0], w, dy.to(DEV), create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate twice"):
         dw.sum().backward()
+
+
+@gpu
+def test_a_recorded_backward_pass_beside_one_that_lives_is_refused():
+    x, r, w = (torch.randn(4, 64, device=DEV, requires_grad=True), torch.randn(4, 64, device=DEV, requires_grad=True), torch.ones(64, device=DEV, requires_grad=True))
+    kept = ops.residual_norm(x, r, weight=w, next_weight=w)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(ops.residual_norm(x, r, weight=w, next_weight=w)[1].sum(), (x, r, w))
+    torch.cuda.synchronize()
+    want = [t.clone() for t in torch.autograd.grad(kept[1].sum(), (x, r, w))]
+    del kept
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = torch.autograd.grad(ops.residual_norm(x, r, weight=w, next_weight=w)[1].sum(), (x, r, w))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
