@@ -2,8 +2,7 @@
 //   dh = dy w_out     dg = dh v act'(g)     dv = dh act(g)     dx = [dg dv] w_in     dw_in = [dg dv]^T x     dw_out = dy^T h
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
-#include "castle_gated.h"
-#include "castle_gelu.h"
+#include "castle_gate.h"
 #include "castle_gemm.h"
 #include "castle_rows.h"
 #include "castle_weights.h"
@@ -15,23 +14,7 @@ namespace {
 
 typedef vec<float, 8> vf;
 
-// act(g) and its derivative
-template <typename T, int ACT> struct Gate {
-  float act, slope;
-  __device__ __forceinline__ explicit Gate(float g) {
-    if constexpr (ACT == kSilu) {
-      const float s = sizeof(T) == 4 ? 1.f / (1.f + expf(-g)) : sigmoid_l2(g * kLog2e);
-      act = g * s;
-      slope = __builtin_fmaf(act, 1.f - s, s);
-    } else {
-      const Normal<T> n(g);
-      act = g * n.cdf;
-      slope = __builtin_fmaf(g * 0.3989422804f, n.e, n.cdf);
-    }
-  }
-};
-
-// ---- fp32: u in memory ----------------------------------------------------------------------------------------------
+// ---- fp32: u in memory, the gate on the store of its product (castle_gemm32.hip) or, where that goes in ranges, by itself -------
 __device__ __forceinline__ vf load8(const float* p) { return *reinterpret_cast<const frag_mem<float>*>(p); }
 __device__ __forceinline__ void store8(float* p, vf v) { *reinterpret_cast<frag_mem<float>*>(p) = v; }
 // h of u = [R][2 F]
@@ -731,8 +714,11 @@ struct Operand2 {
   bool kc;   // contraction-contiguous
 };
 int64_t product_workspace(int M, int N, int K, int dtype) { return up(gemm_workspace(M, N, K, elem_size(dtype), false)); }
+GemmArgs product_args(const Operand2& a, const Operand2& b, void* c, int M, int N, int K) {
+  return {a.p, b.p, c, nullptr, M, N, K, a.ld, b.ld, N, kGemmPlain, 0, nullptr, nullptr, nullptr, 0, 1, nullptr, 0.f, nullptr, nullptr};
+}
 int product(const Operand2& a, const Operand2& b, void* c, int M, int N, int K, int dtype, void* workspace, hipStream_t stream) {
-  const GemmArgs g = {a.p, b.p, c, nullptr, M, N, K, a.ld, b.ld, N, kGemmPlain, 0, nullptr, nullptr, nullptr, 0, 1, nullptr, 0.f, nullptr, nullptr};
+  const GemmArgs g = product_args(a, b, c, M, N, K);
   return launch_gemm(g, a.kc, b.kc, dtype, static_cast<float*>(workspace), stream);
 }
 // Gradients of a projection y = x w^T, dy [R][N], x [R][K], and `more`, the weight gradient of another one of as many rows: of what is asked for (c not nullptr) as much in one launch as is ahead so
@@ -748,16 +734,13 @@ int64_t grads_bytes(int R, int N, int K, int dtype, bool dw, bool dx, int more_m
   return third >= 0 ? up(both + third) : std::max(up(both), more);
 }
 int grads(const Operand2& dy, const Operand2& x, const Operand2& w, void* dw, void* dx, int R, int N, int K, const More& more, int dtype, void* workspace, hipStream_t stream) {
-  const auto args = [](const Operand2& a, const Operand2& b, void* c, int M, int N, int K) {
-    return GemmArgs{a.p, b.p, c, nullptr, M, N, K, a.ld, b.ld, N, kGemmPlain, 0, nullptr, nullptr, nullptr, 0, 1, nullptr, 0.f, nullptr, nullptr};
-  };
   if (dw != nullptr && dx != nullptr && grads_workspace(R, N, K, elem_size(dtype), kGemmPlain, false) >= 0) {
     MoreGradsArgs p = {};
-    p.w = args(dy, x, dw, N, K, R);
-    p.x = args(dy, w, dx, R, K, N);
+    p.w = product_args(dy, x, dw, N, K, R);
+    p.x = product_args(dy, w, dx, R, K, N);
     if (more.c == nullptr) return launch_grads(p, dtype, static_cast<float*>(workspace), nullptr, stream);
     if (grads_more(R, N, K, elem_size(dtype), more.M, more.N) >= 0) {
-      p.v = args(more.a, more.b, more.c, more.M, more.N, R);
+      p.v = product_args(more.a, more.b, more.c, more.M, more.N, R);
       return launch_more_grads(p, dtype, static_cast<float*>(workspace), stream);
     }
     const int rc = product(more.a, more.b, more.c, more.M, more.N, R, dtype, workspace, stream);
@@ -799,6 +782,7 @@ int64_t gated_workspace(int R, int D, int F, int dtype, bool keeps) {
   const bool parts = in_parts(R, D, F, dtype);
   const int64_t h = hidden_bytes(R, D, F, dtype), down = down_by_rows(R, D, F, dtype) ? rows_bytes(R, D, F, parts) : parts ? parts_bytes(R, D, F) : product_workspace(R, D, F, dtype);
   if (dtype != 0) return std::max<int64_t>(256, (keeps ? 0 : h) + down);
+  if (gate_on_store(R, 2 * F, D)) return h + down;
   return h + (keeps ? 0 : 2 * h) + std::max(product_workspace(R, 2 * F, D, 0), down);
 }
 int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* workspace, hipStream_t stream) {
@@ -817,14 +801,21 @@ int launch_gated(const GatedArgs& a, void* y, void* state, int dtype, void* work
     else rc = launch_product<kForward>(p, rows, a.act, parts, dtype, stream);
   } else {
     h = take(hidden);
-    float* u = static_cast<float*>(state != nullptr ? state : take(2 * hidden));
     const int64_t n = (int64_t)a.R * a.F;
-    rc = product({a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, u, a.R, 2 * a.F, a.D, dtype, at, stream);
-    if (rc == 0)
-      rc = by_act(a.act, [&](auto act) {
-        hipLaunchKernelGGL((gate_kernel<decltype(act)::value>), many_blocks((n / 8 + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, u, n, a.F, static_cast<float*>(h));
-        return hipGetLastError() == hipSuccess ? 0 : -3;
-      });
+    const bool fused = gate_on_store(a.R, 2 * a.F, a.D);
+    float* u = static_cast<float*>(state != nullptr ? state : fused ? nullptr : take(2 * hidden));
+    if (fused) {
+      GemmArgs g = product_args({a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, u, a.R, 2 * a.F, a.D);
+      g.h = h;
+      rc = launch_gemm_gate(g, kGateForward, a.act, stream);
+    } else {
+      rc = product({a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, u, a.R, 2 * a.F, a.D, dtype, at, stream);
+      if (rc == 0)
+        rc = by_act(a.act, [&](auto act) {
+          hipLaunchKernelGGL((gate_kernel<decltype(act)::value>), many_blocks((n / 8 + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, u, n, a.F, static_cast<float*>(h));
+          return hipGetLastError() == hipSuccess ? 0 : -3;
+        });
+    }
   }
   if (rc != 0) return rc;
   if (by_rows) return launch_rows(h, a.F, a.w_out, a.ld_out, y, a.R, a.D, a.F, kNoGate, parts, dtype, at, stream);
@@ -844,7 +835,9 @@ int64_t gated_bwd_workspace(int R, int D, int F, int dtype, int gradients) {
   if (dw_in && dw_out && both_weights(R, D, F, dtype, dx, p)) products = std::max(up(weights_workspace(p)), dx ? product_workspace(R, D, 2 * F, dtype) : 0);
   if (in_parts(R, D, F, dtype)) products = (dx ? parts_bytes(R, D, 2 * F) : 0) + (dw_in ? parts_bytes(2 * F, D, R) : 0) + (dw_out ? parts_bytes(F, D, R) : 0);
   if (dtype != 0) return std::max<int64_t>(256, (below ? 2 * hidden : 0) + products);
-  return (dw_out ? hidden : 0) + (below ? 3 * hidden + std::max(products, product_workspace(R, F, D, 0)) : products);
+  const int64_t h = dw_out ? hidden : 0;
+  if (!below) return std::max<int64_t>(256, h + products);
+  return gate_on_store(R, F, D) ? h + 2 * hidden + products : h + 3 * hidden + std::max(products, product_workspace(R, F, D, 0));
 }
 int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void* dx, void* dw_in, void* dw_out, int dtype, void* workspace, hipStream_t stream) {
   char* at = static_cast<char*>(workspace);
@@ -864,12 +857,20 @@ int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void
     float* h32 = dw_out != nullptr ? reinterpret_cast<float*>(take(hidden)) : nullptr;
     const float* dh = nullptr;
     h = h32;
-    if (below) {
+    const bool fused = below && gate_on_store(a.R, a.F, a.D);
+    if (fused) {
+      du = take(2 * hidden);
+      GemmArgs g = product_args({dy, a.D, true}, {a.w_out, a.ld_out, false}, du, a.R, a.F, a.D);
+      g.aux = const_cast<void*>(state);
+      g.ldc = 2 * a.F;
+      g.h = h32;
+      rc = launch_gemm_gate(g, kGateBackward, a.act, stream);
+    } else if (below) {
       dh = reinterpret_cast<const float*>(take(hidden));
       du = take(2 * hidden);
       rc = product({dy, a.D, true}, {a.w_out, a.ld_out, false}, const_cast<float*>(dh), a.R, a.F, a.D, dtype, at, stream);
     }
-    if (rc == 0)
+    if (rc == 0 && !fused)
       rc = by_act(a.act, [&](auto act) {
         hipLaunchKernelGGL((gate_bwd_kernel<decltype(act)::value>), many_blocks((n / 8 + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, static_cast<const float*>(state), dh, n, a.F,
                            static_cast<float*>(du), h32);

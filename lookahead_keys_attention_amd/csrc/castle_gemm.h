@@ -5,6 +5,7 @@
 
 namespace castle {
 
+enum { kGateNone = 0, kGateForward = 1, kGateBackward = 2 };
 enum { kGemmPlain = 0, kGemmGelu = 1, kGemmGeluSlope = 2 };
 struct GemmArgs {
   const void *a, *b;   // contraction-contiguous: [free][ld], else [contraction][ld]
@@ -42,6 +43,10 @@ bool gemm_norm_ok(int M, int N, int K, int elem_size);
 bool gemm_amax_ok(int M, int N, int K, int elem_size, int amax_from, int amax_to);
 void gemm_plan(int M, int N, int K, int elem_size, bool epilogue, int (&out)[4]);
 float gemm_cost(int M, int N, int K, int elem_size);   // what a plain product takes, us
+// fp32 products with the gate of a gated feed-forward block on their store (gate32_kernel), and whether that is ahead of a launch for it
+bool gate_on_store(int M, int N, int K);
+int launch_gemm_gate(GemmArgs a, int gate, int act, hipStream_t stream);
+int launch_gate32(const GemmArgs& a, int gate, int act, int tile, int waves, hipStream_t stream);
 int64_t gemm_workspace(int M, int N, int K, int elem_size, bool epilogue);
 // fp32, castle_gemm32.hip
 int launch_gemm32(const GemmArgs& a, bool a_kc, bool b_kc, int tile, int splits, int waves, hipStream_t stream);

@@ -20,6 +20,7 @@
 // weight gradient of 20 rows 0.82 / 0.65, of 16384 16 / 7.6.
 #include "castle_tiles.h"
 #include "castle_gemm.h"
+#include "castle_gate.h"
 #include "castle_gelu.h"
 #include "castle_waves.h"
 #include <type_traits>
@@ -129,16 +130,41 @@ template <bool KC, int F> struct Operand32 {   // F: 32 or 64
   }
 };
 
+// Contraction-contiguous, the first half of the rows from one place and the second from another, `apart` elements further on.
+template <int F> struct PairOperand32 : Operand32<true, F> {
+  typedef Operand32<true, F> Base;
+  static constexpr int N = Base::kLoads;
+  const float* second;
+  __device__ __forceinline__ uint32_t place(int ld, int q, int steps) const {
+    const int lane = lane_id(), row = 8 * q + (lane >> 3), piece = (lane & 7) ^ (row >> 1 & 7);
+    return 4 * (uint32_t)(min(row % (F / 2), Base::last) * ld + (4 * piece < steps ? 4 * piece : 0));
+  }
+  __device__ __forceinline__ void start(const float* p, int64_t ld, int free0, int free_end, int64_t apart) {
+    Base::base = p + free0 * ld;
+    second = Base::base + apart;
+    Base::last = free_end - 1 - free0;
+#pragma unroll
+    for (int q = 0; q < N; ++q) Base::at[q] = place((int)ld, q, kStep);
+  }
+  __device__ __forceinline__ void load(int64_t ld, int k, int k_end, uint32_t lds) const {
+    const bool whole = k + kStep <= k_end;
+#pragma unroll
+    for (int q = 0; q < N; ++q) load_to_lds((q < N / 2 ? Base::base : second) + k, whole ? Base::at[q] : place((int)ld, q, k_end - k), lds + 1024 * q);
+  }
+};
+
 // sums of a wave in LDS: pieces of 16 bytes from one quad of accumulator registers to the next, such that the readers' pieces of a row meet all banks
 constexpr int kUnit32 = 66;
 constexpr uint32_t kLeastBits = (127u - 90) << 23;   // 2^-90
 template <int TILE> constexpr int wave_bytes() { return max2(TILE * TILE / 256 * kUnit32 * 16, 2 * TILE * kStep * 4); }
 // NORM: the rows of `a` are normalised on their way to the registers.
-template <bool AK, bool BKC, int TILE, int W, bool NORM>
+// GATE, ACT: a gated feed-forward block.  kGateForward: b has the rows of both halves, a.N of them, and a tile half its columns from each; the sums u go to c, if it is there, and act(g) v to h.
+// kGateBackward: the sums are dh, aux is u; [dg dv] goes to c and act(g) v to h, if it is there.
+template <bool AK, bool BKC, int TILE, int W, bool NORM, int GATE = kGateNone, int ACT = 0>
 __device__ __forceinline__ void gemm32_tile(const GemmArgs& a, vec<float, 4>* s_sum, int bx, int by) {   // s_sum: of a wave, operands, then sums
   constexpr int V = 4, NT = 64 * W, BM = TILE, BN = TILE, F = TILE / 32, U = 4 * F * F;   // U: quads of accumulator registers
   typedef Operand32<AK, TILE> OpA;
-  typedef Operand32<BKC, TILE> OpB;
+  typedef std::conditional_t<GATE == kGateForward, PairOperand32<TILE>, Operand32<BKC, TILE>> OpB;
   typedef vec<float, 4> v4;
   constexpr int kWave = wave_bytes<TILE>() / 16;
   const int lane = lane_id(), wave = wave_id(), c = lane & 31, g = lane >> 5;
@@ -156,7 +182,8 @@ __device__ __forceinline__ void gemm32_tile(const GemmArgs& a, vec<float, 4>* s_
   OpA oa;
   OpB ob;
   oa.start(static_cast<const float*>(a.a), a.lda, m0, a.M);
-  ob.start(static_cast<const float*>(a.b), a.ldb, n0, a.N);
+  if constexpr (GATE == kGateForward) ob.start(static_cast<const float*>(a.b), a.ldb, n0 / 2, a.N / 2, a.N / 2 * a.ldb);
+  else ob.start(static_cast<const float*>(a.b), a.ldb, n0, a.N);
   const float* const mine = reinterpret_cast<const float*>(s_sum + wave * kWave);
   const uint32_t lds = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) float*)mine;
   auto fetch = [&](int stage) __attribute__((always_inline)) {
@@ -310,13 +337,54 @@ __device__ __forceinline__ void gemm32_tile(const GemmArgs& a, vec<float, 4>* s_
         for (int q = 0; q < 4; ++q) s_sum[wave * kWave + (4 * (F * i + j) + q) * kUnit32 + 33 * g + c] = pack4<float>(acc[i][j], q);
   }
   __syncthreads();
+  auto sum_at = [&](int row, int p) __attribute__((always_inline)) {
+    const v4* part = s_sum + (row / 32 * (4 * F) + p / 2) * kUnit32 + 33 * (p % 2) + row % 32;
+    v4 x = part[0];
+    for (int w = 1; w < with; ++w) x += part[w * kWave];
+    return x;
+  };
+  if constexpr (GATE != kGateNone) {
+    constexpr int Q = GATE == kGateForward ? BN / 8 : BN / 4;   // quads of hidden columns of a row
+    const int hidden = GATE == kGateForward ? a.N / 2 : a.N, first = GATE == kGateForward ? n0 / 2 : n0;
+#pragma unroll
+    for (int u = threadIdx.x; u < BM * Q; u += NT) {
+      const int row = u / Q, p = u % Q, m = m0 + row, n = first + 4 * p;
+      if (m >= a.M || n >= hidden) continue;
+      const int64_t at = (int64_t)m * a.ldc + n;
+      const v4 s = sum_at(row, p);
+      v4 g, v, y;
+      if constexpr (GATE == kGateForward) {
+        g = s;
+        v = sum_at(row, p + Q);
+        if (a.c != nullptr) {
+          *reinterpret_cast<v4*>(static_cast<float*>(a.c) + at) = g;
+          *reinterpret_cast<v4*>(static_cast<float*>(a.c) + at + hidden) = v;
+        }
+      } else {
+        g = *reinterpret_cast<const v4*>(static_cast<const float*>(a.aux) + at);
+        v = *reinterpret_cast<const v4*>(static_cast<const float*>(a.aux) + at + hidden);
+      }
+      v4 dg, dv;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const Gate<float, ACT> gate(g[e]);
+        y[e] = gate.act * v[e];
+        dg[e] = s[e] * (v[e] * gate.slope);
+        dv[e] = s[e] * gate.act;
+      }
+      if constexpr (GATE == kGateBackward) {
+        *reinterpret_cast<v4*>(static_cast<float*>(a.c) + at) = dg;
+        *reinterpret_cast<v4*>(static_cast<float*>(a.c) + at + hidden) = dv;
+      }
+      if (a.h != nullptr) *reinterpret_cast<v4*>(static_cast<float*>(a.h) + (int64_t)m * hidden + n) = y;
+    }
+    return;
+  }
 #pragma unroll
   for (int u = threadIdx.x; u < BM * BN / 4; u += NT) {
     const int row = u / (BN / 4), p = u % (BN / 4), m = m0 + row, n = n0 + 4 * p;
     if (m >= a.M || n >= a.N) continue;
-    const v4* part = s_sum + (row / 32 * (4 * F) + p / 2) * kUnit32 + 33 * (p % 2) + row % 32;
-    v4 x = part[0];
-    for (int w = 1; w < with; ++w) x += part[w * kWave];
+    v4 x = sum_at(row, p);
     if (a.part != nullptr) {   // partial product of this range of the contraction
       *reinterpret_cast<v4*>(a.part + (int64_t)by * a.M * a.N + (int64_t)m * a.N + n) = x;
       continue;
@@ -356,6 +424,12 @@ template <bool AK, bool BKC, int TILE, int W, bool NORM>
 __global__ __launch_bounds__(64 * W, W / 4 < 2 ? 2 : W / 4) void gemm32_kernel(GemmArgs a) {
   __shared__ __attribute__((aligned(16))) vec<float, 4> s_sum[W * wave_bytes<TILE>() / 16];
   gemm32_tile<AK, BKC, TILE, W, NORM>(a, s_sum, blockIdx.x, blockIdx.y);
+}
+// (kernels of their own: neither the arguments nor the code of the others grows)
+template <int TILE, int W, int GATE, int ACT>
+__global__ __launch_bounds__(64 * W, W / 4 < 2 ? 2 : W / 4) void gate32_kernel(GemmArgs a) {
+  __shared__ __attribute__((aligned(16))) vec<float, 4> s_sum[W * wave_bytes<TILE>() / 16];
+  gemm32_tile<true, GATE == kGateForward, TILE, W, false, GATE, ACT>(a, s_sum, blockIdx.x, 0);
 }
 // both gradients of a projection: workgroups of the weight gradient, then those of the input gradient (castle_gemm.hip; 256 rows 512 -> 3072, us: 12.9 and 16.1, both
 // 24.6, 512 -> 512 5.6 and 6.5, both 8.4)
@@ -405,6 +479,21 @@ int launch_gemm32(const GemmArgs& a, bool a_kc, bool b_kc, int tile, int splits,
   if (a.norm_w != nullptr) return go(yes, yes, yes);
   if (a_kc) return b_kc ? go(yes, yes, no) : go(yes, no, no);
   return b_kc ? -2 : go(no, no, no);
+}
+
+int launch_gate32(const GemmArgs& a, int gate, int act, int tile, int waves, hipStream_t stream) {
+  const dim3 grid((((a.M + tile - 1) / tile) * ((a.N + tile - 1) / tile) + 7) / 8 * 8);
+  auto go = [&](auto gate_, auto act_) {
+    constexpr int GATE = decltype(gate_)::value, ACT = decltype(act_)::value;
+    if (tile == 32 && waves == 8) hipLaunchKernelGGL((gate32_kernel<32, 8, GATE, ACT>), grid, dim3(512), 0, stream, a);
+    else if (tile == 32) hipLaunchKernelGGL((gate32_kernel<32, 4, GATE, ACT>), grid, dim3(256), 0, stream, a);
+    else if (waves == 4) hipLaunchKernelGGL((gate32_kernel<64, 4, GATE, ACT>), grid, dim3(256), 0, stream, a);
+    else if (waves == 2) hipLaunchKernelGGL((gate32_kernel<64, 2, GATE, ACT>), grid, dim3(128), 0, stream, a);
+    else hipLaunchKernelGGL((gate32_kernel<64, 1, GATE, ACT>), grid, dim3(64), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? 0 : -3;
+  };
+  auto of_act = [&](auto gate_) { return act == kSilu ? go(gate_, std::integral_constant<int, kSilu>()) : go(gate_, std::integral_constant<int, kGeluGate>()); };
+  return gate == kGateForward ? of_act(std::integral_constant<int, kGateForward>()) : of_act(std::integral_constant<int, kGateBackward>());
 }
 
 int launch_grads32(const GradsArgs& p, int tile, int waves, hipStream_t stream) { return launch_grads32_as(p, p.w_groups + p.x_groups, tile, waves, stream); }

@@ -160,7 +160,7 @@ def test_weight_gradients_of_one_launch(R, D, F, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("R, D, F", [(2048, 64, 64), (3000, 64, 128), (4096, 128, 320), (777, 768, 2048), (128, 768, 768)])
+@pytest.mark.parametrize("R, D, F", [(2048, 64, 64), (3000, 64, 128), (4096, 128, 320), (777, 768, 2048), (128, 768, 768), (100, 2048, 72)])
 def test_gradients_of_one_launch(R, D, F, dtype):
     """All three products of the backward pass together, in ranges of the rows or not, and the two launches where a third does not fit."""
     t = inputs(R, D, F, dtype, seed=R + F)
@@ -169,6 +169,9 @@ def test_gradients_of_one_launch(R, D, F, dtype):
     for name in ref:
         within(got[name], ref[name], dtype, name)
         assert torch.equal(got[name], again[name])
+    with torch.no_grad():   # (fp32: the gate on the product's store, or where the product goes in ranges by itself)
+        y = ops.gated_feed_forward(*(x.to(DEV) for x in t[:3]))
+    within(y, ref["y"], dtype, "y without gradients")
 
 
 @gpu
