@@ -228,9 +228,9 @@ bool wants_graph(std::initializer_list<Tensor> ts) {
 // In a backward pass that is recorded into a graph: what the gradients go to next has to belong to the graph too.  Nodes that an earlier pass has left alive (a loss that is kept keeps those of its
 // leaves) belong to that pass's stream; autograd would make it wait for the one that records, which nothing ends, and the process ends with the recording.
 void refuse_nodes_outside(const char* what) {
-  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const auto node = torch::autograd::get_current_node();
-  if (!node) return;
+  if (!node || !node->stream() || c10::hip::device_count() == 0) return;   // (tensors without memory are traced on machines without a GPU too)
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   for (const auto& edge : node->next_edges()) {
     if (!edge.is_valid()) continue;
     const auto stream = edge.function->stream();
