@@ -756,11 +756,18 @@ int grads(const Operand2& dy, const Operand2& x, const Operand2& w, void* dw, vo
 // f(activation)
 template <typename F> int by_act(int act, F&& f) { return act == kSilu ? f(std::integral_constant<int, kSilu>()) : f(std::integral_constant<int, kGeluGate>()); }
 
-// Both weight gradients in one launch, where that is ahead of one for each (the second of which may be that of dx too)
-bool both_weights(int R, int D, int F, int dtype, bool dx, WeightsPlan& p) {
+// Both weight gradients in one launch, where that is ahead of one for each (the second of which may be that of dx too); all: dx is in it too
+bool both_weights(int R, int D, int F, int dtype, bool dx, WeightsPlan& p, bool& all) {
+  all = false;
   if (dtype == 0 || (dx && grads_workspace(R, 2 * F, D, 2, kGemmPlain, false) >= 0)) return false;
   p = weights_plan(R, 2 * F, D, D, F);
-  return p.cost < gemm_cost(2 * F, D, R, 2) + gemm_cost(D, F, R, 2);
+  const float weights = gemm_cost(2 * F, D, R, 2) + gemm_cost(D, F, R, 2);
+  if (dx) {
+    const WeightsPlan q = gradients_plan(R, 2 * F, D, D, F, R, D, 2 * F);
+    all = q.cost < 0.9f * (std::min(p.cost, weights) + gemm_cost(R, D, 2 * F, 2));
+    if (all) p = q;
+  }
+  return all || p.cost < weights;
 }
 
 bool few_rows(int R, int dtype) { return R <= kFewRows && dtype != 0; }
@@ -832,7 +839,8 @@ int64_t gated_bwd_workspace(int R, int D, int F, int dtype, int gradients) {
   const int64_t hidden = hidden_bytes(R, D, F, dtype);
   int64_t products = grads_bytes(R, 2 * F, D, dtype, dw_in, dx, dw_out ? D : 0, F);
   WeightsPlan p;
-  if (dw_in && dw_out && both_weights(R, D, F, dtype, dx, p)) products = std::max(up(weights_workspace(p)), dx ? product_workspace(R, D, 2 * F, dtype) : 0);
+  bool all;
+  if (dw_in && dw_out && both_weights(R, D, F, dtype, dx, p, all)) products = std::max(up(weights_workspace(p)), dx && !all ? product_workspace(R, D, 2 * F, dtype) : 0);
   if (in_parts(R, D, F, dtype)) products = (dx ? parts_bytes(R, D, 2 * F) : 0) + (dw_in ? parts_bytes(2 * F, D, R) : 0) + (dw_out ? parts_bytes(F, D, R) : 0);
   if (dtype != 0) return std::max<int64_t>(256, (below ? 2 * hidden : 0) + products);
   const int64_t h = dw_out ? hidden : 0;
@@ -888,9 +896,11 @@ int launch_gated_bwd(const GatedArgs& a, const void* dy, const void* state, void
     return launch_parts(p, dtype, at, stream, [&](auto t, int groups) { hipLaunchKernelGGL((parts_grads_kernel<decltype(t)>), dim3(groups), dim3(64 * kPartsWaves), 0, stream, p); });
   }
   WeightsPlan plan;
-  if (rc == 0 && dw_in != nullptr && dw_out != nullptr && both_weights(a.R, a.D, a.F, dtype, dx != nullptr, plan)) {
-    rc = launch_weights({du, a.x, dw_in, 2 * a.F, a.D, 2 * a.F, a.ld_x}, {dy, h, dw_out, a.D, a.F, a.D, a.F}, a.R, plan, dtype, reinterpret_cast<float*>(at), stream);
-    return rc != 0 || dx == nullptr ? rc : product({du, 2 * a.F, true}, {a.w_in, a.ld_in, false}, dx, a.R, a.D, 2 * a.F, dtype, at, stream);
+  bool all;
+  if (rc == 0 && dw_in != nullptr && dw_out != nullptr && both_weights(a.R, a.D, a.F, dtype, dx != nullptr, plan, all)) {
+    const WeightProduct x = {du, a.w_in, dx, a.R, a.D, 2 * a.F, a.ld_in};
+    rc = launch_weights({du, a.x, dw_in, 2 * a.F, a.D, 2 * a.F, a.ld_x}, {dy, h, dw_out, a.D, a.F, a.D, a.F}, all ? &x : nullptr, 2 * a.F, a.R, plan, dtype, reinterpret_cast<float*>(at), stream);
+    return rc != 0 || dx == nullptr || all ? rc : product({du, 2 * a.F, true}, {a.w_in, a.ld_in, false}, dx, a.R, a.D, 2 * a.F, dtype, at, stream);
   }
   if (rc != 0) return rc;
   return grads({du, 2 * a.F, true}, {a.x, a.ld_x, true}, {a.w_in, a.ld_in, true}, dw_in, dx, a.R, 2 * a.F, a.D, {{dy, a.D, false}, {h, a.F, false}, dw_out, a.D, a.F}, dtype, at, stream);

@@ -15,6 +15,10 @@ __device__ __forceinline__ void settle() {
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
+// the same from an address of each lane
+__device__ __forceinline__ void load_to_lds_from(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
 // LDS traffic of one wave is in order; this keeps the compiler from moving it (and, where registers are short, from
 // requesting operands of the next stage early)
 template <bool STAGES = false> __device__ __forceinline__ void wave_lds_order() {

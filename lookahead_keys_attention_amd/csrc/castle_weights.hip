@@ -25,65 +25,65 @@ struct WeightsArgs {
   WeightProduct p[2];
   int tiles0, R, whole, rest, ranges, steps;
   float* part;   // of range q of tile whole + t: [q][t], in the order of the registers
+  // with the input gradient: dx [R][N] = a b for a [R][lda] and b [K][ldb]
+  WeightProduct x;
+  int x_groups, x_steps, longs, long_steps;   // x_groups: workgroups of an XCD that have a tile of it; x_steps: its whole contraction, K
 };
 // rows of a band of 2048 columns, then those of the next
-__device__ __forceinline__ const WeightProduct& place(const WeightsArgs& a, int t, int& m0, int& n0) {
-  const bool second = t >= a.tiles0;
-  const WeightProduct& p = a.p[second];
-  if (second) t -= a.tiles0;
+__device__ __forceinline__ void place_in(const WeightProduct& p, int t, int& m0, int& n0) {
   constexpr int kBand = 2048 / kTile;
   const int tiles_m = (p.M + kTile - 1) / kTile, tiles_n = (p.N + kTile - 1) / kTile, band = t / (tiles_m * kBand), rest = t - band * tiles_m * kBand, width = min(kBand, tiles_n - band * kBand);
   m0 = rest / width * kTile;
   n0 = (band * kBand + rest % width) * kTile;
+}
+__device__ __forceinline__ WeightProduct place(const WeightsArgs& a, int t, int& m0, int& n0) {
+  const bool second = t >= a.tiles0;
+  const WeightProduct &x = a.p[0], &y = a.p[1];
+  const WeightProduct p = {second ? y.a : x.a, second ? y.b : x.b, second ? y.c : x.c, second ? y.M : x.M, second ? y.N : x.N, second ? y.lda : x.lda, second ? y.ldb : x.ldb};
+  place_in(p, second ? t - a.tiles0 : t, m0, n0);
   return p;
 }
 
-// END: the contraction ends inside a step
-template <typename T, bool END> __global__ __launch_bounds__(kWideThreads, 2) void weights_kernel(WeightsArgs a) {
-  typedef WideOperand<T, false, kTile> Op;
+// What a workgroup does next: steps of a tile's contraction; slot: where the sums of a range go, -1: to the output.
+struct Unit {
+  WeightProduct p;
+  int m0, n0, from, steps, slot;
+};
+// Units 0, 1, ... of the workgroup, as long as at(i, unit) has one.  AKC: a is contraction-contiguous.  K: the whole contraction, END: it ends inside a step.
+template <typename T, bool AKC, bool END, typename At> __device__ __forceinline__ void run_units(At&& at, int K, float* parts) {
+  typedef WideOperand<T, AKC, kTile> OpA;
+  typedef WideOperand<T, false, kTile> OpB;
   typedef vec<T, 8> vt;
   const int lane = lane_id(), wave = wave_id(), c = lane & 31, g = lane >> 5, wm = wave / 2 * 64, wn = wave % 2 * 128;
-  const int all_steps = (a.R + kWideK - 1) / kWideK, stride = gridDim.x, last = a.whole + a.rest * a.ranges;
-  int unit = blockIdx.x % 8 * (stride / 8) + blockIdx.x / 8;   // XCD x takes the x-th eighth of a round
-  if (unit >= last) return;
+  const int all_steps = (K + kWideK - 1) / kWideK;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)castle_weights_lds;
-  auto steps_of = [&](int u, int& tile, int& from) __attribute__((always_inline)) {
-    tile = u;
-    from = 0;
-    if (u < a.whole) return all_steps;
-    const int q = (u - a.whole) / a.rest;
-    tile = u - q * a.rest;
-    from = q * a.steps;
-    return min(a.steps, all_steps - from);
-  };
+  Unit unit, next;
+  if (!at(0, unit)) return;
+  next = unit;
   // the step that is requested next runs ahead of the one that is multiplied, into the next tile or range
-  Op ra, rb;
-  int64_t lda, ldb;
-  int next_unit = unit, next_step, next_end, ahead = 0;   // ahead: steps requested and not waited for
+  OpA ra;
+  OpB rb;
+  int next_i = 0, next_step = 0, ahead = 0;   // ahead: steps requested and not waited for
+  bool left = true;
   auto start = [&]() __attribute__((always_inline)) {
-    int tile, m0, n0;
-    const int n = steps_of(next_unit, tile, next_step);
-    next_end = next_step + n;
-    const WeightProduct& p = place(a, tile, m0, n0);
-    lda = p.lda;
-    ldb = p.ldb;
-    ra.start(static_cast<const T*>(p.a), lda, m0, p.M, next_step * kWideK);
-    rb.start(static_cast<const T*>(p.b), ldb, n0, p.N, next_step * kWideK);
+    next_step = next.from;
+    ra.start(static_cast<const T*>(next.p.a), next.p.lda, next.m0, next.p.M, next_step * kWideK);
+    rb.start(static_cast<const T*>(next.p.b), next.p.ldb, next.n0, next.p.N, next_step * kWideK);
   };
   auto request = [&](int buffer) __attribute__((always_inline)) {
-    if (next_unit >= last) return;
+    if (!left) return;
     ++ahead;
     if (END && next_step == all_steps - 1) {
-      const int left = a.R - next_step * kWideK;
-      ra.load_end(left, reinterpret_cast<const T*>(castle_weights_zeros), lds0 + buffer);
-      rb.load_end(left, reinterpret_cast<const T*>(castle_weights_zeros), lds0 + buffer + kStage / 2);
+      const int rest = K - next_step * kWideK;
+      ra.load_end(rest, reinterpret_cast<const T*>(castle_weights_zeros), lds0 + buffer);
+      rb.load_end(rest, reinterpret_cast<const T*>(castle_weights_zeros), lds0 + buffer + kStage / 2);
     } else {
-      ra.load(lda, lds0 + buffer);
-      rb.load(ldb, lds0 + buffer + kStage / 2);
+      ra.load(next.p.lda, lds0 + buffer);
+      rb.load(next.p.ldb, lds0 + buffer + kStage / 2);
     }
-    if (++next_step == next_end) {
-      next_unit += stride;
-      if (next_unit < last) start();
+    if (++next_step == next.from + next.steps) {
+      left = at(++next_i, next);
+      if (left) start();
     }
   };
   start();
@@ -111,16 +111,15 @@ template <typename T, bool END> __global__ __launch_bounds__(kWideThreads, 2) vo
   frag<T> fa[2][2], fb[2][4];
   auto read = [&](int slot, int s) __attribute__((always_inline)) {
     const T* l = reinterpret_cast<const T*>(castle_weights_lds + buffer);
-    Op::read(l, fa[slot], wm, s, c, g);
-    Op::read(l + kTile * kWideK, fb[slot], wn, s, c, g);
+    OpA::read(l, fa[slot], wm, s, c, g);
+    OpB::read(l + kTile * kWideK, fb[slot], wn, s, c, g);
     __builtin_amdgcn_sched_barrier(0);   // these reads, then the products of the fragments before
   };
   arrive();
   read(0, 0);
-  for (; unit < last; unit += stride) {
-    int tile, from, m0, n0;
-    const int steps = steps_of(unit, tile, from);
-    const WeightProduct& p = place(a, tile, m0, n0);
+  for (int i = 0; i == 0 || at(i, unit); ++i) {
+    const WeightProduct& p = unit.p;
+    const int m0 = unit.m0, n0 = unit.n0;
     acc_t acc[2][4];   // [n rows, m lanes]
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -133,7 +132,7 @@ template <typename T, bool END> __global__ __launch_bounds__(kWideThreads, 2) vo
         for (int j = 0; j < 4; ++j) mma(acc[i][j], fb[slot][j], fa[slot][i]);
     };
     int done = 0;   // buffer of the step that ends
-    for (int it = 0; it < steps; ++it) {
+    for (int it = 0; it < unit.steps; ++it) {
 #pragma unroll
       for (int s = 0; s < kWideK / 16 - 1; ++s) {
         read(1 - s % 2, s + 1);
@@ -142,15 +141,15 @@ template <typename T, bool END> __global__ __launch_bounds__(kWideThreads, 2) vo
       arrive();
       done = buffer;
       buffer = kStage - buffer;
-      if (it + 1 < steps) request(done);
+      if (it + 1 < unit.steps) request(done);
       read(0, 0);   // (behind the last step of all: what is there, for nothing)
       multiply(1);
     }
     asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");   // the loop may end right behind a product
     __builtin_amdgcn_sched_barrier(0);
     request(done);
-    if (unit >= a.whole && a.ranges > 1) {
-      vec<float, 4>* part = reinterpret_cast<vec<float, 4>*>(a.part + (int64_t)(unit - a.whole) * kPart) + wave * 2048 + lane;
+    if (unit.slot >= 0) {
+      vec<float, 4>* part = reinterpret_cast<vec<float, 4>*>(parts + (int64_t)unit.slot * kPart) + wave * 2048 + lane;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -184,6 +183,56 @@ template <typename T, bool END> __global__ __launch_bounds__(kWideThreads, 2) vo
     if (m0 + kTile <= p.M && n0 + kTile <= p.N) stores = 1;
   }
 }
+template <typename T, bool END> __global__ __launch_bounds__(kWideThreads, 2) void weights_kernel(WeightsArgs a) {
+  const int all_steps = (a.R + kWideK - 1) / kWideK, stride = gridDim.x, last = a.whole + a.rest * a.ranges;
+  const int first = blockIdx.x % 8 * (stride / 8) + blockIdx.x / 8;   // XCD x takes the x-th eighth of a round
+  run_units<T, false, END>([&](int i, Unit& u) __attribute__((always_inline)) {
+    const int k = first + i * stride;
+    if (k >= last) return false;
+    int tile = k;
+    u.from = 0;
+    u.steps = all_steps;
+    u.slot = -1;
+    if (k >= a.whole) {
+      const int q = (k - a.whole) / a.rest;
+      tile = k - q * a.rest;
+      u.from = q * a.steps;
+      u.steps = min(a.steps, all_steps - u.from);
+      if (a.ranges > 1) u.slot = k - a.whole;
+    }
+    u.p = place(a, tile, u.m0, u.n0);
+    return true;
+  }, a.R, a.part);
+}
+// The input gradient too, where its tiles do not fill a round of the card: some workgroups of every XCD have one of its tiles and then a short range of the rows, the others a long range.  Backward pass, us, dx by itself / here: 8192
+// rows of 512 through 1408 127 / 116, 12345 of 512 through 1400 183 / 167, 20000 of 256 through 1024 132 / 117; where dx fills its rounds by itself it is behind (16384 of 512 through 1408 200 / 210).
+template <typename T, bool END> __global__ __launch_bounds__(kWideThreads, 2) void gradients_kernel(WeightsArgs a) {
+  const int xcd = blockIdx.x % 8, j = blockIdx.x / 8, all_steps = (a.R + kWideK - 1) / kWideK;
+  const bool has_x = j < a.x_groups;
+  if (has_x) {
+    run_units<T, true, END>([&](int i, Unit& u) __attribute__((always_inline)) {
+      const int t = xcd * a.x_groups + j;
+      if (i > 0 || t >= tiles_of(a.x.M, a.x.N)) return false;
+      u.p = a.x;
+      place_in(a.x, t, u.m0, u.n0);
+      u.from = 0;
+      u.steps = (a.x_steps + kWideK - 1) / kWideK;
+      u.slot = -1;
+      return true;
+    }, a.x_steps, nullptr);
+    __syncthreads();
+  }
+  run_units<T, false, END>([&](int i, Unit& u) __attribute__((always_inline)) {
+    const int others = 32 - a.x_groups, k = has_x ? xcd * a.x_groups + j : xcd * others + j - a.x_groups;   // of the short or of the long ranges
+    if (i > 0 || k >= a.rest * (has_x ? a.ranges - a.longs : a.longs)) return false;
+    const int q = k / a.rest, tile = k - q * a.rest;
+    u.from = has_x ? a.longs * a.long_steps + q * a.steps : q * a.long_steps;
+    u.steps = min(has_x ? a.steps : a.long_steps, all_steps - u.from);
+    u.slot = a.ranges > 1 ? (has_x ? a.longs * a.rest : 0) + k : -1;
+    u.p = place(a, tile, u.m0, u.n0);
+    return true;
+  }, a.R, a.part);
+}
 
 // four columns a thread, in the order of the registers that they come from
 template <typename T> __global__ __launch_bounds__(256) void weights_join_kernel(WeightsArgs a) {
@@ -194,22 +243,25 @@ template <typename T> __global__ __launch_bounds__(256) void weights_join_kernel
 #pragma unroll 4
   for (int q = 1; q < a.ranges; ++q) sum += part[q * next];
   int m0, n0;
-  const WeightProduct& p = place(a, a.whole + t, m0, n0);
+  const WeightProduct p = place(a, a.whole + t, m0, n0);
   const int lane = at & 63, q = at >> 6 & 3, j = at >> 8 & 3, i = at >> 10 & 1, wave = at >> 11;
   const int m = m0 + wave / 2 * 64 + 32 * i + (lane & 31), n = n0 + wave % 2 * 128 + 32 * j + 8 * q + 4 * (lane >> 5);
   if (m < p.M && n < p.N) *reinterpret_cast<vec<T, 4>*>(static_cast<T*>(p.c) + (int64_t)m * p.N + n) = __builtin_convertvector(sum, vec<T, 4>);
 }
 
-template <typename T, bool END> int launch_kernel(const WeightsArgs& a, hipStream_t stream) {
-  static PerDeviceOnce once;
+template <typename Kernel> int launch_kernel(Kernel kernel, PerDeviceOnce& once, int groups, const WeightsArgs& a, hipStream_t stream) {
   bool& configured = once.flag();
   if (!configured) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&weights_kernel<T, END>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) return -3;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) return -3;
     configured = true;
   }
-  const int units = a.whole + a.rest * a.ranges;
-  hipLaunchKernelGGL((weights_kernel<T, END>), dim3(std::min((units + 7) / 8 * 8, kCus)), dim3(kWideThreads), kLds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3(groups), dim3(kWideThreads), kLds, stream, a);
   return hipGetLastError() == hipSuccess ? 0 : -3;
+}
+template <typename T, bool END> int launch_kernels(const WeightsArgs& a, hipStream_t stream) {
+  static PerDeviceOnce once[2];
+  if (a.x.c != nullptr) return launch_kernel(&gradients_kernel<T, END>, once[0], kCus, a, stream);
+  return launch_kernel(&weights_kernel<T, END>, once[1], std::min((a.whole + a.rest * a.ranges + 7) / 8 * 8, kCus), a, stream);
 }
 
 }  // namespace
@@ -233,13 +285,33 @@ WeightsPlan weights_plan(int R, int M0, int N0, int M1, int N1) {
   }
   return best;
 }
+// The input gradient, of M x N over K, in the same launch: cost 1e30 where there is no room for its tiles beside the ranges.  A workgroup that has one goes on to a range that is as much shorter.
+WeightsPlan gradients_plan(int R, int M0, int N0, int M1, int N1, int M, int N, int K) {
+  WeightsPlan p = {0, 0, 1, 0, 1e30f};
+  const int64_t n64 = (int64_t)tiles_of(M0, N0) + tiles_of(M1, N1), x64 = tiles_of(M, N);
+  if (n64 > kCus || x64 > kCus * 3 / 4) return p;
+  const int n = (int)n64, steps = (R + kWideK - 1) / kWideK, x_steps = (K + kWideK - 1) / kWideK, groups = ((int)x64 + 7) / 8;
+  // us a step: 1.9 of ranges, whose rows come from HBM, 1.5 of dx
+  int longs = 8 * (32 - groups) / n, shorts = 8 * groups / n;
+  if (longs == 0) return p;
+  int each = shorts > 0 ? (steps - (int)(longs * (x_steps * 0.79f + 2))) / (longs + shorts) : 0;   // of a short one (2: the change from one to the other)
+  if (each <= 0) each = shorts = 0;
+  const int most = (steps - shorts * each + longs - 1) / longs;
+  longs = std::min(longs, (steps + most - 1) / most);
+  const int left = std::max(0, steps - longs * most);   // of the short ones
+  shorts = left > 0 ? (left + each - 1) / each : 0;
+  p = {0, n, longs + shorts, shorts > 0 ? each : 0, 0, groups, longs, most};
+  const int parts = p.ranges > 1 ? n * p.ranges : 0;
+  p.cost = 8 + std::max(most * 1.9f, x_steps * 1.5f + (shorts > 0 ? 3 + each * 1.9f : 0)) + 4 + (parts > 0 ? 4 + parts * 0.05f : 0);
+  return p;
+}
 int64_t weights_workspace(const WeightsPlan& p) { return p.ranges > 1 ? (int64_t)p.rest * p.ranges * kPart * 4 : 0; }
 
-int launch_weights(const WeightProduct& first, const WeightProduct& second, int R, const WeightsPlan& p, int dtype, float* workspace, hipStream_t stream) {
-  const WeightsArgs a = {{first, second}, tiles_of(first.M, first.N), R, p.whole, p.rest, p.ranges, p.steps, workspace};
+int launch_weights(const WeightProduct& first, const WeightProduct& second, const WeightProduct* x, int K, int R, const WeightsPlan& p, int dtype, float* workspace, hipStream_t stream) {
+  const WeightsArgs a = {{first, second}, tiles_of(first.M, first.N), R, p.whole, p.rest, p.ranges, p.steps, workspace, x != nullptr ? *x : WeightProduct{}, p.x_groups, K, p.longs, p.long_steps};
   return by_type16(dtype, true, [&](auto t, auto) {
     using T = decltype(t);
-    const int rc = R % kWideK == 0 ? launch_kernel<T, false>(a, stream) : launch_kernel<T, true>(a, stream);
+    const int rc = R % kWideK == 0 && (x == nullptr || K % kWideK == 0) ? launch_kernels<T, false>(a, stream) : launch_kernels<T, true>(a, stream);
     if (rc == 0 && p.ranges > 1) hipLaunchKernelGGL((weights_join_kernel<T>), dim3(p.rest * (kPart / 1024)), dim3(256), 0, stream, a);
     return rc != 0 ? rc : hipGetLastError() == hipSuccess ? 0 : -3;
   });

@@ -54,8 +54,7 @@ template <typename T, bool KC, int FREE> struct WideOperand {
         constexpr int PIECES = FREE / 8, ROWS = 64 / PIECES;
         there = ROWS * (first + q) + lane / PIECES < steps;
       }
-      if (there) load_to_lds(at, off[q], lds + 1024 * (first + q));
-      else load_to_lds(zeros, 0, lds + 1024 * (first + q));
+      load_to_lds_from(there ? reinterpret_cast<const unsigned char*>(at) + off[q] : reinterpret_cast<const unsigned char*>(zeros), lds + 1024 * (first + q));
     }
   }
   // operand fragments of the wave's 32 W columns from free0, 16 contraction steps from 16 s

@@ -144,9 +144,9 @@ def test_sizes_of_tiles(R, D, F):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("R, D, F", [(199, 1024, 4096), (3000, 768, 2048), (12345, 200, 520), (1000, 2048, 4096), (2048, 2048, 3000)])
+@pytest.mark.parametrize("R, D, F", [(199, 1024, 4096), (3000, 768, 2048), (12345, 200, 520), (1000, 2048, 4096), (2048, 2048, 3000), (8192, 512, 1408), (12345, 512, 1400), (9999, 256, 1000)])
 def test_weight_gradients_of_one_launch(R, D, F, dtype):
-    """Tiles taken whole, in ranges, both; contractions that end inside a step, with rows behind the end that are not finite; ragged tiles; the same bits again."""
+    """Tiles taken whole, in ranges, both, with the input gradient among them; contractions that end inside a step, with rows behind the end that are not finite; ragged tiles; the same bits again."""
     x, win, wout, dy = (t.to(DEV) for t in inputs(R, D, F, dtype, seed=R))
     ref = {k: (v.cpu(), off.cpu()) for k, (v, off) in reference(x, win, wout, dy, "silu", dtype).items()}
     longer = [torch.cat((t, torch.full((64, D), float("nan"), device=DEV, dtype=dtype))) for t in (x, dy)]
