@@ -237,6 +237,23 @@ def test_strides_of_all_operands():
 
 
 @gpu
+@pytest.mark.parametrize("R, D, F, dtype", [(8, 24, 192, torch.bfloat16), (300, 200, 520, torch.bfloat16), (199, 1024, 4096, torch.bfloat16), (12345, 512, 1400, torch.bfloat16), (300, 200, 520, torch.float32),
+                                            (100, 2048, 72, torch.float32)])
+def test_rows_apart_and_some_of_the_gradients(R, D, F, dtype):
+    """Every way that the backward pass goes: rows of all operands with NaNs between them, and each choice of gradients, which are those of all three."""
+    t = inputs(R, D, F, dtype, seed=R)
+    ref = {k: (v.cpu(), off.cpu()) for k, (v, off) in reference(*(x.to(DEV) for x in t), "silu", dtype).items()}
+    apart = [torch.cat((x, x.new_full((x.shape[0], 40), float("nan"))), 1).to(DEV)[:, :x.shape[1]] for x in t]
+    for need in range(1, 8):
+        leaves = [x.detach().requires_grad_(bool(need >> i & 1)) for i, x in enumerate(apart[:3])]
+        y = ops.gated_feed_forward(*leaves)
+        asked = [(leaf, name) for leaf, name in zip(leaves, ("dx", "dwin", "dwout")) if leaf.requires_grad]
+        for got, (_, name) in zip(torch.autograd.grad(y, [leaf for leaf, _ in asked], apart[3]), asked):
+            within(got, ref[name], dtype, (name, need))
+        within(y, ref["y"], dtype, "y")
+
+
+@gpu
 def test_shapes_and_empty_calls():
     x, win, wout, dy = (t.to(DEV) for t in inputs(24, 64, 72, torch.bfloat16))
     flat = ops.gated_feed_forward(x, win, wout)
