@@ -163,9 +163,21 @@ __global__ __launch_bounds__(1024) void begin_kernel(const double* parts, int co
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 __device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
 
-// Roots and quotients to an ulp or two: correctly rounded ones took a fifth of the kernel with states of 8 bits.  The instruction takes denormal numbers for zero: x below 2^-126, or zero, has the
-// root 2^-63 here (compared as whole numbers, of which a NaN is among the largest).
-__device__ __forceinline__ float fast_sqrt(float x) { return __builtin_amdgcn_sqrtf(__builtin_bit_cast(float, max(bits_of(x), bits_of(0x1p-126f)))); }
+// Roots and quotients to an ulp or two: correctly rounded ones took a fifth of the kernel with states of 8 bits.  The instruction takes denormal numbers for zero: where one of a wave's is, those are
+// scaled before it.  Zero has the root zero; `least`, the bits of 2^-126, where eps is zero: then 2^-63, and the element stays where it is.
+__device__ __forceinline__ bool denormal(float x) { return __builtin_amdgcn_classf(x, 0x90); }
+__device__ __forceinline__ void fast_roots(const vec<float, 8>& v, uint32_t least, vec<float, 8>& r) {
+  bool scaled = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    r[e] = __builtin_amdgcn_sqrtf(__builtin_bit_cast(float, max(bits_of(v[e]), least)));   // (as whole numbers, of which a NaN is among the largest)
+    scaled |= denormal(v[e]);
+  }
+  if (__ballot(scaled) == 0) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (denormal(v[e])) r[e] = __builtin_amdgcn_sqrtf(v[e] * 0x1p64f) * 0x1p-32f;
+}
 
 // Eight numbers to e4m3, up or down by chance: the instruction adds the upper bits of its last operand to what it cuts off, below the normal numbers too, which is what castle_hip.h says (its results
 // are those of that formula for 1.7e7 numbers from 2^-20 to 448 and all that is not finite).
@@ -245,6 +257,7 @@ template <typename T, bool SMALL, bool CHANCE> __global__ __launch_bounds__(kThr
   const int k = __builtin_amdgcn_readfirstlane(tensor_of(a, blockIdx.x));
   const OptimTensor t = a.t[k];
   const StepNumbers s = *numbers;
+  const uint32_t least = eps == 0.f ? bits_of(0x1p-126f) : 0;
   const uint64_t key = SMALL || CHANCE ? (uint64_t)*seed : 0, at_step = (uint64_t)(uint32_t)(a.number + k) << 32 | s.step;
   const int64_t begin = (int64_t)(blockIdx.x - a.first[k]) * (kGroup * kTurns) + threadIdx.x * 8;
   // what a turn reads is requested a turn ahead
@@ -291,10 +304,16 @@ template <typename T, bool SMALL, bool CHANCE> __global__ __launch_bounds__(kThr
       const float g = x[e] * s.clip;
       m[e] = b1 * m[e] + c1 * g;
       v[e] = b2 * v[e] + c2 * (g * g);
-      // (correctly rounded beside parameters of 32 bits: a root that is one unit off is rounded to another state in one of 6 million cases, and those show where parameters keep their 24 bits)
-      r[e] = SMALL && sizeof(T) == 4 ? sqrtf(v[e]) : fast_sqrt(v[e]);
-      q[e] = p[e] * s.keep - s.rate * m[e] * fast_rcp(r[e] * s.root + eps);
     }
+    // (correctly rounded beside parameters of 32 bits: a root that is one unit off is rounded to another state in one of 6 million cases, and those show where parameters keep their 24 bits)
+    if constexpr (SMALL && sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = sqrtf(v[e]);
+    } else {
+      fast_roots(v, least, r);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = p[e] * s.keep - s.rate * m[e] * fast_rcp(r[e] * s.root + eps);
     const uint64_t counter = 4 * (uint64_t)(at >> 3);
     if constexpr (SMALL) {
       // (the largest root is that of the largest square: the exponent goes by the correctly rounded one)

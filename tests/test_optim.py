@@ -495,3 +495,62 @@ def test_a_step_that_begins_inside_a_capture_is_refused():
             optimizer.step()
     optimizer.step()
     assert int(optimizer.state[p]["step"]) == 1
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_second_moments_below_the_normal_numbers(dtype, bits):
+    """Squares that begin around 2^-126 and below, alone in their 256 and beside larger ones, and fade until they are zero: states and parameters are the formula's, whose numbers of 32 bits they are formed from."""
+    n, b, eps, lr = 8 * 256, 0.5, 1e-30, 3e-3
+    grad = torch.exp2(-torch.arange(8.0) * 2).repeat_interleave(256)   # 1 .. 2^-14, by 256
+    grad[:256:2] = 2.0 ** -12   # sizes of many orders side by side
+    grad[1:256:64] = 2.0 ** -14
+    grad[::7] = 0
+    grad[3::5] *= -1
+    grad, nothing = grad.to(dtype).to(DEV), torch.zeros(n, dtype=dtype, device=DEV)
+    p, = tensors([(n,)], dtype, 1, DEV)
+    (m,), (v,), em, ev = empty_states([(n,)], bits)
+    step, one = counter(), torch.ones(1, device=DEV)
+    scale = torch.tensor(1e-18) / (torch.ones(()) + 1e-6)   # of the gradients, by their clipping: fp16 has none of such sizes
+    for t in range(1, 45):
+        g = (grad if t in (1, 2, 40) else nothing).cpu().float() * scale
+        p0 = p.cpu().double()
+        if bits == 8:
+            m0, r0 = values(m, em[0]).float(), values(v, ev[0]).float()
+            v0 = r0 * r0
+        else:
+            m0, v0 = m.cpu(), v.cpu()
+        m1, v1 = b * m0 + b * g, b * v0 + b * (g * g)
+        ops.adamw_step([p], [grad if t in (1, 2, 40) else nothing], [m], [v], step, lr=lr, betas=(b, b), eps=eps, weight_decay=0.0, max_norm=1e-18, norm=one, seed=seed_of() if bits == 8 else None,
+                       exp_avg_exponents=em, exp_avg_sq_exponents=ev)
+        root = v1.double().sqrt()
+        if bits == 8:
+            check_chance(m, em[0], m1.double(), False)
+            check_chance(v, ev[0], root, True)
+        else:
+            assert torch.equal(m.cpu(), m1) and torch.equal(v.cpu(), v1), t
+        change = lr / (1 - b ** t) * m1.double() / (root / math.sqrt(1 - b ** t) + eps)
+        slack = 40 * U * (p0.abs() + change.abs())
+        want = p0 - change
+        kind = {torch.float32: 0.0}.get(dtype, torch.finfo(dtype).eps / (2 if bits == 32 else 1))
+        most = slack + kind * (want.abs() + slack).clamp(min=torch.finfo(dtype).tiny)
+        # (where v has faded to zero and m has not, a step is m / eps by the formula: in fp16 a parameter passes 65504 at last, and is infinite from there on)
+        far = want.abs() > torch.finfo(dtype).max
+        close(p.cpu()[~far], want[~far], most[~far], t)
+        assert torch.equal(p.cpu()[far].double(), torch.copysign(torch.tensor(math.inf, dtype=torch.float64), want[far]))
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_elements_without_gradients_and_an_eps_of_zero(bits):
+    """Parameters of 16 bits that never had a gradient stay where they are, decay aside, whatever eps is."""
+    p, = tensors([(600,)], torch.bfloat16, 1, DEV)
+    g = torch.zeros_like(p)
+    g[7] = 0.25
+    before = p.clone()
+    m, v, em, ev = empty_states([(600,)], bits)
+    for _ in range(2):
+        ops.adamw_step([p], [g], m, v, counter(), lr=1e-2, eps=0.0, weight_decay=0.0, seed=seed_of(), exp_avg_exponents=em, exp_avg_sq_exponents=ev)
+    there = torch.arange(600, device=DEV) == 7
+    assert torch.equal(p[~there], before[~there]) and p.isfinite().all() and p[7] != before[7]
