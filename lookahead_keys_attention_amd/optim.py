@@ -7,8 +7,10 @@ state_bits 8 keeps both moments as e4m3 numbers with an exponent for each 256 of
 are rounded by chance; `stochastic_rounding` says whether parameters of 16 bits are too (of 32 bits they are exact).  `max_norm`
 clips the gradients of all groups by their common norm; it is left in `grad_norm`, a number on the GPU, behind each step.
 
-Steps are counted on the GPU and nothing is read back, so a step can be captured into a graph once one has been taken; `lr` of a
-group may be a float32 tensor of one element on the GPU, which a replay reads anew.
+Steps are counted on the GPU, for each parameter those in which it had a gradient, and nothing is read back, so a step can be
+captured into a graph once one of the same parameters has been taken; `lr` of a group may be a float32 tensor of one element on the
+GPU, which a replay reads anew.  A graph counts for the parameters that shared a count when it was recorded: where some of them
+have paused since, it is recorded again.
 """
 from __future__ import annotations
 
@@ -17,6 +19,7 @@ import torch
 from . import ops
 
 _MOMENTS = ("exp_avg", "exp_avg_sq")
+_ODD = 6364136223846793005   # (seeds go round 64 bits)
 
 
 def _order(t):
@@ -75,10 +78,12 @@ class AdamW(torch.optim.Optimizer):
         return norms[0] if len(norms) == 1 else torch.linalg.vector_norm(torch.stack(norms).double()).float()
 
     def _calls(self, group):
-        """(group, parameters) for each call of a step: parameters of one type whose states began together."""
-        new, calls = {}, {}
+        """(group, parameters) for each call of a step: parameters of one type that have had a gradient in the same steps."""
+        new, calls, paused = {}, {}, set()
         for p in group["params"]:
             if p.grad is None:
+                if self.state.get(p):
+                    paused.add(id(self.state[p]["step"]))
                 continue
             if p.grad.is_sparse:
                 raise RuntimeError("AdamW: gradients are dense")
@@ -91,7 +96,20 @@ class AdamW(torch.optim.Optimizer):
         for p in group["params"]:
             if p.grad is not None:
                 calls.setdefault((p.dtype, id(self.state[p]["step"])), (group, []))[1].append(p)
+        for (_, count), (_, params) in calls.items():
+            if count in paused:
+                self._part(params)
         return list(calls.values())
+
+    def _part(self, params):
+        """Parameters that go on without others of their count: from here on they have one of their own, and a seed."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: some parameters have no gradient that had one in every step so far; take such a step before one is captured")
+        first = self.state[params[0]]
+        place = next(i for i, p in enumerate(q for group in self.param_groups for q in group["params"]) if p is params[0])
+        step, seed = first["step"].clone(), first["seed"] * _ODD + (place + 1)   # (another one for each place, as no parameter parts from the same seed twice)
+        for p in params:
+            self.state[p]["step"], self.state[p]["seed"] = step, seed
 
     def _begin(self, params, device, bits):
         """States of parameters that have a gradient for the first time: one count of steps and one seed for all of them."""

@@ -554,3 +554,51 @@ def test_elements_without_gradients_and_an_eps_of_zero(bits):
         ops.adamw_step([p], [g], m, v, counter(), lr=1e-2, eps=0.0, weight_decay=0.0, seed=seed_of(), exp_avg_exponents=em, exp_avg_sq_exponents=ev)
     there = torch.arange(600, device=DEV) == 7
     assert torch.equal(p[~there], before[~there]) and p.isfinite().all() and p[7] != before[7]
+
+
+@gpu
+def test_parameters_that_pause():
+    """Parameters without a gradient in some steps, which begin together: their counts and what they become are those of torch's AdamW, which counts for each."""
+    nets = [torch.nn.ModuleList(torch.nn.Linear(16, 16) for _ in range(4)) for _ in range(2)]
+    nets[1].load_state_dict(nets[0].state_dict())
+    ours, theirs = (net.to(DEV) for net in nets)
+    a, b = AdamW(ours.parameters(), lr=1e-2, betas=(0.9, 0.99)), torch.optim.AdamW(theirs.parameters(), lr=1e-2, betas=(0.9, 0.99))
+    which = [(0, 1, 2, 3)] + [(0, 1)] * 4 + [(0, 2), (0, 1, 2, 3), (3,), (), (0, 1, 2, 3), (2, 3)]
+    for k, used in enumerate(which):
+        for net, optimizer in ((ours, a), (theirs, b)):
+            torch.manual_seed(k)
+            optimizer.zero_grad(set_to_none=True)
+            for i in used:
+                net[i](torch.randn(8, 16, device=DEV)).square().sum().backward()
+            optimizer.step()
+        for i, (p, q) in enumerate(zip(ours.parameters(), theirs.parameters())):
+            assert int(a.state[p]["step"]) == int(b.state[q]["step"]), (k, i)
+            assert torch.allclose(p, q, rtol=1e-4, atol=1e-5), (k, i)   # as in test_optimizer_against_torch
+    assert len({int(s["seed"]) for s in a.state.values()}) == len({id(s["step"]) for s in a.state.values()}) == 4
+    again = AdamW(ours.parameters())
+    again.load_state_dict(copy.deepcopy(a.state_dict()))
+    assert [int(again.state[p]["step"]) for p in ours.parameters()] == [int(a.state[p]["step"]) for p in ours.parameters()]
+
+
+@gpu
+def test_a_pause_that_begins_inside_a_capture_is_refused():
+    params = [torch.nn.Parameter(torch.ones(8, device=DEV)) for _ in range(2)]
+    optimizer = AdamW(params, lr=1e-2)
+    for p in params:
+        p.grad = torch.ones(8, device=DEV)
+    optimizer.step()
+    params[1].grad = None
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="before one is captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            optimizer.step()
+    assert [int(optimizer.state[p]["step"]) for p in params] == [1, 1]
+    optimizer.step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        optimizer.step()
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert [int(optimizer.state[p]["step"]) for p in params] == [3 + k, 1]
