@@ -5,7 +5,8 @@ gradients, train_triton.py:219-259) as a few launches for all parameters of a gr
 
 state_bits 8 keeps both moments as e4m3 numbers with an exponent for each 256 of them, 2 bytes a parameter instead of 8.  Those
 are rounded by chance; `stochastic_rounding` says whether parameters of 16 bits are too (of 32 bits they are exact).  `max_norm`
-clips the gradients of all groups by their common norm; it is left in `grad_norm`, a number on the GPU, behind each step.
+clips the gradients of all groups by their common norm; it is left in `grad_norm`, a number on the GPU, behind each step.  A saved
+state brings it along, as it does the options of the groups.
 
 Steps are counted on the GPU, for each parameter those in which it had a gradient, and nothing is read back, so a step can be
 captured into a graph once one of the same parameters has been taken; `lr` of a group may be a float32 tensor of one element on the
@@ -44,6 +45,12 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: states of 8 or 32 bits, got {state_bits}")
         self.max_norm, self.grad_norm = max_norm, None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, stochastic_rounding=stochastic_rounding))
+
+    def __getstate__(self):   # (of copies and pickles)
+        return super().__getstate__() | dict(max_norm=self.max_norm, grad_norm=None)
+
+    def state_dict(self):
+        return super().state_dict() | dict(max_norm=self.max_norm)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -142,6 +149,7 @@ class AdamW(torch.optim.Optimizer):
                 if value.dtype != torch.float32 and _order(value) != _order(torch.empty_like(p, device="meta")):
                     raise ValueError("AdamW: a saved state of 8 bits has another order in memory than its parameter, and its exponents go by that")
         super().load_state_dict(state_dict)
+        self.max_norm = state_dict.get("max_norm", self.max_norm)   # (like the options of the groups)
         shared = {}
         for i, p in zip(saved, params):
             if i not in state_dict["state"]:

@@ -4,7 +4,9 @@ Tolerances.  u = 2^-24 is the rounding of a 32-bit operation.  Moments: two prod
 of the step, and where sums cancel of their magnitudes.  What is rounded by chance lies between the two neighbours of the number before: within one step of the type, 2^-3 of an e4m3 number (2^-9 of 448 below its
 normal numbers), eps of a 16-bit one; and its mean over many draws is the number itself, within 6 of the mean's standard deviations, at most half a step each over the root of their number."""
 import copy
+import io
 import math
+import pickle
 
 import pytest
 import torch
@@ -602,3 +604,27 @@ def test_a_pause_that_begins_inside_a_capture_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert [int(optimizer.state[p]["step"]) for p in params] == [3 + k, 1]
+
+
+def test_copies_and_pickles_keep_the_clipping():
+    w = torch.nn.Parameter(torch.zeros(3))
+    optimizer = AdamW([w], max_norm=0.5, lr=1e-2)
+    optimizer.grad_norm = torch.ones(())
+    stored = io.BytesIO()
+    torch.save(optimizer, stored)
+    stored.seek(0)
+    for again in (copy.deepcopy(optimizer), pickle.loads(pickle.dumps(optimizer)), torch.load(stored, weights_only=False)):
+        assert again.max_norm == 0.5 and again.grad_norm is None and again.param_groups[0]["lr"] == 1e-2
+        assert again.step() is None   # (no gradients)
+
+
+def test_saved_states_bring_their_clipping():
+    make = lambda **more: AdamW([torch.nn.Parameter(torch.zeros(3))], **more)
+    for max_norm in (0.5, None):
+        other = make(max_norm=2.0)
+        other.load_state_dict(make(max_norm=max_norm).state_dict())
+        assert other.max_norm == max_norm
+    before = {k: v for k, v in make().state_dict().items() if k in ("state", "param_groups")}   # (as they were saved without it)
+    other = make(max_norm=2.0)
+    other.load_state_dict(before)
+    assert other.max_norm == 2.0
