@@ -59,9 +59,9 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         calls = [call for group in self.param_groups for call in self._calls(group)]
+        self.grad_norm = norm = None
         if not calls:
             return loss
-        self.grad_norm = norm = None
         if self.max_norm is not None and len(calls) > 1:
             norm = self._norm([p.grad for _, params in calls for p in params])
         for group, params in calls:

@@ -628,3 +628,10 @@ def test_saved_states_bring_their_clipping():
     other = make(max_norm=2.0)
     other.load_state_dict(before)
     assert other.max_norm == 2.0
+
+
+def test_a_step_without_gradients_leaves_no_norm():
+    optimizer = AdamW([torch.nn.Parameter(torch.zeros(3))], max_norm=1.0)
+    optimizer.grad_norm = torch.ones(())   # (of the step before)
+    optimizer.step()
+    assert optimizer.grad_norm is None
