@@ -1,10 +1,12 @@
 """`AdamW`: a torch.optim.Optimizer over ops.adamw_step, the optimiser of the reference's training script (Adam with clipped
 gradients, train_triton.py:219-259) as a few launches for all parameters of a group.
 
-    AdamW(params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32, stochastic_rounding=True)
+    AdamW(params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32, stochastic_rounding=True, seed=None)
 
 state_bits 8 keeps both moments as e4m3 numbers with an exponent for each 256 of them, 2 bytes a parameter instead of 8.  Those
-are rounded by chance; `stochastic_rounding` says whether parameters of 16 bits are too (of 32 bits they are exact).  `max_norm`
+are rounded by chance; `stochastic_rounding` says whether parameters of 16 bits are too (of 32 bits they are exact).  `seed`, a whole
+number of 64 bits, decides the random numbers: replicas that are to stay alike, as those of data-parallel processes, need the same.
+Without it one is drawn from the generator of the CPU, which `torch.manual_seed` sets, whenever parameters have their first gradient.  `max_norm`
 clips the gradients of all groups by their common norm; it is left in `grad_norm`, a number on the GPU, behind each step.  A saved
 state brings it along, as it does the options of the groups.
 
@@ -29,7 +31,7 @@ def _order(t):
 
 
 class AdamW(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32, stochastic_rounding=True):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32, stochastic_rounding=True, seed=None):
         if isinstance(lr, torch.Tensor):
             if lr.numel() != 1 or lr.dtype != torch.float32:
                 raise ValueError("AdamW: a learning rate in a tensor is one float32 number")
@@ -43,8 +45,10 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: max_norm is not negative, got {max_norm}")
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: states of 8 or 32 bits, got {state_bits}")
+        if seed is not None and not (isinstance(seed, int) and -2 ** 63 <= seed < 2 ** 64):
+            raise ValueError(f"AdamW: a seed is a whole number of 64 bits, got {seed!r}")
         self.max_norm, self.grad_norm = max_norm, None
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, stochastic_rounding=stochastic_rounding))
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, stochastic_rounding=stochastic_rounding, seed=seed))
 
     def __getstate__(self):   # (of copies and pickles)
         return super().__getstate__() | dict(max_norm=self.max_norm, grad_norm=None)
@@ -99,7 +103,7 @@ class AdamW(torch.optim.Optimizer):
             if not self.state[p]:
                 new.setdefault((p.dtype, p.device), []).append(p)
         for (dtype, device), params in new.items():
-            self._begin(params, device, group["state_bits"])
+            self._begin(params, device, group["state_bits"], group.get("seed"))
         for p in group["params"]:
             if p.grad is not None:
                 calls.setdefault((p.dtype, id(self.state[p]["step"])), (group, []))[1].append(p)
@@ -113,17 +117,24 @@ class AdamW(torch.optim.Optimizer):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: some parameters have no gradient that had one in every step so far; take such a step before one is captured")
         first = self.state[params[0]]
-        place = next(i for i, p in enumerate(q for group in self.param_groups for q in group["params"]) if p is params[0])
-        step, seed = first["step"].clone(), first["seed"] * _ODD + (place + 1)   # (another one for each place, as no parameter parts from the same seed twice)
+        step, seed = first["step"].clone(), first["seed"] * _ODD + self._place(params[0])   # (another one for each place, as no parameter parts from the same seed twice)
         for p in params:
             self.state[p]["step"], self.state[p]["seed"] = step, seed
 
-    def _begin(self, params, device, bits):
+    def _place(self, param):
+        """Which of all parameters it is, from one."""
+        return next(i for i, p in enumerate((p for group in self.param_groups for p in group["params"]), 1) if p is param)
+
+    def _begin(self, params, device, bits, seed):
         """States of parameters that have a gradient for the first time: one count of steps and one seed for all of them."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: take a step before one is captured (states that begin inside a graph would begin again at every replay)")
         step = torch.zeros(1, dtype=torch.int64, device=device)
-        seed = torch.randint(-2 ** 63, 2 ** 63 - 1, (1,)).to(device)   # (from the generator of the CPU, which manual_seed sets)
+        if seed is None:
+            seed = torch.randint(-2 ** 63, 2 ** 63 - 1, (1,)).to(device)
+        else:   # (one for each place: sets of parameters that begin apart have numbers apart)
+            number = (seed * _ODD + self._place(params[0])) % 2 ** 64
+            seed = torch.tensor([number - 2 ** 64 if number >= 2 ** 63 else number], device=device)
         for p in params:
             state = self.state[p]
             state["step"], state["seed"] = step, seed

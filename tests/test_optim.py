@@ -635,3 +635,37 @@ def test_a_step_without_gradients_leaves_no_norm():
     optimizer.grad_norm = torch.ones(())   # (of the step before)
     optimizer.step()
     assert optimizer.grad_norm is None
+
+
+@pytest.mark.parametrize("seed", [1.5, "1", 2 ** 64, -2 ** 63 - 1])
+def test_seeds_that_are_refused(seed):
+    with pytest.raises(ValueError, match="seed"):
+        AdamW([torch.nn.Parameter(torch.zeros(3))], seed=seed)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replicas_with_one_seed_stay_together(bits):
+    """Processes that draw other numbers for their data round alike if their optimizers have one seed, which takes nothing from anyone's generator; sets of parameters that begin apart have numbers of their own."""
+    def run(seed, generator):
+        net = model(torch.bfloat16)
+        optimizer = AdamW(net.parameters(), lr=1e-3, state_bits=bits, seed=seed)
+        torch.manual_seed(generator)
+        state = torch.get_rng_state()
+        for k in range(3):
+            for i, p in enumerate(net.parameters()):
+                p.grad = None if k == 0 and i == 2 else torch.full_like(p, 0.1 * (k + 1)).mul_(torch.arange(p.numel(), device=DEV).view(p.shape) % 7 - 3)
+            optimizer.step()
+        assert torch.equal(state, torch.get_rng_state()) == (seed is not None)
+        return net, optimizer
+
+    for seed in (0, 2 ** 64 - 1):
+        (a, first), (b, _) = run(seed, 1), run(seed, 2)
+        assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+        assert len({int(s["seed"]) for s in first.state.values()}) >= 2
+    for other in (run(1, 1)[0], run(None, 1)[0]):
+        assert not all(torch.equal(p, q) for p, q in zip(a.parameters(), other.parameters()))
+    # one seed in a group does not make sets of parameters one: each has its count behind a saved state too
+    again = AdamW(a.parameters(), state_bits=bits)
+    again.load_state_dict(copy.deepcopy(first.state_dict()))
+    assert [int(again.state[p]["step"]) for p in a.parameters()] == [3, 3, 2, 3] and again.param_groups[0]["seed"] == 2 ** 64 - 1
