@@ -163,6 +163,8 @@ def _declare(lib):
     lib.castle_small_linear.argtypes = [vp, vp, vp, i, i, i, i64, i64, i64, i, vp]
     lib.castle_small_linear_fused.restype = i
     lib.castle_small_linear_fused.argtypes = [vp, vp, vp, i, i, i, i64, i64, i64, i, vp, ctypes.c_float, i, vp, i64, vp]
+    lib.castle_gated_state_bytes.restype = i64
+    lib.castle_gated_state_bytes.argtypes = [i, i, i, i]
     lib.castle_rope.restype = i
     lib.castle_rope.argtypes = [_VP, _VP, i, i, i, i, i, i, vp]
 

@@ -391,3 +391,13 @@ def test_refusals_on_the_gpu():
         w.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward(dy)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1000, 40000, 80000, 131072, 190000])
+def test_traced_states_of_more_than_two_gigabytes(rows, dtype):
+    with FakeTensorMode():
+        x, win, wout = (torch.empty(*s, dtype=dtype) for s in ((rows, 64), (2 * 5504, 64), (64, 5504)))
+        state = torch.ops.castle_hip.gated_feed_forward(x, win, wout, 0, True)[1].numel()
+    least = 8 * rows * 5504   # u; or h and 6 bytes of a and b
+    assert least <= state <= 1.03 * least + (1 << 20)
