@@ -4,7 +4,7 @@ what stands between two blocks, the counterparts of the feed-forward block and t
 
 `use_triton` means what it means for `Castle`: None selects the kernels for GPU tensors, False always runs the PyTorch
 formulation.  True runs the kernels wherever they can be used and the formulation elsewhere (other types, autocast, modules with
-hooks).
+hooks, sizes that the kernels do not take).
 """
 from __future__ import annotations
 
@@ -42,7 +42,7 @@ class GatedFeedForward(nn.Module):
     def forward(self, x):
         up, down = self.to_hidden, self.to_out
         if (_native_tensors(self.use_triton, x, up.weight, down.weight) and _unmodified(up, nn.Linear) and _unmodified(down, nn.Linear) and up.bias is None and down.bias is None
-                and x.shape[-1] % 8 == 0 and down.weight.shape[1] % 8 == 0):
+                and ops.gated_sizes_ok(x.numel() // max(x.shape[-1], 1), x.shape[-1], down.weight.shape[1])):
             return ops.gated_feed_forward(x, up.weight, down.weight, self.activation)
         gate, value = up(x).chunk(2, dim=-1)
         return down((F.silu(gate) if self.activation == "silu" else F.gelu(gate)) * value)

@@ -420,6 +420,13 @@ GATE_ACTIVATIONS = {"silu": 0, "gelu": 1}
 RESIDUAL_NORM_MAX_WIDTH = 8192   # CASTLE_RESIDUAL_MAX_WIDTH
 
 
+def gated_sizes_ok(rows: int, dim: int, hidden: int) -> bool:
+    """Whether gated_feed_forward takes `rows` rows of `dim` through `hidden`."""
+    near = lambda n, ld: (n + 192) * ld < 1 << 31   # (castle_gemm_operand_ok)
+    return (0 < dim <= 1 << 20 and 0 < hidden <= 1 << 20 and dim % 8 == 0 and hidden % 8 == 0
+            and near(rows, 2 * hidden) and near(rows, dim) and near(2 * hidden, dim) and near(dim, hidden))
+
+
 def gated_feed_forward(x: torch.Tensor, weight_in: torch.Tensor, weight_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """(act(x G^T) * (x U^T)) weight_out^T: the feed-forward block with a gate, x (..., D), weight_in (2 F, D) the rows of G above those of U, weight_out (D, F);
     the counterpart of nn.Linear, nn.GELU, nn.Linear in train_triton.py:102-107.  activation: "silu" or "gelu" (erf form).

@@ -8,7 +8,7 @@ import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from lookahead_keys_attention_amd import ops
+from lookahead_keys_attention_amd import GatedFeedForward, _native, ops
 
 DEV = "cuda:0"
 gpu = pytest.mark.gpu
@@ -401,3 +401,32 @@ def test_traced_states_of_more_than_two_gigabytes(rows, dtype):
         state = torch.ops.castle_hip.gated_feed_forward(x, win, wout, 0, True)[1].numel()
     least = 8 * rows * 5504   # u; or h and 6 bytes of a and b
     assert least <= state <= 1.03 * least + (1 << 20)
+
+
+def test_limits_of_the_block_are_those_of_the_operator():
+    """`gated_sizes_ok` says what castle_gated_state_bytes does, on both sides of every limit."""
+    last = (1 << 31) // (2 * 5504) - 192   # rows of which (rows + 192) 2 F is about 2^31
+    sizes = [(r, 64, 5504) for r in range(last - 1, last + 3)] + [((1 << 31) // 4096 - 192 + k, 4096, 64) for k in (-1, 0, 1)]
+    sizes += [(8, 1 << 20, 1024 - 96 + 8 * k) for k in range(-2, 3)] + [(8, 1024, (1 << 20) + 8 * k) for k in (-1, 0, 1)] + [(8, 2048 - 192 + 8 * k, 1 << 20) for k in (-1, 0, 1)]
+    sizes += [(8, 12, 8), (8, 8, 12), (8, 0, 8), (8, 8, 0), (1, 8, 8), (1 << 31, 8, 8), ((1 << 27) - 192, 16, 8), ((1 << 27) - 193, 16, 8)]
+    seen = set()
+    for rows, dim, hidden in sizes:
+        ok = _native.lib().castle_gated_state_bytes(rows, dim, hidden, 1) > 0 if rows < 1 << 31 else False
+        assert ops.gated_sizes_ok(rows, dim, hidden) == ok, (rows, dim, hidden)
+        seen.add(ok)
+    assert seen == {True, False} and ops.gated_sizes_ok(0, 8, 8)
+
+
+@gpu
+def test_module_over_more_rows_than_the_operator_takes():
+    """The formulation, whose rows are those of the operator over fewer."""
+    block = GatedFeedForward(8, 5504).to(DEV, torch.bfloat16)
+    rows = (1 << 31) // (2 * 5504)
+    x = torch.randn(rows, 8, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.gated_feed_forward(x, block.to_hidden.weight, block.to_out.weight)
+    with torch.no_grad():
+        y, part = block(x), block(x[-500:])
+    assert y.shape == x.shape
+    off = (y[-500:].float() - part.float()).abs().max() / part.float().abs().max()
+    assert off < 2.0 ** -6   # the formulation rounds both halves, the gate, and what it times: 4 half steps of bf16, and the result
