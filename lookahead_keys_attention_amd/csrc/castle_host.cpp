@@ -1692,6 +1692,10 @@ OptTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor
     changed(params[i]);
     changed(avgs[i]);
     changed(sqs[i]);
+    if (small) {
+      changed((*avg_exponents)[i]);
+      changed((*sq_exponents)[i]);
+    }
   }
   changed(step);
   return max_norm ? norm : OptTensor();

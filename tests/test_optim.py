@@ -669,3 +669,13 @@ def test_replicas_with_one_seed_stay_together(bits):
     again = AdamW(a.parameters(), state_bits=bits)
     again.load_state_dict(copy.deepcopy(first.state_dict()))
     assert [int(again.state[p]["step"]) for p in a.parameters()] == [3, 3, 2, 3] and again.param_groups[0]["seed"] == 2 ** 64 - 1
+
+
+@gpu
+def test_exponents_that_are_written_say_so():
+    (m,), (v,), em, ev = empty_states([(300,)], 8)
+    p, g = tensors([(300,), (300,)], torch.bfloat16, 1, DEV)
+    written = (p, m, v, *em, *ev)
+    before = [t._version for t in written]
+    ops.adamw_step([p], [g], [m], [v], counter(), lr=1e-3, seed=seed_of(), exp_avg_exponents=em, exp_avg_sq_exponents=ev)
+    assert all(t._version > n for t, n in zip(written, before))
