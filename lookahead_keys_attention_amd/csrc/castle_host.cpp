@@ -1641,8 +1641,15 @@ OptTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor
   const c10::DeviceGuard guard(device);
   std::vector<Tensor> keep;
   std::vector<castle_optim_tensor> t(n);
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
-  written.reserve(3 * n);
+  typedef std::pair<uintptr_t, uintptr_t> Range;   // of memory
+  std::vector<Range> written, read;
+  written.reserve((small ? 5 : 3) * n + 1);
+  read.reserve(n + 3);
+  auto note = [](std::vector<Range>& to, const Tensor& w) {   // (all are dense)
+    if (w.numel() == 0) return;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(w.data_ptr());
+    to.emplace_back(at, at + w.numel() * w.element_size());
+  };
   const at::ScalarType state_type = small ? at::kFloat8_e4m3fn : at::kFloat;
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params[i], &m = avgs[i], &v = sqs[i];
@@ -1665,19 +1672,22 @@ OptTensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor
       t[i].exp_avg_sq_exponents = static_cast<int8_t*>(ev.data_ptr());
       if (p.numel() == 0) t[i].exp_avg_exponents = t[i].exp_avg_sq_exponents = reinterpret_cast<int8_t*>(1);   // (nothing is read or written)
     }
-    auto write = [&](const Tensor& w) {
-      if (w.numel() == 0) return;
-      const uintptr_t at = reinterpret_cast<uintptr_t>(w.data_ptr());
-      written.emplace_back(at, at + w.numel() * w.element_size());
-    };
-    for (const Tensor* w : {&p, &m, &v}) write(*w);
+    for (const Tensor* w : {&p, &m, &v}) note(written, *w);
     if (small) {
-      write((*avg_exponents)[i]);
-      write((*sq_exponents)[i]);
+      note(written, (*avg_exponents)[i]);
+      note(written, (*sq_exponents)[i]);
     }
+    note(read, g);
   }
+  note(written, step);
+  for (const OptTensor* r : {&seed, &lr_device, &norm_given})
+    if (*r) note(read, **r);
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i) TORCH_CHECK_VALUE(written[i - 1].second <= written[i].first, "adamw_step: two parameters, states or their exponents share memory");
+  for (const Range& r : read) {
+    const auto behind = std::lower_bound(written.begin(), written.end(), Range(r.second, 0));   // (the first that begins where r ends or later)
+    TORCH_CHECK_VALUE(behind == written.begin() || (behind - 1)->second <= r.first, "adamw_step: a gradient, the seed, or a learning rate or norm in a tensor shares memory with what the step writes");
+  }
   OptTensor norm = norm_given;
   if (max_norm && !norm) norm = at::empty({}, params[0].options().dtype(at::kFloat).requires_grad(false));
   const castle_adamw_options o = {lr, b1, b2, eps, weight_decay, max_norm.value_or(-1), lr_device ? static_cast<const float*>(lr_device->data_ptr()) : nullptr,

@@ -679,3 +679,19 @@ def test_exponents_that_are_written_say_so():
     before = [t._version for t in written]
     ops.adamw_step([p], [g], [m], [v], counter(), lr=1e-3, seed=seed_of(), exp_avg_exponents=em, exp_avg_sq_exponents=ev)
     assert all(t._version > n for t, n in zip(written, before))
+
+
+@gpu
+def test_what_is_read_shares_no_memory_with_what_is_written():
+    flat = torch.zeros(4096, device=DEV)
+    p, g, m, v = (flat[1024 * i:1024 * i + 700] for i in range(4))
+    good = dict(params=[p], grads=[g], exp_avgs=[m], exp_avg_sqs=[v], step=counter(), lr=1e-3)
+    ops.adamw_step(**good)   # (parts of one buffer)
+    number = lambda t, i, dtype: t[i:i + (8 if dtype == torch.int64 else 4) // t.element_size()].view(dtype)
+    for change in (dict(grads=[p]), dict(grads=[m]), dict(grads=[flat[3072 + 100:3072 + 800]]), dict(lr=number(p, 0, torch.float32)), dict(step=number(v, 10, torch.int64)),
+                   dict(seed=number(m, 698, torch.int64)), dict(max_norm=1.0, norm=number(p, 699, torch.float32))):
+        with pytest.raises(ValueError, match="share"):
+            ops.adamw_step(**(good | change))
+    both = counter()
+    with pytest.raises(ValueError, match="share"):
+        ops.adamw_step(**(good | dict(step=both, seed=both)))
