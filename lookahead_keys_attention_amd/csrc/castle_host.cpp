@@ -1365,9 +1365,9 @@ struct GatedCall {
   }
 };
 std::tuple<Tensor, Tensor> gated_op(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t activation, bool keep_state) {
-  require_gpu(x, "gated_feed_forward");
   const c10::DeviceGuard guard(x.device());
   const GatedCall c(x, w_in, w_out, activation);
+  require_gpu(x, "gated_feed_forward");
   Tensor y = at::empty(x.sizes(), x.options());
   if (c.a.rows == 0) return {y, bytes(0, x)};
   const int64_t sbytes = keep_state ? check(castle_gated_state_bytes(c.a.rows, c.a.dim, c.a.hidden, c.dtype), "castle_gated_state_bytes") : 0;
@@ -1491,9 +1491,9 @@ struct ResidualCall {
 Tensor row_numbers(const Tensor& like, int64_t n) { return at::empty({n}, like.options().dtype(at::kFloat)); }
 std::tuple<Tensor, Tensor, Tensor, Tensor> residual_norm_op(const Tensor& x, const Tensor& residual, const OptTensor& w, const OptTensor& scale, const OptTensor& gate, const OptTensor& next,
                                                             double eps, bool keep) {
-  require_gpu(x, "residual_norm");
   const c10::DeviceGuard guard(x.device());
   ResidualCall c(x, residual, w, scale, gate, next, eps);
+  require_gpu(x, "residual_norm");
   const int64_t R = c.a.rows;
   Tensor y = at::empty(x.sizes(), x.options()), h = next ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
   Tensor rstd = row_numbers(x, keep && w ? R : 0), next_rstd = row_numbers(x, keep && next ? R : 0);

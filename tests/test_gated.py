@@ -430,3 +430,26 @@ def test_module_over_more_rows_than_the_operator_takes():
     assert y.shape == x.shape
     off = (y[-500:].float() - part.float()).abs().max() / part.float().abs().max()
     assert off < 2.0 ** -6   # the formulation rounds both halves, the gate, and what it times: 4 half steps of bf16, and the result
+
+
+@pytest.mark.parametrize("change, error, what", [
+    (dict(x=torch.zeros(2, 24)), ValueError, "x is"),                            # another width
+    (dict(win=torch.zeros(24, 16)), ValueError, "x is"),                         # not twice the hidden width
+    (dict(wout=torch.zeros(8, 16)), ValueError, "x is"),
+    (dict(win=torch.zeros(32, 16, 1)), ValueError, "x is"),
+    (dict(x=torch.zeros(())), ValueError, "x is"),
+    (dict(x=torch.zeros(2, 12), win=torch.zeros(32, 12), wout=torch.zeros(12, 16)), ValueError, "multiples of 8"),
+    (dict(win=torch.zeros(24, 16), wout=torch.zeros(16, 12)), ValueError, "multiples of 8"),
+    (dict(win=torch.zeros(0, 16), wout=torch.zeros(16, 0)), ValueError, "multiples of 8"),
+    (dict(x=torch.zeros(2, 0), win=torch.zeros(32, 0), wout=torch.zeros(0, 16)), ValueError, "multiples of 8"),
+    (dict(wout=torch.zeros(16, 16, dtype=torch.bfloat16)), ValueError, "one type"),
+    (dict(x=torch.zeros(1, 16).expand(1 << 27, 16)), ValueError, "less than 2\\^31 elements"),
+    (dict(x=torch.zeros(2, 16, dtype=torch.float64), win=torch.zeros(32, 16, dtype=torch.float64), wout=torch.zeros(16, 16, dtype=torch.float64)), TypeError, "float64|double|Double"),
+    (dict(), RuntimeError, "on the GPU"),
+])
+def test_each_refusal_by_its_message(change, error, what):
+    """What is wrong with the sizes is said of tensors on the CPU too."""
+    args = dict(x=torch.zeros(2, 16), win=torch.zeros(32, 16), wout=torch.zeros(16, 16)) | change
+    with pytest.raises(error, match=what) as refused:
+        ops.gated_feed_forward(args["x"], args["win"], args["wout"])
+    assert type(refused.value) is error

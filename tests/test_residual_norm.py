@@ -283,3 +283,23 @@ def test_a_recorded_backward_pass_beside_one_that_lives_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+@pytest.mark.parametrize("change, error, what", [
+    (dict(residual=torch.zeros(2, 3, 8)), ValueError, "one shape"), (dict(residual=torch.zeros(1, 3, 16)), ValueError, "one shape"), (dict(x=torch.zeros(()), residual=torch.zeros(())), ValueError, "one shape"),
+    (dict(weight=torch.zeros(8)), ValueError, "columns"), (dict(scale=torch.zeros(1, 16)), ValueError, "columns"), (dict(next_weight=torch.zeros(17)), ValueError, "columns"),
+    (dict(next_weight=torch.zeros(16, dtype=torch.float16)), ValueError, "one type"), (dict(gate=torch.zeros(2, 3, 16).half()), ValueError, "one type"),
+    (dict(residual=torch.zeros(2, 3, 16).half()), ValueError, "one type"),
+    (dict(gate=torch.zeros(1, 3, 16)), ValueError, "gate"), (dict(gate=torch.zeros(3, 16)), ValueError, "gate"), (dict(gate=torch.zeros(2, 3, 1)), ValueError, "gate"),
+    (dict(gate=torch.zeros(3, 1, 16)), ValueError, "gate"), (dict(gate=torch.zeros(8)), ValueError, "gate"),
+    (dict(eps=-1.0), ValueError, "eps"), (dict(eps=float("nan")), ValueError, "eps"),
+    (dict(x=torch.zeros(2, 8193), residual=torch.zeros(2, 8193)), ValueError, "8192"), (dict(x=torch.zeros(2, 0), residual=torch.zeros(2, 0)), ValueError, "8192"),
+    (dict(x=torch.zeros(2, 16).double(), residual=torch.zeros(2, 16).double()), TypeError, "double|Double|float64"),
+    (dict(), RuntimeError, "on the GPU"),
+])
+def test_each_refusal_by_its_message(change, error, what):
+    """What is wrong with the sizes is said of tensors on the CPU too."""
+    args = dict(x=torch.zeros(2, 3, 16), residual=torch.zeros(2, 3, 16)) | change
+    with pytest.raises(error, match=what) as refused:
+        ops.residual_norm(**args)
+    assert type(refused.value) is error
