@@ -209,8 +209,13 @@ class GraphedDecoder:
         self.counters.copy_(torch.tensor([self.length, self.base0], dtype=torch.int32), non_blocking=False)
 
     def _signature(self):
-        """What the captured graph has baked in: the scale of the embedding, the addresses of the weights it reads."""
-        return (self.model.embedding_scale, *(p.data_ptr() for p in self.model.parameters()))
+        """What the captured graph has baked in: the scale of the embedding, the addresses of the weights it reads, what its gated blocks and branches do with them."""
+        model, parts = self.model, []
+        if model.gated:
+            parts += [m for _, feed_forward in model.layers for m in feed_forward.modules()]
+        if model.has_branches:
+            parts += [model.first_norm, *model.next_norms, model.final_norm, *(m for branch in model.branches for m in (branch, branch.norm))]
+        return (model.embedding_scale, *(getattr(m, name, None) for m in parts for name in ("activation", "use_triton", "eps")), *(p.data_ptr() for p in model.parameters()))
 
     def fits(self, caches, max_len: int) -> bool:
         """True if `load(caches)` can reuse this graph for a generation of up to max_len rows."""

@@ -249,3 +249,30 @@ def test_a_training_step_of_all_of_it(bits):
         torch.cuda.synchronize()
         assert abs(float(loss.detach()) - float(want)) <= 10 * 2.0 ** -9 * float(want)
         assert all(torch.equal(p, q) for p, q in zip(params, after))
+
+
+@gpu
+@pytest.mark.parametrize("kind", [dict(gated=True), dict(gated=True, post_norm=True)])
+def test_a_kept_decoder_and_another_gate(kind):
+    """What a graph of a token step has recorded and a module may change: tokens are those of the modules as they are."""
+    native, _ = models(kind)
+    prompt = torch.randint(0, 96, (4, 12), device=DEV)
+    first = native.sample(prompt, 40, temperature=0, graph=True)
+    for _, feed_forward in native.layers:
+        feed_forward[-1].activation = "gelu"
+        feed_forward[-1].to_out.weight.data.mul_(4)   # (so that the gate decides tokens)
+    want = native.sample(prompt, 40, temperature=0, graph=False)
+    kept = native._kept_decoder
+    assert torch.equal(native.sample(prompt, 40, temperature=0, graph=True), want)
+    assert native._kept_decoder is not kept and not torch.equal(first, want)
+    kept = native._kept_decoder
+    native.sample(prompt, 40, temperature=0, graph=True)
+    assert native._kept_decoder is kept
+    native.layers[0][1][-1].use_triton = False
+    native.sample(prompt, 40, temperature=0, graph=True)
+    assert native._kept_decoder is not kept
+    if kind.get("post_norm"):
+        kept = native._kept_decoder
+        native.next_norms[0].eps = 1.0
+        assert torch.equal(native.sample(prompt, 40, temperature=0, graph=True), native.sample(prompt, 40, temperature=0, graph=False))
+        assert native._kept_decoder is not kept
