@@ -177,8 +177,9 @@ struct BwdKernelArgs {
   float* parts;       // [workgroup][2][D]: P and the sums of dnext
   float* unit_sums;   // [unit][D], or nullptr: a unit has a whole span
 };
-// GATES: 0 none, 1 each row one of its own, 2 one of several rows
-template <typename T, typename L, int GATES> __global__ __launch_bounds__(L::kBlock, L::kWavesPerSimd) void residual_bwd_kernel(BwdKernelArgs k) {
+// GATES: 0 none, 1 each row one of its own, 2 one of several rows.  BOTH: there are a norm of x and a gradient of h.  Without one of them its terms are left out, not multiplied by a zero: what the row
+// holds may be infinite or NaN.  (By itself: the conditions cost the other one registers.)
+template <typename T, typename L, int GATES, bool BOTH> __global__ __launch_bounds__(L::kBlock, L::kWavesPerSimd) void residual_bwd_kernel(BwdKernelArgs k) {
   const ResidualBwdArgs& b = k.b;
   const ResidualArgs& a = b.f;
   __shared__ float s[8 * L::WPR];
@@ -192,6 +193,7 @@ template <typename T, typename L, int GATES> __global__ __launch_bounds__(L::kBl
 #pragma unroll
   for (int p = 0; p < L::NP; ++p) sum_p[p] = sum_next[p] = vf{};
   const float per = 1.f / (float)a.D;
+  const bool with_x = BOTH || a.w != nullptr, with_h = BOTH || b.dh != nullptr;
   const int64_t step = (int64_t)gridDim.x * L::kRows;
   // a row of a unit; rows are requested one ahead
   struct Place { int64_t unit, row, last; };
@@ -217,8 +219,8 @@ template <typename T, typename L, int GATES> __global__ __launch_bounds__(L::kBl
       if (b.dh != nullptr) f.dh[p] = read8(static_cast<const T*>(b.dh) + at + i, left);
       if constexpr (GATES == 1) f.g[p] = read8(static_cast<const T*>(a.gate) + at + i, left);
     }
-    f.inv = a.w != nullptr ? a.rstd[row] : 1.f;
-    f.inv_y = b.dh != nullptr ? a.next_rstd[row] : 0.f;
+    f.inv = with_x ? a.rstd[row] : 1.f;
+    f.inv_y = with_h ? a.next_rstd[row] : 0.f;
     return f;
   };
   Place now = {(int64_t)blockIdx.x * L::kRows + row_of_lane<L>(), 0, 0};
@@ -266,7 +268,7 @@ template <typename T, typename L, int GATES> __global__ __launch_bounds__(L::kBl
       }
     }
     row_sums<L>(sum, s, turn);
-    const float m2 = sum[0] * per, m1 = a.w != nullptr ? (sum[1] + f.inv_y * (sum[2] - m2 * sum[3])) * per : 0.f;
+    const float m2 = sum[0] * per, m1 = (with_h ? sum[1] + f.inv_y * (sum[2] - m2 * sum[3]) : sum[1]) * per;
 #pragma unroll
     for (int p = 0; p < L::NP; ++p) {
       const int i = 8 * (p * TPR + sub), left = a.D - i;
@@ -274,13 +276,15 @@ template <typename T, typename L, int GATES> __global__ __launch_bounds__(L::kBl
       vf cg = c[p];
       if constexpr (GATES != 0) cg *= wide<T>(g[p]);
       const vf yh = (wide<T>(f.r[p]) + xh * cg) * f.inv_y, dhp = wide<T>(f.dh[p]), dn = dhp * wide<T>(next_w[p]);
-      const vf d = wide<T>(f.dy[p]) + (dn - yh * m2) * f.inv_y, t = d * xh;
+      vf d = wide<T>(f.dy[p]);
+      if (with_h) d += (dn - yh * m2) * f.inv_y;
+      const vf t = d * xh;
       sum_next[p] += dhp * yh;
       if constexpr (GATES == 2) sum_unit[p] += t;
       else if constexpr (GATES == 1) sum_p[p] += t * wide<T>(g[p]);
       else sum_p[p] += t;
       if (b.dresidual != nullptr) write8<T>(static_cast<T*>(b.dresidual) + at + i, d, left);
-      if (b.dx != nullptr) write8<T>(static_cast<T*>(b.dx) + at + i, (d * cg - xh * m1) * f.inv, left);
+      if (b.dx != nullptr) write8<T>(static_cast<T*>(b.dx) + at + i, with_x ? (d * cg - xh * m1) * f.inv : d * cg, left);
       if constexpr (GATES == 1)
         if (b.dgate != nullptr) write8<T>(static_cast<T*>(b.dgate) + at + i, t * c[p], left);
       if constexpr (GATES == 2)
@@ -441,10 +445,14 @@ int launch_residual_bwd(const ResidualBwdArgs& b, int dtype, void* workspace, hi
       using L = decltype(l);
       const size_t lds = L::WPR == 1 && with_columns ? 2 * (size_t)b.f.D * 4 : 0;
       const dim3 grid(groups), block(L::kBlock);
-      if (b.f.gate == nullptr) hipLaunchKernelGGL((residual_bwd_kernel<T, L, 0>), grid, block, lds, stream, k);
-      else if (b.f.span == 1) hipLaunchKernelGGL((residual_bwd_kernel<T, L, 1>), grid, block, lds, stream, k);
-      else hipLaunchKernelGGL((residual_bwd_kernel<T, L, 2>), grid, block, lds, stream, k);
-      return hipGetLastError() == hipSuccess ? 0 : -3;
+      auto go = [&](auto both_) {
+        constexpr bool BOTH = decltype(both_)::value;
+        if (b.f.gate == nullptr) hipLaunchKernelGGL((residual_bwd_kernel<T, L, 0, BOTH>), grid, block, lds, stream, k);
+        else if (b.f.span == 1) hipLaunchKernelGGL((residual_bwd_kernel<T, L, 1, BOTH>), grid, block, lds, stream, k);
+        else hipLaunchKernelGGL((residual_bwd_kernel<T, L, 2, BOTH>), grid, block, lds, stream, k);
+        return hipGetLastError() == hipSuccess ? 0 : -3;
+      };
+      return b.f.w != nullptr && b.dh != nullptr ? go(std::true_type()) : go(std::false_type());
     });
   });
   if (rc != 0 || (!with_columns && !with_units)) return rc;

@@ -303,3 +303,34 @@ def test_each_refusal_by_its_message(change, error, what):
     with pytest.raises(error, match=what) as refused:
         ops.residual_norm(**args)
     assert type(refused.value) is error
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [24, 200, 700, 1500, 3000, 6000])
+@pytest.mark.parametrize("gate", [None, "each", "shared"])
+def test_gradients_do_not_meet_what_they_do_not_depend_on(gate, D, dtype):
+    """Without a norm behind the block the gradients of x and of the residual are those of finite numbers whatever x and the residual hold, as those of x are with one whatever the residual holds and those of the residual
+    whatever x holds; rows of zeros as gradients have zeros as theirs."""
+    shape = (3, 4, D)
+    bad = [float("inf"), float("nan"), -float("inf")]
+    for without in (("weight", "next_weight"), ("next_weight",), ("weight",), ()):
+        t, dy, _ = inputs(shape, dtype, {None: None, "each": shape, "shared": (3, 1, D)}[gate], without)
+        dy = dy.to(DEV)
+        dy[2, 1] = 0
+
+        def grads(change):
+            leaves = {k: None if v is None else v.to(DEV).clone() for k, v in t.items()}
+            for name in change:
+                for i, b in enumerate(bad):
+                    leaves[name][i, 1, 5 * i] = b
+            leaves = {k: None if v is None else v.requires_grad_() for k, v in leaves.items()}
+            out = call(leaves)
+            y = out if torch.is_tensor(out) else out[0]   # (no gradient of the norm in front of the next block)
+            return torch.autograd.grad(y, (leaves["x"], leaves["residual"]), dy)
+
+        clean = grads(())
+        for change in (("residual",),) if t["weight"] is not None else (("residual",), ("x",), ("x", "residual")):
+            for a, b, name in zip(grads(change), clean, ("x", "residual")):
+                assert torch.equal(a, b), (without, change, name)
+        assert torch.equal(grads(("x",))[1], dy) and torch.equal(clean[1], dy) and not clean[0][2, 1].any()
