@@ -473,7 +473,7 @@ template <typename T, int ACT, int MT, int NT> __global__ __launch_bounds__(64 *
       if (a.low) static_cast<T*>(a.out)[(int64_t)(a.R + row) * a.N + n] = (T)rest<T>(h);
     } else {
       float v = sum(row, col);
-      if (a.out_R < a.R) v += sum(a.out_R + row, col);
+      if (a.out_R < a.R && __builtin_isfinite(v)) v += sum(a.out_R + row, col);   // (else the rest, zeros, may have met an infinity of the weights)
       if (a.part != nullptr) a.part[((int64_t)blockIdx.y * a.out_R + row) * a.N + n] = v;
       else static_cast<T*>(a.out)[(int64_t)row * a.N + n] = (T)v;
     }
@@ -537,6 +537,7 @@ int launch_rows(const void* x, int64_t ld_x, const void* w, int64_t ld_w, void* 
 // ---- 16-bit types, few numbers ---------------------------------------------------------------------------------------
 // Products of an operand in two parts, rounded and what that has left, with one in one: tiles of 32 x 32, four waves that take steps of 16 of the contraction in turns, straight from memory (16 bytes
 // where the contraction is contiguous, else element by element, whose lanes lie side by side), in ranges that fill the card, summed in a launch of their own.
+// What has left nothing is a zero, and makes a NaN of an infinity of the other operand.  So where sums are not finite, those of the rounded part alone count, formed again.
 struct PartsJob {
   const void *a, *low, *b;   // a and low [M][lda] or [K][lda], b [N][ldb] or [K][ldb]
   int64_t lda, ldb, cm, cn;  // element (m, n) of c at m cm + n cn; one of them is 1
@@ -588,18 +589,17 @@ template <typename T, bool AKC, bool BKC> __device__ __forceinline__ void parts_
   const int k_end = min(j.K, (range + 1) * j.k_per_range), step = shared ? 16 * kPartsWaves : 16;
   const T *a = static_cast<const T*>(j.a) + (AKC ? m * j.lda : m), *low = static_cast<const T*>(j.low) + (AKC ? m * j.lda : m), *b = static_cast<const T*>(j.b) + (BKC ? n * j.ldb : n);
   acc_t acc;   // [n rows, m lanes]
-  zero(acc);
-  int k = range * j.k_per_range + (shared ? 16 * wave : 0);
-  auto steps = [&](auto u_, auto last_) __attribute__((always_inline)) {
+  int k;
+  auto steps = [&](auto u_, auto last_, auto both_) __attribute__((always_inline)) {
     constexpr int N = decltype(u_)::value;
-    constexpr bool LAST = decltype(last_)::value;
+    constexpr bool LAST = decltype(last_)::value, BOTH = decltype(both_)::value;
     PartsPiece<T, AKC> pa[N], pl[N];
     PartsPiece<T, BKC> pb[N];
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const int at = k + step * u + 8 * g;
       pa[u].template load<LAST>(a, j.lda, at, k_end);
-      pl[u].template load<LAST>(low, j.lda, at, k_end);
+      if constexpr (BOTH) pl[u].template load<LAST>(low, j.lda, at, k_end);
       pb[u].template load<LAST>(b, j.ldb, at, k_end);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -607,14 +607,28 @@ template <typename T, bool AKC, bool BKC> __device__ __forceinline__ void parts_
     for (int u = 0; u < N; ++u) {
       const int at = k + step * u + 8 * g;
       const frag<T> fb = pb[u].template get<LAST>(at, k_end);
-      mma(acc, fb, pl[u].template get<LAST>(at, k_end));
+      if constexpr (BOTH) mma(acc, fb, pl[u].template get<LAST>(at, k_end));
       mma(acc, fb, pa[u].template get<LAST>(at, k_end));
     }
     k += step * N;
   };
-  while (k + step * (U - 1) + 16 <= k_end) steps(std::integral_constant<int, U>(), std::false_type());
-  while (k < k_end) steps(std::integral_constant<int, 2>(), std::true_type());
-  settle();
+  auto sums = [&](auto both) __attribute__((always_inline)) {
+    zero(acc);
+    k = range * j.k_per_range + (shared ? 16 * wave : 0);
+    while (k + step * (U - 1) + 16 <= k_end) steps(std::integral_constant<int, U>(), std::false_type(), both);
+    while (k < k_end) steps(std::integral_constant<int, 2>(), std::true_type(), both);
+    settle();
+  };
+  sums(std::true_type());
+  float most = 0.f;   // NaN where something is not finite
+#pragma unroll
+  for (int r = 0; r < 16; ++r) most += 0.f * acc[r];
+  if (__ballot(most != 0.f) != 0) {
+    const acc_t both = acc;
+    sums(std::false_type());
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = __builtin_isfinite((float)both[r]) ? both[r] : acc[r];
+  }
   auto store = [&](const vec<float, 4>& x, int q) __attribute__((always_inline)) {
     const int64_t row = m0 + c, col = n0 + 8 * q + 4 * g, at = row * j.cm + col * j.cn;
     if (row >= j.M || col >= j.N) return;   // (columns are multiples of 8)

@@ -453,3 +453,26 @@ def test_each_refusal_by_its_message(change, error, what):
     with pytest.raises(error, match=what) as refused:
         ops.gated_feed_forward(args["x"], args["win"], args["wout"])
     assert type(refused.value) is error
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R, D, F", [(3, 64, 72), (33, 64, 56), (40, 24, 200), (300, 16, 24), (70, 64, 72)])
+def test_infinities_of_weights_and_gradients(R, D, F, dtype):
+    """An infinite weight or gradient meets what the rounding of a hidden number has left, zero where nothing has: results are infinite where the formula's are, and NaN where those are."""
+    x, win, wout, dy = inputs(R, D, F, dtype, seed=R)
+    wout[3, 5], dy[1, 7] = float("inf"), -float("inf")
+    for changed in ((x, win, wout, dy.clamp(-3, 3)), (x, win, wout.clamp(-3, 3), dy)):
+        got = run(*changed, "silu")
+        with torch.no_grad():
+            got["y of tokens"] = ops.gated_feed_forward(*(t.to(DEV) for t in changed[:3]))
+        a, b, c, d = (t.double() for t in changed)
+        g, v = (a @ b.T).chunk(2, 1)
+        act, slope = act_of(g, "silu")
+        h, dh = act * v, d @ c
+        du = torch.cat((dh * (v * slope), dh * act), 1)
+        want = {"y": h @ c.T, "y of tokens": h @ c.T, "dx": du @ b, "dwin": du.T @ a, "dwout": d.T @ h}
+        for name, value in want.items():
+            here = got[name].detach().cpu().double()
+            assert torch.equal(here.isnan(), value.isnan()), name
+            assert torch.equal(here.isinf(), value.isinf()) and torch.equal(here[here.isinf()], value[value.isinf()]), name
