@@ -62,7 +62,8 @@ class ResidualBranch(nn.Module):
     def forward(self, x, residual, next_norm):
         norm = self.norm
         width = x.shape[-1]
-        if (_norm_of_rows(next_norm, width) and (norm is None or _norm_of_rows(norm, width) and norm.eps == next_norm.eps) and width <= ops.RESIDUAL_NORM_MAX_WIDTH
+        if (_norm_of_rows(next_norm, width) and (norm is None or _norm_of_rows(norm, width) and norm.eps == next_norm.eps) and x.shape == residual.shape and width <= ops.RESIDUAL_NORM_MAX_WIDTH
+                and (self.scale is None or self.scale.shape == (width,))
                 and _native_tensors(self.use_triton, x, residual, None if norm is None else norm.weight, self.scale, next_norm.weight)):
             return ops.residual_norm(x, residual, weight=None if norm is None else norm.weight, scale=self.scale, next_weight=next_norm.weight, eps=next_norm.eps)
         if norm is not None:

@@ -276,3 +276,17 @@ def test_a_kept_decoder_and_another_gate(kind):
         native.next_norms[0].eps = 1.0
         assert torch.equal(native.sample(prompt, 40, temperature=0, graph=True), native.sample(prompt, 40, temperature=0, graph=False))
         assert native._kept_decoder is not kept
+
+
+@gpu
+def test_branches_whose_sums_are_broadcast():
+    """Shapes that only add up by broadcasting: the formulation."""
+    branch, norm = ResidualBranch(24, True, 0.3, use_triton=True).to(DEV), torch.nn.RMSNorm(24).to(DEV)
+    x, r = torch.randn(3, 5, 24, device=DEV), torch.randn(1, 5, 24, device=DEV)
+    for a, b in ((x, r), (r, x), (x, r[0, 0])):
+        y, h = branch(a, b, norm)
+        want = b + 0.3 * F.rms_norm(a, (24,))
+        near(y, want, 1e-6, "sum")
+        near(h, F.rms_norm(want, (24,)), 1e-5, "norm")
+    branch.scale = torch.nn.Parameter(torch.full((1,), 0.5, device=DEV))   # (one number for all columns)
+    near(branch(x, x, norm)[0], x + 0.5 * F.rms_norm(x, (24,)), 1e-6, "sum")
