@@ -11,15 +11,16 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 from torch import nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import _native, ops
 from .castle import _unmodified
 
 
 def _native_tensors(use_triton, *tensors) -> bool:
-    """True if the kernels may take these tensors: on one GPU, of one type that they have, nothing that casts in between."""
+    """True if the kernels may take these tensors: on one GPU, of one type that they have, nothing that casts in between and no hooks on all modules."""
     first = tensors[0]
-    return (use_triton is not False and first.is_cuda and first.dtype in _native.DTYPE_CODES and _native.is_built() and not torch.is_autocast_enabled("cuda")
+    return (use_triton is not False and first.is_cuda and first.dtype in _native.DTYPE_CODES and _native.is_built() and not torch.is_autocast_enabled("cuda") and not _has_any_global_hook()
             and all(t is None or t.dtype == first.dtype and t.device == first.device for t in tensors))
 
 

@@ -32,7 +32,6 @@ import math
 import torch
 import torch.nn.functional as F
 from torch import nn
-from torch.nn.modules.module import _has_any_global_hook
 
 from . import _native, ops
 from .blocks import GatedFeedForward, ResidualBranch, _native_tensors
@@ -368,7 +367,7 @@ class CastleLM(nn.Module):
             n = None   # (the norm goes with the projection)
         to_logits = self.to_logits
         # (models without the newer blocks come here for their hooks, and keep their logits)
-        if (return_loss and native and (self.gated or n is not None) and _unmodified(to_logits, nn.Linear) and to_logits.bias is None and not _has_any_global_hook()
+        if (return_loss and native and (self.gated or n is not None) and _unmodified(to_logits, nn.Linear) and to_logits.bias is None
                 and _native_tensors(None, h, to_logits.weight) and linear_loss_is_ahead(target.numel(), to_logits.weight)):
             return ops.linear_cross_entropy(self.final_norm(h) if n is None else n, to_logits.weight, target)
         logits = Castle._project(to_logits, h if n is None else n, token_step, norm=self.final_norm if n is None else None, native=native)

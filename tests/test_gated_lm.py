@@ -290,3 +290,18 @@ def test_branches_whose_sums_are_broadcast():
         near(h, F.rms_norm(want, (24,)), 1e-5, "norm")
     branch.scale = torch.nn.Parameter(torch.full((1,), 0.5, device=DEV))   # (one number for all columns)
     near(branch(x, x, norm)[0], x + 0.5 * F.rms_norm(x, (24,)), 1e-6, "sum")
+
+
+@gpu
+def test_hooks_on_all_modules_see_those_of_blocks_and_branches():
+    block, branch, norm = GatedFeedForward(24, 40, use_triton=True).to(DEV), ResidualBranch(24, True, 0.3, use_triton=True).to(DEV), torch.nn.RMSNorm(24).to(DEV)
+    x, seen = torch.randn(3, 5, 24, device=DEV), []
+    want = branch(block(x), x, norm)
+    hook = torch.nn.modules.module.register_module_forward_hook(lambda module, *_: seen.append(module))
+    try:
+        got = branch(block(x), x, norm)
+    finally:
+        hook.remove()
+    assert {id(m) for m in seen} == {id(m) for m in (block, block.to_hidden, block.to_out, branch, branch.norm, norm)}
+    for a, b in zip(got, want):
+        near(a, b, 1e-4, "with hooks")
