@@ -110,12 +110,13 @@ class AdamW(torch.optim.Optimizer):
         for (_, count), (_, params) in calls.items():
             if count in paused:
                 self._part(params)
+            paused.add(count)   # (each call counts: of two types that began as one, the second goes its own way)
         return list(calls.values())
 
     def _part(self, params):
         """Parameters that go on without others of their count: from here on they have one of their own, and a seed."""
         if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: some parameters have no gradient that had one in every step so far; take such a step before one is captured")
+            raise RuntimeError("AdamW: some parameters have no gradient, or another type, that were in one call with others so far; take such a step before one is captured")
         first = self.state[params[0]]
         step, seed = first["step"].clone(), first["seed"] * _ODD + self._place(params[0])   # (another one for each place, as no parameter parts from the same seed twice)
         for p in params:
@@ -174,7 +175,7 @@ class AdamW(torch.optim.Optimizer):
                     state[key].view(same).copy_(value.view(same))
                 elif key in ("step", "seed"):
                     number = int(value)
-                    state[key] = (key, number, p.device)
+                    state[key] = (key, number, p.device, p.dtype)
                 else:
                     state[key] = value.to(device=p.device, copy=True)
             begun = (state["step"], state["seed"])

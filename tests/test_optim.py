@@ -695,3 +695,28 @@ def test_what_is_read_shares_no_memory_with_what_is_written():
     both = counter()
     with pytest.raises(ValueError, match="share"):
         ops.adamw_step(**(good | dict(step=both, seed=both)))
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_of_a_count_that_change_their_type(bits):
+    """Parameters that began together and are of two types later, as their module or a saved state has it: two calls, of which each counts once."""
+    def step(net, optimizer):
+        for p in net.parameters():
+            p.grad = torch.ones_like(p)
+        optimizer.step()
+
+    make = lambda: torch.nn.ModuleList(torch.nn.Linear(16, 16, device=DEV) for _ in range(2))
+    net = make()
+    optimizer = AdamW(net.parameters(), state_bits=bits)
+    step(net, optimizer)
+    saved = copy.deepcopy(optimizer.state_dict())
+    net[1].bfloat16()
+    other = make()
+    other[1].bfloat16()
+    again = AdamW(other.parameters(), state_bits=bits)
+    again.load_state_dict(saved)
+    for n, o in ((net, optimizer), (other, again)):
+        for k in range(2):
+            step(n, o)
+            assert [int(o.state[p]["step"]) for p in n.parameters()] == [2 + k] * 4
