@@ -346,7 +346,7 @@ template <typename T, int MODE, int ACT, int BM, bool END, bool LOW = false> int
 }
 // Few numbers, 16-bit types: where h and [dg dv] alone are rounded on the way, results are 1.4 times as far from the formula as results rounded once, and of a few hundred numbers now and then twice as
 // far.  There what the roundings leave takes part in the products too, and launches bound them as before (backward pass, us, rounded / in parts: 8 rows of 24 through 192 13.2 / 10.5, 5770 of 16 through 24
-// 19.4 / 15.1, 40 of 96 through 4000 20.7 / 18.5; 1 of 1904 through 5048 51 / 61, whose gradients of 2 x 38 MB are written in pieces of 16 bytes).
+// 19.4 / 15.1, 40 of 96 through 4000 20.7 / 18.5; 1 of 1904 through 5048 51 / 61, whose gradients of 2 x 38 MB are written in pieces of 16 bytes.  Of that the look for what is not finite is 0.1 to 0.7).
 bool few_numbers(int R, int D, int F) { return std::min({(int64_t)R * D, (int64_t)D * F, (int64_t)R * F}) < 4096; }
 // Rows of a tile: those with which the fullest CU is done first (us a step of the contraction, and at a tile's end); of both passes, which share the order of a and b.
 int tile_rows(int R, int D, int F) {

@@ -7,12 +7,13 @@
 // range is half of v's in octaves.  They are rounded up or down by chance, so that the mean is kept.  To the nearest, a state would stay where it is: a step with b2 = 0.999 moves r by
 // 0.05 %, steps of e4m3 are 6 to 12 %.  A second moment that is not zero stays above zero (2^-18 of the largest): as zero its element would move by lr m / eps.  16-bit
 // parameters are rounded by chance too where there is a seed: lr = 1e-4 moves none of bf16 to the nearest.
-// Every number is formed by single 32-bit operations, rounded each (no contraction), in the order of the formulas.
+// Numbers are formed by single 32-bit operations, rounded each (no contraction), in the order of the formulas; the quotient of a step is off by an ulp or two, and so are roots but for those of 8-bit
+// states beside 32-bit parameters.
 //
 // Bound by HBM: per element of 16 bits 10 bytes with states of 8 bits, 22 with 32, 28 of fp32, and the gradients once more for their norm, which has to be there before the first element.
 // us and TB/s: 65M bf16 numbers with states of 32 bits 267 and 5.3, the norm before 42 and 3.1 (of gradients that no writes precede 28 and 4.6); 318M with states of 8 bits 654 and 4.9, where a
 // quarter of the time is instructions (Philox, exponents, e4m3 and back), the norm 142 and 4.5; 2.1M of fp32 12.4, the norm and its join 8.
-// Tensors go 64 to a launch, their addresses in its arguments: a table in memory would have to be written anew for every step, as gradients move.
+// Tensors go 64 to a launch of the step and 192 to one of the norm, their addresses in its arguments: a table in memory would have to be written anew for every step, as gradients move.
 #include "castle_tiles.h"
 #include "castle_dispatch.h"
 #include "castle_optim.h"
@@ -40,7 +41,7 @@ static_assert(sizeof(LaunchTensors) + 64 <= 4096, "arguments of a launch");
 __device__ __forceinline__ int tensor_of(const LaunchTensors& a, uint32_t piece) {
   const int i = min(lane_id(), a.count - 1);
   const uint64_t begun = __ballot(lane_id() < a.count && a.first[i] <= piece);
-  return 63 - __builtin_clzll(begun);   // (sizes of zero are left out on the host, so firsts grow)
+  return 63 - __builtin_clzll(begun);   // (one without elements has a piece too, so firsts grow)
 }
 
 template <typename T> __device__ __forceinline__ vec<T, 8> raw8(const T* p, int left) {
