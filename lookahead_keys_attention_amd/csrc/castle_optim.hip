@@ -11,7 +11,7 @@
 // states beside 32-bit parameters.
 //
 // Bound by HBM: per element of 16 bits 10 bytes with states of 8 bits, 22 with 32, 28 of fp32, and the gradients once more for their norm, which has to be there before the first element.
-// us and TB/s: 65M bf16 numbers with states of 32 bits 267 and 5.3, the norm before 42 and 3.1 (of gradients that no writes precede 28 and 4.6); 318M with states of 8 bits 654 and 4.9, where a
+// us and TB/s: 65M bf16 numbers with states of 32 bits 267 and 5.3, the norm before 42 and 3.1 (of gradients that no writes precede 28 and 4.6); 318M with states of 8 bits 665 and 4.8, where a
 // quarter of the time is instructions (Philox, exponents, e4m3 and back), the norm 142 and 4.5; 2.1M of fp32 12.4, the norm and its join 8.
 // Tensors go 64 to a launch of the step and 192 to one of the norm, their addresses in its arguments: a table in memory would have to be written anew for every step, as gradients move.
 #include "castle_tiles.h"
