@@ -17,6 +17,8 @@ have paused since, it is recorded again.
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import ops
@@ -45,8 +47,10 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: max_norm is not negative, got {max_norm}")
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: states of 8 or 32 bits, got {state_bits}")
-        if seed is not None and not (isinstance(seed, int) and -2 ** 63 <= seed < 2 ** 64):
-            raise ValueError(f"AdamW: a seed is a whole number of 64 bits, got {seed!r}")
+        if seed is not None:
+            if not hasattr(type(seed), "__index__") or isinstance(seed, torch.Tensor) or not -2 ** 63 <= (number := operator.index(seed)) < 2 ** 64:
+                raise ValueError(f"AdamW: a seed is a whole number of 64 bits, got {seed!r}")
+            seed = number
         self.max_norm, self.grad_norm = max_norm, None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, stochastic_rounding=stochastic_rounding, seed=seed))
 

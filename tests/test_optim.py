@@ -720,3 +720,13 @@ def test_parameters_of_a_count_that_change_their_type(bits):
         for k in range(2):
             step(n, o)
             assert [int(o.state[p]["step"]) for p in n.parameters()] == [2 + k] * 4
+
+
+def test_seeds_of_other_kinds_of_whole_numbers():
+    import numpy as np
+
+    for seed, number in ((np.int64(-5), -5), (np.uint64(2 ** 64 - 1), 2 ** 64 - 1), (True, 1)):
+        kept = AdamW([torch.nn.Parameter(torch.zeros(3))], seed=seed).param_groups[0]["seed"]
+        assert type(kept) is int and kept == number
+    with pytest.raises(ValueError, match="seed"):
+        AdamW([torch.nn.Parameter(torch.zeros(3))], seed=torch.tensor(3))
