@@ -688,7 +688,7 @@ def test_what_is_read_shares_no_memory_with_what_is_written():
     good = dict(params=[p], grads=[g], exp_avgs=[m], exp_avg_sqs=[v], step=counter(), lr=1e-3)
     ops.adamw_step(**good)   # (parts of one buffer)
     number = lambda t, i, dtype: t[i:i + (8 if dtype == torch.int64 else 4) // t.element_size()].view(dtype)
-    for change in (dict(grads=[p]), dict(grads=[m]), dict(grads=[flat[3072 + 100:3072 + 800]]), dict(lr=number(p, 0, torch.float32)), dict(step=number(v, 10, torch.int64)),
+    for change in (dict(grads=[p]), dict(grads=[m]), dict(grads=[flat[-924:-224]]), dict(lr=number(p, 0, torch.float32)), dict(step=number(v, 10, torch.int64)),
                    dict(seed=number(m, 698, torch.int64)), dict(max_norm=1.0, norm=number(p, 699, torch.float32))):
         with pytest.raises(ValueError, match="share"):
             ops.adamw_step(**(good | change))
